@@ -32,6 +32,7 @@ enum {
   MLXB_ST_POSITION_RANGE = 2,  // position outside the table / block table
   MLXB_ST_PAGE_RANGE = 4,      // page id outside the pool
   MLXB_ST_WAIT_TIMEOUT = 8,    // a bounded spin-wait gave up
+  MLXB_ST_NOT_FINITE = 16,     // a key or value that a cache in 8 bits cannot hold
 };
 
 static thread_local char g_mlxb_err[512];

@@ -1,0 +1,429 @@
+// Keys and values of a step into pages that hold them in 8 bits, and back.
+//
+// Pages of one layer: codes int8 [n_pages][heads][page][head_dim], scales float32 [n_pages][heads][page / 16]: one scale for
+// each block of 16 positions and head; a code stands for code * scale.
+//
+// append  For a block of a request and a head: A = the largest |x| among the finite numbers that the step brings, S = A / 127 (0
+//         below 2^-100).  A step that brings the block's first position sets the scale to S; a later one to the larger of S and
+//         the scale as it was, and if that grows, the older codes become rint(code * (old / new)).  New codes are
+//         clamp(rint(x * (1 / scale)), -127, 127).  So a scale never falls while a block fills, a code is rounded again only when
+//         a larger number arrives, and what a block holds depends on how the step cut the request only through that second
+//         rounding.  A number that is not finite cannot be held: NaN becomes 0, an infinity the largest code of its sign, and the
+//         status word says so.
+//         Keys (and the step's queries beside them) are turned by their position on the way: the pair (u, v) of dimensions
+//         (i, i + half), or (2i, 2i + 1), becomes (u c - v s, v c + u s), c and s the cosine and sine of the float32 angle
+//         position * freq[i] times `mscale`.  Products, sums, the quotient and the reciprocal are rounded one by one (no fused
+//         multiply-add): x decides a code by its rounding, and another order of roundings would be another code now and then.
+// read    The values at given positions, rounded to the output's type.
+//
+// Rows of a request stand together in order of position (the order in which a step lists them): the row whose predecessor is of
+// another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
+#include "common.cuh"
+
+MLXB_DEFINE_LAST_ERROR()
+
+constexpr int BLK = 16;              // positions that share a scale
+constexpr int MAX_WARPS = 8;
+constexpr uint32_t INF_BITS = 0x7f800000u;
+
+__device__ __forceinline__ void load4(const float* p, bool vec, int n, float (&v)[4]) {
+  if (vec && n >= 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, int n, float (&v)[4]) {
+  if (vec && n >= 4) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(q.x << 16);
+    v[1] = __uint_as_float(q.x & 0xffff0000u);
+    v[2] = __uint_as_float(q.y << 16);
+    v[3] = __uint_as_float(q.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(float* p, bool vec, const float (&v)[4]) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, const float (&v)[4]) {
+  if (vec) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(v[i]);
+  }
+}
+// rint(x * inv) within -127 .. 127 in the low byte.  1.5 * 2^23 + n has n's two's complement in its low bits, and adding it rounds to
+// the nearest whole number, ties to even.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+  const float y = fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f);
+  return __float_as_uint(__fadd_rn(y, 12582912.f));
+}
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], float inv) {
+  const uint32_t lo = __byte_perm(code_of(x[0], inv), code_of(x[1], inv), 0x0040);
+  const uint32_t hi = __byte_perm(code_of(x[2], inv), code_of(x[3], inv), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
+struct AppendArgs {
+  const void *k, *v, *q;         // [T, heads * dk], [T, heads * dv], [T, q heads * dk], or null
+  void* q_out;                   // [T, q heads * dim]
+  int ldk, ldv, ldq, ldo;
+  int T, Hkv, G;                 // G: query heads to a key/value head (0: no queries)
+  int dk, dv, dim;
+  const float* freq;
+  int half, interleaved;
+  float mscale;
+  const int *positions, *token_req, *block_table;
+  int max_pages, n_pages, page;
+  int8_t *k8, *v8;
+  float *ks, *vs;
+  int* status;
+  int chunk, heads_per_cta, vec;  // vec: bit 0 keys, 1 values, 2 queries, 3 q_out: four columns an access
+};
+
+struct Leader {
+  int row, n, pos, page_id;      // page_id < 0: nothing is stored
+};
+
+// A CTA takes the leaders among `chunk` rows and a group of heads: it lists the leaders, forms the sines and cosines of all their rows
+// once in shared memory, and its warps take the pairs (leader, head; keys, values or one query head).  A warp holds all the numbers of
+// a pair (16 rows of up to 128 columns: 64 a lane) in registers between the search for the largest and the codes, so a number is
+// read once.  LPR lanes stand on a row, 8 columns each in two groups of 4: the groups of a lane are a rotation's two halves where
+// these are whole groups, so that a pair's numbers meet in one lane.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(MAX_WARPS * 32)
+append_kernel(const AppendArgs a) {
+  constexpr int RP = 32 / LPR;                 // rows at a time
+  constexpr int PASSES = BLK / RP;
+  extern __shared__ float2 turn[];             // [rows][half]: cosine and sine
+  __shared__ Leader lead[BLK];
+  __shared__ int n_lead, last_row;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  const int row0 = blockIdx.x * a.chunk;
+  if (threadIdx.x == 0) { n_lead = 0; last_row = row0; }
+  __syncthreads();
+  if (threadIdx.x < a.chunk) {
+    const int t = row0 + threadIdx.x;
+    const int r = t < a.T ? a.token_req[t] : -1;
+    if (r >= 0) {
+      const int p = a.positions[t];
+      const bool follows = t > 0 && a.token_req[t - 1] == r && a.positions[t - 1] == p - 1;
+      if (!follows || (p & (BLK - 1)) == 0) {
+        int n = 1;
+        while (t + n < a.T && ((p + n) & (BLK - 1)) != 0 && a.token_req[t + n] == r && a.positions[t + n] == p + n) ++n;
+        const int lp = p / a.page;
+        int pg = -1;
+        if (p < 0 || lp >= a.max_pages) {
+          if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
+        } else {
+          pg = a.block_table[(size_t)r * a.max_pages + lp];
+          if (pg >= a.n_pages) {
+            if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_PAGE_RANGE);
+            pg = -1;
+          }
+        }
+        lead[atomicAdd(&n_lead, 1)] = Leader{t, n, p, pg};
+        atomicMax(&last_row, t + n);
+      }
+    }
+  }
+  __syncthreads();
+  const int nl = n_lead;
+  if (nl == 0) return;
+  // (rows between two leaders that are of no request get an angle nobody uses)
+  for (int e = threadIdx.x; e < (last_row - row0) * a.half; e += blockDim.x) {
+    const int i = e / a.half, j = e - i * a.half;
+    float sn, cs;
+    sincosf(__fmul_rn((float)a.positions[row0 + i], a.freq[j]), &sn, &cs);
+    turn[e] = make_float2(__fmul_rn(cs, a.mscale), __fmul_rn(sn, a.mscale));
+  }
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+
+  const int per = a.page / BLK;
+  const int kinds = (a.k ? 2 : 0) + a.G;
+  const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.heads_per_cta, a.Hkv - h0);
+  const int sub = lane / LPR, l = lane & (LPR - 1);
+  const bool whole = !a.interleaved && (a.half & 3) == 0;       // a lane holds both halves of its pairs
+  const int hg = a.half >> 2;
+  for (int u = warp; u < nl * nh * kinds; u += n_warps) {
+    const Leader ld = lead[u / (nh * kinds)];
+    const int w = u % (nh * kinds), h = h0 + w / kinds;
+    int kind = w % kinds;                      // 0 keys, 1 values, 2 + i query head i of the group
+    if (!a.k) kind += 2;
+    const bool turned = kind != 1 && a.half > 0;
+    const T* src;
+    int ld_src, width;
+    bool vec;
+    if (kind == 0) { src = (const T*)a.k + (size_t)h * a.dk; ld_src = a.ldk; width = a.dk; vec = a.vec & 1; }
+    else if (kind == 1) { src = (const T*)a.v + (size_t)h * a.dv; ld_src = a.ldv; width = a.dv; vec = a.vec & 2; }
+    else { src = (const T*)a.q + ((size_t)h * a.G + kind - 2) * a.dk; ld_src = a.ldq; width = a.dk; vec = a.vec & 4; }
+    src = after_wait(src);
+    // the two groups of four columns of this lane
+    int c0, c1;
+    if (turned && whole) {
+      c0 = l < hg ? 4 * l : 2 * a.half + 8 * (l - hg);
+      c1 = l < hg ? c0 + a.half : c0 + 4;
+    } else {
+      c0 = 8 * l;
+      c1 = c0 + 4;
+    }
+    const bool mine = 8 * l < a.dim;
+    auto value = [&](const T* row, const float2* cs, int i) {      // column i, turned, wherever its partner is
+      const float x = i < width ? to_f(row[i]) : 0.f;
+      if (i >= 2 * a.half) return x;
+      const bool lower = a.interleaved ? !(i & 1) : i < a.half;
+      const int j = a.interleaved ? (i ^ 1) : lower ? i + a.half : i - a.half;
+      const float y = to_f(row[j]);
+      const float2 t = cs[a.interleaved ? i >> 1 : lower ? i : j];
+      return lower ? __fsub_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y)) : __fadd_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y));
+    };
+    auto fetch = [&](int i, float (&x)[4], float (&y)[4]) {        // row i of the leader's
+      const T* row = src + (size_t)(ld.row + i) * ld_src;
+      const float2* cs = turn + (ld.row + i - row0) * a.half;
+      if (turned && !whole) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[e] = value(row, cs, c0 + e); y[e] = value(row, cs, c1 + e); }
+        return;
+      }
+      load4(row + c0, vec, width - c0, x);
+      load4(row + c1, vec, width - c1, y);
+      if (turned && l < hg) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 t = cs[c0 + e];
+          const float p = x[e], q = y[e];
+          x[e] = __fsub_rn(__fmul_rn(p, t.x), __fmul_rn(q, t.y));
+          y[e] = __fadd_rn(__fmul_rn(q, t.x), __fmul_rn(p, t.y));
+        }
+      }
+    };
+    if (kind >= 2) {
+      T* dst = (T*)a.q_out + ((size_t)h * a.G + kind - 2) * a.dim;
+#pragma unroll 4
+      for (int i = sub; i < ld.n; i += RP) {
+        float x[4], y[4];
+        if (mine) {
+          fetch(i, x, y);
+          store4(dst + (size_t)(ld.row + i) * a.ldo + c0, a.vec & 8, x);
+          store4(dst + (size_t)(ld.row + i) * a.ldo + c1, a.vec & 8, y);
+        }
+      }
+      continue;
+    }
+    if (ld.page_id < 0) continue;
+    float x[PASSES][4], y[PASSES][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < PASSES; ++s) {
+      if (s * RP >= ld.n) break;
+      const int i = s * RP + sub;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[s][e] = y[s][e] = 0.f;
+      if (mine && i < ld.n) fetch(i, x[s], y[s]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        top = max(top, max(__float_as_uint(x[s][e]) & 0x7fffffffu, __float_as_uint(y[s][e]) & 0x7fffffffu));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (top >= INF_BITS) {                     // something is not finite: the largest of the others, and NaN becomes 0
+      if (lane == 0) atomicOr(a.status, MLXB_ST_NOT_FINITE);
+      top = 0;
+#pragma unroll
+      for (int s = 0; s < PASSES; ++s) {
+        if (s * RP >= ld.n) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bx = __float_as_uint(x[s][e]) & 0x7fffffffu, by = __float_as_uint(y[s][e]) & 0x7fffffffu;
+          if (bx < INF_BITS) top = max(top, bx);
+          if (by < INF_BITS) top = max(top, by);
+          if (bx > INF_BITS) x[s][e] = 0.f;
+          if (by > INF_BITS) y[s][e] = 0.f;
+        }
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    const float largest = __uint_as_float(top);
+    float scale = largest < 7.888609052210118e-31f ? 0.f : __fdiv_rn(largest, 127.f);
+    const int off = ld.pos & (BLK - 1), in_page = ld.pos & (a.page - 1);
+    int8_t* codes = (kind ? a.v8 : a.k8) + (((size_t)ld.page_id * a.Hkv + h) * a.page + (in_page - off)) * a.dim;
+    float* sp = (kind ? a.vs : a.ks) + ((size_t)ld.page_id * a.Hkv + h) * per + in_page / BLK;
+    if (off > 0) {
+      const float old = *sp;
+      if (scale > old) {                       // older codes of the block to the larger scale
+        const float ratio = __fdiv_rn(old, scale);
+        for (int e = lane * 16; e < off * a.dim; e += 512) {
+          uint4 c = *reinterpret_cast<const uint4*>(codes + e);
+          uint32_t* cw = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const char4 b = *reinterpret_cast<const char4*>(&cw[j]);
+            const float f[4] = {(float)b.x, (float)b.y, (float)b.z, (float)b.w};
+            cw[j] = codes4(f, ratio);
+          }
+          *reinterpret_cast<uint4*>(codes + e) = c;
+        }
+      } else {
+        scale = old;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) *sp = scale;
+    const float inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;
+#pragma unroll
+    for (int s = 0; s < PASSES; ++s) {
+      if (s * RP >= ld.n) break;
+      const int i = s * RP + sub;
+      if (mine && i < ld.n) {
+        int8_t* dst = codes + (off + i) * a.dim;
+        *reinterpret_cast<uint32_t*>(dst + c0) = scale > 0.f ? codes4(x[s], inv) : 0u;
+        *reinterpret_cast<uint32_t*>(dst + c1) = scale > 0.f ? codes4(y[s], inv) : 0u;
+      }
+    }
+  }
+}
+
+// Keys [T, Hkv * dk] and values [T, Hkv * dv] (dtype; rows at strides ldk, ldv) into the pages; queries [T, Hkv * G * dk] turned into
+// q_out [T, Hkv * G * dim] (G 0: none; k and v null: queries only).  Columns of a head from dk (dv) to dim are zeros.  page a power of
+// two of at least 16, dim a multiple of 16 up to 256, freq [half] with 2 * half <= dk.
+MLXB_EXPORT int mlxb_kv8_append(int dtype, const void* k, int ldk, const void* v, int ldv, const void* q, int ldq, void* q_out, int ldo,
+                                int T, int Hkv, int G, int dk, int dv, int dim, const float* freq, int half, int interleaved,
+                                float mscale, const int* positions, const int* token_req, const int* block_table, int max_pages,
+                                int n_pages, int page, int8_t* k8, int8_t* v8, float* ks, float* vs, int* status,
+                                cudaStream_t stream) {
+  if (dtype != MLXB_F32 && dtype != MLXB_BF16) return mlxb_fail(MLXB_BAD_DTYPE, "kv8_append: dtype code %d", dtype);
+  if (T <= 0) return 0;
+  if (Hkv <= 0 || G < 0 || dim % 16 || dim < 16 || dim > 256 || dk <= 0 || dk > dim || dv <= 0 || dv > dim)
+    return mlxb_fail(MLXB_BAD_ARG, "kv8_append: %d heads of %d and %d columns in rows of %d (a multiple of 16 up to 256)", Hkv, dk, dv, dim);
+  if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: page size %d (a power of two of at least %d)", page, BLK);
+  if (half < 0 || 2 * half > dk || (half && !freq)) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: %d pairs of %d columns", half, dk);
+  if ((k == nullptr) != (v == nullptr) || (!k && !G) || (G && (!q || !q_out)))
+    return mlxb_fail(MLXB_BAD_ARG, "kv8_append: keys and values go together, and queries with an output");
+  if (((uintptr_t)k8 | (uintptr_t)v8) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: pools must be 16-byte aligned");
+  const size_t item = dtype == MLXB_F32 ? 4 : 2;
+  auto fits = [&](const void* p, int ld, int d) { return (((uintptr_t)p) % (4 * item)) == 0 && ld % 4 == 0 && d % 4 == 0; };
+  AppendArgs a{k, v, q, q_out, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, freq, half, interleaved, mscale, positions, token_req,
+               block_table, max_pages, n_pages, page, k8, v8, ks, vs, status, 1, 1, 0};
+  a.vec = (fits(k, ldk, dk) ? 1 : 0) | (fits(v, ldv, dv) ? 2 : 0) | (fits(q, ldq, dk) ? 4 : 0) | (fits(q_out, ldo, dim) ? 8 : 0);
+  // few rows: a CTA a row, so that single tokens of different requests spread over the device; many: the rows of a block together
+  a.chunk = T <= 64 ? 1 : BLK;
+  const int kinds = (k ? 2 : 0) + G;
+  a.heads_per_cta = kinds >= MAX_WARPS ? 1 : MAX_WARPS / kinds;
+  if (a.heads_per_cta > Hkv) a.heads_per_cta = Hkv;
+  const int warps = kinds * a.heads_per_cta < MAX_WARPS ? kinds * a.heads_per_cta : MAX_WARPS;
+  const dim3 grid((T + a.chunk - 1) / a.chunk, (Hkv + a.heads_per_cta - 1) / a.heads_per_cta);
+  if (grid.y > 65535) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: %d heads", Hkv);
+  const size_t smem = (size_t)(a.chunk + BLK - 1) * half * sizeof(float2);      // at most 31 rows of 128 pairs: 31 KB
+  auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(32 * warps), smem, stream, a); };
+  const int lanes = dim / 8;
+  if (dtype == MLXB_F32) {
+    if (lanes <= 4) go(append_kernel<float, 4>);
+    else if (lanes <= 8) go(append_kernel<float, 8>);
+    else if (lanes <= 16) go(append_kernel<float, 16>);
+    else go(append_kernel<float, 32>);
+  } else {
+    if (lanes <= 4) go(append_kernel<__nv_bfloat16, 4>);
+    else if (lanes <= 8) go(append_kernel<__nv_bfloat16, 8>);
+    else if (lanes <= 16) go(append_kernel<__nv_bfloat16, 16>);
+    else go(append_kernel<__nv_bfloat16, 32>);
+  }
+  return mlxb_check_launch("kv8_append");
+}
+
+// ---- what the pages hold
+
+// A thread takes 16 codes of a row (keys, then values): 16 bytes in, 32 or 64 out.
+template <typename T>
+__global__ void __launch_bounds__(256)
+read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ block_table, int max_pages,
+            int n_pages, int page, int Hkv, int dim, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, T* k_out,
+            int ldk, T* v_out, int ldv, int n_rows, int vec, int* status) {
+  pdl_wait();
+  pdl_trigger();
+  const int per_row = 2 * Hkv * dim / 16;
+  const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int t = (int)(e / per_row);
+  if (t >= n_rows) return;
+  const int w = (int)(e - (long long)t * per_row);
+  const int r = token_req[t];
+  if (r < 0) return;
+  const int p = positions[t], lp = p / page;
+  int pg = -1;
+  if (p >= 0 && lp < max_pages) pg = block_table[(size_t)r * max_pages + lp];
+  if (pg < 0 || pg >= n_pages) {
+    if (w == 0) atomicOr(status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+    pg = -1;
+  }
+  const int col = w * 16, width = Hkv * dim;
+  const bool is_v = col >= width;
+  const int c = is_v ? col - width : col, h = c / dim, d = c - h * dim;
+  float o[16];
+  if (pg >= 0) {
+    const size_t at = ((size_t)pg * Hkv + h) * page + (p & (page - 1));
+    const int8_t* src = after_wait(is_v ? v8 : k8) + at * dim + d;
+    const float s = after_wait(is_v ? vs : ks)[((size_t)pg * Hkv + h) * (page / BLK) + (p & (page - 1)) / BLK];
+    const uint4 c4 = *reinterpret_cast<const uint4*>(src);
+    const uint32_t cw[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const char4 b = *reinterpret_cast<const char4*>(&cw[j]);
+      o[4 * j] = (float)b.x * s; o[4 * j + 1] = (float)b.y * s; o[4 * j + 2] = (float)b.z * s; o[4 * j + 3] = (float)b.w * s;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = 0.f;
+  }
+  T* dst = is_v ? v_out + (size_t)t * ldv + c : k_out + (size_t)t * ldk + c;
+  if (vec) {
+    if constexpr (sizeof(T) == 2) {
+      float lo[8], hi[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { lo[j] = o[j]; hi[j] = o[8 + j]; }
+      reinterpret_cast<uint4*>(dst)[0] = pack8(lo);
+      reinterpret_cast<uint4*>(dst)[1] = pack8(hi);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) dst[j] = from_f<T>(o[j]);
+  }
+}
+
+// k_out, v_out [n_rows, Hkv * dim]: what the pages stand for at position positions[t] of request token_req[t] (< 0: row left as it is;
+// a position without a page: zeros and a status bit).
+MLXB_EXPORT int mlxb_kv8_read(int dtype, const int* positions, const int* token_req, const int* block_table, int max_pages, int n_pages,
+                              int page, int Hkv, int dim, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs,
+                              void* k_out, int ldk, void* v_out, int ldv, int n_rows, int* status, cudaStream_t stream) {
+  if (dtype != MLXB_F32 && dtype != MLXB_BF16) return mlxb_fail(MLXB_BAD_DTYPE, "kv8_read: dtype code %d", dtype);
+  if (n_rows <= 0) return 0;
+  if (Hkv <= 0 || dim % 16 || dim < 16 || dim > 256) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: %d heads of %d (a multiple of 16 up to 256)", Hkv, dim);
+  if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: page size %d (a power of two of at least %d)", page, BLK);
+  if (((uintptr_t)k8 | (uintptr_t)v8) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: pools must be 16-byte aligned");
+  const size_t item = dtype == MLXB_F32 ? 4 : 2;
+  const int vec = !(((uintptr_t)k_out | (uintptr_t)v_out) & 15) && (ldk * item) % 16 == 0 && (ldv * item) % 16 == 0;
+  const long long n = (long long)n_rows * (2 * Hkv * dim / 16);
+  if ((n + 255) / 256 > 0x7fffffffll) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: %d rows", n_rows);
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (dtype == MLXB_F32)
+    launch_pdl(read_kernel<float>, grid, dim3(256), 0, stream, positions, token_req, block_table, max_pages, n_pages, page, Hkv, dim, k8,
+               v8, ks, vs, (float*)k_out, ldk, (float*)v_out, ldv, n_rows, vec, status);
+  else
+    launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, positions, token_req, block_table, max_pages, n_pages, page, Hkv,
+               dim, k8, v8, ks, vs, (__nv_bfloat16*)k_out, ldk, (__nv_bfloat16*)v_out, ldv, n_rows, vec, status);
+  return mlxb_check_launch("kv8_read");
+}

@@ -1,0 +1,179 @@
+// What the kernels for single queries over pages in 8 bits share: how the rows' keys are cut into items, and how an item's result
+// becomes a row of the output.
+//
+// A row (one query of each head, at position p of its request) sees keys max(0, p - window + 1) .. p.  They are cut into chunks that
+// begin at multiples of 16 positions; how many there are goes by the row's own number of keys and by the numbers of heads, never by
+// what else is in the batch, so that a row's bits do not depend on its neighbours.  An item is a chunk of a row for one tile of query
+// heads that read the same key/value head.  The grid is as large as the device (or the most items there can be) and every CTA walks
+// items blockIdx.x, blockIdx.x + gridDim.x, ...: lengths are known on the device only, and a grid for the longest row would be mostly
+// empty blocks.  The items of all rows are numbered by a prefix sum that each CTA forms for itself.
+#pragma once
+
+#include "common.cuh"
+
+constexpr int BLK = 16;              // positions that share a scale
+constexpr int ROWS_MOST = 4096;      // rows a launch takes: their prefix sums are in shared memory
+
+struct RowsArgs {
+  const void* q;
+  int ldq;
+  const int *rows, *positions, *token_req, *block_table;
+  int max_pages, n_pages, page, Hq, Hkv, dim, window;
+  float scale;
+  const int8_t *k8, *v8;
+  const float *ks, *vs, *sinks;
+  float* partial;
+  int* counters;
+  int most_chunks;                   // of a row
+  void* out;
+  int ldo, n_rows;
+  int* status;
+};
+
+// Keys of a chunk for a row of n keys: a multiple of 64 that cuts them into at most `most` chunks.
+__device__ __forceinline__ int chunk_keys(int n, int most) {
+  const int c = n <= 1024 ? 128 : n <= 4096 ? 256 : 512;
+  const int least = ((n + most - 1) / most + 63) & ~63;
+  return c > least ? c : least;
+}
+
+struct RowSpan { int tok, req, pos, first, n; };      // first: a multiple of 16; n: keys from there to the query (0: no such row)
+
+__device__ __forceinline__ RowSpan row_span(const RowsArgs& a, int i, bool report) {
+  RowSpan s{a.rows ? a.rows[i] : i, -1, 0, 0, 0};
+  s.req = a.token_req[s.tok];
+  if (s.req < 0) return s;                            // a row that pads the step
+  s.pos = a.positions[s.tok];
+  if (s.pos < 0 || s.pos / a.page >= a.max_pages) {
+    if (report) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
+    return s;
+  }
+  const int lo = a.window > 0 && s.pos - a.window + 1 > 0 ? s.pos - a.window + 1 : 0;
+  s.first = lo & ~(BLK - 1);
+  s.n = s.pos + 1 - s.first;
+  return s;
+}
+
+// prefix[i]: chunks of the rows before row i; returns the number of all.  Every thread of the CTA calls it.
+__device__ __forceinline__ int schedule(const RowsArgs& a, int* prefix, int* warp_sums) {
+  const int n = a.n_rows, seg = (n + blockDim.x - 1) / blockDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  const int b = min(n, (int)threadIdx.x * seg), e = min(n, b + seg);
+  int sum = 0;
+  for (int i = b; i < e; ++i) {
+    const RowSpan s = row_span(a, i, blockIdx.x == 0);
+    const int c = s.n ? (s.n + chunk_keys(s.n, a.most_chunks) - 1) / chunk_keys(s.n, a.most_chunks) : 0;
+    prefix[i + 1] = c;
+    sum += c;
+  }
+  int run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) warp_sums[warp] = run;
+  __syncthreads();
+  int before = run - sum;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  int total = 0;
+  for (int w = 0; w < n_warps; ++w) total += warp_sums[w];
+  for (int i = b; i < e; ++i) { before += prefix[i + 1]; prefix[i + 1] = before; }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+  return total;
+}
+
+struct Item {
+  RowSpan row;
+  int index, chunk, n_chunks, begin, end, tile;       // keys begin .. end - 1 (begin a multiple of 16)
+};
+
+// Item `it` of `tiles` tiles of heads: neighbouring items are the tiles of one chunk, whose pages lie together.
+__device__ __forceinline__ Item item_of(const RowsArgs& a, const int* prefix, int it, int tiles) {
+  Item x;
+  const int g = it / tiles;
+  x.tile = it - g * tiles;
+  int lo = 0, hi = a.n_rows - 1;                      // the last row whose prefix is <= g
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= g) lo = mid; else hi = mid - 1;
+  }
+  x.index = lo;
+  x.chunk = g - prefix[lo];
+  x.n_chunks = prefix[lo + 1] - prefix[lo];
+  x.row = row_span(a, lo, false);
+  const int c = chunk_keys(x.row.n, a.most_chunks);
+  x.begin = x.row.first + x.chunk * c;
+  x.end = min(x.begin + c, x.row.pos + 1);
+  return x;
+}
+
+// The page of a key, or -1 where the request has none (reported).
+__device__ __forceinline__ int page_of(const RowsArgs& a, const int* bt, int key) {
+  const int pg = bt[key / a.page];
+  if (pg >= 0 && pg < a.n_pages) return pg;
+  atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+  return -1;
+}
+
+// A CTA's sums for the heads h0 .. h0 + nh - 1 of an item, in shared memory: m[h], l[h], o[h * dim + d].  A row of one chunk goes
+// to the output; else the sums go to scratch memory and the CTA that comes last for the (row, tile) adds them up in the order of the
+// chunks.  Exp(x): the exponential in the unit of m.  Every thread of the CTA calls it; weights: [most_chunks][nh].
+template <typename T, typename Exp>
+__device__ __forceinline__ void finish_item(const RowsArgs& a, const Item& x, int tiles, int tile_heads, int h0, int nh, const float* m,
+                                            const float* l, const float* o, float* weights, int* last, float sink_unit, Exp exp_) {
+  const int D = a.dim;
+  T* out = (T*)a.out + (size_t)x.row.tok * a.ldo + (size_t)h0 * D;
+  if (x.n_chunks == 1) {
+    for (int e = threadIdx.x; e < nh * D; e += blockDim.x) {
+      const int h = e / D;
+      const float total = a.sinks ? l[h] + exp_(a.sinks[h0 + h] * sink_unit - m[h]) : l[h];
+      out[e] = from_f<T>(total != 0.f ? o[e] / total : 0.f);
+    }
+    return;
+  }
+  const size_t per = (size_t)tile_heads * (D + 2);
+  const size_t slot = ((size_t)x.index * tiles + x.tile) * a.most_chunks;
+  float* mine = a.partial + (slot + x.chunk) * per;
+  for (int e = threadIdx.x; e < nh * D; e += blockDim.x) __stcg(mine + 2 * tile_heads + e, o[e]);
+  if (threadIdx.x < nh) {
+    __stcg(mine + threadIdx.x, m[threadIdx.x]);
+    __stcg(mine + tile_heads + threadIdx.x, l[threadIdx.x]);
+  }
+  __threadfence();
+  __syncthreads();
+  int* counter = a.counters + (size_t)x.index * tiles + x.tile;
+  if (threadIdx.x == 0) *last = atomicAdd(counter, 1) == x.n_chunks - 1;
+  __syncthreads();
+  if (!*last) return;
+  __threadfence();
+  if (threadIdx.x == 0) *counter = 0;
+  const float* all = a.partial + slot * per;
+  // weights of the chunks: exp(m_c - M) / total
+  for (int h = threadIdx.x; h < nh; h += blockDim.x) {
+    float top = -INFINITY, total = 0.f;
+    bool odd = false;                                  // fmaxf leaves NaN out
+    for (int c = 0; c < x.n_chunks; ++c) {
+      const float mc = __ldcg(all + c * per + h);
+      odd |= mc != mc;
+      top = fmaxf(top, mc);
+    }
+    if (odd) top = NAN;
+    for (int c = 0; c < x.n_chunks; ++c) {
+      const float w = exp_(__ldcg(all + c * per + h) - top);
+      weights[c * tile_heads + h] = w;
+      total += w * __ldcg(all + c * per + tile_heads + h);
+    }
+    if (a.sinks) total += exp_(a.sinks[h0 + h] * sink_unit - top);
+    weights[a.most_chunks * tile_heads + h] = total != 0.f ? 1.f / total : 0.f;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < nh * D; e += blockDim.x) {
+    const int h = e / D;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int c = 0; c < x.n_chunks; ++c) sum = fmaf(weights[c * tile_heads + h], __ldcg(all + c * per + 2 * tile_heads + e), sum);
+    out[e] = from_f<T>(sum * weights[a.most_chunks * tile_heads + h]);
+  }
+}

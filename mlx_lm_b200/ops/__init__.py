@@ -55,7 +55,7 @@ BF16_ONLY_LIBS = frozenset({"gemm_smallm", "gemm_smallm_fold", "gemm_tcgen05", "
 F32_ONLY_LIBS = frozenset({"gemm_split"})
 
 # status word bits set by kernels (csrc/common.cuh)
-ST_TOKEN_RANGE, ST_POSITION_RANGE, ST_PAGE_RANGE, ST_WAIT_TIMEOUT = 1, 2, 4, 8
+ST_TOKEN_RANGE, ST_POSITION_RANGE, ST_PAGE_RANGE, ST_WAIT_TIMEOUT, ST_NOT_FINITE = 1, 2, 4, 8, 16
 
 
 class KernelError(RuntimeError):
@@ -67,7 +67,8 @@ def describe_status(word: int) -> str:
     names = [n for b, n in ((ST_TOKEN_RANGE, "token id out of range"),
                             (ST_POSITION_RANGE, "position without a page or out of range"),
                             (ST_PAGE_RANGE, "page id outside the pool"),
-                            (ST_WAIT_TIMEOUT, "a bounded wait in a kernel gave up")) if word & b]
+                            (ST_WAIT_TIMEOUT, "a bounded wait in a kernel gave up"),
+                            (ST_NOT_FINITE, "a key or value that is not finite entered a cache in 8 bits")) if word & b]
     return "; ".join(names) or f"status {word}"
 
 
@@ -803,6 +804,190 @@ def attention_decode(q, positions, token_req, block_table, k_pool, v_pool, out, 
           _p(rows), _p(positions), _p(token_req), _p(block_table), block_table.shape[1], n_pages, page, n_heads, Hkv,
           Dh, window, scale, _p(k_pool), _p(v_pool), _p(scratch), _p(counters), n_chunks, chunk, _p(out),
           _rows(out, "attention out"), n, _p(status), _sinks(sinks, n_heads, "attention_decode"), int(beside), stream)
+
+
+# --------------------------------------------------------------------------
+# a cache of keys and values in 8 bits (csrc/kv8.cu, csrc/kv8_rows.cu)
+
+KV8_BLOCK = 16           # positions of a head that share a scale
+KV8_ROWS_MOST = 4096     # rows one launch takes (csrc/kv8_rows.cuh)
+
+
+def kv8_supported(page: int, head_dim: int) -> bool:
+    """Whether pages of this size can hold 8-bit codes of heads of this size."""
+    return page >= KV8_BLOCK and page & (page - 1) == 0 and head_dim % 16 == 0 and 16 <= head_dim <= 256
+
+
+def _kv8_pools(k8, v8, k_scale, v_scale, block_table, what: str):
+    """Shape of the pages ``[n_pages, heads, page, head_dim]`` of a cache in 8 bits."""
+    _need(k8, torch.int8, what + " key codes")
+    _need(v8, torch.int8, what + " value codes")
+    _need(k_scale, torch.float32, what + " key scales")
+    _need(v_scale, torch.float32, what + " value scales")
+    _need(block_table, torch.int32, what + " block_table")
+    if k8.dim() != 4 or v8.shape != k8.shape or not (k8.is_contiguous() and v8.is_contiguous()):
+        raise KernelError(f"{what}: codes {tuple(k8.shape)} and {tuple(v8.shape)}: contiguous [n_pages, heads, page, head_dim], both the same")
+    n_pages, Hkv, page, Dh = k8.shape
+    if not kv8_supported(page, Dh):
+        raise KernelError(f"{what}: pages of {page} positions of heads of {Dh}: a power of two of at least {KV8_BLOCK}, heads a "
+                          "multiple of 16 up to 256")
+    want = (n_pages, Hkv, page // KV8_BLOCK)
+    if k_scale.shape != want or v_scale.shape != want or not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise KernelError(f"{what}: scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)}, expected contiguous {want}")
+    if block_table.dim() != 2 or not block_table.is_contiguous():
+        raise KernelError(f"{what}: block table {tuple(block_table.shape)}: contiguous [requests, pages]")
+    return n_pages, Hkv, page, Dh
+
+
+def _kv8_rows_ints(positions, token_req, n: int, what: str) -> None:
+    _need(positions, torch.int32, what + " positions")
+    _need(token_req, torch.int32, what + " token_req")
+    if positions.numel() < n or token_req.numel() < n or not (positions.is_contiguous() and token_req.is_contiguous()):
+        raise KernelError(f"{what}: {positions.numel()} positions and {token_req.numel()} requests for {n} rows")
+
+
+_KV8_APPEND_ARGS = ([c_int] + [c_void_p, c_int] * 4 + [c_int] * 6 + [c_void_p, c_int, c_int, c_float] + [c_void_p] * 3 + [c_int] * 3
+                    + [c_void_p] * 6)
+
+
+def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale, status, stream, freq=None, interleaved: bool = False,
+               mscale: float = 1.0, q=None, q_out=None) -> None:
+    """This step's keys ``k [T, heads * dk]`` and values ``v [T, heads * dv]`` (rows of any stride, float32 or bfloat16) into pages of
+    int8 codes ``[n_pages, heads, page, head_dim]`` with a float32 scale for each block of 16 positions and head (``[n_pages, heads,
+    page // 16]``), in place; columns of a head beyond ``dk`` / ``dv`` are zeros.  Keys turn by their position on the way: the first
+    ``2 * len(freq)`` dimensions of every head, pairs ``(i, i + len(freq))`` or, ``interleaved``, ``(2i, 2i + 1)``, angle ``position *
+    freq[i]``, cosine and sine times ``mscale``; None: no rotation.  ``q [T, query heads * dk]`` turns likewise into ``q_out [T, query heads *
+    head_dim]``.  ``k`` and ``v`` None: only ``q``.
+
+    With ``A`` the largest magnitude that the call brings for a block and head and ``S = A / 127`` (0 below 2**-100), a call that brings the
+    block's first position sets its scale to ``S``, a later one to the larger of ``S`` and what it was; older codes become ``rint(code *
+    (old / new))`` where it grows.  New codes are ``rint(x * (1 / scale))`` within -127 .. 127.  A NaN is held as 0 and an infinity as the
+    largest code; ``status`` then gets ``ST_NOT_FINITE``.
+
+    Rows of a request stand together in order of position; ``token_req`` < 0: a row of no request, which is left out."""
+    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_append")
+    if (k is None) != (v is None) or (k is None and q is None) or (q is None) != (q_out is None):
+        raise KernelError("kv8_append: keys and values go together, and queries with their output")
+    x = q if k is None else k
+    if x.dim() != 2:
+        raise KernelError(f"kv8_append: rows {tuple(x.shape)}: [tokens, columns]")
+    T = x.shape[0]
+    code, dk, dv, G = dtype_code(x.dtype), 0, Dh, 0
+    _kv8_rows_ints(positions, token_req, T, "kv8_append")
+    if k is not None:
+        for t, what in ((k, "keys"), (v, "values")):
+            _need(t, x.dtype, "kv8_append " + what)
+            _rows(t, "kv8_append " + what)
+            if t.shape[0] != T or t.shape[1] % Hkv or not 0 < t.shape[1] <= Hkv * Dh:
+                raise KernelError(f"kv8_append: {what} {tuple(t.shape)} for {T} rows of {Hkv} heads of at most {Dh}")
+        dk, dv = k.shape[1] // Hkv, v.shape[1] // Hkv
+    if q is not None:
+        _need(q, x.dtype, "kv8_append q")
+        _need(q_out, x.dtype, "kv8_append q_out")
+        if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] % (Hkv * Dh) or q_out.shape[1] == 0:
+            raise KernelError(f"kv8_append: q_out {tuple(q_out.shape)} for {T} rows over {Hkv} key/value heads of {Dh}")
+        G = q_out.shape[1] // (Hkv * Dh)
+        if q.dim() != 2 or q.shape[0] != T or q.shape[1] % (Hkv * G) or not 0 < q.shape[1] <= q_out.shape[1]:
+            raise KernelError(f"kv8_append: q {tuple(q.shape)} for q_out {tuple(q_out.shape)}")
+        if k is not None and q.shape[1] != Hkv * G * dk:
+            raise KernelError(f"kv8_append: q {tuple(q.shape)} for {Hkv * G} heads of {dk}")
+        dk = q.shape[1] // (Hkv * G)
+    half = 0
+    if freq is not None:
+        _need(freq, torch.float32, "kv8_append freq")
+        half = freq.numel()
+        if 2 * half > dk or not freq.is_contiguous():
+            raise KernelError(f"kv8_append: {half} frequencies for heads of {dk}")
+    rows = lambda t, what: 0 if t is None else _rows(t, "kv8_append " + what)
+    _call("kv8", "mlxb_kv8_append", _KV8_APPEND_ARGS, code, _p(k), rows(k, "keys"), _p(v), rows(v, "values"), _p(q), rows(q, "q"),
+          _p(q_out), rows(q_out, "q_out"), T, Hkv, G, dk, dv, Dh, _p(freq) if half else None, half, int(interleaved), float(mscale),
+          _p(positions), _p(token_req), _p(block_table), block_table.shape[1], n_pages, page, _p(k8), _p(v8), _p(k_scale), _p(v_scale),
+          _p(status), stream)
+
+
+_KV8_READ_ARGS = [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_void_p] * 4 + [c_void_p, c_int] * 2 + [c_int, c_void_p, c_void_p]
+
+
+def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out, v_out, status, stream) -> None:
+    """What the pages stand for: row ``t`` of ``k_out`` and ``v_out`` (``[n, heads * head_dim]``, float32 or bfloat16) becomes the key and
+    the value (``code * scale``) at position ``positions[t]`` of request ``token_req[t]`` (< 0: the row is left as it is; a position without
+    a page: zeros, and ``status`` says so)."""
+    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_read")
+    for t, what in ((k_out, "k_out"), (v_out, "v_out")):
+        _need(t, k_out.dtype, "kv8_read " + what)
+        _rows(t, "kv8_read " + what)
+        if t.shape != (k_out.shape[0], Hkv * Dh):
+            raise KernelError(f"kv8_read: {what} {tuple(t.shape)} for {Hkv} heads of {Dh}")
+    n = k_out.shape[0]
+    _kv8_rows_ints(positions, token_req, n, "kv8_read")
+    _call("kv8", "mlxb_kv8_read", _KV8_READ_ARGS, dtype_code(k_out.dtype), _p(positions), _p(token_req), _p(block_table),
+          block_table.shape[1], n_pages, page, Hkv, Dh, _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(k_out), _rows(k_out, "k_out"),
+          _p(v_out), _rows(v_out, "v_out"), n, _p(status), stream)
+
+
+_KV8_ROWS_ARGS = ([c_int, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] + [c_void_p] * 6 + [c_int, c_void_p, c_int, c_int]
+                  + [c_void_p] * 3)
+_KV8_TILE_HEADS = 4      # query heads that a block of csrc/kv8_rows.cu takes
+
+
+def _kv8_tiles(n_heads: int, n_kv_heads: int) -> int:
+    return n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS)
+
+
+def _kv8_most_chunks(n_heads: int, n_kv_heads: int, max_len: int) -> int:
+    """The most parts a row's keys are cut into: what fills the device with one row, and no more than the longest row has."""
+    return max(1, min(3 * 148 // _kv8_tiles(n_heads, n_kv_heads), -(-(max_len + KV8_BLOCK) // 128)))
+
+
+def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
+    """``(float32 elements of scratch memory, int32 counters)`` that ``kv8_attention_rows`` needs for ``n_rows`` rows of requests of up to
+    ``max_len`` positions."""
+    n, tiles = min(n_rows, KV8_ROWS_MOST), _kv8_tiles(n_heads, n_kv_heads)
+    return n * tiles * _kv8_most_chunks(n_heads, n_kv_heads, max_len) * _KV8_TILE_HEADS * (head_dim + 2), n * tiles
+
+
+def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
+                       scratch, counters, max_len: int, status, stream, rows=None, sinks=None) -> None:
+    """Attention of single queries (decode steps) over pages in 8 bits: row ``t`` of ``q`` and ``out`` (``[T, n_heads * head_dim]``, float32
+    or bfloat16) at position ``positions[t]`` of request ``token_req[t]`` sees keys ``max(0, p - window + 1) .. p`` (window 0: all).  ``rows``:
+    int32 row indices, the rows to take.  ``scratch`` and ``counters`` (zero before the first call, left zero) of ``kv8_rows_scratch``'s
+    sizes, one pair for each stream on which calls may overlap; ``max_len``: no row's position reaches it (a row beyond the block table is
+    left out, with a bit in ``status``).  ``sinks``: float32 ``[n_heads]``, one more term of each head's softmax denominator.  Rows of no
+    request (``token_req`` < 0) are left as they are.  A row's bits depend on its own request, ``max_len`` and the heads alone."""
+    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_rows")
+    code = dtype_code(q.dtype)
+    _need(q, None, "kv8_attention_rows q")
+    _need(out, q.dtype, "kv8_attention_rows out")
+    if n_heads <= 0 or n_heads % Hkv or q.dim() != 2 or q.shape != out.shape or q.shape[1] != n_heads * Dh:
+        raise KernelError(f"kv8_attention_rows: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_heads} heads of {Dh} over {Hkv}")
+    _kv8_rows_ints(positions, token_req, q.shape[0], "kv8_attention_rows")
+    n = q.shape[0]
+    if rows is not None:
+        _need(rows, torch.int32, "kv8_attention_rows rows")
+        n = rows.numel()
+    _need(scratch, torch.float32, "kv8_attention_rows scratch")
+    _need(counters, torch.int32, "kv8_attention_rows counters")
+    floats, tickets = kv8_rows_scratch(n, n_heads, Hkv, Dh, max_len)
+    if scratch.numel() < floats or counters.numel() < tickets:
+        raise KernelError(f"kv8_attention_rows: scratch of {scratch.numel()} floats and {counters.numel()} counters, {floats} and "
+                          f"{tickets} are needed")
+    ldq, ldo = _rows(q, "kv8_attention_rows q"), _rows(out, "kv8_attention_rows out")
+    sk = _sinks(sinks, n_heads, "kv8_attention_rows")
+    for a in range(0, n, KV8_ROWS_MOST):
+        b = min(n, a + KV8_ROWS_MOST)
+        if rows is not None:
+            part = (_p(q), ldq, _p(rows) + 4 * a, _p(positions), _p(token_req), _p(out))
+        else:
+            part = (_p(q) + a * ldq * q.element_size(), ldq, None, _p(positions) + 4 * a, _p(token_req) + 4 * a,
+                    _p(out) + a * ldo * out.element_size())
+        _call("kv8_rows", "mlxb_kv8_rows", _KV8_ROWS_ARGS, code, *part[:5], _p(block_table), block_table.shape[1], n_pages, page, n_heads,
+              Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(scratch), _p(counters),
+              _kv8_most_chunks(n_heads, Hkv, max_len), part[5], ldo, b - a, _p(status), sk, stream)
+
+
+def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
+                           status, stream, sinks=None) -> None:
+    raise KernelError("kv8_attention_portions: not built yet")
 
 
 # --------------------------------------------------------------------------
