@@ -1,4 +1,4 @@
-// Attention of single queries over pages in 8 bits on the CUDA cores, all arithmetic in float32.
+// Attention of single float32 queries over pages in 8 bits on the CUDA cores, all arithmetic in float32.
 //
 // y = sum_j exp(s_j - M) v_j / sum_j exp(s_j - M), s_j = scale * (q . k_j), over the keys j that the row sees, k_j and v_j codes
 // times the scale of their block of 16 positions and head; a sink adds exp(sink - M) to the sum below.  One pass over the keys: LPK
@@ -19,7 +19,7 @@ __device__ __forceinline__ void codes16(const uint4& c, float (&f)[16]) {
   for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(__byte_perm(w[i >> 2], 0x4b000000u, 0x7540 + (i & 3))) - 8388736.f;
 }
 
-template <typename T, int LPK>
+template <int LPK>
 __global__ void __launch_bounds__(WARPS * 32)
 rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
   constexpr int KPW = 32 / LPK, NG = WARPS * KPW;     // keys at a time: of a warp, of the CTA
@@ -44,13 +44,13 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
     const int* bt = a.block_table + (size_t)x.row.req * a.max_pages;
     const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
     float q[HT][16], o[HT][16], m[HT], l[HT];
-    const T* qr = after_wait((const T*)a.q) + (size_t)x.row.tok * a.ldq + (size_t)h0 * D + part * 16;
+    const float* qr = after_wait((const float*)a.q) + (size_t)x.row.tok * a.ldq + (size_t)h0 * D + part * 16;
 #pragma unroll
     for (int h = 0; h < HT; ++h) {
       m[h] = -INFINITY; l[h] = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        q[h][i] = mine && h < nh ? to_f(qr[h * D + i]) : 0.f;
+        q[h][i] = mine && h < nh ? qr[h * D + i] : 0.f;
         o[h][i] = 0.f;
       }
     }
@@ -136,7 +136,7 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
       if (d == 0) { fin_m[h] = top; fin_l[h] = tot; }
     }
     __syncthreads();
-    finish_item<T>(a, x, tiles, HT, h0, nh, fin_m, fin_l, fin_o, weights, &last, 1.f, [](float v) { return expf(v); });
+    finish_item<float>(a, x, tiles, HT, h0, nh, fin_m, fin_l, fin_o, weights, &last, 1.f, [](float v) { return expf(v); });
     __syncthreads();
   }
 }
@@ -144,19 +144,19 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
 // out [row, Hq * dim] for the rows `rows` (int32 indices into positions, token_req, q and out; null: rows 0 .. n_rows - 1): one query
 // of each head at the row's position.  partial: n_rows * tiles * most_chunks * 4 * (dim + 2) floats; counters: n_rows * tiles, zero
 // before the first call and left zero (tiles: Hkv * ceil(Hq / Hkv / 4)).
-MLXB_EXPORT int mlxb_kv8_rows(int dtype, const void* q, int ldq, const int* rows, const int* positions, const int* token_req,
+MLXB_EXPORT int mlxb_kv8_rows(const float* q, int ldq, const int* rows, const int* positions, const int* token_req,
                               const int* block_table, int max_pages, int n_pages, int page, int Hq, int Hkv, int dim, int window,
                               float scale, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, float* partial,
-                              int* counters, int most_chunks, void* out, int ldo, int n_rows, int* status, const float* sinks,
+                              int* counters, int most_chunks, float* out, int ldo, int n_rows, int* status, const float* sinks,
                               cudaStream_t stream) {
-  if (dtype != MLXB_F32 && dtype != MLXB_BF16) return mlxb_fail(MLXB_BAD_DTYPE, "kv8_rows: dtype code %d", dtype);
   if (n_rows <= 0) return 0;
   if (n_rows > ROWS_MOST) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d rows, a launch takes %d", n_rows, ROWS_MOST);
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d query heads over %d key/value heads", Hq, Hkv);
   if (dim % 16 || dim < 16 || dim > 256) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: head size %d (a multiple of 16 up to 256)", dim);
   if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: page size %d (a power of two of at least %d)", page, BLK);
   if (most_chunks <= 0) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d chunks of a row", most_chunks);
-  if (((uintptr_t)k8 | (uintptr_t)v8) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: pools must be 16-byte aligned");
+  if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)partial) & 15)
+    return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: pools and scratch memory must be 16-byte aligned");
   const RowsArgs a{q, ldq, rows, positions, token_req, block_table, max_pages, n_pages, page, Hq, Hkv, dim, window, scale, k8, v8, ks,
                    vs, sinks, partial, counters, most_chunks, out, ldo, n_rows, status};
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
@@ -164,18 +164,10 @@ MLXB_EXPORT int mlxb_kv8_rows(int dtype, const void* q, int ldq, const int* rows
   const long long most = (long long)n_rows * most_chunks * tiles, fill = 4ll * mlxb_sm_count();
   const dim3 grid((unsigned)(most < fill ? most : fill));
   auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(WARPS * 32), smem, stream, a, tiles, group_tiles); };
-  if (dtype == MLXB_F32) {
-    if (dim <= 16) go(rows_kernel<float, 1>);
-    else if (dim <= 32) go(rows_kernel<float, 2>);
-    else if (dim <= 64) go(rows_kernel<float, 4>);
-    else if (dim <= 128) go(rows_kernel<float, 8>);
-    else go(rows_kernel<float, 16>);
-  } else {
-    if (dim <= 16) go(rows_kernel<__nv_bfloat16, 1>);
-    else if (dim <= 32) go(rows_kernel<__nv_bfloat16, 2>);
-    else if (dim <= 64) go(rows_kernel<__nv_bfloat16, 4>);
-    else if (dim <= 128) go(rows_kernel<__nv_bfloat16, 8>);
-    else go(rows_kernel<__nv_bfloat16, 16>);
-  }
+  if (dim <= 16) go(rows_kernel<1>);
+  else if (dim <= 32) go(rows_kernel<2>);
+  else if (dim <= 64) go(rows_kernel<4>);
+  else if (dim <= 128) go(rows_kernel<8>);
+  else go(rows_kernel<16>);
   return mlxb_check_launch("kv8_rows");
 }

@@ -150,30 +150,40 @@ __device__ __forceinline__ void finish_item(const RowsArgs& a, const Item& x, in
   __threadfence();
   if (threadIdx.x == 0) *counter = 0;
   const float* all = a.partial + slot * per;
-  // weights of the chunks: exp(m_c - M) / total
-  for (int h = threadIdx.x; h < nh; h += blockDim.x) {
+  // weights of the chunks: exp(m_c - M) / total, a warp a head, a lane a chunk
+  const int lane = threadIdx.x & 31;
+  for (int h = threadIdx.x >> 5; h < nh; h += blockDim.x >> 5) {
     float top = -INFINITY, total = 0.f;
     bool odd = false;                                  // fmaxf leaves NaN out
-    for (int c = 0; c < x.n_chunks; ++c) {
+    for (int c = lane; c < x.n_chunks; c += 32) {
       const float mc = __ldcg(all + c * per + h);
       odd |= mc != mc;
       top = fmaxf(top, mc);
     }
-    if (odd) top = NAN;
-    for (int c = 0; c < x.n_chunks; ++c) {
+    top = __any_sync(0xffffffffu, odd) ? NAN : warp_max(top);
+    for (int c = lane; c < x.n_chunks; c += 32) {
       const float w = exp_(__ldcg(all + c * per + h) - top);
       weights[c * tile_heads + h] = w;
-      total += w * __ldcg(all + c * per + tile_heads + h);
+      total = fmaf(w, __ldcg(all + c * per + tile_heads + h), total);
     }
+    total = warp_sum(total);
     if (a.sinks) total += exp_(a.sinks[h0 + h] * sink_unit - top);
-    weights[a.most_chunks * tile_heads + h] = total != 0.f ? 1.f / total : 0.f;
+    if (lane == 0) weights[a.most_chunks * tile_heads + h] = total != 0.f ? 1.f / total : 0.f;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < nh * D; e += blockDim.x) {
+  for (int e = 4 * threadIdx.x; e < nh * D; e += 4 * blockDim.x) {
     const int h = e / D;
-    float sum = 0.f;
-#pragma unroll 8
-    for (int c = 0; c < x.n_chunks; ++c) sum = fmaf(weights[c * tile_heads + h], __ldcg(all + c * per + 2 * tile_heads + e), sum);
-    out[e] = from_f<T>(sum * weights[a.most_chunks * tile_heads + h]);
+    const float* w = weights + h;
+    const float* p = all + 2 * tile_heads + e;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+    for (int c = 0; c < x.n_chunks; ++c) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + c * per));
+      const float wc = w[c * tile_heads];
+      sum.x = fmaf(wc, v.x, sum.x); sum.y = fmaf(wc, v.y, sum.y); sum.z = fmaf(wc, v.z, sum.z); sum.w = fmaf(wc, v.w, sum.w);
+    }
+    const float r = w[a.most_chunks * tile_heads];
+    out[e] = from_f<T>(sum.x * r); out[e + 1] = from_f<T>(sum.y * r);
+    out[e + 2] = from_f<T>(sum.z * r); out[e + 3] = from_f<T>(sum.w * r);
   }
 }

@@ -807,7 +807,7 @@ def attention_decode(q, positions, token_req, block_table, k_pool, v_pool, out, 
 
 
 # --------------------------------------------------------------------------
-# a cache of keys and values in 8 bits (csrc/kv8.cu, csrc/kv8_rows.cu)
+# a cache of keys and values in 8 bits (csrc/kv8.cu, csrc/kv8_rows.cu, csrc/kv8_rows_tc.cu)
 
 KV8_BLOCK = 16           # positions of a head that share a scale
 KV8_ROWS_MOST = 4096     # rows one launch takes (csrc/kv8_rows.cuh)
@@ -925,25 +925,32 @@ def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out,
           _p(v_out), _rows(v_out, "v_out"), n, _p(status), stream)
 
 
-_KV8_ROWS_ARGS = ([c_int, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] + [c_void_p] * 6 + [c_int, c_void_p, c_int, c_int]
+_KV8_ROWS_ARGS = ([c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] + [c_void_p] * 6 + [c_int, c_void_p, c_int, c_int]
                   + [c_void_p] * 3)
-_KV8_TILE_HEADS = 4      # query heads that a block of csrc/kv8_rows.cu takes
+_KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
+_KV8_CTAS = {torch.float32: 4, torch.bfloat16: 3}            # blocks of these on an SM
 
 
-def _kv8_tiles(n_heads: int, n_kv_heads: int) -> int:
-    return n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS)
+def kv8_rows_library(dtype, head_dim: int) -> str:
+    """The library whose kernel takes single queries of this type (one for each head size in bfloat16)."""
+    return "kv8_rows" if dtype == torch.float32 else f"kv8_rows_tc:MLXB_HEAD_DIM={head_dim}"
 
 
-def _kv8_most_chunks(n_heads: int, n_kv_heads: int, max_len: int) -> int:
-    """The most parts a row's keys are cut into: what fills the device with one row, and no more than the longest row has."""
-    return max(1, min(3 * 148 // _kv8_tiles(n_heads, n_kv_heads), -(-(max_len + KV8_BLOCK) // 128)))
+def _kv8_plan(dtype, n_heads: int, n_kv_heads: int, max_len: int):
+    """``(tiles of heads, most parts of a row's keys)``: as many parts as fill the device with one row, and no more than the longest row has."""
+    tiles = n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS[dtype])
+    return tiles, max(1, min(_KV8_CTAS[dtype] * 148 // tiles, -(-(max_len + KV8_BLOCK) // 128)))
 
 
 def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
     """``(float32 elements of scratch memory, int32 counters)`` that ``kv8_attention_rows`` needs for ``n_rows`` rows of requests of up to
     ``max_len`` positions."""
-    n, tiles = min(n_rows, KV8_ROWS_MOST), _kv8_tiles(n_heads, n_kv_heads)
-    return n * tiles * _kv8_most_chunks(n_heads, n_kv_heads, max_len) * _KV8_TILE_HEADS * (head_dim + 2), n * tiles
+    n = min(n_rows, KV8_ROWS_MOST)
+    floats = tickets = 0
+    for dtype, heads in _KV8_TILE_HEADS.items():
+        tiles, most = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
+        floats, tickets = max(floats, n * tiles * most * heads * (head_dim + 2)), max(tickets, n * tiles)
+    return floats, tickets
 
 
 def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
@@ -955,7 +962,7 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
     left out, with a bit in ``status``).  ``sinks``: float32 ``[n_heads]``, one more term of each head's softmax denominator.  Rows of no
     request (``token_req`` < 0) are left as they are.  A row's bits depend on its own request, ``max_len`` and the heads alone."""
     n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_rows")
-    code = dtype_code(q.dtype)
+    dtype_code(q.dtype)
     _need(q, None, "kv8_attention_rows q")
     _need(out, q.dtype, "kv8_attention_rows out")
     if n_heads <= 0 or n_heads % Hkv or q.dim() != 2 or q.shape != out.shape or q.shape[1] != n_heads * Dh:
@@ -973,6 +980,8 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
                           f"{tickets} are needed")
     ldq, ldo = _rows(q, "kv8_attention_rows q"), _rows(out, "kv8_attention_rows out")
     sk = _sinks(sinks, n_heads, "kv8_attention_rows")
+    most = _kv8_plan(q.dtype, n_heads, Hkv, max_len)[1]
+    lib, name = kv8_rows_library(q.dtype, Dh), "mlxb_kv8_rows" if q.dtype == torch.float32 else "mlxb_kv8_rows_tc"
     for a in range(0, n, KV8_ROWS_MOST):
         b = min(n, a + KV8_ROWS_MOST)
         if rows is not None:
@@ -980,9 +989,9 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         else:
             part = (_p(q) + a * ldq * q.element_size(), ldq, None, _p(positions) + 4 * a, _p(token_req) + 4 * a,
                     _p(out) + a * ldo * out.element_size())
-        _call("kv8_rows", "mlxb_kv8_rows", _KV8_ROWS_ARGS, code, *part[:5], _p(block_table), block_table.shape[1], n_pages, page, n_heads,
-              Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(scratch), _p(counters),
-              _kv8_most_chunks(n_heads, Hkv, max_len), part[5], ldo, b - a, _p(status), sk, stream)
+        _call(lib, name, _KV8_ROWS_ARGS, *part[:5], _p(block_table), block_table.shape[1], n_pages, page, n_heads,
+              Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(scratch), _p(counters), most,
+              part[5], ldo, b - a, _p(status), sk, stream)
 
 
 def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
