@@ -32,7 +32,7 @@ struct RowsArgs {
 
 // Keys of a chunk for a row of n keys: a multiple of 64 that cuts them into at most `most` chunks.
 __device__ __forceinline__ int chunk_keys(int n, int most) {
-  const int c = n <= 1024 ? 128 : n <= 4096 ? 256 : 512;
+  const int c = n <= 1024 ? 128 : 256;
   const int least = ((n + most - 1) / most + 63) & ~63;
   return c > least ? c : least;
 }

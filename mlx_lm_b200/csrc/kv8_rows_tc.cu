@@ -1,13 +1,14 @@
-// Attention of single queries over pages in 8 bits for bfloat16 queries: the products on the tensor cores, the keys and values of a
-// tile straight from memory into the registers that the products take.  Built once for each head size (MLXB_HEAD_DIM).
+// Attention of single queries over pages in 8 bits for bfloat16 queries: the products on the tensor cores, codes turned into their
+// operands in registers.  Built once for each head size (MLXB_HEAD_DIM).
 //
+// A warp works by itself, an item after the other: asynchronous copies bring its tiles into a ring of its own in shared memory, several
+// tiles ahead, and no block-wide wait stands between the items.  Rows of several chunks leave sums that a second kernel adds up.
 // A warp takes 16 keys at a time (a block with one scale; never more than one page) for up to eight query heads that read the same
 // key/value head, as m16n8k16 products:
 //   S^T [16 keys x 8 heads] = K [16 x dim] Q^T      the codes are A, row by row
 //   O^T [dim x 8 heads]    += V^T [dim x 16] P^T    the codes are A again, transposed
 // Which columns of K a thread's registers stand for is free as long as Q's do too, and which rows of O^T likewise, so a thread loads
-// 16 neighbouring bytes of a key where it needs four times four of them, and nothing goes through shared memory.  P leaves the first
-// product as [keys x heads] and enters the second as [heads x keys]: movmatrix turns it in two instructions.
+// 16 neighbouring bytes of a key where it needs four times four of them.  P leaves the first product as [keys x heads] and enters the second as [heads x keys]: movmatrix turns it in two instructions.
 // Codes become fp16: the code + 128 in the low byte of 1024 (one byte permutation for two), less 1152, both exact.  A query is scaled by
 // a power of two so that its largest number lies in [2^14, 2^15): its 8 bits stay exact in fp16 down to 2^-28 of the largest.  The
 // scale of a key block multiplies the scores, the scale of a value block the block's O, both in float32; P is rounded to fp16 (11
@@ -24,7 +25,10 @@ constexpr int DH = MLXB_HEAD_DIM;
 static_assert(DH % 16 == 0 && DH >= 16 && DH <= 256, "head size");
 constexpr int WARPS = 4;
 constexpr int HT = 8;                                   // query heads of an item
-constexpr int CTAS = DH > 128 ? 2 : 3;                  // of an SM
+constexpr int TILE = 2 * 16 * DH;                       // bytes of a tile: 16 keys, 16 values
+constexpr int STAGES = 12288 / TILE < 2 ? 2 : 12288 / TILE;      // of a warp's ring
+constexpr int CTAS = DH > 128 ? 3 : 4;                  // of an SM
+constexpr size_t RING = (size_t)WARPS * STAGES * TILE;
 constexpr int KT = DH / 16;                             // k steps of S, m tiles of O
 constexpr int KW = DH % 64 == 0 ? 16 : DH % 32 == 0 ? 8 : 4;      // bytes of a key a thread loads at once
 constexpr int NK = DH / 4 / KW;
@@ -34,21 +38,37 @@ constexpr int VR = VW >= 4 ? DH / 32 : DH / 16;         // registers of a value
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 8.f;
 
-struct Tile { uint32_t k[2][KT], v[4][VR]; };
-
+// Where 16-byte piece c of row r of a tile's keys (values) lies in shared memory: so that the eight lanes of a wide load meet in no
+// bank.  A key load's lanes stand on rows r, r + 1 (four neighbouring pieces each), a value load's on rows 0, 2, 4, 6 of the same one or
+// two pieces.
+__device__ __forceinline__ int key_at(int r, int c) {
+  if constexpr (DH % 128 == 0) return r * DH + ((c ^ ((r & 1) << 2)) << 4);
+  return r * DH + (c << 4);
+}
+__device__ __forceinline__ int value_at(int r, int c) {
+  if constexpr (DH % 128 == 0) return r * DH + ((c ^ (((r >> 1) & 3) << 1)) << 4);
+  if constexpr (DH == 64) {
+    const int s = (r >> 1) | ((r & 1) << 3);
+    return s * DH + ((c ^ (s & 2)) << 4);
+  }
+  return r * DH + (c << 4);
+}
 template <int W>
-__device__ __forceinline__ void load_bytes(const int8_t* p, uint32_t* r) {
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* r) {
   if constexpr (W == 16) {
-    const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
     r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
   } else if constexpr (W == 8) {
-    const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
     r[0] = u.x; r[1] = u.y;
   } else if constexpr (W == 4) {
-    r[0] = __ldcg(reinterpret_cast<const uint32_t*>(p));
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
   } else {
-    r[0] = __ldcg(reinterpret_cast<const unsigned short*>(p));
+    r[0] = *reinterpret_cast<const unsigned short*>(p);
   }
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const int8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // two codes + 128 (bytes a and b of w) as fp16
 template <int SEL>
@@ -78,34 +98,37 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return y;
 }
 
+constexpr int PART = 8 * (DH + 2);                      // floats of an item's sums: m[8], l[8], then O as the lanes hold it
+
+__device__ __forceinline__ int column_of(int c, int g) { return (c / VW * 8 + g) * VW + c % VW; }      // column c of lane group g's
+
 __global__ void __launch_bounds__(WARPS * 32, CTAS)
 rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
-  extern __shared__ int dyn[];                          // prefix sums, then the weights of the last step
-  __shared__ int warp_sums[WARPS], last;
-  __shared__ float sm_m[WARPS][HT], sm_l[WARPS][HT], fin_m[HT], fin_l[HT];
-  __shared__ float sm_o[WARPS][HT * DH];
-  int* prefix = dyn;
-  float* weights = reinterpret_cast<float*>(dyn + a.n_rows + 1);
+  extern __shared__ __align__(128) uint8_t ring[];      // the warps' tiles, then the prefix sums
+  __shared__ int warp_sums[WARPS];
+  int* prefix = reinterpret_cast<int*>(ring + RING);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int total = schedule(a, prefix, warp_sums) * tiles;
   const int G = a.Hq / a.Hkv, per = a.page / BLK;
+  uint8_t* my_ring = ring + warp * (STAGES * TILE);
+  const uint32_t my_ring_u32 = (uint32_t)__cvta_generic_to_shared(my_ring);
   pdl_wait();
   pdl_trigger();
   const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
   const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
-  for (int it = blockIdx.x; it < total; it += gridDim.x) {
+  for (int it = warp * gridDim.x + blockIdx.x; it < total; it += WARPS * gridDim.x) {
     const Item x = item_of(a, prefix, it, tiles);
     const int hk = x.tile / group_tiles, j0 = (x.tile - hk * group_tiles) * HT, nh = min(HT, G - j0), h0 = hk * G + j0;
     const int* bt = a.block_table + (size_t)x.row.req * a.max_pages;
     const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
-    const int n_tiles = (x.end - x.begin + BLK - 1) / BLK;        // of the item; this warp's: warp, warp + 4, ...
+    const int n_tiles = (x.end - x.begin + BLK - 1) / BLK;
 
-    // lane i knows the page, row and scales of the warp's i-th tile of the next 32
-    int pg_row = -1;                                    // page * page rows + row of the tile in its page, head 0; -1: no page
+    // lane i knows page, row in the page (-1: no page) and scales of the i-th of the next 32 tiles
+    int pg_row = -1;
     float skl = 0.f, svl = 0.f;
     int pg_id = 0;
     auto look_up = [&](int i0) {
-      const int i = warp + WARPS * (i0 + lane), key = x.begin + i * BLK;
+      const int i = i0 + lane, key = x.begin + i * BLK;
       pg_row = -1;
       if (i < n_tiles) {
         pg_id = page_of(a, bt, key);
@@ -119,27 +142,26 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       }
     };
     look_up(0);
-    auto fetch = [&](int i, Tile& f) {                  // tile i of the 32 looked up
-      const int r = __shfl_sync(0xffffffffu, pg_row, i), id = __shfl_sync(0xffffffffu, pg_id, i);
-      if (r < 0) return;
-      const size_t at = (((size_t)id * a.Hkv + hk) * a.page + r) * DH;
-      const int8_t* kp = k8 + at + (size_t)g * DH + t * KW;
+    // tile i of the 32 looked up, on its way into stage st; a group of copies for every tile, an empty one where there is none
+    auto fetch = [&](int i, int n, int st) {
+      if (i < n) {
+        const int r = __shfl_sync(0xffffffffu, pg_row, i), id = __shfl_sync(0xffffffffu, pg_id, i);
+        if (r >= 0) {
+          const size_t at = (((size_t)id * a.Hkv + hk) * a.page + r) * DH;
+          const uint32_t dst = my_ring_u32 + st * TILE;
 #pragma unroll
-      for (int i2 = 0; i2 < NK; ++i2) {
-        load_bytes<KW>(kp + i2 * 4 * KW, &f.k[0][i2 * (KW / 4)]);
-        load_bytes<KW>(kp + 8 * DH + i2 * 4 * KW, &f.k[1][i2 * (KW / 4)]);
+          for (int e0 = 0; e0 < DH; e0 += 32) {
+            const int e = e0 + lane, row = e / (DH / 16), c = e % (DH / 16);
+            if (DH % 32 == 0 || e < DH) {
+              copy16(dst + key_at(row, c), k8 + at + e * 16);
+              copy16(dst + 16 * DH + value_at(row, c), v8 + at + e * 16);
+            }
+          }
+        }
       }
-      const int8_t* vp = v8 + at + (size_t)(2 * t) * DH + g * VW;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int i2 = 0; i2 < NV; ++i2)
-          load_bytes<VW>(vp + ((j & 1) + (j >> 1) * 8) * DH + i2 * 8 * VW, &f.v[j][VW >= 4 ? i2 * (VW / 4) : i2]);
-      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    Tile buf[2];
-    const int mine = n_tiles > warp ? (n_tiles - warp + WARPS - 1) / WARPS : 0;
-    if (mine > 0) fetch(0, buf[0]);
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i, min(32, n_tiles), i);
 
     // the queries of head g: columns (i * 4 + t) * KW ..
     uint32_t qf[KT][2];
@@ -187,14 +209,23 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     for (int j = 0; j < KT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-    auto work = [&](int i, int i32, const Tile& f) {    // the warp's tile i, the i32-th of those looked up
+    auto work = [&](int i, int i32, int st) {           // tile i, the i32-th of those looked up
       if (__shfl_sync(0xffffffffu, pg_row, i32) < 0) return;
       const float sk = __shfl_sync(0xffffffffu, skl, i32), sv = __shfl_sync(0xffffffffu, svl, i32);
-      const int key = x.begin + (warp + WARPS * i) * BLK;
+      const int key = x.begin + i * BLK;
+      const uint8_t* kp = my_ring + st * TILE;
+      const uint8_t* vp = kp + 16 * DH;
+      uint32_t fk[2][KT];
+#pragma unroll
+      for (int i2 = 0; i2 < NK; ++i2) {
+        const int b = (i2 * 4 + t) * KW;
+        load_bytes<KW>(kp + key_at(g, b >> 4) + (b & 15), &fk[0][i2 * (KW / 4)]);
+        load_bytes<KW>(kp + key_at(g + 8, b >> 4) + (b & 15), &fk[1][i2 * (KW / 4)]);
+      }
       float c[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
-        const uint32_t u = f.k[0][j] ^ 0x80808080u, w = f.k[1][j] ^ 0x80808080u;
+        const uint32_t u = fk[0][j] ^ 0x80808080u, w = fk[1][j] ^ 0x80808080u;
         mma(j & 1 ? c2 : c, half2_of<0x5140>(u), half2_of<0x5140>(w), half2_of<0x5342>(u), half2_of<0x5342>(w), qf[j][0], qf[j][1]);
       }
       // scores of keys g and g + 8, heads 2t and 2t + 1, in units of log2
@@ -227,9 +258,18 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       l0 += p0 + p2;
       l1 += p1 + p3;
       const uint32_t pb0 = turned(pack_half2(p0, p1)), pb1 = turned(pack_half2(p2, p3));
+      uint32_t fv[4][VR];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i2 = 0; i2 < NV; ++i2) {
+          const int b = (i2 * 8 + g) * VW;
+          load_bytes<VW>(vp + value_at(2 * t + (j & 1) + (j >> 1) * 8, b >> 4) + (b & 15), &fv[j][VW >= 4 ? i2 * (VW / 4) : i2]);
+        }
+      }
 #pragma unroll
       for (int w = 0; w < VR; ++w) {
-        const uint32_t v0 = f.v[0][w] ^ 0x80808080u, v1 = f.v[1][w] ^ 0x80808080u, v2 = f.v[2][w] ^ 0x80808080u, v3 = f.v[3][w] ^ 0x80808080u;
+        const uint32_t v0 = fv[0][w] ^ 0x80808080u, v1 = fv[1][w] ^ 0x80808080u, v2 = fv[2][w] ^ 0x80808080u, v3 = fv[3][w] ^ 0x80808080u;
         const uint32_t lo01 = __byte_perm(v0, v1, 0x5140), lo23 = __byte_perm(v2, v3, 0x5140);
         constexpr int PER = VW >= 4 ? 2 : 1;            // m tiles of a register
         {
@@ -247,59 +287,130 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         }
       }
     };
-    for (int i0 = 0; i0 < mine; i0 += 32) {
+    for (int i0 = 0; i0 < n_tiles; i0 += 32) {
+      const int n = min(32, n_tiles - i0);
       if (i0 > 0) {
         look_up(i0);
-        fetch(0, buf[0]);
+        for (int i = 0; i < STAGES - 1; ++i) fetch(i, n, i);
       }
-      const int n = min(32, mine - i0);
-      for (int i = 0; i < n; i += 2) {
-        if (i + 1 < n) fetch(i + 1, buf[1]);
-        work(i0 + i, i, buf[0]);
-        if (i + 2 < n) fetch(i + 2, buf[0]);
-        if (i + 1 < n) work(i0 + i + 1, i + 1, buf[1]);
+      int st = 0;
+      for (int i = 0; i < n; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();                                   // every lane's copies of tile i are there, and tile i - 1 has been read
+        fetch(i + STAGES - 1, n, st == 0 ? STAGES - 1 : st - 1);
+        work(i0 + i, i, st);
+        st = st + 1 == STAGES ? 0 : st + 1;
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
     }
-    // the warps' sums
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, d);
       l1 += __shfl_xor_sync(0xffffffffu, l1, d);
     }
-    if (g == 0) {
-      sm_m[warp][2 * t] = m0; sm_m[warp][2 * t + 1] = m1;
-      sm_l[warp][2 * t] = l0; sm_l[warp][2 * t + 1] = l1;
-    }
+    const bool one = 2 * t < nh, two = 2 * t + 1 < nh;
+    if (x.n_chunks > 1) {
+      float* part = a.partial + (((size_t)x.index * tiles + x.tile) * a.most_chunks + x.chunk) * PART;
+      if (g == 0) {
+        reinterpret_cast<float2*>(part)[t] = make_float2(m0, m1);
+        reinterpret_cast<float2*>(part + 8)[t] = make_float2(l0, l1);
+      }
+      if (one) {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) {
+        for (int j = 0; j < KT; ++j)
+          __stcg(reinterpret_cast<float4*>(part + 16) + j * 32 + lane, make_float4(o[j][0], o[j][1], o[j][2], o[j][3]));
+      }
+    } else {
+      if (a.sinks) {
+        if (one) l0 += ex2(a.sinks[h0 + 2 * t] * LOG2E - m0);
+        if (two) l1 += ex2(a.sinks[h0 + 2 * t + 1] * LOG2E - m1);
+      }
+      const float r0 = l0 != 0.f ? 1.f / l0 : 0.f, r1 = l1 != 0.f ? 1.f / l1 : 0.f;
+      __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)x.row.tok * a.ldo + (size_t)(h0 + 2 * t) * DH;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {                     // column 2 j + e of this thread's
-        const int c = 2 * j + e, d = (c / VW * 8 + g) * VW + c % VW;
-        if (2 * t < nh) sm_o[warp][2 * t * DH + d] = o[j][2 * e];
-        if (2 * t + 1 < nh) sm_o[warp][(2 * t + 1) * DH + d] = o[j][2 * e + 1];
+      for (int j = 0; j < KT; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = column_of(2 * j + e, g);
+          if (one) out[d] = __float2bfloat16_rn(o[j][2 * e] * r0);
+          if (two) out[DH + d] = __float2bfloat16_rn(o[j][2 * e + 1] * r1);
+        }
       }
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < nh * DH; e += WARPS * 32) {
-      const int h = e / DH;
-      float top = sm_m[0][h];
-#pragma unroll
-      for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w][h]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, tot = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float c = ex2(sm_m[w][h] - base);
-        sum = fmaf(sm_o[w][e], c, sum);
-        tot = fmaf(sm_l[w][h], c, tot);
-      }
-      sm_o[0][e] = sum;
-      if (e == h * DH) { fin_m[h] = top; fin_l[h] = tot; }
-    }
-    __syncthreads();
-    finish_item<__nv_bfloat16>(a, x, tiles, HT, h0, nh, fin_m, fin_l, sm_o[0], weights, &last, LOG2E, [](float v) { return ex2(v); });
-    __syncthreads();
   }
+}
+
+// The sums of a row's chunks, added in the order of four runs of chunks: a block takes 16 columns of a (row, tile of heads).
+__global__ void __launch_bounds__(128)
+rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
+  extern __shared__ float weights[];                    // [chunk][8]
+  __shared__ float red[4][8];
+  __shared__ float4 sums[4][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
+  const int i = blockIdx.x / tiles, tile = blockIdx.x - i * tiles, j = blockIdx.y;
+  const RowSpan row = row_span(a, i, false);
+  const int c_keys = row.n ? chunk_keys(row.n, a.most_chunks) : 1, n = (row.n + c_keys - 1) / c_keys;
+  pdl_wait();
+  pdl_trigger();
+  if (n <= 1) return;
+  const int hk = tile / group_tiles, G = a.Hq / a.Hkv, j0 = (tile - hk * group_tiles) * HT, nh = min(HT, G - j0), h0 = hk * G + j0;
+  const float* all = after_wait(a.partial) + (size_t)blockIdx.x * a.most_chunks * PART;
+  const bool mine = 2 * t < nh;
+  const int per = (n + 3) / 4, c0 = warp * per, c1 = min(n, c0 + per);
+  const int h = threadIdx.x & 7;
+  float top = -INFINITY;
+  bool odd = false;                                     // fmaxf leaves NaN out
+  for (int c = threadIdx.x >> 3; c < n; c += 16) {
+    const float m = __ldcg(all + (size_t)c * PART + h);
+    weights[c * 8 + h] = m;
+    odd |= m != m;
+    top = fmaxf(top, m);
+  }
+  if (odd) top = INFINITY;                              // inf - inf below: NaN for the whole head
+#pragma unroll
+  for (int d = 8; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane < 8) red[warp][lane] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][h], red[1][h]), fmaxf(red[2][h], red[3][h]));
+  __syncthreads();
+  float total = 0.f;
+  for (int c = threadIdx.x >> 3; c < n; c += 16) {
+    const float w = ex2(weights[c * 8 + h] - top);
+    weights[c * 8 + h] = w;
+    total = fmaf(w, __ldcg(all + (size_t)c * PART + 8 + h), total);
+  }
+#pragma unroll
+  for (int d = 8; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+  if (lane < 8) red[warp][lane] = total;
+  __syncthreads();
+  total = red[0][h] + red[1][h] + red[2][h] + red[3][h];
+  if (a.sinks && h < nh) total += ex2(a.sinks[h0 + h] * LOG2E - top);
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine) {
+#pragma unroll 8
+    for (int c = c0; c < c1; ++c) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(all + (size_t)c * PART + 16) + j * 32 + lane);
+      const float2 w = *reinterpret_cast<const float2*>(weights + c * 8 + 2 * t);
+      s.x = fmaf(w.x, v.x, s.x); s.y = fmaf(w.y, v.y, s.y); s.z = fmaf(w.x, v.z, s.z); s.w = fmaf(w.y, v.w, s.w);
+    }
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (threadIdx.x < 8) red[0][threadIdx.x] = inv;
+  __syncthreads();
+  // 8 heads x 16 columns, one a thread: head hh, the column of lane group gg and slot e
+  const int hh = threadIdx.x & 7, gg = (threadIdx.x >> 3) & 7, e = threadIdx.x >> 6;
+  if (hh >= nh) return;
+  float y = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float4 v = sums[w][gg * 4 + (hh >> 1)];
+    y += e ? (hh & 1 ? v.w : v.z) : (hh & 1 ? v.y : v.x);
+  }
+  __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)row.tok * a.ldo + (size_t)(h0 + hh) * DH;
+  out[column_of(2 * j + e, gg)] = __float2bfloat16_rn(y * red[0][hh]);
 }
 
 // As mlxb_kv8_rows for bfloat16 and heads of MLXB_HEAD_DIM; tiles of eight query heads: partial n_rows * tiles * most_chunks * 8 *
@@ -314,19 +425,21 @@ MLXB_EXPORT int mlxb_kv8_rows_tc(const void* q, int ldq, const int* rows, const 
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d query heads over %d key/value heads", Hq, Hkv);
   if (dim != DH) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: head size %d, this library is for %d", dim, DH);
   if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: page size %d (a power of two of at least %d)", page, BLK);
-  if (most_chunks <= 0) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d chunks of a row", most_chunks);
+  if (most_chunks <= 0 || most_chunks > 1024) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d chunks of a row", most_chunks);
   if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)partial) & 15)
     return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: pools and scratch memory must be 16-byte aligned");
   const RowsArgs a{q, ldq, rows, positions, token_req, block_table, max_pages, n_pages, page, Hq, Hkv, dim, window, scale, k8, v8, ks,
                    vs, sinks, partial, counters, most_chunks, out, ldo, n_rows, status};
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
-  const size_t smem = (size_t)(n_rows + 1 + (most_chunks + 1) * HT) * 4;
+  const size_t smem = RING + (size_t)(n_rows + 1) * 4;
   const long long most = (long long)n_rows * most_chunks * tiles, fill = (long long)CTAS * mlxb_sm_count();
   static SharedLimit limit;
-  const size_t all = (ROWS_MOST + 1 + 4096) * 4;
-  if (smem > all) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d rows, %d chunks", n_rows, most_chunks);
-  if (cudaError_t e = limit.raise(rows_tc_kernel, all)) return mlxb_fail((int)e, "kv8_rows_tc: shared memory: %s", cudaGetErrorString(e));
+  if (cudaError_t e = limit.raise(rows_tc_kernel, RING + (ROWS_MOST + 1) * 4))
+    return mlxb_fail((int)e, "kv8_rows_tc: shared memory: %s", cudaGetErrorString(e));
   launch_pdl(rows_tc_kernel, dim3((unsigned)(most < fill ? most : fill)), dim3(WARPS * 32), smem, stream, a, tiles, group_tiles,
              (ldq % 4 == 0 && !((uintptr_t)q & 7)) ? 1 : 0);
-  return mlxb_check_launch("kv8_rows_tc");
+  if (int e = mlxb_check_launch("kv8_rows_tc")) return e;
+  if (most_chunks == 1) return 0;
+  launch_pdl(rows_tc_join_kernel, dim3((unsigned)n_rows * tiles, KT), dim3(128), (size_t)most_chunks * 32, stream, a, tiles, group_tiles);
+  return mlxb_check_launch("kv8_rows_tc (join)");
 }

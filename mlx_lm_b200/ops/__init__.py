@@ -928,7 +928,7 @@ def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out,
 _KV8_ROWS_ARGS = ([c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] + [c_void_p] * 6 + [c_int, c_void_p, c_int, c_int]
                   + [c_void_p] * 3)
 _KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
-_KV8_CTAS = {torch.float32: 4, torch.bfloat16: 3}            # blocks of these on an SM
+_KV8_ITEMS = {torch.float32: 4 * 148, torch.bfloat16: 8 * 148}      # parts of one row's keys that fill the device
 
 
 def kv8_rows_library(dtype, head_dim: int) -> str:
@@ -939,7 +939,7 @@ def kv8_rows_library(dtype, head_dim: int) -> str:
 def _kv8_plan(dtype, n_heads: int, n_kv_heads: int, max_len: int):
     """``(tiles of heads, most parts of a row's keys)``: as many parts as fill the device with one row, and no more than the longest row has."""
     tiles = n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS[dtype])
-    return tiles, max(1, min(_KV8_CTAS[dtype] * 148 // tiles, -(-(max_len + KV8_BLOCK) // 128)))
+    return tiles, max(1, min(_KV8_ITEMS[dtype] // tiles, -(-(max_len + KV8_BLOCK) // 128)))
 
 
 def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
