@@ -9,11 +9,15 @@
 //   O^T [dim x 8 heads]    += V^T [dim x 16] P^T    the codes are A again, transposed
 // Which columns of K a thread's registers stand for is free as long as Q's do too, and which rows of O^T likewise, so a thread loads
 // 16 neighbouring bytes of a key where it needs four times four of them.  P leaves the first product as [keys x heads] and enters the second as [heads x keys]: movmatrix turns it in two instructions.
-// Codes become fp16: the code + 128 in the low byte of 1024 (one byte permutation for two), less 1152, both exact.  A query is scaled by
-// a power of two so that its largest number lies in [2^14, 2^15): its 8 bits stay exact in fp16 down to 2^-28 of the largest.  The
-// scale of a key block multiplies the scores, the scale of a value block the block's O, both in float32; P is rounded to fp16 (11
-// bits, 2^-12 of a weight).  The maximum that the exponentials are relative to follows a score only once that is more than 8 (a factor
-// 256) beyond it: all scores of a row stay below 2^8 in P, and most tiles need neither shuffles nor another scaling of O.
+// A code enters a product as fp16 bits 00uu, u = code + 128: the subnormal number u * 2^-24, exact, for one bit operation on two codes
+// (two for the odd bytes).  The 128 comes off where a product starts: K Q^T begins at -128 sum(q), known once a row, and V^T P^T at
+// -128 sum(p), which a product with ones gives and which is the softmax's sum below as well (of the weights as they were rounded).
+// A query is scaled by a power of two so that its largest number lies in [2^14, 2^15): its 8 bits stay exact in fp16 down to 2^-28 of
+// the largest.  The scale of a key block multiplies the scores, that of a value block the block's O, both in float32; P is rounded to
+// fp16 (11 bits, 2^-12 of a weight).  The maximum that the exponentials are relative to follows a score only once that is more than 8
+// (a factor 256) beyond it: most tiles need neither shuffles nor another scaling of O.
+#include <cuda_fp16.h>
+
 #include "kv8_rows.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -37,6 +41,8 @@ constexpr int NV = DH / 8 / VW;
 constexpr int VR = VW >= 4 ? DH / 32 : DH / 16;         // registers of a value
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 8.f;
+constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24: what a code's operand counts in
+constexpr uint32_t ONES = 0x3c003c00u;
 
 // Where 16-byte piece c of row r of a tile's keys (values) lies in shared memory: so that the eight lanes of a wide load meet in no
 // bank.  A key load's lanes stand on rows r, r + 1 (four neighbouring pieces each), a value load's on rows 0, 2, 4, 6 of the same one or
@@ -70,21 +76,22 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* r) {
 __device__ __forceinline__ void copy16(uint32_t dst, const int8_t* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// two codes + 128 (bytes a and b of w) as fp16
-template <int SEL>
-__device__ __forceinline__ uint32_t half2_of(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, SEL);
+// Bytes 0 and 2 (1 and 3) of w, each + 128, as the low bits of two fp16: (code + 128) * 2^-24, exact (a subnormal number).
+__device__ __forceinline__ uint32_t even(uint32_t w) {
   uint32_t y;
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(w), "r"(0x00ff00ffu), "r"(0x00800080u));      // (a & b) ^ c
   return y;
 }
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ uint32_t odd(uint32_t w) { return even(w >> 8); }
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                    float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t turned(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -114,6 +121,9 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
   const uint32_t my_ring_u32 = (uint32_t)__cvta_generic_to_shared(my_ring);
   pdl_wait();
   pdl_trigger();
+  // where this lane's pieces of a tile lie, the same for every tile
+  const int key_base = key_at(g, (t * KW) >> 4) + ((t * KW) & 15), key_other = DH % 128 == 0 ? key_base ^ 64 : key_base + 4 * KW;
+  const int value_base = value_at(2 * t, (g * VW) >> 4) + ((g * VW) & 15);
   const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
   const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
   for (int it = warp * gridDim.x + blockIdx.x; it < total; it += WARPS * gridDim.x) {
@@ -123,39 +133,35 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
     const int n_tiles = (x.end - x.begin + BLK - 1) / BLK;
 
-    // lane i knows page, row in the page (-1: no page) and scales of the i-th of the next 32 tiles
-    int pg_row = -1;
+    // lane i knows of the i-th of the next 32 tiles which tile of the pool it is, and its scales; missing: tiles without a page
+    uint32_t tile_id = 0, missing = 0;
     float skl = 0.f, svl = 0.f;
-    int pg_id = 0;
     auto look_up = [&](int i0) {
       const int i = i0 + lane, key = x.begin + i * BLK;
-      pg_row = -1;
+      bool none = false;
       if (i < n_tiles) {
-        pg_id = page_of(a, bt, key);
-        if (pg_id >= 0) {
-          const int r = key & (a.page - 1);
-          pg_row = r;
-          const size_t at = ((size_t)pg_id * a.Hkv + hk) * per + r / BLK;
-          skl = __ldcg(ks + at);
-          svl = __ldcg(vs + at);
+        const int pg = page_of(a, bt, key);
+        none = pg < 0;
+        if (!none) {
+          tile_id = (uint32_t)(pg * a.Hkv + hk) * per + (key & (a.page - 1)) / BLK;
+          skl = __ldcg(ks + tile_id);
+          svl = __ldcg(vs + tile_id);
         }
       }
+      missing = __ballot_sync(0xffffffffu, none);
     };
     look_up(0);
     // tile i of the 32 looked up, on its way into stage st; a group of copies for every tile, an empty one where there is none
     auto fetch = [&](int i, int n, int st) {
-      if (i < n) {
-        const int r = __shfl_sync(0xffffffffu, pg_row, i), id = __shfl_sync(0xffffffffu, pg_id, i);
-        if (r >= 0) {
-          const size_t at = (((size_t)id * a.Hkv + hk) * a.page + r) * DH;
-          const uint32_t dst = my_ring_u32 + st * TILE;
+      if (i < n && !(missing >> i & 1)) {
+        const size_t at = (size_t)__shfl_sync(0xffffffffu, tile_id, i) * (16 * DH) + lane * 16;
+        const uint32_t dst = my_ring_u32 + st * TILE;
 #pragma unroll
-          for (int e0 = 0; e0 < DH; e0 += 32) {
-            const int e = e0 + lane, row = e / (DH / 16), c = e % (DH / 16);
-            if (DH % 32 == 0 || e < DH) {
-              copy16(dst + key_at(row, c), k8 + at + e * 16);
-              copy16(dst + 16 * DH + value_at(row, c), v8 + at + e * 16);
-            }
+        for (int e0 = 0; e0 < DH; e0 += 32) {
+          const int e = e0 + lane, row = e / (DH / 16), c = e % (DH / 16);
+          if (DH % 32 == 0 || e < DH) {
+            copy16(dst + key_at(row, c), k8 + at + e0 * 16);
+            copy16(dst + 16 * DH + value_at(row, c), v8 + at + e0 * 16);
           }
         }
       }
@@ -165,7 +171,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
 
     // the queries of head g: columns (i * 4 + t) * KW ..
     uint32_t qf[KT][2];
-    float fac;
+    float fac, bias = 0.f;
     {
       const __nv_bfloat16* qr = after_wait((const __nv_bfloat16*)a.q) + (size_t)x.row.tok * a.ldq + (size_t)(h0 + g) * DH;
       float v[KT][4];
@@ -197,11 +203,20 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       const float up = __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
-        qf[j][0] = pack_half2(v[j][0] * up, v[j][1] * up);
-        qf[j][1] = pack_half2(v[j][2] * up, v[j][3] * up);
+        qf[j][0] = pack_half2(v[j][0] * up, v[j][2] * up);
+        qf[j][1] = pack_half2(v[j][1] * up, v[j][3] * up);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {                   // (the sum of what the products take)
+          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&qf[j][e]));
+          bias += u.x + u.y;
+        }
       }
-      fac = __uint_as_float((uint32_t)(127 - 14 + e2) << 23) * (a.scale * LOG2E);
+      bias += __shfl_xor_sync(0xffffffffu, bias, 1);
+      bias += __shfl_xor_sync(0xffffffffu, bias, 2);
+      bias *= -128.f * UNIT;
+      fac = __uint_as_float((uint32_t)(127 - 14 + e2) << 23) * (a.scale * LOG2E / UNIT);
     }
+    const float bias0 = __shfl_sync(0xffffffffu, bias, 8 * t), bias1 = __shfl_sync(0xffffffffu, bias, 8 * t + 4);
     const float fac0 = __shfl_sync(0xffffffffu, fac, 8 * t), fac1 = __shfl_sync(0xffffffffu, fac, 8 * t + 4);      // of heads 2t, 2t + 1
 
     float o[KT][4];
@@ -210,28 +225,28 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     auto work = [&](int i, int i32, int st) {           // tile i, the i32-th of those looked up
-      if (__shfl_sync(0xffffffffu, pg_row, i32) < 0) return;
+      if (missing >> i32 & 1) return;
       const float sk = __shfl_sync(0xffffffffu, skl, i32), sv = __shfl_sync(0xffffffffu, svl, i32);
-      const int key = x.begin + i * BLK;
       const uint8_t* kp = my_ring + st * TILE;
-      const uint8_t* vp = kp + 16 * DH;
+      const uint8_t* vp = kp + 16 * DH + value_base;
       uint32_t fk[2][KT];
 #pragma unroll
       for (int i2 = 0; i2 < NK; ++i2) {
-        const int b = (i2 * 4 + t) * KW;
-        load_bytes<KW>(kp + key_at(g, b >> 4) + (b & 15), &fk[0][i2 * (KW / 4)]);
-        load_bytes<KW>(kp + key_at(g + 8, b >> 4) + (b & 15), &fk[1][i2 * (KW / 4)]);
+        const uint8_t* p = DH % 128 == 0 ? kp + (i2 & 1 ? key_other : key_base) + (i2 >> 1) * 128 : kp + key_base + i2 * 4 * KW;
+        load_bytes<KW>(p, &fk[0][i2 * (KW / 4)]);
+        load_bytes<KW>(p + 8 * DH, &fk[1][i2 * (KW / 4)]);
       }
-      float c[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+      float c[4] = {bias0, bias1, bias0, bias1}, c2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
-        const uint32_t u = fk[0][j] ^ 0x80808080u, w = fk[1][j] ^ 0x80808080u;
-        mma(j & 1 ? c2 : c, half2_of<0x5140>(u), half2_of<0x5140>(w), half2_of<0x5342>(u), half2_of<0x5342>(w), qf[j][0], qf[j][1]);
+        float (&d)[4] = j & 1 ? c2 : c;
+        mma(d, even(fk[0][j]), even(fk[1][j]), odd(fk[0][j]), odd(fk[1][j]), qf[j][0], qf[j][1], d[0], d[1], d[2], d[3]);
       }
       // scores of keys g and g + 8, heads 2t and 2t + 1, in units of log2
       const float a0 = sk * fac0, a1 = sk * fac1;
       float s0 = (c[0] + c2[0]) * a0, s1 = (c[1] + c2[1]) * a1, s2 = (c[2] + c2[2]) * a0, s3 = (c[3] + c2[3]) * a1;
-      if (key < lo || key + BLK > x.end) {
+      if (i == 0 || i == n_tiles - 1) {                 // (a window begins in a row's first tile)
+        const int key = x.begin + i * BLK;
         const bool in = key + g >= lo && key + g < x.end, in8 = key + g + 8 >= lo && key + g + 8 < x.end;
         if (!in) s0 = s1 = -INFINITY;
         if (!in8) s2 = s3 = -INFINITY;
@@ -255,35 +270,33 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       }
       const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
       const float p0 = ex2(s0 - b0), p1 = ex2(s1 - b1), p2 = ex2(s2 - b0), p3 = ex2(s3 - b1);
-      l0 += p0 + p2;
-      l1 += p1 + p3;
       const uint32_t pb0 = turned(pack_half2(p0, p1)), pb1 = turned(pack_half2(p2, p3));
+      float sum[4];                                     // of the weights as they were rounded, in every row
+      mma(sum, ONES, ONES, ONES, ONES, pb0, pb1, 0.f, 0.f, 0.f, 0.f);
+      l0 += sum[0];
+      l1 += sum[1];
+      const float n0 = sum[0] * (-128.f * UNIT), n1 = sum[1] * (-128.f * UNIT);
       uint32_t fv[4][VR];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int i2 = 0; i2 < NV; ++i2) {
-          const int b = (i2 * 8 + g) * VW;
-          load_bytes<VW>(vp + value_at(2 * t + (j & 1) + (j >> 1) * 8, b >> 4) + (b & 15), &fv[j][VW >= 4 ? i2 * (VW / 4) : i2]);
+          // row 2t + (j & 1) + 8 (j >> 1): the same pieces of it as of row 2t
+          const int at = DH == 64 ? (4 * (j >> 1) + 8 * (j & 1)) * DH : ((j & 1) + (j >> 1) * 8) * DH;
+          load_bytes<VW>(vp + at + i2 * 8 * VW, &fv[j][VW >= 4 ? i2 * (VW / 4) : i2]);
         }
       }
 #pragma unroll
       for (int w = 0; w < VR; ++w) {
-        const uint32_t v0 = fv[0][w] ^ 0x80808080u, v1 = fv[1][w] ^ 0x80808080u, v2 = fv[2][w] ^ 0x80808080u, v3 = fv[3][w] ^ 0x80808080u;
-        const uint32_t lo01 = __byte_perm(v0, v1, 0x5140), lo23 = __byte_perm(v2, v3, 0x5140);
-        constexpr int PER = VW >= 4 ? 2 : 1;            // m tiles of a register
-        {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma(d, half2_of<0x5140>(lo01), half2_of<0x5342>(lo01), half2_of<0x5140>(lo23), half2_of<0x5342>(lo23), pb0, pb1);
+        constexpr int PER = VW >= 4 ? 2 : 1;            // m tiles of a register: columns (0, 1) of two keys, then (2, 3)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[PER * w][e] = fmaf(sv, d[e], o[PER * w][e]);
-        }
-        if constexpr (PER == 2) {
-          const uint32_t hi01 = __byte_perm(v0, v1, 0x7362), hi23 = __byte_perm(v2, v3, 0x7362);
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma(d, half2_of<0x5140>(hi01), half2_of<0x5342>(hi01), half2_of<0x5140>(hi23), half2_of<0x5342>(hi23), pb0, pb1);
+        for (int r = 0; r < PER; ++r) {
+          const uint32_t x01 = __byte_perm(fv[0][w], fv[1][w], r ? 0x7632 : 0x5410);
+          const uint32_t x23 = __byte_perm(fv[2][w], fv[3][w], r ? 0x7632 : 0x5410);
+          float d[4];
+          mma(d, even(x01), odd(x01), even(x23), odd(x23), pb0, pb1, n0, n1, n0, n1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[PER * w + 1][e] = fmaf(sv, d[e], o[PER * w + 1][e]);
+          for (int e = 0; e < 4; ++e) o[PER * w + r][e] = fmaf(sv, d[e], o[PER * w + r][e]);
         }
       }
     };
@@ -304,11 +317,6 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
     }
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-    }
     const bool one = 2 * t < nh, two = 2 * t + 1 < nh;
     if (x.n_chunks > 1) {
       float* part = a.partial + (((size_t)x.index * tiles + x.tile) * a.most_chunks + x.chunk) * PART;
@@ -326,7 +334,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         if (one) l0 += ex2(a.sinks[h0 + 2 * t] * LOG2E - m0);
         if (two) l1 += ex2(a.sinks[h0 + 2 * t + 1] * LOG2E - m1);
       }
-      const float r0 = l0 != 0.f ? 1.f / l0 : 0.f, r1 = l1 != 0.f ? 1.f / l1 : 0.f;
+      const float r0 = l0 != 0.f ? 1.f / (l0 * UNIT) : 0.f, r1 = l1 != 0.f ? 1.f / (l1 * UNIT) : 0.f;
       __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)x.row.tok * a.ldo + (size_t)(h0 + 2 * t) * DH;
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
@@ -386,7 +394,7 @@ rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
   __syncthreads();
   total = red[0][h] + red[1][h] + red[2][h] + red[3][h];
   if (a.sinks && h < nh) total += ex2(a.sinks[h0 + h] * LOG2E - top);
-  const float inv = total != 0.f ? 1.f / total : 0.f;
+  const float inv = total != 0.f ? 1.f / (total * UNIT) : 0.f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine) {
 #pragma unroll 8
