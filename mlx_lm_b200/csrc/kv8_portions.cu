@@ -1,0 +1,541 @@
+// Attention of prompt portions over pages in 8 bits on the 5th-generation tensor cores, bfloat16 queries, heads of up to 128.
+//
+// A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs) and walks the request's
+// keys in blocks of 128 positions:
+//   converters  4 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
+//               the scales of the block's eight groups of 16 positions beside them
+//   issuer      1 warp: S_t = Q_t K^T (M 128 x N 128) into tensor memory, and O_t += P_t V with P_t read from tensor memory
+//   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 over S
+// With two heads one's products run beside the other's softmax, and a converted block serves twice as many queries.
+//
+// Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
+// operation), and 128 * 2^-24 sum(q), a number of the query, comes off S in the multiply-add that scales it.  V enters as the exact
+// codes (1024 + u less 1152).  Both give the bytes 0, 2, 1, 3 of every four in that order: Q's columns are stored in the same order, and
+// O's are put back when a row is written.  Queries are scaled by a power of two to [2^14, 2^15) at most, as fp16 exact to 2^-28 of their
+// largest number.
+// Scales: s = scale * sk * (q . codes) with sk the block's key scale; the weight that meets V's codes is w = exp(s) * sv, so the exponent
+// gets log2(sv), the running maximum is that of s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
+// its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) counts as codes of
+// 0 with sv 1.  The maximum follows a score only once that is more than 2^8 beyond it (fp16 holds 2^15), so O is scaled again, by the softmax threads
+// in tensor memory, a few times a row at most.
+//
+// Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
+// MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone.
+#include <cuda_fp16.h>
+
+#include "tcgen05.cuh"
+
+MLXB_DEFINE_LAST_ERROR()
+
+constexpr int BLK = 16;              // positions that share a scale
+constexpr int TQ = 128;              // queries of a tile
+constexpr int TK = 128;              // keys of a block
+constexpr int GR = TK / BLK;         // groups of a block
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
+constexpr float SLACK = 8.f;
+
+struct PortionArgs {
+  const __nv_bfloat16* q;
+  int ldq;
+  const int4* tiles;
+  const int* block_table;
+  int max_pages, n_pages, page, Hq, Hkv, dim, window;
+  float scale;
+  const int8_t *k8, *v8;
+  const float *ks, *vs, *sinks;
+  __nv_bfloat16* out;
+  int ldo, vec;
+  int* status;
+};
+
+template <int DP, int NT>
+struct Shape {
+  static constexpr int KST = NT == 1 && DP == 128 ? 1 : 2;        // buffers of K and of V: two CTAs an SM where a CTA has one head
+  static constexpr int SOFT = 4 * NT, CONV = 4;                   // warps
+  static constexpr int THREADS = 32 * (SOFT + CONV + 1);
+  static constexpr int CTAS = NT == 1 ? 2 : 1;
+  static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, O_t behind them
+  static constexpr int SPAN = 128 * 128;                          // bytes of 128 rows of 64 columns
+  static constexpr int TILE = SPAN * (DP / 64);
+};
+
+template <int DP, int NT>
+struct Smem {
+  using H = Shape<DP, NT>;
+  alignas(1024) uint8_t q[NT][H::TILE];
+  alignas(1024) uint8_t k[H::KST][H::TILE];
+  alignas(1024) uint8_t v[H::KST][H::TILE];
+  float sk[4][GR], lsv[4][GR], rsv[4][GR];              // of the last four blocks: key scale, log2 and reciprocal of the value scale
+  uint32_t missing[4];                                  // groups without a page
+  alignas(8) uint64_t q_full[NT], k_full[2], k_free[2], v_full[2], v_free[2], x_full[4], s_full[NT], p_full[NT], pv_done[NT], drained;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ uint64_t desc_of(uint32_t saddr, uint32_t lbo_bytes) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor for kind::f16: float32 accumulator, A and B fp16, A K-major, B K-major or MN-major (bit 16), N/8 in bits
+// 17-22, M/16 in bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TQ >> 4) << 24);
+}
+// A from tensor memory
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+__device__ __forceinline__ uint32_t masked_xor(uint32_t w, uint32_t x) {      // (w & 0x00ff00ff) ^ x
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(w), "r"(0x00ff00ffu), "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t less1152(uint32_t x) {
+  uint32_t y;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+  return y;
+}
+
+// tiles: int32 [n_tiles][4] = (row of the tile's first token, queries (0: skipped) up to 128, block-table row of the request, position of
+// the first query).
+template <int DP, int NT>
+__global__ void __launch_bounds__(Shape<DP, NT>::THREADS, Shape<DP, NT>::CTAS)
+portions_kernel(const PortionArgs a) {
+  using H = Shape<DP, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  Smem<DP, NT>& sm = *reinterpret_cast<Smem<DP, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 tile = a.tiles[blockIdx.x];
+  if (tile.y <= 0) return;
+  const int row0 = tile.x, n_rows = min(tile.y, TQ), req = tile.z, pos0 = tile.w;
+  const int h0 = blockIdx.y * NT, hk = h0 / (a.Hq / a.Hkv);
+  const int last_pos = pos0 + n_rows - 1;
+  const int first_key = a.window > 0 && pos0 - a.window + 1 > 0 ? pos0 - a.window + 1 : 0;
+  const int kb_lo = first_key / TK, n_blocks = last_pos / TK - kb_lo + 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NT; ++i) { mbar_init(&sm.q_full[i], 4); mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_full[i], 4); mbar_init(&sm.pv_done[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sm.k_full[i], H::CONV); mbar_init(&sm.v_full[i], H::CONV); mbar_init(&sm.k_free[i], 1); mbar_init(&sm.v_free[i], 1); }
+    for (int i = 0; i < 4; ++i) mbar_init(&sm.x_full[i], H::CONV);
+    mbar_init(&sm.drained, 1);
+    sm.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == H::SOFT + H::CONV) {   // the issuer owns the tensor memory
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(H::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem_o = tmem + NT * TK;               // O_t at tmem_o + DP t
+  volatile int* abort_flag = &sm.abort_flag;
+  pdl_trigger();
+
+  if (warp == H::SOFT + H::CONV) {
+    const uint32_t idesc_s = idesc_of(TK, false), idesc_o = idesc_of(DP, true);
+    const int steps = a.dim / 16;
+    auto issue_s = [&](int t, int i) {
+      after_sync();
+      if (elect_one()) {
+        const uint64_t dq = desc_of(smem_u32(sm.q[t]), 16), dk = desc_of(smem_u32(sm.k[i % H::KST]), 16);
+        for (int j = 0; j < steps; ++j) {               // 16 columns: 32 bytes inside a span of 64, then the next span
+          const uint32_t at = (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3));
+          asm volatile(
+              "{\n\t.reg .pred p;\n\t"
+              "setp.ne.b32 p, %4, 0;\n\t"
+              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+              ::"r"(tmem + t * TK), "l"(dq + at), "l"(dk + at), "r"(idesc_s), "r"(j > 0 ? 1u : 0u) : "memory");
+        }
+        umma_commit(&sm.s_full[t]);
+        if (t == NT - 1) umma_commit(&sm.k_free[i % H::KST]);
+      }
+      __syncwarp();
+    };
+    bool ok = mbar_wait_warp(&sm.k_full[0], 0, abort_flag);
+    for (int t = 0; t < NT && ok; ++t) {
+      ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
+      if (ok) issue_s(t, 0);
+    }
+    for (int i = 0; i < n_blocks && ok; ++i) {
+      const uint32_t ph = (uint32_t)(i & 1);
+      if (!(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (!(ok = mbar_wait_warp(&sm.p_full[t], ph, abort_flag))) break;      // P_t is written, S_t has been read
+        after_sync();
+        if (elect_one()) {
+          const uint64_t dv = desc_of(smem_u32(sm.v[i % H::KST]), H::SPAN);
+#pragma unroll
+          for (int j = 0; j < TK / 16; ++j)             // 16 keys: 8 columns of P, 16 rows of V
+            umma_ts(tmem_o + t * DP, tmem + t * TK + 8 * j, dv + (uint32_t)(j * (16 * 128 / 16)), idesc_o, i > 0 || j > 0 ? 1u : 0u);
+          umma_commit(&sm.pv_done[t]);
+          if (t == NT - 1) umma_commit(&sm.v_free[i % H::KST]);
+        }
+        __syncwarp();
+        if (i + 1 < n_blocks) {
+          if (t == 0 && !(ok = mbar_wait_warp(&sm.k_full[(i + 1) % H::KST], (uint32_t)(((i + 1) / H::KST) & 1), abort_flag))) break;
+          if (!(ok = mbar_wait_warp(&sm.pv_done[t], ph, abort_flag))) break;   // P_t lies in S_t's columns
+          issue_s(t, i + 1);
+        }
+      }
+    }
+    // whatever ended the loop: no product is under way when the tensor memory is freed
+    if (elect_one()) umma_commit(&sm.drained);
+    __syncwarp();
+    int never = 0;
+    mbar_wait_warp(&sm.drained, 0, &never);
+  } else if (warp >= H::SOFT) {
+    // converters: thread c of 128 takes 16 codes (piece c % pieces) of row c / pieces + ... of every group of 16 rows
+    const int c = threadIdx.x - 32 * H::SOFT, cw = warp - H::SOFT;
+    const int pieces = a.dim / 16, per = a.page / BLK;
+    const int* bt = a.block_table + (size_t)req * a.max_pages;
+    // pad columns: zeros, once
+    for (int e = c; e < (DP / 16 - pieces) * TK; e += 32 * H::CONV) {
+      const int r = e % TK, p16 = pieces + e / TK;
+      for (int b = 0; b < H::KST; ++b)
+        for (int s = 0; s < 2; ++s) {
+          const int p = (p16 & 3) * 2 + s, at = (p16 >> 2) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(sm.k[b] + at) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(sm.v[b] + at) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    // lane i of a warp (i < 8) knows the tile of the pool that group i of a block is in, or -1
+    auto look_up = [&](int i) {
+      int id = -1;
+      const int key = (kb_lo + i) * TK + (lane & 7) * BLK;
+      if (i < n_blocks && key <= last_pos && key + BLK > first_key) {
+        const int lp = key / a.page;
+        const int pg = lp < a.max_pages ? bt[lp] : -1;
+        if (pg >= 0 && pg < a.n_pages) id = (pg * a.Hkv + hk) * per + (key & (a.page - 1)) / BLK;
+        else if (c < 8) atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+      }
+      return id;
+    };
+    constexpr int PIECES = DP / 16;                     // at most: 8 or 4 pieces of a row
+    constexpr int N = TK * PIECES / (32 * H::CONV);     // 16-byte loads of a thread
+    // a thread stands on one piece and every 128 / PIECES-th row: rows of one group of 16 (PIECES 8) or of two (PIECES 4) at a time
+    const int piece = c % PIECES, r_first = c / PIECES;
+    const bool mine = piece < pieces;
+    constexpr int STEP = 32 * H::CONV / PIECES;         // rows between a thread's loads: 16 or 32
+    uint4 kr[N], vr[N];
+    auto load = [&](const int8_t* pool, uint4 (&x)[N], int id) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int r = r_first + n * STEP;
+        const int at = __shfl_sync(0xffffffffu, id, r / BLK);
+        x[n] = make_uint4(0, 0, 0, 0);
+        if (mine && at >= 0) x[n] = __ldcg(reinterpret_cast<const uint4*>(pool + ((size_t)(uint32_t)at * BLK + (r & 15)) * a.dim + piece * 16));
+      }
+    };
+    auto place = [&](int r, int s) {                    // 16 bytes s of the piece's 32
+      const int p = (piece & 3) * 2 + s;
+      return (piece >> 2) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4);
+    };
+    int id = look_up(0);
+    pdl_wait();
+    const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
+    const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
+    load(k8, kr, id);
+    bool ok = true;
+    for (int i = 0; i < n_blocks && ok; ++i) {
+      const int b = i % H::KST;
+      const uint32_t turn = (uint32_t)((i / H::KST) & 1);
+      float sk = 0.f, sv = 0.f;
+      if (lane < GR && id >= 0) { sk = __ldcg(ks + id); sv = __ldcg(vs + id); }
+      load(v8, vr, id);
+      const int next = look_up(i + 1);
+      if (i >= H::KST && !(ok = mbar_wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int r = r_first + n * STEP;
+        if (!mine) continue;
+        const uint32_t w[4] = {kr[n].x, kr[n].y, kr[n].z, kr[n].w};
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y[2 * e] = masked_xor(w[e], 0x00800080u); y[2 * e + 1] = masked_xor(w[e] >> 8, 0x00800080u); }
+        *reinterpret_cast<uint4*>(sm.k[b] + place(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(sm.k[b] + place(r, 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      if (cw == 0) {
+        const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 0xffu;
+        if (lane < GR) {
+          sm.sk[i & 3][lane] = sk;
+          sm.lsv[i & 3][lane] = sv > 0.f ? log2f(sv) : 0.f;
+          sm.rsv[i & 3][lane] = sv > 0.f ? 1.f / sv : 1.f;
+          if (lane == 0) sm.missing[i & 3] = gone;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.k_full[b]);
+        mbar_arrive(&sm.x_full[i & 3]);
+      }
+      const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
+      if (i + 1 < n_blocks) load(k8, kr, next);
+      if (i >= H::KST && !(ok = mbar_wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int r = r_first + n * STEP;
+        if (!mine) continue;
+        if (nothing >> (r / BLK) & 1) vr[n] = make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {vr[n].x, vr[n].y, vr[n].z, vr[n].w};
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = less1152(masked_xor(w[e], 0x64806480u));
+          y[2 * e + 1] = less1152(masked_xor(w[e] >> 8, 0x64806480u));
+        }
+        *reinterpret_cast<uint4*>(sm.v[b] + place(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(sm.v[b] + place(r, 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.v_full[b]);
+      id = next;
+    }
+  } else {
+    // softmax: thread r of a head's 128 owns query row r, which is lane r of tensor memory
+    const int t = warp >> 2, r = threadIdx.x & 127, h = h0 + t;
+    const int pos = pos0 + r;
+    const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t * TK + lanes, t_o = tmem_o + t * DP + lanes;
+    float fac, off;
+    pdl_wait();
+    {
+      const __nv_bfloat16* qr = after_wait(a.q) + (size_t)(row0 + r) * a.ldq + (size_t)h * a.dim;
+      uint32_t x[DP / 2];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < DP / 8; ++e) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && 8 * e < a.dim) {
+          if (a.vec & 1) {
+            u = *reinterpret_cast<const uint4*>(qr + 8 * e);
+          } else {
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(qr) + 8 * e;
+            u = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+          }
+        }
+        x[4 * e] = u.x; x[4 * e + 1] = u.y; x[4 * e + 2] = u.z; x[4 * e + 3] = u.w;
+      }
+#pragma unroll
+      for (int e = 0; e < DP / 2; ++e) top = max(top, max(x[e] << 16 & 0x7fffffffu, x[e] & 0x7fff0000u));
+      const int e2 = max((int)(top >> 23) - 127, -100);
+      const float up = __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < DP / 8; ++e) {
+        uint32_t y[4];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {                   // columns 0, 2 and 1, 3 of four
+          const uint32_t x0 = x[4 * e + 2 * w], x1 = x[4 * e + 2 * w + 1];
+          y[2 * w] = half2_of(__uint_as_float(x0 << 16) * up, __uint_as_float(x1 << 16) * up);
+          y[2 * w + 1] = half2_of(__uint_as_float(x0 & 0xffff0000u) * up, __uint_as_float(x1 & 0xffff0000u) * up);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y[w]));
+          sum += f.x + f.y;
+        }
+        const int p = e & 7;
+        *reinterpret_cast<uint4*>(sm.q[t] + (e >> 3) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+      off = sum * (128.f * UNIT);
+      fac = __uint_as_float((uint32_t)(127 - 14 + e2) << 23) * (a.scale * LOG2E / UNIT);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full[t]);
+    }
+    float m = -INFINITY, l = 0.f;      // the running maximum of s + log2(sv), in units of the exponent; the sum
+    bool ok = true;
+    for (int i = 0; i < n_blocks && ok; ++i) {
+      const int key0 = (kb_lo + i) * TK, x4 = i & 3;
+      if (!(ok = mbar_wait_warp(&sm.x_full[x4], (uint32_t)((i >> 2) & 1), abort_flag))) break;
+      if (!(ok = mbar_wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
+      after_sync();
+      const uint32_t gone = sm.missing[x4];
+      // blocks that every row of the tile sees whole need no mask
+      const bool open = gone == 0 && key0 + TK - 1 <= pos0 && (a.window <= 0 || key0 >= last_pos - a.window + 1);
+      uint32_t s[32];
+      auto seen = [&](int c, int e) {                   // column 32 c + e
+        const int key = key0 + 32 * c + e;
+        return key <= pos && key >= lo && !(gone >> (2 * c + e / BLK) & 1);
+      };
+      // The largest of s + log2(sv).  In a group the scale is one number and positive, so its largest score is the largest raw
+      // score's.
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < TK / 32; ++c) {
+        tmem_ld32(t_s + 32 * c, s);
+        ld_wait();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float x = -INFINITY, x1 = -INFINITY;
+          if (open) {
+#pragma unroll
+            for (int e = 0; e < BLK; e += 2) {
+              x = fmaxf(x, __uint_as_float(s[16 * g + e]));
+              x1 = fmaxf(x1, __uint_as_float(s[16 * g + e + 1]));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < BLK; ++e) if (seen(c, 16 * g + e)) x = fmaxf(x, __uint_as_float(s[16 * g + e]));
+          }
+          x = fmaxf(x, x1);
+          if (x > -INFINITY) mx = fmaxf(mx, fmaf(x - off, fac * sm.sk[x4][2 * c + g], sm.lsv[x4][2 * c + g]));
+        }
+        __syncwarp();                                   // together for the next load from tensor memory
+      }
+      const bool grow = mx > m + SLACK;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float corr = grow ? ex2(m - mx) : 1.f;    // 2^-inf = 0
+        if (grow) m = mx;
+        l *= corr;
+        if (i > 0) {                                    // S(i) came behind P V(i - 1): O is at rest
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            tmem_ld32(t_o + 32 * c, s);
+            ld_wait();
+            uint32_t y[16];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(s[16 * half + e]) * corr);
+              st16(t_o + 32 * c + 16 * half, y);
+            }
+          }
+          st_wait();
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int c = 0; c < TK / 32; ++c) {
+        tmem_ld32(t_s + 32 * c, s);
+        ld_wait();
+        uint32_t packed[16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float f = fac * sm.sk[x4][2 * c + g], k = fmaf(-off, f, sm.lsv[x4][2 * c + g] - base);
+          float sum = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < BLK; e += 2) {
+            float p0 = ex2(fmaf(__uint_as_float(s[16 * g + e]), f, k)), p1 = ex2(fmaf(__uint_as_float(s[16 * g + e + 1]), f, k));
+            if (!open) {
+              if (!seen(c, 16 * g + e)) p0 = 0.f;
+              if (!seen(c, 16 * g + e + 1)) p1 = 0.f;
+            }
+            sum += p0;
+            sum1 += p1;
+            packed[8 * g + (e >> 1)] = half2_of(p0, p1);
+          }
+          l = fmaf(sum + sum1, sm.rsv[x4][2 * c + g], l);
+        }
+        __syncwarp();
+        st16(t_s + 16 * c, packed);                     // over columns that have been read
+      }
+      st_wait();
+      before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[t]);
+    }
+    if (ok) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 1) & 1), abort_flag);
+    if (ok) {
+      after_sync();
+      if (a.sinks) l += ex2(a.sinks[h] * LOG2E - m);
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      __nv_bfloat16* dst = a.out + (size_t)(row0 + r) * a.ldo + (size_t)h * a.dim;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(t_o + 32 * c, o);
+        ld_wait();
+        if (r < n_rows) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (32 * c + e >= a.dim) break;
+          float y[8];
+#pragma unroll
+          for (int w = 0; w < 8; w += 4) {              // stored as columns 0, 2, 1, 3
+            y[w] = __uint_as_float(o[e + w]) * inv;
+            y[w + 2] = __uint_as_float(o[e + w + 1]) * inv;
+            y[w + 1] = __uint_as_float(o[e + w + 2]) * inv;
+            y[w + 3] = __uint_as_float(o[e + w + 3]) * inv;
+          }
+          if (a.vec & 2) {
+            *reinterpret_cast<uint4*>(dst + 32 * c + e) = pack8(y);
+          } else {
+#pragma unroll
+            for (int w = 0; w < 8; ++w) dst[32 * c + e + w] = __float2bfloat16_rn(y[w]);
+          }
+        }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && sm.abort_flag) atomicOr(a.status, MLXB_ST_WAIT_TIMEOUT);
+  if (warp == H::SOFT + H::CONV) {
+    after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(H::COLS) : "memory");
+  }
+}
+
+template <int DP, int NT>
+static int launch(const PortionArgs& a, int n_tiles, cudaStream_t stream) {
+  const size_t smem = sizeof(Smem<DP, NT>) + 1024;
+  static SharedLimit limit;
+  if (cudaError_t e = limit.raise(portions_kernel<DP, NT>, smem))
+    return mlxb_fail((int)e, "kv8_portions: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  launch_pdl(portions_kernel<DP, NT>, dim3(n_tiles, a.Hq / NT), dim3(Shape<DP, NT>::THREADS), smem, stream, a);
+  return mlxb_check_launch("kv8_portions");
+}
+
+// q, out: [n_tokens, Hq * dim] at row strides ldq, ldo; dim a multiple of 16 up to 128; scale > 0.
+MLXB_EXPORT int mlxb_kv8_portions(const void* q, int ldq, const int* tiles, int n_tiles, const int* block_table, int max_pages, int n_pages,
+                                  int page, int Hq, int Hkv, int dim, int window, float scale, const int8_t* k8, const int8_t* v8,
+                                  const float* ks, const float* vs, void* out, int ldo, int* status, const float* sinks,
+                                  cudaStream_t stream) {
+  if (n_tiles <= 0) return 0;
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: %d query heads over %d key/value heads", Hq, Hkv);
+  if (dim % 16 || dim < 16 || dim > 128) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: head size %d (a multiple of 16 up to 128)", dim);
+  if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: page size %d (a power of two of at least %d)", page, BLK);
+  if (!(scale > 0.f)) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: scale %g", (double)scale);
+  if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)tiles) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: pools and tiles must be 16-byte aligned");
+  const int vec = (ldq % 8 == 0 && !((uintptr_t)q & 15) ? 1 : 0) | (ldo % 8 == 0 && !((uintptr_t)out & 15) ? 2 : 0);
+  const PortionArgs a{(const __nv_bfloat16*)q, ldq, (const int4*)tiles, block_table, max_pages, n_pages, page, Hq, Hkv, dim, window, scale,
+                      k8, v8, ks, vs, sinks, (__nv_bfloat16*)out, ldo, vec, status};
+  const bool pairs = (Hq / Hkv) % 2 == 0;
+  if (dim <= 64) return pairs ? launch<64, 2>(a, n_tiles, stream) : launch<64, 1>(a, n_tiles, stream);
+  return pairs ? launch<128, 2>(a, n_tiles, stream) : launch<128, 1>(a, n_tiles, stream);
+}

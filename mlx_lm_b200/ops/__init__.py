@@ -49,7 +49,7 @@ _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
 # kernel sources that only a bfloat16 run launches from: a float32 run neither compiles nor loads them
 BF16_ONLY_LIBS = frozenset({"gemm_smallm", "gemm_smallm_fold", "gemm_tcgen05", "attention_prefill",
-                            "attention_prefill_tc", "attention_wide_tc", "attention_wide_tcgen05", "moe_tcgen05", "recurrent_chunks"})
+                            "attention_prefill_tc", "attention_wide_tc", "attention_wide_tcgen05", "moe_tcgen05", "recurrent_chunks", "kv8_portions"})
 
 # ... and those that only a float32 run launches from
 F32_ONLY_LIBS = frozenset({"gemm_split"})
@@ -994,9 +994,34 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
               part[5], ldo, b - a, _p(status), sk, stream)
 
 
+_KV8_PORTION_ARGS = ([c_void_p, c_int, c_void_p, c_int, c_void_p] + [c_int] * 7 + [c_float] + [c_void_p] * 5 + [c_int]
+                     + [c_void_p] * 3)
+
+
+def kv8_portions_supported(dtype, head_dim: int, scale: float = 1.0) -> bool:
+    """Whether ``kv8_attention_portions`` takes these queries; portions that it does not take go row by row (``kv8_attention_rows``)."""
+    return dtype == torch.bfloat16 and head_dim % 16 == 0 and 16 <= head_dim <= 128 and scale > 0
+
+
 def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
                            status, stream, sinks=None) -> None:
-    raise KernelError("kv8_attention_portions: not built yet")
+    """Attention of prompt portions over pages in 8 bits, bfloat16, heads of up to 128.  ``tiles``: int32 ``[n_tiles, 4]`` = (row of the
+    tile's first token in ``q`` and ``out``, its queries (0: skipped) up to ``PREFILL_TILE``, row of the block table, position of the first
+    query); window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are."""
+    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_portions")
+    _need(q, torch.bfloat16, "kv8_attention_portions q")
+    _need(out, torch.bfloat16, "kv8_attention_portions out")
+    _need(tiles, torch.int32, "kv8_attention_portions tiles")
+    if n_heads <= 0 or n_heads % Hkv or q.dim() != 2 or q.shape != out.shape or q.shape[1] != n_heads * Dh:
+        raise KernelError(f"kv8_attention_portions: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_heads} heads of {Dh} over {Hkv}")
+    if not kv8_portions_supported(q.dtype, Dh, scale):
+        raise KernelError(f"kv8_attention_portions: heads of {Dh}, scale {scale}: heads of up to 128, a scale above 0")
+    if not tiles.is_contiguous() or tiles.numel() < 4 * n_tiles:
+        raise KernelError(f"kv8_attention_portions: tiles {tuple(tiles.shape)} for {n_tiles} tiles")
+    _call("kv8_portions", "mlxb_kv8_portions", _KV8_PORTION_ARGS, _p(q), _rows(q, "kv8_attention_portions q"), _p(tiles), int(n_tiles),
+          _p(block_table), block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale),
+          _p(v_scale), _p(out), _rows(out, "kv8_attention_portions out"), _p(status), _sinks(sinks, n_heads, "kv8_attention_portions"),
+          stream)
 
 
 # --------------------------------------------------------------------------

@@ -306,6 +306,88 @@ def test_rows_out_of_range(ops, dtype):
         assert float((out[0].double().cpu() - want).abs().max()) <= tol
 
 
+def tiles_of(spans):
+    """Tiles of up to 128 queries for requests that bring ``[(first position, tokens)]``, rows one behind the other."""
+    out, row = [], 0
+    for r, (a, n) in enumerate(spans):
+        out += [(row + i, min(128, n - i), r, a + i) for i in range(0, n, 128)]
+        row += n
+    return torch.tensor(out, dtype=torch.int32).view(-1, 4)
+
+
+def portions_call(ops, cache, q, tiles, n_heads, scale, window=0, sinks=None, table=None, n_tiles=None):
+    status = word()
+    out = torch.full(q.shape, 9.0, dtype=q.dtype, device="cuda")
+    ops.kv8_attention_portions(q, tiles.cuda(), tiles.shape[0] if n_tiles is None else n_tiles, (cache.table if table is None else table).cuda(),
+                               *cache.cuda(), out, n_heads, scale, window, status, stream(), sinks=None if sinks is None else sinks.cuda())
+    return out, status
+
+
+PORTION_SPANS = [[(0, 1)], [(0, 128)], [(130, 7)], [(3, 129), (0, 17)], [(600, 40), (250, 140)]]
+
+
+@pytest.mark.parametrize("spans", PORTION_SPANS)
+@pytest.mark.parametrize("n_heads,heads,dim,page", [(2, 2, 64, 16), (4, 2, 64, 16), (4, 1, 128, 32), (3, 3, 128, 16), (6, 3, 48, 128), (5, 1, 96, 16),
+                                                    (2, 1, 16, 16), (2, 2, 80, 64), (8, 2, 112, 16)])
+@pytest.mark.parametrize("window,with_sinks", [(0, False), (45, True), (300, False)])
+def test_portions(ops, spans, n_heads, heads, dim, page, window, with_sinks):
+    cache = R.Cache([a + n for a, n in spans], heads, dim, page, seed=dim + n_heads)
+    pos, req = R.steps(spans)
+    T = pos.numel()
+    wide = normal(dim + T, T, n_heads * dim + 3).bfloat16().cuda()
+    q = wide[:, 1:1 + n_heads * dim] if page == 16 else wide[:, :n_heads * dim].contiguous()      # also rows without alignment
+    sinks = normal(1, n_heads) if with_sinks else None
+    scale = 1.5 * dim ** -0.5
+    out, status = portions_call(ops, cache, q, tiles_of(spans), n_heads, scale, window, sinks)
+    want = R.attention(cache, q.cpu(), pos, req, n_heads, scale, window, sinks)
+    assert int(status.item()) == 0
+    err = (out.double().cpu() - want).abs()
+    assert float(err.max()) <= 1e-2 * float(cache.vs.max() * 127), float(err.max())
+
+
+def test_portions_with_scales_far_apart_and_released_pages(ops):
+    """Blocks of nothing, blocks of very large values, pages a window has given back, tiles that pad the list, rows of no tile."""
+    n_heads, heads, dim, window = 4, 2, 64, 70
+    spans = [(700, 130)]
+    cache = R.Cache([830], heads, dim, 16, seed=6)
+    cache.vs[int(cache.table[0, 42])] = 0.0
+    cache.ks[int(cache.table[0, 44])] = 0.0
+    cache.vs[int(cache.table[0, 46])] *= 3e4
+    cache.vs[int(cache.table[0, 47])] *= 1e-6
+    pos, req = R.steps(spans)
+    q = (normal(8, 140, n_heads * dim) * 3).bfloat16().cuda()
+    tiles = torch.cat([tiles_of(spans), torch.zeros(2, 4, dtype=torch.int32)])
+    table = cache.table.clone()
+    table[0, :(700 - window + 1) // 16] = -1
+    for w, t in ((window, table), (0, cache.table)):
+        out, status = portions_call(ops, cache, q, tiles, n_heads, 0.3, w, table=t)
+        assert int(status.item()) == 0
+        want = R.attention(cache, q[:130].cpu(), pos, req, n_heads, 0.3, w).view(130, n_heads, dim)
+        got = out[:130].double().cpu().view(130, n_heads, dim)
+        assert float((out[130:].float() - 9.0).abs().max()) == 0.0
+        top = want.abs().amax(2, keepdim=True).clamp(min=1e-3)        # each query and head by its own largest number
+        assert float(((got - want).abs() / top).max()) <= 2e-2
+    # a visible page that the request does not have is reported, and its keys are left out
+    t = cache.table.clone()
+    t[0, 45] = -1
+    out, status = portions_call(ops, cache, q, tiles, n_heads, 0.3, 0, table=t)
+    assert int(status.item()) == ops.ST_POSITION_RANGE
+    assert bool(torch.isfinite(out[:130].float()).all())
+
+
+def test_portions_and_rows_agree(ops):
+    """A portion's queries one by one: the same numbers to bfloat16's precision."""
+    n_heads, heads, dim = 8, 2, 128
+    spans = [(1000, 150), (5, 64)]
+    cache = R.Cache([1150, 69], heads, dim, 64, seed=11)
+    pos, req = R.steps(spans)
+    q = (normal(4, 214, n_heads * dim) * 2).bfloat16().cuda()
+    out, status = portions_call(ops, cache, q, tiles_of(spans), n_heads, dim ** -0.5)
+    one, _ = rows_call(ops, cache, q, pos, req, n_heads, dim ** -0.5)
+    assert int(status.item()) == 0
+    assert float((out.float() - one.float()).abs().max()) <= 1e-2 * float(cache.vs.max() * 127)
+
+
 def test_pool_beyond_31_bits(ops):
     """Codes whose offset in the pool passes 2**31."""
     heads, dim, page = 8, 128, 128
@@ -396,4 +478,14 @@ def test_refusals(ops):
                    dict(rows=torch.zeros(2, device="cuda")), dict(counters=rows["counters"].float())]:
         with pytest.raises(ops.KernelError):
             ops.kv8_attention_rows(**{**rows, **change})
+    q = q.bfloat16()
+    tiles = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    portions = dict(q=q, tiles=tiles, n_tiles=2, block_table=table, k8=k8, v8=v8, k_scale=ks, v_scale=vs, out=q.clone(), n_heads=4, scale=0.1,
+                    window=0, status=s, stream=stream())
+    ops.kv8_attention_portions(**portions)
+    for change in [dict(n_heads=3), dict(q=q.float()), dict(out=q[:2]), dict(tiles=tiles.long()), dict(n_tiles=3), dict(scale=0.0),
+                   dict(scale=-1.0), dict(sinks=torch.zeros(3, device="cuda")), dict(block_table=table.long())]:
+        with pytest.raises(ops.KernelError):
+            ops.kv8_attention_portions(**{**portions, **change})
+    assert not ops.kv8_portions_supported(torch.float32, 64) and not ops.kv8_portions_supported(torch.bfloat16, 256)
     assert int(s.item()) == 0
