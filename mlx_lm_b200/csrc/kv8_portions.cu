@@ -53,7 +53,9 @@ template <int DP, int NT>
 struct Shape {
   static constexpr int KST = NT == 1 && DP == 128 ? 1 : 2;        // buffers of K and of V: two CTAs an SM where a CTA has one head
   static constexpr int SOFT = 4 * NT, CONV = 4;                   // warps
-  static constexpr int THREADS = 32 * (SOFT + CONV + 1);
+  static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (of the last four one issues, the others end at once)
+  // registers a thread: 512 x 128 or 384 x 80 at launch; a row of S takes 128 of a softmax thread's
+  static constexpr int R_SOFT = NT == 2 ? 184 : 160, R_CONV = NT == 2 ? 96 : 56, R_ISSUE = NT == 2 ? 32 : 24;
   static constexpr int CTAS = NT == 1 ? 2 : 1;
   static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, O_t behind them
   static constexpr int SPAN = 128 * 128;                          // bytes of 128 rows of 64 columns
@@ -96,6 +98,19 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+// two float32 at a time
+__device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}" : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
 }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -157,7 +172,9 @@ portions_kernel(const PortionArgs a) {
   volatile int* abort_flag = &sm.abort_flag;
   pdl_trigger();
 
-  if (warp == H::SOFT + H::CONV) {
+  if (warp >= H::SOFT + H::CONV) {
+    fewer_registers<H::R_ISSUE>();
+    if (warp == H::SOFT + H::CONV) {
     const uint32_t idesc_s = idesc_of(TK, false), idesc_o = idesc_of(DP, true);
     const int steps = a.dim / 16;
     auto issue_s = [&](int t, int i) {
@@ -210,7 +227,9 @@ portions_kernel(const PortionArgs a) {
     __syncwarp();
     int never = 0;
     mbar_wait_warp(&sm.drained, 0, &never);
+    }
   } else if (warp >= H::SOFT) {
+    fewer_registers<H::R_CONV>();
     // converters: thread c of 128 takes 16 codes (piece c % pieces) of row c / pieces + ... of every group of 16 rows
     const int c = threadIdx.x - 32 * H::SOFT, cw = warp - H::SOFT;
     const int pieces = a.dim / 16, per = a.page / BLK;
@@ -321,6 +340,7 @@ portions_kernel(const PortionArgs a) {
       id = next;
     }
   } else {
+    more_registers<H::R_SOFT>();
     // softmax: thread r of a head's 128 owns query row r, which is lane r of tensor memory
     const int t = warp >> 2, r = threadIdx.x & 127, h = h0 + t;
     const int pos = pos0 + r;
@@ -382,37 +402,37 @@ portions_kernel(const PortionArgs a) {
       if (!(ok = mbar_wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
       after_sync();
       const uint32_t gone = sm.missing[x4];
+      uint32_t s[TK / 32][32];
+#pragma unroll
+      for (int c = 0; c < TK / 32; ++c) tmem_ld32(t_s + 32 * c, s[c]);
+      ld_wait();
       // blocks that every row of the tile sees whole need no mask
-      const bool open = gone == 0 && key0 + TK - 1 <= pos0 && (a.window <= 0 || key0 >= last_pos - a.window + 1);
-      uint32_t s[32];
-      auto seen = [&](int c, int e) {                   // column 32 c + e
-        const int key = key0 + 32 * c + e;
-        return key <= pos && key >= lo && !(gone >> (2 * c + e / BLK) & 1);
-      };
-      // The largest of s + log2(sv).  In a group the scale is one number and positive, so its largest score is the largest raw
-      // score's.
+      if (gone != 0 || key0 + TK - 1 > pos0 || (a.window > 0 && key0 < last_pos - a.window + 1)) {
+        const int first = lo - key0, last = pos - key0;
+#pragma unroll
+        for (int c = 0; c < TK / 32; ++c) {
+          const int f = first - 32 * c, e1 = last - 32 * c;
+          uint32_t bits = f <= 0 ? 0xffffffffu : f > 31 ? 0u : 0xffffffffu << f;
+          bits &= e1 >= 31 ? 0xffffffffu : e1 < 0 ? 0u : (2u << e1) - 1u;
+          if (gone >> (2 * c) & 1) bits &= 0xffff0000u;
+          if (gone >> (2 * c + 1) & 1) bits &= 0x0000ffffu;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(bits >> e & 1)) s[c][e] = 0xff800000u;          // -inf: its exponential below is 0
+        }
+      }
+      // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
+      // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < TK / 32; ++c) {
-        tmem_ld32(t_s + 32 * c, s);
-        ld_wait();
+      for (int g = 0; g < GR; ++g) {
+        const uint32_t* x = &s[g >> 1][16 * (g & 1)];
+        float y[4];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float x = -INFINITY, x1 = -INFINITY;
-          if (open) {
-#pragma unroll
-            for (int e = 0; e < BLK; e += 2) {
-              x = fmaxf(x, __uint_as_float(s[16 * g + e]));
-              x1 = fmaxf(x1, __uint_as_float(s[16 * g + e + 1]));
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < BLK; ++e) if (seen(c, 16 * g + e)) x = fmaxf(x, __uint_as_float(s[16 * g + e]));
-          }
-          x = fmaxf(x, x1);
-          if (x > -INFINITY) mx = fmaxf(mx, fmaf(x - off, fac * sm.sk[x4][2 * c + g], sm.lsv[x4][2 * c + g]));
-        }
-        __syncwarp();                                   // together for the next load from tensor memory
+        for (int e = 0; e < 4; ++e)
+          y[e] = fmaxf(fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 4])), fmaxf(__uint_as_float(x[e + 8]), __uint_as_float(x[e + 12])));
+        const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+        mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
       }
       const bool grow = mx > m + SLACK;
       if (__any_sync(0xffffffffu, grow)) {
@@ -420,17 +440,15 @@ portions_kernel(const PortionArgs a) {
         if (grow) m = mx;
         l *= corr;
         if (i > 0) {                                    // S(i) came behind P V(i - 1): O is at rest
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            tmem_ld32(t_o + 32 * c, s);
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t y[32];
+            tmem_ld16(t_o + 16 * c, y);
             ld_wait();
-            uint32_t y[16];
+            uint32_t z[16];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(s[16 * half + e]) * corr);
-              st16(t_o + 32 * c + 16 * half, y);
-            }
+            for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[e]) * corr);
+            st16(t_o + 16 * c, z);
           }
           st_wait();
         }
@@ -438,27 +456,23 @@ portions_kernel(const PortionArgs a) {
       const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int c = 0; c < TK / 32; ++c) {
-        tmem_ld32(t_s + 32 * c, s);
-        ld_wait();
         uint32_t packed[16];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float f = fac * sm.sk[x4][2 * c + g], k = fmaf(-off, f, sm.lsv[x4][2 * c + g] - base);
-          float sum = 0.f, sum1 = 0.f;
+        for (int gg = 0; gg < 2; ++gg) {
+          const int g = 2 * c + gg;
+          const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f), k = fmaf(-off, f, sm.lsv[x4][g] - base);
+          float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
           for (int e = 0; e < BLK; e += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(s[16 * g + e]), f, k)), p1 = ex2(fmaf(__uint_as_float(s[16 * g + e + 1]), f, k));
-            if (!open) {
-              if (!seen(c, 16 * g + e)) p0 = 0.f;
-              if (!seen(c, 16 * g + e + 1)) p1 = 0.f;
-            }
-            sum += p0;
-            sum1 += p1;
-            packed[8 * g + (e >> 1)] = half2_of(p0, p1);
+            float p0, p1;
+            fma2(p0, p1, __uint_as_float(s[c][16 * gg + e]), __uint_as_float(s[c][16 * gg + e + 1]), f, k);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            add2(sum0, sum1, p0, p1);
+            packed[8 * gg + (e >> 1)] = half2_of(p0, p1);
           }
-          l = fmaf(sum + sum1, sm.rsv[x4][2 * c + g], l);
+          l = fmaf(sum0 + sum1, sm.rsv[x4][g], l);
         }
-        __syncwarp();
         st16(t_s + 16 * c, packed);                     // over columns that have been read
       }
       st_wait();
@@ -469,7 +483,7 @@ portions_kernel(const PortionArgs a) {
     if (ok) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 1) & 1), abort_flag);
     if (ok) {
       after_sync();
-      if (a.sinks) l += ex2(a.sinks[h] * LOG2E - m);
+      if (a.sinks && m != -INFINITY) l += ex2(a.sinks[h] * LOG2E - m);
       const float inv = l != 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* dst = a.out + (size_t)(row0 + r) * a.ldo + (size_t)h * a.dim;
 #pragma unroll

@@ -161,6 +161,7 @@ __device__ __forceinline__ void finish_item(const RowsArgs& a, const Item& x, in
       top = fmaxf(top, mc);
     }
     top = __any_sync(0xffffffffu, odd) ? NAN : warp_max(top);
+    if (top == -INFINITY) top = 0.f;                  // no key at all has a page: zeros
     for (int c = lane; c < x.n_chunks; c += 32) {
       const float w = exp_(__ldcg(all + c * per + h) - top);
       weights[c * tile_heads + h] = w;

@@ -381,6 +381,7 @@ rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
   if (lane < 8) red[warp][lane] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0][h], red[1][h]), fmaxf(red[2][h], red[3][h]));
+  if (top == -INFINITY) top = 0.f;                      // no key at all has a page: zeros
   __syncthreads();
   float total = 0.f;
   for (int c = threadIdx.x >> 3; c < n; c += 16) {
