@@ -2,7 +2,7 @@
 //
 // A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs) and walks the request's
 // keys in blocks of 128 positions:
-//   converters  4 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
+//   converters  4 or 8 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
 //               the scales of the block's eight groups of 16 positions beside them
 //   issuer      1 warp: S_t = Q_t K^T (M 128 x N 128) into tensor memory, and O_t += P_t V with P_t read from tensor memory
 //   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 over S
@@ -52,10 +52,11 @@ struct PortionArgs {
 template <int DP, int NT>
 struct Shape {
   static constexpr int KST = NT == 1 && DP == 128 ? 1 : 2;        // buffers of K and of V: two CTAs an SM where a CTA has one head
-  static constexpr int SOFT = 4 * NT, CONV = 4;                   // warps
+  static constexpr int SOFT = 4 * NT, CONV = NT == 2 && DP == 128 ? 8 : 4;      // warps
   static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (of the last four one issues, the others end at once)
-  // registers a thread: 512 x 128 or 384 x 80 at launch; a row of S takes 128 of a softmax thread's
-  static constexpr int R_SOFT = NT == 2 ? 184 : 160, R_CONV = NT == 2 ? 96 : 56, R_ISSUE = NT == 2 ? 32 : 24;
+  // registers a thread: 640 x 96, 512 x 128 or 384 x 80 at launch; a row of S takes 128 of a softmax thread's
+  static constexpr int R_SOFT = NT == 2 ? (DP == 128 ? 168 : 184) : (DP == 128 ? 144 : 160);
+  static constexpr int R_CONV = NT == 2 ? (DP == 128 ? 56 : 96) : (DP == 128 ? 72 : 56), R_ISSUE = 24;
   static constexpr int CTAS = NT == 1 ? 2 : 1;
   static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, O_t behind them
   static constexpr int SPAN = 128 * 128;                          // bytes of 128 rows of 64 columns
@@ -230,7 +231,7 @@ portions_kernel(const PortionArgs a) {
     }
   } else if (warp >= H::SOFT) {
     fewer_registers<H::R_CONV>();
-    // converters: thread c of 128 takes 16 codes (piece c % pieces) of row c / pieces + ... of every group of 16 rows
+    // converters: a thread takes 16 codes (a piece of a row) at a time
     const int c = threadIdx.x - 32 * H::SOFT, cw = warp - H::SOFT;
     const int pieces = a.dim / 16, per = a.page / BLK;
     const int* bt = a.block_table + (size_t)req * a.max_pages;
@@ -256,13 +257,13 @@ portions_kernel(const PortionArgs a) {
       }
       return id;
     };
-    constexpr int PIECES = DP / 16;                     // at most: 8 or 4 pieces of a row
+    constexpr int PIECES = DP / 16;                     // of a row at most: 8 or 4
     constexpr int N = TK * PIECES / (32 * H::CONV);     // 16-byte loads of a thread
-    // a thread stands on one piece and every 128 / PIECES-th row: rows of one group of 16 (PIECES 8) or of two (PIECES 4) at a time
-    const int piece = c % PIECES, r_first = c / PIECES;
+    // eight neighbouring threads stand on four pieces of two rows: their stores meet in no bank
+    const int piece = PIECES == 8 ? (c & 3) + 4 * (c >> 3 & 1) : c & 3, r_first = PIECES == 8 ? (c >> 2 & 1) + 2 * (c >> 4) : c >> 2;
     const bool mine = piece < pieces;
-    constexpr int STEP = 32 * H::CONV / PIECES;         // rows between a thread's loads: 16 or 32
-    uint4 kr[N], vr[N];
+    constexpr int STEP = 32 * H::CONV / PIECES;         // rows between a thread's loads
+    uint4 kr[N], vr[N];                                 // a block's codes, on their way while the block before is converted
     auto load = [&](const int8_t* pool, uint4 (&x)[N], int id) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -272,34 +273,30 @@ portions_kernel(const PortionArgs a) {
         if (mine && at >= 0) x[n] = __ldcg(reinterpret_cast<const uint4*>(pool + ((size_t)(uint32_t)at * BLK + (r & 15)) * a.dim + piece * 16));
       }
     };
-    auto place = [&](int r, int s) {                    // 16 bytes s of the piece's 32
-      const int p = (piece & 3) * 2 + s;
-      return (piece >> 2) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4);
-    };
-    int id = look_up(0);
+    const int place0 = (piece >> 2) * H::SPAN + r_first * 128 + ((((piece & 3) * 2) ^ (r_first & 7)) << 4);      // (STEP is a multiple of 8)
+    int id = look_up(0), id1 = look_up(1);
     pdl_wait();
     const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
     const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
+    float sk = 0.f, sv = 0.f;
     load(k8, kr, id);
+    if (lane < GR && id >= 0) { sk = __ldcg(ks + id); sv = __ldcg(vs + id); }
+    load(v8, vr, id);
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
       const int b = i % H::KST;
       const uint32_t turn = (uint32_t)((i / H::KST) & 1);
-      float sk = 0.f, sv = 0.f;
-      if (lane < GR && id >= 0) { sk = __ldcg(ks + id); sv = __ldcg(vs + id); }
-      load(v8, vr, id);
-      const int next = look_up(i + 1);
       if (i >= H::KST && !(ok = mbar_wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
+      uint8_t* dst = sm.k[b] + place0;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int r = r_first + n * STEP;
         if (!mine) continue;
         const uint32_t w[4] = {kr[n].x, kr[n].y, kr[n].z, kr[n].w};
         uint32_t y[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) { y[2 * e] = masked_xor(w[e], 0x00800080u); y[2 * e + 1] = masked_xor(w[e] >> 8, 0x00800080u); }
-        *reinterpret_cast<uint4*>(sm.k[b] + place(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(sm.k[b] + place(r, 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+        *reinterpret_cast<uint4*>(dst + n * STEP * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(sm.k[b] + ((place0 ^ 16) + n * STEP * 128)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
       if (cw == 0) {
         const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 0xffu;
@@ -317,13 +314,16 @@ portions_kernel(const PortionArgs a) {
         mbar_arrive(&sm.x_full[i & 3]);
       }
       const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
-      if (i + 1 < n_blocks) load(k8, kr, next);
+      load(k8, kr, id1);
+      sk = sv = 0.f;
+      if (lane < GR && id1 >= 0) { sk = __ldcg(ks + id1); sv = __ldcg(vs + id1); }
+      const int id2 = look_up(i + 2);
       if (i >= H::KST && !(ok = mbar_wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
+      dst = sm.v[b] + place0;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int r = r_first + n * STEP;
         if (!mine) continue;
-        if (nothing >> (r / BLK) & 1) vr[n] = make_uint4(0, 0, 0, 0);
+        if (nothing >> ((r_first + n * STEP) / BLK) & 1) vr[n] = make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {vr[n].x, vr[n].y, vr[n].z, vr[n].w};
         uint32_t y[8];
 #pragma unroll
@@ -331,13 +331,15 @@ portions_kernel(const PortionArgs a) {
           y[2 * e] = less1152(masked_xor(w[e], 0x64806480u));
           y[2 * e + 1] = less1152(masked_xor(w[e] >> 8, 0x64806480u));
         }
-        *reinterpret_cast<uint4*>(sm.v[b] + place(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(sm.v[b] + place(r, 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+        *reinterpret_cast<uint4*>(dst + n * STEP * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(sm.v[b] + ((place0 ^ 16) + n * STEP * 128)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.v_full[b]);
-      id = next;
+      load(v8, vr, id1);
+      id = id1;
+      id1 = id2;
     }
   } else {
     more_registers<H::R_SOFT>();
