@@ -1,12 +1,14 @@
 // Attention of prompt portions over pages in 8 bits on the 5th-generation tensor cores, bfloat16 queries, heads of up to 128.
 //
 // A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs) and walks the request's
-// keys in blocks of 128 positions:
+// keys in blocks of 64 positions:
 //   converters  4 or 8 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
 //               the scales of the block's eight groups of 16 positions beside them
-//   issuer      1 warp: S_t = Q_t K^T (M 128 x N 128) into tensor memory, and O_t += P_t V with P_t read from tensor memory
+//   issuer      1 warp: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
 //   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 over S
-// With two heads one's products run beside the other's softmax, and a converted block serves twice as many queries.
+// A head has two buffers of S: while the softmax works on one block, P V of the block before and S of the one behind are formed, so that
+// the chain of a tile's blocks is its softmax alone.  (With blocks of 128 keys and one buffer P V and S stood in that chain: 398 us
+// where this takes 0.)  Two heads of a CTA have chains of their own, and a converted block serves both.
 //
 // Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
 // operation), and 128 * 2^-24 sum(q), a number of the query, comes off S in the multiply-add that scales it.  V enters as the exact
@@ -29,8 +31,9 @@ MLXB_DEFINE_LAST_ERROR()
 
 constexpr int BLK = 16;              // positions that share a scale
 constexpr int TQ = 128;              // queries of a tile
-constexpr int TK = 128;              // keys of a block
+constexpr int TK = 64;               // keys of a block
 constexpr int GR = TK / BLK;         // groups of a block
+constexpr int XR = 8;                // blocks whose scales are kept
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
 constexpr float SLACK = 8.f;
@@ -51,27 +54,29 @@ struct PortionArgs {
 
 template <int DP, int NT>
 struct Shape {
-  static constexpr int KST = NT == 1 && DP == 128 ? 1 : 2;        // buffers of K and of V: two CTAs an SM where a CTA has one head
+  static constexpr int KST = NT == 1 && DP == 128 ? 2 : 4;        // buffers of K and of V: two CTAs an SM where a CTA has one head
   static constexpr int SOFT = 4 * NT, CONV = NT == 2 && DP == 128 ? 8 : 4;      // warps
   static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (of the last four one issues, the others end at once)
-  // registers a thread: 640 x 96, 512 x 128 or 384 x 80 at launch; a row of S takes 128 of a softmax thread's
-  static constexpr int R_SOFT = NT == 2 ? (DP == 128 ? 168 : 184) : (DP == 128 ? 144 : 160);
-  static constexpr int R_CONV = NT == 2 ? (DP == 128 ? 56 : 96) : (DP == 128 ? 72 : 56), R_ISSUE = 24;
+  // registers a thread, at launch (what the launch bounds leave: 640 x 96, 512 x 128, 384 x 80 twice) and then by role, no more in all
+  static constexpr int R_LAUNCH = NT == 1 ? 80 : DP == 128 ? 96 : 128;
+  static constexpr int R_SOFT = NT == 1 ? 120 : DP == 128 ? 128 : 144, R_CONV = DP == 128 || NT == 1 ? 88 : 96, R_ISSUE = NT == 1 ? 24 : 40;
+  static_assert(32 * (SOFT * R_SOFT + CONV * R_CONV + 4 * R_ISSUE) <= THREADS * R_LAUNCH, "registers");
   static constexpr int CTAS = NT == 1 ? 2 : 1;
-  static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, O_t behind them
-  static constexpr int SPAN = 128 * 128;                          // bytes of 128 rows of 64 columns
-  static constexpr int TILE = SPAN * (DP / 64);
+  static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: two buffers of S_t at 128 t, O_t behind them
+  static constexpr int QSPAN = TQ * 128, SPAN = TK * 128;         // bytes of a tile's rows of 64 columns
+  static constexpr int QTILE = QSPAN * (DP / 64), TILE = SPAN * (DP / 64);
 };
 
 template <int DP, int NT>
 struct Smem {
   using H = Shape<DP, NT>;
-  alignas(1024) uint8_t q[NT][H::TILE];
+  alignas(1024) uint8_t q[NT][H::QTILE];
   alignas(1024) uint8_t k[H::KST][H::TILE];
   alignas(1024) uint8_t v[H::KST][H::TILE];
-  float sk[4][GR], lsv[4][GR], rsv[4][GR];              // of the last four blocks: key scale, log2 and reciprocal of the value scale
-  uint32_t missing[4];                                  // groups without a page
-  alignas(8) uint64_t q_full[NT], k_full[2], k_free[2], v_full[2], v_free[2], x_full[4], s_full[NT], p_full[NT], pv_done[NT], drained;
+  float sk[XR][GR], lsv[XR][GR], rsv[XR][GR];           // of the last blocks: key scale, log2 and reciprocal of the value scale
+  uint32_t missing[XR];                                 // groups without a page
+  alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST], x_full[XR];
+  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT], drained;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -92,18 +97,30 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads from tensor memory so far.  The registers they fill go through the statement: what is done with them stays behind it.
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[2][32]) {
+  ld_wait(r[0]);
+  ld_wait(r[1]);
+}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+// Registers a thread from here on.  More are asked for with `inc`, fewer with `dec`: the other way round is an illegal instruction.
+template <int N, int AT_LAUNCH>
+__device__ __forceinline__ void registers() {
+  if constexpr (N > AT_LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  else if constexpr (N < AT_LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 // two float32 at a time
 __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
@@ -144,7 +161,7 @@ portions_kernel(const PortionArgs a) {
   using H = Shape<DP, NT>;
   extern __shared__ uint8_t smem_raw[];
   Smem<DP, NT>& sm = *reinterpret_cast<Smem<DP, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int4 tile = a.tiles[blockIdx.x];
   if (tile.y <= 0) return;
   const int row0 = tile.x, n_rows = min(tile.y, TQ), req = tile.z, pos0 = tile.w;
@@ -154,9 +171,18 @@ portions_kernel(const PortionArgs a) {
   const int kb_lo = first_key / TK, n_blocks = last_pos / TK - kb_lo + 1;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NT; ++i) { mbar_init(&sm.q_full[i], 4); mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_full[i], 4); mbar_init(&sm.pv_done[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sm.k_full[i], H::CONV); mbar_init(&sm.v_full[i], H::CONV); mbar_init(&sm.k_free[i], 1); mbar_init(&sm.v_free[i], 1); }
-    for (int i = 0; i < 4; ++i) mbar_init(&sm.x_full[i], H::CONV);
+    for (int i = 0; i < NT; ++i) {
+      mbar_init(&sm.q_full[i], 4);
+      mbar_init(&sm.pv_done[i], 1);
+      for (int b = 0; b < 2; ++b) { mbar_init(&sm.s_full[i][b], 1); mbar_init(&sm.p_full[i][b], 4); }
+    }
+    for (int i = 0; i < H::KST; ++i) {
+      mbar_init(&sm.k_full[i], H::CONV);
+      mbar_init(&sm.v_full[i], H::CONV);
+      mbar_init(&sm.k_free[i], 1);
+      mbar_init(&sm.v_free[i], 1);
+    }
+    for (int i = 0; i < XR; ++i) mbar_init(&sm.x_full[i], H::CONV);
     mbar_init(&sm.drained, 1);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -169,57 +195,59 @@ portions_kernel(const PortionArgs a) {
   __syncthreads();
   after_sync();
   const uint32_t tmem = sm.tmem_base;
-  const uint32_t tmem_o = tmem + NT * TK;               // O_t at tmem_o + DP t
+  const uint32_t tmem_o = tmem + NT * 2 * TK;           // O_t at tmem_o + DP t
   volatile int* abort_flag = &sm.abort_flag;
   pdl_trigger();
 
   if (warp >= H::SOFT + H::CONV) {
-    fewer_registers<H::R_ISSUE>();
+    registers<H::R_ISSUE, H::R_LAUNCH>();
     if (warp == H::SOFT + H::CONV) {
-    const uint32_t idesc_s = idesc_of(TK, false), idesc_o = idesc_of(DP, true);
-    const int steps = a.dim / 16;
+    // One value for the warp, and known as that to the compiler: what the products take stays in uniform registers.
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), tm_o = tm + NT * 2 * TK;
+    const int n = __shfl_sync(0xffffffffu, n_blocks, 0);
+    constexpr uint32_t idesc_s = idesc_of(TK, false), idesc_o = idesc_of(DP, true);
+    const uint64_t dq0 = desc_of(smem_u32(sm.q[0]), 16), dk0 = desc_of(smem_u32(sm.k[0]), 16), dv0 = desc_of(smem_u32(sm.v[0]), H::SPAN);
+    // S_t of block i, once its keys are there; its buffer of tensor memory is free
     auto issue_s = [&](int t, int i) {
+      if (!mbar_wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag)) return false;
       after_sync();
       if (elect_one()) {
-        const uint64_t dq = desc_of(smem_u32(sm.q[t]), 16), dk = desc_of(smem_u32(sm.k[i % H::KST]), 16);
-        for (int j = 0; j < steps; ++j) {               // 16 columns: 32 bytes inside a span of 64, then the next span
-          const uint32_t at = (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3));
-          asm volatile(
-              "{\n\t.reg .pred p;\n\t"
-              "setp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-              ::"r"(tmem + t * TK), "l"(dq + at), "l"(dk + at), "r"(idesc_s), "r"(j > 0 ? 1u : 0u) : "memory");
-        }
-        umma_commit(&sm.s_full[t]);
+        const uint64_t dq = dq0 + (uint32_t)(t * (H::QTILE / 16)), dk = dk0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j)               // 16 columns: 32 bytes inside a span of 64, then the next span
+          umma_bf16(tm + (uint32_t)((2 * t + (i & 1)) * TK), dq + (uint32_t)((j >> 2) * (H::QSPAN / 16) + 2 * (j & 3)),
+                    dk + (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3)), idesc_s, j > 0 ? 1u : 0u);
+        umma_commit(&sm.s_full[t][i & 1]);
         if (t == NT - 1) umma_commit(&sm.k_free[i % H::KST]);
       }
       __syncwarp();
+      return true;
     };
-    bool ok = mbar_wait_warp(&sm.k_full[0], 0, abort_flag);
-    for (int t = 0; t < NT && ok; ++t) {
-      ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
-      if (ok) issue_s(t, 0);
-    }
-    for (int i = 0; i < n_blocks && ok; ++i) {
-      const uint32_t ph = (uint32_t)(i & 1);
-      if (!(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+    bool ok = true;
+    for (int t = 0; t < NT && ok; ++t) ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
+    for (int i = 0; i < 2 && i < n; ++i)
+      for (int t = 0; t < NT && ok; ++t) ok = issue_s(t, i);
+    for (int i = 0; i < n && ok; ++i) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        if (!(ok = mbar_wait_warp(&sm.p_full[t], ph, abort_flag))) break;      // P_t is written, S_t has been read
+        if (!(ok = mbar_wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
+        if (t == 0 && !(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
         after_sync();
         if (elect_one()) {
-          const uint64_t dv = desc_of(smem_u32(sm.v[i % H::KST]), H::SPAN);
+          const uint64_t dv = dv0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
 #pragma unroll
           for (int j = 0; j < TK / 16; ++j)             // 16 keys: 8 columns of P, 16 rows of V
-            umma_ts(tmem_o + t * DP, tmem + t * TK + 8 * j, dv + (uint32_t)(j * (16 * 128 / 16)), idesc_o, i > 0 || j > 0 ? 1u : 0u);
+            umma_ts(tm_o + t * DP, tm + (uint32_t)((2 * t + (i & 1)) * TK + 8 * j), dv + (uint32_t)(j * (16 * 128 / 16)), idesc_o,
+                    i > 0 || j > 0 ? 1u : 0u);
           umma_commit(&sm.pv_done[t]);
           if (t == NT - 1) umma_commit(&sm.v_free[i % H::KST]);
         }
         __syncwarp();
-        if (i + 1 < n_blocks) {
-          if (t == 0 && !(ok = mbar_wait_warp(&sm.k_full[(i + 1) % H::KST], (uint32_t)(((i + 1) / H::KST) & 1), abort_flag))) break;
-          if (!(ok = mbar_wait_warp(&sm.pv_done[t], ph, abort_flag))) break;   // P_t lies in S_t's columns
-          issue_s(t, i + 1);
+        // the S that takes the place of the P used before this one: with two heads the other head's, so that nothing is waited for
+        const int to = NT == 1 ? 0 : t ^ 1, io = NT == 1 || t == 1 ? i : i - 1;
+        if (io >= 0 && io + 2 < n) {
+          if (!(ok = mbar_wait_warp(&sm.pv_done[to], (uint32_t)(io & 1), abort_flag))) break;
+          if (!(ok = issue_s(to, io + 2))) break;
         }
       }
     }
@@ -230,7 +258,7 @@ portions_kernel(const PortionArgs a) {
     mbar_wait_warp(&sm.drained, 0, &never);
     }
   } else if (warp >= H::SOFT) {
-    fewer_registers<H::R_CONV>();
+    registers<H::R_CONV, H::R_LAUNCH>();
     // converters: a thread takes 16 codes (a piece of a row) at a time
     const int c = threadIdx.x - 32 * H::SOFT, cw = warp - H::SOFT;
     const int pieces = a.dim / 16, per = a.page / BLK;
@@ -245,15 +273,15 @@ portions_kernel(const PortionArgs a) {
           *reinterpret_cast<uint4*>(sm.v[b] + at) = make_uint4(0, 0, 0, 0);
         }
     }
-    // lane i of a warp (i < 8) knows the tile of the pool that group i of a block is in, or -1
+    // lane i of a warp (i < GR, and the lanes behind them again) knows the tile of the pool that group i of a block is in, or -1
     auto look_up = [&](int i) {
       int id = -1;
-      const int key = (kb_lo + i) * TK + (lane & 7) * BLK;
+      const int key = (kb_lo + i) * TK + (lane & (GR - 1)) * BLK;
       if (i < n_blocks && key <= last_pos && key + BLK > first_key) {
         const int lp = key / a.page;
         const int pg = lp < a.max_pages ? bt[lp] : -1;
         if (pg >= 0 && pg < a.n_pages) id = (pg * a.Hkv + hk) * per + (key & (a.page - 1)) / BLK;
-        else if (c < 8) atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+        else if (c < GR) atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
       }
       return id;
     };
@@ -299,19 +327,19 @@ portions_kernel(const PortionArgs a) {
         *reinterpret_cast<uint4*>(sm.k[b] + ((place0 ^ 16) + n * STEP * 128)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
       if (cw == 0) {
-        const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 0xffu;
+        const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & ((1u << GR) - 1);
         if (lane < GR) {
-          sm.sk[i & 3][lane] = sk;
-          sm.lsv[i & 3][lane] = sv > 0.f ? log2f(sv) : 0.f;
-          sm.rsv[i & 3][lane] = sv > 0.f ? 1.f / sv : 1.f;
-          if (lane == 0) sm.missing[i & 3] = gone;
+          sm.sk[i % XR][lane] = sk;
+          sm.lsv[i % XR][lane] = sv > 0.f ? log2f(sv) : 0.f;
+          sm.rsv[i % XR][lane] = sv > 0.f ? 1.f / sv : 1.f;
+          if (lane == 0) sm.missing[i % XR] = gone;
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sm.k_full[b]);
-        mbar_arrive(&sm.x_full[i & 3]);
+        mbar_arrive(&sm.x_full[i % XR]);
       }
       const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
       load(k8, kr, id1);
@@ -342,13 +370,13 @@ portions_kernel(const PortionArgs a) {
       id1 = id2;
     }
   } else {
-    more_registers<H::R_SOFT>();
+    registers<H::R_SOFT, H::R_LAUNCH>();
     // softmax: thread r of a head's 128 owns query row r, which is lane r of tensor memory
     const int t = warp >> 2, r = threadIdx.x & 127, h = h0 + t;
     const int pos = pos0 + r;
     const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + t * TK + lanes, t_o = tmem_o + t * DP + lanes;
+    const uint32_t t_s0 = tmem + 2 * t * TK + lanes, t_o = tmem_o + t * DP + lanes;
     float fac, off;
     pdl_wait();
     {
@@ -388,7 +416,7 @@ portions_kernel(const PortionArgs a) {
           sum += f.x + f.y;
         }
         const int p = e & 7;
-        *reinterpret_cast<uint4*>(sm.q[t] + (e >> 3) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(sm.q[t] + (e >> 3) * H::QSPAN + r * 128 + ((p ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
       }
       off = sum * (128.f * UNIT);
       fac = __uint_as_float((uint32_t)(127 - 14 + e2) << 23) * (a.scale * LOG2E / UNIT);
@@ -399,15 +427,16 @@ portions_kernel(const PortionArgs a) {
     float m = -INFINITY, l = 0.f;      // the running maximum of s + log2(sv), in units of the exponent; the sum
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
-      const int key0 = (kb_lo + i) * TK, x4 = i & 3;
-      if (!(ok = mbar_wait_warp(&sm.x_full[x4], (uint32_t)((i >> 2) & 1), abort_flag))) break;
-      if (!(ok = mbar_wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
+      const int key0 = (kb_lo + i) * TK, x4 = i % XR;
+      const uint32_t t_s = t_s0 + (uint32_t)((i & 1) * TK);
+      if (!(ok = mbar_wait_warp(&sm.x_full[x4], (uint32_t)((i / XR) & 1), abort_flag))) break;
+      if (!(ok = mbar_wait_warp(&sm.s_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;
       after_sync();
       const uint32_t gone = sm.missing[x4];
       uint32_t s[TK / 32][32];
 #pragma unroll
       for (int c = 0; c < TK / 32; ++c) tmem_ld32(t_s + 32 * c, s[c]);
-      ld_wait();
+      ld_wait(s);
       // blocks that every row of the tile sees whole need no mask
       if (gone != 0 || key0 + TK - 1 > pos0 || (a.window > 0 && key0 < last_pos - a.window + 1)) {
         const int first = lo - key0, last = pos - key0;
@@ -441,16 +470,21 @@ portions_kernel(const PortionArgs a) {
         const float corr = grow ? ex2(m - mx) : 1.f;    // 2^-inf = 0
         if (grow) m = mx;
         l *= corr;
-        if (i > 0) {                                    // S(i) came behind P V(i - 1): O is at rest
+        if (i > 0) {                                    // O as P V of the block before leaves it
+          if (!(ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((i - 1) & 1), abort_flag))) break;
+          after_sync();
 #pragma unroll 1
-          for (int c = 0; c < DP / 16; ++c) {
+          for (int c = 0; c < DP / 32; ++c) {
             uint32_t y[32];
-            tmem_ld16(t_o + 16 * c, y);
-            ld_wait();
-            uint32_t z[16];
+            tmem_ld32(t_o + 32 * c, y);
+            ld_wait(y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[e]) * corr);
-            st16(t_o + 16 * c, z);
+            for (int half = 0; half < 2; ++half) {
+              uint32_t z[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[16 * half + e]) * corr);
+              st16(t_o + 32 * c + 16 * half, z);
+            }
           }
           st_wait();
         }
@@ -480,8 +514,10 @@ portions_kernel(const PortionArgs a) {
       st_wait();
       before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full[t]);
+      if (lane == 0) mbar_arrive(&sm.p_full[t][i & 1]);
     }
+    // S of the last block needed P V of the third last alone: the last two may both be under way, and a parity tells neighbours apart only
+    if (ok && n_blocks > 1) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 2) & 1), abort_flag);
     if (ok) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 1) & 1), abort_flag);
     if (ok) {
       after_sync();
@@ -492,7 +528,7 @@ portions_kernel(const PortionArgs a) {
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(t_o + 32 * c, o);
-        ld_wait();
+        ld_wait(o);
         if (r < n_rows) {
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
