@@ -4,7 +4,7 @@
 // keys in blocks of 64 positions:
 //   converters  4 or 8 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
 //               the scales of the block's eight groups of 16 positions beside them
-//   issuer      1 warp: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
+//   issuers     2 warps a head: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
 //   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 over S
 // A head has two buffers of S: while the softmax works on one block, P V of the block before and S of the one behind are formed, so that
 // the chain of a tile's blocks is its softmax alone.  (With blocks of 128 keys and one buffer P V and S stood in that chain: 398 us
@@ -56,7 +56,8 @@ template <int DP, int NT>
 struct Shape {
   static constexpr int KST = NT == 1 && DP == 128 ? 2 : 4;        // buffers of K and of V: two CTAs an SM where a CTA has one head
   static constexpr int SOFT = 4 * NT, CONV = NT == 2 && DP == 128 ? 8 : 4;      // warps
-  static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (of the last four one issues, the others end at once)
+  static constexpr int GW = CONV / 2;                             // converters work in two groups, a block each
+  static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (the last four issue products)
   // registers a thread, at launch (what the launch bounds leave: 640 x 96, 512 x 128, 384 x 80 twice) and then by role, no more in all
   static constexpr int R_LAUNCH = NT == 1 ? 80 : DP == 128 ? 96 : 128;
   static constexpr int R_SOFT = NT == 1 ? 120 : DP == 128 ? 128 : 144, R_CONV = DP == 128 || NT == 1 ? 88 : 96, R_ISSUE = NT == 1 ? 24 : 40;
@@ -76,7 +77,7 @@ struct Smem {
   float sk[XR][GR], lsv[XR][GR], rsv[XR][GR];           // of the last blocks: key scale, log2 and reciprocal of the value scale
   uint32_t missing[XR];                                 // groups without a page
   alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST], x_full[XR];
-  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT], drained;
+  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT][2], drained[2 * NT];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -173,21 +174,20 @@ portions_kernel(const PortionArgs a) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < NT; ++i) {
       mbar_init(&sm.q_full[i], 4);
-      mbar_init(&sm.pv_done[i], 1);
-      for (int b = 0; b < 2; ++b) { mbar_init(&sm.s_full[i][b], 1); mbar_init(&sm.p_full[i][b], 4); }
+      for (int b = 0; b < 2; ++b) { mbar_init(&sm.s_full[i][b], 1); mbar_init(&sm.p_full[i][b], 4); mbar_init(&sm.pv_done[i][b], 1); }
     }
     for (int i = 0; i < H::KST; ++i) {
-      mbar_init(&sm.k_full[i], H::CONV);
-      mbar_init(&sm.v_full[i], H::CONV);
-      mbar_init(&sm.k_free[i], 1);
-      mbar_init(&sm.v_free[i], 1);
+      mbar_init(&sm.k_full[i], H::GW);
+      mbar_init(&sm.v_full[i], H::GW);
+      mbar_init(&sm.k_free[i], NT);
+      mbar_init(&sm.v_free[i], NT);
     }
-    for (int i = 0; i < XR; ++i) mbar_init(&sm.x_full[i], H::CONV);
-    mbar_init(&sm.drained, 1);
+    for (int i = 0; i < XR; ++i) mbar_init(&sm.x_full[i], H::GW);
+    for (int i = 0; i < 2 * NT; ++i) mbar_init(&sm.drained[i], 1);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == H::SOFT + H::CONV) {   // the issuer owns the tensor memory
+  if (warp == H::SOFT + H::CONV) {   // an issuer owns the tensor memory
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(H::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -201,97 +201,99 @@ portions_kernel(const PortionArgs a) {
 
   if (warp >= H::SOFT + H::CONV) {
     registers<H::R_ISSUE, H::R_LAUNCH>();
-    if (warp == H::SOFT + H::CONV) {
-    // One value for the warp, and known as that to the compiler: what the products take stays in uniform registers.
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), tm_o = tm + NT * 2 * TK;
+    // Warp t of these issues S_t, warp NT + t the products P_t V.  (One warp for all of them was the bound: a product took it about 145
+    // clocks whatever its size.)  One value for the warp, and known as that to the compiler: what the products take stays in uniform
+    // registers.
+    const int w = warp - H::SOFT - H::CONV, t = w % NT;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)(2 * t * TK);      // this head's two buffers of S
     const int n = __shfl_sync(0xffffffffu, n_blocks, 0);
-    constexpr uint32_t idesc_s = idesc_of(TK, false), idesc_o = idesc_of(DP, true);
-    const uint64_t dq0 = desc_of(smem_u32(sm.q[0]), 16), dk0 = desc_of(smem_u32(sm.k[0]), 16), dv0 = desc_of(smem_u32(sm.v[0]), H::SPAN);
-    // S_t of block i, once its keys are there; its buffer of tensor memory is free
-    auto issue_s = [&](int t, int i) {
-      if (!mbar_wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag)) return false;
-      after_sync();
-      if (elect_one()) {
-        const uint64_t dq = dq0 + (uint32_t)(t * (H::QTILE / 16)), dk = dk0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j)               // 16 columns: 32 bytes inside a span of 64, then the next span
-          umma_bf16(tm + (uint32_t)((2 * t + (i & 1)) * TK), dq + (uint32_t)((j >> 2) * (H::QSPAN / 16) + 2 * (j & 3)),
-                    dk + (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3)), idesc_s, j > 0 ? 1u : 0u);
-        umma_commit(&sm.s_full[t][i & 1]);
-        if (t == NT - 1) umma_commit(&sm.k_free[i % H::KST]);
-      }
-      __syncwarp();
-      return true;
-    };
     bool ok = true;
-    for (int t = 0; t < NT && ok; ++t) ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
-    for (int i = 0; i < 2 && i < n; ++i)
-      for (int t = 0; t < NT && ok; ++t) ok = issue_s(t, i);
-    for (int i = 0; i < n && ok; ++i) {
+    if (w < NT) {
+      constexpr uint32_t idesc = idesc_of(TK, false);
+      const uint64_t dq = desc_of(smem_u32(sm.q[0]), 16) + (uint32_t)(t * (H::QTILE / 16)), dk0 = desc_of(smem_u32(sm.k[0]), 16);
+      ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
+      for (int i = 0; i < n && ok; ++i) {
+        // the buffer is free when P V of the block before last has been formed
+        if (i >= 2 && !(ok = mbar_wait_warp(&sm.pv_done[t][i & 1], (uint32_t)(((i - 2) >> 1) & 1), abort_flag))) break;
+        if (!(ok = mbar_wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        after_sync();
+        if (elect_one()) {
+          const uint64_t dk = dk0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+          for (int j = 0; j < DP / 16; ++j)             // 16 columns: 32 bytes inside a span of 64, then the next span
+            umma_bf16(tm + (uint32_t)((i & 1) * TK), dq + (uint32_t)((j >> 2) * (H::QSPAN / 16) + 2 * (j & 3)),
+                      dk + (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3)), idesc, j > 0 ? 1u : 0u);
+          umma_commit(&sm.s_full[t][i & 1]);
+          umma_commit(&sm.k_free[i % H::KST]);
+        }
+        __syncwarp();
+      }
+    } else if (w < 2 * NT) {
+      constexpr uint32_t idesc = idesc_of(DP, true);
+      const uint64_t dv0 = desc_of(smem_u32(sm.v[0]), H::SPAN);
+      const uint32_t to = __shfl_sync(0xffffffffu, tmem_o, 0) + (uint32_t)(t * DP);
+      for (int i = 0; i < n && ok; ++i) {
         if (!(ok = mbar_wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
-        if (t == 0 && !(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        if (!(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
         after_sync();
         if (elect_one()) {
           const uint64_t dv = dv0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
 #pragma unroll
           for (int j = 0; j < TK / 16; ++j)             // 16 keys: 8 columns of P, 16 rows of V
-            umma_ts(tm_o + t * DP, tm + (uint32_t)((2 * t + (i & 1)) * TK + 8 * j), dv + (uint32_t)(j * (16 * 128 / 16)), idesc_o,
-                    i > 0 || j > 0 ? 1u : 0u);
-          umma_commit(&sm.pv_done[t]);
-          if (t == NT - 1) umma_commit(&sm.v_free[i % H::KST]);
+            umma_ts(to, tm + (uint32_t)((i & 1) * TK + 8 * j), dv + (uint32_t)(j * (16 * 128 / 16)), idesc, i > 0 || j > 0 ? 1u : 0u);
+          umma_commit(&sm.pv_done[t][i & 1]);
+          umma_commit(&sm.v_free[i % H::KST]);
         }
         __syncwarp();
-        // the S that takes the place of the P used before this one: with two heads the other head's, so that nothing is waited for
-        const int to = NT == 1 ? 0 : t ^ 1, io = NT == 1 || t == 1 ? i : i - 1;
-        if (io >= 0 && io + 2 < n) {
-          if (!(ok = mbar_wait_warp(&sm.pv_done[to], (uint32_t)(io & 1), abort_flag))) break;
-          if (!(ok = issue_s(to, io + 2))) break;
-        }
       }
     }
-    // whatever ended the loop: no product is under way when the tensor memory is freed
-    if (elect_one()) umma_commit(&sm.drained);
-    __syncwarp();
-    int never = 0;
-    mbar_wait_warp(&sm.drained, 0, &never);
+    if (w < 2 * NT) {
+      // whatever ended the loop: no product is under way when the tensor memory is freed
+      if (elect_one()) umma_commit(&sm.drained[w]);
+      __syncwarp();
+      int never = 0;
+      mbar_wait_warp(&sm.drained[w], 0, &never);
     }
   } else if (warp >= H::SOFT) {
     registers<H::R_CONV, H::R_LAUNCH>();
     // converters: a thread takes 16 codes (a piece of a row) at a time
-    const int c = threadIdx.x - 32 * H::SOFT, cw = warp - H::SOFT;
+    const int group = (warp - H::SOFT) / H::GW, c = threadIdx.x - 32 * (H::SOFT + group * H::GW), cw = (warp - H::SOFT) % H::GW;
     const int pieces = a.dim / 16, per = a.page / BLK;
     const int* bt = a.block_table + (size_t)req * a.max_pages;
     // pad columns: zeros, once
-    for (int e = c; e < (DP / 16 - pieces) * TK; e += 32 * H::CONV) {
+    for (int e = c; e < (DP / 16 - pieces) * TK; e += 32 * H::GW) {
       const int r = e % TK, p16 = pieces + e / TK;
-      for (int b = 0; b < H::KST; ++b)
+      for (int b = group; b < H::KST; b += 2)
         for (int s = 0; s < 2; ++s) {
           const int p = (p16 & 3) * 2 + s, at = (p16 >> 2) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4);
           *reinterpret_cast<uint4*>(sm.k[b] + at) = make_uint4(0, 0, 0, 0);
           *reinterpret_cast<uint4*>(sm.v[b] + at) = make_uint4(0, 0, 0, 0);
         }
     }
-    // lane i of a warp (i < GR, and the lanes behind them again) knows the tile of the pool that group i of a block is in, or -1
+    // Lane i of a warp (i < GR, and the lanes behind them again) knows in which page group i of a block is, and then which tile of the
+    // pool that is (-1: none).  The two are apart because a load that is used at once holds the warp up for its whole latency.
+    const int shift = __ffs(a.page) - 1;
+    auto first_of = [&](int i) { return (kb_lo + i) * TK + (lane & (GR - 1)) * BLK; };
+    auto wanted = [&](int i) { return i < n_blocks && first_of(i) <= last_pos && first_of(i) + BLK > first_key; };
     auto look_up = [&](int i) {
-      int id = -1;
-      const int key = (kb_lo + i) * TK + (lane & (GR - 1)) * BLK;
-      if (i < n_blocks && key <= last_pos && key + BLK > first_key) {
-        const int lp = key / a.page;
-        const int pg = lp < a.max_pages ? bt[lp] : -1;
-        if (pg >= 0 && pg < a.n_pages) id = (pg * a.Hkv + hk) * per + (key & (a.page - 1)) / BLK;
-        else if (c < GR) atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+      const int lp = first_of(i) >> shift;
+      return wanted(i) && lp < a.max_pages ? bt[lp] : -1;
+    };
+    auto tile_of = [&](int i, int pg) {
+      if (!wanted(i)) return -1;
+      if (pg < 0 || pg >= a.n_pages) {
+        if (c < GR) atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+        return -1;
       }
-      return id;
+      return (pg * a.Hkv + hk) * per + ((first_of(i) & (a.page - 1)) / BLK);
     };
     constexpr int PIECES = DP / 16;                     // of a row at most: 8 or 4
-    constexpr int N = TK * PIECES / (32 * H::CONV);     // 16-byte loads of a thread
+    constexpr int N = TK * PIECES / (32 * H::GW);       // 16-byte loads of a thread
     // eight neighbouring threads stand on four pieces of two rows: their stores meet in no bank
     const int piece = PIECES == 8 ? (c & 3) + 4 * (c >> 3 & 1) : c & 3, r_first = PIECES == 8 ? (c >> 2 & 1) + 2 * (c >> 4) : c >> 2;
     const bool mine = piece < pieces;
-    constexpr int STEP = 32 * H::CONV / PIECES;         // rows between a thread's loads
-    uint4 kr[N], vr[N];                                 // a block's codes, on their way while the block before is converted
+    constexpr int STEP = 32 * H::GW / PIECES;           // rows between a thread's loads
+    uint4 kr[N], vr[N];                                 // a block's codes, on their way while the group's block before is converted
     auto load = [&](const int8_t* pool, uint4 (&x)[N], int id) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -302,7 +304,8 @@ portions_kernel(const PortionArgs a) {
       }
     };
     const int place0 = (piece >> 2) * H::SPAN + r_first * 128 + ((((piece & 3) * 2) ^ (r_first & 7)) << 4);      // (STEP is a multiple of 8)
-    int id = look_up(0), id1 = look_up(1);
+    int pg1 = look_up(group + 2), pg2 = look_up(group + 4);       // of this group's blocks behind the first
+    int id = tile_of(group, look_up(group));
     pdl_wait();
     const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
     const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
@@ -311,7 +314,7 @@ portions_kernel(const PortionArgs a) {
     if (lane < GR && id >= 0) { sk = __ldcg(ks + id); sv = __ldcg(vs + id); }
     load(v8, vr, id);
     bool ok = true;
-    for (int i = 0; i < n_blocks && ok; ++i) {
+    for (int i = group; i < n_blocks && ok; i += 2) {
       const int b = i % H::KST;
       const uint32_t turn = (uint32_t)((i / H::KST) & 1);
       if (i >= H::KST && !(ok = mbar_wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
@@ -342,10 +345,12 @@ portions_kernel(const PortionArgs a) {
         mbar_arrive(&sm.x_full[i % XR]);
       }
       const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
+      const int id1 = tile_of(i + 2, pg1);
+      pg1 = pg2;
+      pg2 = look_up(i + 6);
       load(k8, kr, id1);
       sk = sv = 0.f;
       if (lane < GR && id1 >= 0) { sk = __ldcg(ks + id1); sv = __ldcg(vs + id1); }
-      const int id2 = look_up(i + 2);
       if (i >= H::KST && !(ok = mbar_wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
       dst = sm.v[b] + place0;
 #pragma unroll
@@ -367,7 +372,6 @@ portions_kernel(const PortionArgs a) {
       if (lane == 0) mbar_arrive(&sm.v_full[b]);
       load(v8, vr, id1);
       id = id1;
-      id1 = id2;
     }
   } else {
     registers<H::R_SOFT, H::R_LAUNCH>();
@@ -471,7 +475,7 @@ portions_kernel(const PortionArgs a) {
         if (grow) m = mx;
         l *= corr;
         if (i > 0) {                                    // O as P V of the block before leaves it
-          if (!(ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((i - 1) & 1), abort_flag))) break;
+          if (!(ok = mbar_wait_warp(&sm.pv_done[t][(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1), abort_flag))) break;
           after_sync();
 #pragma unroll 1
           for (int c = 0; c < DP / 32; ++c) {
@@ -516,9 +520,8 @@ portions_kernel(const PortionArgs a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[t][i & 1]);
     }
-    // S of the last block needed P V of the third last alone: the last two may both be under way, and a parity tells neighbours apart only
-    if (ok && n_blocks > 1) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 2) & 1), abort_flag);
-    if (ok) ok = mbar_wait_warp(&sm.pv_done[t], (uint32_t)((n_blocks - 1) & 1), abort_flag);
+    // (the products of a head are formed in order: with the last one all are there)
+    if (ok) ok = mbar_wait_warp(&sm.pv_done[t][(n_blocks - 1) & 1], (uint32_t)(((n_blocks - 1) >> 1) & 1), abort_flag);
     if (ok) {
       after_sync();
       if (a.sinks && m != -INFINITY) l += ex2(a.sinks[h] * LOG2E - m);
