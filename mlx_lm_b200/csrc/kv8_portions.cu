@@ -5,10 +5,11 @@
 //   converters  4 or 8 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
 //               the scales of the block's eight groups of 16 positions beside them
 //   issuers     2 warps a head: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
-//   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 over S
-// A head has two buffers of S: while the softmax works on one block, P V of the block before and S of the one behind are formed, so that
-// the chain of a tile's blocks is its softmax alone.  (With blocks of 128 keys and one buffer P V and S stood in that chain: 398 us
-// where this takes 0.)  Two heads of a CTA have chains of their own, and a converted block serves both.
+//   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 beside S
+// The softmax threads take a row of S into registers and let go of it: S of the next block is formed while they work on this one, and
+// P V of the block before as well (two buffers of P), so that the chain of a tile's blocks is its softmax alone.  (With P over S in
+// blocks of 128 keys P V and S stood in that chain: 398 us for 2048 queries of 32/8 heads of 128 at position 6144.)
+// Two heads of a CTA have chains of their own, and a converted block serves both.
 //
 // Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
 // operation), and 128 * 2^-24 sum(q), a number of the query, comes off S in the multiply-add that scales it.  V enters as the exact
@@ -18,8 +19,8 @@
 // Scales: s = scale * sk * (q . codes) with sk the block's key scale; the weight that meets V's codes is w = exp(s) * sv, so the exponent
 // gets log2(sv), the running maximum is that of s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
 // its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) counts as codes of
-// 0 with sv 1.  The maximum follows a score only once that is more than 2^8 beyond it (fp16 holds 2^15), so O is scaled again, by the softmax threads
-// in tensor memory, a few times a row at most.
+// 0 with sv 1.  The maximum follows a score only once its weight is above 2^12 (fp16 holds 2^15), so O is scaled again, by the softmax
+// threads in tensor memory, a few times a row at most.
 //
 // Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
 // MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone.
@@ -36,7 +37,7 @@ constexpr int GR = TK / BLK;         // groups of a block
 constexpr int XR = 8;                // blocks whose scales are kept
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
-constexpr float SLACK = 8.f;
+constexpr uint32_t HIGH = 0x6c00;    // 2^12 as fp16: the largest weight that a pass leaves be
 
 struct PortionArgs {
   const __nv_bfloat16* q;
@@ -63,7 +64,7 @@ struct Shape {
   static constexpr int R_SOFT = NT == 1 ? 120 : DP == 128 ? 128 : 144, R_CONV = DP == 128 || NT == 1 ? 88 : 96, R_ISSUE = NT == 1 ? 24 : 40;
   static_assert(32 * (SOFT * R_SOFT + CONV * R_CONV + 4 * R_ISSUE) <= THREADS * R_LAUNCH, "registers");
   static constexpr int CTAS = NT == 1 ? 2 : 1;
-  static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: two buffers of S_t at 128 t, O_t behind them
+  static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, two buffers of P_t behind it; then O_t
   static constexpr int QSPAN = TQ * 128, SPAN = TK * 128;         // bytes of a tile's rows of 64 columns
   static constexpr int QTILE = QSPAN * (DP / 64), TILE = SPAN * (DP / 64);
 };
@@ -76,8 +77,8 @@ struct Smem {
   alignas(1024) uint8_t v[H::KST][H::TILE];
   float sk[XR][GR], lsv[XR][GR], rsv[XR][GR];           // of the last blocks: key scale, log2 and reciprocal of the value scale
   uint32_t missing[XR];                                 // groups without a page
-  alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST], x_full[XR];
-  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT][2], drained[2 * NT];
+  alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST];
+  uint64_t s_full[NT], s_read[NT], p_full[NT][2], pv_done[NT][2], drained[2 * NT];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -122,6 +123,11 @@ __device__ __forceinline__ void registers() {
   if constexpr (N > AT_LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
   else if constexpr (N < AT_LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
 // two float32 at a time
 __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
@@ -130,6 +136,16 @@ __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, f
 __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
   asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
       "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
+}
+// mbar_wait_warp with one look at the barrier in front of its loop.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, done != 0) || mbar_wait_warp(bar, parity, abort_flag);
 }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -174,7 +190,9 @@ portions_kernel(const PortionArgs a) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < NT; ++i) {
       mbar_init(&sm.q_full[i], 4);
-      for (int b = 0; b < 2; ++b) { mbar_init(&sm.s_full[i][b], 1); mbar_init(&sm.p_full[i][b], 4); mbar_init(&sm.pv_done[i][b], 1); }
+      mbar_init(&sm.s_full[i], 2);
+      mbar_init(&sm.s_read[i], 4);
+      for (int b = 0; b < 2; ++b) { mbar_init(&sm.p_full[i][b], 4); mbar_init(&sm.pv_done[i][b], 1); }
     }
     for (int i = 0; i < H::KST; ++i) {
       mbar_init(&sm.k_full[i], H::GW);
@@ -182,7 +200,6 @@ portions_kernel(const PortionArgs a) {
       mbar_init(&sm.k_free[i], NT);
       mbar_init(&sm.v_free[i], NT);
     }
-    for (int i = 0; i < XR; ++i) mbar_init(&sm.x_full[i], H::GW);
     for (int i = 0; i < 2 * NT; ++i) mbar_init(&sm.drained[i], 1);
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -205,25 +222,28 @@ portions_kernel(const PortionArgs a) {
     // clocks whatever its size.)  One value for the warp, and known as that to the compiler: what the products take stays in uniform
     // registers.
     const int w = warp - H::SOFT - H::CONV, t = w % NT;
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)(2 * t * TK);      // this head's two buffers of S
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)(2 * t * TK);      // this head's S, P 64 columns on
     const int n = __shfl_sync(0xffffffffu, n_blocks, 0);
     bool ok = true;
     if (w < NT) {
       constexpr uint32_t idesc = idesc_of(TK, false);
       const uint64_t dq = desc_of(smem_u32(sm.q[0]), 16) + (uint32_t)(t * (H::QTILE / 16)), dk0 = desc_of(smem_u32(sm.k[0]), 16);
-      ok = mbar_wait_warp(&sm.q_full[t], 0, abort_flag);
+      ok = wait_warp(&sm.q_full[t], 0, abort_flag);
       for (int i = 0; i < n && ok; ++i) {
-        // the buffer is free when P V of the block before last has been formed
-        if (i >= 2 && !(ok = mbar_wait_warp(&sm.pv_done[t][i & 1], (uint32_t)(((i - 2) >> 1) & 1), abort_flag))) break;
-        if (!(ok = mbar_wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        if (i > 0 && !(ok = wait_warp(&sm.s_read[t], (uint32_t)((i - 1) & 1), abort_flag))) break;     // S is in registers
+        if (!(ok = wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        // P V of the block before last has read the buffer that this block's P goes to
+        if (i >= 2 && !(ok = wait_warp(&sm.pv_done[t][i & 1], (uint32_t)(((i - 2) >> 1) & 1), abort_flag))) break;
         after_sync();
+        // with the scales, which came with the keys, and that buffer the softmax has all it needs once S is there
+        if (lane == 0) mbar_arrive(&sm.s_full[t]);
         if (elect_one()) {
           const uint64_t dk = dk0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
 #pragma unroll
           for (int j = 0; j < DP / 16; ++j)             // 16 columns: 32 bytes inside a span of 64, then the next span
-            umma_bf16(tm + (uint32_t)((i & 1) * TK), dq + (uint32_t)((j >> 2) * (H::QSPAN / 16) + 2 * (j & 3)),
+            umma_bf16(tm, dq + (uint32_t)((j >> 2) * (H::QSPAN / 16) + 2 * (j & 3)),
                       dk + (uint32_t)((j >> 2) * (H::SPAN / 16) + 2 * (j & 3)), idesc, j > 0 ? 1u : 0u);
-          umma_commit(&sm.s_full[t][i & 1]);
+          umma_commit(&sm.s_full[t]);
           umma_commit(&sm.k_free[i % H::KST]);
         }
         __syncwarp();
@@ -233,14 +253,14 @@ portions_kernel(const PortionArgs a) {
       const uint64_t dv0 = desc_of(smem_u32(sm.v[0]), H::SPAN);
       const uint32_t to = __shfl_sync(0xffffffffu, tmem_o, 0) + (uint32_t)(t * DP);
       for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = mbar_wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
-        if (!(ok = mbar_wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        if (!(ok = wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
+        if (!(ok = wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
         after_sync();
         if (elect_one()) {
           const uint64_t dv = dv0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
 #pragma unroll
           for (int j = 0; j < TK / 16; ++j)             // 16 keys: 8 columns of P, 16 rows of V
-            umma_ts(to, tm + (uint32_t)((i & 1) * TK + 8 * j), dv + (uint32_t)(j * (16 * 128 / 16)), idesc, i > 0 || j > 0 ? 1u : 0u);
+            umma_ts(to, tm + (uint32_t)(TK + (i & 1) * (TK / 2) + 8 * j), dv + (uint32_t)(j * (16 * 128 / 16)), idesc, i > 0 || j > 0 ? 1u : 0u);
           umma_commit(&sm.pv_done[t][i & 1]);
           umma_commit(&sm.v_free[i % H::KST]);
         }
@@ -317,7 +337,7 @@ portions_kernel(const PortionArgs a) {
     for (int i = group; i < n_blocks && ok; i += 2) {
       const int b = i % H::KST;
       const uint32_t turn = (uint32_t)((i / H::KST) & 1);
-      if (i >= H::KST && !(ok = mbar_wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
+      if (i >= H::KST && !(ok = wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
       uint8_t* dst = sm.k[b] + place0;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -340,10 +360,7 @@ portions_kernel(const PortionArgs a) {
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.k_full[b]);
-        mbar_arrive(&sm.x_full[i % XR]);
-      }
+      if (lane == 0) mbar_arrive(&sm.k_full[b]);
       const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
       const int id1 = tile_of(i + 2, pg1);
       pg1 = pg2;
@@ -351,7 +368,7 @@ portions_kernel(const PortionArgs a) {
       load(k8, kr, id1);
       sk = sv = 0.f;
       if (lane < GR && id1 >= 0) { sk = __ldcg(ks + id1); sv = __ldcg(vs + id1); }
-      if (i >= H::KST && !(ok = mbar_wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
+      if (i >= H::KST && !(ok = wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
       dst = sm.v[b] + place0;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -380,7 +397,7 @@ portions_kernel(const PortionArgs a) {
     const int pos = pos0 + r;
     const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s0 = tmem + 2 * t * TK + lanes, t_o = tmem_o + t * DP + lanes;
+    const uint32_t t_s = tmem + 2 * t * TK + lanes, t_o = tmem_o + t * DP + lanes;
     float fac, off;
     pdl_wait();
     {
@@ -432,15 +449,16 @@ portions_kernel(const PortionArgs a) {
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
       const int key0 = (kb_lo + i) * TK, x4 = i % XR;
-      const uint32_t t_s = t_s0 + (uint32_t)((i & 1) * TK);
-      if (!(ok = mbar_wait_warp(&sm.x_full[x4], (uint32_t)((i / XR) & 1), abort_flag))) break;
-      if (!(ok = mbar_wait_warp(&sm.s_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;
+      if (!(ok = wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
       after_sync();
       const uint32_t gone = sm.missing[x4];
       uint32_t s[TK / 32][32];
 #pragma unroll
       for (int c = 0; c < TK / 32; ++c) tmem_ld32(t_s + 32 * c, s[c]);
       ld_wait(s);
+      before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.s_read[t]);        // the next S may be formed over it
       // blocks that every row of the tile sees whole need no mask
       if (gone != 0 || key0 + TK - 1 > pos0 || (a.window > 0 && key0 < last_pos - a.window + 1)) {
         const int first = lo - key0, last = pos - key0;
@@ -456,72 +474,87 @@ portions_kernel(const PortionArgs a) {
             if (!(bits >> e & 1)) s[c][e] = 0xff800000u;          // -inf: its exponential below is 0
         }
       }
-      // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
-      // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
-      float mx = -INFINITY;
+      // A pass with the maximum as it is; its numbers show whether it was too low (the search for the largest score would take as long as
+      // a third of the exponentials).  Then, and in blocks before which a row has seen nothing, the maximum first and the pass again.
+      const uint32_t t_p = t_s + TK + (uint32_t)((i & 1) * (TK / 2));
+      bool search = __any_sync(0xffffffffu, m == -INFINITY);
+      for (;;) {
+        if (search) {
+          // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
+          // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
+          float mx = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        const uint32_t* x = &s[g >> 1][16 * (g & 1)];
-        float y[4];
+          for (int g = 0; g < GR; ++g) {
+            const uint32_t* x = &s[g >> 1][16 * (g & 1)];
+            float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = fmaxf(fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 4])), fmaxf(__uint_as_float(x[e + 8]), __uint_as_float(x[e + 12])));
-        const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-        mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
-      }
-      const bool grow = mx > m + SLACK;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float corr = grow ? ex2(m - mx) : 1.f;    // 2^-inf = 0
-        if (grow) m = mx;
-        l *= corr;
-        if (i > 0) {                                    // O as P V of the block before leaves it
-          if (!(ok = mbar_wait_warp(&sm.pv_done[t][(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1), abort_flag))) break;
-          after_sync();
+            for (int e = 0; e < 4; ++e)
+              y[e] = fmaxf(fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 4])), fmaxf(__uint_as_float(x[e + 8]), __uint_as_float(x[e + 12])));
+            const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+            mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
+          }
+          const bool grow = mx > m;
+          const float corr = grow ? ex2(m - mx) : 1.f;  // 2^-inf = 0
+          if (grow) m = mx;
+          l *= corr;
+          if (i > 0 && __any_sync(0xffffffffu, grow)) { // O as P V of the block before leaves it
+            if (!(ok = wait_warp(&sm.pv_done[t][(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1), abort_flag))) break;
+            after_sync();
 #pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t y[32];
-            tmem_ld32(t_o + 32 * c, y);
-            ld_wait(y);
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t y[32];
+              tmem_ld32(t_o + 32 * c, y);
+              ld_wait(y);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t z[16];
+              for (int half = 0; half < 2; ++half) {
+                uint32_t z[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[16 * half + e]) * corr);
-              st16(t_o + 32 * c + 16 * half, z);
+                for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[16 * half + e]) * corr);
+                st16(t_o + 32 * c + 16 * half, z);
+              }
             }
+            st_wait();
           }
-          st_wait();
         }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
+        const float base = m == -INFINITY ? 0.f : m;
+        float add = 0.f;
+        uint32_t high = 0;                              // the largest two weights, as fp16
 #pragma unroll
-      for (int c = 0; c < TK / 32; ++c) {
-        uint32_t packed[16];
+        for (int c = 0; c < TK / 32; ++c) {
+          uint32_t packed[16];
 #pragma unroll
-        for (int gg = 0; gg < 2; ++gg) {
-          const int g = 2 * c + gg;
-          const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f), k = fmaf(-off, f, sm.lsv[x4][g] - base);
-          float sum0 = 0.f, sum1 = 0.f;
+          for (int gg = 0; gg < 2; ++gg) {
+            const int g = 2 * c + gg;
+            const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f), k = fmaf(-off, f, sm.lsv[x4][g] - base);
+            float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < BLK; e += 2) {
-            float p0, p1;
-            fma2(p0, p1, __uint_as_float(s[c][16 * gg + e]), __uint_as_float(s[c][16 * gg + e + 1]), f, k);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            add2(sum0, sum1, p0, p1);
-            packed[8 * gg + (e >> 1)] = half2_of(p0, p1);
+            for (int e = 0; e < BLK; e += 2) {
+              float p0, p1;
+              fma2(p0, p1, __uint_as_float(s[c][16 * gg + e]), __uint_as_float(s[c][16 * gg + e + 1]), f, k);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              add2(sum0, sum1, p0, p1);
+              packed[8 * gg + (e >> 1)] = half2_of(p0, p1);
+              high = max_half2(high, packed[8 * gg + (e >> 1)]);
+            }
+            add = fmaf(sum0 + sum1, sm.rsv[x4][g], add);
           }
-          l = fmaf(sum0 + sum1, sm.rsv[x4][g], l);
+          st16(t_p + 16 * c, packed);
         }
-        st16(t_s + 16 * c, packed);                     // over columns that have been read
+        if (search || !__any_sync(0xffffffffu, (high & 0xffffu) > HIGH || high >> 16 > HIGH)) {
+          l += add;
+          break;
+        }
+        search = true;
       }
+      if (!ok) break;
       st_wait();
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[t][i & 1]);
     }
     // (the products of a head are formed in order: with the last one all are there)
-    if (ok) ok = mbar_wait_warp(&sm.pv_done[t][(n_blocks - 1) & 1], (uint32_t)(((n_blocks - 1) >> 1) & 1), abort_flag);
+    if (ok) ok = wait_warp(&sm.pv_done[t][(n_blocks - 1) & 1], (uint32_t)(((n_blocks - 1) >> 1) & 1), abort_flag);
     if (ok) {
       after_sync();
       if (a.sinks && m != -INFINITY) l += ex2(a.sinks[h] * LOG2E - m);
