@@ -23,6 +23,7 @@ def setup_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--prefill-step-size", default=2048, type=int, help="Tokens of a prompt run per step")
     p.add_argument("--delay", type=float, default=0, help="Seconds to wait between trials")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--kv-bits", type=int, choices=[8], default=None, help="Keys and values in 8 bits")
     return p
 
 
@@ -37,14 +38,14 @@ def main(argv=None) -> None:
     def single_bench():
         response = None
         for response in stream_generate(model, tokenizer, prompts[0], max_tokens=args.generation_tokens,
-                                        prefill_step_size=args.prefill_step_size):
+                                        prefill_step_size=args.prefill_step_size, kv_bits=args.kv_bits):
             pass
         return response
 
     def batch_bench():
         return batch_generate(model, tokenizer, prompts, max_tokens=args.generation_tokens,
                               prefill_step_size=args.prefill_step_size, completion_batch_size=args.batch_size,
-                              prefill_batch_size=args.batch_size).stats
+                              prefill_batch_size=args.batch_size, kv_bits=args.kv_bits).stats
 
     bench = single_bench if args.batch_size == 1 else batch_bench
     print("Running warmup..")

@@ -22,6 +22,12 @@ Life of a request: ``add_request`` takes a state slot; before a step
 ``truncate`` rewinds; ``release`` gives everything back.  Freed pages go on
 top of the free list (LIFO), so a small pool re-uses pages at once.
 
+``kv_bits=8`` keeps keys and values as int8 codes, with a float32 scale for
+each block of 16 positions and head in pools beside them (mlx-lm's quantized
+cache, mlx_lm/models/cache.py:230-322, which has a scale for every token and
+group of columns and grows with its request): a little more than half the bytes
+of bfloat16.  Every cache of the model has to allow it (``PagedKVSpec.eight_bits``).
+
 The bookkeeping is plain Python and runs without a GPU; device tensors are
 created only when a device is given.
 """
@@ -93,6 +99,8 @@ class KVGroup:
     pool: PagePool
     k: object = None   # device tensor [len(cache_ids), n_pages, heads, page, head_dim]
     v: object = None
+    k_scale: object = None   # 8-bit caches: float32 [len(cache_ids), n_pages, heads, page / 16]
+    v_scale: object = None
 
     def index_of(self, cache_id: int) -> int:
         return self.cache_ids.index(cache_id)
@@ -119,9 +127,14 @@ class RequestCache:
 
 class CacheManager:
     def __init__(self, cache_specs: Dict[int, object], page_size: int = 16, n_pages: int = 64,
-                 max_requests: int = 64, max_len: int = 1024, dtype=None, device=None):
+                 max_requests: int = 64, max_len: int = 1024, dtype=None, device=None, kv_bits: Optional[int] = None):
         if page_size <= 0 or page_size & (page_size - 1):
             raise ValueError(f"page size {page_size} must be a power of two")
+        if kv_bits not in (None, 8):
+            raise ValueError(f"kv_bits {kv_bits!r}: a cache in the run's type (None) or in 8 bits")
+        if kv_bits:
+            self._check_eight_bits(cache_specs, page_size)
+        self.kv_bits = kv_bits
         self.page_size, self.max_requests, self.max_len = page_size, max_requests, max_len
         self.table_width = (max_len + page_size - 1) // page_size
         self.dtype, self.device = dtype, device
@@ -156,10 +169,31 @@ class CacheManager:
         if device is not None:
             self._allocate_device(n_pages)
 
+    SCALE_BLOCK = 16       # positions of a head that share a scale in an 8-bit cache
+
+    @classmethod
+    def _check_eight_bits(cls, cache_specs: Dict[int, object], page_size: int) -> None:
+        bad = [c for c, s in cache_specs.items() if isinstance(s, PagedKVSpec) and not s.eight_bits]
+        if bad or not any(isinstance(s, PagedKVSpec) for s in cache_specs.values()):
+            what = f"those of {bad[:4]}{' ...' if len(bad) > 4 else ''} cannot" if bad else "this model has none"
+            raise ValueError(f"kv_bits=8 needs attention layers that can read keys and values in 8 bits: {what}")
+        if page_size < cls.SCALE_BLOCK:
+            raise ValueError(f"kv_bits=8: pages of {page_size} positions: at least {cls.SCALE_BLOCK} (a block with one scale)")
+
     # ------------------------------------------------------------ device side
     def _allocate_device(self, n_pages: int) -> None:
         import torch
 
+        if self.kv_bits:
+            for g in self.kv_groups:
+                shape = (len(g.cache_ids), n_pages, g.spec.n_kv_heads, self.page_size, g.spec.head_dim)
+                g.k, g.v = (torch.zeros(shape, dtype=torch.int8, device=self.device) for _ in range(2))
+                g.k_scale, g.v_scale = (torch.zeros(shape[:3] + (self.page_size // self.SCALE_BLOCK,), dtype=torch.float32,
+                                                    device=self.device) for _ in range(2))
+            for g in self.state_groups:
+                g.data = torch.zeros((len(g.cache_ids), self.max_requests) + tuple(g.spec.shape), dtype=torch.float32,
+                                     device=self.device)
+            return
         for g in self.kv_groups:
             shape = (len(g.cache_ids), n_pages, g.spec.n_kv_heads, self.page_size, g.spec.head_dim)
             # zeros, not empty: a masked key's value row is multiplied by a zero weight and must be finite
@@ -180,6 +214,8 @@ class CacheManager:
                 n += g.k.numel() * g.k.element_size()
                 if g.v is not g.k:
                     n += g.v.numel() * g.v.element_size()
+                if g.k_scale is not None:
+                    n += 4 * (g.k_scale.numel() + g.v_scale.numel())
         for g in self.state_groups:
             if g.data is not None:
                 n += g.data.numel() * 4

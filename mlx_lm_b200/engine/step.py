@@ -27,6 +27,7 @@ import torch
 from .. import ops
 from ..cache import CacheManager
 from ..ops import build as kernel_build
+from ..parts.base import PagedKVSpec
 from ..parts.model import Model, RunEntry
 
 
@@ -82,6 +83,8 @@ class LayerCacheView:
     write: bool = True
     k: Optional[torch.Tensor] = None             # [n_pages, heads, page, head_dim]
     v: Optional[torch.Tensor] = None
+    k_scale: Optional[torch.Tensor] = None       # 8-bit caches (k, v int8): float32 [n_pages, heads, page / 16]
+    v_scale: Optional[torch.Tensor] = None
     block_table: Optional[torch.Tensor] = None   # int32 [R, table_width] on the device
     page_size: int = 0
     state: Optional[torch.Tensor] = None         # [n_slots, *shape] float32
@@ -198,8 +201,9 @@ class StepContext:
         if kind == "kv":
             g = mgr.kv_groups[gi]
             i = g.index_of(key)
-            return LayerCacheView("kv", entry.write, k=g.k[i], v=g.v[i], block_table=self._tables[gi],
-                                  page_size=mgr.page_size)
+            eight = g.k_scale is not None
+            return LayerCacheView("kv", entry.write, k=g.k[i], v=g.v[i], k_scale=g.k_scale[i] if eight else None,
+                                  v_scale=g.v_scale[i] if eight else None, block_table=self._tables[gi], page_size=mgr.page_size)
         g = mgr.state_groups[gi]
         return LayerCacheView("state", entry.write, state=g.data[g.index_of(key)], slots=self._slots)
 
@@ -217,7 +221,10 @@ class Engine:
     DEFAULT_MAX_LEN = 8192
 
     def __init__(self, model: Model, page_size: int = 16, max_tokens: Optional[int] = None,
-                 n_pages: Optional[int] = None, max_requests: int = 64, max_len: Optional[int] = None):
+                 n_pages: Optional[int] = None, max_requests: int = 64, max_len: Optional[int] = None,
+                 kv_bits: Optional[int] = None):
+        """``kv_bits=8``: keys and values are kept as 8-bit codes with a scale for each block of 16 positions and head, for models whose
+        attention layers can read them (GPT-2, Lelatar); None: in the model's type."""
         ops.require_cuda()
         self.model = model
         d = model.description
@@ -230,9 +237,15 @@ class Engine:
             n_pages = (max_tokens + page_size - 1) // page_size
         others = ops.F32_ONLY_LIBS if model.dtype == torch.bfloat16 else ops.BF16_ONLY_LIBS
         libs = [n for n in d.kernel_libs() if n not in others]
+        specs = d.cache_specs()
+        if kv_bits:
+            heads = {s.head_dim for s in specs.values() if isinstance(s, PagedKVSpec)}
+            libs += ["kv8"] + [ops.kv8_rows_library(model.dtype, h) for h in sorted(heads)]
+            if any(ops.kv8_portions_supported(model.dtype, h) for h in heads):
+                libs.append("kv8_portions")
+        self.cache = CacheManager(specs, page_size=page_size, n_pages=n_pages, max_requests=max_requests,
+                                  max_len=self.max_len, dtype=model.dtype, device=model.device, kv_bits=kv_bits)
         kernel_build.ensure_built(libs)      # compiled now, in parallel, if this is their first use
-        self.cache = CacheManager(d.cache_specs(), page_size=page_size, n_pages=n_pages, max_requests=max_requests,
-                                  max_len=self.max_len, dtype=model.dtype, device=model.device)
         self.ws = Workspace(model.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=model.device)
         self.h2d_bytes = self.d2h_bytes = 0     # bytes the steps copied to and from the device (counted at the copies)
@@ -565,6 +578,30 @@ class Engine:
     def decode_collect(self, step):
         """Wait for a step launched by ``decode_launch``: ``(tokens, logprobs)`` as lists."""
         return self._graphs[step.key].collect(step)
+
+    def read_cache(self, rid: Hashable, cache_id):
+        """What the cache holds of a live request: keys and values ``[positions, heads, size]`` in the model's type, of cache ``cache_id`` (the
+        block's number, or ``(number, name)`` for one of several of a block).  Positions whose pages a window has given back are zeros.
+        An 8-bit cache gives what its codes stand for."""
+        mgr = self.cache
+        kind, gi = mgr.where(cache_id)
+        if kind != "kv":
+            raise ValueError(f"cache {cache_id!r} holds no keys and values")
+        g, n = mgr.kv_groups[gi], mgr.length(rid)
+        i, dev = g.index_of(cache_id), self.model.device
+        pages = torch.tensor((mgr.requests[rid].pages[gi] or [-1])[:max(1, (n + mgr.page_size - 1) // mgr.page_size)], dtype=torch.int32)
+        held = (pages >= 0).repeat_interleave(mgr.page_size)[:n]
+        if g.k_scale is None:
+            at = pages.clamp(min=0).to(dev).long()
+            out = [x[i][at].transpose(1, 2).flatten(0, 1)[:n] * held.to(dev)[:, None, None] for x in (g.k, g.v)]
+            return out[0], out[1]
+        heads, dim = g.spec.n_kv_heads, g.spec.head_dim
+        k, v = (torch.zeros((n, heads * dim), dtype=self.model.dtype, device=dev) for _ in range(2))
+        if n:
+            req = torch.where(held, 0, -1).to(torch.int32).to(dev)
+            ops.kv8_read(torch.arange(n, dtype=torch.int32, device=dev), req, pages.view(1, -1).to(dev), g.k[i], g.v[i], g.k_scale[i],
+                         g.v_scale[i], k, v, self.status, ops.current_stream())
+        return k.view(n, heads, dim), v.view(n, heads, dim)
 
     def read_status(self) -> int:
         """Bits kernels set instead of faulting (token, position or page id out of range, a bounded wait that

@@ -2,8 +2,11 @@
 ``batch_generate``, ``BatchGenerator`` and the ``generate`` command line
 (mlx_lm/generate.py:54-213, 648-790, 1565-2060, 2063-2186; ``load`` is
 mlx_lm/utils.py:483-541).  Names and meanings of options follow mlx-lm where
-it has them; what this engine does not build (adapters, draft models,
-quantized caches, chat templates, prompt-cache files) is not offered.
+it has them; what this engine does not build (adapters, draft models, chat
+templates, prompt-cache files) is not offered.  ``kv_bits`` is None or 8: the
+whole cache in 8 bits from the first token on, a scale for each block of 16
+positions and head (mlx-lm's ``kv_group_size`` and ``quantized_kv_start`` have no
+counterpart).
 
 All generation, single or batched, runs through one ``Scheduler`` over one
 ``Engine``: a single request is a batch of one.
@@ -59,14 +62,24 @@ def load(path: str, tokenizer_config: Optional[dict] = None, model_config: Optio
     return (model, tokenizer, config) if return_config else (model, tokenizer)
 
 
-def get_engine(model, page_size: int = 16, num_pages: Optional[int] = None, max_requests: int = 64) -> Engine:
+def get_engine(model, page_size: int = 16, num_pages: Optional[int] = None, max_requests: int = 64,
+               kv_bits: Optional[int] = None) -> Engine:
     """The engine of a model, made on first use and kept on the model (the page pool is allocated once)."""
-    key = (page_size, num_pages, max_requests)
+    key = (page_size, num_pages, max_requests, kv_bits)
     cache = model.__dict__.setdefault("_engines", {})
     if key not in cache:
         cache.clear()    # one pool at a time: the old one is freed before the new one is made
-        cache[key] = Engine(model, page_size=page_size, n_pages=num_pages, max_requests=max_requests)
+        cache[key] = Engine(model, page_size=page_size, n_pages=num_pages, max_requests=max_requests, kv_bits=kv_bits)
     return cache[key]
+
+
+def _engine_for(model, engine: Optional[Engine], kv_bits: Optional[int], **sizes) -> Engine:
+    """The caller's engine, or the model's own with a cache of ``kv_bits``."""
+    if engine is None:
+        return get_engine(model, **sizes) if kv_bits is None else get_engine(model, kv_bits=kv_bits, **sizes)
+    if kv_bits is not None and engine.cache.kv_bits != kv_bits:
+        raise ValueError(f"kv_bits={kv_bits}: the engine that was given keeps its cache with kv_bits={engine.cache.kv_bits}")
+    return engine
 
 
 # ---------------------------------------------------------------------- single stream
@@ -102,12 +115,13 @@ def stream_generate(model, tokenizer: TokenizerWrapper, prompt: Union[str, List[
                     logits_processors: Optional[Sequence] = None, prefill_step_size: int = 2048,
                     prompt_progress_callback: Optional[Callable[[int, int], None]] = None,
                     seed: Optional[int] = None, return_logprobs: bool = False, engine: Optional[Engine] = None,
-                    ) -> Generator[GenerationResponse, None, None]:
+                    kv_bits: Optional[int] = None) -> Generator[GenerationResponse, None, None]:
     """Yield the generated text segment by segment.  Stops at an end-of-sequence token
     (``finish_reason="stop"``, the token is not part of the text) or after ``max_tokens``
-    (``"length"``); the last response carries the reason.  ``seed=None``: a fresh seed for every call."""
+    (``"length"``); the last response carries the reason.  ``seed=None``: a fresh seed for every call.  ``kv_bits=8``: keys
+    and values in 8 bits (where no ``engine`` is given: that has its own)."""
     tokens = _encode(tokenizer, prompt)
-    engine = engine or get_engine(model)
+    engine = _engine_for(model, engine, kv_bits)
     dev_sampler = DeviceSampler(model.device, seed=seed, return_logprobs=return_logprobs, engine=engine)
     sched = Scheduler(engine, dev_sampler, max_requests=1, max_prefilling=1, prefill_step_size=prefill_step_size,
                       max_tokens_per_step=max(prefill_step_size, 1))
@@ -146,13 +160,13 @@ def generate_step(prompt: Union[List[int], torch.Tensor], model, *, max_tokens: 
                   sampler: Optional[Sampler] = None, logits_processors: Optional[Sequence] = None,
                   prefill_step_size: int = 2048,
                   prompt_progress_callback: Optional[Callable[[int, int], None]] = None,
-                  seed: Optional[int] = None,
-                  engine: Optional[Engine] = None) -> Generator[Tuple[int, torch.Tensor], None, None]:
+                  seed: Optional[int] = None, engine: Optional[Engine] = None,
+                  kv_bits: Optional[int] = None) -> Generator[Tuple[int, torch.Tensor], None, None]:
     """Token ids in, ``(token, log-probabilities)`` out, one pair per generated token
     (mlx_lm/generate.py:298-462): the log-probabilities are the float32 ``[vocab]`` vector the token was drawn
     from, on the device.  No tokenizer and no end-of-sequence token: it stops after ``max_tokens``."""
     tokens = [int(t) for t in (prompt.flatten().tolist() if isinstance(prompt, torch.Tensor) else prompt)]
-    engine = engine or get_engine(model)
+    engine = _engine_for(model, engine, kv_bits)
     dev_sampler = DeviceSampler(model.device, seed=seed, return_logprobs=True, engine=engine)
     sched = Scheduler(engine, dev_sampler, max_requests=1, max_prefilling=1, prefill_step_size=prefill_step_size,
                       max_tokens_per_step=max(prefill_step_size, 1))
@@ -220,7 +234,7 @@ class BatchGenerator:
     ``completion_batch_size`` bounds the requests that run at once, ``prefill_batch_size`` those of
     them still in their prompt, ``prefill_step_size`` the portion of one prompt per step; added
     here: ``max_tokens_per_step`` (token budget of a step), ``seed``, and the pool's ``page_size``
-    / ``num_pages``.  Prompt caches cannot be passed in or handed out (``caches`` must be None)."""
+    / ``num_pages`` and ``kv_bits`` (8: keys and values in 8 bits).  Prompt caches cannot be passed in or handed out (``caches`` must be None)."""
 
     Response = Response
 
@@ -229,7 +243,7 @@ class BatchGenerator:
                  completion_batch_size: int = 32, prefill_batch_size: int = 8, prefill_step_size: int = 2048,
                  max_kv_size: Optional[int] = None, stream=None, max_tokens_per_step: Optional[int] = None,
                  seed: Optional[int] = None, page_size: int = 16, num_pages: Optional[int] = None,
-                 engine: Optional[Engine] = None, return_logprobs: bool = False):
+                 engine: Optional[Engine] = None, return_logprobs: bool = False, kv_bits: Optional[int] = None):
         if max_kv_size is not None:
             raise ValueError("max_kv_size (a rotating cache for the whole run) is not offered: which keys a layer "
                              "keeps is a property of its mixer (a window), not an option of a run")
@@ -239,8 +253,8 @@ class BatchGenerator:
         self.logits_processors = tuple(logits_processors or ())
         self.completion_batch_size = max(completion_batch_size, prefill_batch_size)
         self.prefill_batch_size, self.prefill_step_size = prefill_batch_size, prefill_step_size
-        self.engine = engine or get_engine(model, page_size=page_size, num_pages=num_pages,
-                                           max_requests=max(64, self.completion_batch_size))
+        self.engine = _engine_for(model, engine, kv_bits, page_size=page_size, num_pages=num_pages,
+                                  max_requests=max(64, self.completion_batch_size))
         self._sampler = DeviceSampler(model.device, seed=seed, return_logprobs=return_logprobs, engine=self.engine)
         self._sched = Scheduler(self.engine, self._sampler, max_requests=self.completion_batch_size,
                                 max_prefilling=prefill_batch_size, prefill_step_size=prefill_step_size,
@@ -405,6 +419,8 @@ def setup_arg_parser() -> argparse.ArgumentParser:
                    help="bfloat16: the serving kernels; float32: the whole model in true 32-bit arithmetic")
     p.add_argument("--page-size", type=int, default=16, help="tokens in one page of the key/value cache")
     p.add_argument("--num-pages", type=int, default=None, help="pages in the pool (default: enough for 64 requests)")
+    p.add_argument("--kv-bits", type=int, choices=[8], default=None,
+                   help="keep keys and values in 8 bits with a scale for each block of 16 positions and head (default: in --dtype)")
     return p
 
 
@@ -438,7 +454,7 @@ def main(argv: Optional[Sequence[str]] = None) -> None:
                            xtc_probability=args.xtc_probability, xtc_threshold=args.xtc_threshold,
                            xtc_special_tokens=tuple(newline) + tuple(tokenizer.eos_token_ids))
     engine = get_engine(model, page_size=args.page_size, num_pages=args.num_pages, max_requests=1 if args.num_pages
-                        else 64)
+                        else 64, kv_bits=args.kv_bits)
     response = generate(model, tokenizer, prompt, verbose=args.verbose, max_tokens=args.max_tokens, sampler=sampler,
                         prefill_step_size=args.prefill_step_size, seed=args.seed, engine=engine)
     if not args.verbose:

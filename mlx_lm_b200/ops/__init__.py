@@ -810,7 +810,7 @@ def attention_decode(q, positions, token_req, block_table, k_pool, v_pool, out, 
 # a cache of keys and values in 8 bits (csrc/kv8.cu, csrc/kv8_rows.cu, csrc/kv8_rows_tc.cu)
 
 KV8_BLOCK = 16           # positions of a head that share a scale
-KV8_ROWS_MOST = 4096     # rows one launch takes (csrc/kv8_rows.cuh)
+KV8_ROWS_MOST = 512      # rows of a launch: what bounds the scratch memory of many rows (csrc/kv8_rows.cuh takes more)
 
 
 def kv8_supported(page: int, head_dim: int) -> bool:

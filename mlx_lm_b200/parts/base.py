@@ -27,7 +27,7 @@ instances directly.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Mapping, Optional, Sequence, Set, Tuple
 
 import torch
@@ -66,7 +66,9 @@ class PagedKVSpec:
     ``head_dim``; 0: no value pool at all, values are read out of the key rows (a cache of latent rows).
     ``keep_first``: beside a window, the first so many positions of the sequence stay readable for good (their pages
     are never given back).  ``value_heads``: heads of the value pool if they are fewer than the key heads (a divisor of
-    them: several key heads, each a score map of its own, then read the same value head)."""
+    them: several key heads, each a score map of its own, then read the same value head).
+    ``eight_bits``: the mixer can also keep and read these pages as 8-bit codes with a scale for each block of positions
+    and head (``LayerCacheView.k_scale`` is then not None); it is no part of what makes two caches equal."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
@@ -74,6 +76,7 @@ class PagedKVSpec:
     value_dim: Optional[int] = None
     keep_first: Optional[int] = None
     value_heads: Optional[int] = None
+    eight_bits: bool = field(default=False, compare=False)
 
 
 @dataclass(frozen=True)

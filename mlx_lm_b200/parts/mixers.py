@@ -49,7 +49,7 @@ class Attention(Mixer):
         return (self.qkv, self.out)
 
     def cache_spec(self):
-        return PagedKVSpec(self.n_kv_heads, self.head_dim, self.window)
+        return PagedKVSpec(self.n_kv_heads, self.head_dim, self.window, eight_bits=True)
 
     def fold_input_norm(self, norm) -> bool:
         return self.qkv.fold_norm(norm)
@@ -59,7 +59,7 @@ class Attention(Mixer):
         qkv = ctx.ws.get("qkv", T, self.q_width + 2 * self.kv_width, x.dtype)
         q = qkv[:, :self.q_width]
         src = x.source if isinstance(x, Normed) else x      # a Normed: the norm is folded into the projection
-        if (cache.write and self.position is None and x.dtype == torch.bfloat16 and self.width % 8 == 0
+        if (cache.write and cache.k_scale is None and self.position is None and x.dtype == torch.bfloat16 and self.width % 8 == 0
                 and src.stride(0) % 8 == 0 and src.data_ptr() % 16 == 0):
             # nothing to do to q and k before the cache: the projection's epilogue puts keys and values
             # into the pages itself
@@ -76,7 +76,10 @@ class Attention(Mixer):
             v = qkv[:, self.q_width + self.kv_width:]
             if self.position is not None:
                 self.position.rotate(ctx, q, k)
-            if cache.write:
+            if cache.write and cache.k_scale is not None:
+                ops.kv8_append(k, v, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                               ctx.status, ctx.stream)
+            elif cache.write:
                 ops.kv_write(k, v, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, ctx.status,
                              ctx.stream)
         o = ctx.ws.get("attn_out", T, self.q_width, x.dtype)
@@ -95,6 +98,8 @@ def paged_attention(ctx, q, cache, o, n_heads: int, head_dim: int, scale: float,
     128, else the split-key kernel on the CUDA cores), the rest to the kernel for portions; all write their rows
     of ``o``.  ``sinks``: float32 ``[n_heads]``, one more term of each head's softmax denominator, or None."""
     window = window or 0
+    if cache.k_scale is not None:
+        return paged_attention_kv8(ctx, q, cache, o, n_heads, head_dim, scale, window, sinks)
     single_tiles = getattr(ctx, "single_tiles", None)
     portions = (ctx.n_portion and ctx.portion_tiles is not None
                 and ops.attention_portions_supported(q.dtype, head_dim, scale))
@@ -132,6 +137,26 @@ def paged_attention(ctx, q, cache, o, n_heads: int, head_dim: int, scale: float,
                                   rows=ctx.portion_rows, sinks=sinks)
 
 
+def paged_attention_kv8(ctx, q, cache, o, n_heads: int, head_dim: int, scale: float, window: int, sinks=None) -> None:
+    """``paged_attention`` over pages in 8 bits: single rows to their kernel, portions to theirs, or row by row where that does
+    not take them (float32, heads above 128)."""
+    pools = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+
+    def by_row(n: int, rows) -> None:
+        floats, tickets = ops.kv8_rows_scratch(n, n_heads, cache.k.shape[1], head_dim, ctx.max_len)
+        ops.kv8_attention_rows(q, ctx.positions, ctx.token_req, cache.block_table, *pools, o, n_heads, scale, window,
+                               ctx.ws.flat("kv8_partial", floats, torch.float32), ctx.ws.flat("kv8_tickets", tickets, torch.int32),
+                               ctx.max_len, ctx.status, ctx.stream, rows=rows, sinks=sinks)
+
+    if ctx.n_portion and ctx.portion_tiles is not None and ops.kv8_portions_supported(q.dtype, head_dim, scale):
+        ops.kv8_attention_portions(q, ctx.portion_tiles, ctx.n_portion_tiles, cache.block_table, *pools, o, n_heads, scale, window,
+                                   ctx.status, ctx.stream, sinks=sinks)
+    elif ctx.n_portion:
+        by_row(ctx.n_portion, ctx.portion_rows)
+    if ctx.n_single:
+        by_row(ctx.n_single, ctx.single_rows)
+
+
 register_part("mixer", "attention", Attention)
 
 
@@ -150,7 +175,7 @@ class SinkAttention(Mixer):
     ``mix`` returns the output projection in float32 (for a caller that combines it with something else);
     ``forward`` adds it to a float32 residual stream in that projection's epilogue."""
     replayable = True
-    kernel_libs = ("attention", "attention_prefill", "attention_prefill_tc", "rotary")
+    kernel_libs = ("attention", "attention_prefill", "attention_prefill_tc", "rotary", "rms")
 
     def __init__(self, name: str, width: int, n_heads: int, n_kv_heads: int, dim: int, vdim: int, scale: float,
                  eps: float, rot_dims: int = 0, rot_base: float = 10000.0, qk_norm: bool = True, sink: bool = True,
@@ -176,7 +201,7 @@ class SinkAttention(Mixer):
         return (self.qkv, self.out)
 
     def cache_spec(self):
-        return PagedKVSpec(self.n_kv_heads, self.head_dim, self.window)
+        return PagedKVSpec(self.n_kv_heads, self.head_dim, self.window, eight_bits=True)
 
     def param_specs(self) -> List[ParamSpec]:
         specs = []
@@ -213,13 +238,31 @@ class SinkAttention(Mixer):
         self.qkv.forward(ctx, x, proj)
         q = ctx.ws.get("attn_q", T, H * self.head_dim, x.dtype)
         ops.label(self.name + ".prepare", 8.0 * T * n, 2.0 * x.element_size() * T * n)
-        ops.qkv_prepare(proj, 0, H * self.dim, (H + G) * self.dim, H, G, self.dim, self.vdim, self.q_norm, self.k_norm,
-                        self.eps, self.freq, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, q,
-                        cache.write, ctx.status, ctx.stream)
+        if cache.k_scale is not None:
+            self._prepare_kv8(ctx, proj, q, cache)
+        else:
+            ops.qkv_prepare(proj, 0, H * self.dim, (H + G) * self.dim, H, G, self.dim, self.vdim, self.q_norm, self.k_norm,
+                            self.eps, self.freq, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, q,
+                            cache.write, ctx.status, ctx.stream)
         o = ctx.ws.get("attn_out", T, H * self.head_dim, x.dtype)
         ops.label(self.name + ".attention")
         paged_attention(ctx, q, cache, o, H, self.head_dim, self.scale, self.window, sinks=self.sinks)
         return o
+
+    def _prepare_kv8(self, ctx, proj, q, cache) -> None:
+        """Queries, keys and values on their way to an 8-bit cache: the norms first (rounded to the run's type), then one kernel that turns
+        queries and keys and puts keys and values into the pages."""
+        T, H, G = proj.shape[0], self.n_heads, self.n_kv_heads
+        pq, pk, pv = proj[:, :H * self.dim], proj[:, H * self.dim:(H + G) * self.dim], proj[:, (H + G) * self.dim:]
+        if self.qk_norm:
+            nq, nk = ctx.ws.get("attn_q_normed", T, H * self.dim, proj.dtype), ctx.ws.get("attn_k_normed", T, G * self.dim, proj.dtype)
+            ops.rmsnorm(pq, self.q_norm, nq, self.eps, ctx.stream)
+            ops.rmsnorm(pk, self.k_norm, nk, self.eps, ctx.stream)
+            pq, pk = nq, nk
+        if not cache.write:
+            pk = pv = None
+        ops.kv8_append(pk, pv, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                       ctx.status, ctx.stream, freq=self.freq, q=pq, q_out=q)
 
     def mix(self, ctx, x, cache, tag: str = "mix_left"):
         o = self._heads_out(ctx, x, cache)
