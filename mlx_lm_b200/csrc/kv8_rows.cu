@@ -144,21 +144,11 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
 // out [row, Hq * dim] for the rows `rows` (int32 indices into positions, token_req, q and out; null: rows 0 .. n_rows - 1): one query
 // of each head at the row's position.  partial: n_rows * tiles * most_chunks * 4 * (dim + 2) floats; counters: n_rows * tiles, zero
 // before the first call and left zero (tiles: Hkv * ceil(Hq / Hkv / 4)).
-MLXB_EXPORT int mlxb_kv8_rows(const float* q, int ldq, const int* rows, const int* positions, const int* token_req,
-                              const int* block_table, int max_pages, int n_pages, int page, int Hq, int Hkv, int dim, int window,
-                              float scale, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, float* partial,
-                              int* counters, int most_chunks, float* out, int ldo, int n_rows, int* status, const float* sinks,
-                              cudaStream_t stream) {
-  if (n_rows <= 0) return 0;
-  if (n_rows > ROWS_MOST) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d rows, a launch takes %d", n_rows, ROWS_MOST);
-  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d query heads over %d key/value heads", Hq, Hkv);
-  if (dim % 16 || dim < 16 || dim > 256) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: head size %d (a multiple of 16 up to 256)", dim);
-  if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: page size %d (a power of two of at least %d)", page, BLK);
-  if (most_chunks <= 0) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: %d chunks of a row", most_chunks);
-  if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)partial) & 15)
-    return mlxb_fail(MLXB_BAD_ARG, "kv8_rows: pools and scratch memory must be 16-byte aligned");
-  const RowsArgs a{q, ldq, rows, positions, token_req, block_table, max_pages, n_pages, page, Hq, Hkv, dim, window, scale, k8, v8, ks,
-                   vs, sinks, partial, counters, most_chunks, out, ldo, n_rows, status};
+MLXB_EXPORT int mlxb_kv8_rows(const RowsRecord* rec, long long bytes, cudaStream_t stream) {
+  RowsArgs a;
+  if (int e = rows_args(rec, bytes, "kv8_rows", a)) return e;
+  if (a.n_rows <= 0) return 0;
+  const int Hq = a.Hq, Hkv = a.Hkv, dim = a.dim, n_rows = a.n_rows, most_chunks = a.most_chunks;
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
   const size_t smem = (size_t)(n_rows + 1 + (most_chunks + 1) * HT) * 4;
   const long long most = (long long)n_rows * most_chunks * tiles, fill = 4ll * mlxb_sm_count();

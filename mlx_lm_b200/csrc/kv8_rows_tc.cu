@@ -424,21 +424,12 @@ rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
 
 // As mlxb_kv8_rows for bfloat16 and heads of MLXB_HEAD_DIM; tiles of eight query heads: partial n_rows * tiles * most_chunks * 8 *
 // (dim + 2) floats, counters n_rows * tiles (tiles: Hkv * ceil(Hq / Hkv / 8)).
-MLXB_EXPORT int mlxb_kv8_rows_tc(const void* q, int ldq, const int* rows, const int* positions, const int* token_req,
-                                 const int* block_table, int max_pages, int n_pages, int page, int Hq, int Hkv, int dim, int window,
-                                 float scale, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, float* partial,
-                                 int* counters, int most_chunks, void* out, int ldo, int n_rows, int* status, const float* sinks,
-                                 cudaStream_t stream) {
-  if (n_rows <= 0) return 0;
-  if (n_rows > ROWS_MOST) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d rows, a launch takes %d", n_rows, ROWS_MOST);
-  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d query heads over %d key/value heads", Hq, Hkv);
-  if (dim != DH) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: head size %d, this library is for %d", dim, DH);
-  if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: page size %d (a power of two of at least %d)", page, BLK);
-  if (most_chunks <= 0 || most_chunks > 1024) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: %d chunks of a row", most_chunks);
-  if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)partial) & 15)
-    return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: pools and scratch memory must be 16-byte aligned");
-  const RowsArgs a{q, ldq, rows, positions, token_req, block_table, max_pages, n_pages, page, Hq, Hkv, dim, window, scale, k8, v8, ks,
-                   vs, sinks, partial, counters, most_chunks, out, ldo, n_rows, status};
+MLXB_EXPORT int mlxb_kv8_rows_tc(const RowsRecord* rec, long long bytes, cudaStream_t stream) {
+  RowsArgs a;
+  if (int e = rows_args(rec, bytes, "kv8_rows_tc", a)) return e;
+  if (a.n_rows <= 0) return 0;
+  if (a.dim != DH) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: head size %d, this library is for %d", a.dim, DH);
+  const int Hq = a.Hq, Hkv = a.Hkv, n_rows = a.n_rows, most_chunks = a.most_chunks;
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
   const size_t smem = RING + (size_t)(n_rows + 1) * 4;
   const long long most = (long long)n_rows * most_chunks * tiles, fill = (long long)CTAS * mlxb_sm_count();
@@ -446,7 +437,7 @@ MLXB_EXPORT int mlxb_kv8_rows_tc(const void* q, int ldq, const int* rows, const 
   if (cudaError_t e = limit.raise(rows_tc_kernel, RING + (ROWS_MOST + 1) * 4))
     return mlxb_fail((int)e, "kv8_rows_tc: shared memory: %s", cudaGetErrorString(e));
   launch_pdl(rows_tc_kernel, dim3((unsigned)(most < fill ? most : fill)), dim3(WARPS * 32), smem, stream, a, tiles, group_tiles,
-             (ldq % 4 == 0 && !((uintptr_t)q & 7)) ? 1 : 0);
+             (a.ldq % 4 == 0 && !((uintptr_t)a.q & 7)) ? 1 : 0);
   if (int e = mlxb_check_launch("kv8_rows_tc")) return e;
   if (most_chunks == 1) return 0;
   launch_pdl(rows_tc_join_kernel, dim3((unsigned)n_rows * tiles, KT), dim3(128), (size_t)most_chunks * 32, stream, a, tiles, group_tiles);

@@ -13,7 +13,9 @@ runs in here.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_void_p
+import functools
+import struct
+from ctypes import c_char_p, c_float, c_int, c_void_p
 from typing import NamedTuple, Optional
 
 import torch
@@ -87,7 +89,8 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The handle of torch's current stream (without the stream object around it, which takes 3 us to make)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -818,36 +821,69 @@ def kv8_supported(page: int, head_dim: int) -> bool:
     return page >= KV8_BLOCK and page & (page - 1) == 0 and head_dim % 16 == 0 and 16 <= head_dim <= 256
 
 
+_I8, _I32, _F32T, _BF16T = torch.int8, torch.int32, torch.float32, torch.bfloat16
+
+
 def _kv8_pools(k8, v8, k_scale, v_scale, block_table, what: str):
     """Shape of the pages ``[n_pages, heads, page, head_dim]`` of a cache in 8 bits."""
+    shape = k8.shape
+    if (len(shape) == 4 and k8.dtype is _I8 and v8.dtype is _I8 and k_scale.dtype is _F32T and v_scale.dtype is _F32T
+            and block_table.dtype is _I32 and k8.is_cuda and v8.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
+            and v8.shape == shape and k8.is_contiguous() and v8.is_contiguous() and kv8_supported(shape[2], shape[3])):
+        n_pages, Hkv, page, Dh = shape
+        want = (n_pages, Hkv, page // KV8_BLOCK)
+        if (k_scale.shape == want and v_scale.shape == want and k_scale.is_contiguous() and v_scale.is_contiguous()
+                and block_table.dim() == 2 and block_table.is_contiguous()):
+            return shape
+    # something is wrong: say what
     _need(k8, torch.int8, what + " key codes")
     _need(v8, torch.int8, what + " value codes")
     _need(k_scale, torch.float32, what + " key scales")
     _need(v_scale, torch.float32, what + " value scales")
     _need(block_table, torch.int32, what + " block_table")
-    if k8.dim() != 4 or v8.shape != k8.shape or not (k8.is_contiguous() and v8.is_contiguous()):
+    if len(shape) != 4 or v8.shape != shape or not (k8.is_contiguous() and v8.is_contiguous()):
         raise KernelError(f"{what}: codes {tuple(k8.shape)} and {tuple(v8.shape)}: contiguous [n_pages, heads, page, head_dim], both the same")
-    n_pages, Hkv, page, Dh = k8.shape
+    n_pages, Hkv, page, Dh = shape
     if not kv8_supported(page, Dh):
         raise KernelError(f"{what}: pages of {page} positions of heads of {Dh}: a power of two of at least {KV8_BLOCK}, heads a "
                           "multiple of 16 up to 256")
-    want = (n_pages, Hkv, page // KV8_BLOCK)
-    if k_scale.shape != want or v_scale.shape != want or not (k_scale.is_contiguous() and v_scale.is_contiguous()):
-        raise KernelError(f"{what}: scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)}, expected contiguous {want}")
     if block_table.dim() != 2 or not block_table.is_contiguous():
         raise KernelError(f"{what}: block table {tuple(block_table.shape)}: contiguous [requests, pages]")
-    return n_pages, Hkv, page, Dh
+    raise KernelError(f"{what}: scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)}, expected contiguous "
+                      f"{(n_pages, Hkv, page // KV8_BLOCK)}")
+
+
+def _kv8_matrix(t, dtype, what: str):
+    """``(rows, columns, row stride)`` of a 2-D tensor of this type whose rows are contiguous."""
+    strides = t.stride()
+    if len(strides) == 2 and strides[1] == 1 and t.dtype is dtype and t.is_cuda:
+        shape = t.shape
+        return shape[0], shape[1], strides[0]
+    _need(t, dtype, what)
+    ld = _rows(t, what)
+    return t.shape[0], t.shape[1], ld
+
+
+def _kv8_record(layout: str):
+    """Packs the arguments of a launcher into the record of 8-byte fields that it takes: a tenth of the time of as many arguments."""
+    pack = struct.Struct("=" + layout).pack
+    n = struct.calcsize("=" + layout)
+    return lambda *values: (pack(*values), n)
+
+
+_KV8_ARGS = [c_char_p, ctypes.c_longlong, c_void_p]
 
 
 def _kv8_rows_ints(positions, token_req, n: int, what: str) -> None:
+    if (positions.dtype is _I32 and token_req.dtype is _I32 and positions.is_cuda and token_req.is_cuda and positions.numel() >= n
+            and token_req.numel() >= n and positions.is_contiguous() and token_req.is_contiguous()):
+        return
     _need(positions, torch.int32, what + " positions")
     _need(token_req, torch.int32, what + " token_req")
-    if positions.numel() < n or token_req.numel() < n or not (positions.is_contiguous() and token_req.is_contiguous()):
-        raise KernelError(f"{what}: {positions.numel()} positions and {token_req.numel()} requests for {n} rows")
+    raise KernelError(f"{what}: {positions.numel()} positions and {token_req.numel()} requests for {n} rows, contiguous ones")
 
 
-_KV8_APPEND_ARGS = ([c_int] + [c_void_p, c_int] * 4 + [c_int] * 6 + [c_void_p, c_int, c_int, c_float] + [c_void_p] * 3 + [c_int] * 3
-                    + [c_void_p] * 6)
+_kv8_append_record = _kv8_record("13Q16qd")
 
 
 def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale, status, stream, freq=None, interleaved: bool = False,
@@ -868,44 +904,39 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
     n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_append")
     if (k is None) != (v is None) or (k is None and q is None) or (q is None) != (q_out is None):
         raise KernelError("kv8_append: keys and values go together, and queries with their output")
-    x = q if k is None else k
-    if x.dim() != 2:
-        raise KernelError(f"kv8_append: rows {tuple(x.shape)}: [tokens, columns]")
-    T = x.shape[0]
-    code, dk, dv, G = dtype_code(x.dtype), 0, Dh, 0
-    _kv8_rows_ints(positions, token_req, T, "kv8_append")
+    dtype = (q if k is None else k).dtype
+    code, dk, dv, G = dtype_code(dtype), 0, Dh, 0
+    kp = vp = qp = op = fp = ldk = ldv = ldq = ldo = half = 0
+    wide = Hkv * Dh
     if k is not None:
-        for t, what in ((k, "keys"), (v, "values")):
-            _need(t, x.dtype, "kv8_append " + what)
-            _rows(t, "kv8_append " + what)
-            if t.shape[0] != T or t.shape[1] % Hkv or not 0 < t.shape[1] <= Hkv * Dh:
-                raise KernelError(f"kv8_append: {what} {tuple(t.shape)} for {T} rows of {Hkv} heads of at most {Dh}")
-        dk, dv = k.shape[1] // Hkv, v.shape[1] // Hkv
+        T, nk, ldk = _kv8_matrix(k, dtype, "kv8_append keys")
+        Tv, nv, ldv = _kv8_matrix(v, dtype, "kv8_append values")
+        if Tv != T or nk % Hkv or nv % Hkv or not 0 < nk <= wide or not 0 < nv <= wide:
+            raise KernelError(f"kv8_append: keys {tuple(k.shape)} and values {tuple(v.shape)} of {Hkv} heads of at most {Dh}")
+        dk, dv, kp, vp = nk // Hkv, nv // Hkv, k.data_ptr(), v.data_ptr()
     if q is not None:
-        _need(q, x.dtype, "kv8_append q")
-        _need(q_out, x.dtype, "kv8_append q_out")
-        if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] % (Hkv * Dh) or q_out.shape[1] == 0:
-            raise KernelError(f"kv8_append: q_out {tuple(q_out.shape)} for {T} rows over {Hkv} key/value heads of {Dh}")
-        G = q_out.shape[1] // (Hkv * Dh)
-        if q.dim() != 2 or q.shape[0] != T or q.shape[1] % (Hkv * G) or not 0 < q.shape[1] <= q_out.shape[1]:
-            raise KernelError(f"kv8_append: q {tuple(q.shape)} for q_out {tuple(q_out.shape)}")
-        if k is not None and q.shape[1] != Hkv * G * dk:
-            raise KernelError(f"kv8_append: q {tuple(q.shape)} for {Hkv * G} heads of {dk}")
-        dk = q.shape[1] // (Hkv * G)
-    half = 0
+        Tq, nq, ldq = _kv8_matrix(q, dtype, "kv8_append q")
+        To, no, ldo = _kv8_matrix(q_out, dtype, "kv8_append q_out")
+        if no == 0 or no % wide or To != Tq or (k is not None and Tq != T):
+            raise KernelError(f"kv8_append: q {tuple(q.shape)} and q_out {tuple(q_out.shape)} over {Hkv} key/value heads of {Dh}")
+        T, G = Tq, no // wide
+        if nq % (Hkv * G) or not 0 < nq <= no or (k is not None and nq != Hkv * G * dk):
+            raise KernelError(f"kv8_append: q {tuple(q.shape)} for q_out {tuple(q_out.shape)}" + (f" and keys of {dk}" if dk else ""))
+        dk, qp, op = nq // (Hkv * G), q.data_ptr(), q_out.data_ptr()
+    _kv8_rows_ints(positions, token_req, T, "kv8_append")
     if freq is not None:
         _need(freq, torch.float32, "kv8_append freq")
-        half = freq.numel()
+        half, fp = freq.numel(), freq.data_ptr()
         if 2 * half > dk or not freq.is_contiguous():
             raise KernelError(f"kv8_append: {half} frequencies for heads of {dk}")
-    rows = lambda t, what: 0 if t is None else _rows(t, "kv8_append " + what)
-    _call("kv8", "mlxb_kv8_append", _KV8_APPEND_ARGS, code, _p(k), rows(k, "keys"), _p(v), rows(v, "values"), _p(q), rows(q, "q"),
-          _p(q_out), rows(q_out, "q_out"), T, Hkv, G, dk, dv, Dh, _p(freq) if half else None, half, int(interleaved), float(mscale),
-          _p(positions), _p(token_req), _p(block_table), block_table.shape[1], n_pages, page, _p(k8), _p(v8), _p(k_scale), _p(v_scale),
-          _p(status), stream)
+    record, size = _kv8_append_record(
+        kp, vp, qp, op, fp, positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), status.data_ptr(), code, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, Dh, half, interleaved,
+        block_table.shape[1], n_pages, page, mscale)
+    _call("kv8", "mlxb_kv8_append", _KV8_ARGS, record, size, stream)
 
 
-_KV8_READ_ARGS = [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_void_p] * 4 + [c_void_p, c_int] * 2 + [c_int, c_void_p, c_void_p]
+_kv8_read_record = _kv8_record("10Q9q")
 
 
 def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out, v_out, status, stream) -> None:
@@ -913,35 +944,42 @@ def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out,
     the value (``code * scale``) at position ``positions[t]`` of request ``token_req[t]`` (< 0: the row is left as it is; a position without
     a page: zeros, and ``status`` says so)."""
     n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_read")
-    for t, what in ((k_out, "k_out"), (v_out, "v_out")):
-        _need(t, k_out.dtype, "kv8_read " + what)
-        _rows(t, "kv8_read " + what)
-        if t.shape != (k_out.shape[0], Hkv * Dh):
-            raise KernelError(f"kv8_read: {what} {tuple(t.shape)} for {Hkv} heads of {Dh}")
-    n = k_out.shape[0]
+    dtype = k_out.dtype
+    code = dtype_code(dtype)
+    n, nk, ldk = _kv8_matrix(k_out, dtype, "kv8_read k_out")
+    n2, nv, ldv = _kv8_matrix(v_out, dtype, "kv8_read v_out")
+    if n2 != n or nk != Hkv * Dh or nv != nk:
+        raise KernelError(f"kv8_read: k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} for {Hkv} heads of {Dh}")
     _kv8_rows_ints(positions, token_req, n, "kv8_read")
-    _call("kv8", "mlxb_kv8_read", _KV8_READ_ARGS, dtype_code(k_out.dtype), _p(positions), _p(token_req), _p(block_table),
-          block_table.shape[1], n_pages, page, Hkv, Dh, _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(k_out), _rows(k_out, "k_out"),
-          _p(v_out), _rows(v_out, "v_out"), n, _p(status), stream)
+    record, size = _kv8_read_record(
+        positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), status.data_ptr(), code, block_table.shape[1], n_pages, page, Hkv, Dh, ldk,
+        ldv, n)
+    _call("kv8", "mlxb_kv8_read", _KV8_ARGS, record, size, stream)
 
 
-_KV8_ROWS_ARGS = ([c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] + [c_void_p] * 6 + [c_int, c_void_p, c_int, c_int]
-                  + [c_void_p] * 3)
+_kv8_rows_record = _kv8_record("14Q11qd")
 _KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
 _KV8_ITEMS = {torch.float32: 4 * 148, torch.bfloat16: 8 * 148}      # parts of one row's keys that fill the device
 
 
+_KV8_F32_ROWS = ("kv8_rows", "mlxb_kv8_rows")
+
+
+@functools.lru_cache(maxsize=64)
 def kv8_rows_library(dtype, head_dim: int) -> str:
     """The library whose kernel takes single queries of this type (one for each head size in bfloat16)."""
     return "kv8_rows" if dtype == torch.float32 else f"kv8_rows_tc:MLXB_HEAD_DIM={head_dim}"
 
 
+@functools.lru_cache(maxsize=256)
 def _kv8_plan(dtype, n_heads: int, n_kv_heads: int, max_len: int):
     """``(tiles of heads, most parts of a row's keys)``: as many parts as fill the device with one row, and no more than the longest row has."""
     tiles = n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS[dtype])
     return tiles, max(1, min(_KV8_ITEMS[dtype] // tiles, -(-(max_len + KV8_BLOCK) // 128)))
 
 
+@functools.lru_cache(maxsize=256)
 def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
     """``(float32 elements of scratch memory, int32 counters)`` that ``kv8_attention_rows`` needs for ``n_rows`` rows of requests of up to
     ``max_len`` positions."""
@@ -962,40 +1000,39 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
     left out, with a bit in ``status``).  ``sinks``: float32 ``[n_heads]``, one more term of each head's softmax denominator.  Rows of no
     request (``token_req`` < 0) are left as they are.  A row's bits depend on its own request, ``max_len`` and the heads alone."""
     n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_rows")
-    dtype_code(q.dtype)
-    _need(q, None, "kv8_attention_rows q")
-    _need(out, q.dtype, "kv8_attention_rows out")
-    if n_heads <= 0 or n_heads % Hkv or q.dim() != 2 or q.shape != out.shape or q.shape[1] != n_heads * Dh:
+    dtype = q.dtype
+    dtype_code(dtype)
+    T, width, ldq = _kv8_matrix(q, dtype, "kv8_attention_rows q")
+    To, wo, ldo = _kv8_matrix(out, dtype, "kv8_attention_rows out")
+    if n_heads <= 0 or n_heads % Hkv or To != T or width != n_heads * Dh or wo != width:
         raise KernelError(f"kv8_attention_rows: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_heads} heads of {Dh} over {Hkv}")
-    _kv8_rows_ints(positions, token_req, q.shape[0], "kv8_attention_rows")
-    n = q.shape[0]
+    _kv8_rows_ints(positions, token_req, T, "kv8_attention_rows")
+    n, rp = T, 0
     if rows is not None:
         _need(rows, torch.int32, "kv8_attention_rows rows")
-        n = rows.numel()
-    _need(scratch, torch.float32, "kv8_attention_rows scratch")
-    _need(counters, torch.int32, "kv8_attention_rows counters")
+        n, rp = rows.numel(), rows.data_ptr()
     floats, tickets = kv8_rows_scratch(n, n_heads, Hkv, Dh, max_len)
-    if scratch.numel() < floats or counters.numel() < tickets:
+    if (scratch.dtype is not _F32T or counters.dtype is not _I32 or not scratch.is_cuda or not counters.is_cuda or scratch.numel() < floats
+            or counters.numel() < tickets):
+        _need(scratch, torch.float32, "kv8_attention_rows scratch")
+        _need(counters, torch.int32, "kv8_attention_rows counters")
         raise KernelError(f"kv8_attention_rows: scratch of {scratch.numel()} floats and {counters.numel()} counters, {floats} and "
                           f"{tickets} are needed")
-    ldq, ldo = _rows(q, "kv8_attention_rows q"), _rows(out, "kv8_attention_rows out")
-    sk = _sinks(sinks, n_heads, "kv8_attention_rows")
-    most = _kv8_plan(q.dtype, n_heads, Hkv, max_len)[1]
-    lib, name = kv8_rows_library(q.dtype, Dh), "mlxb_kv8_rows" if q.dtype == torch.float32 else "mlxb_kv8_rows_tc"
+    sk = _sinks(sinks, n_heads, "kv8_attention_rows") or 0
+    most = _kv8_plan(dtype, n_heads, Hkv, max_len)[1]
+    lib, name = (_KV8_F32_ROWS if dtype is _F32T else (kv8_rows_library(dtype, Dh), "mlxb_kv8_rows_tc"))
+    qp, op, pp, tp, item = q.data_ptr(), out.data_ptr(), positions.data_ptr(), token_req.data_ptr(), q.element_size()
     for a in range(0, n, KV8_ROWS_MOST):
-        b = min(n, a + KV8_ROWS_MOST)
-        if rows is not None:
-            part = (_p(q), ldq, _p(rows) + 4 * a, _p(positions), _p(token_req), _p(out))
-        else:
-            part = (_p(q) + a * ldq * q.element_size(), ldq, None, _p(positions) + 4 * a, _p(token_req) + 4 * a,
-                    _p(out) + a * ldo * out.element_size())
-        _call(lib, name, _KV8_ROWS_ARGS, *part[:5], _p(block_table), block_table.shape[1], n_pages, page, n_heads,
-              Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale), _p(v_scale), _p(scratch), _p(counters), most,
-              part[5], ldo, b - a, _p(status), sk, stream)
+        # the rows of the list from its a-th on, or rows a and on of the tensors
+        r, t = (rp + 4 * a, 0) if rp else (0, a)
+        record, size = _kv8_rows_record(
+            qp + t * ldq * item, r, pp + 4 * t, tp + 4 * t, block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), sk, scratch.data_ptr(), counters.data_ptr(), op + t * ldo * item, status.data_ptr(), ldq,
+            block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, most, ldo, min(n - a, KV8_ROWS_MOST), scale)
+        _call(lib, name, _KV8_ARGS, record, size, stream)
 
 
-_KV8_PORTION_ARGS = ([c_void_p, c_int, c_void_p, c_int, c_void_p] + [c_int] * 7 + [c_float] + [c_void_p] * 5 + [c_int]
-                     + [c_void_p] * 3)
+_kv8_portion_record = _kv8_record("10Q10qd")
 
 
 def kv8_portions_supported(dtype, head_dim: int, scale: float = 1.0) -> bool:
@@ -1009,19 +1046,20 @@ def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale,
     tile's first token in ``q`` and ``out``, its queries (0: skipped) up to ``PREFILL_TILE``, row of the block table, position of the first
     query); window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are."""
     n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_portions")
-    _need(q, torch.bfloat16, "kv8_attention_portions q")
-    _need(out, torch.bfloat16, "kv8_attention_portions out")
-    _need(tiles, torch.int32, "kv8_attention_portions tiles")
-    if n_heads <= 0 or n_heads % Hkv or q.dim() != 2 or q.shape != out.shape or q.shape[1] != n_heads * Dh:
+    T, width, ldq = _kv8_matrix(q, _BF16T, "kv8_attention_portions q")
+    To, wo, ldo = _kv8_matrix(out, _BF16T, "kv8_attention_portions out")
+    if n_heads <= 0 or n_heads % Hkv or To != T or width != n_heads * Dh or wo != width:
         raise KernelError(f"kv8_attention_portions: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_heads} heads of {Dh} over {Hkv}")
-    if not kv8_portions_supported(q.dtype, Dh, scale):
+    if not kv8_portions_supported(_BF16T, Dh, scale):
         raise KernelError(f"kv8_attention_portions: heads of {Dh}, scale {scale}: heads of up to 128, a scale above 0")
-    if not tiles.is_contiguous() or tiles.numel() < 4 * n_tiles:
+    if tiles.dtype is not _I32 or not tiles.is_cuda or not tiles.is_contiguous() or tiles.numel() < 4 * n_tiles:
+        _need(tiles, torch.int32, "kv8_attention_portions tiles")
         raise KernelError(f"kv8_attention_portions: tiles {tuple(tiles.shape)} for {n_tiles} tiles")
-    _call("kv8_portions", "mlxb_kv8_portions", _KV8_PORTION_ARGS, _p(q), _rows(q, "kv8_attention_portions q"), _p(tiles), int(n_tiles),
-          _p(block_table), block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, int(window), float(scale), _p(k8), _p(v8), _p(k_scale),
-          _p(v_scale), _p(out), _rows(out, "kv8_attention_portions out"), _p(status), _sinks(sinks, n_heads, "kv8_attention_portions"),
-          stream)
+    sk = _sinks(sinks, n_heads, "kv8_attention_portions") or 0
+    record, size = _kv8_portion_record(
+        q.data_ptr(), tiles.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), sk,
+        out.data_ptr(), status.data_ptr(), ldq, n_tiles, block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, ldo, scale)
+    _call("kv8_portions", "mlxb_kv8_portions", _KV8_ARGS, record, size, stream)
 
 
 # --------------------------------------------------------------------------

@@ -1,8 +1,9 @@
 """The bookkeeping of a cache in 8 bits, the options that ask for one, and what is refused: no GPU needed."""
+import importlib
+
 import pytest
 import torch
 
-from mlx_lm_b200 import generate as G
 from mlx_lm_b200 import ops
 from mlx_lm_b200.cache import CacheManager
 from mlx_lm_b200.config import get_architecture
@@ -11,6 +12,9 @@ from mlx_lm_b200.parts.base import PagedKVSpec, StateSpec
 from helpers import CONFIG_A
 from lelatar_cases import CONFIG_P
 from nufetar_cases import CONFIG_A as NUFETAR
+
+
+G = importlib.import_module("mlx_lm_b200.generate")      # (the package has a function of that name)
 
 
 def specs_of(config):
