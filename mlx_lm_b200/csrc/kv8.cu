@@ -18,6 +18,8 @@
 //
 // Rows of a request stand together in order of position (the order in which a step lists them): the row whose predecessor is of
 // another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
+#include <type_traits>
+
 #include "common.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -26,26 +28,21 @@ constexpr int BLK = 16;              // positions that share a scale
 constexpr int MAX_WARPS = 8;
 constexpr uint32_t INF_BITS = 0x7f800000u;
 
-__device__ __forceinline__ void load4(const float* p, bool vec, int n, float (&v)[4]) {
-  if (vec && n >= 4) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int n, float (&v)[4]) {      // the first n of four columns
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
-  }
+  for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
 }
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, int n, float (&v)[4]) {
-  if (vec && n >= 4) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(q.x << 16);
-    v[1] = __uint_as_float(q.x & 0xffff0000u);
-    v[2] = __uint_as_float(q.y << 16);
-    v[3] = __uint_as_float(q.y & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
-  }
+// Four neighbouring elements as they lie in memory, and as numbers.
+template <typename T> struct Four;
+template <> struct Four<float> { float4 v; };
+template <> struct Four<__nv_bfloat16> { uint2 v; };
+__device__ __forceinline__ void unpack4(const Four<float>& r, float (&v)[4]) { v[0] = r.v.x; v[1] = r.v.y; v[2] = r.v.z; v[3] = r.v.w; }
+__device__ __forceinline__ void unpack4(const Four<__nv_bfloat16>& r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.v.x << 16);
+  v[1] = __uint_as_float(r.v.x & 0xffff0000u);
+  v[2] = __uint_as_float(r.v.y << 16);
+  v[3] = __uint_as_float(r.v.y & 0xffff0000u);
 }
 __device__ __forceinline__ void store4(float* p, bool vec, const float (&v)[4]) {
   if (vec) {
@@ -90,7 +87,7 @@ struct AppendArgs {
   int8_t *k8, *v8;
   float *ks, *vs;
   int* status;
-  int chunk, heads_per_cta, vec;  // vec: bit 0 keys, 1 values, 2 queries, 3 q_out: four columns an access
+  int chunk, heads_per_cta;
 };
 
 struct Leader {
@@ -102,42 +99,49 @@ struct Leader {
 // a pair (16 rows of up to 128 columns: 64 a lane) in registers between the search for the largest and the codes, so a number is
 // read once.  LPR lanes stand on a row, 8 columns each in two groups of 4: the groups of a lane are a rotation's two halves where
 // these are whole groups, so that a pair's numbers meet in one lane.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(MAX_WARPS * 32)
+// WIDE: four columns an access, and where something turns, both halves of a pair in one lane; else column by column.
+template <typename T, int LPR, bool WIDE>
+__global__ void __launch_bounds__(MAX_WARPS * 32, WIDE && sizeof(T) == 2 && LPR <= 16 ? 3 : 1)
 append_kernel(const AppendArgs a) {
   constexpr int RP = 32 / LPR;                 // rows at a time
   constexpr int PASSES = BLK / RP;
   extern __shared__ float2 turn[];             // [rows][half]: cosine and sine
   __shared__ Leader lead[BLK];
-  __shared__ int n_lead, last_row;
+  __shared__ int n_lead, last_row, pos_of[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
   const int row0 = blockIdx.x * a.chunk;
-  if (threadIdx.x == 0) { n_lead = 0; last_row = row0; }
-  __syncthreads();
-  if (threadIdx.x < a.chunk) {
-    const int t = row0 + threadIdx.x;
-    const int r = t < a.T ? a.token_req[t] : -1;
-    if (r >= 0) {
-      const int p = a.positions[t];
-      const bool follows = t > 0 && a.token_req[t - 1] == r && a.positions[t - 1] == p - 1;
-      if (!follows || (p & (BLK - 1)) == 0) {
-        int n = 1;
-        while (t + n < a.T && ((p + n) & (BLK - 1)) != 0 && a.token_req[t + n] == r && a.positions[t + n] == p + n) ++n;
-        const int lp = p / a.page;
-        int pg = -1;
-        if (p < 0 || lp >= a.max_pages) {
-          if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
-        } else {
-          pg = a.block_table[(size_t)r * a.max_pages + lp];
-          if (pg >= a.n_pages) {
-            if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_PAGE_RANGE);
-            pg = -1;
-          }
+  if (warp == 0) {
+    // Lane i looks at row row0 + i (a leader of this CTA is among the first `chunk`, its rows among the 15 behind it): where a row
+    // begins something new shows how far the rows before it reach.
+    const int t = row0 + lane;
+    const int r = t < a.T ? a.token_req[t] : -1, p = t < a.T ? a.positions[t] : 0;
+    int rb = __shfl_up_sync(0xffffffffu, r, 1), pb = __shfl_up_sync(0xffffffffu, p, 1);
+    if (lane == 0) { rb = row0 > 0 ? a.token_req[row0 - 1] : -1; pb = row0 > 0 ? a.positions[row0 - 1] : 0; }
+    const bool fresh = r < 0 || rb != r || pb != p - 1 || (p & (BLK - 1)) == 0;
+    const uint32_t starts = __ballot_sync(0xffffffffu, fresh);
+    pos_of[lane] = p;
+    const bool leads = fresh && r >= 0 && lane < a.chunk;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+    int end = row0;
+    if (leads) {
+      const uint32_t behind = lane < 31 ? starts >> (lane + 1) : 0u;
+      const int n = behind ? __ffs(behind) : BLK;           // (a block ends after 16 rows at most: with a chunk of 16 within the 32)
+      const int lp = p / a.page;
+      int pg = -1;
+      if (p < 0 || lp >= a.max_pages) {
+        if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
+      } else {
+        pg = a.block_table[(size_t)r * a.max_pages + lp];
+        if (pg >= a.n_pages) {
+          if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_PAGE_RANGE);
+          pg = -1;
         }
-        lead[atomicAdd(&n_lead, 1)] = Leader{t, n, p, pg};
-        atomicMax(&last_row, t + n);
       }
+      lead[__popc(leaders & ((1u << lane) - 1u))] = Leader{t, n, p, pg};
+      end = t + n;
     }
+    end = __reduce_max_sync(0xffffffffu, end);
+    if (lane == 0) { n_lead = __popc(leaders); last_row = end; }
   }
   __syncthreads();
   const int nl = n_lead;
@@ -146,7 +150,7 @@ append_kernel(const AppendArgs a) {
   for (int e = threadIdx.x; e < (last_row - row0) * a.half; e += blockDim.x) {
     const int i = e / a.half, j = e - i * a.half;
     float sn, cs;
-    sincosf(__fmul_rn((float)a.positions[row0 + i], a.freq[j]), &sn, &cs);
+    sincosf(__fmul_rn((float)pos_of[i], a.freq[j]), &sn, &cs);
     turn[e] = make_float2(__fmul_rn(cs, a.mscale), __fmul_rn(sn, a.mscale));
   }
   pdl_wait();
@@ -157,7 +161,6 @@ append_kernel(const AppendArgs a) {
   const int kinds = (a.k ? 2 : 0) + a.G;
   const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.heads_per_cta, a.Hkv - h0);
   const int sub = lane / LPR, l = lane & (LPR - 1);
-  const bool whole = !a.interleaved && (a.half & 3) == 0;       // a lane holds both halves of its pairs
   const int hg = a.half >> 2;
   for (int u = warp; u < nl * nh * kinds; u += n_warps) {
     const Leader ld = lead[u / (nh * kinds)];
@@ -167,14 +170,13 @@ append_kernel(const AppendArgs a) {
     const bool turned = kind != 1 && a.half > 0;
     const T* src;
     int ld_src, width;
-    bool vec;
-    if (kind == 0) { src = (const T*)a.k + (size_t)h * a.dk; ld_src = a.ldk; width = a.dk; vec = a.vec & 1; }
-    else if (kind == 1) { src = (const T*)a.v + (size_t)h * a.dv; ld_src = a.ldv; width = a.dv; vec = a.vec & 2; }
-    else { src = (const T*)a.q + ((size_t)h * a.G + kind - 2) * a.dk; ld_src = a.ldq; width = a.dk; vec = a.vec & 4; }
+    if (kind == 0) { src = (const T*)a.k + (size_t)h * a.dk; ld_src = a.ldk; width = a.dk; }
+    else if (kind == 1) { src = (const T*)a.v + (size_t)h * a.dv; ld_src = a.ldv; width = a.dv; }
+    else { src = (const T*)a.q + ((size_t)h * a.G + kind - 2) * a.dk; ld_src = a.ldq; width = a.dk; }
     src = after_wait(src);
     // the two groups of four columns of this lane
     int c0, c1;
-    if (turned && whole) {
+    if (WIDE && turned) {
       c0 = l < hg ? 4 * l : 2 * a.half + 8 * (l - hg);
       c1 = l < hg ? c0 + a.half : c0 + 4;
     } else {
@@ -191,67 +193,88 @@ append_kernel(const AppendArgs a) {
       const float2 t = cs[a.interleaved ? i >> 1 : lower ? i : j];
       return lower ? __fsub_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y)) : __fadd_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y));
     };
-    auto fetch = [&](int i, float (&x)[4], float (&y)[4]) {        // row i of the leader's
-      const T* row = src + (size_t)(ld.row + i) * ld_src;
-      const float2* cs = turn + (ld.row + i - row0) * a.half;
-      if (turned && !whole) {
+    const float2* cs0 = turn + (ld.row - row0) * a.half;
+    // All loads of a pair go out before the first number is used: one latency a pair, not one a row.  What is loaded stays as it is; the
+    // numbers are formed from it twice (for the largest, then for the codes), which takes fewer registers than keeping them.
+    Four<T> raw[WIDE ? PASSES : 1][2];
+    if constexpr (WIDE) {
+      const T* row = src + (size_t)(ld.row + sub) * ld_src;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = value(row, cs, c0 + e); y[e] = value(row, cs, c1 + e); }
-        return;
+      for (int s = 0; s < PASSES; ++s) {
+        const bool in = mine && s * RP + sub < ld.n;
+        raw[s][0] = Four<T>{};
+        raw[s][1] = Four<T>{};
+        if (in && c0 < width) raw[s][0] = *reinterpret_cast<const Four<T>*>(row + (size_t)(s * RP) * ld_src + c0);
+        if (in && c1 < width) raw[s][1] = *reinterpret_cast<const Four<T>*>(row + (size_t)(s * RP) * ld_src + c1);
       }
-      load4(row + c0, vec, width - c0, x);
-      load4(row + c1, vec, width - c1, y);
-      if (turned && l < hg) {
+    }
+    auto numbers = [&](int s, float (&x)[4], float (&y)[4]) {      // both groups of row s * RP + sub, turned
+      const float2* cs = cs0 + (s * RP + sub) * a.half;
+      if constexpr (WIDE) {
+        unpack4(raw[s][0], x);
+        unpack4(raw[s][1], y);
+        if (turned && l < hg) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 t = cs[c0 + e];
-          const float p = x[e], q = y[e];
-          x[e] = __fsub_rn(__fmul_rn(p, t.x), __fmul_rn(q, t.y));
-          y[e] = __fadd_rn(__fmul_rn(q, t.x), __fmul_rn(p, t.y));
+          for (int e = 0; e < 4; ++e) {
+            const float2 t = cs[c0 + e];
+            const float p = x[e], q = y[e];
+            x[e] = __fsub_rn(__fmul_rn(p, t.x), __fmul_rn(q, t.y));
+            y[e] = __fadd_rn(__fmul_rn(q, t.x), __fmul_rn(p, t.y));
+          }
+        }
+      } else {
+        const T* row = src + (size_t)(ld.row + s * RP + sub) * ld_src;
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { x[e] = value(row, cs, c0 + e); y[e] = value(row, cs, c1 + e); }
+        } else {
+          load4(row + c0, width - c0, x);
+          load4(row + c1, width - c1, y);
         }
       }
     };
     if (kind >= 2) {
-      T* dst = (T*)a.q_out + ((size_t)h * a.G + kind - 2) * a.dim;
-#pragma unroll 4
-      for (int i = sub; i < ld.n; i += RP) {
+      T* dst = (T*)a.q_out + ((size_t)h * a.G + kind - 2) * a.dim + (size_t)(ld.row + sub) * a.ldo;
+#pragma unroll
+      for (int s = 0; s < PASSES; ++s) {
+        if (!mine || s * RP + sub >= ld.n) continue;
         float x[4], y[4];
-        if (mine) {
-          fetch(i, x, y);
-          store4(dst + (size_t)(ld.row + i) * a.ldo + c0, a.vec & 8, x);
-          store4(dst + (size_t)(ld.row + i) * a.ldo + c1, a.vec & 8, y);
-        }
+        numbers(s, x, y);
+        store4(dst + (size_t)(s * RP) * a.ldo + c0, WIDE, x);
+        store4(dst + (size_t)(s * RP) * a.ldo + c1, WIDE, y);
       }
       continue;
     }
     if (ld.page_id < 0) continue;
-    float x[PASSES][4], y[PASSES][4];
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < PASSES; ++s) {
       if (s * RP >= ld.n) break;
-      const int i = s * RP + sub;
+      if (mine && s * RP + sub < ld.n) {
+        float x[4], y[4];
+        numbers(s, x, y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[s][e] = y[s][e] = 0.f;
-      if (mine && i < ld.n) fetch(i, x[s], y[s]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        top = max(top, max(__float_as_uint(x[s][e]) & 0x7fffffffu, __float_as_uint(y[s][e]) & 0x7fffffffu));
+        for (int e = 0; e < 4; ++e)
+          top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
+      }
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (top >= INF_BITS) {                     // something is not finite: the largest of the others, and NaN becomes 0
+    const bool odd = top >= INF_BITS;          // something is not finite: the largest of the others, and NaN becomes 0
+    if (odd) {
       if (lane == 0) atomicOr(a.status, MLXB_ST_NOT_FINITE);
       top = 0;
 #pragma unroll
       for (int s = 0; s < PASSES; ++s) {
         if (s * RP >= ld.n) break;
+        if (mine && s * RP + sub < ld.n) {
+          float x[4], y[4];
+          numbers(s, x, y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t bx = __float_as_uint(x[s][e]) & 0x7fffffffu, by = __float_as_uint(y[s][e]) & 0x7fffffffu;
-          if (bx < INF_BITS) top = max(top, bx);
-          if (by < INF_BITS) top = max(top, by);
-          if (bx > INF_BITS) x[s][e] = 0.f;
-          if (by > INF_BITS) y[s][e] = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bx = __float_as_uint(x[e]) & 0x7fffffffu, by = __float_as_uint(y[e]) & 0x7fffffffu;
+            if (bx < INF_BITS) top = max(top, bx);
+            if (by < INF_BITS) top = max(top, by);
+          }
         }
       }
       top = __reduce_max_sync(0xffffffffu, top);
@@ -289,8 +312,14 @@ append_kernel(const AppendArgs a) {
       const int i = s * RP + sub;
       if (mine && i < ld.n) {
         int8_t* dst = codes + (off + i) * a.dim;
-        *reinterpret_cast<uint32_t*>(dst + c0) = scale > 0.f ? codes4(x[s], inv) : 0u;
-        *reinterpret_cast<uint32_t*>(dst + c1) = scale > 0.f ? codes4(y[s], inv) : 0u;
+        float x[4], y[4];
+        numbers(s, x, y);
+        if (odd) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { x[e] = x[e] != x[e] ? 0.f : x[e]; y[e] = y[e] != y[e] ? 0.f : y[e]; }
+        }
+        *reinterpret_cast<uint32_t*>(dst + c0) = scale > 0.f ? codes4(x, inv) : 0u;
+        *reinterpret_cast<uint32_t*>(dst + c1) = scale > 0.f ? codes4(y, inv) : 0u;
       }
     }
   }
@@ -333,12 +362,17 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   const size_t item = dtype == MLXB_F32 ? 4 : 2;
   auto fits = [&](const void* p, int ld, int d) { return (((uintptr_t)p) % (4 * item)) == 0 && ld % 4 == 0 && d % 4 == 0; };
   AppendArgs a{k, v, q, q_out, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, freq, half, (int)x.interleaved, (float)x.mscale,
-               x.positions, x.token_req, x.block_table, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status, 1, 1, 0};
-  a.vec = (fits(k, ldk, dk) ? 1 : 0) | (fits(v, ldv, dv) ? 2 : 0) | (fits(q, ldq, dk) ? 4 : 0) | (fits(q_out, ldo, dim) ? 8 : 0);
+               x.positions, x.token_req, x.block_table, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status, 1, 1};
+  // four columns an access: whole groups of four, aligned, and pairs that are whole groups apart
+  const bool wide = (!k || (fits(k, ldk, dk) && fits(v, ldv, dv))) && (!G || (fits(q, ldq, dk) && fits(q_out, ldo, dim))) &&
+                    (half == 0 || (!x.interleaved && half % 4 == 0));
   // few rows: a CTA a row, so that single tokens of different requests spread over the device; many: the rows of a block together
   a.chunk = T <= 64 ? 1 : BLK;
   const int kinds = (k ? 2 : 0) + G;
+  // heads of a CTA: as many as keep its warps busy, and more (they share the sines) while there are still four CTAs for every SM
   a.heads_per_cta = kinds >= MAX_WARPS ? 1 : MAX_WARPS / kinds;
+  const long long chunks = (T + a.chunk - 1) / a.chunk;
+  while (2 * a.heads_per_cta <= Hkv && chunks * ((Hkv + 2 * a.heads_per_cta - 1) / (2 * a.heads_per_cta)) >= 4ll * mlxb_sm_count()) a.heads_per_cta *= 2;
   if (a.heads_per_cta > Hkv) a.heads_per_cta = Hkv;
   const int warps = kinds * a.heads_per_cta < MAX_WARPS ? kinds * a.heads_per_cta : MAX_WARPS;
   const dim3 grid((T + a.chunk - 1) / a.chunk, (Hkv + a.heads_per_cta - 1) / a.heads_per_cta);
@@ -346,78 +380,83 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   const size_t smem = (size_t)(a.chunk + BLK - 1) * half * sizeof(float2);      // at most 31 rows of 128 pairs: 31 KB
   auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(32 * warps), smem, stream, a); };
   const int lanes = dim / 8;
+  auto sized = [&](auto type, auto w) {
+    using T = decltype(type);
+    constexpr bool W = decltype(w)::value;
+    if (lanes <= 4) go(append_kernel<T, 4, W>);
+    else if (lanes <= 8) go(append_kernel<T, 8, W>);
+    else if (lanes <= 16) go(append_kernel<T, 16, W>);
+    else go(append_kernel<T, 32, W>);
+  };
   if (dtype == MLXB_F32) {
-    if (lanes <= 4) go(append_kernel<float, 4>);
-    else if (lanes <= 8) go(append_kernel<float, 8>);
-    else if (lanes <= 16) go(append_kernel<float, 16>);
-    else go(append_kernel<float, 32>);
+    if (wide) sized(float{}, std::true_type{}); else sized(float{}, std::false_type{});
   } else {
-    if (lanes <= 4) go(append_kernel<__nv_bfloat16, 4>);
-    else if (lanes <= 8) go(append_kernel<__nv_bfloat16, 8>);
-    else if (lanes <= 16) go(append_kernel<__nv_bfloat16, 16>);
-    else go(append_kernel<__nv_bfloat16, 32>);
+    if (wide) sized(__nv_bfloat16{}, std::true_type{}); else sized(__nv_bfloat16{}, std::false_type{});
   }
   return mlxb_check_launch("kv8_append");
 }
 
 // ---- what the pages hold
 
-// A thread takes 16 codes of a row (keys, then values): 16 bytes in, 32 or 64 out.
+// A warp takes a row (its page looked up once), a lane 16 codes at a time, keys and values: 16 bytes in, 32 or 64 out.
 template <typename T>
 __global__ void __launch_bounds__(256)
 read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ block_table, int max_pages,
             int n_pages, int page, int Hkv, int dim, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, T* k_out,
             int ldk, T* v_out, int ldv, int n_rows, int vec, int* status) {
+  const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int r = t < n_rows ? token_req[t] : -1;
+  int p = 0, pg = -1;
+  if (r >= 0) {
+    p = positions[t];
+    const int lp = p / page;
+    if (p >= 0 && lp < max_pages) pg = block_table[(size_t)r * max_pages + lp];
+    if (pg < 0 || pg >= n_pages) {
+      if (lane == 0) atomicOr(status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
+      pg = -1;
+    }
+  }
   pdl_wait();
   pdl_trigger();
-  const int per_row = 2 * Hkv * dim / 16;
-  const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int t = (int)(e / per_row);
-  if (t >= n_rows) return;
-  const int w = (int)(e - (long long)t * per_row);
-  const int r = token_req[t];
   if (r < 0) return;
-  const int p = positions[t], lp = p / page;
-  int pg = -1;
-  if (p >= 0 && lp < max_pages) pg = block_table[(size_t)r * max_pages + lp];
-  if (pg < 0 || pg >= n_pages) {
-    if (w == 0) atomicOr(status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
-    pg = -1;
-  }
-  const int col = w * 16, width = Hkv * dim;
-  const bool is_v = col >= width;
-  const int c = is_v ? col - width : col, h = c / dim, d = c - h * dim;
-  float o[16];
-  if (pg >= 0) {
-    const size_t at = ((size_t)pg * Hkv + h) * page + (p & (page - 1));
-    const int8_t* src = after_wait(is_v ? v8 : k8) + at * dim + d;
-    const float s = after_wait(is_v ? vs : ks)[((size_t)pg * Hkv + h) * (page / BLK) + (p & (page - 1)) / BLK];
-    const uint4 c4 = *reinterpret_cast<const uint4*>(src);
-    const uint32_t cw[4] = {c4.x, c4.y, c4.z, c4.w};
+  k8 = after_wait(k8); v8 = after_wait(v8);
+  ks = after_wait(ks); vs = after_wait(vs);
+  const int per_head = dim / 16, per = page / BLK, in = p & (page - 1);
+#pragma unroll 2
+  for (int w = lane; w < 2 * Hkv * per_head; w += 32) {
+    const bool is_v = w >= Hkv * per_head;
+    const int e = is_v ? w - Hkv * per_head : w, h = e / per_head, d = (e - h * per_head) * 16;
+    float o[16];
+    if (pg >= 0) {
+      const size_t head = (size_t)pg * Hkv + h;
+      const uint4 c4 = *reinterpret_cast<const uint4*>((is_v ? v8 : k8) + (head * page + in) * dim + d);
+      const float s = (is_v ? vs : ks)[head * per + in / BLK];
+      const uint32_t cw[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const char4 b = *reinterpret_cast<const char4*>(&cw[j]);
-      o[4 * j] = (float)b.x * s; o[4 * j + 1] = (float)b.y * s; o[4 * j + 2] = (float)b.z * s; o[4 * j + 3] = (float)b.w * s;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = 0.f;
-  }
-  T* dst = is_v ? v_out + (size_t)t * ldv + c : k_out + (size_t)t * ldk + c;
-  if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      float lo[8], hi[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) { lo[j] = o[j]; hi[j] = o[8 + j]; }
-      reinterpret_cast<uint4*>(dst)[0] = pack8(lo);
-      reinterpret_cast<uint4*>(dst)[1] = pack8(hi);
+      for (int j = 0; j < 4; ++j) {
+        const char4 b = *reinterpret_cast<const char4*>(&cw[j]);
+        o[4 * j] = (float)b.x * s; o[4 * j + 1] = (float)b.y * s; o[4 * j + 2] = (float)b.z * s; o[4 * j + 3] = (float)b.w * s;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+      for (int j = 0; j < 16; ++j) o[j] = 0.f;
     }
-  } else {
+    T* dst = is_v ? v_out + (size_t)t * ldv + e * 16 : k_out + (size_t)t * ldk + e * 16;
+    if (vec) {
+      if constexpr (sizeof(T) == 2) {
+        float lo[8], hi[8];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) dst[j] = from_f<T>(o[j]);
+        for (int j = 0; j < 8; ++j) { lo[j] = o[j]; hi[j] = o[8 + j]; }
+        reinterpret_cast<uint4*>(dst)[0] = pack8(lo);
+        reinterpret_cast<uint4*>(dst)[1] = pack8(hi);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dst[j] = from_f<T>(o[j]);
+    }
   }
 }
 
@@ -449,9 +488,7 @@ MLXB_EXPORT int mlxb_kv8_read(const ReadRecord* rec, long long bytes, cudaStream
   if (((uintptr_t)k8 | (uintptr_t)v8) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: pools must be 16-byte aligned");
   const size_t item = dtype == MLXB_F32 ? 4 : 2;
   const int vec = !(((uintptr_t)k_out | (uintptr_t)v_out) & 15) && (ldk * item) % 16 == 0 && (ldv * item) % 16 == 0;
-  const long long n = (long long)n_rows * (2 * Hkv * dim / 16);
-  if ((n + 255) / 256 > 0x7fffffffll) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: %d rows", n_rows);
-  const dim3 grid((unsigned)((n + 255) / 256));
+  const dim3 grid((unsigned)((n_rows + 7) / 8));
   if (dtype == MLXB_F32)
     launch_pdl(read_kernel<float>, grid, dim3(256), 0, stream, positions, token_req, block_table, max_pages, n_pages, page, Hkv, dim, k8,
                v8, ks, vs, (float*)k_out, ldk, (float*)v_out, ldv, n_rows, vec, status);

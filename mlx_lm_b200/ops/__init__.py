@@ -923,6 +923,8 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
         if nq % (Hkv * G) or not 0 < nq <= no or (k is not None and nq != Hkv * G * dk):
             raise KernelError(f"kv8_append: q {tuple(q.shape)} for q_out {tuple(q_out.shape)}" + (f" and keys of {dk}" if dk else ""))
         dk, qp, op = nq // (Hkv * G), q.data_ptr(), q_out.data_ptr()
+        if qp == op:
+            raise KernelError("kv8_append: q cannot turn in place")
     _kv8_rows_ints(positions, token_req, T, "kv8_append")
     if freq is not None:
         _need(freq, torch.float32, "kv8_append freq")

@@ -456,7 +456,7 @@ def test_refusals(ops):
            dict(k8=k8.float()), dict(v8=v8[:, :1]), dict(k_scale=ks.half()), dict(k_scale=ks[:1]), dict(v_scale=vs.transpose(0, 1)),
            dict(block_table=table.long()), dict(block_table=table[0]), dict(positions=pos[:2]), dict(token_req=req.cpu()),
            dict(freq=torch.ones(33, device="cuda")), dict(freq=torch.ones(4, device="cuda").double()), dict(q=x), dict(q=x, q_out=x[:, :64]),
-           dict(q=x[:, :120], q_out=x.clone()), dict(k=torch.zeros(4, 144, device="cuda")),
+           dict(q=x[:, :120], q_out=x.clone()), dict(q=x, q_out=x), dict(k=torch.zeros(4, 144, device="cuda")),
            dict(k8=k8.view(-1, 2, 8, 64), v8=v8.view(-1, 2, 8, 64))]
     for change in bad:
         with pytest.raises(ops.KernelError):
