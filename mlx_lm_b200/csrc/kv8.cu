@@ -61,16 +61,19 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, const float (
     for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(v[i]);
   }
 }
-// rint(x * inv) within -127 .. 127 in the low byte.  1.5 * 2^23 + n has n's two's complement in its low bits, and adding it rounds to
-// the nearest whole number, ties to even.
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-  const float y = fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f);
-  return __float_as_uint(__fadd_rn(y, 12582912.f));
-}
+// rint(x * inv) in the low byte, for |x * inv| < 127.5.  1.5 * 2^23 + n has n's two's complement in its low bits, and adding it rounds
+// to the nearest whole number, ties to even.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float inv) {
   const uint32_t lo = __byte_perm(code_of(x[0], inv), code_of(x[1], inv), 0x0040);
   const uint32_t hi = __byte_perm(code_of(x[2], inv), code_of(x[3], inv), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
+}
+// The larger magnitudes of two pairs (signs are of no meaning); NaN if one is.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
 }
 
 struct AppendArgs {
@@ -105,7 +108,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, WIDE && sizeof(T) == 2 && LPR 
 append_kernel(const AppendArgs a) {
   constexpr int RP = 32 / LPR;                 // rows at a time
   constexpr int PASSES = BLK / RP;
-  extern __shared__ float2 turn[];             // [rows][half]: cosine and sine
+  extern __shared__ __align__(16) float2 turn[];      // [rows][half]: cosine and sine
   __shared__ Leader lead[BLK];
   __shared__ int n_lead, last_row, pos_of[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
@@ -147,11 +150,17 @@ append_kernel(const AppendArgs a) {
   const int nl = n_lead;
   if (nl == 0) return;
   // (rows between two leaders that are of no request get an angle nobody uses)
-  for (int e = threadIdx.x; e < (last_row - row0) * a.half; e += blockDim.x) {
-    const int i = e / a.half, j = e - i * a.half;
-    float sn, cs;
-    sincosf(__fmul_rn((float)pos_of[i], a.freq[j]), &sn, &cs);
-    turn[e] = make_float2(__fmul_rn(cs, a.mscale), __fmul_rn(sn, a.mscale));
+  if (a.half > 0) {
+    const int di = blockDim.x / a.half, dj = blockDim.x - di * a.half, n = (last_row - row0) * a.half;
+    int i = threadIdx.x / a.half, j = threadIdx.x - i * a.half;
+    for (int e = threadIdx.x; e < n; e += blockDim.x) {
+      float sn, cs;
+      sincosf(__fmul_rn((float)pos_of[i], a.freq[j]), &sn, &cs);
+      turn[e] = make_float2(__fmul_rn(cs, a.mscale), __fmul_rn(sn, a.mscale));
+      i += di;
+      j += dj;
+      if (j >= a.half) { j -= a.half; ++i; }
+    }
   }
   pdl_wait();
   pdl_trigger();
@@ -162,10 +171,16 @@ append_kernel(const AppendArgs a) {
   const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.heads_per_cta, a.Hkv - h0);
   const int sub = lane / LPR, l = lane & (LPR - 1);
   const int hg = a.half >> 2;
-  for (int u = warp; u < nl * nh * kinds; u += n_warps) {
-    const Leader ld = lead[u / (nh * kinds)];
-    const int w = u % (nh * kinds), h = h0 + w / kinds;
-    int kind = w % kinds;                      // 0 keys, 1 values, 2 + i query head i of the group
+  // the pairs (leader, w), w = head * kinds + kind, one after the other without a division a pair
+  const int nk = nh * kinds;
+  const uint32_t by_kinds = (65536u + kinds - 1) / kinds;       // w / kinds = w * by_kinds >> 16 for w * kinds < 65536
+  int li = 0, w = warp;
+  for (;; w += n_warps) {
+    while (w >= nk && li < nl) { w -= nk; ++li; }
+    if (li >= nl) break;
+    const Leader ld = lead[li];
+    const int hw = (int)(w * by_kinds >> 16), h = h0 + hw;
+    int kind = w - hw * kinds;                 // 0 keys, 1 values, 2 + i query head i of the group
     if (!a.k) kind += 2;
     const bool turned = kind != 1 && a.half > 0;
     const T* src;
@@ -198,14 +213,16 @@ append_kernel(const AppendArgs a) {
     // numbers are formed from it twice (for the largest, then for the codes), which takes fewer registers than keeping them.
     Four<T> raw[WIDE ? PASSES : 1][2];
     if constexpr (WIDE) {
-      const T* row = src + (size_t)(ld.row + sub) * ld_src;
+      const T* row = src + (size_t)(ld.row + sub) * ld_src + c0;
+      const size_t step = (size_t)RP * ld_src;
+      const int apart = c1 - c0, left = ld.n - sub;
+      const bool lower = mine && c0 < width, upper = mine && c1 < width;
 #pragma unroll
-      for (int s = 0; s < PASSES; ++s) {
-        const bool in = mine && s * RP + sub < ld.n;
+      for (int s = 0; s < PASSES; ++s, row += step) {
         raw[s][0] = Four<T>{};
         raw[s][1] = Four<T>{};
-        if (in && c0 < width) raw[s][0] = *reinterpret_cast<const Four<T>*>(row + (size_t)(s * RP) * ld_src + c0);
-        if (in && c1 < width) raw[s][1] = *reinterpret_cast<const Four<T>*>(row + (size_t)(s * RP) * ld_src + c1);
+        if (lower && s * RP < left) raw[s][0] = *reinterpret_cast<const Four<T>*>(row);
+        if (upper && s * RP < left) raw[s][1] = *reinterpret_cast<const Four<T>*>(row + apart);
       }
     }
     auto numbers = [&](int s, float (&x)[4], float (&y)[4]) {      // both groups of row s * RP + sub, turned
@@ -214,12 +231,13 @@ append_kernel(const AppendArgs a) {
         unpack4(raw[s][0], x);
         unpack4(raw[s][1], y);
         if (turned && l < hg) {
+          const float4 t01 = *reinterpret_cast<const float4*>(cs + c0), t23 = *reinterpret_cast<const float4*>(cs + c0 + 2);
+          const float2 t[4] = {make_float2(t01.x, t01.y), make_float2(t01.z, t01.w), make_float2(t23.x, t23.y), make_float2(t23.z, t23.w)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 t = cs[c0 + e];
             const float p = x[e], q = y[e];
-            x[e] = __fsub_rn(__fmul_rn(p, t.x), __fmul_rn(q, t.y));
-            y[e] = __fadd_rn(__fmul_rn(q, t.x), __fmul_rn(p, t.y));
+            x[e] = __fsub_rn(__fmul_rn(p, t[e].x), __fmul_rn(q, t[e].y));
+            y[e] = __fadd_rn(__fmul_rn(q, t[e].x), __fmul_rn(p, t[e].y));
           }
         }
       } else {
@@ -234,29 +252,47 @@ append_kernel(const AppendArgs a) {
       }
     };
     if (kind >= 2) {
-      T* dst = (T*)a.q_out + ((size_t)h * a.G + kind - 2) * a.dim + (size_t)(ld.row + sub) * a.ldo;
+      T* dst = (T*)a.q_out + ((size_t)h * a.G + kind - 2) * a.dim + (size_t)(ld.row + sub) * a.ldo + c0;
+      const size_t step = (size_t)RP * a.ldo;
+      const int apart = c1 - c0, left = mine ? ld.n - sub : 0;
 #pragma unroll
-      for (int s = 0; s < PASSES; ++s) {
-        if (!mine || s * RP + sub >= ld.n) continue;
+      for (int s = 0; s < PASSES; ++s, dst += step) {
+        if (s * RP >= left) break;
         float x[4], y[4];
         numbers(s, x, y);
-        store4(dst + (size_t)(s * RP) * a.ldo + c0, WIDE, x);
-        store4(dst + (size_t)(s * RP) * a.ldo + c1, WIDE, y);
+        store4(dst, WIDE, x);
+        store4(dst + apart, WIDE, y);
       }
       continue;
     }
     if (ld.page_id < 0) continue;
+    // the largest magnitude, as bits; NaN and infinities come out on top
     uint32_t top = 0;
+    if constexpr (WIDE && sizeof(T) == 2) {
+      // as the numbers came, two at a time: all there is to it for values, and whether a key is not finite
+      uint32_t pairs = 0;
 #pragma unroll
-    for (int s = 0; s < PASSES; ++s) {
-      if (s * RP >= ld.n) break;
-      if (mine && s * RP + sub < ld.n) {
-        float x[4], y[4];
-        numbers(s, x, y);
+      for (int s = 0; s < PASSES; ++s)
+        pairs = max_abs2(max_abs2(max_abs2(max_abs2(pairs, raw[s][0].v.x), raw[s][0].v.y), raw[s][1].v.x), raw[s][1].v.y);
+      top = max(pairs << 16 & 0x7fffffffu, pairs & 0x7fff0000u);
+    }
+    if (!(WIDE && sizeof(T) == 2) || (turned && top < INF_BITS)) {
+      top = 0;
+      float large = 0.f;                       // (no NaN comes from finite numbers, and fmaxf finds infinities)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
+      for (int s = 0; s < PASSES; ++s) {
+        if (s * RP >= ld.n) break;
+        if (mine && s * RP + sub < ld.n) {
+          float x[4], y[4];
+          numbers(s, x, y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (WIDE && sizeof(T) == 2) large = fmaxf(large, fmaxf(fabsf(x[e]), fabsf(y[e])));
+            else top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
+          }
+        }
       }
+      top = max(top, __float_as_uint(large));
     }
     top = __reduce_max_sync(0xffffffffu, top);
     const bool odd = top >= INF_BITS;          // something is not finite: the largest of the others, and NaN becomes 0
@@ -316,7 +352,11 @@ append_kernel(const AppendArgs a) {
         numbers(s, x, y);
         if (odd) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { x[e] = x[e] != x[e] ? 0.f : x[e]; y[e] = y[e] != y[e] ? 0.f : y[e]; }
+          for (int e = 0; e < 4; ++e) {
+            const float most = 127.f * scale;          // (of an infinity the largest code)
+            x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -most), most);
+            y[e] = y[e] != y[e] ? 0.f : fminf(fmaxf(y[e], -most), most);
+          }
         }
         *reinterpret_cast<uint32_t*>(dst + c0) = scale > 0.f ? codes4(x, inv) : 0u;
         *reinterpret_cast<uint32_t*>(dst + c1) = scale > 0.f ? codes4(y, inv) : 0u;
@@ -352,7 +392,7 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   int8_t *k8 = x.k8, *v8 = x.v8;
   if (dtype != MLXB_F32 && dtype != MLXB_BF16) return mlxb_fail(MLXB_BAD_DTYPE, "kv8_append: dtype code %d", dtype);
   if (T <= 0) return 0;
-  if (Hkv <= 0 || G < 0 || dim % 16 || dim < 16 || dim > 256 || dk <= 0 || dk > dim || dv <= 0 || dv > dim)
+  if (Hkv <= 0 || G < 0 || G > 250 || dim % 16 || dim < 16 || dim > 256 || dk <= 0 || dk > dim || dv <= 0 || dv > dim)
     return mlxb_fail(MLXB_BAD_ARG, "kv8_append: %d heads of %d and %d columns in rows of %d (a multiple of 16 up to 256)", Hkv, dk, dv, dim);
   if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: page size %d (a power of two of at least %d)", page, BLK);
   if (half < 0 || 2 * half > dk || (half && !freq)) return mlxb_fail(MLXB_BAD_ARG, "kv8_append: %d pairs of %d columns", half, dk);
@@ -372,7 +412,7 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   // heads of a CTA: as many as keep its warps busy, and more (they share the sines) while there are still four CTAs for every SM
   a.heads_per_cta = kinds >= MAX_WARPS ? 1 : MAX_WARPS / kinds;
   const long long chunks = (T + a.chunk - 1) / a.chunk;
-  while (2 * a.heads_per_cta <= Hkv && chunks * ((Hkv + 2 * a.heads_per_cta - 1) / (2 * a.heads_per_cta)) >= 4ll * mlxb_sm_count()) a.heads_per_cta *= 2;
+  while (2 * a.heads_per_cta <= Hkv && 2 * a.heads_per_cta * kinds * kinds < 65536 && chunks * ((Hkv + 2 * a.heads_per_cta - 1) / (2 * a.heads_per_cta)) >= 4ll * mlxb_sm_count()) a.heads_per_cta *= 2;
   if (a.heads_per_cta > Hkv) a.heads_per_cta = Hkv;
   const int warps = kinds * a.heads_per_cta < MAX_WARPS ? kinds * a.heads_per_cta : MAX_WARPS;
   const dim3 grid((T + a.chunk - 1) / a.chunk, (Hkv + a.heads_per_cta - 1) / a.heads_per_cta);
@@ -422,21 +462,20 @@ read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req
   k8 = after_wait(k8); v8 = after_wait(v8);
   ks = after_wait(ks); vs = after_wait(vs);
   const int per_head = dim / 16, per = page / BLK, in = p & (page - 1);
-#pragma unroll 2
+  const uint32_t by_head = (65536u + per_head - 1) / per_head;       // e / per_head = e * by_head >> 16 for e * per_head < 65536
+#pragma unroll 4
   for (int w = lane; w < 2 * Hkv * per_head; w += 32) {
     const bool is_v = w >= Hkv * per_head;
-    const int e = is_v ? w - Hkv * per_head : w, h = e / per_head, d = (e - h * per_head) * 16;
+    const int e = is_v ? w - Hkv * per_head : w, h = (int)(e * by_head >> 16), d = (e - h * per_head) * 16;
     float o[16];
     if (pg >= 0) {
       const size_t head = (size_t)pg * Hkv + h;
       const uint4 c4 = *reinterpret_cast<const uint4*>((is_v ? v8 : k8) + (head * page + in) * dim + d);
       const float s = (is_v ? vs : ks)[head * per + in / BLK];
-      const uint32_t cw[4] = {c4.x, c4.y, c4.z, c4.w};
+      // code + 128 in the low byte of 2^23, less 2^23 + 128
+      const uint32_t cw[4] = {c4.x ^ 0x80808080u, c4.y ^ 0x80808080u, c4.z ^ 0x80808080u, c4.w ^ 0x80808080u};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const char4 b = *reinterpret_cast<const char4*>(&cw[j]);
-        o[4 * j] = (float)b.x * s; o[4 * j + 1] = (float)b.y * s; o[4 * j + 2] = (float)b.z * s; o[4 * j + 3] = (float)b.w * s;
-      }
+      for (int j = 0; j < 16; ++j) o[j] = (__uint_as_float(__byte_perm(cw[j >> 2], 0x4b000000u, 0x7540 + (j & 3))) - 8388736.f) * s;
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[j] = 0.f;
@@ -483,7 +522,8 @@ MLXB_EXPORT int mlxb_kv8_read(const ReadRecord* rec, long long bytes, cudaStream
   int* status = x.status;
   if (dtype != MLXB_F32 && dtype != MLXB_BF16) return mlxb_fail(MLXB_BAD_DTYPE, "kv8_read: dtype code %d", dtype);
   if (n_rows <= 0) return 0;
-  if (Hkv <= 0 || dim % 16 || dim < 16 || dim > 256) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: %d heads of %d (a multiple of 16 up to 256)", Hkv, dim);
+  if (Hkv <= 0 || Hkv > 255 || dim % 16 || dim < 16 || dim > 256)
+    return mlxb_fail(MLXB_BAD_ARG, "kv8_read: %d heads of %d (255 at most, a multiple of 16 up to 256)", Hkv, dim);
   if (page < BLK || (page & (page - 1))) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: page size %d (a power of two of at least %d)", page, BLK);
   if (((uintptr_t)k8 | (uintptr_t)v8) & 15) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: pools must be 16-byte aligned");
   const size_t item = dtype == MLXB_F32 ? 4 : 2;
