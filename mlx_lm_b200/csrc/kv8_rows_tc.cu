@@ -4,20 +4,20 @@
 // A warp works by itself, an item after the other: asynchronous copies bring its tiles into a ring of its own in shared memory, several
 // tiles ahead, and no block-wide wait stands between the items.  Rows of several chunks leave sums that a second kernel adds up.
 // A warp takes 16 keys at a time (a block with one scale; never more than one page) for up to eight query heads that read the same
-// key/value head, as m16n8k16 products:
-//   S^T [16 keys x 8 heads] = K [16 x dim] Q^T      the codes are A, row by row
-//   O^T [dim x 8 heads]    += V^T [dim x 16] P^T    the codes are A again, transposed
+// key/value head:
+//   S^T [16 keys x 8 heads] = K [16 x dim] Q^T      m16n8k32 in whole numbers: K's codes are A as they lie in memory
+//   O^T [dim x 8 heads]    += V^T [dim x 16] P^T    m16n8k16 in fp16: V's codes are A, transposed
 // Which columns of K a thread's registers stand for is free as long as Q's do too, and which rows of O^T likewise, so a thread loads
-// 16 neighbouring bytes of a key where it needs four times four of them.  P leaves the first product as [keys x heads] and enters the second as [heads x keys]: movmatrix turns it in two instructions.
-// A code enters a product as fp16 bits 00uu, u = code + 128: the subnormal number u * 2^-24, exact, for one bit operation on two codes
-// (two for the odd bytes).  The 128 comes off where a product starts: K Q^T begins at -128 sum(q), known once a row, and V^T P^T at
-// -128 sum(p), which a product with ones gives and which is the softmax's sum below as well (of the weights as they were rounded).
-// A query is scaled by a power of two so that its largest number lies in [2^14, 2^15): its 8 bits stay exact in fp16 down to 2^-28 of
-// the largest.  The scale of a key block multiplies the scores, that of a value block the block's O, both in float32; P is rounded to
-// fp16 (11 bits, 2^-12 of a weight).  The maximum that the exponentials are relative to follows a score only once that is more than 8
-// (a factor 256) beyond it: most tiles need neither shuffles nor another scaling of O.
-#include <cuda_fp16.h>
-
+// 16 neighbouring bytes of a key where it needs four times four of them.  P leaves the first product as [keys x heads] and enters the
+// second as [heads x keys]: movmatrix turns it in two instructions.
+// A query enters as whole numbers of 16 bits, its largest at 32512, in two products (high and low byte): a number is off by 2^-16 of the
+// largest at most, the scores by 3e-5 of their spread for normal numbers, a tenth of what rounding P costs; the sums are exact.  (Codes as
+// fp16 cost three operations for every four of them: 404 instructions a tile of 128 columns, so 350.)
+// A code of V enters as fp16 bits 00uu, u = code + 128: the subnormal number u * 2^-24, exact, for one bit operation on two codes (two for
+// the odd bytes).  The 128 comes off where the product starts: at -128 sum(p), which a product with ones gives and which is the softmax's
+// sum below as well (of the weights as they were rounded).  The scale of a key block multiplies the scores, that of a value block the
+// block's O, both in float32; P is rounded to fp16 (11 bits, 2^-12 of a weight).  The maximum that the exponentials are relative to
+// follows a score only once that is more than 8 (a factor 256) beyond it: most tiles need neither shuffles nor another scaling of O.
 #include "kv8_rows.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -33,7 +33,8 @@ constexpr int TILE = 2 * 16 * DH;                       // bytes of a tile: 16 k
 constexpr int STAGES = 12288 / TILE < 2 ? 2 : 12288 / TILE;      // of a warp's ring
 constexpr int CTAS = DH > 128 ? 3 : 4;                  // of an SM
 constexpr size_t RING = (size_t)WARPS * STAGES * TILE;
-constexpr int KT = DH / 16;                             // k steps of S, m tiles of O
+constexpr int KT = DH / 16;                             // words of a key a thread holds, m tiles of O
+constexpr int KS = (KT + 1) / 2;                        // k steps of S
 constexpr int KW = DH % 64 == 0 ? 16 : DH % 32 == 0 ? 8 : 4;      // bytes of a key a thread loads at once
 constexpr int NK = DH / 4 / KW;
 constexpr int VW = DH % 128 == 0 ? 16 : DH % 64 == 0 ? 8 : DH % 32 == 0 ? 4 : 2;      // ... of a value
@@ -88,6 +89,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+// whole numbers: 16 x 32 codes by 32 x 8
+__device__ __forceinline__ void imma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t turned(uint32_t x) {
   uint32_t y;
@@ -169,9 +175,9 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     };
     for (int i = 0; i < STAGES - 1; ++i) fetch(i, min(32, n_tiles), i);
 
-    // the queries of head g: columns (i * 4 + t) * KW ..
-    uint32_t qf[KT][2];
-    float fac, bias = 0.f;
+    // The queries of head g, columns (i * 4 + t) * KW .., as 256 * high + low with the largest at 32512.
+    uint32_t qh[KS][2], ql[KS][2];
+    float fac;
     {
       const __nv_bfloat16* qr = after_wait((const __nv_bfloat16*)a.q) + (size_t)x.row.tok * a.ldq + (size_t)(h0 + g) * DH;
       float v[KT][4];
@@ -199,24 +205,28 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e2 = max((int)(top >> 23) - 127, -100);           // the exponent of the largest
-      const float up = __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
+      // a query that is not finite: scores of NaN; one of next to nothing: scores of 0
+      const float largest = __uint_as_float(top);
+      const bool fine = top < 0x7f800000u && top >= 0x0d800000u;        // 2^-100
+      const float up = fine ? 32512.f / largest : 0.f;
+      fac = top >= 0x7f800000u ? NAN : fine ? largest / 32512.f * (a.scale * LOG2E) : 0.f;
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        qf[j][0] = pack_half2(v[j][0] * up, v[j][2] * up);
-        qf[j][1] = pack_half2(v[j][1] * up, v[j][3] * up);
+      for (int j = 0; j < KS * 2; ++j) {
+        uint32_t high = 0, low = 0;
+        if (j < KT) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                   // (the sum of what the products take)
-          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&qf[j][e]));
-          bias += u.x + u.y;
+          for (int e = 0; e < 4; ++e) {
+            // 1.5 * 2^23 + n: n's two's complement in the low bits
+            const int n = (int)(__float_as_uint(fmaf(v[j < KT ? j : 0][e], up, 12582912.f)) << 16) >> 16;
+            const int h = (n + 128) >> 8;
+            high |= (uint32_t)(h & 0xff) << (8 * e);
+            low |= (uint32_t)(n & 0xff) << (8 * e);
+          }
         }
+        qh[j >> 1][j & 1] = high;
+        ql[j >> 1][j & 1] = low;
       }
-      bias += __shfl_xor_sync(0xffffffffu, bias, 1);
-      bias += __shfl_xor_sync(0xffffffffu, bias, 2);
-      bias *= -128.f * UNIT;
-      fac = __uint_as_float((uint32_t)(127 - 14 + e2) << 23) * (a.scale * LOG2E / UNIT);
     }
-    const float bias0 = __shfl_sync(0xffffffffu, bias, 8 * t), bias1 = __shfl_sync(0xffffffffu, bias, 8 * t + 4);
     const float fac0 = __shfl_sync(0xffffffffu, fac, 8 * t), fac1 = __shfl_sync(0xffffffffu, fac, 8 * t + 4);      // of heads 2t, 2t + 1
 
     float o[KT][4];
@@ -236,15 +246,18 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         load_bytes<KW>(p, &fk[0][i2 * (KW / 4)]);
         load_bytes<KW>(p + 8 * DH, &fk[1][i2 * (KW / 4)]);
       }
-      float c[4] = {bias0, bias1, bias0, bias1}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+      int c[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        float (&d)[4] = j & 1 ? c2 : c;
-        mma(d, even(fk[0][j]), even(fk[1][j]), odd(fk[0][j]), odd(fk[1][j]), qf[j][0], qf[j][1], d[0], d[1], d[2], d[3]);
+      for (int j = 0; j < KS; ++j) {
+        const bool pair = 2 * j + 1 < KT;
+        const uint32_t a2 = pair ? fk[0][pair ? 2 * j + 1 : 0] : 0u, a3 = pair ? fk[1][pair ? 2 * j + 1 : 0] : 0u;
+        imma(c, fk[0][2 * j], fk[1][2 * j], a2, a3, qh[j][0], qh[j][1]);
+        imma(c2, fk[0][2 * j], fk[1][2 * j], a2, a3, ql[j][0], ql[j][1]);
       }
-      // scores of keys g and g + 8, heads 2t and 2t + 1, in units of log2
+      // scores of keys g and g + 8, heads 2t and 2t + 1, in units of log2 (the sums stay below 2^31 for heads of up to 256)
       const float a0 = sk * fac0, a1 = sk * fac1;
-      float s0 = (c[0] + c2[0]) * a0, s1 = (c[1] + c2[1]) * a1, s2 = (c[2] + c2[2]) * a0, s3 = (c[3] + c2[3]) * a1;
+      float s0 = (float)(c[0] * 256 + c2[0]) * a0, s1 = (float)(c[1] * 256 + c2[1]) * a1;
+      float s2 = (float)(c[2] * 256 + c2[2]) * a0, s3 = (float)(c[3] * 256 + c2[3]) * a1;
       if (i == 0 || i == n_tiles - 1) {                 // (a window begins in a row's first tile)
         const int key = x.begin + i * BLK;
         const bool in = key + g >= lo && key + g < x.end, in8 = key + g + 8 >= lo && key + g + 8 < x.end;
