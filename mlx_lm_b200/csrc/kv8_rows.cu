@@ -23,14 +23,14 @@ template <int LPK>
 __global__ void __launch_bounds__(WARPS * 32)
 rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
   constexpr int KPW = 32 / LPK, NG = WARPS * KPW;     // keys at a time: of a warp, of the CTA
-  extern __shared__ int dyn[];                        // prefix sums, then the weights of the last step
+  extern __shared__ int dyn[];                        // what is kept of the rows, then the weights of the last step
   __shared__ int warp_sums[WARPS], last;
   __shared__ float sm_m[WARPS][HT], sm_l[WARPS][HT], sm_o[WARPS][HT][256];
   __shared__ float fin_m[HT], fin_l[HT], fin_o[HT * 256];
-  int* prefix = dyn;
-  float* weights = reinterpret_cast<float*>(dyn + a.n_rows + 1);
+  const Rows rows(dyn, a.n_rows);
+  float* weights = reinterpret_cast<float*>(dyn + 4 * a.n_rows + 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int total = schedule(a, prefix, warp_sums) * tiles;
+  const int total = schedule(a, rows, warp_sums) * tiles;
   const int G = a.Hq / a.Hkv, D = a.dim, per = a.page / BLK;
   const int grp = warp * KPW + lane / LPK, part = lane & (LPK - 1);
   const bool mine = part * 16 < D;
@@ -39,7 +39,7 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
   const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
   const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
   for (int it = blockIdx.x; it < total; it += gridDim.x) {
-    const Item x = item_of(a, prefix, it, tiles);
+    const Item x = item_of(a, rows, it, tiles);
     const int hk = x.tile / group_tiles, j0 = (x.tile - hk * group_tiles) * HT, nh = min(HT, G - j0), h0 = hk * G + j0;
     const int* bt = a.block_table + (size_t)x.row.req * a.max_pages;
     const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
@@ -150,7 +150,7 @@ MLXB_EXPORT int mlxb_kv8_rows(const RowsRecord* rec, long long bytes, cudaStream
   if (a.n_rows <= 0) return 0;
   const int Hq = a.Hq, Hkv = a.Hkv, dim = a.dim, n_rows = a.n_rows, most_chunks = a.most_chunks;
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
-  const size_t smem = (size_t)(n_rows + 1 + (most_chunks + 1) * HT) * 4;
+  const size_t smem = rows_bytes(n_rows) + (size_t)(most_chunks + 1) * HT * 4;
   const long long most = (long long)n_rows * most_chunks * tiles, fill = 4ll * mlxb_sm_count();
   const dim3 grid((unsigned)(most < fill ? most : fill));
   auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(WARPS * 32), smem, stream, a, tiles, group_tiles); };

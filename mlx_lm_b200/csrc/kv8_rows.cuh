@@ -12,7 +12,7 @@
 #include "common.cuh"
 
 constexpr int BLK = 16;              // positions that share a scale
-constexpr int ROWS_MOST = 4096;      // rows a launch takes: their prefix sums are in shared memory
+constexpr int ROWS_MOST = 1024;      // rows a launch takes: what a CTA knows of them is in shared memory
 
 struct RowsArgs {
   const void* q;
@@ -24,46 +24,59 @@ struct RowsArgs {
   const float *ks, *vs, *sinks;
   float* partial;
   int* counters;
-  int most_chunks;                   // of a row
+  int most_chunks, least_chunk;      // how many chunks of a row at most, of how many keys at least
   void* out;
   int ldo, n_rows;
   int* status;
 };
 
-// Keys of a chunk for a row of n keys: a multiple of 64 that cuts them into at most `most` chunks.
-__device__ __forceinline__ int chunk_keys(int n, int most) {
-  const int c = n <= 1024 ? 128 : 256;
-  const int least = ((n + most - 1) / most + 63) & ~63;
+// Keys of a chunk for a row of n keys: `least` (a multiple of 64) or more, in at most `most` chunks.
+__device__ __forceinline__ int chunk_keys(int n, int most, int least) {
+  const int c = ((n + most - 1) / most + 63) & ~63;
   return c > least ? c : least;
 }
 
 struct RowSpan { int tok, req, pos, first, n; };      // first: a multiple of 16; n: keys from there to the query (0: no such row)
 
-__device__ __forceinline__ RowSpan row_span(const RowsArgs& a, int i, bool report) {
-  RowSpan s{a.rows ? a.rows[i] : i, -1, 0, 0, 0};
-  s.req = a.token_req[s.tok];
-  if (s.req < 0) return s;                            // a row that pads the step
-  s.pos = a.positions[s.tok];
-  if (s.pos < 0 || s.pos / a.page >= a.max_pages) {
-    if (report) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
-    return s;
-  }
-  const int lo = a.window > 0 && s.pos - a.window + 1 > 0 ? s.pos - a.window + 1 : 0;
+__device__ __forceinline__ RowSpan span_of(const RowsArgs& a, int tok, int req, int pos) {
+  RowSpan s{tok, req, pos, 0, 0};
+  if (req < 0 || pos < 0 || pos / a.page >= a.max_pages) return s;      // a row that pads the step, or one out of range
+  const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
   s.first = lo & ~(BLK - 1);
-  s.n = s.pos + 1 - s.first;
+  s.n = pos + 1 - s.first;
   return s;
 }
+__device__ __forceinline__ RowSpan row_span(const RowsArgs& a, int i) {
+  const int tok = a.rows ? a.rows[i] : i, req = a.token_req[tok], pos = a.positions[tok];
+  return span_of(a, tok, req, pos);
+}
+__device__ __forceinline__ int chunks_of(const RowsArgs& a, int n) {
+  if (n == 0) return 0;
+  const int keys = chunk_keys(n, a.most_chunks, a.least_chunk);
+  return (n + keys - 1) / keys;
+}
 
-// prefix[i]: chunks of the rows before row i; returns the number of all.  Every thread of the CTA calls it.
-__device__ __forceinline__ int schedule(const RowsArgs& a, int* prefix, int* warp_sums) {
+// What a CTA keeps of the rows: 4 n_rows + 1 integers.
+struct Rows {
+  int *prefix, *tok, *req, *pos;     // prefix[i]: chunks of the rows before row i
+  __device__ __forceinline__ Rows(int* mem, int n) : prefix(mem), tok(mem + n + 1), req(tok + n), pos(req + n) {}
+};
+static inline size_t rows_bytes(int n_rows) { return (size_t)(4 * n_rows + 1) * 4; }
+
+// Fills `rows` in; returns the number of all chunks.  Every thread of the CTA calls it.
+__device__ __forceinline__ int schedule(const RowsArgs& a, const Rows& rows, int* warp_sums) {
   const int n = a.n_rows, seg = (n + blockDim.x - 1) / blockDim.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
   const int b = min(n, (int)threadIdx.x * seg), e = min(n, b + seg);
   int sum = 0;
   for (int i = b; i < e; ++i) {
-    const RowSpan s = row_span(a, i, blockIdx.x == 0);
-    const int c = s.n ? (s.n + chunk_keys(s.n, a.most_chunks) - 1) / chunk_keys(s.n, a.most_chunks) : 0;
-    prefix[i + 1] = c;
+    const RowSpan s = row_span(a, i);
+    if (s.n == 0 && s.req >= 0 && blockIdx.x == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
+    const int c = chunks_of(a, s.n);
+    rows.tok[i] = s.tok;
+    rows.req[i] = s.req;
+    rows.pos[i] = s.pos;
+    rows.prefix[i + 1] = c;
     sum += c;
   }
   int run = sum;
@@ -78,8 +91,8 @@ __device__ __forceinline__ int schedule(const RowsArgs& a, int* prefix, int* war
   for (int w = 0; w < warp; ++w) before += warp_sums[w];
   int total = 0;
   for (int w = 0; w < n_warps; ++w) total += warp_sums[w];
-  for (int i = b; i < e; ++i) { before += prefix[i + 1]; prefix[i + 1] = before; }
-  if (threadIdx.x == 0) prefix[0] = 0;
+  for (int i = b; i < e; ++i) { before += rows.prefix[i + 1]; rows.prefix[i + 1] = before; }
+  if (threadIdx.x == 0) rows.prefix[0] = 0;
   __syncthreads();
   return total;
 }
@@ -90,20 +103,20 @@ struct Item {
 };
 
 // Item `it` of `tiles` tiles of heads: neighbouring items are the tiles of one chunk, whose pages lie together.
-__device__ __forceinline__ Item item_of(const RowsArgs& a, const int* prefix, int it, int tiles) {
+__device__ __forceinline__ Item item_of(const RowsArgs& a, const Rows& rows, int it, int tiles) {
   Item x;
   const int g = it / tiles;
   x.tile = it - g * tiles;
   int lo = 0, hi = a.n_rows - 1;                      // the last row whose prefix is <= g
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] <= g) lo = mid; else hi = mid - 1;
+    if (rows.prefix[mid] <= g) lo = mid; else hi = mid - 1;
   }
   x.index = lo;
-  x.chunk = g - prefix[lo];
-  x.n_chunks = prefix[lo + 1] - prefix[lo];
-  x.row = row_span(a, lo, false);
-  const int c = chunk_keys(x.row.n, a.most_chunks);
+  x.chunk = g - rows.prefix[lo];
+  x.n_chunks = rows.prefix[lo + 1] - rows.prefix[lo];
+  x.row = span_of(a, rows.tok[lo], rows.req[lo], rows.pos[lo]);
+  const int c = chunk_keys(x.row.n, a.most_chunks, a.least_chunk);
   x.begin = x.row.first + x.chunk * c;
   x.end = min(x.begin + c, x.row.pos + 1);
   return x;
@@ -200,7 +213,7 @@ struct RowsRecord {
   int* counters;
   void* out;
   int* status;
-  long long ldq, max_pages, n_pages, page, Hq, Hkv, dim, window, most_chunks, ldo, n_rows;
+  long long ldq, max_pages, n_pages, page, Hq, Hkv, dim, window, most_chunks, least_chunk, ldo, n_rows;
   double scale;
 };
 
@@ -209,13 +222,14 @@ static inline int rows_args(const RowsRecord* rec, long long bytes, const char* 
   const RowsRecord& x = *rec;
   a = RowsArgs{x.q, (int)x.ldq, x.rows, x.positions, x.token_req, x.block_table, (int)x.max_pages, (int)x.n_pages, (int)x.page, (int)x.Hq,
                (int)x.Hkv, (int)x.dim, (int)x.window, (float)x.scale, x.k8, x.v8, x.ks, x.vs, x.sinks, x.partial, x.counters,
-               (int)x.most_chunks, x.out, (int)x.ldo, (int)x.n_rows, x.status};
+               (int)x.most_chunks, (int)x.least_chunk, x.out, (int)x.ldo, (int)x.n_rows, x.status};
   if (a.n_rows > ROWS_MOST) return mlxb_fail(MLXB_BAD_ARG, "%s: %d rows, a launch takes %d", what, a.n_rows, ROWS_MOST);
   if (a.Hkv <= 0 || a.Hq <= 0 || a.Hq % a.Hkv) return mlxb_fail(MLXB_BAD_ARG, "%s: %d query heads over %d key/value heads", what, a.Hq, a.Hkv);
   if (a.dim % 16 || a.dim < 16 || a.dim > 256) return mlxb_fail(MLXB_BAD_ARG, "%s: head size %d (a multiple of 16 up to 256)", what, a.dim);
   if (a.page < BLK || (a.page & (a.page - 1)))
     return mlxb_fail(MLXB_BAD_ARG, "%s: page size %d (a power of two of at least %d)", what, a.page, BLK);
-  if (a.most_chunks <= 0 || a.most_chunks > 1024) return mlxb_fail(MLXB_BAD_ARG, "%s: %d chunks of a row", what, a.most_chunks);
+  if (a.most_chunks <= 0 || a.most_chunks > 1024 || a.least_chunk < 64 || a.least_chunk % 64)
+    return mlxb_fail(MLXB_BAD_ARG, "%s: %d chunks of a row, of %d keys at least", what, a.most_chunks, a.least_chunk);
   if (((uintptr_t)a.k8 | (uintptr_t)a.v8 | (uintptr_t)a.partial) & 15)
     return mlxb_fail(MLXB_BAD_ARG, "%s: pools and scratch memory must be 16-byte aligned", what);
   return 0;

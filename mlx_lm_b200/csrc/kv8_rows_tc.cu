@@ -1,8 +1,9 @@
 // Attention of single queries over pages in 8 bits for bfloat16 queries: the products on the tensor cores, codes turned into their
 // operands in registers.  Built once for each head size (MLXB_HEAD_DIM).
 //
-// A warp works by itself, an item after the other: asynchronous copies bring its tiles into a ring of its own in shared memory, several
-// tiles ahead, and no block-wide wait stands between the items.  Rows of several chunks leave sums that a second kernel adds up.
+// A block takes an item after the other, its warps a quarter of the item's keys each: asynchronous copies bring a warp's tiles into a
+// ring of its own in shared memory, several ahead, the first of the next item while the warps' sums of this one come together.  Rows
+// of several chunks leave sums that a second kernel adds up.
 // A warp takes 16 keys at a time (a block with one scale; never more than one page) for up to eight query heads that read the same
 // key/value head:
 //   S^T [16 keys x 8 heads] = K [16 x dim] Q^T      m16n8k32 in whole numbers: K's codes are A as they lie in memory
@@ -115,13 +116,22 @@ constexpr int PART = 8 * (DH + 2);                      // floats of an item's s
 
 __device__ __forceinline__ int column_of(int c, int g) { return (c / VW * 8 + g) * VW + c % VW; }      // column c of lane group g's
 
+// An item and a warp's share of it.
+struct Job {
+  Item x;
+  int hk, h0, nh, first, mine;                          // key/value head, first query head, how many; first key and number of tiles
+  uint32_t tile_id, missing;
+  float sk, sv;
+};
+
 __global__ void __launch_bounds__(WARPS * 32, CTAS)
 rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
-  extern __shared__ __align__(128) uint8_t ring[];      // the warps' tiles, then the prefix sums
-  __shared__ int warp_sums[WARPS];
-  int* prefix = reinterpret_cast<int*>(ring + RING);
+  extern __shared__ __align__(128) uint8_t ring[];      // the warps' tiles, then what is kept of the rows
+  __shared__ int warp_sums[WARPS], sm_spare[WARPS];
+  __shared__ float sm_m[WARPS][HT], sm_l[WARPS][HT];
+  const Rows rows(reinterpret_cast<int*>(ring + RING), a.n_rows);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int total = schedule(a, prefix, warp_sums) * tiles;
+  const int total = schedule(a, rows, warp_sums) * tiles;
   const int G = a.Hq / a.Hkv, per = a.page / BLK;
   uint8_t* my_ring = ring + warp * (STAGES * TILE);
   const uint32_t my_ring_u32 = (uint32_t)__cvta_generic_to_shared(my_ring);
@@ -132,48 +142,59 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
   const int value_base = value_at(2 * t, (g * VW) >> 4) + ((g * VW) & 15);
   const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
   const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
-  for (int it = warp * gridDim.x + blockIdx.x; it < total; it += WARPS * gridDim.x) {
-    const Item x = item_of(a, prefix, it, tiles);
-    const int hk = x.tile / group_tiles, j0 = (x.tile - hk * group_tiles) * HT, nh = min(HT, G - j0), h0 = hk * G + j0;
-    const int* bt = a.block_table + (size_t)x.row.req * a.max_pages;
-    const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
-    const int n_tiles = (x.end - x.begin + BLK - 1) / BLK;
-
-    // lane i knows of the i-th of the next 32 tiles which tile of the pool it is, and its scales; missing: tiles without a page
-    uint32_t tile_id = 0, missing = 0;
-    float skl = 0.f, svl = 0.f;
-    auto look_up = [&](int i0) {
-      const int i = i0 + lane, key = x.begin + i * BLK;
-      bool none = false;
-      if (i < n_tiles) {
-        const int pg = page_of(a, bt, key);
-        none = pg < 0;
-        if (!none) {
-          tile_id = (uint32_t)(pg * a.Hkv + hk) * per + (key & (a.page - 1)) / BLK;
-          skl = __ldcg(ks + tile_id);
-          svl = __ldcg(vs + tile_id);
-        }
+  Job job;
+  // lane i learns of the i-th of the warp's next 32 tiles which tile of the pool it is, and its scales; missing: tiles without a page
+  auto look_up = [&](Job& b, int i0) {
+    const int i = i0 + lane, key = b.first + i * BLK;
+    bool none = false;
+    if (i < b.mine) {
+      const int pg = page_of(a, a.block_table + (size_t)b.x.row.req * a.max_pages, key);
+      none = pg < 0;
+      if (!none) {
+        b.tile_id = (uint32_t)(pg * a.Hkv + b.hk) * per + (key & (a.page - 1)) / BLK;
+        b.sk = __ldcg(ks + b.tile_id);
+        b.sv = __ldcg(vs + b.tile_id);
       }
-      missing = __ballot_sync(0xffffffffu, none);
-    };
-    look_up(0);
-    // tile i of the 32 looked up, on its way into stage st; a group of copies for every tile, an empty one where there is none
-    auto fetch = [&](int i, int n, int st) {
-      if (i < n && !(missing >> i & 1)) {
-        const size_t at = (size_t)__shfl_sync(0xffffffffu, tile_id, i) * (16 * DH) + lane * 16;
-        const uint32_t dst = my_ring_u32 + st * TILE;
+    }
+    b.missing = __ballot_sync(0xffffffffu, none);
+  };
+  // tile i of the n looked up, on its way into stage st; a group of copies for every tile, an empty one where there is none
+  auto fetch = [&](const Job& b, int i, int n, int st) {
+    if (i < n && !(b.missing >> i & 1)) {
+      const size_t at = (size_t)__shfl_sync(0xffffffffu, b.tile_id, i) * (16 * DH) + lane * 16;
+      const uint32_t dst = my_ring_u32 + st * TILE;
 #pragma unroll
-        for (int e0 = 0; e0 < DH; e0 += 32) {
-          const int e = e0 + lane, row = e / (DH / 16), c = e % (DH / 16);
-          if (DH % 32 == 0 || e < DH) {
-            copy16(dst + key_at(row, c), k8 + at + e0 * 16);
-            copy16(dst + 16 * DH + value_at(row, c), v8 + at + e0 * 16);
-          }
+      for (int e0 = 0; e0 < DH; e0 += 32) {
+        const int e = e0 + lane, row = e / (DH / 16), c = e % (DH / 16);
+        if (DH % 32 == 0 || e < DH) {
+          copy16(dst + key_at(row, c), k8 + at + e0 * 16);
+          copy16(dst + 16 * DH + value_at(row, c), v8 + at + e0 * 16);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int i = 0; i < STAGES - 1; ++i) fetch(i, min(32, n_tiles), i);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int st = 0;                                           // the stage of the warp's next tile
+  // the first tiles of an item: all stages but the one before st
+  auto begin = [&](Job& b, int it) {
+    b.x = item_of(a, rows, it, tiles);
+    b.hk = b.x.tile / group_tiles;
+    const int j0 = (b.x.tile - b.hk * group_tiles) * HT;
+    b.nh = min(HT, G - j0);
+    b.h0 = b.hk * G + j0;
+    // a quarter of the item's tiles each
+    const int n = (b.x.end - b.x.begin + BLK - 1) / BLK, each = (n + WARPS - 1) / WARPS;
+    b.first = b.x.begin + warp * each * BLK;
+    b.mine = max(0, min(each, n - warp * each));
+    look_up(b, 0);
+    for (int i = 0, s = st; i < STAGES - 1; ++i, s = s + 1 == STAGES ? 0 : s + 1) fetch(b, i, min(32, b.mine), s);
+  };
+  int it = blockIdx.x;
+  if (it < total) begin(job, it);
+  while (it < total) {
+    const int h0 = job.h0, nh = job.nh, n_tiles = job.mine;
+    const Item& x = job.x;
+    const int lo = a.window > 0 ? x.row.pos - a.window + 1 : 0;
 
     // The queries of head g, columns (i * 4 + t) * KW .., as 256 * high + low with the largest at 32512.
     uint32_t qh[KS][2], ql[KS][2];
@@ -235,8 +256,8 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     auto work = [&](int i, int i32, int st) {           // tile i, the i32-th of those looked up
-      if (missing >> i32 & 1) return;
-      const float sk = __shfl_sync(0xffffffffu, skl, i32), sv = __shfl_sync(0xffffffffu, svl, i32);
+      if (job.missing >> i32 & 1) return;
+      const float sk = __shfl_sync(0xffffffffu, job.sk, i32), sv = __shfl_sync(0xffffffffu, job.sv, i32);
       const uint8_t* kp = my_ring + st * TILE;
       const uint8_t* vp = kp + 16 * DH + value_base;
       uint32_t fk[2][KT];
@@ -259,7 +280,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       float s0 = (float)(c[0] * 256 + c2[0]) * a0, s1 = (float)(c[1] * 256 + c2[1]) * a1;
       float s2 = (float)(c[2] * 256 + c2[2]) * a0, s3 = (float)(c[3] * 256 + c2[3]) * a1;
       if (i == 0 || i == n_tiles - 1) {                 // (a window begins in a row's first tile)
-        const int key = x.begin + i * BLK;
+        const int key = job.first + i * BLK;
         const bool in = key + g >= lo && key + g < x.end, in8 = key + g + 8 >= lo && key + g + 8 < x.end;
         if (!in) s0 = s1 = -INFINITY;
         if (!in8) s2 = s3 = -INFINITY;
@@ -316,73 +337,116 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     for (int i0 = 0; i0 < n_tiles; i0 += 32) {
       const int n = min(32, n_tiles - i0);
       if (i0 > 0) {
-        look_up(i0);
-        for (int i = 0; i < STAGES - 1; ++i) fetch(i, n, i);
+        look_up(job, i0);
+        for (int i = 0, s = st; i < STAGES - 1; ++i, s = s + 1 == STAGES ? 0 : s + 1) fetch(job, i, n, s);
       }
-      int st = 0;
       for (int i = 0; i < n; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                                   // every lane's copies of tile i are there, and tile i - 1 has been read
-        fetch(i + STAGES - 1, n, st == 0 ? STAGES - 1 : st - 1);
+        fetch(job, i + STAGES - 1, n, st == 0 ? STAGES - 1 : st - 1);
         work(i0 + i, i, st);
         st = st + 1 == STAGES ? 0 : st + 1;
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncwarp();
     }
-    const bool one = 2 * t < nh, two = 2 * t + 1 < nh;
-    if (x.n_chunks > 1) {
-      float* part = a.partial + (((size_t)x.index * tiles + x.tile) * a.most_chunks + x.chunk) * PART;
-      if (g == 0) {
-        reinterpret_cast<float2*>(part)[t] = make_float2(m0, m1);
-        reinterpret_cast<float2*>(part + 8)[t] = make_float2(l0, l1);
-      }
-      if (one) {
+    __syncwarp();
+    // the next item's first tiles are on their way while the warps' sums come together in the stage that they leave free
+    const Item done = job.x;
+    it += gridDim.x;
+    if (it < total) begin(job, it);
+    const int spare = st == 0 ? STAGES - 1 : st - 1;
+    float4* mine4 = reinterpret_cast<float4*>(my_ring + spare * TILE);
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
-          __stcg(reinterpret_cast<float4*>(part + 16) + j * 32 + lane, make_float4(o[j][0], o[j][1], o[j][2], o[j][3]));
-      }
-    } else {
-      if (a.sinks) {
-        if (one) l0 += ex2(a.sinks[h0 + 2 * t] * LOG2E - m0);
-        if (two) l1 += ex2(a.sinks[h0 + 2 * t + 1] * LOG2E - m1);
-      }
-      const float r0 = l0 != 0.f ? 1.f / (l0 * UNIT) : 0.f, r1 = l1 != 0.f ? 1.f / (l1 * UNIT) : 0.f;
-      __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)x.row.tok * a.ldo + (size_t)(h0 + 2 * t) * DH;
+    for (int j = 0; j < KT; ++j) mine4[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+    if (g == 0) {
+      sm_m[warp][2 * t] = m0; sm_m[warp][2 * t + 1] = m1;
+      sm_l[warp][2 * t] = l0; sm_l[warp][2 * t + 1] = l1;
+    }
+    if (lane == 0) sm_spare[warp] = warp * (STAGES * TILE) + spare * TILE;
+    __syncthreads();
+    {
+      float w0[WARPS], w1[WARPS], tot0 = 0.f, tot1 = 0.f;      // of heads 2t, 2t + 1
+      float top0 = sm_m[0][2 * t], top1 = sm_m[0][2 * t + 1];
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
+      for (int w = 1; w < WARPS; ++w) { top0 = fmaxf(top0, sm_m[w][2 * t]); top1 = fmaxf(top1, sm_m[w][2 * t + 1]); }
+      const float b0 = top0 == -INFINITY ? 0.f : top0, b1 = top1 == -INFINITY ? 0.f : top1;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = column_of(2 * j + e, g);
-          if (one) out[d] = __float2bfloat16_rn(o[j][2 * e] * r0);
-          if (two) out[DH + d] = __float2bfloat16_rn(o[j][2 * e + 1] * r1);
+      for (int w = 0; w < WARPS; ++w) {
+        w0[w] = ex2(sm_m[w][2 * t] - b0);
+        w1[w] = ex2(sm_m[w][2 * t + 1] - b1);
+        tot0 = fmaf(w0[w], sm_l[w][2 * t], tot0);
+        tot1 = fmaf(w1[w], sm_l[w][2 * t + 1], tot1);
+      }
+      const bool one = 2 * t < nh, two = 2 * t + 1 < nh;
+      float* part = a.partial + (((size_t)done.index * tiles + done.tile) * a.most_chunks + done.chunk) * PART;
+      if (done.n_chunks > 1 && threadIdx.x < 4) {
+        reinterpret_cast<float2*>(part)[t] = make_float2(top0, top1);
+        reinterpret_cast<float2*>(part + 8)[t] = make_float2(tot0, tot1);
+      }
+      if (done.n_chunks == 1) {
+        if (a.sinks) {
+          if (one) tot0 += ex2(a.sinks[h0 + 2 * t] * LOG2E - b0);
+          if (two) tot1 += ex2(a.sinks[h0 + 2 * t + 1] * LOG2E - b1);
+        }
+        tot0 = tot0 != 0.f ? 1.f / (tot0 * UNIT) : 0.f;
+        tot1 = tot1 != 0.f ? 1.f / (tot1 * UNIT) : 0.f;
+      }
+      __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)done.row.tok * a.ldo + (size_t)(h0 + 2 * t) * DH;
+      for (int j = warp; j < KT; j += WARPS) {
+        if (!one) continue;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float4 v = reinterpret_cast<const float4*>(ring + sm_spare[w])[j * 32 + lane];
+          y.x = fmaf(w0[w], v.x, y.x); y.y = fmaf(w1[w], v.y, y.y); y.z = fmaf(w0[w], v.z, y.z); y.w = fmaf(w1[w], v.w, y.w);
+        }
+        if (done.n_chunks > 1) {
+          __stcg(reinterpret_cast<float4*>(part + 16) + j * 32 + lane, y);
+        } else {
+          const int d0 = column_of(2 * j, g), d1 = column_of(2 * j + 1, g);
+          out[d0] = __float2bfloat16_rn(y.x * tot0);
+          out[d1] = __float2bfloat16_rn(y.z * tot0);
+          if (two) {
+            out[DH + d0] = __float2bfloat16_rn(y.y * tot1);
+            out[DH + d1] = __float2bfloat16_rn(y.w * tot1);
+          }
         }
       }
     }
+    __syncthreads();
   }
 }
 
-// The sums of a row's chunks, added in the order of four runs of chunks: a block takes 16 columns of a (row, tile of heads).
-__global__ void __launch_bounds__(128)
-rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
+constexpr int JOIN = 8;                                 // warps of a block that joins
+
+// The sums of a row's chunks, added in the order of `runs` runs of chunks (1, 2, 4 or 8: few chunks make few blocks, many are read in
+// parallel).  A block has JOIN / runs pairs of eight columns of a (row, tile of heads), a warp one pair of them and one run.  The first O
+// of a run are on their way with the maxima and sums: one latency, not three, where a run is short.
+__global__ void __launch_bounds__(32 * JOIN)
+rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles, int runs) {
   extern __shared__ float weights[];                    // [chunk][8]
-  __shared__ float red[4][8];
-  __shared__ float4 sums[4][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
-  const int i = blockIdx.x / tiles, tile = blockIdx.x - i * tiles, j = blockIdx.y;
-  const RowSpan row = row_span(a, i, false);
-  const int c_keys = row.n ? chunk_keys(row.n, a.most_chunks) : 1, n = (row.n + c_keys - 1) / c_keys;
+  __shared__ float red[JOIN][8], red2[JOIN][8];
+  __shared__ float4 sums[JOIN][32];
+  constexpr int EARLY = 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, pairs = JOIN / runs;
+  const int i = blockIdx.x / tiles, tile = blockIdx.x - i * tiles, run = warp / pairs, j = blockIdx.y * pairs + warp - run * pairs;
+  const RowSpan row = row_span(a, i);
+  const int n = chunks_of(a, row.n);
   pdl_wait();
   pdl_trigger();
   if (n <= 1) return;
   const int hk = tile / group_tiles, G = a.Hq / a.Hkv, j0 = (tile - hk * group_tiles) * HT, nh = min(HT, G - j0), h0 = hk * G + j0;
   const float* all = after_wait(a.partial) + (size_t)blockIdx.x * a.most_chunks * PART;
-  const bool mine = 2 * t < nh;
-  const int per = (n + 3) / 4, c0 = warp * per, c1 = min(n, c0 + per);
-  const int h = threadIdx.x & 7;
+  const bool mine = 2 * t < nh && j < KT;
+  const int each = (n + runs - 1) / runs, c0 = run * each, c1 = min(n, c0 + each);
+  auto o_of = [&](int c) { return __ldcg(reinterpret_cast<const float4*>(all + (size_t)c * PART + 16) + j * 32 + lane); };
+  float4 early[EARLY];
+#pragma unroll
+  for (int e = 0; e < EARLY; ++e) early[e] = mine && c0 + e < c1 ? o_of(c0 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const int h = threadIdx.x & 7, first = threadIdx.x >> 3;
+  const float l_first = first < n ? __ldcg(all + (size_t)first * PART + 8 + h) : 0.f;
   float top = -INFINITY;
   bool odd = false;                                     // fmaxf leaves NaN out
-  for (int c = threadIdx.x >> 3; c < n; c += 16) {
+  for (int c = first; c < n; c += 4 * JOIN) {
     const float m = __ldcg(all + (size_t)c * PART + h);
     weights[c * 8 + h] = m;
     odd |= m != m;
@@ -393,46 +457,56 @@ rows_tc_join_kernel(const RowsArgs a, int tiles, int group_tiles) {
   for (int d = 8; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (lane < 8) red[warp][lane] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0][h], red[1][h]), fmaxf(red[2][h], red[3][h]));
+#pragma unroll
+  for (int w = 0; w < JOIN; ++w) top = fmaxf(top, red[w][h]);
   if (top == -INFINITY) top = 0.f;                      // no key at all has a page: zeros
-  __syncthreads();
   float total = 0.f;
-  for (int c = threadIdx.x >> 3; c < n; c += 16) {
+  for (int c = first; c < n; c += 4 * JOIN) {
     const float w = ex2(weights[c * 8 + h] - top);
     weights[c * 8 + h] = w;
-    total = fmaf(w, __ldcg(all + (size_t)c * PART + 8 + h), total);
+    total = fmaf(w, c == first ? l_first : __ldcg(all + (size_t)c * PART + 8 + h), total);
   }
+  // the sink's term by lanes that all of a head share: into the first warp's sum
+  if (a.sinks && threadIdx.x < 8 && h < nh) total += ex2(a.sinks[h0 + h] * LOG2E - top);
 #pragma unroll
   for (int d = 8; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-  if (lane < 8) red[warp][lane] = total;
+  if (lane < 8) red2[warp][lane] = total;
   __syncthreads();
-  total = red[0][h] + red[1][h] + red[2][h] + red[3][h];
-  if (a.sinks && h < nh) total += ex2(a.sinks[h0 + h] * LOG2E - top);
-  const float inv = total != 0.f ? 1.f / (total * UNIT) : 0.f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine) {
-#pragma unroll 8
-    for (int c = c0; c < c1; ++c) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(all + (size_t)c * PART + 16) + j * 32 + lane);
+    auto add = [&](int c, const float4& v) {
       const float2 w = *reinterpret_cast<const float2*>(weights + c * 8 + 2 * t);
       s.x = fmaf(w.x, v.x, s.x); s.y = fmaf(w.y, v.y, s.y); s.z = fmaf(w.x, v.z, s.z); s.w = fmaf(w.y, v.w, s.w);
+    };
+#pragma unroll
+    for (int e = 0; e < EARLY; ++e)
+      if (c0 + e < c1) add(c0 + e, early[e]);
+#pragma unroll 4
+    for (int c = c0 + EARLY; c < c1; ++c) add(c, o_of(c));
+  }
+  if (runs > 1) {
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (run) return;
+    for (int w = warp + pairs; w < JOIN; w += pairs) {
+      const float4 v = sums[w][lane];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
   }
-  sums[warp][lane] = s;
-  __syncthreads();
-  if (threadIdx.x < 8) red[0][threadIdx.x] = inv;
-  __syncthreads();
-  // 8 heads x 16 columns, one a thread: head hh, the column of lane group gg and slot e
-  const int hh = threadIdx.x & 7, gg = (threadIdx.x >> 3) & 7, e = threadIdx.x >> 6;
-  if (hh >= nh) return;
-  float y = 0.f;
+  if (!mine) return;
+  float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float4 v = sums[w][gg * 4 + (hh >> 1)];
-    y += e ? (hh & 1 ? v.w : v.z) : (hh & 1 ? v.y : v.x);
+  for (int w = 0; w < JOIN; ++w) { l0 += red2[w][2 * t]; l1 += red2[w][2 * t + 1]; }
+  l0 = l0 != 0.f ? 1.f / (l0 * UNIT) : 0.f;
+  l1 = l1 != 0.f ? 1.f / (l1 * UNIT) : 0.f;
+  __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)row.tok * a.ldo + (size_t)(h0 + 2 * t) * DH;
+  const int lo = column_of(2 * j, lane >> 2), hi = column_of(2 * j + 1, lane >> 2);
+  out[lo] = __float2bfloat16_rn(s.x * l0);
+  out[hi] = __float2bfloat16_rn(s.z * l0);
+  if (2 * t + 1 < nh) {
+    out[DH + lo] = __float2bfloat16_rn(s.y * l1);
+    out[DH + hi] = __float2bfloat16_rn(s.w * l1);
   }
-  __nv_bfloat16* out = (__nv_bfloat16*)a.out + (size_t)row.tok * a.ldo + (size_t)(h0 + hh) * DH;
-  out[column_of(2 * j + e, gg)] = __float2bfloat16_rn(y * red[0][hh]);
 }
 
 // As mlxb_kv8_rows for bfloat16 and heads of MLXB_HEAD_DIM; tiles of eight query heads: partial n_rows * tiles * most_chunks * 8 *
@@ -444,15 +518,18 @@ MLXB_EXPORT int mlxb_kv8_rows_tc(const RowsRecord* rec, long long bytes, cudaStr
   if (a.dim != DH) return mlxb_fail(MLXB_BAD_ARG, "kv8_rows_tc: head size %d, this library is for %d", a.dim, DH);
   const int Hq = a.Hq, Hkv = a.Hkv, n_rows = a.n_rows, most_chunks = a.most_chunks;
   const int group_tiles = (Hq / Hkv + HT - 1) / HT, tiles = Hkv * group_tiles;
-  const size_t smem = RING + (size_t)(n_rows + 1) * 4;
+  const size_t smem = RING + rows_bytes(n_rows);
   const long long most = (long long)n_rows * most_chunks * tiles, fill = (long long)CTAS * mlxb_sm_count();
   static SharedLimit limit;
-  if (cudaError_t e = limit.raise(rows_tc_kernel, RING + (ROWS_MOST + 1) * 4))
+  if (cudaError_t e = limit.raise(rows_tc_kernel, RING + rows_bytes(ROWS_MOST)))
     return mlxb_fail((int)e, "kv8_rows_tc: shared memory: %s", cudaGetErrorString(e));
   launch_pdl(rows_tc_kernel, dim3((unsigned)(most < fill ? most : fill)), dim3(WARPS * 32), smem, stream, a, tiles, group_tiles,
              (a.ldq % 4 == 0 && !((uintptr_t)a.q & 7)) ? 1 : 0);
   if (int e = mlxb_check_launch("kv8_rows_tc")) return e;
   if (most_chunks == 1) return 0;
-  launch_pdl(rows_tc_join_kernel, dim3((unsigned)n_rows * tiles, KT), dim3(128), (size_t)most_chunks * 32, stream, a, tiles, group_tiles);
+  int runs = 1;                                         // eight chunks at once, then more warps
+  while (runs < JOIN && runs * 8 < most_chunks) runs *= 2;
+  launch_pdl(rows_tc_join_kernel, dim3((unsigned)n_rows * tiles, (KT * runs + JOIN - 1) / JOIN), dim3(32 * JOIN), (size_t)most_chunks * 32, stream,
+             a, tiles, group_tiles, runs);
   return mlxb_check_launch("kv8_rows_tc (join)");
 }

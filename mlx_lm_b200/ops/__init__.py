@@ -960,9 +960,10 @@ def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out,
     _call("kv8", "mlxb_kv8_read", _KV8_ARGS, record, size, stream)
 
 
-_kv8_rows_record = _kv8_record("14Q11qd")
+_kv8_rows_record = _kv8_record("14Q12qd")
 _KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
-_KV8_ITEMS = {torch.float32: 4 * 148, torch.bfloat16: 8 * 148}      # parts of one row's keys that fill the device
+_KV8_ITEMS = {torch.float32: 4 * 148, torch.bfloat16: 4 * 148}      # parts of one row's keys that fill the device
+_KV8_LEAST = {torch.float32: 128, torch.bfloat16: 1024}      # keys of a part at least (multiples of 64)
 
 
 _KV8_F32_ROWS = ("kv8_rows", "mlxb_kv8_rows")
@@ -976,9 +977,10 @@ def kv8_rows_library(dtype, head_dim: int) -> str:
 
 @functools.lru_cache(maxsize=256)
 def _kv8_plan(dtype, n_heads: int, n_kv_heads: int, max_len: int):
-    """``(tiles of heads, most parts of a row's keys)``: as many parts as fill the device with one row, and no more than the longest row has."""
-    tiles = n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS[dtype])
-    return tiles, max(1, min(_KV8_ITEMS[dtype] // tiles, -(-(max_len + KV8_BLOCK) // 128)))
+    """``(tiles of heads, most parts of a row's keys, keys of a part at least)``: as many parts as fill the device with one row, and no more
+    than the longest row has."""
+    tiles, least = n_kv_heads * -(-(n_heads // n_kv_heads) // _KV8_TILE_HEADS[dtype]), _KV8_LEAST[dtype]
+    return tiles, max(1, min(_KV8_ITEMS[dtype] // tiles, -(-(max_len + KV8_BLOCK - 1) // least))), least
 
 
 @functools.lru_cache(maxsize=256)
@@ -988,7 +990,7 @@ def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, 
     n = min(n_rows, KV8_ROWS_MOST)
     floats = tickets = 0
     for dtype, heads in _KV8_TILE_HEADS.items():
-        tiles, most = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
+        tiles, most, _ = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
         floats, tickets = max(floats, n * tiles * most * heads * (head_dim + 2)), max(tickets, n * tiles)
     return floats, tickets
 
@@ -1021,7 +1023,7 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         raise KernelError(f"kv8_attention_rows: scratch of {scratch.numel()} floats and {counters.numel()} counters, {floats} and "
                           f"{tickets} are needed")
     sk = _sinks(sinks, n_heads, "kv8_attention_rows") or 0
-    most = _kv8_plan(dtype, n_heads, Hkv, max_len)[1]
+    _, most, least = _kv8_plan(dtype, n_heads, Hkv, max_len)
     lib, name = (_KV8_F32_ROWS if dtype is _F32T else (kv8_rows_library(dtype, Dh), "mlxb_kv8_rows_tc"))
     qp, op, pp, tp, item = q.data_ptr(), out.data_ptr(), positions.data_ptr(), token_req.data_ptr(), q.element_size()
     for a in range(0, n, KV8_ROWS_MOST):
@@ -1030,7 +1032,7 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         record, size = _kv8_rows_record(
             qp + t * ldq * item, r, pp + 4 * t, tp + 4 * t, block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), sk, scratch.data_ptr(), counters.data_ptr(), op + t * ldo * item, status.data_ptr(), ldq,
-            block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, most, ldo, min(n - a, KV8_ROWS_MOST), scale)
+            block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, most, least, ldo, min(n - a, KV8_ROWS_MOST), scale)
         _call(lib, name, _KV8_ARGS, record, size, stream)
 
 
