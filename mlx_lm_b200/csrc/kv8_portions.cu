@@ -2,8 +2,8 @@
 //
 // A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs) and walks the request's
 // keys in blocks of 64 positions:
-//   converters  4 or 8 warps: codes from the pages to fp16 operands of K and V in 128-byte-swizzled shared memory, once for all NT heads;
-//               the scales of the block's eight groups of 16 positions beside them
+//   converters  4 or 8 warps: codes (bulk copies of 16 positions each, two blocks ahead) to fp16 operands of K and V in 128-byte-swizzled
+//               shared memory, once for all NT heads; the scales of the block's four groups of 16 positions beside them
 //   issuers     2 warps a head: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
 //   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 beside S
 // The softmax threads take a row of S into registers and let go of it: S of the next block is formed while they work on this one, and
@@ -37,7 +37,7 @@ constexpr int GR = TK / BLK;         // groups of a block
 constexpr int XR = 8;                // blocks whose scales are kept
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
-constexpr uint32_t HIGH = 0x6c00;    // 2^12 as fp16: the largest weight that a pass leaves be
+constexpr float HIGH = 4096.f;       // the largest sum of a group's weights that a pass leaves be: fp16 holds up to 65504
 
 struct PortionArgs {
   const __nv_bfloat16* q;
@@ -55,18 +55,19 @@ struct PortionArgs {
 
 template <int DP, int NT>
 struct Shape {
-  static constexpr int KST = NT == 1 && DP == 128 ? 2 : 4;        // buffers of K and of V: two CTAs an SM where a CTA has one head
   static constexpr int SOFT = 4 * NT, CONV = NT == 2 && DP == 128 ? 8 : 4;      // warps
-  static constexpr int GW = CONV / 2;                             // converters work in two groups, a block each
+  // converters work in NG groups, a block each, that have RD blocks of codes each under way; KST buffers of K and of V: what fits
+  static constexpr int NG = NT == 1 && DP == 128 ? 1 : 2, RD = NG, GW = CONV / NG;
+  static constexpr int KST = NT == 1 && DP == 128 ? 2 : NT == 2 && DP == 64 ? 4 : 3;
   static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (the last four issue products)
   // registers a thread, at launch (what the launch bounds leave: 640 x 96, 512 x 128, 384 x 80 twice) and then by role, no more in all
   static constexpr int R_LAUNCH = NT == 1 ? 80 : DP == 128 ? 96 : 128;
-  static constexpr int R_SOFT = NT == 1 ? 120 : DP == 128 ? 128 : 144, R_CONV = DP == 128 || NT == 1 ? 88 : 96, R_ISSUE = NT == 1 ? 24 : 40;
+  static constexpr int R_SOFT = NT == 1 ? 128 : 144, R_CONV = 72, R_ISSUE = NT == 1 ? 24 : 40;
   static_assert(32 * (SOFT * R_SOFT + CONV * R_CONV + 4 * R_ISSUE) <= THREADS * R_LAUNCH, "registers");
   static constexpr int CTAS = NT == 1 ? 2 : 1;
   static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, two buffers of P_t behind it; then O_t
   static constexpr int QSPAN = TQ * 128, SPAN = TK * 128;         // bytes of a tile's rows of 64 columns
-  static constexpr int QTILE = QSPAN * (DP / 64), TILE = SPAN * (DP / 64);
+  static constexpr int QTILE = QSPAN * (DP / 64), TILE = SPAN * (DP / 64), RAW = TK * DP;
 };
 
 template <int DP, int NT>
@@ -75,10 +76,13 @@ struct Smem {
   alignas(1024) uint8_t q[NT][H::QTILE];
   alignas(1024) uint8_t k[H::KST][H::TILE];
   alignas(1024) uint8_t v[H::KST][H::TILE];
+  alignas(1024) uint8_t raw_k[H::NG][H::RD][H::RAW], raw_v[H::NG][H::RD][H::RAW];      // codes as they come
   float sk[XR][GR], lsv[XR][GR], rsv[XR][GR];           // of the last blocks: key scale, log2 and reciprocal of the value scale
   uint32_t missing[XR];                                 // groups without a page
+  uint32_t nothing[H::NG];                              // groups whose values are 0 whatever their codes
   alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST];
   uint64_t s_full[NT], s_read[NT], p_full[NT][2], pv_done[NT][2], drained[2 * NT];
+  uint64_t rk_full[H::NG][H::RD], rv_full[H::NG][H::RD];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -123,11 +127,6 @@ __device__ __forceinline__ void registers() {
   if constexpr (N > AT_LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
   else if constexpr (N < AT_LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
-__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
-  uint32_t y;
-  asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  return y;
-}
 // two float32 at a time
 __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
@@ -147,6 +146,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
       : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, done != 0) || mbar_wait_warp(bar, parity, abort_flag);
 }
+// `bytes` (a multiple of 16, as both addresses) from global to shared memory; the barrier counts them.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// A barrier of some of the CTA's warps.
+__device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -176,13 +182,14 @@ template <int DP, int NT>
 __global__ void __launch_bounds__(Shape<DP, NT>::THREADS, Shape<DP, NT>::CTAS)
 portions_kernel(const PortionArgs a) {
   using H = Shape<DP, NT>;
-  extern __shared__ uint8_t smem_raw[];
-  Smem<DP, NT>& sm = *reinterpret_cast<Smem<DP, NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem<DP, NT>& sm = *reinterpret_cast<Smem<DP, NT>*>(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int4 tile = a.tiles[blockIdx.x];
+  const int heads = a.Hq / NT, by_tile = blockIdx.x / heads;
+  const int4 tile = a.tiles[gridDim.x / heads - 1 - by_tile];      // a portion's last tiles, the longest, first
   if (tile.y <= 0) return;
   const int row0 = tile.x, n_rows = min(tile.y, TQ), req = tile.z, pos0 = tile.w;
-  const int h0 = blockIdx.y * NT, hk = h0 / (a.Hq / a.Hkv);
+  const int h0 = (blockIdx.x - by_tile * heads) * NT, hk = h0 / (a.Hq / a.Hkv);
   const int last_pos = pos0 + n_rows - 1;
   const int first_key = a.window > 0 && pos0 - a.window + 1 > 0 ? pos0 - a.window + 1 : 0;
   const int kb_lo = first_key / TK, n_blocks = last_pos / TK - kb_lo + 1;
@@ -201,6 +208,7 @@ portions_kernel(const PortionArgs a) {
       mbar_init(&sm.v_free[i], NT);
     }
     for (int i = 0; i < 2 * NT; ++i) mbar_init(&sm.drained[i], 1);
+    for (int i = 0; i < H::NG * H::RD; ++i) { mbar_init(&sm.rk_full[0][0] + i, 1); mbar_init(&sm.rv_full[0][0] + i, 1); }
     sm.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -230,10 +238,10 @@ portions_kernel(const PortionArgs a) {
       const uint64_t dq = desc_of(smem_u32(sm.q[0]), 16) + (uint32_t)(t * (H::QTILE / 16)), dk0 = desc_of(smem_u32(sm.k[0]), 16);
       ok = wait_warp(&sm.q_full[t], 0, abort_flag);
       for (int i = 0; i < n && ok; ++i) {
-        if (i > 0 && !(ok = wait_warp(&sm.s_read[t], (uint32_t)((i - 1) & 1), abort_flag))) break;     // S is in registers
         if (!(ok = wait_warp(&sm.k_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
         // P V of the block before last has read the buffer that this block's P goes to
         if (i >= 2 && !(ok = wait_warp(&sm.pv_done[t][i & 1], (uint32_t)(((i - 2) >> 1) & 1), abort_flag))) break;
+        if (i > 0 && !(ok = wait_warp(&sm.s_read[t], (uint32_t)((i - 1) & 1), abort_flag))) break;     // S is in registers
         after_sync();
         // with the scales, which came with the keys, and that buffer the softmax has all it needs once S is there
         if (lane == 0) mbar_arrive(&sm.s_full[t]);
@@ -253,8 +261,8 @@ portions_kernel(const PortionArgs a) {
       const uint64_t dv0 = desc_of(smem_u32(sm.v[0]), H::SPAN);
       const uint32_t to = __shfl_sync(0xffffffffu, tmem_o, 0) + (uint32_t)(t * DP);
       for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
         if (!(ok = wait_warp(&sm.v_full[i % H::KST], (uint32_t)((i / H::KST) & 1), abort_flag))) break;
+        if (!(ok = wait_warp(&sm.p_full[t][i & 1], (uint32_t)((i >> 1) & 1), abort_flag))) break;      // P_t is written
         after_sync();
         if (elect_one()) {
           const uint64_t dv = dv0 + (uint32_t)((i % H::KST) * (H::TILE / 16));
@@ -276,14 +284,16 @@ portions_kernel(const PortionArgs a) {
     }
   } else if (warp >= H::SOFT) {
     registers<H::R_CONV, H::R_LAUNCH>();
-    // converters: a thread takes 16 codes (a piece of a row) at a time
-    const int group = (warp - H::SOFT) / H::GW, c = threadIdx.x - 32 * (H::SOFT + group * H::GW), cw = (warp - H::SOFT) % H::GW;
-    const int pieces = a.dim / 16, per = a.page / BLK;
+    // converters: a thread takes 16 codes (a piece of a row) at a time.  The first warp of a group has the codes copied, a group of 16
+    // positions a copy, and knows the scales.
+    const int group = (warp - H::SOFT) / H::GW, c = threadIdx.x - 32 * (H::SOFT + group * H::GW);
+    const bool leads = (warp - H::SOFT) % H::GW == 0;
+    const int pieces = a.dim / 16, per = a.page / BLK, copy = BLK * a.dim;
     const int* bt = a.block_table + (size_t)req * a.max_pages;
     // pad columns: zeros, once
     for (int e = c; e < (DP / 16 - pieces) * TK; e += 32 * H::GW) {
       const int r = e % TK, p16 = pieces + e / TK;
-      for (int b = group; b < H::KST; b += 2)
+      for (int b = group; b < H::KST; b += H::NG)
         for (int s = 0; s < 2; ++s) {
           const int p = (p16 & 3) * 2 + s, at = (p16 >> 2) * H::SPAN + r * 128 + ((p ^ (r & 7)) << 4);
           *reinterpret_cast<uint4*>(sm.k[b] + at) = make_uint4(0, 0, 0, 0);
@@ -307,88 +317,144 @@ portions_kernel(const PortionArgs a) {
       }
       return (pg * a.Hkv + hk) * per + ((first_of(i) & (a.page - 1)) / BLK);
     };
-    constexpr int PIECES = DP / 16;                     // of a row at most: 8 or 4
-    constexpr int N = TK * PIECES / (32 * H::GW);       // 16-byte loads of a thread
-    // eight neighbouring threads stand on four pieces of two rows: their stores meet in no bank
-    const int piece = PIECES == 8 ? (c & 3) + 4 * (c >> 3 & 1) : c & 3, r_first = PIECES == 8 ? (c >> 2 & 1) + 2 * (c >> 4) : c >> 2;
-    const bool mine = piece < pieces;
-    constexpr int STEP = 32 * H::GW / PIECES;           // rows between a thread's loads
-    uint4 kr[N], vr[N];                                 // a block's codes, on their way while the group's block before is converted
-    auto load = [&](const int8_t* pool, uint4 (&x)[N], int id) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int r = r_first + n * STEP;
-        const int at = __shfl_sync(0xffffffffu, id, r / BLK);
-        x[n] = make_uint4(0, 0, 0, 0);
-        if (mine && at >= 0) x[n] = __ldcg(reinterpret_cast<const uint4*>(pool + ((size_t)(uint32_t)at * BLK + (r & 15)) * a.dim + piece * 16));
-      }
+    // the codes of a block: what has no page is left as it is (any byte is a code, and its weight will be 0)
+    auto fetch = [&](const int8_t* pool, uint8_t* dst, uint64_t* bar, int id) {
+      const uint32_t have = __ballot_sync(0xffffffffu, lane < GR && id >= 0);
+      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(have) * copy));
+      __syncwarp();
+      if (have >> lane & 1)
+        bulk_load(dst + lane * copy, pool + (size_t)(uint32_t)id * copy, (uint32_t)copy, bar);
     };
-    const int place0 = (piece >> 2) * H::SPAN + r_first * 128 + ((((piece & 3) * 2) ^ (r_first & 7)) << 4);      // (STEP is a multiple of 8)
-    int pg1 = look_up(group + 2), pg2 = look_up(group + 4);       // of this group's blocks behind the first
-    int id = tile_of(group, look_up(group));
-    pdl_wait();
-    const int8_t *k8 = after_wait(a.k8), *v8 = after_wait(a.v8);
-    const float *ks = after_wait(a.ks), *vs = after_wait(a.vs);
+    constexpr int PIECES = DP / 16;                     // of a row at most: 8 or 4
+    constexpr int N = TK * PIECES / (32 * H::GW);       // of a thread
+    static_assert(N == GR, "a thread has a row of each group");
+    // eight neighbouring threads take four pieces of a row and four of the next: neither their loads nor their stores meet in a bank
+    const int odd = c >> 2 & 1;
+    const int piece = PIECES == 8 ? (c & 3) + 4 * (odd ^ (c >> 3 & 1)) : c & 3, r_first = PIECES == 8 ? odd + 2 * (c >> 4) : c >> 2;
+    const bool mine = piece < pieces;
+    const int from0 = r_first * a.dim + piece * 16;
+    const int place0 = (piece >> 2) * H::SPAN + r_first * 128 + ((((piece & 3) * 2) ^ (r_first & 7)) << 4);
+    constexpr int AHEAD = H::NG * H::RD;
+    auto bar_of = [&](uint64_t (&bars)[H::NG][H::RD], int i) { return &bars[group][i / H::NG % H::RD]; };
+    auto turn_of = [&](int i) { return (uint32_t)(i / AHEAD & 1); };
+    int page_next = leads ? look_up(group + AHEAD) : -1;
+    int ids[H::RD];                                     // of the blocks under way
     float sk = 0.f, sv = 0.f;
-    load(k8, kr, id);
-    if (lane < GR && id >= 0) { sk = __ldcg(ks + id); sv = __ldcg(vs + id); }
-    load(v8, vr, id);
+    const int8_t *k8 = a.k8, *v8 = a.v8;
+    const float *ks = a.ks, *vs = a.vs;
+    int last_k = -1, last_v = -1;                       // blocks whose codes were asked for last
+    if (leads) {
+      int pages[H::RD];
+#pragma unroll
+      for (int d = 0; d < H::RD; ++d) pages[d] = look_up(group + d * H::NG);
+#pragma unroll
+      for (int d = 0; d < H::RD; ++d) ids[d] = tile_of(group + d * H::NG, pages[d]);
+      pdl_wait();
+      k8 = after_wait(a.k8), v8 = after_wait(a.v8);
+      ks = after_wait(a.ks), vs = after_wait(a.vs);
+#pragma unroll
+      for (int d = 0; d < H::RD; ++d) {
+        const int i = group + d * H::NG;
+        if (i >= n_blocks) break;
+        fetch(k8, sm.raw_k[group][d], &sm.rk_full[group][d], ids[d]);
+        if (d == 0 && lane < GR && ids[0] >= 0) { sk = __ldcg(ks + ids[0]); sv = __ldcg(vs + ids[0]); }
+        fetch(v8, sm.raw_v[group][d], &sm.rv_full[group][d], ids[d]);
+        last_k = last_v = i;
+      }
+    }
+    // A warp that gives up goes on to meet the others of its group at their barrier.
     bool ok = true;
-    for (int i = group; i < n_blocks && ok; i += 2) {
-      const int b = i % H::KST;
+    for (int i = group; i < n_blocks; i += H::NG) {
+      const int b = i % H::KST, stage = i / H::NG % H::RD;
       const uint32_t turn = (uint32_t)((i / H::KST) & 1);
-      if (i >= H::KST && !(ok = wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag))) break;
-      uint8_t* dst = sm.k[b] + place0;
+      int id = -1;
+      ok = ok && wait_warp(bar_of(sm.rk_full, i), turn_of(i), abort_flag);
+      ok = ok && (i < H::KST || wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag));
+      if (ok) {
+        const uint8_t* src = sm.raw_k[group][stage] + from0;
+        uint8_t *dst = sm.k[b] + place0, *dst2 = sm.k[b] + (place0 ^ 16);
+        if (mine) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (!mine) continue;
-        const uint32_t w[4] = {kr[n].x, kr[n].y, kr[n].z, kr[n].w};
-        uint32_t y[8];
+          for (int n = 0; n < N; ++n) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + n * copy);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { y[2 * e] = masked_xor(w[e], 0x00800080u); y[2 * e + 1] = masked_xor(w[e] >> 8, 0x00800080u); }
-        *reinterpret_cast<uint4*>(dst + n * STEP * 128) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(sm.k[b] + ((place0 ^ 16) + n * STEP * 128)) = make_uint4(y[4], y[5], y[6], y[7]);
-      }
-      if (cw == 0) {
-        const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & ((1u << GR) - 1);
-        if (lane < GR) {
-          sm.sk[i % XR][lane] = sk;
-          sm.lsv[i % XR][lane] = sv > 0.f ? log2f(sv) : 0.f;
-          sm.rsv[i % XR][lane] = sv > 0.f ? 1.f / sv : 1.f;
-          if (lane == 0) sm.missing[i % XR] = gone;
+            for (int e = 0; e < 4; ++e) { y[2 * e] = masked_xor(w[e], 0x00800080u); y[2 * e + 1] = masked_xor(w[e] >> 8, 0x00800080u); }
+            *reinterpret_cast<uint4*>(dst + n * BLK * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst2 + n * BLK * 128) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
         }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.k_full[b]);
-      const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f);      // groups whose values are 0 whatever their codes
-      const int id1 = tile_of(i + 2, pg1);
-      pg1 = pg2;
-      pg2 = look_up(i + 6);
-      load(k8, kr, id1);
-      sk = sv = 0.f;
-      if (lane < GR && id1 >= 0) { sk = __ldcg(ks + id1); sv = __ldcg(vs + id1); }
-      if (i >= H::KST && !(ok = wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag))) break;
-      dst = sm.v[b] + place0;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (!mine) continue;
-        if (nothing >> ((r_first + n * STEP) / BLK) & 1) vr[n] = make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {vr[n].x, vr[n].y, vr[n].z, vr[n].w};
-        uint32_t y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] = less1152(masked_xor(w[e], 0x64806480u));
-          y[2 * e + 1] = less1152(masked_xor(w[e] >> 8, 0x64806480u));
+        if (leads) {
+          const uint32_t gone = __ballot_sync(0xffffffffu, ids[0] < 0) & ((1u << GR) - 1);
+          const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f) & ((1u << GR) - 1);
+          if (lane < GR) {
+            sm.sk[i % XR][lane] = sk;
+            sm.lsv[i % XR][lane] = sv > 0.f ? log2f(sv) : 0.f;
+            sm.rsv[i % XR][lane] = sv > 0.f ? 1.f / sv : 1.f;
+            if (lane == 0) { sm.missing[i % XR] = gone; sm.nothing[group] = nothing; }
+          }
         }
-        *reinterpret_cast<uint4*>(dst + n * STEP * 128) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(sm.v[b] + ((place0 ^ 16) + n * STEP * 128)) = make_uint4(y[4], y[5], y[6], y[7]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.k_full[b]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.v_full[b]);
-      load(v8, vr, id1);
-      id = id1;
+      group_sync(1 + group, 32 * H::GW);                // these codes of K were read by all
+      if (leads) {
+        id = tile_of(i + AHEAD, page_next);
+        page_next = look_up(i + AHEAD + H::NG);
+        if (ok && i + AHEAD < n_blocks) {
+          fetch(k8, sm.raw_k[group][stage], &sm.rk_full[group][stage], id);
+          last_k = i + AHEAD;
+        }
+        const int next = H::RD == 1 ? id : ids[H::RD - 1];
+        sk = sv = 0.f;
+        if (lane < GR && next >= 0) { sk = __ldcg(ks + next); sv = __ldcg(vs + next); }
+      }
+      ok = ok && wait_warp(bar_of(sm.rv_full, i), turn_of(i), abort_flag);
+      ok = ok && (i < H::KST || wait_warp(&sm.v_free[b], turn ^ 1u, abort_flag));
+      if (ok) {
+        const uint32_t nothing = sm.nothing[group];
+        const uint8_t* src = sm.raw_v[group][stage] + from0;
+        uint8_t *dst = sm.v[b] + place0, *dst2 = sm.v[b] + (place0 ^ 16);
+        if (mine) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            uint4 x = *reinterpret_cast<const uint4*>(src + n * copy);
+            if (nothing >> n & 1) x = make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = less1152(masked_xor(w[e], 0x64806480u));
+              y[2 * e + 1] = less1152(masked_xor(w[e] >> 8, 0x64806480u));
+            }
+            *reinterpret_cast<uint4*>(dst + n * BLK * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst2 + n * BLK * 128) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.v_full[b]);
+      }
+      group_sync(1 + group, 32 * H::GW);
+      if (leads) {
+        if (ok && i + AHEAD < n_blocks) {
+          fetch(v8, sm.raw_v[group][stage], &sm.rv_full[group][stage], id);
+          last_v = i + AHEAD;
+        }
+#pragma unroll
+        for (int d = 0; d + 1 < H::RD; ++d) ids[d] = ids[d + 1];
+        ids[H::RD - 1] = id;
+      }
+    }
+    if (leads && !ok) {                                 // no copy is under way when the shared memory is given up
+      int never = 0;
+#pragma unroll
+      for (int d = 0; d < H::RD; ++d) {
+        if (last_k - d * H::NG >= 0) mbar_wait_warp(bar_of(sm.rk_full, last_k - d * H::NG), turn_of(last_k - d * H::NG), &never);
+        if (last_v - d * H::NG >= 0) mbar_wait_warp(bar_of(sm.rv_full, last_v - d * H::NG), turn_of(last_v - d * H::NG), &never);
+      }
     }
   } else {
     registers<H::R_SOFT, H::R_LAUNCH>();
@@ -474,51 +540,52 @@ portions_kernel(const PortionArgs a) {
             if (!(bits >> e & 1)) s[c][e] = 0xff800000u;          // -inf: its exponential below is 0
         }
       }
-      // A pass with the maximum as it is; its numbers show whether it was too low (the search for the largest score would take as long as
-      // a third of the exponentials).  Then, and in blocks before which a row has seen nothing, the maximum first and the pass again.
+      // A pass with the maximum as it is; the sums of its groups show whether it was too low (the search for the largest score would take
+      // as long as a third of the exponentials).  Then, and in blocks before which a row has seen nothing, the maximum first.
       const uint32_t t_p = t_s + TK + (uint32_t)((i & 1) * (TK / 2));
-      bool search = __any_sync(0xffffffffu, m == -INFINITY);
-      for (;;) {
-        if (search) {
-          // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
-          // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
-          float mx = -INFINITY;
+      auto raise_max = [&]() {
+        // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
+        // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
+        float mx = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < GR; ++g) {
-            const uint32_t* x = &s[g >> 1][16 * (g & 1)];
-            float y[4];
+        for (int g = 0; g < GR; ++g) {
+          const uint32_t* x = &s[g >> 1][16 * (g & 1)];
+          float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              y[e] = fmaxf(fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 4])), fmaxf(__uint_as_float(x[e + 8]), __uint_as_float(x[e + 12])));
-            const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-            mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
-          }
-          const bool grow = mx > m;
-          const float corr = grow ? ex2(m - mx) : 1.f;  // 2^-inf = 0
-          if (grow) m = mx;
-          l *= corr;
-          if (i > 0 && __any_sync(0xffffffffu, grow)) { // O as P V of the block before leaves it
-            if (!(ok = wait_warp(&sm.pv_done[t][(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1), abort_flag))) break;
-            after_sync();
-#pragma unroll 1
-            for (int c = 0; c < DP / 32; ++c) {
-              uint32_t y[32];
-              tmem_ld32(t_o + 32 * c, y);
-              ld_wait(y);
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                uint32_t z[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[16 * half + e]) * corr);
-                st16(t_o + 32 * c + 16 * half, z);
-              }
-            }
-            st_wait();
-          }
+          for (int e = 0; e < 4; ++e)
+            y[e] = fmaxf(fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 4])), fmaxf(__uint_as_float(x[e + 8]), __uint_as_float(x[e + 12])));
+          const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+          mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
         }
+        const bool grow = mx > m;
+        const float corr = grow ? ex2(m - mx) : 1.f;  // 2^-inf = 0
+        if (grow) m = mx;
+        l *= corr;
+        if (i > 0 && __any_sync(0xffffffffu, grow)) { // O as P V of the block before leaves it
+          if (!wait_warp(&sm.pv_done[t][(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1), abort_flag)) return false;
+          after_sync();
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t y[32];
+            tmem_ld32(t_o + 32 * c, y);
+            ld_wait(y);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t z[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(y[16 * half + e]) * corr);
+              st16(t_o + 32 * c + 16 * half, z);
+            }
+          }
+          st_wait();
+        }
+        return true;
+      };
+      float add;
+      auto weigh = [&]() {
         const float base = m == -INFINITY ? 0.f : m;
-        float add = 0.f;
-        uint32_t high = 0;                              // the largest two weights, as fp16
+        add = 0.f;
+        float top = -INFINITY;                          // the largest sum of a group's weights
 #pragma unroll
         for (int c = 0; c < TK / 32; ++c) {
           uint32_t packed[16];
@@ -535,18 +602,18 @@ portions_kernel(const PortionArgs a) {
               p1 = ex2(p1);
               add2(sum0, sum1, p0, p1);
               packed[8 * gg + (e >> 1)] = half2_of(p0, p1);
-              high = max_half2(high, packed[8 * gg + (e >> 1)]);
             }
-            add = fmaf(sum0 + sum1, sm.rsv[x4][g], add);
+            sum0 += sum1;
+            top = fmaxf(top, sum0);
+            add = fmaf(sum0, sm.rsv[x4][g], add);
           }
           st16(t_p + 16 * c, packed);
         }
-        if (search || !__any_sync(0xffffffffu, (high & 0xffffu) > HIGH || high >> 16 > HIGH)) {
-          l += add;
-          break;
-        }
-        search = true;
-      }
+        return __any_sync(0xffffffffu, top > HIGH);
+      };
+      if (__any_sync(0xffffffffu, m == -INFINITY)) ok = raise_max();
+      if (ok && weigh()) ok = raise_max() && (weigh(), true);
+      l += add;
       if (!ok) break;
       st_wait();
       before_sync();
@@ -601,11 +668,14 @@ portions_kernel(const PortionArgs a) {
 
 template <int DP, int NT>
 static int launch(const PortionArgs& a, int n_tiles, cudaStream_t stream) {
-  const size_t smem = sizeof(Smem<DP, NT>) + 1024;
+  constexpr size_t smem = sizeof(Smem<DP, NT>);
+  static_assert((smem + 1024) * Shape<DP, NT>::CTAS <= 228 * 1024, "shared memory");
   static SharedLimit limit;
   if (cudaError_t e = limit.raise(portions_kernel<DP, NT>, smem))
     return mlxb_fail((int)e, "kv8_portions: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-  launch_pdl(portions_kernel<DP, NT>, dim3(n_tiles, a.Hq / NT), dim3(Shape<DP, NT>::THREADS), smem, stream, a);
+  const long long blocks = (long long)n_tiles * (a.Hq / NT);
+  if (blocks > INT_MAX) return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: %d tiles of %d heads", n_tiles, a.Hq);
+  launch_pdl(portions_kernel<DP, NT>, dim3((unsigned)blocks), dim3(Shape<DP, NT>::THREADS), smem, stream, a);
   return mlxb_check_launch("kv8_portions");
 }
 
