@@ -1,6 +1,6 @@
 // Attention of prompt portions over pages in 8 bits on the 5th-generation tensor cores, bfloat16 queries, heads of up to 128.
 //
-// A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs) and walks the request's
+// A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs, and CTAs are many) and walks the request's
 // keys in blocks of 64 positions:
 //   converters  4 or 8 warps: codes (bulk copies of 16 positions each, two blocks ahead) to fp16 operands of K and V in 128-byte-swizzled
 //               shared memory, once for all NT heads; the scales of the block's four groups of 16 positions beside them
@@ -34,6 +34,7 @@ constexpr int BLK = 16;              // positions that share a scale
 constexpr int TQ = 128;              // queries of a tile
 constexpr int TK = 64;               // keys of a block
 constexpr int GR = TK / BLK;         // groups of a block
+constexpr int SMS = 148;
 constexpr int XR = 8;                // blocks whose scales are kept
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
@@ -55,16 +56,15 @@ struct PortionArgs {
 
 template <int DP, int NT>
 struct Shape {
-  static constexpr int SOFT = 4 * NT, CONV = NT == 2 && DP == 128 ? 8 : 4;      // warps
+  static constexpr int CTAS = NT == 1 && DP == 64 ? 2 : 1;        // on an SM
+  static constexpr int SOFT = 4 * NT, CONV = DP == 128 ? 8 : 4;   // warps
   // converters work in NG groups, a block each, that have RD blocks of codes each under way; KST buffers of K and of V: what fits
-  static constexpr int NG = NT == 1 && DP == 128 ? 1 : 2, RD = NG, GW = CONV / NG;
-  static constexpr int KST = NT == 1 && DP == 128 ? 2 : NT == 2 && DP == 64 ? 4 : 3;
+  static constexpr int NG = 2, RD = 2, GW = CONV / NG, KST = (NT == 2) == (DP == 64) ? 4 : 3;
   static constexpr int THREADS = 32 * (SOFT + CONV + 4);          // (the last four issue products)
   // registers a thread, at launch (what the launch bounds leave: 640 x 96, 512 x 128, 384 x 80 twice) and then by role, no more in all
-  static constexpr int R_LAUNCH = NT == 1 ? 80 : DP == 128 ? 96 : 128;
-  static constexpr int R_SOFT = NT == 1 ? 128 : 144, R_CONV = 72, R_ISSUE = NT == 1 ? 24 : 40;
+  static constexpr int R_LAUNCH = CTAS == 2 ? 80 : NT == 2 && DP == 128 ? 96 : 128;
+  static constexpr int R_SOFT = CTAS == 2 ? 128 : 144, R_CONV = 72, R_ISSUE = NT == 1 ? 24 : 40;
   static_assert(32 * (SOFT * R_SOFT + CONV * R_CONV + 4 * R_ISSUE) <= THREADS * R_LAUNCH, "registers");
-  static constexpr int CTAS = NT == 1 ? 2 : 1;
   static constexpr uint32_t COLS = NT == 1 ? 256 : 512;           // of tensor memory: S_t at 128 t, two buffers of P_t behind it; then O_t
   static constexpr int QSPAN = TQ * 128, SPAN = TK * 128;         // bytes of a tile's rows of 64 columns
   static constexpr int QTILE = QSPAN * (DP / 64), TILE = SPAN * (DP / 64), RAW = TK * DP;
@@ -707,7 +707,10 @@ MLXB_EXPORT int mlxb_kv8_portions(const PortionRecord* rec, long long bytes, cud
   const PortionArgs a{(const __nv_bfloat16*)x.q, (int)x.ldq, (const int4*)x.tiles, x.block_table, (int)x.max_pages, (int)x.n_pages, page, Hq,
                       Hkv, dim, (int)x.window, (float)x.scale, x.k8, x.v8, x.ks, x.vs, x.sinks, (__nv_bfloat16*)x.out, (int)x.ldo, vec,
                       x.status};
-  const bool pairs = (Hq / Hkv) % 2 == 0;
+  // Two heads a CTA halve the conversions, one head a CTA fills more SMs and has an SM's arithmetic for itself: pairs where single heads
+  // would be more CTAs than run at once.  256 queries of 32/8 heads of 128 at position 1000 22.8 us by single heads, 33.4 by pairs; 512 of
+  // 16/4 heads of 64 at 2000 40.4 and 44.1; but 1024 of 32/8 heads of 128 at 0 (256 CTAs or 128) 32.1 and 29.5.  A row's bits are the same.
+  const bool pairs = (Hq / Hkv) % 2 == 0 && (long long)n_tiles * Hq > SMS * (dim <= 64 ? Shape<64, 1>::CTAS : Shape<128, 1>::CTAS);
   if (dim <= 64) return pairs ? launch<64, 2>(a, n_tiles, stream) : launch<64, 1>(a, n_tiles, stream);
   return pairs ? launch<128, 2>(a, n_tiles, stream) : launch<128, 1>(a, n_tiles, stream);
 }

@@ -345,6 +345,26 @@ def test_portions(ops, spans, n_heads, heads, dim, page, window, with_sinks):
     assert float(err.max()) <= 1e-2 * float(cache.vs.max() * 127), float(err.max())
 
 
+@pytest.mark.parametrize("n_heads,heads,dim,page", [(4, 2, 64, 16), (4, 1, 128, 32), (6, 3, 48, 128), (2, 1, 16, 16), (8, 2, 112, 16)])
+@pytest.mark.parametrize("window,with_sinks", [(0, False), (45, True), (300, False)])
+def test_portions_do_not_depend_on_how_many_there_are(ops, n_heads, heads, dim, page, window, with_sinks):
+    """Where there are many tiles a block takes two heads, where there are few one: the same bits."""
+    spans = [(3, 129), (600, 40), (0, 17), (250, 140)]
+    cache = R.Cache([a + n for a, n in spans], heads, dim, page, seed=dim)
+    pos, req = R.steps(spans)
+    T = pos.numel()
+    q = (normal(dim, T, n_heads * dim) * 2).bfloat16().cuda()
+    sinks = normal(1, n_heads) if with_sinks else None
+    scale = 1.5 * dim ** -0.5
+    tiles = tiles_of(spans)
+    few, status = portions_call(ops, cache, q, tiles, n_heads, scale, window, sinks)
+    many, status2 = portions_call(ops, cache, q, torch.cat([tiles, torch.zeros(400, 4, dtype=torch.int32)]), n_heads, scale, window, sinks)
+    assert int(status.item()) == 0 and int(status2.item()) == 0
+    assert torch.equal(few, many)
+    want = R.attention(cache, q.cpu(), pos, req, n_heads, scale, window, sinks)
+    assert float((many.double().cpu() - want).abs().max()) <= 1e-2 * float(cache.vs.max() * 127)
+
+
 def test_portions_with_scales_far_apart_and_released_pages(ops):
     """Blocks of nothing, blocks of very large values, pages a window has given back, tiles that pad the list, rows of no tile."""
     n_heads, heads, dim, window = 4, 2, 64, 70
