@@ -408,6 +408,36 @@ def test_portions_and_rows_agree(ops):
     assert float((out.float() - one.float()).abs().max()) <= 1e-2 * float(cache.vs.max() * 127)
 
 
+@pytest.mark.parametrize("pad", [0, 400])      # a head a block, two heads a block
+def test_a_portion_whose_wait_runs_out(ops, pad):
+    """A build with a short limit on its waits and one arrival left out (the softmax warps are never told of a tile's first scores): the
+    kernel comes back by itself and says so, and the next launch of the same library, with the switch off, is right."""
+    from ctypes import c_int
+    from mlx_lm_b200.ops import build
+    name = "kv8_portions:MLXB_TEST_WAIT_TIMEOUT=1"
+    lib = build.load(name)
+    lib.mlxb_test_withhold_arrival.argtypes, lib.mlxb_test_withhold_arrival.restype = [c_int], c_int
+    n_heads, heads, dim = 4, 2, 128
+    spans = [(500, 200)]
+    cache = R.Cache([700], heads, dim, 16, seed=2)
+    q = normal(3, 200, n_heads * dim).bfloat16().cuda()
+    tiles = torch.cat([tiles_of(spans), torch.zeros(pad, 4, dtype=torch.int32)])
+    want, _ = portions_call(ops, cache, q, tiles, n_heads, 0.1)
+    real = ops._call
+    try:
+        ops._call = lambda lib_name, *a: real(name, *a)
+        assert lib.mlxb_test_withhold_arrival(1) == 0
+        out, status = portions_call(ops, cache, q, tiles, n_heads, 0.1)
+        torch.cuda.synchronize()
+        assert int(status.item()) == ops.ST_WAIT_TIMEOUT and bool((out == 9.0).all())
+        assert lib.mlxb_test_withhold_arrival(0) == 0
+        out, status = portions_call(ops, cache, q, tiles, n_heads, 0.1)
+        assert int(status.item()) == 0 and torch.equal(out, want)
+    finally:
+        ops._call = real
+        assert lib.mlxb_test_withhold_arrival(0) == 0
+
+
 def test_pool_beyond_31_bits(ops):
     """Codes whose offset in the pool passes 2**31."""
     heads, dim, page = 8, 128, 128
