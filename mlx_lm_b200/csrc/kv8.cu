@@ -16,6 +16,13 @@
 //         multiply-add): x decides a code by its rounding, and another order of roundings would be another code now and then.
 // read    The values at given positions, rounded to the output's type.
 //
+// Both are bound by bytes where rows are many, and by their latencies where they are few.  8192 rows of 32/8 heads of 128 at position 0,
+// turned, append and the read behind it 56 us: 234 MB, 4.1 TB/s; the append alone 46, its issue slots half used (23 million instructions).
+// (232 us with divisions in the loops and sines for each row of each head: sines are a CTA's now, and every number is formed twice, for its
+// block's largest and for its code, since registers for a block's numbers would cost a third of the warps.)  One row of a request 5.0 us,
+// 64 requests' 6.6.  A lane of the read takes 16 codes: 8, so that a warp's stores are whole runs of 512 bytes, took 1 us longer for one row
+// (twice the steps) and no less for 8192.
+//
 // Rows of a request stand together in order of position (the order in which a step lists them): the row whose predecessor is of
 // another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
 #include <type_traits>
@@ -406,13 +413,18 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   // four columns an access: whole groups of four, aligned, and pairs that are whole groups apart
   const bool wide = (!k || (fits(k, ldk, dk) && fits(v, ldv, dv))) && (!G || (fits(q, ldq, dk) && fits(q_out, ldo, dim))) &&
                     (half == 0 || (!x.interleaved && half % 4 == 0));
-  // few rows: a CTA a row, so that single tokens of different requests spread over the device; many: the rows of a block together
-  a.chunk = T <= 64 ? 1 : BLK;
+  // Few rows: a CTA a row, so that single tokens of different requests spread over the device; many: 16 rows, mostly a block's, share a
+  // CTA, its sines and its look-ups.  Microseconds with the read behind it, 32/8 heads of 128, a row a CTA and 16: 64 single tokens
+  // 6.6 and 22.6, 256 19.1 and 31.2, a portion of 256 11.0 and 10.5, of 512 14.4 and 10.7, of 8192 74 and 56.
+  a.chunk = T <= 256 ? 1 : BLK;
   const int kinds = (k ? 2 : 0) + G;
-  // heads of a CTA: as many as keep its warps busy, and more (they share the sines) while there are still four CTAs for every SM
+  // Heads of a CTA: as many as keep its warps busy, and more (they share the sines) while there are still four CTAs for every SM: a portion
+  // of 8192 56 us, 71 without the second half of the rule.
   a.heads_per_cta = kinds >= MAX_WARPS ? 1 : MAX_WARPS / kinds;
   const long long chunks = (T + a.chunk - 1) / a.chunk;
-  while (2 * a.heads_per_cta <= Hkv && 2 * a.heads_per_cta * kinds * kinds < 65536 && chunks * ((Hkv + 2 * a.heads_per_cta - 1) / (2 * a.heads_per_cta)) >= 4ll * mlxb_sm_count()) a.heads_per_cta *= 2;
+  while (2 * a.heads_per_cta <= Hkv && 2 * a.heads_per_cta * kinds * kinds < 65536 &&
+         chunks * ((Hkv + 2 * a.heads_per_cta - 1) / (2 * a.heads_per_cta)) >= 4ll * mlxb_sm_count())
+    a.heads_per_cta *= 2;
   if (a.heads_per_cta > Hkv) a.heads_per_cta = Hkv;
   const int warps = kinds * a.heads_per_cta < MAX_WARPS ? kinds * a.heads_per_cta : MAX_WARPS;
   const dim3 grid((T + a.chunk - 1) / a.chunk, (Hkv + a.heads_per_cta - 1) / a.heads_per_cta);

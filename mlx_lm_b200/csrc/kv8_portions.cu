@@ -1,15 +1,23 @@
 // Attention of prompt portions over pages in 8 bits on the 5th-generation tensor cores, bfloat16 queries, heads of up to 128.
 //
-// A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs, and CTAs are many) and walks the request's
-// keys in blocks of 64 positions:
+// A CTA takes 128 queries of NT query heads that read the same key/value head (NT 2 where heads come in pairs, and CTAs are many) and
+// walks the request's keys in blocks of 64 positions:
 //   converters  4 or 8 warps: codes (bulk copies of 16 positions each, two blocks ahead) to fp16 operands of K and V in 128-byte-swizzled
 //               shared memory, once for all NT heads; the scales of the block's four groups of 16 positions beside them
 //   issuers     2 warps a head: S_t = Q_t K^T (M 128 x N 64) into tensor memory, and O_t += P_t V with P_t read from tensor memory
 //   softmax     4 warps for each head, a thread a query: S from tensor memory, masks, running maximum and sum in float32, P as fp16 beside S
 // The softmax threads take a row of S into registers and let go of it: S of the next block is formed while they work on this one, and
 // P V of the block before as well (two buffers of P), so that the chain of a tile's blocks is its softmax alone.  (With P over S in
-// blocks of 128 keys P V and S stood in that chain: 398 us for 2048 queries of 32/8 heads of 128 at position 6144.)
+// blocks of 128 keys P V and S stood in that chain: 398 us for the 2048 queries below, against 357 at that time.)
 // Two heads of a CTA have chains of their own, and a converted block serves both.
+//
+// Bound by the softmax warps' chain.  2048 queries of 32/8 heads of 128 at position 6144: 284 us, 845 TFLOP/s of products, the tensor pipe 47 %
+// busy (64 keys and two heads: products 1344 clocks, a block 2120, of which 1670 are a thread's 64 exponentials beside another head's on the
+// same scheduler, 120 the scores' way into registers, 330 barriers), and 256 CTAs on 148 SMs.  Steps on the way: a look at every weight for one that is
+// too large 359 us, at the sums of a group of them 342; then bulk copies of the codes (converters that loaded them had taken more time for
+// addresses than for codes), a pass that is done again as code of its own (no register is copied for it) and the tiles with the most keys
+// first: 284.  A polynomial for a part of the exponentials (a
+// quarter: 282, a half: 296) moves them from one busy unit to another and was left out.
 //
 // Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
 // operation), and 128 * 2^-24 sum(q), a number of the query, comes off S in the multiply-add that scales it.  V enters as the exact
@@ -19,8 +27,8 @@
 // Scales: s = scale * sk * (q . codes) with sk the block's key scale; the weight that meets V's codes is w = exp(s) * sv, so the exponent
 // gets log2(sv), the running maximum is that of s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
 // its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) counts as codes of
-// 0 with sv 1.  The maximum follows a score only once its weight is above 2^12 (fp16 holds 2^15), so O is scaled again, by the softmax
-// threads in tensor memory, a few times a row at most.
+// 0 with sv 1.  The maximum follows the scores only once the weights of a group sum to more than 2^12 (fp16 holds 2^15), so O is scaled
+// again, by the softmax threads in tensor memory, a few times a row at most.
 //
 // Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
 // MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone.

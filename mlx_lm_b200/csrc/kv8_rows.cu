@@ -101,7 +101,7 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const int d = (2 * c + half) * 16;
-        kx[c] = d < D ? __ldcg(reinterpret_cast<const uint4*>(k8 + at + key * D + d)) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+        kx[c] = d < D ? __ldcg(reinterpret_cast<const uint4*>(k8 + at + key * D + d)) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int s = 0; s < ST; ++s)

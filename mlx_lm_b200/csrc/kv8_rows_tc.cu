@@ -12,13 +12,21 @@
 // 16 neighbouring bytes of a key where it needs four times four of them.  P leaves the first product as [keys x heads] and enters the
 // second as [heads x keys]: movmatrix turns it in two instructions.
 // A query enters as whole numbers of 16 bits, its largest at 32512, in two products (high and low byte): a number is off by 2^-16 of the
-// largest at most, the scores by 3e-5 of their spread for normal numbers, a tenth of what rounding P costs; the sums are exact.  (Codes as
-// fp16 cost three operations for every four of them: 404 instructions a tile of 128 columns, so 350.)
+// largest at most, the scores by 3e-5 of their spread for normal numbers, a tenth of what rounding P costs; the sums are exact.
 // A code of V enters as fp16 bits 00uu, u = code + 128: the subnormal number u * 2^-24, exact, for one bit operation on two codes (two for
 // the odd bytes).  The 128 comes off where the product starts: at -128 sum(p), which a product with ones gives and which is the softmax's
 // sum below as well (of the weights as they were rounded).  The scale of a key block multiplies the scores, that of a value block the
 // block's O, both in float32; P is rounded to fp16 (11 bits, 2^-12 of a weight).  The maximum that the exponentials are relative to
 // follows a score only once that is more than 8 (a factor 256) beyond it: most tiles need neither shuffles nor another scaling of O.
+//
+// Bound by the bytes of the cache, and for few or short rows by the latencies of a part: rows, pages, tiles, sums, the join.  64 rows of up to
+// 8192 positions, 32/8 heads of 128: 110 us, 5.1 TB/s (the same copies without any arithmetic: 109 to 124); one row at 131072: 56 us, 4.8 TB/s;
+// 8 rows of up to 4000: 19.3; one row of 16 heads of 64 at 520: 7.0.  What decided it, for the 64 rows: neighbouring heads of a page read at
+// about the same time (items are numbered with the heads innermost); a chunk shared by a block's four warps instead of a warp's own (157 us:
+// four times the partial sums); the next item's first tiles under way while sums are merged; the join in a kernel of its own (a block that
+// finds itself the last of a row by a counter waits for a fence, an atomic and the sums in turn).  Blocks of 8 warps, two an SM, have
+// longer waits at each merge: 129 us, but 13.0 instead of 14.6 for one row of 8192.  Three blocks an SM with rings of four tiles: 110, one
+// row at 131072 51 us, but 31.8 instead of 26.6 for 64 rows of up to 1000, 16 heads of 64 (1024 items in rounds of 444, not 592).
 #include "kv8_rows.cuh"
 
 MLXB_DEFINE_LAST_ERROR()

@@ -964,8 +964,8 @@ _kv8_rows_record = _kv8_record("14Q12qd")
 _KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
 # Parts that a row's keys are cut into at most (over the tiles of heads), and keys of a part at least (a multiple of 64).  A function of the
 # row alone: a batch has parts enough, one row alone would have more, and a row's bits must be the same in both.  Microseconds, B200, heads
-# of 128, 32/8: bfloat16, parts of 512, 1024 and 2048 keys: 64 rows of up to 8192 positions 130, 110, 112; 8 of up to 4000 18.8, 19.3, 21;
-# one of 8192 12.3, 14.6, 19; 64 of up to 1000, 16 heads of 64, 34.5, 26.5, 26.5.  Float32, parts of 128, 256 and 512 keys of a row of 8192: 8
+# of 128, 32/8: bfloat16, parts of 512 and of 1024 keys: 64 rows of up to 8192 positions 130 and 110; 8 of up to 4000 18.8 and 19.3; one of 8192
+# 12.3 and 14.6; 64 of up to 1000, 16 heads of 64, 34.5 and 26.5.  Float32, parts of 128, 256 and 512 keys of a row of 8192: 8
 # rows 179, 108, 82; one row 26.2, 19.1, 22.8; 32 rows of up to 1000, 16 heads of 64, parts of 128 and 256: 43 and 33.
 _KV8_ITEMS = {torch.float32: 148, torch.bfloat16: 4 * 148}
 _KV8_LEAST = {torch.float32: 256, torch.bfloat16: 1024}
