@@ -295,10 +295,14 @@ portions_kernel(const PortionArgs a) {
     }
   } else if (warp >= H::SOFT) {
     registers<H::R_CONV, H::R_LAUNCH>();
-    // converters: a thread takes 16 codes (a piece of a row) at a time.  The first warp of a group has the codes copied, a group of 16
-    // positions a copy, and knows the scales.
+    // converters: a thread takes 16 codes (a piece of a row) at a time.  The codes are copied 16 positions at a time.
+    // Where a CTA has one head, one warp of a group sees to the codes of K, another to those of V, a third to the scales: with one for all of
+    // it that warp was what the blocks waited for (128 queries of 32/8 heads of 128 at 8000: 117 us, 108 so).  Where it has two, the softmax is,
+    // and every warp that looks pages up takes issue slots from it (2048 queries at 6144: 290 us so, 284 with one).
     const int group = (warp - H::SOFT) / H::GW, c = threadIdx.x - 32 * (H::SOFT + group * H::GW);
-    const bool leads = (warp - H::SOFT) % H::GW == 0;
+    const int cw = (warp - H::SOFT) % H::GW;
+    constexpr int V_BY = NT == 1 ? 1 : 0, SCALES_BY = NT == 1 && H::GW > 2 ? 2 : 0;
+    const bool brings_k = cw == 0, brings_v = cw == V_BY, brings_scales = cw == SCALES_BY, leads = brings_k || brings_v || brings_scales;
     const int pieces = a.dim / 16, per = a.page / BLK, copy = BLK * a.dim;
     const int* bt = a.block_table + (size_t)req * a.max_pages;
     // pad columns: zeros, once
@@ -350,6 +354,8 @@ portions_kernel(const PortionArgs a) {
     auto turn_of = [&](int i) { return (uint32_t)(i / AHEAD & 1); };
     int page_next = leads ? look_up(group + AHEAD) : -1;
     int ids[H::RD];                                     // of the blocks under way
+#pragma unroll
+    for (int d = 0; d < H::RD; ++d) ids[d] = -1;
     float sk = 0.f, sv = 0.f;
     const int8_t *k8 = a.k8, *v8 = a.v8;
     const float *ks = a.ks, *vs = a.vs;
@@ -367,10 +373,15 @@ portions_kernel(const PortionArgs a) {
       for (int d = 0; d < H::RD; ++d) {
         const int i = group + d * H::NG;
         if (i >= n_blocks) break;
-        fetch(k8, sm.raw_k[group][d], &sm.rk_full[group][d], ids[d]);
-        if (d == 0 && lane < GR && ids[0] >= 0) { sk = __ldcg(ks + ids[0]); sv = __ldcg(vs + ids[0]); }
-        fetch(v8, sm.raw_v[group][d], &sm.rv_full[group][d], ids[d]);
-        last_k = last_v = i;
+        if (brings_k) {
+          fetch(k8, sm.raw_k[group][d], &sm.rk_full[group][d], ids[d]);
+          last_k = i;
+        }
+        if (d == 0 && brings_scales && lane < GR && ids[0] >= 0) { sk = __ldcg(ks + ids[0]); sv = __ldcg(vs + ids[0]); }
+        if (brings_v) {
+          fetch(v8, sm.raw_v[group][d], &sm.rv_full[group][d], ids[d]);
+          last_v = i;
+        }
       }
     }
     // A warp that gives up goes on to meet the others of its group at their barrier.
@@ -379,6 +390,10 @@ portions_kernel(const PortionArgs a) {
       const int b = i % H::KST, stage = i / H::NG % H::RD;
       const uint32_t turn = (uint32_t)((i / H::KST) & 1);
       int id = -1;
+      if (leads) {
+        id = tile_of(i + AHEAD, page_next);
+        page_next = look_up(i + AHEAD + H::NG);
+      }
       ok = ok && wait_warp(bar_of(sm.rk_full, i), turn_of(i), abort_flag);
       ok = ok && (i < H::KST || wait_warp(&sm.k_free[b], turn ^ 1u, abort_flag));
       if (ok) {
@@ -396,7 +411,7 @@ portions_kernel(const PortionArgs a) {
             *reinterpret_cast<uint4*>(dst2 + n * BLK * 128) = make_uint4(y[4], y[5], y[6], y[7]);
           }
         }
-        if (leads) {
+        if (brings_scales) {
           const uint32_t gone = __ballot_sync(0xffffffffu, ids[0] < 0) & ((1u << GR) - 1);
           const uint32_t nothing = __ballot_sync(0xffffffffu, sv == 0.f) & ((1u << GR) - 1);
           if (lane < GR) {
@@ -411,15 +426,13 @@ portions_kernel(const PortionArgs a) {
         if (lane == 0) mbar_arrive(&sm.k_full[b]);
       }
       group_sync(1 + group, 32 * H::GW);                // these codes of K were read by all
-      if (leads) {
-        id = tile_of(i + AHEAD, page_next);
-        page_next = look_up(i + AHEAD + H::NG);
-        if (ok && i + AHEAD < n_blocks) {
-          fetch(k8, sm.raw_k[group][stage], &sm.rk_full[group][stage], id);
-          last_k = i + AHEAD;
-        }
-        const int next = H::RD == 1 ? id : ids[H::RD - 1];
+      if (brings_k && ok && i + AHEAD < n_blocks) {
+        fetch(k8, sm.raw_k[group][stage], &sm.rk_full[group][stage], id);
+        last_k = i + AHEAD;
+      }
+      if (brings_scales) {                              // of the group's next block
         sk = sv = 0.f;
+        const int next = H::RD == 1 ? id : ids[H::RD - 1];
         if (lane < GR && next >= 0) { sk = __ldcg(ks + next); sv = __ldcg(vs + next); }
       }
       ok = ok && wait_warp(bar_of(sm.rv_full, i), turn_of(i), abort_flag);
@@ -449,17 +462,15 @@ portions_kernel(const PortionArgs a) {
         if (lane == 0) mbar_arrive(&sm.v_full[b]);
       }
       group_sync(1 + group, 32 * H::GW);
-      if (leads) {
-        if (ok && i + AHEAD < n_blocks) {
-          fetch(v8, sm.raw_v[group][stage], &sm.rv_full[group][stage], id);
-          last_v = i + AHEAD;
-        }
-#pragma unroll
-        for (int d = 0; d + 1 < H::RD; ++d) ids[d] = ids[d + 1];
-        ids[H::RD - 1] = id;
+      if (brings_v && ok && i + AHEAD < n_blocks) {
+        fetch(v8, sm.raw_v[group][stage], &sm.rv_full[group][stage], id);
+        last_v = i + AHEAD;
       }
+#pragma unroll
+      for (int d = 0; d + 1 < H::RD; ++d) ids[d] = ids[d + 1];
+      ids[H::RD - 1] = id;
     }
-    if (leads && !ok) {                                 // no copy is under way when the shared memory is given up
+    if (!ok) {                                 // no copy is under way when the shared memory is given up
       int never = 0;
 #pragma unroll
       for (int d = 0; d < H::RD; ++d) {
