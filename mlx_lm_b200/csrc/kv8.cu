@@ -93,7 +93,7 @@ struct AppendArgs {
   int half, interleaved;
   float mscale;
   const int *positions, *token_req, *block_table;
-  int max_pages, n_pages, page;
+  int n_req, max_pages, n_pages, page;
   int8_t *k8, *v8;
   float *ks, *vs;
   int* status;
@@ -138,7 +138,7 @@ append_kernel(const AppendArgs a) {
       const int n = behind ? __ffs(behind) : BLK;           // (a block ends after 16 rows at most: with a chunk of 16 within the 32)
       const int lp = p / a.page;
       int pg = -1;
-      if (p < 0 || lp >= a.max_pages) {
+      if (r >= a.n_req || p < 0 || lp >= a.max_pages) {
         if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
       } else {
         pg = a.block_table[(size_t)r * a.max_pages + lp];
@@ -381,7 +381,7 @@ struct AppendRecord {
   int8_t *k8, *v8;
   float *ks, *vs;
   int* status;
-  long long dtype, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, half, interleaved, max_pages, n_pages, page;
+  long long dtype, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, half, interleaved, n_req, max_pages, n_pages, page;
   double mscale;
 };
 
@@ -409,7 +409,8 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   const size_t item = dtype == MLXB_F32 ? 4 : 2;
   auto fits = [&](const void* p, int ld, int d) { return (((uintptr_t)p) % (4 * item)) == 0 && ld % 4 == 0 && d % 4 == 0; };
   AppendArgs a{k, v, q, q_out, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, freq, half, (int)x.interleaved, (float)x.mscale,
-               x.positions, x.token_req, x.block_table, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status, 1, 1};
+               x.positions, x.token_req, x.block_table, (int)x.n_req, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status, 1,
+               1};
   // four columns an access: whole groups of four, aligned, and pairs that are whole groups apart
   const bool wide = (!k || (fits(k, ldk, dk) && fits(v, ldv, dv))) && (!G || (fits(q, ldq, dk) && fits(q_out, ldo, dim))) &&
                     (half == 0 || (!x.interleaved && half % 4 == 0));
@@ -453,8 +454,8 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
 // A warp takes a row (its page looked up once), a lane 16 codes at a time, keys and values: 16 bytes in, 32 or 64 out.
 template <typename T>
 __global__ void __launch_bounds__(256)
-read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ block_table, int max_pages,
-            int n_pages, int page, int Hkv, int dim, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, T* k_out,
+read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ block_table, int n_req,
+            int max_pages, int n_pages, int page, int Hkv, int dim, const int8_t* k8, const int8_t* v8, const float* ks, const float* vs, T* k_out,
             int ldk, T* v_out, int ldv, int n_rows, int vec, int* status) {
   const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int r = t < n_rows ? token_req[t] : -1;
@@ -462,7 +463,7 @@ read_kernel(const int* __restrict__ positions, const int* __restrict__ token_req
   if (r >= 0) {
     p = positions[t];
     const int lp = p / page;
-    if (p >= 0 && lp < max_pages) pg = block_table[(size_t)r * max_pages + lp];
+    if (r < n_req && p >= 0 && lp < max_pages) pg = block_table[(size_t)r * max_pages + lp];
     if (pg < 0 || pg >= n_pages) {
       if (lane == 0) atomicOr(status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
       pg = -1;
@@ -517,7 +518,7 @@ struct ReadRecord {
   const float *ks, *vs;
   void *k_out, *v_out;
   int* status;
-  long long dtype, max_pages, n_pages, page, Hkv, dim, ldk, ldv, n_rows;
+  long long dtype, n_req, max_pages, n_pages, page, Hkv, dim, ldk, ldv, n_rows;
 };
 
 // k_out, v_out [n_rows, Hkv * dim]: what the pages stand for at position positions[t] of request token_req[t] (< 0: row left as it is;
@@ -525,7 +526,7 @@ struct ReadRecord {
 MLXB_EXPORT int mlxb_kv8_read(const ReadRecord* rec, long long bytes, cudaStream_t stream) {
   if (!rec || bytes != sizeof(ReadRecord)) return mlxb_fail(MLXB_BAD_ARG, "kv8_read: a record of %lld bytes", bytes);
   const ReadRecord& x = *rec;
-  const int dtype = (int)x.dtype, max_pages = (int)x.max_pages, n_pages = (int)x.n_pages, page = (int)x.page, Hkv = (int)x.Hkv;
+  const int dtype = (int)x.dtype, n_req = (int)x.n_req, max_pages = (int)x.max_pages, n_pages = (int)x.n_pages, page = (int)x.page, Hkv = (int)x.Hkv;
   const int dim = (int)x.dim, ldk = (int)x.ldk, ldv = (int)x.ldv, n_rows = (int)x.n_rows;
   const int *positions = x.positions, *token_req = x.token_req, *block_table = x.block_table;
   const int8_t *k8 = x.k8, *v8 = x.v8;
@@ -542,10 +543,10 @@ MLXB_EXPORT int mlxb_kv8_read(const ReadRecord* rec, long long bytes, cudaStream
   const int vec = !(((uintptr_t)k_out | (uintptr_t)v_out) & 15) && (ldk * item) % 16 == 0 && (ldv * item) % 16 == 0;
   const dim3 grid((unsigned)((n_rows + 7) / 8));
   if (dtype == MLXB_F32)
-    launch_pdl(read_kernel<float>, grid, dim3(256), 0, stream, positions, token_req, block_table, max_pages, n_pages, page, Hkv, dim, k8,
-               v8, ks, vs, (float*)k_out, ldk, (float*)v_out, ldv, n_rows, vec, status);
+    launch_pdl(read_kernel<float>, grid, dim3(256), 0, stream, positions, token_req, block_table, n_req, max_pages, n_pages, page, Hkv, dim,
+               k8, v8, ks, vs, (float*)k_out, ldk, (float*)v_out, ldv, n_rows, vec, status);
   else
-    launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, positions, token_req, block_table, max_pages, n_pages, page, Hkv,
-               dim, k8, v8, ks, vs, (__nv_bfloat16*)k_out, ldk, (__nv_bfloat16*)v_out, ldv, n_rows, vec, status);
+    launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, positions, token_req, block_table, n_req, max_pages, n_pages, page,
+               Hkv, dim, k8, v8, ks, vs, (__nv_bfloat16*)k_out, ldk, (__nv_bfloat16*)v_out, ldv, n_rows, vec, status);
   return mlxb_check_launch("kv8_read");
 }

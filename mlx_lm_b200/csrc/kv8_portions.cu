@@ -53,7 +53,7 @@ struct PortionArgs {
   int ldq;
   const int4* tiles;
   const int* block_table;
-  int max_pages, n_pages, page, Hq, Hkv, dim, window;
+  int n_tokens, n_req, max_pages, n_pages, page, Hq, Hkv, dim, window;
   float scale;
   const int8_t *k8, *v8;
   const float *ks, *vs, *sinks;
@@ -197,6 +197,10 @@ portions_kernel(const PortionArgs a) {
   const int4 tile = a.tiles[gridDim.x / heads - 1 - by_tile];      // a portion's last tiles, the longest, first
   if (tile.y <= 0) return;
   const int row0 = tile.x, n_rows = min(tile.y, TQ), req = tile.z, pos0 = tile.w;
+  if (row0 < 0 || row0 > a.n_tokens - n_rows || req < 0 || req >= a.n_req || pos0 < 0 || pos0 > INT_MAX - TQ) {
+    if (threadIdx.x == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
+    return;
+  }
   const int h0 = (blockIdx.x - by_tile * heads) * NT, hk = h0 / (a.Hq / a.Hkv);
   const int last_pos = pos0 + n_rows - 1;
   const int first_key = a.window > 0 && pos0 - a.window + 1 > 0 ? pos0 - a.window + 1 : 0;
@@ -709,7 +713,7 @@ struct PortionRecord {
   const float *ks, *vs, *sinks;
   void* out;
   int* status;
-  long long ldq, n_tiles, max_pages, n_pages, page, Hq, Hkv, dim, window, ldo;
+  long long ldq, n_tokens, n_tiles, n_req, max_pages, n_pages, page, Hq, Hkv, dim, window, ldo;
   double scale;
 };
 
@@ -726,7 +730,7 @@ MLXB_EXPORT int mlxb_kv8_portions(const PortionRecord* rec, long long bytes, cud
   if (((uintptr_t)x.k8 | (uintptr_t)x.v8 | (uintptr_t)x.tiles) & 15)
     return mlxb_fail(MLXB_BAD_ARG, "kv8_portions: pools and tiles must be 16-byte aligned");
   const int vec = (x.ldq % 8 == 0 && !((uintptr_t)x.q & 15) ? 1 : 0) | (x.ldo % 8 == 0 && !((uintptr_t)x.out & 15) ? 2 : 0);
-  const PortionArgs a{(const __nv_bfloat16*)x.q, (int)x.ldq, (const int4*)x.tiles, x.block_table, (int)x.max_pages, (int)x.n_pages, page, Hq,
+  const PortionArgs a{(const __nv_bfloat16*)x.q, (int)x.ldq, (const int4*)x.tiles, x.block_table, (int)x.n_tokens, (int)x.n_req, (int)x.max_pages, (int)x.n_pages, page, Hq,
                       Hkv, dim, (int)x.window, (float)x.scale, x.k8, x.v8, x.ks, x.vs, x.sinks, (__nv_bfloat16*)x.out, (int)x.ldo, vec,
                       x.status};
   // Two heads a CTA halve the conversions, one head a CTA fills more SMs and has an SM's arithmetic for itself: pairs where single heads

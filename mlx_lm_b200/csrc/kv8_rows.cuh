@@ -18,7 +18,7 @@ struct RowsArgs {
   const void* q;
   int ldq;
   const int *rows, *positions, *token_req, *block_table;
-  int max_pages, n_pages, page, Hq, Hkv, dim, window;
+  int n_tokens, n_req, max_pages, n_pages, page, Hq, Hkv, dim, window;
   float scale;
   const int8_t *k8, *v8;
   const float *ks, *vs, *sinks;
@@ -40,15 +40,16 @@ struct RowSpan { int tok, req, pos, first, n; };      // first: a multiple of 16
 
 __device__ __forceinline__ RowSpan span_of(const RowsArgs& a, int tok, int req, int pos) {
   RowSpan s{tok, req, pos, 0, 0};
-  if (req < 0 || pos < 0 || pos / a.page >= a.max_pages) return s;      // a row that pads the step, or one out of range
+  if (req < 0 || req >= a.n_req || pos < 0 || pos / a.page >= a.max_pages) return s;      // a row that pads the step, or one out of range
   const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
   s.first = lo & ~(BLK - 1);
   s.n = pos + 1 - s.first;
   return s;
 }
 __device__ __forceinline__ RowSpan row_span(const RowsArgs& a, int i) {
-  const int tok = a.rows ? a.rows[i] : i, req = a.token_req[tok], pos = a.positions[tok];
-  return span_of(a, tok, req, pos);
+  const int tok = a.rows ? a.rows[i] : i;
+  if ((unsigned)tok >= (unsigned)a.n_tokens) return RowSpan{0, a.n_req, 0, 0, 0};
+  return span_of(a, tok, a.token_req[tok], a.positions[tok]);
 }
 __device__ __forceinline__ int chunks_of(const RowsArgs& a, int n) {
   if (n == 0) return 0;
@@ -213,15 +214,15 @@ struct RowsRecord {
   int* counters;
   void* out;
   int* status;
-  long long ldq, max_pages, n_pages, page, Hq, Hkv, dim, window, most_chunks, least_chunk, ldo, n_rows;
+  long long ldq, n_tokens, n_req, max_pages, n_pages, page, Hq, Hkv, dim, window, most_chunks, least_chunk, ldo, n_rows;
   double scale;
 };
 
 static inline int rows_args(const RowsRecord* rec, long long bytes, const char* what, RowsArgs& a) {
   if (!rec || bytes != sizeof(RowsRecord)) return mlxb_fail(MLXB_BAD_ARG, "%s: a record of %lld bytes", what, bytes);
   const RowsRecord& x = *rec;
-  a = RowsArgs{x.q, (int)x.ldq, x.rows, x.positions, x.token_req, x.block_table, (int)x.max_pages, (int)x.n_pages, (int)x.page, (int)x.Hq,
-               (int)x.Hkv, (int)x.dim, (int)x.window, (float)x.scale, x.k8, x.v8, x.ks, x.vs, x.sinks, x.partial, x.counters,
+  a = RowsArgs{x.q, (int)x.ldq, x.rows, x.positions, x.token_req, x.block_table, (int)x.n_tokens, (int)x.n_req, (int)x.max_pages, (int)x.n_pages,
+               (int)x.page, (int)x.Hq, (int)x.Hkv, (int)x.dim, (int)x.window, (float)x.scale, x.k8, x.v8, x.ks, x.vs, x.sinks, x.partial, x.counters,
                (int)x.most_chunks, (int)x.least_chunk, x.out, (int)x.ldo, (int)x.n_rows, x.status};
   if (a.n_rows > ROWS_MOST) return mlxb_fail(MLXB_BAD_ARG, "%s: %d rows, a launch takes %d", what, a.n_rows, ROWS_MOST);
   if (a.Hkv <= 0 || a.Hq <= 0 || a.Hq % a.Hkv) return mlxb_fail(MLXB_BAD_ARG, "%s: %d query heads over %d key/value heads", what, a.Hq, a.Hkv);

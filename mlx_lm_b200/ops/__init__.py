@@ -824,23 +824,24 @@ def kv8_supported(page: int, head_dim: int) -> bool:
 _I8, _I32, _F32T, _BF16T = torch.int8, torch.int32, torch.float32, torch.bfloat16
 
 
-def _kv8_pools(k8, v8, k_scale, v_scale, block_table, what: str):
-    """Shape of the pages ``[n_pages, heads, page, head_dim]`` of a cache in 8 bits."""
-    shape = k8.shape
-    if (len(shape) == 4 and k8.dtype is _I8 and v8.dtype is _I8 and k_scale.dtype is _F32T and v_scale.dtype is _F32T
+def _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, what: str):
+    """Shape of the pages ``[n_pages, heads, page, head_dim]`` of a cache in 8 bits, and that of the block table."""
+    shape, table = k8.shape, block_table.shape
+    if (len(shape) == 4 and len(table) == 2 and k8.dtype is _I8 and v8.dtype is _I8 and k_scale.dtype is _F32T and v_scale.dtype is _F32T
             and block_table.dtype is _I32 and k8.is_cuda and v8.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
             and v8.shape == shape and k8.is_contiguous() and v8.is_contiguous() and kv8_supported(shape[2], shape[3])):
         n_pages, Hkv, page, Dh = shape
         want = (n_pages, Hkv, page // KV8_BLOCK)
         if (k_scale.shape == want and v_scale.shape == want and k_scale.is_contiguous() and v_scale.is_contiguous()
-                and block_table.dim() == 2 and block_table.is_contiguous()):
-            return shape
+                and block_table.is_contiguous() and status.dtype is _I32 and status.is_cuda):
+            return (*shape, *table)
     # something is wrong: say what
     _need(k8, torch.int8, what + " key codes")
     _need(v8, torch.int8, what + " value codes")
     _need(k_scale, torch.float32, what + " key scales")
     _need(v_scale, torch.float32, what + " value scales")
     _need(block_table, torch.int32, what + " block_table")
+    _need(status, torch.int32, what + " status")
     if len(shape) != 4 or v8.shape != shape or not (k8.is_contiguous() and v8.is_contiguous()):
         raise KernelError(f"{what}: codes {tuple(k8.shape)} and {tuple(v8.shape)}: contiguous [n_pages, heads, page, head_dim], both the same")
     n_pages, Hkv, page, Dh = shape
@@ -883,7 +884,7 @@ def _kv8_rows_ints(positions, token_req, n: int, what: str) -> None:
     raise KernelError(f"{what}: {positions.numel()} positions and {token_req.numel()} requests for {n} rows, contiguous ones")
 
 
-_kv8_append_record = _kv8_record("13Q16qd")
+_kv8_append_record = _kv8_record("13Q17qd")
 
 
 def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale, status, stream, freq=None, interleaved: bool = False,
@@ -900,8 +901,9 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
     (old / new))`` where it grows.  New codes are ``rint(x * (1 / scale))`` within -127 .. 127.  A NaN is held as 0 and an infinity as the
     largest code; ``status`` then gets ``ST_NOT_FINITE``.
 
-    Rows of a request stand together in order of position; ``token_req`` < 0: a row of no request, which is left out."""
-    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_append")
+    Rows of a request stand together in order of position; ``token_req`` < 0: a row of no request, which is left out (as is a row of a request
+    that the block table has no row for, with ``ST_POSITION_RANGE`` in ``status``)."""
+    n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_append")
     if (k is None) != (v is None) or (k is None and q is None) or (q is None) != (q_out is None):
         raise KernelError("kv8_append: keys and values go together, and queries with their output")
     dtype = (q if k is None else k).dtype
@@ -934,18 +936,18 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
     record, size = _kv8_append_record(
         kp, vp, qp, op, fp, positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), status.data_ptr(), code, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, Dh, half, interleaved,
-        block_table.shape[1], n_pages, page, mscale)
+        n_req, max_pages, n_pages, page, mscale)
     _call("kv8", "mlxb_kv8_append", _KV8_ARGS, record, size, stream)
 
 
-_kv8_read_record = _kv8_record("10Q9q")
+_kv8_read_record = _kv8_record("10Q10q")
 
 
 def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out, v_out, status, stream) -> None:
     """What the pages stand for: row ``t`` of ``k_out`` and ``v_out`` (``[n, heads * head_dim]``, float32 or bfloat16) becomes the key and
     the value (``code * scale``) at position ``positions[t]`` of request ``token_req[t]`` (< 0: the row is left as it is; a position without
     a page: zeros, and ``status`` says so)."""
-    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_read")
+    n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_read")
     dtype = k_out.dtype
     code = dtype_code(dtype)
     n, nk, ldk = _kv8_matrix(k_out, dtype, "kv8_read k_out")
@@ -955,12 +957,12 @@ def kv8_read(positions, token_req, block_table, k8, v8, k_scale, v_scale, k_out,
     _kv8_rows_ints(positions, token_req, n, "kv8_read")
     record, size = _kv8_read_record(
         positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), status.data_ptr(), code, block_table.shape[1], n_pages, page, Hkv, Dh, ldk,
-        ldv, n)
+        v_scale.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), status.data_ptr(), code, n_req, max_pages, n_pages, page, Hkv, Dh, ldk, ldv,
+        n)
     _call("kv8", "mlxb_kv8_read", _KV8_ARGS, record, size, stream)
 
 
-_kv8_rows_record = _kv8_record("14Q12qd")
+_kv8_rows_record = _kv8_record("14Q14qd")
 _KV8_TILE_HEADS = {torch.float32: 4, torch.bfloat16: 8}      # query heads that a block of csrc/kv8_rows.cu, kv8_rows_tc.cu takes
 # Parts that a row's keys are cut into at most (over the tiles of heads), and keys of a part at least (a multiple of 64).  A function of the
 # row alone: a batch has parts enough, one row alone would have more, and a row's bits must be the same in both.  Microseconds, B200, heads
@@ -1008,7 +1010,7 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
     sizes, one pair for each stream on which calls may overlap; ``max_len``: no row's position reaches it (a row beyond the block table is
     left out, with a bit in ``status``).  ``sinks``: float32 ``[n_heads]``, one more term of each head's softmax denominator.  Rows of no
     request (``token_req`` < 0) are left as they are.  A row's bits depend on its own request, ``max_len`` and the heads alone."""
-    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_rows")
+    n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_attention_rows")
     dtype = q.dtype
     dtype_code(dtype)
     T, width, ldq = _kv8_matrix(q, dtype, "kv8_attention_rows q")
@@ -1019,6 +1021,8 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
     n, rp = T, 0
     if rows is not None:
         _need(rows, torch.int32, "kv8_attention_rows rows")
+        if not rows.is_contiguous():
+            raise KernelError(f"kv8_attention_rows: rows of strides {rows.stride()}")
         n, rp = rows.numel(), rows.data_ptr()
     floats, tickets = kv8_rows_scratch(n, n_heads, Hkv, Dh, max_len)
     if (scratch.dtype is not _F32T or counters.dtype is not _I32 or not scratch.is_cuda or not counters.is_cuda or scratch.numel() < floats
@@ -1037,11 +1041,11 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         record, size = _kv8_rows_record(
             qp + t * ldq * item, r, pp + 4 * t, tp + 4 * t, block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), sk, scratch.data_ptr(), counters.data_ptr(), op + t * ldo * item, status.data_ptr(), ldq,
-            block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, most, least, ldo, min(n - a, KV8_ROWS_MOST), scale)
+            T - t, n_req, max_pages, n_pages, page, n_heads, Hkv, Dh, window, most, least, ldo, min(n - a, KV8_ROWS_MOST), scale)
         _call(lib, name, _KV8_ARGS, record, size, stream)
 
 
-_kv8_portion_record = _kv8_record("10Q10qd")
+_kv8_portion_record = _kv8_record("10Q12qd")
 
 
 def kv8_portions_supported(dtype, head_dim: int, scale: float = 1.0) -> bool:
@@ -1053,8 +1057,9 @@ def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale,
                            status, stream, sinks=None) -> None:
     """Attention of prompt portions over pages in 8 bits, bfloat16, heads of up to 128.  ``tiles``: int32 ``[n_tiles, 4]`` = (row of the
     tile's first token in ``q`` and ``out``, its queries (0: skipped) up to ``PREFILL_TILE``, row of the block table, position of the first
-    query); window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are."""
-    n_pages, Hkv, page, Dh = _kv8_pools(k8, v8, k_scale, v_scale, block_table, "kv8_attention_portions")
+    query); window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are; a tile of rows or of a request that do not
+    exist is left out and reported (``ST_POSITION_RANGE``)."""
+    n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_attention_portions")
     T, width, ldq = _kv8_matrix(q, _BF16T, "kv8_attention_portions q")
     To, wo, ldo = _kv8_matrix(out, _BF16T, "kv8_attention_portions out")
     if n_heads <= 0 or n_heads % Hkv or To != T or width != n_heads * Dh or wo != width:
@@ -1067,7 +1072,7 @@ def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale,
     sk = _sinks(sinks, n_heads, "kv8_attention_portions") or 0
     record, size = _kv8_portion_record(
         q.data_ptr(), tiles.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), sk,
-        out.data_ptr(), status.data_ptr(), ldq, n_tiles, block_table.shape[1], n_pages, page, n_heads, Hkv, Dh, window, ldo, scale)
+        out.data_ptr(), status.data_ptr(), ldq, T, n_tiles, n_req, max_pages, n_pages, page, n_heads, Hkv, Dh, window, ldo, scale)
     _call("kv8_portions", "mlxb_kv8_portions", _KV8_ARGS, record, size, stream)
 
 

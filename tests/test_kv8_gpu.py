@@ -493,6 +493,39 @@ def test_on_another_stream(ops):
     assert float((out.float() - 2.0).abs().max()) <= 2e-2
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_requests_rows_and_tiles_that_do_not_exist(ops, dtype):
+    """A request the block table has no row for, a row of a list or of a tile beyond the queries: left out and reported."""
+    n_heads, heads, dim = 4, 2, 64
+    cache = R.Cache([40, 30], heads, dim, 16, seed=1)
+    pos = torch.tensor([39, 5, 29], dtype=torch.int32)
+    req = torch.tensor([0, 2, 1], dtype=torch.int32)         # the table has rows 0 and 1
+    q = normal(2, 3, n_heads * dim).to(dtype).cuda()
+    out, status = rows_call(ops, cache, q, pos, req, n_heads, 0.2)
+    right, _ = rows_call(ops, cache, q, pos, torch.tensor([0, -1, 1], dtype=torch.int32), n_heads, 0.2)
+    assert int(status.item()) == ops.ST_POSITION_RANGE and torch.equal(out, right)
+    out, status = rows_call(ops, cache, q, pos, req, n_heads, 0.2, rows=torch.tensor([2, 3, -1, 1 << 30], dtype=torch.int32))
+    assert int(status.item()) == ops.ST_POSITION_RANGE and torch.equal(out[2], right[2]) and bool((out[:2] == 9.0).all())
+
+    dev = cache.cuda()
+    before = [t.clone() for t in dev]
+    x = normal(3, 3, heads * dim).to(dtype).cuda()
+    s = word()
+    ops.kv8_append(x, x, torch.tensor([3, 4, 5], dtype=torch.int32).cuda(), torch.tensor([2, 2, 7], dtype=torch.int32).cuda(),
+                   cache.table.cuda(), *dev, s, stream())
+    assert int(s.item()) == ops.ST_POSITION_RANGE and all(torch.equal(a, b) for a, b in zip(dev, before))
+    s = word()
+    k, v = torch.full((3, heads * dim), 9.0, dtype=dtype, device="cuda"), torch.full((3, heads * dim), 9.0, dtype=dtype, device="cuda")
+    ops.kv8_read(pos.cuda(), req.cuda(), cache.table.cuda(), *dev, k, v, s, stream())
+    assert int(s.item()) == ops.ST_POSITION_RANGE and not k[1].any() and not v[1].any() and k[0].any() and k[2].any()
+    if dtype == torch.bfloat16:
+        good = torch.tensor([(0, 2, 0, 38)], dtype=torch.int32)
+        want, _ = portions_call(ops, cache, q, good, n_heads, 0.2)
+        bad = torch.tensor([(2, 2, 0, 3), (-1, 1, 0, 3), (2, 1, 2, 3), (2, 1, -1, 3), (2, 1, 0, -1), (2, 1, 0, 2 ** 31 - 1)], dtype=torch.int32)
+        out, status = portions_call(ops, cache, q, torch.cat([bad, good]), n_heads, 0.2)
+        assert int(status.item()) == ops.ST_POSITION_RANGE and torch.equal(out, want)
+
+
 def test_refusals(ops):
     cache = R.Cache([40], 2, 64, 16, seed=1)
     k8, v8, ks, vs = cache.cuda()
@@ -507,7 +540,7 @@ def test_refusals(ops):
            dict(block_table=table.long()), dict(block_table=table[0]), dict(positions=pos[:2]), dict(token_req=req.cpu()),
            dict(freq=torch.ones(33, device="cuda")), dict(freq=torch.ones(4, device="cuda").double()), dict(q=x), dict(q=x, q_out=x[:, :64]),
            dict(q=x[:, :120], q_out=x.clone()), dict(q=x, q_out=x), dict(k=torch.zeros(4, 144, device="cuda")),
-           dict(k8=k8.view(-1, 2, 8, 64), v8=v8.view(-1, 2, 8, 64))]
+           dict(k8=k8.view(-1, 2, 8, 64), v8=v8.view(-1, 2, 8, 64)), dict(status=s.cpu()), dict(status=s.float())]
     for change in bad:
         with pytest.raises(ops.KernelError):
             ops.kv8_append(**{**good, **change})
@@ -525,7 +558,8 @@ def test_refusals(ops):
     ops.kv8_attention_rows(**rows)
     for change in [dict(n_heads=3), dict(q=q[:, :128]), dict(out=q.bfloat16()), dict(q=q.half(), out=q.half()), dict(scratch=rows["scratch"][:-1]),
                    dict(counters=rows["counters"][:-1]), dict(positions=pos[:3]), dict(sinks=torch.zeros(3, device="cuda")),
-                   dict(rows=torch.zeros(2, device="cuda")), dict(counters=rows["counters"].float())]:
+                   dict(rows=torch.zeros(2, device="cuda")), dict(counters=rows["counters"].float()),
+                   dict(rows=torch.zeros(4, dtype=torch.int32, device="cuda")[::2])]:
         with pytest.raises(ops.KernelError):
             ops.kv8_attention_rows(**{**rows, **change})
     q = q.bfloat16()
