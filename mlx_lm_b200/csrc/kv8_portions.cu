@@ -17,7 +17,8 @@
 // too large 359 us, at the sums of a group of them 342; then bulk copies of the codes (converters that loaded them had taken more time for
 // addresses than for codes), a pass that is done again as code of its own (no register is copied for it) and the tiles with the most keys
 // first: 284.  A polynomial for a part of the exponentials (a
-// quarter: 282, a half: 296) moves them from one busy unit to another and was left out.
+// quarter: 282, a half: 296) moves them from one busy unit to another and was left out; so were two threads a query, 32 keys of a block
+// each: 304, the pair has to agree on its maximum in every block.
 //
 // Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
 // operation), and 128 * 2^-24 sum(q), a number of the query, comes off S in the multiply-add that scales it.  V enters as the exact
