@@ -973,9 +973,6 @@ _KV8_ITEMS = {torch.float32: 148, torch.bfloat16: 4 * 148}
 _KV8_LEAST = {torch.float32: 256, torch.bfloat16: 1024}
 
 
-_KV8_F32_ROWS = ("kv8_rows", "mlxb_kv8_rows")
-
-
 @functools.lru_cache(maxsize=64)
 def kv8_rows_library(dtype, head_dim: int) -> str:
     """The library whose kernel takes single queries of this type (one for each head size in bfloat16)."""
@@ -1002,6 +999,15 @@ def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, 
     return floats, tickets
 
 
+@functools.lru_cache(maxsize=256)
+def _kv8_rows_launch(dtype, n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
+    """What a call's sizes decide: library and launcher, parts of a row, sizes of its scratch memory."""
+    dtype_code(dtype)
+    _, most, least = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
+    return (kv8_rows_library(dtype, head_dim), "mlxb_kv8_rows" if dtype == torch.float32 else "mlxb_kv8_rows_tc", most, least,
+            *kv8_rows_scratch(n_rows, n_heads, n_kv_heads, head_dim, max_len))
+
+
 def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_scale, out, n_heads: int, scale: float, window: int,
                        scratch, counters, max_len: int, status, stream, rows=None, sinks=None) -> None:
     """Attention of single queries (decode steps) over pages in 8 bits: row ``t`` of ``q`` and ``out`` (``[T, n_heads * head_dim]``, float32
@@ -1012,7 +1018,6 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
     request (``token_req`` < 0) are left as they are.  A row's bits depend on its own request, ``max_len`` and the heads alone."""
     n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_attention_rows")
     dtype = q.dtype
-    dtype_code(dtype)
     T, width, ldq = _kv8_matrix(q, dtype, "kv8_attention_rows q")
     To, wo, ldo = _kv8_matrix(out, dtype, "kv8_attention_rows out")
     if n_heads <= 0 or n_heads % Hkv or To != T or width != n_heads * Dh or wo != width:
@@ -1024,16 +1029,14 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         if not rows.is_contiguous():
             raise KernelError(f"kv8_attention_rows: rows of strides {rows.stride()}")
         n, rp = rows.numel(), rows.data_ptr()
-    floats, tickets = kv8_rows_scratch(n, n_heads, Hkv, Dh, max_len)
+    lib, name, most, least, floats, tickets = _kv8_rows_launch(dtype, n, n_heads, Hkv, Dh, max_len)
     if (scratch.dtype is not _F32T or counters.dtype is not _I32 or not scratch.is_cuda or not counters.is_cuda or scratch.numel() < floats
             or counters.numel() < tickets):
         _need(scratch, torch.float32, "kv8_attention_rows scratch")
         _need(counters, torch.int32, "kv8_attention_rows counters")
         raise KernelError(f"kv8_attention_rows: scratch of {scratch.numel()} floats and {counters.numel()} counters, {floats} and "
                           f"{tickets} are needed")
-    sk = _sinks(sinks, n_heads, "kv8_attention_rows") or 0
-    _, most, least = _kv8_plan(dtype, n_heads, Hkv, max_len)
-    lib, name = (_KV8_F32_ROWS if dtype is _F32T else (kv8_rows_library(dtype, Dh), "mlxb_kv8_rows_tc"))
+    sk = 0 if sinks is None else _sinks(sinks, n_heads, "kv8_attention_rows")
     qp, op, pp, tp, item = q.data_ptr(), out.data_ptr(), positions.data_ptr(), token_req.data_ptr(), q.element_size()
     for a in range(0, n, KV8_ROWS_MOST):
         # the rows of the list from its a-th on, or rows a and on of the tensors
