@@ -33,6 +33,76 @@ __device__ __forceinline__ void codes4(uint32_t c, float (&f)[4]) {
   for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(c, 0x4b000000u, 0x7540 + i)) - 8388736.f;
 }
 
+// A CTA's sums for the heads h0 .. h0 + nh - 1 of an item, in shared memory: m[h], l[h], o[h * dim + d].  A row of one chunk goes
+// to the output; else the sums go to scratch memory and the CTA that comes last for the (row, tile) adds them up in the order of the
+// chunks.  Every thread of the CTA calls it; weights: [most_chunks + 1][HT].
+__device__ __forceinline__ void finish_item(const RowsArgs& a, const Item& x, int tiles, int h0, int nh, const float* m, const float* l,
+                                            const float* o, float* weights, int* last) {
+  const int D = a.dim;
+  float* out = (float*)a.out + (size_t)x.row.tok * a.ldo + (size_t)h0 * D;
+  if (x.n_chunks == 1) {
+    for (int e = threadIdx.x; e < nh * D; e += blockDim.x) {
+      const int h = e / D;
+      const float total = a.sinks ? l[h] + expf(a.sinks[h0 + h] - m[h]) : l[h];
+      out[e] = total != 0.f ? o[e] / total : 0.f;
+    }
+    return;
+  }
+  const size_t per = (size_t)HT * (D + 2);
+  const size_t slot = ((size_t)x.index * tiles + x.tile) * a.most_chunks;
+  float* mine = a.partial + (slot + x.chunk) * per;
+  for (int e = threadIdx.x; e < nh * D; e += blockDim.x) __stcg(mine + 2 * HT + e, o[e]);
+  if (threadIdx.x < nh) {
+    __stcg(mine + threadIdx.x, m[threadIdx.x]);
+    __stcg(mine + HT + threadIdx.x, l[threadIdx.x]);
+  }
+  __threadfence();
+  __syncthreads();
+  int* counter = a.counters + (size_t)x.index * tiles + x.tile;
+  if (threadIdx.x == 0) *last = atomicAdd(counter, 1) == x.n_chunks - 1;
+  __syncthreads();
+  if (!*last) return;
+  __threadfence();
+  if (threadIdx.x == 0) *counter = 0;
+  const float* all = a.partial + slot * per;
+  // weights of the chunks: exp(m_c - M) / total, a warp a head, a lane a chunk
+  const int lane = threadIdx.x & 31;
+  for (int h = threadIdx.x >> 5; h < nh; h += blockDim.x >> 5) {
+    float top = -INFINITY, total = 0.f;
+    bool odd = false;                                  // fmaxf leaves NaN out
+    for (int c = lane; c < x.n_chunks; c += 32) {
+      const float mc = __ldcg(all + c * per + h);
+      odd |= mc != mc;
+      top = fmaxf(top, mc);
+    }
+    top = __any_sync(0xffffffffu, odd) ? NAN : warp_max(top);
+    if (top == -INFINITY) top = 0.f;                  // no key at all has a page: zeros
+    for (int c = lane; c < x.n_chunks; c += 32) {
+      const float w = expf(__ldcg(all + c * per + h) - top);
+      weights[c * HT + h] = w;
+      total = fmaf(w, __ldcg(all + c * per + HT + h), total);
+    }
+    total = warp_sum(total);
+    if (a.sinks) total += expf(a.sinks[h0 + h] - top);
+    if (lane == 0) weights[a.most_chunks * HT + h] = total != 0.f ? 1.f / total : 0.f;
+  }
+  __syncthreads();
+  for (int e = 4 * threadIdx.x; e < nh * D; e += 4 * blockDim.x) {
+    const int h = e / D;
+    const float* w = weights + h;
+    const float* p = all + 2 * HT + e;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+    for (int c = 0; c < x.n_chunks; ++c) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + c * per));
+      const float wc = w[c * HT];
+      sum.x = fmaf(wc, v.x, sum.x); sum.y = fmaf(wc, v.y, sum.y); sum.z = fmaf(wc, v.z, sum.z); sum.w = fmaf(wc, v.w, sum.w);
+    }
+    const float r = w[a.most_chunks * HT];
+    out[e] = sum.x * r; out[e + 1] = sum.y * r; out[e + 2] = sum.z * r; out[e + 3] = sum.w * r;
+  }
+}
+
 // DP: the head size or the power of two above it; HN: query heads of an item at most (1 or 4).
 template <int DP, int HN>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -241,7 +311,7 @@ rows_kernel(const RowsArgs a, int tiles, int group_tiles) {
       if (d == 0) { fin_m[h] = top; fin_l[h] = tot; }
     }
     __syncthreads();
-    finish_item<float>(a, x, tiles, HT, h0, nh, fin_m, fin_l, fin_o, weights, &last, 1.f, [](float v) { return expf(v); });
+    finish_item(a, x, tiles, h0, nh, fin_m, fin_l, fin_o, weights, &last);
     __syncthreads();
   }
 }

@@ -1,5 +1,4 @@
-// What the kernels for single queries over pages in 8 bits share: how the rows' keys are cut into items, and how an item's result
-// becomes a row of the output.
+// What the kernels for single queries over pages in 8 bits share: their arguments, and how the rows' keys are cut into items.
 //
 // A row (one query of each head, at position p of its request) sees keys max(0, p - window + 1) .. p.  They are cut into chunks that
 // begin at multiples of 16 positions; how many there are goes by the row's own number of keys and by the numbers of heads, never by
@@ -129,78 +128,6 @@ __device__ __forceinline__ int page_of(const RowsArgs& a, const int* bt, int key
   if (pg >= 0 && pg < a.n_pages) return pg;
   atomicOr(a.status, pg < 0 ? MLXB_ST_POSITION_RANGE : MLXB_ST_PAGE_RANGE);
   return -1;
-}
-
-// A CTA's sums for the heads h0 .. h0 + nh - 1 of an item, in shared memory: m[h], l[h], o[h * dim + d].  A row of one chunk goes
-// to the output; else the sums go to scratch memory and the CTA that comes last for the (row, tile) adds them up in the order of the
-// chunks.  Exp(x): the exponential in the unit of m.  Every thread of the CTA calls it; weights: [most_chunks][nh].
-template <typename T, typename Exp>
-__device__ __forceinline__ void finish_item(const RowsArgs& a, const Item& x, int tiles, int tile_heads, int h0, int nh, const float* m,
-                                            const float* l, const float* o, float* weights, int* last, float sink_unit, Exp exp_) {
-  const int D = a.dim;
-  T* out = (T*)a.out + (size_t)x.row.tok * a.ldo + (size_t)h0 * D;
-  if (x.n_chunks == 1) {
-    for (int e = threadIdx.x; e < nh * D; e += blockDim.x) {
-      const int h = e / D;
-      const float total = a.sinks ? l[h] + exp_(a.sinks[h0 + h] * sink_unit - m[h]) : l[h];
-      out[e] = from_f<T>(total != 0.f ? o[e] / total : 0.f);
-    }
-    return;
-  }
-  const size_t per = (size_t)tile_heads * (D + 2);
-  const size_t slot = ((size_t)x.index * tiles + x.tile) * a.most_chunks;
-  float* mine = a.partial + (slot + x.chunk) * per;
-  for (int e = threadIdx.x; e < nh * D; e += blockDim.x) __stcg(mine + 2 * tile_heads + e, o[e]);
-  if (threadIdx.x < nh) {
-    __stcg(mine + threadIdx.x, m[threadIdx.x]);
-    __stcg(mine + tile_heads + threadIdx.x, l[threadIdx.x]);
-  }
-  __threadfence();
-  __syncthreads();
-  int* counter = a.counters + (size_t)x.index * tiles + x.tile;
-  if (threadIdx.x == 0) *last = atomicAdd(counter, 1) == x.n_chunks - 1;
-  __syncthreads();
-  if (!*last) return;
-  __threadfence();
-  if (threadIdx.x == 0) *counter = 0;
-  const float* all = a.partial + slot * per;
-  // weights of the chunks: exp(m_c - M) / total, a warp a head, a lane a chunk
-  const int lane = threadIdx.x & 31;
-  for (int h = threadIdx.x >> 5; h < nh; h += blockDim.x >> 5) {
-    float top = -INFINITY, total = 0.f;
-    bool odd = false;                                  // fmaxf leaves NaN out
-    for (int c = lane; c < x.n_chunks; c += 32) {
-      const float mc = __ldcg(all + c * per + h);
-      odd |= mc != mc;
-      top = fmaxf(top, mc);
-    }
-    top = __any_sync(0xffffffffu, odd) ? NAN : warp_max(top);
-    if (top == -INFINITY) top = 0.f;                  // no key at all has a page: zeros
-    for (int c = lane; c < x.n_chunks; c += 32) {
-      const float w = exp_(__ldcg(all + c * per + h) - top);
-      weights[c * tile_heads + h] = w;
-      total = fmaf(w, __ldcg(all + c * per + tile_heads + h), total);
-    }
-    total = warp_sum(total);
-    if (a.sinks) total += exp_(a.sinks[h0 + h] * sink_unit - top);
-    if (lane == 0) weights[a.most_chunks * tile_heads + h] = total != 0.f ? 1.f / total : 0.f;
-  }
-  __syncthreads();
-  for (int e = 4 * threadIdx.x; e < nh * D; e += 4 * blockDim.x) {
-    const int h = e / D;
-    const float* w = weights + h;
-    const float* p = all + 2 * tile_heads + e;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 16
-    for (int c = 0; c < x.n_chunks; ++c) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + c * per));
-      const float wc = w[c * tile_heads];
-      sum.x = fmaf(wc, v.x, sum.x); sum.y = fmaf(wc, v.y, sum.y); sum.z = fmaf(wc, v.z, sum.z); sum.w = fmaf(wc, v.w, sum.w);
-    }
-    const float r = w[a.most_chunks * tile_heads];
-    out[e] = from_f<T>(sum.x * r); out[e + 1] = from_f<T>(sum.y * r);
-    out[e + 2] = from_f<T>(sum.z * r); out[e + 3] = from_f<T>(sum.w * r);
-  }
 }
 
 // Arguments of the entry points as one record of 8-byte fields: the caller fills it in a tenth of the time that as many arguments of a
