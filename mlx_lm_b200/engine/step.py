@@ -45,6 +45,13 @@ class Workspace:
         self.device = device
         self._bufs: Dict[tuple, torch.Tensor] = {}
         self.generation = 0      # goes up whenever a buffer is made or replaced (its address changes)
+        self._asked: set = set()
+        self.moved = False       # since ``watch``: a buffer that had been handed out was replaced by a larger one
+
+    def watch(self) -> None:
+        """From here on note whether a buffer is replaced after it has been handed out (``moved``): launches in between then name
+        memory that is no longer kept."""
+        self._asked, self.moved = set(), False
 
     def get(self, tag: str, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
         key = (tag, cols, dtype)
@@ -53,9 +60,11 @@ class Workspace:
             cap = max(rows, 16)
             if buf is not None:
                 cap = max(cap, 2 * buf.shape[0])
+                self.moved |= key in self._asked
             buf = torch.zeros((cap, cols), dtype=dtype, device=self.device)   # rows a step never writes stay finite
             self._bufs[key] = buf
             self.generation += 1
+        self._asked.add(key)
         return buf[:rows]
 
     def flat(self, tag: str, n: int, dtype: torch.dtype, most: Optional[int] = None) -> torch.Tensor:
@@ -67,9 +76,11 @@ class Workspace:
             room = max(n, 1024, 2 * (buf.numel() if buf is not None else 0))
             if most is not None:
                 room = max(n, min(room, most))
+            self.moved |= buf is not None and key in self._asked
             buf = torch.zeros(room, dtype=dtype, device=self.device)   # zero: ticket counters of kernels start from zero
             self._bufs[key] = buf
             self.generation += 1
+        self._asked.add(key)
         return buf
 
     def nbytes(self) -> int:
@@ -527,15 +538,18 @@ class Engine:
             self.n_replayed += 1
             self.last_calls = plan[1]
             return plan[2]
+        self.ws.watch()
         ops.start_recording()
         try:
             logits = self.model.run(ctx)
         finally:
             calls = ops.stop_recording()
+        self.last_calls = calls
+        if self.ws.moved:
+            return logits      # some of these launches name a buffer that was replaced behind them: the next such step is recorded
         if len(self._plans) >= 256:
             self._plans.clear()
         self._plans[shape] = (self.ws.generation, calls, logits)
-        self.last_calls = calls
         return logits
 
     # ------------------------------------------------------------------ decode steps as CUDA graphs

@@ -141,20 +141,21 @@ def paged_attention_kv8(ctx, q, cache, o, n_heads: int, head_dim: int, scale: fl
     """``paged_attention`` over pages in 8 bits: single rows to their kernel, portions to theirs, or row by row where that does
     not take them (float32, heads above 128)."""
     pools = (cache.k, cache.v, cache.k_scale, cache.v_scale)
-
-    def by_row(n: int, rows) -> None:
-        floats, tickets = ops.kv8_rows_scratch(n, n_heads, cache.k.shape[1], head_dim, ctx.max_len)
-        ops.kv8_attention_rows(q, ctx.positions, ctx.token_req, cache.block_table, *pools, o, n_heads, scale, window,
-                               ctx.ws.flat("kv8_partial", floats, torch.float32), ctx.ws.flat("kv8_tickets", tickets, torch.int32),
-                               ctx.max_len, ctx.status, ctx.stream, rows=rows, sinks=sinks)
-
-    if ctx.n_portion and ctx.portion_tiles is not None and ops.kv8_portions_supported(q.dtype, head_dim, scale):
+    in_tiles = ctx.n_portion and ctx.portion_tiles is not None and ops.kv8_portions_supported(q.dtype, head_dim, scale)
+    by_row = [(ctx.n_portion, ctx.portion_rows)] if ctx.n_portion and not in_tiles else []
+    if ctx.n_single:
+        by_row.append((ctx.n_single, ctx.single_rows))
+    if in_tiles:
         ops.kv8_attention_portions(q, ctx.portion_tiles, ctx.n_portion_tiles, cache.block_table, *pools, o, n_heads, scale, window,
                                    ctx.status, ctx.stream, sinks=sinks)
-    elif ctx.n_portion:
-        by_row(ctx.n_portion, ctx.portion_rows)
-    if ctx.n_single:
-        by_row(ctx.n_single, ctx.single_rows)
+    if by_row:
+        # Scratch memory is asked for once a layer, for the larger of the launches: a second, larger request would replace the memory that
+        # the first launch was given, and a recorded step would go on naming it.
+        floats, tickets = ops.kv8_rows_scratch(max(n for n, _ in by_row), n_heads, cache.k.shape[1], head_dim, ctx.max_len)
+        partial, counters = ctx.ws.flat("kv8_partial", floats, torch.float32), ctx.ws.flat("kv8_tickets", tickets, torch.int32)
+        for _, rows in by_row:
+            ops.kv8_attention_rows(q, ctx.positions, ctx.token_req, cache.block_table, *pools, o, n_heads, scale, window, partial, counters,
+                                   ctx.max_len, ctx.status, ctx.stream, rows=rows, sinks=sinks)
 
 
 register_part("mixer", "attention", Attention)

@@ -1,0 +1,91 @@
+"""Scratch memory of attention over 8-bit pages: every launch of a step works on memory that is kept, and a step whose buffers moved
+while it was recorded is not issued again from that recording.  No GPU needed."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from mlx_lm_b200 import ops
+from mlx_lm_b200.engine.step import Engine, Workspace
+from mlx_lm_b200.parts import mixers
+
+
+def layer(monkeypatch, ws, dtype, n_portion, n_single, tiles, head_dim=64):
+    """The launches of one layer's attention: name, scratch and counters of each."""
+    calls = []
+    monkeypatch.setattr(ops, "kv8_attention_rows", lambda q, pos, req, table, k8, v8, ks, vs, out, n_heads, scale, window, scratch, counters,
+                        max_len, status, stream, rows=None, sinks=None: calls.append(("rows", rows, scratch, counters)))
+    monkeypatch.setattr(ops, "kv8_attention_portions", lambda *a, **kw: calls.append(("portions", None, None, None)))
+    ctx = SimpleNamespace(ws=ws, n_portion=n_portion, n_single=n_single, portion_rows="portion rows", single_rows="single rows",
+                          portion_tiles="tiles" if tiles else None, n_portion_tiles=2, positions=None, token_req=None, max_len=300,
+                          status=None, stream=0)
+    cache = SimpleNamespace(k=torch.zeros(2, 2, 16, head_dim, dtype=torch.int8), v=None, k_scale=torch.zeros(1), v_scale=None, block_table=None)
+    mixers.paged_attention_kv8(ctx, torch.zeros(1, dtype=dtype), cache, None, 4, head_dim, 0.1, 0)
+    return calls
+
+
+@pytest.mark.parametrize("n_portion,n_single", [(128, 192), (192, 128), (64, 64), (0, 192), (256, 0)])
+def test_launches_of_a_step_share_memory_that_is_kept(monkeypatch, n_portion, n_single):
+    ws = Workspace("cpu")
+    calls = [c for _ in range(2) for c in layer(monkeypatch, ws, torch.float32, n_portion, n_single, tiles=True)]
+    assert [c[0] for c in calls] == ["rows"] * (2 * ((n_portion > 0) + (n_single > 0)))
+    floats, tickets = ops.kv8_rows_scratch(max(n_portion, n_single), 4, 2, 64, 300)
+    kept = {b.data_ptr() for b in ws._bufs.values()}
+    for _, _, scratch, counters in calls:
+        assert scratch.data_ptr() in kept and counters.data_ptr() in kept
+        assert scratch.numel() >= floats and counters.numel() >= tickets
+
+
+def test_which_launch_takes_what(monkeypatch):
+    ws = Workspace("cpu")
+    assert [c[:2] for c in layer(monkeypatch, ws, torch.bfloat16, 128, 64, tiles=True)] == [("portions", None), ("rows", "single rows")]
+    assert [c[:2] for c in layer(monkeypatch, ws, torch.bfloat16, 128, 0, tiles=True)] == [("portions", None)]
+    both = [("rows", "portion rows"), ("rows", "single rows")]
+    assert [c[:2] for c in layer(monkeypatch, ws, torch.bfloat16, 128, 64, tiles=True, head_dim=256)] == both
+    assert [c[:2] for c in layer(monkeypatch, ws, torch.float32, 128, 64, tiles=False)] == both
+
+
+def test_a_buffer_that_moves_after_it_was_handed_out():
+    ws = Workspace("cpu")
+    ws.watch()
+    ws.flat("a", 10, torch.float32)
+    ws.flat("a", 500, torch.float32)          # (fits)
+    ws.get("b", 3, 4, torch.float32)
+    ws.get("c", 40, 4, torch.float32)
+    assert not ws.moved
+    ws.watch()
+    ws.flat("a", 5000, torch.float32)         # grows at its first use: nobody has the old one
+    ws.get("b", 300, 4, torch.float32)
+    assert not ws.moved
+    ws.get("b", 3000, 4, torch.float32)
+    assert ws.moved
+    ws.watch()
+    ws.flat("a", 5000, torch.float32)
+    assert not ws.moved
+    ws.flat("a", 50000, torch.float32)
+    assert ws.moved
+
+
+def test_no_recording_of_a_step_whose_buffers_moved(monkeypatch):
+    """A model whose second launch asks for more of the same buffer than its first."""
+    monkeypatch.setattr(ops, "replay", lambda calls: ran.append("replayed"))
+    ran = []
+
+    class Model:
+        def run(self, ctx):
+            ran.append("ran")
+            for n in sizes:
+                b = engine.ws.flat("tag", n, torch.float32)
+                ops._recording.append(b.data_ptr())
+            return "logits"
+
+    engine = Engine.__new__(Engine)
+    engine.ws, engine.model, engine.use_replay, engine._plans, engine.n_replayed = Workspace("cpu"), Model(), True, {}, 0
+    sizes = (2000, 4000)
+    for want in ("ran", "ran", "replayed", "replayed"):
+        assert engine._run(None, ("shape",)) == "logits"
+        assert ran[-1] == want
+        for gen, calls, _ in engine._plans.values():
+            if gen == engine.ws.generation:
+                assert set(calls) <= {b.data_ptr() for b in engine.ws._bufs.values()}
+    assert engine.n_replayed == 2
