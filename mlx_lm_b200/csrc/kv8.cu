@@ -155,7 +155,11 @@ append_kernel(const AppendArgs a) {
   }
   __syncthreads();
   const int nl = n_lead;
-  if (nl == 0) return;
+  if (nl == 0) {
+    // a step of rows of no request alone must not end before its predecessor has: what comes next waits for this grid only
+    if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+    return;
+  }
   // (rows between two leaders that are of no request get an angle nobody uses)
   if (a.half > 0) {
     const int di = blockDim.x / a.half, dj = blockDim.x - di * a.half, n = (last_row - row0) * a.half;

@@ -196,9 +196,14 @@ portions_kernel(const PortionArgs a) {
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int heads = a.Hq / NT, by_tile = blockIdx.x / heads;
   const int4 tile = a.tiles[gridDim.x / heads - 1 - by_tile];      // a portion's last tiles, the longest, first
-  if (tile.y <= 0) return;
+  // (a list without one tile to do must not end before its predecessor has: what comes next waits for this grid only)
+  if (tile.y <= 0) {
+    if (blockIdx.x == 0) pdl_wait();
+    return;
+  }
   const int row0 = tile.x, n_rows = min(tile.y, TQ), req = tile.z, pos0 = tile.w;
   if (row0 < 0 || row0 > a.n_tokens - n_rows || req < 0 || req >= a.n_req || pos0 < 0 || pos0 > INT_MAX - TQ) {
+    if (blockIdx.x == 0) pdl_wait();
     if (threadIdx.x == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
     return;
   }
