@@ -23,8 +23,10 @@
 // 64 requests' 6.6.  A lane of the read takes 16 codes: 8, so that a warp's stores are whole runs of 512 bytes, took 1 us longer for one row
 // (twice the steps) and no less for 8192.
 //
-// Rows of a request stand together in order of position (the order in which a step lists them): the row whose predecessor is of
-// another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
+// Rows of a request stand together in order of position without gaps (the order in which a step lists them): the row whose predecessor
+// is of another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
+// A row that goes back, or leaves positions out inside its block, would lead a block that has a leader already: it and the rows that
+// follow on from it are left out and reported.
 #include <type_traits>
 
 #include "common.cuh"
@@ -128,6 +130,7 @@ append_kernel(const AppendArgs a) {
     int rb = __shfl_up_sync(0xffffffffu, r, 1), pb = __shfl_up_sync(0xffffffffu, p, 1);
     if (lane == 0) { rb = row0 > 0 ? a.token_req[row0 - 1] : -1; pb = row0 > 0 ? a.positions[row0 - 1] : 0; }
     const bool fresh = r < 0 || rb != r || pb != p - 1 || (p & (BLK - 1)) == 0;
+    const bool astray = rb == r && pb != p - 1 && (p <= pb || p / BLK == pb / BLK);
     const uint32_t starts = __ballot_sync(0xffffffffu, fresh);
     pos_of[lane] = p;
     const bool leads = fresh && r >= 0 && lane < a.chunk;
@@ -138,7 +141,7 @@ append_kernel(const AppendArgs a) {
       const int n = behind ? __ffs(behind) : BLK;           // (a block ends after 16 rows at most: with a chunk of 16 within the 32)
       const int lp = p / a.page;
       int pg = -1;
-      if (r >= a.n_req || p < 0 || lp >= a.max_pages) {
+      if (r >= a.n_req || p < 0 || lp >= a.max_pages || (astray && a.k)) {
         if (a.k && blockIdx.y == 0) atomicOr(a.status, MLXB_ST_POSITION_RANGE);
       } else {
         pg = a.block_table[(size_t)r * a.max_pages + lp];

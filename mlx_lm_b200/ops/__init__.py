@@ -901,8 +901,9 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
     (old / new))`` where it grows.  New codes are ``rint(x * (1 / scale))`` within -127 .. 127.  A NaN is held as 0 and an infinity as the
     largest code; ``status`` then gets ``ST_NOT_FINITE``.
 
-    Rows of a request stand together in order of position; ``token_req`` < 0: a row of no request, which is left out (as is a row of a request
-    that the block table has no row for, with ``ST_POSITION_RANGE`` in ``status``)."""
+    Rows of a request stand together in order of position, without gaps inside a block; ``token_req`` < 0: a row of no request, which is
+    left out.  A row of a request that the block table has no row for, and one that goes back or leaves a gap (with those that follow on
+    from it), is left out too, with ``ST_POSITION_RANGE`` in ``status``."""
     n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_append")
     if (k is None) != (v is None) or (k is None and q is None) or (q is None) != (q_out is None):
         raise KernelError("kv8_append: keys and values go together, and queries with their output")
