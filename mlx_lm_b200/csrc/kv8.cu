@@ -27,6 +27,8 @@
 // is of another request or block leads its block's rows.  A leader's block and head are one warp's, so nothing is written by two warps.
 // A row that goes back, or leaves positions out inside its block, would lead a block that has a leader already: it and the rows that
 // follow on from it are left out and reported.
+#include <float.h>
+
 #include <type_traits>
 
 #include "common.cuh"
@@ -367,7 +369,7 @@ append_kernel(const AppendArgs a) {
         if (odd) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float most = 127.f * scale;          // (of an infinity the largest code)
+            const float most = fminf(127.f * scale, FLT_MAX);      // (of an infinity the largest code; 127 * (FLT_MAX / 127) rounds up)
             x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -most), most);
             y[e] = y[e] != y[e] ? 0.f : fminf(fmaxf(y[e], -most), most);
           }

@@ -52,3 +52,26 @@ def test_rows_out_of_order_or_with_gaps(ops, dtype, ahead, positions, enter):
         assert torch.equal(got.cpu(), want)
     assert int(status.item()) == (0 if len(enter) == len(positions) else ops.ST_POSITION_RANGE)
     assert torch.equal(q_out, q)                # (queries write to rows of their own: any order will do)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("aligned", [True, False])
+def test_infinities_beside_the_largest_number(ops, dtype, aligned):
+    """An infinity is held as the largest code of its sign whatever else its block holds, up to the type's largest number."""
+    top = torch.finfo(dtype).max
+    x = torch.zeros(4, 33)
+    x[0, :4] = torch.tensor([top, float("inf"), float("-inf"), float("nan")])
+    x[1, 1] = -top
+    x[2, 0] = float("inf")
+    x = x.to(dtype).cuda()
+    k = x[:, :32].contiguous() if aligned else x[:, :32]
+    cache = R.Cache([4], 1, 32, 16, seed=1, filled=False)
+    dev, status = cache.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    pos, req = R.steps([(0, 4)])
+    ops.kv8_append(k, k, pos.cuda(), req.cuda(), cache.table.cuda(), *dev, status, ops.current_stream())
+    page = int(cache.table[0, 0])
+    for codes, scale in ((dev[0], dev[2]), (dev[1], dev[3])):
+        row = codes[page, 0].cpu()
+        assert row[0, :5].tolist() == [127, 127, -127, 0, 0] and row[1, :3].tolist() == [0, -127, 0] and int(row[2, 0]) == 127
+        assert float(scale[page, 0, 0]) == float(torch.tensor(top) / 127)
+    assert int(status.item()) == ops.ST_NOT_FINITE
