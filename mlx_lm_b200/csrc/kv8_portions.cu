@@ -27,8 +27,9 @@
 // largest number.
 // Scales: s = scale * sk * (q . codes) with sk the block's key scale; the weight that meets V's codes is w = exp(s) * sv, so the exponent
 // gets log2(sv), the running maximum is that of s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
-// its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) counts as codes of
-// 0 with sv 1.  The maximum follows the scores only once the weights of a group sum to more than 2^12 (fp16 holds 2^15), so O is scaled
+// its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) adds to the sum alone, which
+// it does beside the others, with a maximum of its own (as codes of 0 with some sv it would raise the maximum that the weights of groups
+// of small values are stored relative to, and these would round away).  The maximum follows the scores only once the weights of a group sum to more than 2^12 (fp16 holds 2^15), so O is scaled
 // again, by the softmax threads in tensor memory, a few times a row at most.
 //
 // Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
@@ -87,7 +88,7 @@ struct Smem {
   alignas(1024) uint8_t v[H::KST][H::TILE];
   alignas(1024) uint8_t raw_k[H::NG][H::RD][H::RAW], raw_v[H::NG][H::RD][H::RAW];      // codes as they come
   float sk[XR][GR], lsv[XR][GR], rsv[XR][GR];           // of the last blocks: key scale, log2 and reciprocal of the value scale
-  uint32_t missing[XR];                                 // groups without a page
+  uint32_t marks[XR];                                   // bit g: group g has no page; bit 8 + g: its values are 0
   uint32_t nothing[H::NG];                              // groups whose values are 0 whatever their codes
   alignas(8) uint64_t q_full[NT], k_full[H::KST], k_free[H::KST], v_full[H::KST], v_free[H::KST];
   uint64_t s_full[NT], s_read[NT], p_full[NT][2], pv_done[NT][2], drained[2 * NT];
@@ -428,7 +429,7 @@ portions_kernel(const PortionArgs a) {
             sm.sk[i % XR][lane] = sk;
             sm.lsv[i % XR][lane] = sv > 0.f ? log2f(sv) : 0.f;
             sm.rsv[i % XR][lane] = sv > 0.f ? 1.f / sv : 1.f;
-            if (lane == 0) { sm.missing[i % XR] = gone; sm.nothing[group] = nothing; }
+            if (lane == 0) { sm.marks[i % XR] = gone | (nothing & ~gone) << 8; sm.nothing[group] = nothing; }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -544,12 +545,13 @@ portions_kernel(const PortionArgs a) {
       if (lane == 0) mbar_arrive(&sm.q_full[t]);
     }
     float m = -INFINITY, l = 0.f;      // the running maximum of s + log2(sv), in units of the exponent; the sum
+    float m0 = -INFINITY, l0 = 0.f;    // the maximum of s, and the sum, of groups whose values are 0
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
       const int key0 = (kb_lo + i) * TK, x4 = i % XR;
       if (!(ok = wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
       after_sync();
-      const uint32_t gone = sm.missing[x4];
+      const uint32_t marks = sm.marks[x4], gone = marks & 0xffu;
       uint32_t s[TK / 32][32];
 #pragma unroll
       for (int c = 0; c < TK / 32; ++c) tmem_ld32(t_s + 32 * c, s[c]);
@@ -570,6 +572,27 @@ portions_kernel(const PortionArgs a) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!(bits >> e & 1)) s[c][e] = 0xff800000u;          // -inf: its exponential below is 0
+        }
+      }
+      if (marks >> 8) {
+        // groups whose values are 0: into their own sum, and out of what follows
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+          if (!(marks >> (8 + g) & 1)) continue;
+          uint32_t* x = &s[g >> 1][16 * (g & 1)];
+          const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f);
+          float top = __uint_as_float(x[0]);
+#pragma unroll
+          for (int e = 1; e < BLK; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+          top = fmaxf((top - off) * f, m0);
+          const float base = top == -INFINITY ? 0.f : top, k = fmaf(-off, f, -base);
+          l0 *= ex2(m0 - base);
+          m0 = top;
+#pragma unroll
+          for (int e = 0; e < BLK; ++e) {
+            l0 += ex2(fmaf(__uint_as_float(x[e]), f, k));
+            x[e] = 0xff800000u;
+          }
         }
       }
       // A pass with the maximum as it is; the sums of its groups show whether it was too low (the search for the largest score would take
@@ -656,6 +679,7 @@ portions_kernel(const PortionArgs a) {
     if (ok) ok = wait_warp(&sm.pv_done[t][(n_blocks - 1) & 1], (uint32_t)(((n_blocks - 1) >> 1) & 1), abort_flag);
     if (ok) {
       after_sync();
+      l += l0 * (m != -INFINITY ? ex2(m0 - m) : 0.f);
       if (a.sinks && m != -INFINITY) l += ex2(a.sinks[h] * LOG2E - m);
       const float inv = l != 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* dst = a.out + (size_t)(row0 + r) * a.ldo + (size_t)h * a.dim;
