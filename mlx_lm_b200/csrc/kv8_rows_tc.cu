@@ -15,9 +15,13 @@
 // largest at most, the scores by 3e-5 of their spread for normal numbers, a tenth of what rounding P costs; the sums are exact.
 // A code of V enters as fp16 bits 00uu, u = code + 128: the subnormal number u * 2^-24, exact, for one bit operation on two codes (two for
 // the odd bytes).  The 128 comes off where the product starts: at -128 sum(p), which a product with ones gives and which is the softmax's
-// sum below as well (of the weights as they were rounded).  The scale of a key block multiplies the scores, that of a value block the
-// block's O, both in float32; P is rounded to fp16 (11 bits, 2^-12 of a weight).  The maximum that the exponentials are relative to
-// follows a score only once that is more than 8 (a factor 256) beyond it: most tiles need neither shuffles nor another scaling of O.
+// sum below as well (of the weights as they were rounded).  The scale sk of a key block multiplies the scores in float32; that of a value
+// block, sv, is in the exponent: P is exp(s) sv, rounded to fp16 relative to a base m that follows the largest s + log2(sv), so that what
+// rounds away is small in O and not merely in weight (a first token that takes most of the weight often has values of next to nothing).
+// The sum below takes P / sv, a tile at a time.  The base is set 7 below the largest (P up to 2^7) and set again once a P would pass 2^15,
+// which fp16 just takes: most tiles need neither shuffles nor another scaling of O.  A P loses 2^-12 of itself down to 2^-14, below that
+// 2^-25 at most: 2^-32 of the largest.  A tile of values of nothing (sv 0) adds to the sum alone, and moves the base only where
+// the sum would pass 2^100.
 //
 // Bound by the bytes of the cache, and for few or short rows by the latencies of a part: rows, pages, tiles, sums, the join.  64 rows of up to
 // 8192 positions, 32/8 heads of 128: 110 us, 5.1 TB/s (the same copies without any arithmetic: 109 to 124); one row at 131072: 56 us, 4.8 TB/s;
@@ -27,6 +31,8 @@
 // finds itself the last of a row by a counter waits for a fence, an atomic and the sums in turn).  Blocks of 8 warps, two an SM, have
 // longer waits at each merge: 129 us, but 13.0 instead of 14.6 for one row of 8192.  Three blocks an SM with rings of four tiles: 110, one
 // row at 131072 51 us, but 31.8 instead of 26.6 for 64 rows of up to 1000, 16 heads of 64 (1024 items in rounds of 444, not 592).
+#include <float.h>
+
 #include "kv8_rows.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -50,7 +56,8 @@ constexpr int VW = DH % 128 == 0 ? 16 : DH % 64 == 0 ? 8 : DH % 32 == 0 ? 4 : 2;
 constexpr int NV = DH / 8 / VW;
 constexpr int VR = VW >= 4 ? DH / 32 : DH / 16;         // registers of a value
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float SLACK = 8.f;
+// log2 of the largest P: where the base of the exponentials is set anew, and at most; of the largest weight where values are nothing
+constexpr float UP = 7.f, MOST = 15.f, ABOVE = 100.f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24: what a code's operand counts in
 constexpr uint32_t ONES = 0x3c003c00u;
 
@@ -121,6 +128,9 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 
 constexpr int PART = 8 * (DH + 2);                      // floats of an item's sums: m[8], l[8], then O as the lanes hold it
+
+// A sum for those that multiply it by weights, some of them 0: of values around 2^-100 it may pass the range of float32.
+__device__ __forceinline__ float in_range(float x) { return x == INFINITY ? FLT_MAX : x; }
 
 __device__ __forceinline__ int column_of(int c, int g) { return (c / VW * 8 + g) * VW + c % VW; }      // column c of lane group g's
 
@@ -262,10 +272,12 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
 #pragma unroll
     for (int j = 0; j < KT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float lsv_of = 0.f, rsv_of = 0.f;                   // of the tiles looked up: log2 and reciprocal of the value scale (0, 0: values of nothing)
 
     auto work = [&](int i, int i32, int st) {           // tile i, the i32-th of those looked up
       if (job.missing >> i32 & 1) return;
-      const float sk = __shfl_sync(0xffffffffu, job.sk, i32), sv = __shfl_sync(0xffffffffu, job.sv, i32);
+      const float sk = __shfl_sync(0xffffffffu, job.sk, i32), lsv = __shfl_sync(0xffffffffu, lsv_of, i32);
+      const float rsv = __shfl_sync(0xffffffffu, rsv_of, i32);
       const uint8_t* kp = my_ring + st * TILE;
       const uint8_t* vp = kp + 16 * DH + value_base;
       uint32_t fk[2][KT];
@@ -283,25 +295,26 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         imma(c, fk[0][2 * j], fk[1][2 * j], a2, a3, qh[j][0], qh[j][1]);
         imma(c2, fk[0][2 * j], fk[1][2 * j], a2, a3, ql[j][0], ql[j][1]);
       }
-      // scores of keys g and g + 8, heads 2t and 2t + 1, in units of log2 (the sums stay below 2^31 for heads of up to 256)
+      // s + log2(sv) of keys g and g + 8, heads 2t and 2t + 1, in units of log2 (the sums stay below 2^31 for heads of up to 256)
       const float a0 = sk * fac0, a1 = sk * fac1;
-      float s0 = (float)(c[0] * 256 + c2[0]) * a0, s1 = (float)(c[1] * 256 + c2[1]) * a1;
-      float s2 = (float)(c[2] * 256 + c2[2]) * a0, s3 = (float)(c[3] * 256 + c2[3]) * a1;
+      float s0 = fmaf((float)(c[0] * 256 + c2[0]), a0, lsv), s1 = fmaf((float)(c[1] * 256 + c2[1]), a1, lsv);
+      float s2 = fmaf((float)(c[2] * 256 + c2[2]), a0, lsv), s3 = fmaf((float)(c[3] * 256 + c2[3]), a1, lsv);
       if (i == 0 || i == n_tiles - 1) {                 // (a window begins in a row's first tile)
         const int key = job.first + i * BLK;
         const bool in = key + g >= lo && key + g < x.end, in8 = key + g + 8 >= lo && key + g + 8 < x.end;
         if (!in) s0 = s1 = -INFINITY;
         if (!in8) s2 = s3 = -INFINITY;
       }
-      if (__any_sync(0xffffffffu, s0 > m0 + SLACK || s2 > m0 + SLACK || s1 > m1 + SLACK || s3 > m1 + SLACK)) {
+      if (__any_sync(0xffffffffu, rsv == 0.f || s0 > m0 + MOST || s2 > m0 + MOST || s1 > m1 + MOST || s3 > m1 + MOST)) {
         float t0 = fmaxf(s0, s2), t1 = fmaxf(s1, s3);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
           t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
         }
-        t0 = fmaxf(t0, m0);
-        t1 = fmaxf(t1, m1);
+        const float above = rsv == 0.f ? ABOVE : UP;
+        t0 = fmaxf(t0 - above, m0);
+        t1 = fmaxf(t1 - above, m1);
         const float r0 = ex2(m0 - (t0 == -INFINITY ? 0.f : t0)), r1 = ex2(m1 - (t1 == -INFINITY ? 0.f : t1));
         m0 = t0;
         m1 = t1;
@@ -309,14 +322,26 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         l1 *= r1;
 #pragma unroll
         for (int j = 0; j < KT; ++j) { o[j][0] *= r0; o[j][1] *= r1; o[j][2] *= r0; o[j][3] *= r1; }
+        if (rsv == 0.f) {
+          const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+          float y0 = ex2(s0 - b0) + ex2(s2 - b0), y1 = ex2(s1 - b1) + ex2(s3 - b1);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            y0 += __shfl_xor_sync(0xffffffffu, y0, d);
+            y1 += __shfl_xor_sync(0xffffffffu, y1, d);
+          }
+          l0 += y0;
+          l1 += y1;
+          return;
+        }
       }
       const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
       const float p0 = ex2(s0 - b0), p1 = ex2(s1 - b1), p2 = ex2(s2 - b0), p3 = ex2(s3 - b1);
       const uint32_t pb0 = turned(pack_half2(p0, p1)), pb1 = turned(pack_half2(p2, p3));
       float sum[4];                                     // of the weights as they were rounded, in every row
       mma(sum, ONES, ONES, ONES, ONES, pb0, pb1, 0.f, 0.f, 0.f, 0.f);
-      l0 += sum[0];
-      l1 += sum[1];
+      l0 = fmaf(sum[0], rsv, l0);
+      l1 = fmaf(sum[1], rsv, l1);
       const float n0 = sum[0] * (-128.f * UNIT), n1 = sum[1] * (-128.f * UNIT);
       uint32_t fv[4][VR];
 #pragma unroll
@@ -338,7 +363,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
           float d[4];
           mma(d, even(x01), odd(x01), even(x23), odd(x23), pb0, pb1, n0, n1, n0, n1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[PER * w + r][e] = fmaf(sv, d[e], o[PER * w + r][e]);
+          for (int e = 0; e < 4; ++e) o[PER * w + r][e] += d[e];
         }
       }
     };
@@ -348,6 +373,9 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
         look_up(job, i0);
         for (int i = 0, s = st; i < STAGES - 1; ++i, s = s + 1 == STAGES ? 0 : s + 1) fetch(job, i, n, s);
       }
+      // (here, behind the first copies: the scales are on their way as long as the tiles)
+      lsv_of = job.sv > 0.f ? __log2f(job.sv) : 0.f;
+      rsv_of = job.sv > 0.f ? __fdividef(1.f, job.sv) : 0.f;
       for (int i = 0; i < n; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                                   // every lane's copies of tile i are there, and tile i - 1 has been read
@@ -367,7 +395,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
     for (int j = 0; j < KT; ++j) mine4[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
     if (g == 0) {
       sm_m[warp][2 * t] = m0; sm_m[warp][2 * t + 1] = m1;
-      sm_l[warp][2 * t] = l0; sm_l[warp][2 * t + 1] = l1;
+      sm_l[warp][2 * t] = in_range(l0); sm_l[warp][2 * t + 1] = in_range(l1);
     }
     if (lane == 0) sm_spare[warp] = warp * (STAGES * TILE) + spare * TILE;
     __syncthreads();
@@ -388,7 +416,7 @@ rows_tc_kernel(const RowsArgs a, int tiles, int group_tiles, int q_vec) {
       float* part = a.partial + (((size_t)done.index * tiles + done.tile) * a.most_chunks + done.chunk) * PART;
       if (done.n_chunks > 1 && threadIdx.x < 4) {
         reinterpret_cast<float2*>(part)[t] = make_float2(top0, top1);
-        reinterpret_cast<float2*>(part + 8)[t] = make_float2(tot0, tot1);
+        reinterpret_cast<float2*>(part + 8)[t] = make_float2(in_range(tot0), in_range(tot1));
       }
       if (done.n_chunks == 1) {
         if (a.sinks) {
