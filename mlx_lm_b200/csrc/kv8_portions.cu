@@ -26,11 +26,13 @@
 // O's are put back when a row is written.  Queries are scaled by a power of two to [2^14, 2^15) at most, as fp16 exact to 2^-28 of their
 // largest number.
 // Scales: s = scale * sk * (q . codes) with sk the block's key scale; the weight that meets V's codes is w = exp(s) * sv, so the exponent
-// gets log2(sv), the running maximum is that of s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
+// gets log2(sv), the base follows the largest s + log2(sv) (w is what enters O: a weight that is small beside it may round away, whatever
 // its sv), and the sum below takes exp(s) = w / sv a group at a time.  A group of values of nothing (sv 0) adds to the sum alone, which
-// it does beside the others, with a maximum of its own (as codes of 0 with some sv it would raise the maximum that the weights of groups
-// of small values are stored relative to, and these would round away).  The maximum follows the scores only once the weights of a group sum to more than 2^12 (fp16 holds 2^15), so O is scaled
-// again, by the softmax threads in tensor memory, a few times a row at most.
+// it does beside the others, with a maximum of its own (as codes of 0 with some sv it would raise the base, and the weights of groups
+// of small values would round away).  The base is set 2^7 below the largest, and again once the weights of a group sum to more than the
+// largest fp16, so O is scaled again, by the softmax threads in tensor memory, a few times a row at most.  A weight loses
+// 2^-12 of itself down to 2^-14, below that 2^-25 at most: 2^-32 of the largest, of 131072 keys together 3e-5 of it (with the base at
+// the largest and room for 2^12 beyond it, 2^-25 of it for each: a flat tail that holds a 250th of the weight could vanish).
 //
 // Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
 // MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone.
@@ -48,7 +50,8 @@ constexpr int SMS = 148;
 constexpr int XR = 8;                // blocks whose scales are kept
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNIT = 5.9604644775390625e-8f;          // 2^-24
-constexpr float HIGH = 4096.f;       // the largest sum of a group's weights that a pass leaves be: fp16 holds up to 65504
+constexpr float UP = 7.f;            // log2 of the largest weight after the base of the exponentials has been set
+constexpr float HIGH = 65504.f;      // the largest sum of a group's weights that a pass leaves be: the largest fp16
 
 struct PortionArgs {
   const __nv_bfloat16* q;
@@ -544,14 +547,14 @@ portions_kernel(const PortionArgs a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[t]);
     }
-    float m = -INFINITY, l = 0.f;      // the running maximum of s + log2(sv), in units of the exponent; the sum
+    float m = -INFINITY, l = 0.f;      // the base of the exponentials, which follows the largest s + log2(sv); the sum
     float m0 = -INFINITY, l0 = 0.f;    // the maximum of s, and the sum, of groups whose values are 0
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
       const int key0 = (kb_lo + i) * TK, x4 = i % XR;
       if (!(ok = wait_warp(&sm.s_full[t], (uint32_t)(i & 1), abort_flag))) break;
       after_sync();
-      const uint32_t marks = sm.marks[x4], gone = marks & 0xffu;
+      const uint32_t marks = sm.marks[x4];
       uint32_t s[TK / 32][32];
 #pragma unroll
       for (int c = 0; c < TK / 32; ++c) tmem_ld32(t_s + 32 * c, s[c]);
@@ -559,39 +562,39 @@ portions_kernel(const PortionArgs a) {
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.s_read[t]);        // the next S may be formed over it
-      // blocks that every row of the tile sees whole need no mask
-      if (gone != 0 || key0 + TK - 1 > pos0 || (a.window > 0 && key0 < last_pos - a.window + 1)) {
+      // blocks that every row of the tile sees whole, with values in every group, need none of this
+      if (marks != 0 || key0 + TK - 1 > pos0 || (a.window > 0 && key0 < last_pos - a.window + 1)) {
         const int first = lo - key0, last = pos - key0;
 #pragma unroll
         for (int c = 0; c < TK / 32; ++c) {
           const int f = first - 32 * c, e1 = last - 32 * c;
           uint32_t bits = f <= 0 ? 0xffffffffu : f > 31 ? 0u : 0xffffffffu << f;
           bits &= e1 >= 31 ? 0xffffffffu : e1 < 0 ? 0u : (2u << e1) - 1u;
-          if (gone >> (2 * c) & 1) bits &= 0xffff0000u;
-          if (gone >> (2 * c + 1) & 1) bits &= 0x0000ffffu;
+          if (marks >> (2 * c) & 1) bits &= 0xffff0000u;
+          if (marks >> (2 * c + 1) & 1) bits &= 0x0000ffffu;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!(bits >> e & 1)) s[c][e] = 0xff800000u;          // -inf: its exponential below is 0
         }
-      }
-      if (marks >> 8) {
-        // groups whose values are 0: into their own sum, and out of what follows
+        if (marks >> 8) {
+          // groups whose values are 0: into their own sum, and out of what follows
 #pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          if (!(marks >> (8 + g) & 1)) continue;
-          uint32_t* x = &s[g >> 1][16 * (g & 1)];
-          const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f);
-          float top = __uint_as_float(x[0]);
+          for (int g = 0; g < GR; ++g) {
+            if (!(marks >> (8 + g) & 1)) continue;
+            uint32_t* x = &s[g >> 1][16 * (g & 1)];
+            const float f = fmaxf(fac * sm.sk[x4][g], 1e-30f);
+            float top = __uint_as_float(x[0]);
 #pragma unroll
-          for (int e = 1; e < BLK; ++e) top = fmaxf(top, __uint_as_float(x[e]));
-          top = fmaxf((top - off) * f, m0);
-          const float base = top == -INFINITY ? 0.f : top, k = fmaf(-off, f, -base);
-          l0 *= ex2(m0 - base);
-          m0 = top;
+            for (int e = 1; e < BLK; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+            top = fmaxf((top - off) * f, m0);
+            const float base = top == -INFINITY ? 0.f : top, k = fmaf(-off, f, -base);
+            l0 *= ex2(m0 - base);
+            m0 = top;
 #pragma unroll
-          for (int e = 0; e < BLK; ++e) {
-            l0 += ex2(fmaf(__uint_as_float(x[e]), f, k));
-            x[e] = 0xff800000u;
+            for (int e = 0; e < BLK; ++e) {
+              l0 += ex2(fmaf(__uint_as_float(x[e]), f, k));
+              x[e] = 0xff800000u;
+            }
           }
         }
       }
@@ -599,7 +602,7 @@ portions_kernel(const PortionArgs a) {
       // as long as a third of the exponentials).  Then, and in blocks before which a row has seen nothing, the maximum first.
       const uint32_t t_p = t_s + TK + (uint32_t)((i & 1) * (TK / 2));
       auto raise_max = [&]() {
-        // The largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
+        // UP below the largest of s + log2(sv).  In a group the scale is one number above 0 (a key scale of 0 counts as one that leaves scores of
         // next to nothing, so that -inf stays -inf), so its largest score is the largest raw score's.
         float mx = -INFINITY;
 #pragma unroll
@@ -612,6 +615,7 @@ portions_kernel(const PortionArgs a) {
           const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
           mx = fmaxf(mx, fmaf(top - off, fmaxf(fac * sm.sk[x4][g], 1e-30f), sm.lsv[x4][g]));
         }
+        mx -= UP;
         const bool grow = mx > m;
         const float corr = grow ? ex2(m - mx) : 1.f;  // 2^-inf = 0
         if (grow) m = mx;

@@ -86,7 +86,7 @@ def test_zeros_among_scales_of_two_sizes(ops, kind, small):
     check(ops, kind, cache, spans, q, n_heads, 0.25)
 
 
-TAIL_KINDS = ["rows", "rows float32"]
+TAIL_KINDS = KINDS
 
 
 @pytest.mark.parametrize("kind", TAIL_KINDS)
