@@ -11,13 +11,14 @@
 // blocks of 128 keys P V and S stood in that chain: 398 us for the 2048 queries below, against 357 at that time.)
 // Two heads of a CTA have chains of their own, and a converted block serves both.
 //
-// Bound by the softmax warps' chain.  2048 queries of 32/8 heads of 128 at position 6144: 284 us, 845 TFLOP/s of products, the tensor pipe 47 %
-// busy (64 keys and two heads: products 1344 clocks, a block 2120, of which 1670 are a thread's 64 exponentials beside another head's on the
-// same scheduler, 120 the scores' way into registers, 330 barriers), and 256 CTAs on 148 SMs.  Steps on the way: a look at every weight for one that is
-// too large 359 us, at the sums of a group of them 342; then bulk copies of the codes (converters that loaded them had taken more time for
-// addresses than for codes), a pass that is done again as code of its own (no register is copied for it) and the tiles with the most keys
-// first: 284.  A polynomial for a part of the exponentials (a
-// quarter: 282, a half: 296) moves them from one busy unit to another and was left out; so were two threads a query, 32 keys of a block
+// Bound by the softmax warps' chain.  2048 queries of 32/8 heads of 128 at position 6144: 263 us, 915 TFLOP/s of products (64 keys and two
+// heads: products 1344 clocks, a block 2120, of which 1670 are a thread's 64 exponentials beside another head's on the same scheduler,
+// 120 the scores' way into registers, 330 barriers), and 256 CTAs on 148 SMs.  Steps on the way: a look at every weight for one that is too
+// large 359 us, at the sums of a group of them 342; then bulk copies of the codes (converters that loaded them had taken more time for
+// addresses than for codes) and a pass that is done again as code of its own (no register is copied for it): 284.  The tiles start in the
+// order of their list, the most keys first as the engine lists them: 263; from its end it was 281 (2048 queries at 0: 56 and 73, 8192 at 0:
+// 581 and 645, 4096 of 16 heads of 64 at 0: 75 and 104).  A polynomial for a part of the exponentials (a quarter: 282, a half: 296, when
+// the kernel took 284) moves them from one busy unit to another and was left out; so were two threads a query, 32 keys of a block
 // each: 304, the pair has to agree on its maximum in every block.
 //
 // Codes: u = code + 128 in the low byte of an fp16 is the subnormal number u * 2^-24, exact; K enters that way (two codes a bit
@@ -199,7 +200,7 @@ portions_kernel(const PortionArgs a) {
   Smem<DP, NT>& sm = *reinterpret_cast<Smem<DP, NT>*>(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int heads = a.Hq / NT, by_tile = blockIdx.x / heads;
-  const int4 tile = a.tiles[gridDim.x / heads - 1 - by_tile];      // a portion's last tiles, the longest, first
+  const int4 tile = a.tiles[by_tile];                   // in the list's order: its first tiles start first
   // (a list without one tile to do must not end before its predecessor has: what comes next waits for this grid only)
   if (tile.y <= 0) {
     if (blockIdx.x == 0) pdl_wait();

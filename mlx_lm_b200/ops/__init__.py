@@ -1061,7 +1061,8 @@ def kv8_attention_portions(q, tiles, n_tiles: int, block_table, k8, v8, k_scale,
                            status, stream, sinks=None) -> None:
     """Attention of prompt portions over pages in 8 bits, bfloat16, heads of up to 128.  ``tiles``: int32 ``[n_tiles, 4]`` = (row of the
     tile's first token in ``q`` and ``out``, its queries (0: skipped) up to ``PREFILL_TILE``, row of the block table, position of the first
-    query); window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are; a tile of rows or of a request that do not
+    query); they start in the order of the list, so the tiles with the most keys stand first (a long one at the end runs when the others
+    are done).  Window and sinks as in ``kv8_attention_rows``.  Rows of no tile are left as they are; a tile of rows or of a request that do not
     exist is left out and reported (``ST_POSITION_RANGE``)."""
     n_pages, Hkv, page, Dh, n_req, max_pages = _kv8_pools(k8, v8, k_scale, v_scale, block_table, status, "kv8_attention_portions")
     T, width, ldq = _kv8_matrix(q, _BF16T, "kv8_attention_portions q")

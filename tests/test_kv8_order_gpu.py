@@ -43,3 +43,35 @@ def test_a_launch_with_nothing_to_do_keeps_the_order(between):
         for got in (k, v):
             assert float((got - (i + 1)).abs().max()) <= (i + 1) * 2.0 ** -22
     assert int(status.item()) == (ops.ST_POSITION_RANGE if between == "portions out of range" else 0)
+
+
+def test_tiles_start_in_the_order_of_their_list():
+    """One tile of many keys and as much work in short tiles: with the long one first they run beside one another, with it last they add
+    up.  (Blocks start in the order of their numbers; the least of several times, and a wide margin.)"""
+    from mlx_lm_b200 import ops
+    heads, dim, page, long, short, n = 16, 64, 128, 16384, 0, 650
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n_pages = long // page + 2
+    k8, v8 = (torch.randint(-127, 128, (n_pages, heads, page, dim), generator=g, device="cuda", dtype=torch.int32).to(torch.int8) for _ in range(2))
+    ks, vs = (torch.full((n_pages, heads, page // 16), 0.01, device="cuda") for _ in range(2))
+    table = torch.arange(n_pages, dtype=torch.int32, device="cuda").view(1, -1)
+    q = torch.randn((n + 1) * 128, heads * dim, generator=g, device="cuda").bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tiles = [(0, 128, 0, long)] + [(128 * (i + 1), 128, 0, short) for i in range(n)]
+
+    def run(order):
+        t, out, best = torch.tensor(order, dtype=torch.int32, device="cuda"), torch.empty_like(q), float("inf")
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            ops.kv8_attention_portions(q, t, len(order), table, k8, v8, ks, vs, out, heads, 0.125, 0, status, ops.current_stream())
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best, out
+
+    (first, out), (last, same) = run(tiles), run(tiles[::-1])
+    assert int(status.item()) == 0 and torch.equal(out, same)
+    print(f"the long tile first {first * 1e3:.0f} us, last {last * 1e3:.0f} us")
+    assert first < 0.8 * last
