@@ -20,6 +20,7 @@
 //            name a range of the list the launcher is given;
 //     top-k  keeps the k largest of what is left (:129-151).
 //   Tokens of equal logit are kept or dropped together.
+//   A row of nothing but NaN and -infinity gives token 0 with a log-probability of NaN.
 //
 // process: logit_bias, then repetition, presence and frequency penalties over the last
 //          `context` tokens of each row (mlx_lm/sample_utils.py:72-126, 284-369).
@@ -144,7 +145,7 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ lg, int V, 
   }
   block_argmax(bv, bi, redf, redi);
   const float m = bv;
-  const int amax = bi;
+  const int amax = bi == 0x7fffffff ? 0 : bi;         // (a row without a number above -infinity: token 0)
   float s = 0.f;
   for (int i = tid; i < V; i += nt) s += expf(lg[i] - m);
   const float lse = m + logf(block_sum(s, redf));
@@ -417,7 +418,8 @@ sample_split_kernel(const float* __restrict__ logits, int ld, int V, const Sampl
       if (rg[k] > bg) { bg = rg[k]; bgi = rgi[k]; }
     }
     const float lse = all.m + logf(all.s);
-    const int tok = (draws && bgi != 0x7fffffff) ? bgi : all.idx;
+    const int best = (draws && bgi != 0x7fffffff) ? bgi : all.idx;
+    const int tok = best == 0x7fffffff ? 0 : best;      // as in sample_row
     out_token[row] = tok;
     out_logprob[row] = lg[tok] - lse;
   }
