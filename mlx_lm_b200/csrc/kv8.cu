@@ -9,7 +9,7 @@
 //         clamp(rint(x * (1 / scale)), -127, 127).  So a scale never falls while a block fills, a code is rounded again only when
 //         a larger number arrives, and what a block holds depends on how the step cut the request only through that second
 //         rounding.  A number that is not finite cannot be held: NaN becomes 0, an infinity the largest code of its sign, and the
-//         status word says so.
+//         status word says so, and where the caller gives flags for its requests, that of the request.
 //         Keys (and the step's queries beside them) are turned by their position on the way: the pair (u, v) of dimensions
 //         (i, i + half), or (2i, 2i + 1), becomes (u c - v s, v c + u s), c and s the cosine and sine of the float32 angle
 //         position * freq[i] times `mscale`.  Products, sums, the quotient and the reciprocal are rounded one by one (no fused
@@ -101,11 +101,14 @@ struct AppendArgs {
   int8_t *k8, *v8;
   float *ks, *vs;
   int* status;
+  const int* slots;              // [n_req]: a request's place among the flags
+  int* not_finite;               // [n_flags], or null
+  int n_flags;
   int chunk, heads_per_cta;
 };
 
 struct Leader {
-  int row, n, pos, page_id;      // page_id < 0: nothing is stored
+  int row, n, pos, page_id, req;      // page_id < 0: nothing is stored
 };
 
 // A CTA takes the leaders among `chunk` rows and a group of heads: it lists the leaders, forms the sines and cosines of all their rows
@@ -152,7 +155,7 @@ append_kernel(const AppendArgs a) {
           pg = -1;
         }
       }
-      lead[__popc(leaders & ((1u << lane) - 1u))] = Leader{t, n, p, pg};
+      lead[__popc(leaders & ((1u << lane) - 1u))] = Leader{t, n, p, pg, r};
       end = t + n;
     }
     end = __reduce_max_sync(0xffffffffu, end);
@@ -313,7 +316,13 @@ append_kernel(const AppendArgs a) {
     top = __reduce_max_sync(0xffffffffu, top);
     const bool odd = top >= INF_BITS;          // something is not finite: the largest of the others, and NaN becomes 0
     if (odd) {
-      if (lane == 0) atomicOr(a.status, MLXB_ST_NOT_FINITE);
+      if (lane == 0) {
+        atomicOr(a.status, MLXB_ST_NOT_FINITE);
+        if (a.not_finite) {
+          const int i = a.slots[ld.req];
+          if ((unsigned)i < (unsigned)a.n_flags) a.not_finite[i] = 1;
+        }
+      }
       top = 0;
 #pragma unroll
       for (int s = 0; s < PASSES; ++s) {
@@ -390,7 +399,9 @@ struct AppendRecord {
   int8_t *k8, *v8;
   float *ks, *vs;
   int* status;
-  long long dtype, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, half, interleaved, n_req, max_pages, n_pages, page;
+  const int* slots;
+  int* not_finite;
+  long long dtype, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, half, interleaved, n_req, max_pages, n_pages, page, n_flags;
   double mscale;
 };
 
@@ -418,8 +429,8 @@ MLXB_EXPORT int mlxb_kv8_append(const AppendRecord* rec, long long bytes, cudaSt
   const size_t item = dtype == MLXB_F32 ? 4 : 2;
   auto fits = [&](const void* p, int ld, int d) { return (((uintptr_t)p) % (4 * item)) == 0 && ld % 4 == 0 && d % 4 == 0; };
   AppendArgs a{k, v, q, q_out, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, dim, freq, half, (int)x.interleaved, (float)x.mscale,
-               x.positions, x.token_req, x.block_table, (int)x.n_req, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status, 1,
-               1};
+               x.positions, x.token_req, x.block_table, (int)x.n_req, (int)x.max_pages, (int)x.n_pages, page, k8, v8, x.ks, x.vs, x.status,
+               x.slots, x.not_finite, (int)x.n_flags, 1, 1};
   // four columns an access: whole groups of four, aligned, and pairs that are whole groups apart
   const bool wide = (!k || (fits(k, ldk, dk) && fits(v, ldv, dv))) && (!G || (fits(q, ldq, dk) && fits(q_out, ldo, dim))) &&
                     (half == 0 || (!x.interleaved && half % 4 == 0));

@@ -35,7 +35,9 @@ which is dropped when that step is read.  The tokens are the same with and witho
 
 After every step that hands out tokens the scheduler looks at the status word the kernels set instead of
 faulting (a token, position or page id out of range, a bounded wait that gave up), which the sampler brought
-back with the tokens, and raises ``KernelError`` rather than hand out tokens of a step that went wrong.
+back with the tokens, and raises ``KernelError`` rather than hand out tokens of a step that went wrong.  A key or value that
+is not finite and so cannot be held by an 8-bit cache concerns its own request alone: that ends with
+``finish_reason="not_finite"`` and no token (-1), and the others go on.
 
 The scheduler talks to an engine through five calls (``add_request``, ``finish``, ``step``,
 ``cache`` for page arithmetic, ``max_len``), and to a ``sample`` callable; tests drive it with fakes.
@@ -317,9 +319,8 @@ class Scheduler:
         else:
             logits = self.engine.step(entries)
             tokens, logprobs = self.sample(logits, sampled) if sampled else ([], [])
-        if sampled:
-            self._check_status()
-        prompts, responses = self._account(planned, tokens, logprobs)
+        failed = self._check_status() if sampled else []
+        prompts, responses = self._account(planned, tokens, logprobs, failed)
         return prompts, cancelled + responses
 
     def _read_inflight(self) -> List[Response]:
@@ -329,9 +330,9 @@ class Scheduler:
         self._inflight = None
         ahead = self._launch_ahead(handle, planned)
         tokens, logprobs = self.engine.decode_collect(handle)
-        self._check_status()
+        failed = self._check_status()
         self.last_step_tokens = self.last_step_prompt_tokens = 0
-        _, responses = self._account(planned, tokens, logprobs)
+        _, responses = self._account(planned, tokens, logprobs, failed)
         self._inflight = ahead
         return responses
 
@@ -368,9 +369,10 @@ class Scheduler:
             return None
         return ahead, [PlannedEntry(r, 1, True) for r in goes_on]
 
-    def _account(self, planned: List[PlannedEntry], tokens, logprobs) -> Tuple[List[PromptProgress], List[Response]]:
+    def _account(self, planned: List[PlannedEntry], tokens, logprobs,
+                 failed: Sequence[Request] = ()) -> Tuple[List[PromptProgress], List[Response]]:
         """Book a finished step: progress of prompts, the new tokens, who is done.  Rows of requests that have left
-        meanwhile (stopped or cancelled while the step was in flight) are dropped."""
+        meanwhile (stopped or cancelled while the step was in flight) are dropped.  ``failed`` requests end here without a token."""
         self.stats.steps += 1
         self.stats.most_running = max(self.stats.most_running, len(self.running))
         live = {id(r) for r in self.running}
@@ -389,8 +391,15 @@ class Scheduler:
             self.last_step_tokens += p.n_tokens
         responses: List[Response] = []
         sampled = [p.request for p in planned if p.wants_logits]
+        ended = {id(r): Response(r.uid, -1, 0.0, "not_finite", all_tokens=list(r.tokens)) for r in failed}
+        for r in failed:
+            self.engine.finish(r.rid)
+            self.running.remove(r)
         for r, tok, lp in zip(sampled, tokens, logprobs):
             if id(r) not in live:
+                continue
+            if id(r) in ended:
+                responses.append(ended.pop(id(r)))      # in its row's place
                 continue
             r.tokens.append(int(tok))
             r.n_generated += 1
@@ -405,14 +414,21 @@ class Scheduler:
                 self.running.remove(r)
             responses.append(Response(r.uid, int(tok), lp, reason,
                                       all_tokens=list(r.tokens) if reason is not None else None))
-        return prompts, responses
+        return prompts, responses + list(ended.values())
 
-    def _check_status(self) -> None:
+    def _check_status(self) -> List[Request]:
         """Raise if a kernel of the steps since the last look reported something (``Engine.host_status``: the
-        status word as the sampler's copy of the tokens brought it to the host; no synchronisation here)."""
+        status word as the sampler's copy of the tokens brought it to the host; no synchronisation here unless it is not zero).
+        Returns the running requests that alone are concerned (``Engine.failed``)."""
         word = getattr(self.engine, "host_status", 0)
         if word:
-            from ..ops import KernelError, describe_status
+            from ..ops import ST_NOT_FINITE, KernelError, describe_status
+            if word & ST_NOT_FINITE and hasattr(self.engine, "find_not_finite"):
+                self.engine.find_not_finite()
+                word &= ~ST_NOT_FINITE
+        if word:
             self.engine.clear_status()
             raise KernelError("a kernel reported: " + describe_status(word) + "; the tokens of this step are not "
                               "handed out")
+        failed = getattr(self.engine, "failed", ())
+        return [r for r in self.running if r.rid in failed] if failed else []

@@ -96,6 +96,7 @@ class LayerCacheView:
     v: Optional[torch.Tensor] = None
     k_scale: Optional[torch.Tensor] = None       # 8-bit caches (k, v int8): float32 [n_pages, heads, page / 16]
     v_scale: Optional[torch.Tensor] = None
+    not_finite: Optional[torch.Tensor] = None    # int32 [n_slots]: requests whose keys or values could not be held
     block_table: Optional[torch.Tensor] = None   # int32 [R, table_width] on the device
     page_size: int = 0
     state: Optional[torch.Tensor] = None         # [n_slots, *shape] float32
@@ -214,7 +215,8 @@ class StepContext:
             i = g.index_of(key)
             eight = g.k_scale is not None
             return LayerCacheView("kv", entry.write, k=g.k[i], v=g.v[i], k_scale=g.k_scale[i] if eight else None,
-                                  v_scale=g.v_scale[i] if eight else None, block_table=self._tables[gi], page_size=mgr.page_size)
+                                  v_scale=g.v_scale[i] if eight else None, not_finite=self.engine.not_finite if eight else None,
+                                  block_table=self._tables[gi], page_size=mgr.page_size, slots=self._slots if eight else None)
         g = mgr.state_groups[gi]
         return LayerCacheView("state", entry.write, state=g.data[g.index_of(key)], slots=self._slots)
 
@@ -259,6 +261,10 @@ class Engine:
         kernel_build.ensure_built(libs)      # compiled now, in parallel, if this is their first use
         self.ws = Workspace(model.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=model.device)
+        # 8-bit caches: a flag for each state slot, set by the kernel that could not hold a request's key or value, and the live requests
+        # that were found that way (``find_not_finite``)
+        self.not_finite = torch.zeros(max_requests, dtype=torch.int32, device=model.device) if kv_bits else None
+        self.failed: set = set()
         self.h2d_bytes = self.d2h_bytes = 0     # bytes the steps copied to and from the device (counted at the copies)
         self.last_calls = None    # the recorded launches of the last step that went through a launch plan
         self.host_status = 0      # the status word as a sampler's copy of a step's tokens last brought it to the host
@@ -282,10 +288,23 @@ class Engine:
 
     # ------------------------------------------------------------------ requests
     def add_request(self, rid: Hashable) -> None:
-        self.cache.add_request(rid)
+        slot = self.cache.add_request(rid)
+        if self.not_finite is not None:
+            self.not_finite[slot:slot + 1].zero_()      # whatever became of the slot's last request
 
     def finish(self, rid: Hashable) -> None:
         self.cache.release(rid)
+        self.failed.discard(rid)
+
+    def find_not_finite(self) -> None:
+        """Which live requests brought an 8-bit cache a number that is not finite: into ``failed``, and the status bit that says there are
+        some is cleared.  Synchronises with the device."""
+        flags = self.not_finite.tolist() if self.not_finite is not None else []
+        self.failed.update(rid for rid, r in self.cache.requests.items() if r.slot < len(flags) and flags[r.slot])
+        if self.not_finite is not None:
+            self.not_finite.zero_()
+        self.status &= ~ops.ST_NOT_FINITE
+        self.host_status &= ~ops.ST_NOT_FINITE
 
     def has_request(self, rid: Hashable) -> bool:
         return rid in self.cache.requests

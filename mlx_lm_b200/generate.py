@@ -19,11 +19,13 @@ import contextlib
 import json
 import sys
 import time
+import warnings
 from dataclasses import dataclass
 from typing import Any, Callable, Dict, Generator, List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from . import ops
 from .engine.scheduler import PromptProgress, Response, Scheduler, StopSequenceMatcher
 from .engine.step import Engine
 from .sampling import GREEDY, Sampler, make_logits_processors, make_sampler
@@ -84,6 +86,14 @@ def _engine_for(model, engine: Optional[Engine], kv_bits: Optional[int], **sizes
 
 # ---------------------------------------------------------------------- single stream
 
+def _held(r: Response) -> Response:
+    """The response, unless it says that the request has ended because its cache could not hold it: an error where there is no other
+    request."""
+    if r.finish_reason == "not_finite":
+        raise ops.KernelError("a kernel reported: " + ops.describe_status(ops.ST_NOT_FINITE))
+    return r
+
+
 @dataclass
 class GenerationResponse:
     """What ``stream_generate`` yields (mlx_lm/generate.py:260-287).  ``logprobs`` is the
@@ -138,7 +148,7 @@ def stream_generate(model, tokenizer: TokenizerWrapper, prompt: Union[str, List[
                 for p in progress:
                     prompt_progress_callback(*p.progress)
             for r in responses:
-                if r.finish_reason == "cancelled":
+                if _held(r).finish_reason == "cancelled":
                     continue
                 if n == 0:
                     prompt_tps = len(tokens) / max(time.perf_counter() - tic, 1e-9)
@@ -178,7 +188,7 @@ def generate_step(prompt: Union[List[int], torch.Tensor], model, *, max_tokens: 
                 for p in progress:
                     prompt_progress_callback(*p.progress)
             for r in responses:
-                if r.finish_reason != "cancelled":
+                if _held(r).finish_reason != "cancelled":
                     yield r.token, dev_sampler.last_logprobs[0].clone()
     finally:
         sched.remove([uid])
@@ -234,7 +244,8 @@ class BatchGenerator:
     ``completion_batch_size`` bounds the requests that run at once, ``prefill_batch_size`` those of
     them still in their prompt, ``prefill_step_size`` the portion of one prompt per step; added
     here: ``max_tokens_per_step`` (token budget of a step), ``seed``, and the pool's ``page_size``
-    / ``num_pages`` and ``kv_bits`` (8: keys and values in 8 bits).  Prompt caches cannot be passed in or handed out (``caches`` must be None)."""
+    / ``num_pages`` and ``kv_bits`` (8: keys and values in 8 bits; a request that brings such a cache a number that is not finite ends with
+    ``finish_reason="not_finite"`` and token -1).  Prompt caches cannot be passed in or handed out (``caches`` must be None)."""
 
     Response = Response
 
@@ -315,8 +326,11 @@ class BatchGenerator:
         self._prompt_tokens += n_prompt
         self._gen_tokens += len(gens)
         if self._sampler.return_logprobs and gens:
-            for i, r in enumerate(gens):
-                r.logprobs = self._sampler.last_logprobs[i].clone()
+            # cancelled requests come first and have no row, nor have those behind the sampled ones
+            rows = [r for r in gens if r.finish_reason != "cancelled"]
+            for r, lp in zip(rows, self._sampler.last_logprobs if rows else ()):
+                if r.finish_reason != "not_finite":
+                    r.logprobs = lp.clone()
         return prompts, gens
 
     def next_generated(self) -> List[Response]:
@@ -354,7 +368,10 @@ def batch_generate(model, tokenizer, prompts: List[List[int]], prompt_caches=Non
                 if r.finish_reason is not None and verbose:
                     fin += 1
                     print(f"[batch_generate] Finished processing {fin}/{n} ...", end="\r")
-                if r.finish_reason not in ("stop", "cancelled"):
+                if r.finish_reason == "not_finite":
+                    warnings.warn(f"request {uids.index(r.uid)} ended after {len(results[r.uid])} tokens: "
+                                  + ops.describe_status(ops.ST_NOT_FINITE))
+                elif r.finish_reason not in ("stop", "cancelled"):
                     results[r.uid].append(r.token)
                     lps[r.uid].append(float(r.logprobs))
     gen.close()

@@ -884,11 +884,11 @@ def _kv8_rows_ints(positions, token_req, n: int, what: str) -> None:
     raise KernelError(f"{what}: {positions.numel()} positions and {token_req.numel()} requests for {n} rows, contiguous ones")
 
 
-_kv8_append_record = _kv8_record("13Q17qd")
+_kv8_append_record = _kv8_record("15Q18qd")
 
 
 def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale, status, stream, freq=None, interleaved: bool = False,
-               mscale: float = 1.0, q=None, q_out=None) -> None:
+               mscale: float = 1.0, q=None, q_out=None, not_finite=None, slots=None) -> None:
     """This step's keys ``k [T, heads * dk]`` and values ``v [T, heads * dv]`` (rows of any stride, float32 or bfloat16) into pages of
     int8 codes ``[n_pages, heads, page, head_dim]`` with a float32 scale for each block of 16 positions and head (``[n_pages, heads,
     page // 16]``), in place; columns of a head beyond ``dk`` / ``dv`` are zeros.  Keys turn by their position on the way: the first
@@ -899,7 +899,8 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
     With ``A`` the largest magnitude that the call brings for a block and head and ``S = A / 127`` (0 below 2**-100), a call that brings the
     block's first position sets its scale to ``S``, a later one to the larger of ``S`` and what it was; older codes become ``rint(code *
     (old / new))`` where it grows.  New codes are ``rint(x * (1 / scale))`` within -127 .. 127.  A NaN is held as 0 and an infinity as the
-    largest code; ``status`` then gets ``ST_NOT_FINITE``.
+    largest code; ``status`` then gets ``ST_NOT_FINITE``, and with ``not_finite`` (int32 flags) element ``slots[r]`` of it becomes 1,
+    ``slots`` int32 with one element for each row r of the block table: which request it was.
 
     Rows of a request stand together in order of position, without gaps inside a block; ``token_req`` < 0: a row of no request, which is
     left out.  A row of a request that the block table has no row for, and one that goes back or leaves a gap (with those that follow on
@@ -934,10 +935,19 @@ def kv8_append(k, v, positions, token_req, block_table, k8, v8, k_scale, v_scale
         half, fp = freq.numel(), freq.data_ptr()
         if 2 * half > dk or not freq.is_contiguous():
             raise KernelError(f"kv8_append: {half} frequencies for heads of {dk}")
+    flags = sp = n_flags = 0
+    if not_finite is not None or slots is not None:
+        if not_finite is None or slots is None:
+            raise KernelError("kv8_append: flags of requests and the requests' places among them go together")
+        _need(not_finite, torch.int32, "kv8_append not_finite")
+        _need(slots, torch.int32, "kv8_append slots")
+        if slots.numel() < n_req or not slots.is_contiguous() or not not_finite.is_contiguous():
+            raise KernelError(f"kv8_append: {slots.numel()} slots for {n_req} requests, contiguous ones")
+        flags, sp, n_flags = not_finite.data_ptr(), slots.data_ptr(), not_finite.numel()
     record, size = _kv8_append_record(
         kp, vp, qp, op, fp, positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(),
-        k_scale.data_ptr(), v_scale.data_ptr(), status.data_ptr(), code, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, Dh, half, interleaved,
-        n_req, max_pages, n_pages, page, mscale)
+        k_scale.data_ptr(), v_scale.data_ptr(), status.data_ptr(), sp, flags, code, ldk, ldv, ldq, ldo, T, Hkv, G, dk, dv, Dh, half,
+        interleaved, n_req, max_pages, n_pages, page, n_flags, mscale)
     _call("kv8", "mlxb_kv8_append", _KV8_ARGS, record, size, stream)
 
 

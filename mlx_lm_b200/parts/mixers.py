@@ -78,7 +78,7 @@ class Attention(Mixer):
                 self.position.rotate(ctx, q, k)
             if cache.write and cache.k_scale is not None:
                 ops.kv8_append(k, v, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, cache.k_scale, cache.v_scale,
-                               ctx.status, ctx.stream)
+                               ctx.status, ctx.stream, not_finite=cache.not_finite, slots=cache.slots)
             elif cache.write:
                 ops.kv_write(k, v, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, ctx.status,
                              ctx.stream)
@@ -263,7 +263,7 @@ class SinkAttention(Mixer):
         if not cache.write:
             pk = pv = None
         ops.kv8_append(pk, pv, ctx.positions, ctx.token_req, cache.block_table, cache.k, cache.v, cache.k_scale, cache.v_scale,
-                       ctx.status, ctx.stream, freq=self.freq, q=pq, q_out=q)
+                       ctx.status, ctx.stream, freq=self.freq, q=pq, q_out=q, not_finite=cache.not_finite, slots=cache.slots)
 
     def mix(self, ctx, x, cache, tag: str = "mix_left"):
         o = self._heads_out(ctx, x, cache)
