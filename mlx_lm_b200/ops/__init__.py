@@ -813,7 +813,8 @@ def attention_decode(q, positions, token_req, block_table, k_pool, v_pool, out, 
 # a cache of keys and values in 8 bits (csrc/kv8.cu, csrc/kv8_rows.cu, csrc/kv8_rows_tc.cu)
 
 KV8_BLOCK = 16           # positions of a head that share a scale
-KV8_ROWS_MOST = 512      # rows of a launch: what bounds the scratch memory of many rows (csrc/kv8_rows.cuh takes more)
+KV8_ROWS_MOST = 512      # rows of a launch (csrc/kv8_rows.cuh takes more) ...
+KV8_SCRATCH_MOST = 256 << 20      # ... and bytes of its scratch memory: rows of 131072 positions of 32/8 heads of 128 take 2.5 MB each
 
 
 def kv8_supported(page: int, head_dim: int) -> bool:
@@ -999,23 +1000,31 @@ def _kv8_plan(dtype, n_heads: int, n_kv_heads: int, max_len: int):
 
 
 @functools.lru_cache(maxsize=256)
-def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
-    """``(float32 elements of scratch memory, int32 counters)`` that ``kv8_attention_rows`` needs for ``n_rows`` rows of requests of up to
-    ``max_len`` positions."""
-    n = min(n_rows, KV8_ROWS_MOST)
+def _kv8_rows_at_once(n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
+    """``(rows of a launch at most, float32 elements and counters of a row)``: of queries of either type."""
     floats = tickets = 0
     for dtype, heads in _KV8_TILE_HEADS.items():
         tiles, most, _ = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
-        floats, tickets = max(floats, n * tiles * most * heads * (head_dim + 2)), max(tickets, n * tiles)
-    return floats, tickets
+        floats, tickets = max(floats, tiles * most * heads * (head_dim + 2)), max(tickets, tiles)
+    return max(1, min(KV8_ROWS_MOST, KV8_SCRATCH_MOST // (4 * floats))), floats, tickets
+
+
+def kv8_rows_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
+    """``(float32 elements of scratch memory, int32 counters)`` that ``kv8_attention_rows`` needs for ``n_rows`` rows of requests of up to
+    ``max_len`` positions.  Many rows go in several launches on the same memory: no more than ``KV8_ROWS_MOST`` rows at once, nor than
+    ``KV8_SCRATCH_MOST`` bytes take."""
+    at_once, floats, tickets = _kv8_rows_at_once(n_heads, n_kv_heads, head_dim, max_len)
+    n = min(n_rows, at_once)
+    return n * floats, n * tickets
 
 
 @functools.lru_cache(maxsize=256)
 def _kv8_rows_launch(dtype, n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int):
-    """What a call's sizes decide: library and launcher, parts of a row, sizes of its scratch memory."""
+    """What a call's sizes decide: library and launcher, parts of a row, rows of a launch, sizes of its scratch memory."""
     dtype_code(dtype)
     _, most, least = _kv8_plan(dtype, n_heads, n_kv_heads, max_len)
     return (kv8_rows_library(dtype, head_dim), "mlxb_kv8_rows" if dtype == torch.float32 else "mlxb_kv8_rows_tc", most, least,
+            _kv8_rows_at_once(n_heads, n_kv_heads, head_dim, max_len)[0],
             *kv8_rows_scratch(n_rows, n_heads, n_kv_heads, head_dim, max_len))
 
 
@@ -1040,7 +1049,7 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         if not rows.is_contiguous():
             raise KernelError(f"kv8_attention_rows: rows of strides {rows.stride()}")
         n, rp = rows.numel(), rows.data_ptr()
-    lib, name, most, least, floats, tickets = _kv8_rows_launch(dtype, n, n_heads, Hkv, Dh, max_len)
+    lib, name, most, least, at_once, floats, tickets = _kv8_rows_launch(dtype, n, n_heads, Hkv, Dh, max_len)
     if (scratch.dtype is not _F32T or counters.dtype is not _I32 or not scratch.is_cuda or not counters.is_cuda or scratch.numel() < floats
             or counters.numel() < tickets):
         _need(scratch, torch.float32, "kv8_attention_rows scratch")
@@ -1049,13 +1058,13 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
                           f"{tickets} are needed")
     sk = 0 if sinks is None else _sinks(sinks, n_heads, "kv8_attention_rows")
     qp, op, pp, tp, item = q.data_ptr(), out.data_ptr(), positions.data_ptr(), token_req.data_ptr(), q.element_size()
-    for a in range(0, n, KV8_ROWS_MOST):
+    for a in range(0, n, at_once):
         # the rows of the list from its a-th on, or rows a and on of the tensors
         r, t = (rp + 4 * a, 0) if rp else (0, a)
         record, size = _kv8_rows_record(
             qp + t * ldq * item, r, pp + 4 * t, tp + 4 * t, block_table.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), sk, scratch.data_ptr(), counters.data_ptr(), op + t * ldo * item, status.data_ptr(), ldq,
-            T - t, n_req, max_pages, n_pages, page, n_heads, Hkv, Dh, window, most, least, ldo, min(n - a, KV8_ROWS_MOST), scale)
+            T - t, n_req, max_pages, n_pages, page, n_heads, Hkv, Dh, window, most, least, ldo, min(n - a, at_once), scale)
         _call(lib, name, _KV8_ARGS, record, size, stream)
 
 

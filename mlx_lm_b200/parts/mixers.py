@@ -151,8 +151,10 @@ def paged_attention_kv8(ctx, q, cache, o, n_heads: int, head_dim: int, scale: fl
     if by_row:
         # Scratch memory is asked for once a layer, for the larger of the launches: a second, larger request would replace the memory that
         # the first launch was given, and a recorded step would go on naming it.
-        floats, tickets = ops.kv8_rows_scratch(max(n for n, _ in by_row), n_heads, cache.k.shape[1], head_dim, ctx.max_len)
-        partial, counters = ctx.ws.flat("kv8_partial", floats, torch.float32), ctx.ws.flat("kv8_tickets", tickets, torch.int32)
+        sizes = (n_heads, cache.k.shape[1], head_dim, ctx.max_len)
+        (floats, tickets), most = ops.kv8_rows_scratch(max(n for n, _ in by_row), *sizes), ops.kv8_rows_scratch(ops.KV8_ROWS_MOST, *sizes)
+        partial = ctx.ws.flat("kv8_partial", floats, torch.float32, most[0])
+        counters = ctx.ws.flat("kv8_tickets", tickets, torch.int32, most[1])
         for _, rows in by_row:
             ops.kv8_attention_rows(q, ctx.positions, ctx.token_req, cache.block_table, *pools, o, n_heads, scale, window, partial, counters,
                                    ctx.max_len, ctx.status, ctx.stream, rows=rows, sinks=sinks)

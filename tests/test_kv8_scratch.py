@@ -89,3 +89,24 @@ def test_no_recording_of_a_step_whose_buffers_moved(monkeypatch):
             if gen == engine.ws.generation:
                 assert set(calls) <= {b.data_ptr() for b in engine.ws._bufs.values()}
     assert engine.n_replayed == 2
+
+
+def test_scratch_memory_is_bounded(monkeypatch):
+    """However long the requests may be: a launch takes fewer rows then."""
+    for sizes in ((32, 8, 128, 131072), (64, 8, 128, 1 << 20), (16, 16, 64, 8192), (32, 32, 256, 131072)):
+        one = ops.kv8_rows_scratch(1, *sizes)
+        for n in (64, 512, 5000):
+            floats, tickets = ops.kv8_rows_scratch(n, *sizes)
+            assert one[0] <= floats and 4 * floats <= ops.KV8_SCRATCH_MOST and floats % one[0] == 0 and tickets // one[1] == floats // one[0]
+    # a buffer that grows by doubling stops at what the most rows take
+    ws = Workspace("cpu")
+    monkeypatch.setattr(ops, "KV8_SCRATCH_MOST", 1 << 20)
+    ops._kv8_rows_at_once.cache_clear()
+    try:
+        for n in (40, 64, 100, 128, 512):
+            layer(monkeypatch, ws, torch.float32, n, 0, tiles=False, head_dim=256)
+        most = ops.kv8_rows_scratch(512, 4, 2, 256, 300)[0]
+        assert max(b.numel() for b in ws._bufs.values()) == most and 4 * most <= 1 << 20
+    finally:
+        monkeypatch.undo()
+        ops._kv8_rows_at_once.cache_clear()
