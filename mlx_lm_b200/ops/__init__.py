@@ -1051,11 +1051,11 @@ def kv8_attention_rows(q, positions, token_req, block_table, k8, v8, k_scale, v_
         n, rp = rows.numel(), rows.data_ptr()
     lib, name, most, least, at_once, floats, tickets = _kv8_rows_launch(dtype, n, n_heads, Hkv, Dh, max_len)
     if (scratch.dtype is not _F32T or counters.dtype is not _I32 or not scratch.is_cuda or not counters.is_cuda or scratch.numel() < floats
-            or counters.numel() < tickets):
+            or counters.numel() < tickets or not scratch.is_contiguous() or not counters.is_contiguous()):
         _need(scratch, torch.float32, "kv8_attention_rows scratch")
         _need(counters, torch.int32, "kv8_attention_rows counters")
         raise KernelError(f"kv8_attention_rows: scratch of {scratch.numel()} floats and {counters.numel()} counters, {floats} and "
-                          f"{tickets} are needed")
+                          f"{tickets} are needed, contiguous ones")
     sk = 0 if sinks is None else _sinks(sinks, n_heads, "kv8_attention_rows")
     qp, op, pp, tp, item = q.data_ptr(), out.data_ptr(), positions.data_ptr(), token_req.data_ptr(), q.element_size()
     for a in range(0, n, at_once):

@@ -110,3 +110,30 @@ def test_scratch_memory_is_bounded(monkeypatch):
     finally:
         monkeypatch.undo()
         ops._kv8_rows_at_once.cache_clear()
+
+
+def test_scratch_memory_that_is_not_all_there(monkeypatch):
+    """Memory that repeats itself or lies apart has the elements and not the bytes: refused before anything is launched.  (Tensors on the
+    CPU that say they are on a device; no launch gets through.)"""
+    class OnDevice(torch.Tensor):
+        is_cuda = True
+
+    device = lambda t: t.as_subclass(OnDevice)
+    monkeypatch.setattr(ops, "_call", lambda *a: launched.append(a[1]))
+    launched = []
+    codes = [device(torch.zeros(3, 2, 16, 64, dtype=torch.int8)) for _ in range(2)] + [device(torch.zeros(3, 2, 1)) for _ in range(2)]
+    ints = lambda *shape: device(torch.zeros(*shape, dtype=torch.int32))
+    q = device(torch.zeros(4, 256))
+    floats, tickets = ops.kv8_rows_scratch(4, 4, 2, 64, 40)
+
+    def call(scratch, counters):
+        ops.kv8_attention_rows(q, ints(4), ints(4), ints(1, 3), *codes, q, 4, 0.1, 0, device(scratch), device(counters), 40, ints(1), 0)
+
+    good = torch.zeros(floats), torch.zeros(tickets, dtype=torch.int32)
+    call(*good)
+    assert launched == ["mlxb_kv8_rows"]
+    for bad in ((torch.zeros(1).expand(floats), good[1]), (good[0], torch.zeros(1, dtype=torch.int32).expand(tickets)),
+                (torch.zeros(2 * floats)[::2], good[1]), (good[0], torch.zeros(2 * tickets, dtype=torch.int32)[::2])):
+        with pytest.raises(ops.KernelError, match="contiguous"):
+            call(*bad)
+    assert len(launched) == 1
