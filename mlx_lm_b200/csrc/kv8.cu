@@ -16,11 +16,13 @@
 //         multiply-add): x decides a code by its rounding, and another order of roundings would be another code now and then.
 // read    The values at given positions, rounded to the output's type.
 //
-// Both are bound by bytes where rows are many, and by their latencies where they are few.  8192 rows of 32/8 heads of 128 at position 0,
-// turned, append and the read behind it 56 us: 234 MB, 4.1 TB/s; the append alone 46, its issue slots half used (23 million instructions).
+// Both are bound by their latencies: where rows are few, by that of the look-ups, the loads and the stores in turn; where they are many, of a
+// warp's loads, which nothing but the other four warps of its scheduler hides.  8192 rows of 32/8 heads of 128 at position 0, turned, append
+// and the read behind it 57 us: 234 MB, 4.1 TB/s; the append alone 46, DRAM 37 % and issue slots 54 % used (a warp waits 2.2 issues for
+// a load, 1.5 for arithmetic, 1.2 for instructions, 0.9 for shared memory, 0.8 at barriers, for each that it makes).
 // (232 us with divisions in the loops and sines for each row of each head: sines are a CTA's now, and every number is formed twice, for its
-// block's largest and for its code, since registers for a block's numbers would cost a third of the warps.)  One row of a request 5.0 us,
-// 64 requests' 6.6.  A lane of the read takes 16 codes: 8, so that a warp's stores are whole runs of 512 bytes, took 1 us longer for one row
+// block's largest and for its code, since registers for a block's numbers would cost a third of the warps.)  One row of a request 5.5 us,
+// 64 requests' 6.5.  A lane of the read takes 16 codes: 8, so that a warp's stores are whole runs of 512 bytes, took 1 us longer for one row
 // (twice the steps) and no less for 8192.
 //
 // Rows of a request stand together in order of position without gaps (the order in which a step lists them): the row whose predecessor

@@ -36,7 +36,8 @@
 // the largest and room for 2^12 beyond it, 2^-25 of it for each: a flat tail that holds a 250th of the weight could vanish).
 //
 // Every wait is bounded; a wait that gives up sets an abort flag that all roles see, the CTA frees its tensor memory and reports
-// MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone.
+// MLXB_ST_WAIT_TIMEOUT.  The order in which a query's keys are added depends on its position and window alone; when its base is set again
+// is a vote of the 32 queries of a warp, so its last bits depend on the queries beside it too, that is on how a prompt was cut.
 #include <cuda_fp16.h>
 
 #include "tcgen05.cuh"

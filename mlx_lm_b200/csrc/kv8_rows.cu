@@ -7,9 +7,11 @@
 //   weights  two of the heads each of the two lanes, to shared memory (times the value block's scale)
 //   values   a lane four columns, all 16 keys; fewer lanes a key, and more keys at a time, where heads are small
 // The maximum follows a score only once that is more than 8 beyond it.  The next block's codes are loaded before a block's are used.
-// Bound by its float32 arithmetic (two operations a code to turn it, eight for four heads) and, for short rows, by the latencies of a part:
-// its query, its pages, its codes, the sums.  8 rows of 8192 positions, 32/8 heads of 128: 82 us, 13 TFLOP/s, 1.6 TB/s of codes; 4 rows under
-// a window of 1000, 16/4 heads of 64: 10.7 us.  (With eight lanes a key, each with 16 columns of it and of the output, the sums of a score
+// Bound by latencies: long rows by that of a block's codes and of the chain from its scores to its weights, with 166 registers a thread and so less
+// than three warps a scheduler to hide them (issue slots 55 %, FMA pipe 31 %, DRAM 19 % used; of the 4 issues that a warp waits for each
+// that it makes 1.2 are for loads, 0.6 for arithmetic, 0.4 for shared memory); short rows by those of a part: its query, its pages, its codes, the
+// sums.  8 rows of 8192 positions, 32/8 heads of 128: 82 us, 13 TFLOP/s, 1.6 TB/s of codes; 4 rows under a window of 1000, 16/4
+// heads of 64: 10.8 us.  (With eight lanes a key, each with 16 columns of it and of the output, the sums of a score
 // went through shuffles and all eight lanes formed the same exponential: 250 and 13.2 us, at two warps a scheduler for the registers.)
 #include <type_traits>
 

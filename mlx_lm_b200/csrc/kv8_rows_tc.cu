@@ -24,8 +24,10 @@
 // the sum would pass 2^100.
 //
 // Bound by the bytes of the cache, and for few or short rows by the latencies of a part: rows, pages, tiles, sums, the join.  64 rows of up to
-// 8192 positions, 32/8 heads of 128: 110 us, 5.1 TB/s (the same copies without any arithmetic: 109 to 124); one row at 131072: 56 us, 4.8 TB/s;
-// 8 rows of up to 4000: 19.3; one row of 16 heads of 64 at 520: 7.0.  What decided it, for the 64 rows: neighbouring heads of a page read at
+// 8192 positions, 32/8 heads of 128: 112 us, 5.0 TB/s (the same copies without any arithmetic: 109 to 124); one row at 131072: 56 us, 4.8 TB/s;
+// 8 rows of up to 4000: 19.4; one row of 16 heads of 64 at 520: 7.0.  A chunk of at least 1024 keys leaves one row of 8192 positions with 64
+// blocks (14.8 us); its four quarters as blocks of their own, joined in the same order, would give the same bits, and are not built.  What decided
+// it, for the 64 rows: neighbouring heads of a page read at
 // about the same time (items are numbered with the heads innermost); a chunk shared by a block's four warps instead of a warp's own (157 us:
 // four times the partial sums); the next item's first tiles under way while sums are merged; the join in a kernel of its own (a block that
 // finds itself the last of a row by a counter waits for a fence, an atomic and the sums in turn).  Blocks of 8 warps, two an SM, have

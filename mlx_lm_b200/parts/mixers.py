@@ -253,8 +253,10 @@ class SinkAttention(Mixer):
         return o
 
     def _prepare_kv8(self, ctx, proj, q, cache) -> None:
-        """Queries, keys and values on their way to an 8-bit cache: the norms first (rounded to the run's type), then one kernel that turns
-        queries and keys and puts keys and values into the pages."""
+        """Queries, keys and values on their way to an 8-bit cache: the norms first, then one kernel that turns queries and keys and puts keys
+        and values into the pages.  In a bfloat16 run the normed queries and keys are rounded to bfloat16 in between, before they turn (the
+        kernel for other caches rounds them once, behind): the append takes its three inputs in one type, and a key is rounded to a
+        step of its block's largest number / 127 right after, some ten times as coarse."""
         T, H, G = proj.shape[0], self.n_heads, self.n_kv_heads
         pq, pk, pv = proj[:, :H * self.dim], proj[:, H * self.dim:(H + G) * self.dim], proj[:, (H + G) * self.dim:]
         if self.qk_norm:
