@@ -1,0 +1,117 @@
+// Rows of numbers in 8-bit floating point, and what the products of such rows share.
+//
+// Format.  A row of K numbers is K codes (e4m3) and one scale 2^e for each run of 128 columns.  e is the least whole number with
+// (largest finite magnitude of the run) <= 448 * 2^e, within -127 .. 127; a code is x * 2^-e rounded to nearest, ties to even.  The scale is a
+// power of two because a floating-point code loses nothing by it but what lies between the run's largest magnitude and 448, scaling is then
+// exact, and block-scaled tcgen05.mma multiplies by such scales itself (a byte e + 127 for each 32 columns; here four
+// runs of 32 share one).  A number that is not finite becomes the code for NaN, and so does every sum that it enters.
+//
+// Layout.  Codes: rows of `ld` bytes, ld a multiple of 16, zeros behind column K.  Scales: tiles of 512 bytes for 128 rows of a group
+// and 512 columns, [groups][ceil(rows / 128)][ceil(K / 512)][512]; the byte of row r and run b is at (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4.
+// That is the order in which tcgen05.cp (32x128b.warpx4) puts them in tensor memory where the products want them: row r in lane r % 32,
+// column r / 32, byte b % 4.  Groups: the matrices of a stack (experts), or the tiles of a plan.
+#pragma once
+
+#include "tcgen05.cuh"
+
+constexpr int FP8_RUN = 128;                 // columns with one scale
+constexpr int FP8_TILE = 512;                // bytes of a tile of scales: 128 rows, 4 runs
+
+// The exponent e of a run's scale, from the bits of its largest finite magnitude: 448 = 1.75 * 2^8.
+__device__ __forceinline__ int fp8_exponent(uint32_t top_bits) {
+  if (top_bits == 0) return 0;
+  const int e = (int)(top_bits >> 23) - 127 - 8 + ((top_bits & 0x7fffffu) > 0x600000u);
+  return max(-127, min(127, e));
+}
+// 2^e for -127 <= e <= 127 (2^-127 is subnormal)
+__device__ __forceinline__ float fp8_power(int e) { return __uint_as_float(e > -127 ? (uint32_t)(e + 127) << 23 : 1u << 22); }
+// the magnitude's bits, 0 for what is not finite
+__device__ __forceinline__ uint32_t fp8_magnitude(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+// Two codes (the first in the low byte) of numbers that were scaled; not finite: NaN (0x7f).  The conversion itself saturates, infinities
+// too, so these are made NaN before it.
+__device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
+  const float nan = __uint_as_float(0x7fffffffu);
+  lo = fabsf(lo) < INFINITY ? lo : nan;
+  hi = fabsf(hi) < INFINITY ? hi : nan;
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t fp8_quad(float a, float b, float c, float d) { return fp8_pair(a, b) | fp8_pair(c, d) << 16; }
+
+// Bytes from a row's place to its scales in a tile, without the run.
+__device__ __forceinline__ int fp8_scale_row(int r) { return (r & 31) * 16 + ((r >> 5) & 3) * 4; }
+
+// ---- products
+
+// Instruction descriptor for kind::mxf8f6f4: A and B e4m3 (bits 7-9 and 10-12 = 0), both K-major, N/8 in bits 17-22, scales of type e8m0
+// (bit 23), M/16 in bits 24-28; which byte of a scale's column: bits 4-5 for B, 29-30 for A.
+__host__ __device__ constexpr uint32_t fp8_idesc(int m, int n) {
+  return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t fp8_idesc_byte(uint32_t b) { return b << 4 | b << 29; }
+
+// 32 columns of K: D (+)= (A * its scales) (B * its scales)^T
+template <int CG>
+__device__ __forceinline__ void fp8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+}
+
+// Descriptor of a tile of scales in shared memory: 32 rows of 16 bytes without swizzle, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t fp8_scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
+}
+// A tile of scales into four columns of tensor memory, the same for the four quarters of its lanes.  Products that are issued behind it by
+// the same thread find them there.
+template <int CG>
+__device__ __forceinline__ void fp8_copy_scales(uint32_t tmem, uint64_t desc) {
+  if (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void fp8_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void fp8_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fp8_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fp8_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// A bounded wait that looks at no flag: for the way out, where copies and products already issued must come to their end.
+__device__ __forceinline__ void fp8_drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t p = 0; p < (1u << 20); ++p) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return;
+  }
+}
+
+// ---- host side: a matrix of codes, `rows` of `cols` bytes at a row stride of `ld` bytes, in boxes of box_rows x 128 columns
+static inline int fp8_make_map(CUtensorMap* map, const void* base, long long rows, int cols, int ld, int box_rows, const char* what) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)FP8_RUN, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return 0;
+  const char* msg = nullptr;
+  cuGetErrorString(r, &msg);
+  return mlxb_fail(MLXB_BAD_ARG, "%s: cuTensorMapEncodeTiled(%lld x %d, ld %d): %s", what, rows, cols, ld, msg ? msg : "?");
+}

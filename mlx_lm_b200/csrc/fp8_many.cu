@@ -1,0 +1,565 @@
+// Products with weights in 8-bit floating point for many rows (prompt portions), on the 5th-generation tensor cores.
+//
+//   linear      out[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) (+ residual[m, n])
+//   gated       per tile of a plan (128 slots of one expert): 128 columns of the unit of (gate, up), rounded to 8 bits in the epilogue
+//   experts     per tile of a plan: out[slot, n] = sum_k h[row, k] w[expert][n, k]
+//
+// Operands are rows of codes with scales (fp8.cuh).  Persistent CTAs: warp 0 copies (TMA, 128-byte swizzle, a ring of stages of 128 of K;
+// the scales of 512 of K come with every fourth), warp 1 issues tcgen05.mma kind::mxf8f6f4 (scales by tcgen05.cp into one of four places
+// in turn), warps 2-9 are the epilogue: two a quadrant of the lanes, a lane a row, half of the columns each.
+//
+// Tiles of 256 columns fill half of the tensor memory and scales want some of the rest, so there is one accumulator: the epilogue takes all of
+// its numbers into registers at once (128 a thread) and hands it back before it does anything with them.  That costs some 500 clocks a
+// tile; two accumulators of 128 columns would cost the main loop, whose products read shared memory 128 bytes a clock then.
+//
+// Pairs (CG = 2): two CTAs on a tile of 256 rows x BN columns; each brings its own rows of x, half of the rows of W and its own scales (of all BN
+// columns: each SM multiplies its rows by all of them), the leader issues the products for both.
+//
+// Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
+#include "activations.cuh"
+#include "fp8.cuh"
+#include "gated_unit.cuh"
+
+MLXB_DEFINE_LAST_ERROR()
+
+enum { MANY_LINEAR = 0, MANY_GATED = 1, MANY_EXPERTS = 2 };
+
+struct ManyArgs {
+  int M, N, runs, kgs, x_tiles, w_tiles;       // x_tiles, w_tiles: of 128 rows (of one matrix of W)
+  int tiles_m, tiles_n;                        // of the result; of a plan: tiles_m is what the plan holds
+  const int *sorted, *tile_info, *n_tiles;
+  const float* sel_weight;
+  const float* bias;
+  const void* residual;
+  void* out;
+  long long ldo;
+  uint8_t* out_scales;
+  int out_kgs;
+  int* status;
+  int act;
+  float limit;
+};
+struct ManyMaps { CUtensorMap x, w, xs, ws; };
+
+constexpr int MANY_EPI = 8, MANY_THREADS = 64 + 32 * MANY_EPI;
+
+template <int BN, int CG>
+struct ManyShape {
+  static constexpr int W_ROWS = BN / CG, W_TILES = BN / 128;
+  static constexpr int STAGE = 16384 + W_ROWS * 128 + (1 + W_TILES) * FP8_TILE;
+  static constexpr int STAGES = (227 * 1024 - 2048 - MANY_EPI * 2048) / STAGE < 8 ? (227 * 1024 - 2048 - MANY_EPI * 2048) / STAGE : 8;
+  static constexpr int SCALES = 4 + 4 * W_TILES;
+  static constexpr int ACC = BN == 256 ? 1 : 2;
+};
+
+template <int BN, int CG>
+struct ManySmem {
+  using S = ManyShape<BN, CG>;
+  alignas(1024) uint8_t x[S::STAGES][16384];
+  alignas(1024) uint8_t w[S::STAGES][S::W_ROWS * 128];
+  alignas(128) uint8_t xs[S::STAGES][FP8_TILE];
+  alignas(128) uint8_t ws[S::STAGES][S::W_TILES * FP8_TILE];
+  alignas(16) uint4 stage[MANY_EPI][32 * 4];        // 64 bytes of results of each of a warp's rows on their way out
+  alignas(8) uint64_t full[S::STAGES];
+  uint64_t empty[S::STAGES];
+  uint64_t acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+__device__ __forceinline__ int many_stage(int row, int piece) { return row * 4 + (piece ^ ((row >> 1) & 3)); }
+
+template <int ACT, bool FAST, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
+}
+
+template <typename TO>
+__device__ __forceinline__ void store_whole(uint4 u, int n, int N, TO* row) {
+  constexpr int PER = 16 / sizeof(TO);
+  if (n + PER <= N && ((uintptr_t)(row + n) & 15) == 0) {
+    *reinterpret_cast<uint4*>(row + n) = u;
+  } else {
+    const TO* e = reinterpret_cast<const TO*>(&u);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (n + i < N) row[n + i] = e[i];
+  }
+}
+
+template <int BN, int CG, int KIND, typename TO>
+__global__ void __launch_bounds__(MANY_THREADS)
+fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
+  using S = ManyShape<BN, CG>;
+  constexpr int STAGES = S::STAGES, HALF = BN / 2;
+  extern __shared__ uint8_t smem_raw[];
+  auto& sm = *reinterpret_cast<ManySmem<BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  const bool leader = rank == 0;
+  const int first_tile = (int)blockIdx.x / CG, step = (int)gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&sm.full[s], 1); mbar_init(&sm.empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&sm.acc_full[b], 1); mbar_init(&sm.acc_empty[b], CG * 32 * MANY_EPI); }
+    mbar_init(&sm.drained, 1);
+    sm.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.xs) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.ws) : "memory");
+  }
+  if (warp == 1) {
+    if (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  volatile int* abort_flag = &sm.abort_flag;
+  const uint32_t peer_abort = CG == 2 ? peer_addr(&sm.abort_flag, (uint32_t)(rank ^ 1)) : 0u;
+  fp8_before_sync();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  fp8_after_sync();
+  const uint32_t tmem = sm.tmem;
+  pdl_trigger();
+
+  // Where a tile lies.  A linear layer's tiles go by groups of 8 row tiles, columns after columns, so that those which run together read few
+  // rows of either operand; a plan's by column blocks, neighbours share an expert's rows of W.
+  struct Place { int m, n; };
+  const int* tile_info = a.tile_info;
+  int tiles_m = a.tiles_m;
+  auto place_of = [&](int t) {
+    if (KIND != MANY_LINEAR) return Place{t % tiles_m, t / tiles_m};
+    const int per = 8 * a.tiles_n, g = t / per, r = t - g * per, rows = min(8, tiles_m - 8 * g);
+    return Place{8 * g + r % rows, r / rows};
+  };
+  auto brings = [&](int k) { return (k & 3) == 0; };
+  auto load_x = [&](int s, int k, int m0) {
+    const int t = min(m0 >> 7, a.x_tiles - 1) * a.kgs + (k >> 2);
+    if (CG == 2) {
+      const uint32_t bar = peer_addr(&sm.full[s], 0);
+      tma_load_2d_pair(sm.x[s], &maps.x, k * FP8_RUN, m0, bar);
+      if (brings(k)) tma_load_2d_pair(sm.xs[s], &maps.xs, 0, t, bar);
+    } else {
+      tma_load_2d(sm.x[s], &maps.x, k * FP8_RUN, m0, &sm.full[s]);
+      if (brings(k)) tma_load_2d(sm.xs[s], &maps.xs, 0, t, &sm.full[s]);
+    }
+  };
+  auto load_w = [&](int s, int k, int expert, int nb) {
+    const uint32_t bar = CG == 2 ? peer_addr(&sm.full[s], 0) : 0u;
+    if (KIND == MANY_GATED) {             // 128 gate rows, then the up rows of the same columns
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int group = 2 * expert + h;
+        tma_load_2d(sm.w[s] + h * 16384, &maps.w, k * FP8_RUN, group * a.N + nb * 128, &sm.full[s]);
+        if (brings(k)) tma_load_2d(sm.ws[s] + h * FP8_TILE, &maps.ws, 0, (group * a.w_tiles + nb) * a.kgs + (k >> 2), &sm.full[s]);
+      }
+    } else {
+      const int row = expert * a.N + nb * BN + rank * S::W_ROWS;
+      if (CG == 2) tma_load_2d_pair(sm.w[s], &maps.w, k * FP8_RUN, row, bar);
+      else tma_load_2d(sm.w[s], &maps.w, k * FP8_RUN, row, &sm.full[s]);
+      if (brings(k))
+#pragma unroll
+        for (int i = 0; i < S::W_TILES; ++i) {
+          const int t = (expert * a.w_tiles + min(nb * S::W_TILES + i, a.w_tiles - 1)) * a.kgs + (k >> 2);
+          if (CG == 2) tma_load_2d_pair(sm.ws[s] + i * FP8_TILE, &maps.ws, 0, t, bar);
+          else tma_load_2d(sm.ws[s] + i * FP8_TILE, &maps.ws, 0, t, &sm.full[s]);
+        }
+    }
+  };
+  auto stage_bytes = [&](int k) { return (uint32_t)(CG * (16384 + S::W_ROWS * 128 + (brings(k) ? (1 + S::W_TILES) * FP8_TILE : 0))); };
+
+  pdl_wait();
+  tile_info = after_wait(tile_info);
+  const int* sorted = after_wait(a.sorted);
+  const float* sel_weight = after_wait(a.sel_weight);
+  if (KIND != MANY_LINEAR) tiles_m = min(tiles_m, after_wait(a.n_tiles)[0]);
+  const int n_tiles = tiles_m * a.tiles_n;
+
+  if (warp == 0) {
+    int issued = 0, s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = first_tile; t < n_tiles && ok; t += step) {
+      const Place p = place_of(t);
+      const int m0 = p.m * (CG * 128) + rank * 128, expert = KIND == MANY_LINEAR ? 0 : tile_info[3 * p.m];
+      for (int k = 0; k < a.runs; ++k) {
+        if (issued >= STAGES) {
+          ok = mbar_wait_warp(&sm.empty[s], ph ^ 1, abort_flag, peer_abort);
+          if (!ok) break;
+        }
+        if (elect_one()) {
+          if (leader) mbar_expect_tx(&sm.full[s], stage_bytes(k));
+          load_x(s, k, m0);
+          load_w(s, k, expert, p.n);
+        }
+        ++issued;
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+    if (__any_sync(0xffffffffu, *abort_flag) && leader && lane == 0)      // gave up: copies already issued land before the CTA exits
+      for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i) fp8_drain(&sm.full[i % STAGES], (uint32_t)((i / STAGES) & 1));
+  } else if (warp == 1) {
+    if (leader) {
+      constexpr uint32_t idesc = fp8_idesc(CG * 128, BN);
+      const uint32_t scales0 = tmem + S::ACC * BN;
+      const uint64_t dx0 = umma_desc(smem_u32(sm.x[0])), dw0 = umma_desc(smem_u32(sm.w[0]));
+      const uint64_t dxs0 = fp8_scale_desc(smem_u32(sm.xs[0])), dws0 = fp8_scale_desc(smem_u32(sm.ws[0]));
+      int s = 0, it = 0, place = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = first_tile; t < n_tiles && ok; t += step, ++it) {
+        const int b = S::ACC == 2 ? it & 1 : 0;
+        ok = mbar_wait_warp(&sm.acc_empty[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1) ^ 1, abort_flag, peer_abort);
+        if (!ok) break;
+        fp8_after_sync();
+        const uint32_t acc = tmem + (uint32_t)(b * BN);
+        for (int k = 0; k < a.runs; ++k) {
+          ok = mbar_wait_warp(&sm.full[s], ph, abort_flag, peer_abort);
+          if (!ok) break;
+          fp8_after_sync();
+          const bool fresh = brings(k);
+          if (fresh) place = (place + 1) & 3;
+          const uint32_t sx = scales0 + (uint32_t)(place * S::SCALES), sw = sx + 4;
+          if (elect_one()) {
+            if (fresh) {
+              fp8_copy_scales<CG>(sx, dxs0 + (uint32_t)(s * (FP8_TILE / 16)));
+#pragma unroll
+              for (int i = 0; i < S::W_TILES; ++i) fp8_copy_scales<CG>(sw + 4 * i, dws0 + (uint32_t)((s * S::W_TILES + i) * (FP8_TILE / 16)));
+            }
+            const uint32_t id = idesc | fp8_idesc_byte((uint32_t)(k & 3));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              fp8_mma<CG>(acc, dx0 + (uint32_t)(s * 1024 + 2 * j), dw0 + (uint32_t)(s * S::W_ROWS * 8 + 2 * j), id, sx, sw, k > 0 || j > 0);
+            if (CG == 2) umma_commit_both(&sm.empty[s]);
+            else umma_commit(&sm.empty[s]);
+          }
+          __syncwarp();
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+#ifdef MLXB_TEST_WAIT_TIMEOUT
+        if (g_test_withhold_arrival && it == 0) continue;
+#endif
+        if (ok && elect_one()) {
+          if (CG == 2) umma_commit_both(&sm.acc_full[b]);
+          else umma_commit(&sm.acc_full[b]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane;
+    uint4* stg = sm.stage[warp - 2];
+    const int o_row = lane >> 2, o_piece = lane & 3;
+    int it = 0;
+    for (int t = first_tile; t < n_tiles; t += step, ++it) {
+      const int b = S::ACC == 2 ? it & 1 : 0;
+      const Place p = place_of(t);
+      bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag, peer_abort);
+      if (KIND == MANY_GATED) {             // the two warps of a quadrant meet below
+        uint32_t all;
+        asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred r, %2, 64, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
+                     : "=r"(all) : "r"((uint32_t)ok), "r"(q + 1) : "memory");
+        ok = all != 0;
+      }
+      if (!ok) break;
+      fp8_after_sync();
+      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN);
+      constexpr int CHUNKS = HALF / 32;
+      uint32_t r[CHUNKS][32];
+      if (KIND == MANY_GATED) {             // 64 columns: gate, then up
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) tmem_ld32(acc + (uint32_t)((c >> 1) * 128 + half * 64 + (c & 1) * 32), r[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) tmem_ld32(acc + (uint32_t)(half * HALF + c * 32), r[c]);
+      }
+      fp8_wait_ld();
+      fp8_before_sync();
+      if (CG == 2) mbar_arrive_cluster(peer_addr(&sm.acc_empty[b], 0));
+      else mbar_arrive(&sm.acc_empty[b]);
+
+      if constexpr (KIND == MANY_GATED) {
+        const int first = tile_info[3 * p.m + 1], cnt = tile_info[3 * p.m + 2];
+        const bool live = row < cnt;
+        const float wgt = live && sel_weight ? sel_weight[sorted[first + row]] : 1.f;
+        const int n0 = p.n * 128 + half * 64;
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float h = n0 + 32 * c + i < a.N ? mlxb_gated_unit(a.act, __uint_as_float(r[c][i]), __uint_as_float(r[2 + c][i]), wgt, a.limit) : 0.f;
+            r[c][i] = __float_as_uint(h);
+            top = max(top, fp8_magnitude(h));
+          }
+        // the other warp has the other half of the run's columns
+        uint32_t* mine = reinterpret_cast<uint32_t*>(stg);
+        const uint32_t* other = reinterpret_cast<const uint32_t*>(sm.stage[(warp - 2) ^ 4]);
+        const int at = (it & 1) * 32 + lane;
+        mine[at] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
+        const int e = fp8_exponent(max(top, other[at]));
+        const float f = fp8_power(-e);
+        if (live) {
+          uint8_t* o = reinterpret_cast<uint8_t*>(a.out) + ((long long)p.m * 128 + row) * a.ldo;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int j = 16 * g + 4 * i;
+                w[i] = fp8_quad(__uint_as_float(r[c][j]) * f, __uint_as_float(r[c][j + 1]) * f, __uint_as_float(r[c][j + 2]) * f, __uint_as_float(r[c][j + 3]) * f);
+              }
+              const int n = n0 + 32 * c + 16 * g;
+              if (n < a.ldo) *reinterpret_cast<uint4*>(o + n) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          if (half == 0) a.out_scales[((long long)p.m * a.out_kgs + (p.n >> 2)) * FP8_TILE + fp8_scale_row(row) + (p.n & 3)] = (uint8_t)(e + 127);
+        }
+      } else {
+        constexpr int PER = 16 / sizeof(TO);
+        TO* out = reinterpret_cast<TO*>(a.out);
+        const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = p.n * BN + half * HALF;
+        const int first = KIND == MANY_EXPERTS ? tile_info[3 * p.m + 1] : 0;
+        const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
+        int slot = 0;
+        if (KIND == MANY_EXPERTS && lane < rows) slot = sorted[first + row];
+        const TO* res = reinterpret_cast<const TO*>(after_wait(a.residual));
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          float* v = reinterpret_cast<float*>(r[c]);
+          const int nc = n0 + 32 * c;
+          if (nc >= a.N) break;
+          if (KIND == MANY_LINEAR) {
+            if (a.bias != nullptr) {
+              const float mine = nc + lane < a.N ? a.bias[nc + lane] : 0.f;
+              reinterpret_cast<float*>(stg)[lane] = mine;
+              __syncwarp();
+              const float4* bp = reinterpret_cast<const float4*>(stg);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 x = bp[i];
+                v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
+              }
+              __syncwarp();
+            }
+            float (&vv)[32] = *reinterpret_cast<float (*)[32]>(r[c]);
+            switch (a.act) {
+              case EPI_GELU_NEW: activate_all<EPI_GELU_NEW, sizeof(TO) == 2>(vv); break;
+              case EPI_RELU: activate_all<EPI_RELU, sizeof(TO) == 2>(vv); break;
+              case EPI_TANH: activate_all<EPI_TANH, sizeof(TO) == 2>(vv); break;
+              default: break;
+            }
+            if (sizeof(TO) == 2 && res != nullptr && lane < rows) {       // added before the sum is rounded, by rows
+              const TO* rr = res + (long long)(m0 + lane) * a.ldo;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int n = nc + 8 * i;
+                if (n + 8 <= a.N && ((uintptr_t)(rr + n) & 15) == 0) {
+                  float e[8];
+                  unpack8(*reinterpret_cast<const uint4*>(rr + n), e);
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    if (n + j < a.N) v[8 * i + j] += to_f(rr[n + j]);
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int p0 = 0; p0 < 32; p0 += 4 * PER) {          // 64 bytes of each row at a time, written four lanes a row
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint4 u;
+              if (sizeof(TO) == 2) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = v[(x * 8 + i) & 31];
+                u = pack8(w);
+              } else {
+                const int i = (p0 + x * 4) & 31;
+                u = make_uint4(r[c][i], r[c][i + 1], r[c][i + 2], r[c][i + 3]);
+              }
+              stg[many_stage(lane, x)] = u;
+            }
+            __syncwarp();
+            const int n = nc + p0 + o_piece * PER;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int rr = 8 * j + o_row;
+              uint4 u = stg[many_stage(rr, o_piece)];
+              const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
+              if (rr < rows && n < a.N) {
+                TO* o = out + (long long)to * a.ldo;
+                if (KIND == MANY_LINEAR && sizeof(TO) == 4 && res != nullptr) {
+                  float* e = reinterpret_cast<float*>(&u);
+                  const float* x = reinterpret_cast<const float*>(res) + (long long)to * a.ldo + n;
+                  if (n + 4 <= a.N && ((uintptr_t)x & 15) == 0) {
+                    const float4 y = *reinterpret_cast<const float4*>(x);
+                    e[0] += y.x; e[1] += y.y; e[2] += y.z; e[3] += y.w;
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      if (n + i < a.N) e[i] += x[i];
+                  }
+                }
+                store_whole<TO>(u, n, a.N, o);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  fp8_before_sync();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  const bool aborted = sm.abort_flag != 0;
+  if (threadIdx.x == 0 && aborted) atomicOr(a.status, MLXB_ST_WAIT_TIMEOUT);
+  if (warp == 1 && leader) {
+    if (aborted && lane == 0) {
+      if (CG == 2) umma_commit_pair_local(&sm.drained);
+      else umma_commit(&sm.drained);
+      fp8_drain(&sm.drained, 0u);
+    }
+    __syncwarp();
+  }
+  if (CG == 2 && aborted) cluster_sync();
+  if (warp == 1) {
+    fp8_after_sync();
+    if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+
+// scales as rows of 512 bytes, a row a copy
+static int scales_map(CUtensorMap* map, const void* base, long long tiles, const char* what) {
+  const cuuint64_t dims[2] = {FP8_TILE / 4, (cuuint64_t)tiles};
+  const cuuint64_t strides[1] = {FP8_TILE};
+  const cuuint32_t box[2] = {FP8_TILE / 4, 1};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem,
+                                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return 0;
+  const char* msg = nullptr;
+  cuGetErrorString(r, &msg);
+  return mlxb_fail(MLXB_BAD_ARG, "%s: cuTensorMapEncodeTiled(%lld tiles of scales): %s", what, tiles, msg ? msg : "?");
+}
+
+template <int BN, int CG, int KIND, typename TO>
+static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(ManySmem<BN, CG>) + 1024;
+  static_assert(smem <= 227 * 1024, "stages and staging buffers fit a CTA's shared memory");
+  auto kern = fp8_many_kernel<BN, CG, KIND, TO>;
+  static SharedLimit limit;
+  if (cudaError_t e = limit.raise(kern, smem)) return mlxb_fail((int)e, "linear (8 bits): %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  const long long tiles = (long long)a.tiles_m * a.tiles_n;
+  const int units = mlxb_sm_count() / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CG * (unsigned)(tiles < units ? tiles : units));
+  cfg.blockDim = dim3(MANY_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CG == 2) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CG;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (mlxb_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kern, maps, a);
+  return mlxb_check_launch("linear (8 bits)");
+}
+
+static int many_check(const char* what, const void* x, const void* xs, const void* w, const void* ws, int N, int K, const void* out) {
+  if (!x || !xs || !w || !ws || !out || N <= 0 || K <= 0 || (K & 15) ||
+      (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws) & 15))
+    return mlxb_fail(MLXB_BAD_ARG, "%s: codes of %d x %d (rows of whole 16 bytes, 16-byte aligned)", what, N, K);
+  return 0;
+}
+
+struct ManyForm { int bn, cg; };
+static ManyForm many_form(int M, int N, int K) {
+  const char *want_pair = getenv("MLXB_FP8_PAIR"), *want_bn = getenv("MLXB_FP8_BN");     // experiments and tests
+  ManyForm f = {256, 2};
+  if (M <= 128) f.cg = 1;
+  if (want_pair && M > 128) f.cg = want_pair[0] == '1' ? 2 : 1;
+  if (want_bn) f.bn = atoi(want_bn) == 128 ? 128 : 256;
+  return f;
+}
+
+// As mlxb_fp8_linear_few, for any number of rows.
+MLXB_EXPORT int mlxb_fp8_linear_many(int out_f32, const void* x, const void* xs, const void* w, const void* ws, const float* bias, const void* residual,
+                                     void* out, int M, int N, int K, long long ldo, int epi, int* status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
+  if (int e = many_check("linear (8 bits)", x, xs, w, ws, N, K, out)) return e;
+  if (ldo < N || !activation_known(epi)) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d outputs at stride %lld, epilogue %d", N, ldo, epi);
+  const ManyForm f = many_form(M, N, K);
+  ManyArgs a = {};
+  a.M = M; a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = (M + 127) / 128; a.w_tiles = (N + 127) / 128;
+  a.tiles_m = (M + 128 * f.cg - 1) / (128 * f.cg); a.tiles_n = (N + f.bn - 1) / f.bn;
+  a.bias = bias; a.residual = residual; a.out = out; a.ldo = ldo; a.status = status; a.act = epi;
+  if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d x %d outputs", M, N);
+  ManyMaps maps;
+  if (int e = fp8_make_map(&maps.x, x, M, K, K, 128, "linear (8 bits) x")) return e;
+  if (int e = fp8_make_map(&maps.w, w, N, K, K, f.bn / f.cg, "linear (8 bits) w")) return e;
+  if (int e = scales_map(&maps.xs, xs, (long long)a.x_tiles * a.kgs, "linear (8 bits)")) return e;
+  if (int e = scales_map(&maps.ws, ws, (long long)a.w_tiles * a.kgs, "linear (8 bits)")) return e;
+#define GO(BN, CG) return out_f32 ? many_launch<BN, CG, MANY_LINEAR, float>(maps, a, stream) : many_launch<BN, CG, MANY_LINEAR, __nv_bfloat16>(maps, a, stream);
+  if (f.cg == 2) {
+    if (f.bn == 256) GO(256, 2)
+    GO(128, 2)
+  }
+  if (f.bn == 256) GO(256, 1)
+  GO(128, 1)
+#undef GO
+}
+
+// As mlxb_fp8_experts_few, for plans with tiles of 128 slots.
+MLXB_EXPORT int mlxb_fp8_experts_many(int gated, int out_f32, const void* x, const void* xs, const void* w, const void* ws, int E, int N, int K,
+                                      const int* sorted, const int* tile_info, const int* n_tiles, int max_tiles, int at_most, const float* sel_weight,
+                                      void* out, long long ldo, void* out_scales, int* status, int act, float limit, cudaStream_t stream) {
+  if (max_tiles <= 0 || at_most <= 0) return 0;
+  if (int e = many_check("moe_gemm_fp8", x, xs, w, ws, N, K, out)) return e;
+  if (E <= 0 || ldo < N || (gated && (!out_scales || ldo != ((N + 15) & ~15) || ((uintptr_t)out & 15))) || (long long)E * N * 2 > 0x7fffffffLL ||
+      (long long)max_tiles * 128 > 0x7fffffffLL)
+    return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d experts of %d x %d, results at stride %lld", E, N, K, ldo);
+  ManyArgs a = {};
+  a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = max_tiles; a.w_tiles = (N + 127) / 128;
+  const int bn = 256;
+  a.tiles_m = min(max_tiles, at_most); a.tiles_n = gated ? a.w_tiles : (N + bn - 1) / bn;
+  a.sorted = sorted; a.tile_info = tile_info; a.n_tiles = n_tiles; a.sel_weight = sel_weight;
+  a.out = out; a.ldo = ldo; a.out_scales = (uint8_t*)out_scales; a.out_kgs = (N + 511) / 512; a.status = status; a.act = act; a.limit = limit;
+  if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d tiles of %d outputs", max_tiles, N);
+  ManyMaps maps;
+  if (int e = fp8_make_map(&maps.x, x, (long long)max_tiles * 128, K, K, 128, "moe_gemm_fp8 x")) return e;
+  if (int e = fp8_make_map(&maps.w, w, (long long)E * (gated ? 2 : 1) * N, K, K, gated ? 128 : bn, "moe_gemm_fp8 w")) return e;
+  if (int e = scales_map(&maps.xs, xs, (long long)max_tiles * a.kgs, "moe_gemm_fp8")) return e;
+  if (int e = scales_map(&maps.ws, ws, (long long)E * (gated ? 2 : 1) * a.w_tiles * a.kgs, "moe_gemm_fp8")) return e;
+  if (gated) return many_launch<256, 1, MANY_GATED, float>(maps, a, stream);
+  return out_f32 ? many_launch<256, 1, MANY_EXPERTS, float>(maps, a, stream) : many_launch<256, 1, MANY_EXPERTS, __nv_bfloat16>(maps, a, stream);
+}

@@ -51,7 +51,8 @@ _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
 # kernel sources that only a bfloat16 run launches from: a float32 run neither compiles nor loads them
 BF16_ONLY_LIBS = frozenset({"gemm_smallm", "gemm_smallm_fold", "gemm_tcgen05", "attention_prefill",
-                            "attention_prefill_tc", "attention_wide_tc", "attention_wide_tcgen05", "moe_tcgen05", "recurrent_chunks", "kv8_portions"})
+                            "attention_prefill_tc", "attention_wide_tc", "attention_wide_tcgen05", "moe_tcgen05", "recurrent_chunks", "kv8_portions",
+                            "fp8_rows", "fp8_few", "fp8_many"})
 
 # ... and those that only a float32 run launches from
 F32_ONLY_LIBS = frozenset({"gemm_split"})
@@ -2479,6 +2480,239 @@ def moe_gemm_tc05(a, w, n_out: int, sorted_slots, tile_info, n_tiles, max_tiles:
           int(bool(gated)), _p(a), _rows(a, "moe_gemm_tc05 a"), a.shape[0], _p(w), E, NW, n_out, K, _p(sorted_slots),
           _p(tile_info), _p(n_tiles), int(max_tiles), _p(sel_weight), _p(out), _rows(out, "moe_gemm_tc05 out"), _p(status),
           GATED_UNITS[unit], float(limit), stream)
+
+
+# --------------------------------------------------------------------------
+# weights in 8-bit floating point (csrc/fp8.cuh, fp8_rows.cu, fp8_few.cu, fp8_many.cu)
+
+FP8_RUN = 128            # columns of a row that share a scale
+FP8_FEW_ROWS = 128       # up to so many rows, a linear layer streams its weights (csrc/fp8_few.cu)
+
+
+def fp8_empty(rows: int, columns: int, device, groups: int = 1):
+    """Memory for ``groups`` matrices of ``rows`` rows: ``(codes, scales)``.  ``codes`` float8_e4m3fn ``[groups * rows, columns]`` with the
+    columns rounded up to 16; ``scales`` uint8 ``[groups, ceil(rows / 128), ceil(columns / 512), 512]``: the scale of row ``r`` and run ``b`` of
+    128 columns is ``2**(byte - 127)``, the byte at ``[r // 128, b // 4, r % 32 * 16 + r // 32 % 4 * 4 + b % 4]`` of its group."""
+    if rows <= 0 or columns <= 0 or groups <= 0:
+        raise KernelError(f"fp8_empty: {groups} matrices of {rows} x {columns}")
+    codes = torch.zeros((groups * rows, (columns + 15) // 16 * 16), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    scales = torch.zeros((groups, (rows + 127) // 128, (columns + 511) // 512, 512), dtype=torch.uint8, device=device)
+    return codes, scales
+
+
+def _fp8_pair(codes, scales, group_rows: int, what: str):
+    """Checks a matrix (or stack) of codes and its scales; ``(rows, columns of codes, groups)``."""
+    _need(codes, torch.float8_e4m3fn, what + " codes")
+    _need(scales, torch.uint8, what + " scales")
+    if codes.dim() != 2 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
+        raise KernelError(f"{what}: codes {tuple(codes.shape)} strides {codes.stride()}: contiguous rows of whole 16 bytes")
+    rows, width = codes.shape
+    if group_rows <= 0 or rows % group_rows:
+        raise KernelError(f"{what}: {rows} rows of codes in matrices of {group_rows}")
+    groups = rows // group_rows
+    if scales.shape != (groups, (group_rows + 127) // 128, (width + 511) // 512, 512) or not scales.is_contiguous():
+        raise KernelError(f"{what}: scales {tuple(scales.shape)} for {groups} matrices of {group_rows} x {width}")
+    if scales.device != codes.device:
+        raise KernelError(f"{what}: codes on {codes.device}, scales on {scales.device}")
+    return rows, width, groups
+
+
+def _fp8_here(t, what: str) -> None:
+    """The launch goes to the current device."""
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+_FP8Q_ARGS = [c_int, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p]
+
+
+def fp8_quantize(x, codes, scales, stream, group_rows: Optional[int] = None) -> None:
+    """The rows of ``x`` (bfloat16 or float32 ``[rows, columns]``) in 8-bit floating point, into memory of ``fp8_empty``: e4m3 codes, and a
+    scale ``2**e`` for each run of 128 columns with ``e`` the least whole number for which the run's largest finite magnitude is at most
+    ``448 * 2**e`` (within -127 .. 127).  Codes are rounded to nearest, ties to even; what is not finite becomes NaN.  ``group_rows``:
+    ``x`` is a stack of matrices of so many rows (default: one matrix)."""
+    _need(x, None, "fp8_quantize x")
+    ldx = _rows(x, "fp8_quantize x")
+    M, K = x.shape
+    group_rows = M if group_rows is None else int(group_rows)
+    if M == 0:
+        return
+    rows, width, _ = _fp8_pair(codes, scales, group_rows, "fp8_quantize")
+    if rows != M or width != (K + 15) // 16 * 16 or codes.device != x.device:
+        raise KernelError(f"fp8_quantize: x {tuple(x.shape)} on {x.device} into codes {tuple(codes.shape)} on {codes.device}")
+    _fp8_here(x, "fp8_quantize")
+    _call("fp8_rows", "mlxb_fp8_quantize", _FP8Q_ARGS, dtype_code(x.dtype), _p(x), ldx, M, K, group_rows, _p(codes), width, _p(scales), stream)
+
+
+_FP8L_ARGS = [c_int] + [c_void_p] * 7 + [c_int] * 3 + [ctypes.c_longlong, c_int, c_void_p, c_void_p]
+
+
+def linear_fp8(codes, scales, w_codes, w_scales, bias, out, status, stream, epilogue: int = EPI_NONE, residual=None) -> None:
+    """``linear_generic``'s contract for rows and weights in 8-bit floating point (``fp8_quantize``): ``out = act(x w^T + bias) (+ residual)``
+    with ``x`` and ``w`` the numbers that codes and scales stand for, float32 sums and epilogue; ``out`` (and ``residual``, which may be ``out``)
+    bfloat16 or float32.  Up to ``FP8_FEW_ROWS`` rows run in the kernel that streams the weights, more on tiles of rows.  ``status`` receives
+    ``ST_WAIT_TIMEOUT`` if a bounded wait gives up."""
+    M, N = out.shape
+    if M == 0:
+        return
+    rows, K, groups = _fp8_pair(codes, scales, M, "linear (8 bits) x")
+    n, k, w_groups = _fp8_pair(w_codes, w_scales, N, "linear (8 bits) w")
+    if (rows, groups) != (M, 1) or (n, k, w_groups) != (N, K, 1):
+        raise KernelError(f"linear (8 bits): x {tuple(codes.shape)}, w {tuple(w_codes.shape)}, out {tuple(out.shape)}")
+    _need(out, None, "linear (8 bits) out")
+    _need(status, torch.int32, "linear (8 bits) status")
+    ldo = _rows(out, "linear (8 bits) out")
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"linear (8 bits): output dtype {out.dtype}")
+    if bias is not None:
+        _need(bias, torch.float32, "linear (8 bits) bias")
+        if bias.numel() != N or not bias.is_contiguous():
+            raise KernelError(f"linear (8 bits): bias of {bias.numel()} for {N} outputs")
+    if residual is not None:
+        _need(residual, out.dtype, "linear (8 bits) residual")
+        if residual.shape != out.shape or _rows(residual, "linear (8 bits) residual") != ldo:
+            raise KernelError("linear (8 bits): residual must have the output's shape and row stride")
+    if len({t.device for t in (codes, w_codes, bias, out, status, residual) if t is not None}) > 1:
+        raise KernelError("linear (8 bits): tensors on different devices")
+    _fp8_here(codes, "linear (8 bits)")
+    few = M <= FP8_FEW_ROWS
+    _call("fp8_few" if few else "fp8_many", "mlxb_fp8_linear_few" if few else "mlxb_fp8_linear_many", _FP8L_ARGS,
+          int(out.dtype == torch.float32), _p(codes), _p(scales), _p(w_codes), _p(w_scales), _p(bias), _p(residual), _p(out), M, N, K, ldo,
+          int(epilogue), _p(status), stream)
+
+
+def moe_fp8_tile_rows(n_slots: int, n_experts: int) -> int:
+    """Slots a tile of a plan for ``moe_gemm_fp8`` had best take, by how many an expert gets on average."""
+    each = n_slots / max(1, n_experts)
+    return 16 if each <= 8 else 32 if each <= 16 else 64 if each <= 32 else 128
+
+
+def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, what: str) -> None:
+    for t, name in ((sorted_slots, "sorted"), (tile_info, "tile_info"), (n_tiles, "n_tiles")):
+        _need(t, torch.int32, f"{what} {name}")
+        if not t.is_contiguous():
+            raise KernelError(f"{what}: {name} is not contiguous")
+    if tile_rows not in (16, 32, 64, 128) or tile_info.numel() < 3 * max_tiles or n_tiles.numel() < 1:
+        raise KernelError(f"{what}: tiles of {tile_rows} rows (16, 32, 64 or 128), room for {tile_info.numel() // 3} of {max_tiles}")
+
+
+_FP8G_ARGS = [c_int, c_void_p, ctypes.c_longlong, c_int, c_int] + [c_void_p] * 3 + [c_int, c_int, c_void_p, c_int, c_void_p, c_void_p]
+
+
+def moe_gather_fp8(x, a_div: int, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, codes, scales, stream) -> None:
+    """The rows ``x[slot // a_div]`` of a plan's slots in 8-bit floating point (``fp8_quantize``): place ``i`` of tile ``t`` is row ``t * tile_rows + i`` of
+    ``codes``, and every tile is a matrix of its own in ``scales`` (``fp8_empty(tile_rows, columns, device, groups=max_tiles)``).  Rows of a tile
+    behind its last slot, and tiles behind the last, are left as they were."""
+    _need(x, None, "moe_gather_fp8 x")
+    ldx = _rows(x, "moe_gather_fp8 x")
+    _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gather_fp8")
+    rows, width, groups = _fp8_pair(codes, scales, tile_rows, "moe_gather_fp8")
+    if groups < max_tiles or width != (x.shape[1] + 15) // 16 * 16 or codes.device != x.device or a_div <= 0 or sorted_slots.numel() > x.shape[0] * a_div:
+        raise KernelError(f"moe_gather_fp8: x {tuple(x.shape)}, {sorted_slots.numel()} slots, {a_div} a row, codes {tuple(codes.shape)} for {max_tiles} tiles")
+    _fp8_here(x, "moe_gather_fp8")
+    _call("fp8_rows", "mlxb_fp8_gather", _FP8G_ARGS, dtype_code(x.dtype), _p(x), ldx, x.shape[1], int(a_div), _p(sorted_slots), _p(tile_info),
+          _p(n_tiles), int(max_tiles), int(tile_rows), _p(codes), width, _p(scales), stream)
+
+
+_FP8E_FEW = ([c_int, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 3
+             + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_int, c_float, c_void_p])
+_FP8E_MANY = ([c_int, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 2
+              + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_int, c_float, c_void_p])
+
+
+def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, out, status, stream,
+                 sel_weight=None, gated: bool = False, out_scales=None, unit: str = "silu", limit: float = 0.0) -> None:
+    """The experts' products over a plan with weights in 8-bit floating point.  ``codes``, ``scales``: the slots' rows by tiles (``moe_gather_fp8``, or
+    the gated product's result).  ``gated``: ``w_codes`` is a stack of two matrices an expert, gate rows and up rows, and the result is the gated
+    unit of the two products (``unit``, ``limit`` and the slot's routing weight as in ``moe_gemm``), in float32 and then in 8-bit floating point: ``out``
+    and ``out_scales`` by tiles, as the second product reads them.  Else ``w_codes`` is one matrix an expert and the product of place ``i`` of the plan goes to row
+    ``sorted_slots[i]`` of ``out`` (bfloat16 or float32).  Rows of no slot are left as they were.  ``status`` receives ``ST_WAIT_TIMEOUT`` if
+    a bounded wait gives up."""
+    _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gemm_fp8")
+    rows, K, groups = _fp8_pair(codes, scales, tile_rows, "moe_gemm_fp8 a")
+    if w_scales.dim() != 4 or w_codes.dim() != 2 or not w_scales.shape[0] or w_scales.shape[0] % (2 if gated else 1):
+        raise KernelError(f"moe_gemm_fp8: weights {tuple(w_codes.shape)} with scales {tuple(w_scales.shape)}")
+    n_out = w_codes.shape[0] // w_scales.shape[0]
+    _, k, w_groups = _fp8_pair(w_codes, w_scales, n_out, "moe_gemm_fp8 w")
+    E = w_groups // (2 if gated else 1)
+    S = sorted_slots.numel()
+    if groups < max_tiles or k != K:
+        raise KernelError(f"moe_gemm_fp8: rows {tuple(codes.shape)} for {max_tiles} tiles of {tile_rows}, weights {tuple(w_codes.shape)}")
+    _need(status, torch.int32, "moe_gemm_fp8 status")
+    if gated:
+        o_rows, ldo, o_groups = _fp8_pair(out, out_scales, tile_rows, "moe_gemm_fp8 out")
+        if o_groups < max_tiles or ldo != (n_out + 15) // 16 * 16:
+            raise KernelError(f"moe_gemm_fp8: {n_out} columns of {max_tiles} tiles into {tuple(out.shape)}")
+        if sel_weight is not None:
+            _need(sel_weight, torch.float32, "moe_gemm_fp8 sel_weight")
+            if sel_weight.numel() < S or not sel_weight.is_contiguous():
+                raise KernelError(f"moe_gemm_fp8: {sel_weight.numel()} weights for {S} slots")
+    else:
+        _need(out, None, "moe_gemm_fp8 out")
+        ldo = _rows(out, "moe_gemm_fp8 out")
+        if out.dtype not in (torch.bfloat16, torch.float32) or out.shape[0] < S or out.shape[1] != n_out:
+            raise KernelError(f"moe_gemm_fp8: {S} rows of {n_out} into {out.dtype} {tuple(out.shape)}")
+    if len({t.device for t in (codes, w_codes, sorted_slots, tile_info, n_tiles, out, status)}) > 1:
+        raise KernelError("moe_gemm_fp8: tensors on different devices")
+    _fp8_here(codes, "moe_gemm_fp8")
+    args = [int(bool(gated)), int(out.dtype == torch.float32), _p(codes), _p(scales), _p(w_codes), _p(w_scales), E, n_out, K, _p(sorted_slots),
+            _p(tile_info), _p(n_tiles), groups, min(int(max_tiles), S)]
+    tail = [_p(sel_weight) if gated else None, _p(out), ldo, _p(out_scales) if gated else None, _p(status), GATED_UNITS[unit], float(limit), stream]
+    if tile_rows == 128:
+        _call("fp8_many", "mlxb_fp8_experts_many", _FP8E_MANY, *args, *tail)
+    else:
+        _call("fp8_few", "mlxb_fp8_experts_few", _FP8E_FEW, *args, int(tile_rows), *tail)
+
+
+# --------------------------------------------------------------------------
+# the router with the plan of the experts' products (csrc/moe_router.cu)
+
+MOE_GROUP_SCORES = {"best": 0, "two": 1}
+
+
+def moe_route_scratch(n_tokens: int, n_experts: int) -> int:
+    """Elements of int32 scratch memory that ``moe_route_plan`` wants for a step of ``n_tokens``."""
+    f, _ = _fn("moe_router", "mlxb_moe_route_scratch", [c_int, c_int])
+    return int(f(int(n_tokens), int(n_experts)))
+
+
+_ROUTE_PLAN_ARGS = ([c_void_p, ctypes.c_longlong, c_void_p, c_void_p] + [c_int] * 9 + [c_float, c_float] + [c_void_p] * 3 + [c_int, c_int]
+                    + [c_void_p] * 4)
+
+
+def moe_route_plan(logits, token_req, top: int, sel_expert, sel_weight, tile_rows: int, sorted_slots, tile_info, n_tiles, scratch, stream,
+                   score: str = "sigmoid", renormalize: bool = False, correction=None, groups: int = 1, keep_groups: int = 1, group_score: str = "best",
+                   identity: int = 0, renormalize_eps: float = 0.0, weight_scale: float = 1.0) -> None:
+    """``moe_route`` and ``moe_plan`` in one call, with a choice that is exact and a plan in a fixed order.  ``group_score``: a group is judged by its
+    ``best`` choice score or by the sum of its ``two`` best.  Of equal scores the lower index is chosen; scores that float32 cannot tell apart
+    are formed again in 64 bits.  A score that is NaN is never chosen, a place nobody can take gets expert -1 and weight 0.  The plan: slots sorted by
+    expert and, within one, by number (``sorted_slots``), tiles of at most ``tile_rows`` of them (``tile_info``, ``n_tiles``); what lies behind the last slot
+    and tile is left as it was.  ``scratch``: int32, ``moe_route_scratch`` elements.  Up to 1024 experts, 128 groups, 64 choices."""
+    _need(logits, torch.float32, "moe_route_plan logits")
+    ldl = _rows(logits, "moe_route_plan logits")
+    T, E = logits.shape
+    S, n_real = T * int(top), E - int(identity)
+    if score not in MOE_SCORES or group_score not in MOE_GROUP_SCORES:
+        raise KernelError(f"moe_route_plan: score {score!r}, groups judged by {group_score!r}")
+    max_tiles = moe_max_tiles(S, max(0, n_real), max(1, int(tile_rows)))
+    _need(sel_weight, torch.float32, "moe_route_plan sel_weight")
+    for t, n, what in ((sel_expert, S, "sel_expert"), (sel_weight, S, "sel_weight"), (sorted_slots, S, "sorted"), (tile_info, 3 * max_tiles, "tile_info"),
+                       (n_tiles, 1, "n_tiles"), (scratch, moe_route_scratch(T, E), "scratch")):
+        _need(t, None if t is sel_weight else torch.int32, "moe_route_plan " + what)
+        if t.numel() < n or not t.is_contiguous():
+            raise KernelError(f"moe_route_plan: {what} of {t.numel()} elements for {T} tokens and {top} of {E} experts: {n} in one piece")
+    if token_req is not None:
+        _need(token_req, torch.int32, "moe_route_plan token_req")
+        if token_req.numel() < T or not token_req.is_contiguous():
+            raise KernelError(f"moe_route_plan: requests of {token_req.numel()} tokens for {T}")
+    if correction is not None:
+        _need(correction, torch.float32, "moe_route_plan correction")
+        if correction.numel() != E or not correction.is_contiguous():
+            raise KernelError(f"moe_route_plan: a correction of {correction.numel()} for {E} experts")
+    _fp8_here(logits, "moe_route_plan")
+    _call("moe_router", "mlxb_moe_route_plan", _ROUTE_PLAN_ARGS, _p(logits), ldl, _p(token_req), _p(correction), T, E, int(top), MOE_SCORES[score],
+          MOE_GROUP_SCORES[group_score], int(groups), int(keep_groups), n_real, int(bool(renormalize)), float(renormalize_eps), float(weight_scale),
+          _p(sel_expert), _p(sel_weight), _p(scratch), int(tile_rows), max_tiles, _p(sorted_slots), _p(tile_info), _p(n_tiles), stream)
 
 
 # --------------------------------------------------------------------------

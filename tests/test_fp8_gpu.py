@@ -1,0 +1,257 @@
+"""Weights in 8-bit floating point: rows into codes, linear layers, the experts' products, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import fp8_refs as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+    from mlx_lm_b200 import ops as o
+    return o
+
+
+def normal(shape, seed, dtype=torch.float32, outliers=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g)
+    if outliers and len(shape) == 2 and shape[1] > 3:
+        x[:, 3::61] *= 8.0
+    return x.to(dtype).cuda()
+
+
+def kept(w, group_rows=None):
+    o = ops()
+    rows = w.shape[0] if group_rows is None else group_rows
+    codes, scales = o.fp8_empty(rows, w.shape[1], w.device, groups=w.shape[0] // rows)
+    o.fp8_quantize(w, codes, scales, o.current_stream(), group_rows=rows)
+    return codes, scales
+
+
+def status():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------------ rows
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,columns,group", [(1, 1, 1), (1, 16, 1), (3, 100, 3), (5, 128, 5), (129, 513, 129), (40, 1000, 20), (300, 640, 300),
+                                                (260, 1504, 130), (7, 4096, 7)])
+def test_rows(rows, columns, group, dtype):
+    x = normal((rows, columns), rows + columns, dtype)
+    codes, scales = kept(x, group)
+    want_c, want_e = ref.held(x)
+    got_c, got_e = ref.read(codes, scales, columns, group)
+    assert torch.equal(got_e, want_e)
+    assert torch.equal(got_c, want_c)
+    assert not codes.view(torch.uint8)[:, columns:].any()
+
+
+def test_rows_at_the_borders():
+    """Ties, the largest code, numbers just above it, subnormal codes and scales, signed zeros, and what is not finite."""
+    rows = [[448.0, 1.0], [449.0, 1.0], [464.0, 29.0], [448.0 * 2 ** 100, 2.0 ** 98], [2.0 ** -140, 2.0 ** -141], [0.0, -0.0], [3.4e38, 1.0],
+            [1.0, 2.0 ** -9], [256.0, 2.0 ** -10], [256.0, 1.5 * 2.0 ** -9], [256.0, 17.0], [256.0, 19.0], [-448.0, 18.0],
+            [math.inf, 1.0], [-math.inf, 300.0], [math.nan, 5.0], [math.nan, math.inf]]
+    x = torch.tensor(rows, dtype=torch.float32).repeat(1, 100).cuda()
+    codes, scales = kept(x)
+    want_c, want_e = ref.held(x)
+    got_c, got_e = ref.read(codes, scales, 200, len(rows))
+    assert torch.equal(got_e, want_e)
+    assert torch.equal(torch.nan_to_num(got_c, nan=1e9), torch.nan_to_num(want_c, nan=1e9))
+
+
+def test_rows_of_a_view():
+    """Strided rows, a base that is not 16-byte aligned."""
+    wide = normal((50, 700), 3, torch.bfloat16)
+    for x in (wide[:, 8:8 + 512], wide[:, 1:1 + 512], wide[:, 3:3 + 130], wide[::2, 16:16 + 256]):
+        codes, scales = kept(x)
+        want_c, want_e = ref.held(x)
+        got_c, got_e = ref.read(codes, scales, x.shape[1], x.shape[0])
+        assert torch.equal(got_c, want_c) and torch.equal(got_e, want_e)
+
+
+# ------------------------------------------------------------------------------------------------ linear layers
+
+def bound(x, w, out_dtype):
+    """How far a sum of K products may be off: the products are exact, each addition rounds the sum so far (and a tensor core may cut off
+    what lies below 2^-24 of the largest of 32 it adds), so K 2^-23 of the sum of magnitudes bounds it; it stays far below since
+    roundings cancel.  Half a step of the output's type on top."""
+    K = x.shape[1]
+    return (x.abs() @ w.abs().T) * (K * 2.0 ** -23 if K < 64 else 8.0 * math.sqrt(K) * 2.0 ** -23)
+
+
+def check_linear(M, N, K, x_dtype=torch.bfloat16, out_dtype=torch.bfloat16, bias=False, act="none", residual=False, pad=0, seed=0):
+    o = ops()
+    x, w = normal((M, K), seed + 1, x_dtype), normal((N, K), seed + 2, torch.bfloat16, outliers=False) * K ** -0.5
+    b = normal((N,), seed + 3) if bias else None
+    room = torch.full((M, N + pad), 7.0, dtype=out_dtype, device="cuda")
+    out = room[:, :N]
+    res = normal((M, N), seed + 4).to(out_dtype) if residual else None
+    if residual:
+        out.copy_(res)
+    st = status()
+    xc, xs = kept(x)
+    wc, ws = kept(w)
+    o.linear_fp8(xc, xs, wc, ws, b, out, st, o.current_stream(), epilogue=o.ACTIVATION_CODES[act], residual=out if residual else None)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    xv, wv = ref.values(x), ref.values(w)
+    y = xv @ wv.T
+    off = bound(xv, wv, out_dtype)
+    if bias:
+        y = y + b.double()
+        off = off + y.abs() * 2.0 ** -24
+    z = ref.ACTS[act](y)
+    # slopes are at most 1.13 (gelu_new); its fast form is 2^-20 of its argument off at most, in bfloat16 runs
+    off = 1.13 * off + (z.abs() + 1e-3) * (2.0 ** -18 if act != "none" else 0.0)
+    if residual:
+        z = z + res.double()
+        off = off + z.abs() * 2.0 ** -24
+    off = off + z.abs() * torch.finfo(out_dtype).eps / 2 + 1e-30
+    err = (out.double() - z).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= off).all(), f"{float((err / off).max())} of the bound at {M} x {N} x {K}"
+    if pad:
+        assert (room[:, N:] == 7.0).all()
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 32, 33, 64, 65, 127, 128])
+@pytest.mark.parametrize("N,K", [(128, 128), (64, 1024), (200, 400)])
+def test_linear_few_rows(M, N, K):
+    check_linear(M, N, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (3, 1, 16), (16, 5, 30), (1, 129, 2100), (64, 1280, 5120), (8, 300, 8192), (1, 50257, 768), (20, 1000, 129)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_linear_few_sizes(M, N, K, out_dtype):
+    check_linear(M, N, K, out_dtype=out_dtype, bias=True, residual=True)
+
+
+@pytest.mark.parametrize("M,N,K", [(129, 128, 128), (256, 256, 128), (257, 300, 640), (400, 1000, 1000), (517, 1501, 1000), (1000, 136, 4096), (640, 2048, 512),
+                                   (300, 40, 16), (2048, 1600, 1600)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_linear_many_sizes(M, N, K, out_dtype):
+    check_linear(M, N, K, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("M", [9, 300])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu_new", "tanh"])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_epilogues(M, act, out_dtype, residual):
+    check_linear(M, 333, 272, out_dtype=out_dtype, bias=True, act=act, residual=residual, pad=3)
+
+
+# ------------------------------------------------------------------------------------------------ experts
+
+def planned(sel, n_experts, tile_rows, most=None):
+    """A plan on the device for the choices ``sel`` (a list), with room behind it."""
+    order, tiles = ref.plan(sel, n_experts, tile_rows)
+    most = -(-len(sel) // tile_rows) + n_experts if most is None else most
+    dev = dict(dtype=torch.int32, device="cuda")
+    return (torch.tensor(order + [-1] * (len(sel) - len(order)), **dev), torch.tensor(tiles + [(-1, -1, -1)] * (most - len(tiles)), **dev),
+            torch.tensor([len(tiles)], **dev), most, tile_rows)
+
+
+@pytest.mark.parametrize("tile_rows", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("columns", [72, 512, 1000])
+def test_gather(tile_rows, dtype, columns):
+    o = ops()
+    T, top, E = 50, 3, 5
+    g = torch.Generator().manual_seed(columns)
+    sel = torch.randint(-1, E, (T * top,), generator=g).tolist()
+    x = normal((T, columns), 1, dtype)
+    plan = planned(sel, E, tile_rows)
+    codes, scales = o.fp8_empty(tile_rows, columns, "cuda", groups=plan[3])
+    codes.view(torch.uint8).fill_(1)
+    scales.fill_(2)
+    o.moe_gather_fp8(x, top, *plan, codes, scales, o.current_stream())
+    got_c, got_e = ref.read(codes, scales, columns, tile_rows)
+    order, tiles = ref.plan(sel, E, tile_rows)
+    touched = torch.zeros(codes.shape[0], dtype=torch.bool, device="cuda")
+    for t, (_, first, n) in enumerate(tiles):
+        rows = torch.tensor([s // top for s in order[first:first + n]], device="cuda")
+        want_c, want_e = ref.held(x[rows])
+        assert torch.equal(got_c[t * tile_rows:t * tile_rows + n], want_c)
+        assert torch.equal(got_e[t * tile_rows:t * tile_rows + n], want_e)
+        touched[t * tile_rows:t * tile_rows + n] = True
+    assert (codes.view(torch.uint8)[~touched] == 1).all()
+
+
+def check_experts(T, top, E, D, F, tile_rows, unit="silu", limit=0.0, weighted=True, out_dtype=torch.float32, seed=0, sel=None, empty=0.1):
+    """Both products; the hidden rows are taken from the device for the second, so that each is held to its own bound."""
+    o = ops()
+    g = torch.Generator().manual_seed(seed)
+    if sel is None:
+        sel = [-1 if torch.rand((), generator=g) < empty else int(torch.randint(0, E, (), generator=g)) for _ in range(T * top)]
+    S = T * top
+    x = normal((T, D), seed + 1, torch.bfloat16)
+    w_in = normal((E * 2 * F, D), seed + 2, torch.bfloat16, outliers=False) * D ** -0.5
+    w_out = normal((E * D, F), seed + 3, torch.bfloat16, outliers=False) * F ** -0.5
+    weight = torch.rand(S, generator=g).cuda() if weighted else None
+    plan = planned(sel, E, tile_rows)
+    order, tiles = ref.plan(sel, E, tile_rows)
+    codes, scales = o.fp8_empty(tile_rows, D, "cuda", groups=plan[3])
+    hc, hs = o.fp8_empty(tile_rows, F, "cuda", groups=plan[3])
+    st, out = status(), torch.full((S, D), 3.0, dtype=out_dtype, device="cuda")
+    stream = o.current_stream()
+    wi, wo = kept(w_in, F), kept(w_out, D)
+    o.moe_gather_fp8(x, top, *plan, codes, scales, stream)
+    o.moe_gemm_fp8(codes, scales, *wi, *plan, hc, st, stream, sel_weight=weight, gated=True, out_scales=hs, unit=unit, limit=limit)
+    o.moe_gemm_fp8(hc, hs, *wo, *plan, out, st, stream)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    xv, wiv, wov = ref.values(x), ref.values(w_in).view(E, 2, F, D), ref.values(w_out).view(E, D, F)
+    h_all, (_, h_exp) = ref.numbers(hc, hs, F, tile_rows), ref.read(hc, hs, F, tile_rows)
+    written = torch.zeros(S, dtype=torch.bool, device="cuda")
+    for t, (e, first, n) in enumerate(tiles):
+        slots = torch.tensor(order[first:first + n], device="cuda")
+        rows = xv[slots // top]
+        gate, up = rows @ wiv[e, 0].T, rows @ wiv[e, 1].T
+        wgt = (weight[slots] if weighted else torch.ones(n, device="cuda")).double()[:, None]
+        h = ref.unit(unit, gate, up, wgt, limit)
+        got_h = h_all[t * tile_rows:t * tile_rows + n]
+        # the float32 sums' bound through the unit (its slopes are below 1.1 |w| (1 + |the other factor|)), then half a step of the code: 2^-4
+        # of the value, or 2^-10 of the scale below 2^-6 of it; a scale one power up where a float32 magnitude crossed its border
+        off = 1.2 * wgt * (bound(rows, wiv[e, 0], None) * (1 + up.abs()) + bound(rows, wiv[e, 1], None) * (1 + gate.abs())) + h.abs() * 2.0 ** -20
+        scale = torch.ldexp(torch.ones_like(h), h_exp[t * tile_rows:t * tile_rows + n].repeat_interleave(ref.RUN, 1)[:, :F])
+        err = (got_h - h).abs()
+        assert (err <= off + torch.maximum((h.abs() + off) * 2.0 ** -4, scale * 2.0 ** -10)).all(), (t, float(err.max()))
+        top_h = torch.nn.functional.pad(h.abs(), (0, -F % ref.RUN)).view(n, -1, ref.RUN).amax(-1)
+        got_scale = torch.ldexp(torch.ones_like(top_h), h_exp[t * tile_rows:t * tile_rows + n])
+        assert (top_h <= 448.0 * got_scale * (1 + 1e-4)).all() and ((top_h >= 224.0 * got_scale * (1 - 1e-4)) | (top_h == 0)).all()
+        y = got_h @ wov[e].T
+        got = out[slots].double()
+        assert ((got - y).abs() <= bound(got_h, wov[e], None) + y.abs() * torch.finfo(out_dtype).eps / 2 + 1e-30).all(), t
+        written[slots] = True
+    assert (out[~written] == 3.0).all()
+
+
+@pytest.mark.parametrize("tile_rows", [16, 32, 64, 128])
+@pytest.mark.parametrize("D,F", [(128, 128), (256, 640), (200, 72), (1000, 520), (2048, 768)])
+def test_experts(tile_rows, D, F):
+    check_experts(37, 3, 6, D, F, tile_rows)
+
+
+@pytest.mark.parametrize("T,top,E,tile_rows", [(1, 1, 1, 16), (1, 8, 64, 16), (2, 2, 2, 32), (64, 8, 8, 64), (300, 4, 16, 128), (500, 2, 3, 16),
+                                               (700, 1, 2, 64), (90, 8, 40, 128)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_experts_counts(T, top, E, tile_rows, out_dtype):
+    check_experts(T, top, E, 384, 272, tile_rows, out_dtype=out_dtype, seed=T)
+
+
+@pytest.mark.parametrize("tile_rows", [16, 128])
+@pytest.mark.parametrize("unit,weighted", [("silu", False), ("bounded", True), ("bounded", False)])
+def test_experts_units(tile_rows, unit, weighted):
+    check_experts(40, 2, 4, 256, 200, tile_rows, unit=unit, limit=2.0, weighted=weighted)
+
+
+@pytest.mark.parametrize("tile_rows", [16, 128])
+def test_experts_of_one_and_of_nobody(tile_rows):
+    """All slots on one expert; all but one slot on nobody; none at all."""
+    check_experts(60, 2, 5, 256, 128, tile_rows, sel=[3] * 120)
+    check_experts(60, 2, 5, 256, 128, tile_rows, sel=[-1] * 119 + [4])
+    check_experts(60, 2, 5, 256, 128, tile_rows, sel=[-1] * 120)
