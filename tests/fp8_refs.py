@@ -77,7 +77,7 @@ def route(logits, live, top, score="sigmoid", correction=None, groups=1, keep=1,
             weight.append([0.0] * top)
             continue
         if score == "sigmoid":
-            s = [1.0 / (1.0 + math.exp(-v)) if v > -700 else 0.0 for v in z]
+            s = [v if v != v else 1.0 / (1.0 + math.exp(-v)) if v > -700 else 0.0 for v in z]
         else:
             m = max(v for v in z if v == v)
             x = [math.exp(v - m) if v == v else math.nan for v in z]
