@@ -12,6 +12,7 @@
 // column r / 32, byte b % 4.  Groups: the matrices of a stack (experts), or the tiles of a plan.
 #pragma once
 
+#include "gated_unit.cuh"
 #include "tcgen05.cuh"
 
 constexpr int FP8_RUN = 128;                 // columns with one scale
@@ -30,12 +31,10 @@ __device__ __forceinline__ uint32_t fp8_magnitude(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
 }
-// Two codes (the first in the low byte) of numbers that were scaled; not finite: NaN (0x7f).  The conversion itself saturates, infinities
-// too, so these are made NaN before it.
+// what the conversion is to make NaN of: it saturates by itself, infinities too
+__device__ __forceinline__ float fp8_or_nan(float v) { return fabsf(v) < INFINITY ? v : __uint_as_float(0x7fffffffu); }
+// Codes of numbers that were scaled, the first in the low byte.
 __device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
-  const float nan = __uint_as_float(0x7fffffffu);
-  lo = fabsf(lo) < INFINITY ? lo : nan;
-  hi = fabsf(hi) < INFINITY ? hi : nan;
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
@@ -99,6 +98,17 @@ __device__ __forceinline__ void fp8_drain(uint64_t* bar, uint32_t parity) {
                  : "=r"(done) : "r"(addr), "r"(parity) : "memory");
     if (done) return;
   }
+}
+
+// The gated unit of gated_unit.cuh with the hardware's exponential and quotient (some 2^-21 of the value off; the result is rounded to 8 bits).
+__device__ __forceinline__ float fp8_gated_unit(int kind, float g, float u, float w, float limit) {
+  if (kind == MLXB_GU_BOUNDED) {
+    g = fminf(g, limit);
+    u = fminf(fmaxf(u, -limit), limit);
+    return w * __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
+  }
+  const float a = w * g;
+  return __fdividef(a, 1.f + __expf(-a)) * (w * u);
 }
 
 // ---- host side: a matrix of codes, `rows` of `cols` bytes at a row stride of `ld` bytes, in boxes of box_rows x 128 columns

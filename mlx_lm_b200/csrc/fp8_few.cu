@@ -23,7 +23,6 @@
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
 #include "activations.cuh"
 #include "fp8.cuh"
-#include "gated_unit.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
 
@@ -246,7 +245,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       for (int j = 0; j < CH; ++j) {
         const bool on = tok0 + j < live;
         const float wgt = on && sel_weight ? sel_weight[sorted[first + tok0 + j]] : 1.f;
-        v[j] = on && n < a.N ? mlxb_gated_unit(a.act, v[j], u[j], wgt, a.limit) : 0.f;
+        v[j] = on && n < a.N ? fp8_gated_unit(a.act, v[j], u[j], wgt, a.limit) : 0.f;
         const uint32_t top = __reduce_max_sync(0xffffffffu, fp8_magnitude(v[j]));
         if (lane == j) sm.top[flip][q][j] = top;
       }
@@ -257,7 +256,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const uint32_t top = max(max(sm.top[flip][0][j], sm.top[flip][1][j]), max(sm.top[flip][2][j], sm.top[flip][3][j]));
         const int e = fp8_exponent(top);
         const long long row = (long long)tile * NT + tok0 + j;
-        if (n < a.ldo) reinterpret_cast<uint8_t*>(a.out)[row * a.ldo + n] = (uint8_t)fp8_pair(v[j] * fp8_power(-e), 0.f);
+        if (n < a.ldo) reinterpret_cast<uint8_t*>(a.out)[row * a.ldo + n] = (uint8_t)fp8_pair(fp8_or_nan(v[j]) * fp8_power(-e), 0.f);
         if (in_tile == 0) {
           const int run = n0 >> 7;
           a.out_scales[((long long)tile * a.out_kgs + (run >> 2)) * FP8_TILE + fp8_scale_row(tok0 + j) + (run & 3)] = (uint8_t)(e + 127);
@@ -317,12 +316,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         if (c >= live) continue;
         if (SPLIT) {
-          const int share = NT / ranks;
+          const int share = NT / ranks, shift = 31 - __clz(share);       // powers of two
+          const float* mine = &sm.sums[rank * share * NH * 128 + in_tile];
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
             if (c + j >= live) break;
-            const int to = (c + j) / share, i = c + j - to * share;
-            const uint32_t at = peer_addr(&sm.sums[((rank * share + i) * NH) * 128 + in_tile], (uint32_t)to);
+            const uint32_t at = peer_addr(mine + ((c + j) & (share - 1)) * NH * 128, (uint32_t)((c + j) >> shift));
 #pragma unroll
             for (int h = 0; h < NH; ++h)
               asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + (uint32_t)(h * 512)), "r"(r[h][j]) : "memory");

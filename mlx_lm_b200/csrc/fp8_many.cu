@@ -18,7 +18,6 @@
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
 #include "activations.cuh"
 #include "fp8.cuh"
-#include "gated_unit.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
 
@@ -291,14 +290,29 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
         const float wgt = live && sel_weight ? sel_weight[sorted[first + row]] : 1.f;
         const int n0 = p.n * 128 + half * 64;
         uint32_t top = 0;
+        auto units = [&](auto kind) {
+          constexpr int KIND_OF = decltype(kind)::value;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float h = n0 + 32 * c + i < a.N ? mlxb_gated_unit(a.act, __uint_as_float(r[c][i]), __uint_as_float(r[2 + c][i]), wgt, a.limit) : 0.f;
-            r[c][i] = __float_as_uint(h);
-            top = max(top, fp8_magnitude(h));
-          }
+            for (int i = 0; i < 32; ++i) {
+              r[c][i] = __float_as_uint(fp8_gated_unit(KIND_OF, __uint_as_float(r[c][i]), __uint_as_float(r[2 + c][i]), wgt, a.limit));
+              if (n0 + 64 > a.N && n0 + 32 * c + i >= a.N) r[c][i] = 0u;
+              top = max(top, r[c][i] & 0x7fffffffu);
+            }
+        };
+        if (a.act == MLXB_GU_BOUNDED) units(std::integral_constant<int, MLXB_GU_BOUNDED>{});
+        else units(std::integral_constant<int, MLXB_GU_SILU>{});
+        if (top >= 0x7f800000u) {             // rare: something is not finite
+          top = 0;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              top = max(top, fp8_magnitude(__uint_as_float(r[c][i])));
+              r[c][i] = __float_as_uint(fp8_or_nan(__uint_as_float(r[c][i])));
+            }
+        }
         // the other warp has the other half of the run's columns
         uint32_t* mine = reinterpret_cast<uint32_t*>(stg);
         const uint32_t* other = reinterpret_cast<const uint32_t*>(sm.stage[(warp - 2) ^ 4]);

@@ -13,60 +13,86 @@ MLXB_DEFINE_LAST_ERROR()
 
 constexpr int FQ_WARPS = 8;
 
-// 16 numbers from column c on; zeros behind column K.  VEC: K, the row's stride and its address are such that 16 of them are whole 16-byte pieces.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* row, int c, int K, float (&v)[16]) {
-  if (VEC) {
-    if (c < K) {
-      const uint4* p = reinterpret_cast<const uint4*>(row + c);
-      if (sizeof(T) == 2) {
-        const uint4 a = p[0], b = p[1];
-        float lo[8], hi[8];
-        unpack8(a, lo);
-        unpack8(b, hi);
+// 16 neighbours of a row of T, as they lie in memory; zeros behind column K.  VEC: K, the row's stride and its address are such that 16 of them
+// are whole 16-byte pieces.
+template <typename T>
+struct Sixteen {
+  uint32_t w[4 * sizeof(T)];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* row, int c, int K) {
+    if (VEC) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { v[i] = lo[i]; v[8 + i] = hi[i]; }
-      } else {
+      for (int i = 0; i < (int)sizeof(T); ++i) {
+        const uint4 u = c < K ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+      }
+    } else if (sizeof(T) == 2) {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 a = p[i];
-          v[4 * i] = __uint_as_float(a.x); v[4 * i + 1] = __uint_as_float(a.y);
-          v[4 * i + 2] = __uint_as_float(a.z); v[4 * i + 3] = __uint_as_float(a.w);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t lo = c + 2 * i < K ? p[c + 2 * i] : 0u, hi = c + 2 * i + 1 < K ? p[c + 2 * i + 1] : 0u;
+        w[i] = lo | hi << 16;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      for (int i = 0; i < 16; ++i) w[i] = c + i < K ? reinterpret_cast<const uint32_t*>(row)[c + i] : 0u;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c + i < K ? to_f(row[c + i]) : 0.f;
   }
+  __device__ __forceinline__ float number(int i) const {
+    if (sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    return __uint_as_float(w[i]);
+  }
+  // the bits (of a float32) of the largest magnitude, not finite ones too
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t top = 0;
+    if (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i] & 0x7fff7fffu));
+      return max(top << 16, top & 0xffff0000u);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, w[i] & 0x7fffffffu);
+    return top;
+  }
+};
+
+__device__ __forceinline__ uint32_t run_max(uint32_t v) {        // over the eight lanes of a run
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
 // 512 columns from 512 * kg on of one row, by a warp: codes to `out` (the row), the four scales to `scale` (the row's word in its tile)
-template <typename T, bool VEC>
-__device__ __forceinline__ void quantize512(const T* row, int kg, int K, int ld, uint8_t* out, uint8_t* scale, int lane) {
+template <typename T>
+__device__ __forceinline__ void quantize512(const Sixteen<T>& x, int kg, int ld, uint8_t* out, uint8_t* scale, int lane) {
   const int c = 512 * kg + 16 * lane;
-  float v[16];
-  load16<T, VEC>(row, c, K, v);
-  uint32_t top = 0;
+  uint32_t top = run_max(x.largest());
+  const bool odd = __any_sync(0xffffffffu, top >= 0x7f800000u);   // rare: something is not finite
+  if (odd) {
+    top = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, fp8_magnitude(v[i]));
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < 16; ++i) top = max(top, fp8_magnitude(x.number(i)));
+    top = run_max(top);
+  }
   const int e = fp8_exponent(top);
   const float f = fp8_power(-e);
-  uint4 u;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = fp8_quad(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
-  if (c < ld) *reinterpret_cast<uint4*>(out + c) = u;
+  for (int i = 0; i < 4; ++i) w[i] = fp8_quad(x.number(4 * i) * f, x.number(4 * i + 1) * f, x.number(4 * i + 2) * f, x.number(4 * i + 3) * f);
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = fp8_quad(fp8_or_nan(x.number(4 * i)) * f, fp8_or_nan(x.number(4 * i + 1)) * f, fp8_or_nan(x.number(4 * i + 2)) * f, fp8_or_nan(x.number(4 * i + 3)) * f);
+  }
+  if (c < ld) *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
   uint32_t s = (uint32_t)(e + 127) << (8 * (lane >> 3));
   s |= __shfl_xor_sync(0xffffffffu, s, 8);
   s |= __shfl_xor_sync(0xffffffffu, s, 16);
   if (lane == 0) *reinterpret_cast<uint32_t*>(scale) = s;
 }
+
+// FQ_AT_ONCE items of a warp have their loads out together.
+constexpr int FQ_AT_ONCE = 2;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * FQ_WARPS)
@@ -74,14 +100,21 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
   pdl_wait();
   pdl_trigger();
   x = after_wait(x);
-  const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9;
-  const long long w = (long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5);
-  const long long r = w / kgs;
-  if (r >= rows) return;
-  const int kg = (int)(w - r * kgs);
-  const int group = (int)(r / group_rows), in = (int)(r - (long long)group * group_rows);
-  const int tiles = (group_rows + 127) >> 7;
-  quantize512<T, VEC>(x + r * ldx, kg, K, ld, codes + r * ld, scales + (((long long)group * tiles + (in >> 7)) * kgs + kg) * FP8_TILE + fp8_scale_row(in), lane);
+  const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, tiles = (group_rows + 127) >> 7;
+  const long long items = (long long)rows * kgs, first = ((long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5)) * FQ_AT_ONCE;
+  Sixteen<T> v[FQ_AT_ONCE];
+#pragma unroll
+  for (int j = 0; j < FQ_AT_ONCE; ++j) {
+    const long long w = min(first + j, items - 1), r = w / kgs;
+    v[j].template load<VEC>(x + r * ldx, 512 * (int)(w - r * kgs) + 16 * lane, K);
+  }
+#pragma unroll
+  for (int j = 0; j < FQ_AT_ONCE; ++j) {
+    const long long w = first + j, r = w / kgs;
+    if (w >= items) return;
+    const int kg = (int)(w - r * kgs), group = (int)(r / group_rows), in = (int)(r - (long long)group * group_rows);
+    quantize512<T>(v[j], kg, ld, codes + r * ld, scales + (((long long)group * tiles + (in >> 7)) * kgs + kg) * FP8_TILE + fp8_scale_row(in), lane);
+  }
 }
 
 template <typename T, bool VEC>
@@ -95,12 +128,22 @@ fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted
   tile_info = after_wait(tile_info);
   const int t = blockIdx.x;
   if (t >= after_wait(n_tiles)[0]) return;
-  const int first = tile_info[3 * t + 1], items = tile_info[3 * t + 2];
-  const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9;
-  for (int w = blockIdx.y * FQ_WARPS + (threadIdx.x >> 5); w < items * kgs; w += gridDim.y * FQ_WARPS) {
-    const int r = w / kgs, kg = w - r * kgs;
-    const long long src = sorted[first + r] / a_div;
-    quantize512<T, VEC>(x + src * ldx, kg, K, ld, codes + ((long long)t * tile_rows + r) * ld, scales + ((long long)t * kgs + kg) * FP8_TILE + fp8_scale_row(r), lane);
+  const int first = tile_info[3 * t + 1], kgs = (K + 511) >> 9, items = tile_info[3 * t + 2] * kgs;
+  const int lane = threadIdx.x & 31;
+  for (int w0 = (blockIdx.y * FQ_WARPS + (threadIdx.x >> 5)) * FQ_AT_ONCE; w0 < items; w0 += gridDim.y * FQ_WARPS * FQ_AT_ONCE) {
+    Sixteen<T> v[FQ_AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < FQ_AT_ONCE; ++j) {
+      const int w = min(w0 + j, items - 1), r = w / kgs;
+      const long long src = sorted[first + r] / a_div;
+      v[j].template load<VEC>(x + src * ldx, 512 * (w - r * kgs) + 16 * lane, K);
+    }
+#pragma unroll
+    for (int j = 0; j < FQ_AT_ONCE; ++j) {
+      const int w = w0 + j, r = w / kgs, kg = w - r * kgs;
+      if (w < items)
+        quantize512<T>(v[j], kg, ld, codes + ((long long)t * tile_rows + r) * ld, scales + ((long long)t * kgs + kg) * FP8_TILE + fp8_scale_row(r), lane);
+    }
   }
 }
 
@@ -121,7 +164,7 @@ MLXB_EXPORT int mlxb_fp8_quantize(int dtype, const void* x, long long ldx, int r
   if (rows <= 0) return 0;
   if (int e = check("fp8_quantize", x, K, ldx, codes, ld, scales)) return e;
   if (group_rows <= 0 || rows % group_rows) return mlxb_fail(MLXB_BAD_ARG, "fp8_quantize: %d rows in groups of %d", rows, group_rows);
-  const long long blocks = ((long long)rows * ((K + 511) / 512) + FQ_WARPS - 1) / FQ_WARPS;
+  const long long blocks = ((long long)rows * ((K + 511) / 512) + FQ_WARPS * FQ_AT_ONCE - 1) / (FQ_WARPS * FQ_AT_ONCE);
   if (blocks > 0x7fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "fp8_quantize: %d rows of %d", rows, K);
 #define GO(T, V)                                                                                                                             \
   launch_pdl(fp8_quantize_kernel<T, V>, dim3((unsigned)blocks), dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, rows, K, group_rows, \

@@ -108,12 +108,12 @@ __device__ __noinline__ void choose_exactly(const RouterArgs& a, const float* z,
 
 // One token by one warp.  VPT experts a lane, neighbours.  sS: [E] scores, sC: room for [E] doubles, sPick: [top].
 template <int VPT>
-__device__ __forceinline__ void route_token(const RouterArgs& a, int t, float* sS, double* sC, int* sPick, int* sCount, int lane) {
+__device__ __forceinline__ void route_token(const RouterArgs& a, const float* logits, int t, float* sS, double* sC, int* sPick, int* sCount, int lane) {
   if (a.token_req && a.token_req[t] < 0) {
     for (int c = lane; c < a.top; c += 32) { a.sel[(size_t)t * a.top + c] = -1; a.weight[(size_t)t * a.top + c] = 0.f; }
     return;
   }
-  const float* z = a.logits + (size_t)t * a.ldl;
+  const float* z = logits + (size_t)t * a.ldl;
   const int e0 = lane * VPT;
   float s[VPT];
   uint32_t key[VPT];
@@ -316,7 +316,7 @@ __device__ __forceinline__ void plan_experts(const RouterArgs& a, const int* sTo
 // ONE: the whole step in this block, with its plan.  Shared memory: counts [E], places [E], by warp: scores [E], doubles [E], picks [top]; the
 // plan's [RP_WARPS][E] lie over the latter.
 template <int VPT, bool ONE>
-__global__ void __launch_bounds__(RP_THREADS) route_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(RP_THREADS) route_kernel(const __grid_constant__ RouterArgs a) {
   extern __shared__ __align__(16) uint8_t rp_smem[];
   int* sCount = reinterpret_cast<int*>(rp_smem);
   int* sFirst = sCount + a.E;
@@ -327,11 +327,11 @@ __global__ void __launch_bounds__(RP_THREADS) route_kernel(RouterArgs a) {
   for (int e = threadIdx.x; e < a.E; e += RP_THREADS) sCount[e] = 0;
   pdl_wait();
   pdl_trigger();
-  a.logits = after_wait(a.logits);
+  const float* logits = after_wait(a.logits);
   __syncthreads();
   const int t0 = blockIdx.x * a.tokens_a_block, t1 = min(a.T, t0 + a.tokens_a_block);
   for (int t = t0 + warp; t < t1; t += RP_WARPS)
-    route_token<VPT>(a, t, sS + (size_t)warp * a.E, sC + (size_t)warp * a.E, sPick + warp * a.top, sCount, lane);
+    route_token<VPT>(a, logits, t, sS + (size_t)warp * a.E, sC + (size_t)warp * a.E, sPick + warp * a.top, sCount, lane);
   __syncthreads();
   if (ONE) {
     plan_experts(a, sCount, sFirst, true);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(RP_THREADS) route_kernel(RouterArgs a) {
   }
 }
 
-__global__ void __launch_bounds__(RP_THREADS) plan_kernel(RouterArgs a, int blocks) {
+__global__ void __launch_bounds__(RP_THREADS) plan_kernel(const __grid_constant__ RouterArgs a, int blocks) {
   extern __shared__ __align__(16) uint8_t rp_smem[];
   int* sTotal = reinterpret_cast<int*>(rp_smem);
   int* sFirst = sTotal + a.E;
