@@ -5,20 +5,24 @@
 //            scores (ties: the lower index); weights: the scores s, divided by their sum plus eps if wanted, times a factor.
 // plan       the (token, choice) slots sorted by expert and, within one, by number; tiles of at most tile_rows slots of one expert.
 //
-// The choice is exact.  Without a correction the order of the scores is the order of the logits.  With one, or where sums of two decide, a warp
-// compares the float32 scores it forms first, and where a choice was by less than they can be off (2^-20 of a score's range, some 16 times their
-// error) it forms that token's scores again in 64 bits.  A score that is NaN, or that a correction makes minus infinity, is never chosen; places
-// that nobody can take hold expert -1 and weight 0.
+// The choice is exact: without a correction scores are in the order of the logits, and these are compared; with one, a warp compares float32 scores, which it forms with the hardware's exponential and quotient, and where any choice was by less than they can be off it forms the token's scores again in 64 bits and chooses
+// by those.  A score that is NaN, or that a correction makes minus infinity, is never chosen; places that nobody can take hold expert -1 and weight 0.
 //
-// A warp takes a token, a lane neighbouring experts, so that the lowest lane with the largest number has the lowest index: a choice is one
-// redux.sync and one vote.  Steps of up to 64 tokens are one block and one launch.  More are two launches: blocks of tokens that also count
-// their slots by expert, then the same blocks, which add up the counts before theirs and put their slots in place.  No atomics decide
-// an order.
+// A warp takes a token, a lane neighbouring experts.  Each lane sorts its scores once (a network of minima and maxima); a choice is then a redux.sync
+// over the lanes' best, a vote, and a shift in the lane that had it.  Groups: 2^p lanes search one
+// group's scores in shared memory and merge their two best; a group's rank is the number of better ones.
+//
+// Steps of up to 128 tokens are one launch: a cluster of up to eight CTAs, a warp a token, of which the first makes the plan.  More are two launches:
+// blocks of tokens that also count their slots by expert, then the same blocks, which add up the counts before theirs and put their slots in place.
+// No atomics decide an order.
+#include <float.h>
+
 #include "common.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
 
-constexpr int RP_THREADS = 512, RP_WARPS = RP_THREADS / 32, RP_ONE_BLOCK = 64, RP_MOST_BLOCKS = 148;
+constexpr int RP_THREADS = 512, RP_WARPS = RP_THREADS / 32, RP_CLUSTER = 8, RP_ONE_LAUNCH = RP_CLUSTER * RP_WARPS, RP_MOST_BLOCKS = 148;
+constexpr int PL_THREADS = 1024, PL_WARPS = PL_THREADS / 32;
 
 struct RouterArgs {
   const float* logits;
@@ -26,11 +30,12 @@ struct RouterArgs {
   const int* token_req;
   const float* correction;
   int T, E, top, softmax, two, groups, keep, n_real, renorm;
+  int part;                    // lanes that search a group: a power of two, part * groups <= 32 (0: more than 32 groups)
   float eps, factor;
   int* sel;
   float* weight;
-  int* counts;                 // [blocks][E] slots by expert of each block of tokens
-  int tokens_a_block, tile_rows, max_tiles;
+  int* counts;                 // [blocks][n_real] slots by expert of each block of tokens
+  int tokens_a_block, tile_rows, tile_shift, max_tiles;       // tile_shift: -1 where tile_rows is no power of two
   int *sorted, *tile_info, *n_tiles;
 };
 
@@ -41,74 +46,120 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 }
 __device__ __forceinline__ float number_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// The choice in 64 bits, for tokens whose float32 scores are too close: plain and slow.  sC: [E] doubles of this warp.
+__device__ __forceinline__ unsigned long long order_of(double v) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  return v == v ? (b >> 63 ? ~b : b | 1ull << 63) : 0ull;
+}
+
+// The choice in 64 bits, for tokens whose float32 scores are too close.  sC: [E] doubles of this warp.  No two scores are taken for different
+// that are equal here; of equal ones the lower index is chosen.
+template <int VPT>
 __device__ __noinline__ void choose_exactly(const RouterArgs& a, const float* z, float zmax, double* sC, int* sPick, int lane) {
-  double sum = 0.;
-  if (a.softmax) {
-    for (int e = lane; e < a.E; e += 32) sum += z[e] == z[e] ? exp((double)z[e] - (double)zmax) : 0.;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int e0 = lane * VPT, per = a.E / a.groups;
+  double v[VPT], sum = 0.;
+#pragma unroll 1
+  for (int i = 0; i < VPT; ++i) {
+    const double x = e0 + i < a.E ? (double)z[e0 + i] : NAN;
+    if (a.softmax && x == x) sum += exp(x - (double)zmax);
   }
-  for (int e = lane; e < a.E; e += 32) {
-    double s = a.softmax ? exp((double)z[e] - (double)zmax) / sum : 1. / (1. + exp(-(double)z[e]));
-    if (a.correction) s += (double)a.correction[e];
-    sC[e] = s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  // what the choice goes by (without a correction: the logits), NaN out of the race; in shared memory what groups are judged by
+#pragma unroll 1
+  for (int i = 0; i < VPT; ++i) {
+    const int e = e0 + i;
+    const double x = e < a.E ? (double)z[e] : NAN;
+    const double s = a.softmax ? exp(x - (double)zmax) / sum : 1. / (1. + exp(-x));
+    const double c = s + (a.correction && e < a.E ? (double)a.correction[e] : 0.);
+    if (e < a.E) sC[e] = !(c > -INFINITY) ? NAN : a.correction || a.two ? c : x;
   }
   __syncwarp();
-  const int per = a.E / a.groups;
-  uint32_t kept[4] = {~0u, ~0u, ~0u, ~0u};                 // of up to 128 groups
-  if (a.keep < a.groups) {
-    kept[0] = kept[1] = kept[2] = kept[3] = 0;
-    for (int c = 0; c < a.keep; ++c) {
-      double best = -INFINITY;
-      int best_g = 0x7fffffff;
-      for (int g = lane; g < a.groups; g += 32) {
-        if (kept[g >> 5] >> (g & 31) & 1) continue;
-        double b1 = -INFINITY, b2 = -INFINITY;
-        int n = 0;
-        for (int i = 0; i < per; ++i) {
-          const double v = sC[g * per + i];
-          if (!(v > -INFINITY)) continue;
-          ++n;
-          if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) { b2 = v; }
-        }
-        const double v = a.two && n > 1 ? b1 + b2 : b1;
-        if (n && (best_g == 0x7fffffff || v > best)) { best = v; best_g = g; }
-      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double ob = __shfl_xor_sync(0xffffffffu, best, o);
-        const int og = __shfl_xor_sync(0xffffffffu, best_g, o);
-        if (og != 0x7fffffff && (best_g == 0x7fffffff || ob > best || (ob == best && og < best_g))) { best = ob; best_g = og; }
-      }
-      if (best_g != 0x7fffffff) kept[best_g >> 5] |= 1u << (best_g & 31);
+  for (int i = 0; i < VPT; ++i) {
+    v[i] = e0 + i < a.E ? sC[e0 + i] : NAN;
+    if (!a.correction && v[i] == v[i]) v[i] = (double)z[e0 + i];
+  }
+  if (a.keep < a.groups) {
+    unsigned long long judged[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int g = lane + 32 * x;
+      double b1 = -INFINITY, b2 = -INFINITY;
+      bool any = false, two = false;
+      if (g < a.groups)
+        for (int i = 0; i < per; ++i) {
+          const double c = sC[g * per + i];
+          if (!(c == c)) continue;
+          two = any;
+          any = true;
+          if (c > b1) { b2 = b1; b1 = c; } else if (c > b2) { b2 = c; }
+        }
+      judged[x] = any ? order_of(a.two && two ? b1 + b2 : b1) : 0ull;
+    }
+    __syncwarp();
+    unsigned long long* all = reinterpret_cast<unsigned long long*>(sC);     // [groups], no more than experts
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (lane + 32 * x < a.groups) all[lane + 32 * x] = judged[x];
+    __syncwarp();
+    uint32_t kept[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      int better = 0;
+      if (lane + 32 * x < a.groups)
+        for (int g = 0; g < a.groups; ++g) better += all[g] > judged[x] || (all[g] == judged[x] && g < lane + 32 * x);
+      kept[x] = __ballot_sync(0xffffffffu, judged[x] != 0ull && better < a.keep);
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int g = (e0 + i) / per;
+      const uint32_t bits = g < 32 ? kept[0] : g < 64 ? kept[1] : g < 96 ? kept[2] : kept[3];
+      if (!(bits >> (g & 31) & 1)) v[i] = NAN;
     }
   }
   for (int c = 0; c < a.top; ++c) {
-    double best = -INFINITY;
-    int best_e = 0x7fffffff;
-    for (int e = lane; e < a.E; e += 32) {
-      const int g = e / per;
-      const double v = sC[e];
-      if (!(v > -INFINITY) || !(kept[g >> 5] >> (g & 31) & 1)) continue;
-      if (best_e == 0x7fffffff || v > best) { best = v; best_e = e; }
-    }
+    unsigned long long best = 0ull;
+    int at = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ob = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-      if (oe != 0x7fffffff && (best_e == 0x7fffffff || ob > best || (ob == best && oe < best_e))) { best = ob; best_e = oe; }
+    for (int i = 0; i < VPT; ++i) {
+      const unsigned long long k = order_of(v[i]);
+      if (k > best) { best = k; at = i; }
     }
-    if (lane == 0) sPick[c] = best_e == 0x7fffffff ? -1 : best_e;
-    __syncwarp();
-    if (best_e != 0x7fffffff && (best_e & 31) == lane) sC[best_e] = NAN;
-    __syncwarp();
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+    const unsigned long long top = (unsigned long long)hi << 32 | lo;
+    const int l = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+    if (lane == l) {
+      sPick[c] = top ? e0 + at : -1;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (i == at) v[i] = NAN;
+    }
   }
+  __syncwarp();
 }
 
-// One token by one warp.  VPT experts a lane, neighbours.  sS: [E] scores, sC: room for [E] doubles, sPick: [top].
+// Descending, by a network of comparisons (odd-even merging).
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t x = k[i + j], y = k[i + j + q];
+            k[i + j] = max(x, y);
+            k[i + j + q] = min(x, y);
+          }
+}
+
+// One token by one warp.  VPT (a power of two) experts a lane, neighbours.  sC: room for [E] doubles, sPick: [top].
 template <int VPT>
-__device__ __forceinline__ void route_token(const RouterArgs& a, const float* logits, int t, float* sS, double* sC, int* sPick, int* sCount, int lane) {
+__device__ __forceinline__ void route_token(const RouterArgs& a, const float* logits, int t, double* sC, int* sPick, int* sCount, int lane) {
   if (a.token_req && a.token_req[t] < 0) {
     for (int c = lane; c < a.top; c += 32) { a.sel[(size_t)t * a.top + c] = -1; a.weight[(size_t)t * a.top + c] = 0.f; }
     return;
@@ -116,150 +167,151 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
   const float* z = logits + (size_t)t * a.ldl;
   const int e0 = lane * VPT;
   float s[VPT];
-  uint32_t key[VPT];
+  if (VPT >= 4 && !(a.ldl & 3) && !(a.E & 3) && !((uintptr_t)logits & 15)) {
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) s[i] = e0 + i < a.E ? z[e0 + i] : NAN;
-  float zmax = -INFINITY;
+    for (int i = 0; i < VPT; i += 4) {
+      const float4 v = e0 + i < a.E ? *reinterpret_cast<const float4*>(z + e0 + i) : make_float4(NAN, NAN, NAN, NAN);
+      s[i] = v.x; s[(i + 1) % VPT] = v.y; s[(i + 2) % VPT] = v.z; s[(i + 3) % VPT] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) s[i] = e0 + i < a.E ? z[e0 + i] : NAN;
+  }
+  float v[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) v[i] = s[i];
+  float zmax = -INFINITY, sum = 0.f, range = 1.f;           // range: no score is larger
   if (a.softmax) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) zmax = fmaxf(zmax, s[i]);
     zmax = warp_max(zmax);
-  }
-  const bool by_logit = a.correction == nullptr;
-  if (by_logit) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) key[i] = order_of(s[i]);
-  }
-  float range = 1.f;                                        // no score is larger
-  if (a.softmax) {
-    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      s[i] = expf(s[i] - zmax);
+      s[i] = __expf(s[i] - zmax);
       sum += s[i] == s[i] ? s[i] : 0.f;
     }
     sum = warp_sum(sum);
-    range = 1.f / sum;
+    range = __fdividef(1.f, sum);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) s[i] = s[i] / sum;
+    for (int i = 0; i < VPT; ++i) s[i] *= range;
   } else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) s[i] = 1.f / (1.f + expf(-s[i]));
+    for (int i = 0; i < VPT; ++i) s[i] = __fdividef(1.f, 1.f + __expf(-s[i]));
   }
+  if (a.correction) {
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (e0 + i < a.E) sS[e0 + i] = s[i];
+    for (int i = 0; i < VPT; ++i) s[i] += e0 + i < a.E ? a.correction[e0 + i] : 0.f;
+  } else {                       // in the race: z is what the choice goes by
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const float c = s[i] + (!by_logit && e0 + i < a.E ? a.correction[e0 + i] : 0.f);
-    if (!(c > -INFINITY)) key[i] = 0;
-    else if (!by_logit) key[i] = order_of(c);
+    for (int i = 0; i < VPT; ++i) v[i] = s[i] == s[i] ? fmaxf(v[i], -FLT_MAX) : NAN;
+    if (!a.two) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) s[i] = v[i];
+    }
   }
+  // A score is off by less than 2^-22 of the range (sigmoid: a quarter of the exponential's relative error; softmax: that error grows with its
+  // argument, 2^-24 of it, but the value falls faster), its sum with a correction or of two by 2^-24 of itself.
   bool close = false;
-  auto near = [&](float hi, float lo) { return hi - lo <= 9.5e-7f * range + 4.8e-7f * (fabsf(hi) + fabsf(lo)); };
+  auto near = [&](float hi, float lo, bool logits) { return !(hi - lo > (logits ? 0.f : 9.6e-7f * range + 1.2e-7f * (fabsf(hi) + fabsf(lo)))); };
 
+  uint32_t kept = ~0u;                                      // by the first lane of a group
+  const int per = a.E / a.groups;
   if (a.keep < a.groups) {
-    // a group's members are neighbours, and so are the lanes that hold them; by logits, the sums of two want the scores
-    const int per = a.E / a.groups;
-    const bool sums = a.two && per > 1;
-    uint32_t mine[4];                                       // lane l: groups l, l + 32, ...
-#pragma unroll
-    for (int x = 0; x < 4; ++x) mine[x] = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const int lo = g * per, hi = lo + per;
-      uint32_t b1 = 0, b2 = 0;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const uint32_t k = e0 + i >= lo && e0 + i < hi ? key[i] : 0u;
-        if (k > b1) { b2 = b1; b1 = k; } else if (k > b2) { b2 = k; }
-      }
-      const uint32_t top1 = __reduce_max_sync(0xffffffffu, b1);
-      uint32_t v = top1;
-      if (sums && top1) {
-        const bool owner = __ffs(__ballot_sync(0xffffffffu, b1 == top1)) - 1 == lane;
-        const uint32_t top2 = __reduce_max_sync(0xffffffffu, owner ? b2 : b1);
-        float f1 = number_of(top1), f2 = top2 ? number_of(top2) : 0.f;
-        if (by_logit) {
-          f1 = a.softmax ? expf(f1 - zmax) * range : 1.f / (1.f + expf(-f1));
-          f2 = !top2 ? 0.f : a.softmax ? expf(f2 - zmax) * range : 1.f / (1.f + expf(-f2));
-        }
-        v = order_of(f1 + f2);
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (g == lane + 32 * x) mine[x] = v;
-    }
-    uint32_t kept[4] = {0, 0, 0, 0}, last = 0;
-    for (int c = 0; c <= a.keep; ++c) {                      // one more than stay: was the last choice close?
-      uint32_t b = 0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) b = max(b, mine[x]);
-      const uint32_t best = __reduce_max_sync(0xffffffffu, b);
-      if (c > 0 && best && near(number_of(last), number_of(best)) && (sums || !by_logit)) close = true;
-      if (!best || c == a.keep) break;
-      last = best;
-      bool done = false;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t who = __ballot_sync(0xffffffffu, mine[x] == best);
-        if (!done && who) {
-          const int l = __ffs(who) - 1;
-          kept[x] |= 1u << l;
-          if (lane == l) mine[x] = 0;
-          done = true;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int g = (e0 + i) / per;
-      uint32_t bits = kept[0];
-#pragma unroll
-      for (int x = 1; x < 4; ++x) bits = g >> 5 == x ? kept[x] : bits;
-      if (!(bits >> (g & 31) & 1)) key[i] = 0;
-    }
-  }
-
-  uint32_t last = 0;
-  for (int c = 0; c <= a.top; ++c) {
-    uint32_t b = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (key[i] > b) { b = key[i]; at = i; }
-    const uint32_t best = __reduce_max_sync(0xffffffffu, b);
-    if (c > 0 && best && last && !by_logit && near(number_of(last), number_of(best))) close = true;
-    if (c == a.top) break;
-    last = best;
-    const int l = __ffs(__ballot_sync(0xffffffffu, b == best)) - 1;
-    if (lane == l) {
-      sPick[c] = best ? e0 + at : -1;
+    if (a.part == 0) {
+      close = true;
+    } else {
+      float* sF = reinterpret_cast<float*>(sC);
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
-        if (i == at) key[i] = 0;
+        if (e0 + i < a.E) sF[e0 + i] = s[i];
+      __syncwarp();
+      const int g = lane / a.part, j = lane - g * a.part;
+      float b1 = -INFINITY, b2 = -INFINITY;
+      if (g < a.groups)
+        for (int i = j; i < per; i += a.part) {
+          const float x = sF[g * per + i];                  // NaN: neither maximum takes it
+          b2 = fmaxf(b2, fminf(b1, x == x ? x : -INFINITY));
+          b1 = fmaxf(b1, x);
+        }
+      for (int o = a.part >> 1; o > 0; o >>= 1) {
+        const float o1 = __shfl_xor_sync(0xffffffffu, b1, o), o2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
+        b1 = fmaxf(b1, o1);
+      }
+      const float score = a.two && b2 > -INFINITY ? b1 + b2 : b1;
+      int better = 0;
+      for (int x = 0; x < a.groups; ++x) {
+        const float other = __shfl_sync(0xffffffffu, score, x * a.part);
+        better += other > score || (other == score && x < g);
+      }
+      const bool mine = g < a.groups && score > -INFINITY, stays = mine && better < a.keep;
+      kept = __ballot_sync(0xffffffffu, stays && j == 0);
+      // the worst that stays against the best that goes
+      const uint32_t worst = __reduce_min_sync(0xffffffffu, stays ? order_of(score) : ~0u);
+      const uint32_t best = __reduce_max_sync(0xffffffffu, mine && !stays ? order_of(score) : 0u);
+      if (best && worst != ~0u && near(number_of(worst), number_of(best), !a.correction && !a.two)) close = true;
+      __syncwarp();
+    }
+  }
+
+  uint32_t key[VPT], was[VPT];
+  const float inv_per = 1.f / (float)per;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (a.correction) v[i] = s[i];
+    const int g = kept == ~0u ? 0 : (int)(((float)(e0 + i) + 0.5f) * inv_per);
+    const bool in = v[i] > -INFINITY && (kept == ~0u || kept >> ((g * a.part) & 31) & 1);
+    was[i] = key[i] = in ? order_of(v[i]) : 0u;
+  }
+  sort_down(key);
+  uint32_t last = 0;
+  for (int c = 0; c <= a.top; ++c) {                        // one more than are chosen: was the last choice close?
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
+    if (c > 0 && best && near(number_of(last), number_of(best), !a.correction)) { close = true; break; }
+    if (c == a.top) break;
+    last = best;
+    if (!best) {
+      for (int x = c + lane; x < a.top; x += 32) sPick[x] = -1;
+      break;
+    }
+    const int l = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+    if (lane == l) {
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) at = was[i] == best ? i : at;     // two equal ones are close
+      sPick[c] = e0 + at;
+#pragma unroll
+      for (int i = 0; i + 1 < VPT; ++i) key[i] = key[i + 1];
+      key[VPT - 1] = 0;
     }
   }
   __syncwarp();
-  if (close) choose_exactly(a, z, zmax, sC, sPick, lane);    // the same answer in every lane: all it goes by came from votes
+  if (close) choose_exactly<VPT>(a, z, zmax, sC, sPick, lane);    // the same answer in every lane: all it goes by came from votes
   __syncwarp();
-  float sum = 0.f;
-  for (int c = 0; c < a.top; ++c) sum += sPick[c] >= 0 ? sS[sPick[c]] : 0.f;
+  // the weights of those that were chosen, with the library's exponential
+  float mass = 0.f;
+  for (int c0 = 0; c0 < a.top; c0 += 32) {
+    const int e = c0 + lane < a.top ? sPick[c0 + lane] : -1;
+    const float w = e < 0 ? 0.f : a.softmax ? expf(z[e] - zmax) / sum : 1.f / (1.f + expf(-z[e]));
+    mass += a.renorm ? warp_sum(w) : 0.f;
+  }
   for (int c = lane; c < a.top; c += 32) {
     const int e = sPick[c];
-    float w = e >= 0 ? sS[e] : 0.f;
-    if (a.renorm && e >= 0) w = w / (sum + a.eps);
+    float w = e < 0 ? 0.f : a.softmax ? expf(z[e] - zmax) / sum : 1.f / (1.f + expf(-z[e]));
+    if (a.renorm && e >= 0) w = w / (mass + a.eps);
     a.weight[(size_t)t * a.top + c] = w * a.factor;
     a.sel[(size_t)t * a.top + c] = e < 0 ? -1 : e < a.n_real ? e : -2;
-    if (e >= 0 && e < a.n_real) atomicAdd(&sCount[e], 1);    // only a number of slots: no order comes of it
+    if (sCount && e >= 0 && e < a.n_real) atomicAdd(&sCount[e], 1);    // only a number of slots: no order comes of it
   }
   __syncwarp();
 }
 
-// Puts the slots first .. first + n - 1 of one block in place.  sBase [E]: the place of the block's next slot of each expert; sWarp [RP_WARPS][E].
+// Puts the slots first .. first + n - 1 of one block in place.  sBase [E]: the place of the block's next slot of each expert; sWarp [warps][E].
 __device__ __forceinline__ void place_slots(const RouterArgs& a, const int* sel, int first, int n, int* sBase, int* sWarp) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int at = 0; at < n; at += RP_THREADS) {
-    for (int i = threadIdx.x; i < RP_WARPS * a.n_real; i += RP_THREADS) sWarp[i] = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x, warps = threads >> 5;
+  for (int at = 0; at < n; at += threads) {
+    const int used = min(warps, (n - at + 31) >> 5);         // warps with slots in this round
+    for (int i = threadIdx.x; i < used * a.n_real; i += threads) sWarp[i] = 0;
     __syncthreads();
     const int i = at + threadIdx.x;
     int e = i < n ? sel[first + i] : -1;
@@ -268,9 +320,10 @@ __device__ __forceinline__ void place_slots(const RouterArgs& a, const int* sel,
     const int before = __popc(same & ((1u << lane) - 1u));
     if (e >= 0 && before == 0) sWarp[warp * a.n_real + e] = __popc(same);
     __syncthreads();
-    for (int x = threadIdx.x; x < a.n_real; x += RP_THREADS) {
+    for (int x = threadIdx.x; x < a.n_real; x += threads) {
       int acc = sBase[x];
-      for (int w = 0; w < RP_WARPS; ++w) {
+#pragma unroll 4
+      for (int w = 0; w < used; ++w) {
         const int c = sWarp[w * a.n_real + x];
         sWarp[w * a.n_real + x] = acc;
         acc += c;
@@ -283,12 +336,16 @@ __device__ __forceinline__ void place_slots(const RouterArgs& a, const int* sel,
   }
 }
 
-// From totals sTotal [n_real] by expert: places sFirst; `tiles`: writes the list of tiles too.  By the whole block.
-__device__ __forceinline__ void plan_experts(const RouterArgs& a, const int* sTotal, int* sFirst, bool tiles) {
+__device__ __forceinline__ int tiles_of(const RouterArgs& a, int n) {
+  return a.tile_shift >= 0 ? (n + a.tile_rows - 1) >> a.tile_shift : (n + a.tile_rows - 1) / a.tile_rows;
+}
+
+// From totals sTotal [n_real] by expert: places sFirst; `tiles`: writes the list of tiles too (sTile [n_real]).  By the whole block.
+__device__ __forceinline__ void plan_experts(const RouterArgs& a, const int* sTotal, int* sFirst, int* sTile, bool tiles) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, per = (a.n_real + 31) / 32, lo = lane * per, hi = min(a.n_real, lo + per);
     int n = 0, nt = 0;
-    for (int e = lo; e < hi; ++e) { n += sTotal[e]; nt += (sTotal[e] + a.tile_rows - 1) / a.tile_rows; }
+    for (int e = lo; e < hi; ++e) { n += sTotal[e]; nt += tiles_of(a, sTotal[e]); }
     int pn = n, pt = nt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -300,29 +357,32 @@ __device__ __forceinline__ void plan_experts(const RouterArgs& a, const int* sTo
     pt -= nt;
     for (int e = lo; e < hi; ++e) {
       sFirst[e] = pn;
-      if (tiles)
-        for (int r = 0; r < sTotal[e]; r += a.tile_rows, ++pt)
-          if (pt < a.max_tiles) {
-            a.tile_info[3 * pt] = e;
-            a.tile_info[3 * pt + 1] = pn + r;
-            a.tile_info[3 * pt + 2] = min(a.tile_rows, sTotal[e] - r);
-          }
+      sTile[e] = pt;
       pn += sTotal[e];
+      pt += tiles_of(a, sTotal[e]);
     }
   }
   __syncthreads();
+  if (tiles)
+    for (int e = threadIdx.x; e < a.n_real; e += blockDim.x)
+      for (int r = 0, t = sTile[e]; r < sTotal[e] && t < a.max_tiles; r += a.tile_rows, ++t) {
+        a.tile_info[3 * t] = e;
+        a.tile_info[3 * t + 1] = sFirst[e] + r;
+        a.tile_info[3 * t + 2] = min(a.tile_rows, sTotal[e] - r);
+      }
+  __syncthreads();                 // the places move on below
 }
 
-// ONE: the whole step in this block, with its plan.  Shared memory: counts [E], places [E], by warp: scores [E], doubles [E], picks [top]; the
+// ONE: the whole step in this cluster, with its plan.  Shared memory: totals, places and tiles [E], by warp: doubles [E], picks [top]; the
 // plan's [RP_WARPS][E] lie over the latter.
 template <int VPT, bool ONE>
 __global__ void __launch_bounds__(RP_THREADS) route_kernel(const __grid_constant__ RouterArgs a) {
   extern __shared__ __align__(16) uint8_t rp_smem[];
   int* sCount = reinterpret_cast<int*>(rp_smem);
   int* sFirst = sCount + a.E;
-  double* sC = reinterpret_cast<double*>(rp_smem + ((size_t)8 * a.E + 15) / 16 * 16);
-  float* sS = reinterpret_cast<float*>(sC + (size_t)RP_WARPS * a.E);
-  int* sPick = reinterpret_cast<int*>(sS + (size_t)RP_WARPS * a.E);
+  int* sTile = sFirst + a.E;
+  double* sC = reinterpret_cast<double*>(rp_smem + ((size_t)12 * a.E + 15) / 16 * 16);
+  int* sPick = reinterpret_cast<int*>(sC + (size_t)RP_WARPS * a.E);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += RP_THREADS) sCount[e] = 0;
   pdl_wait();
@@ -331,53 +391,69 @@ __global__ void __launch_bounds__(RP_THREADS) route_kernel(const __grid_constant
   __syncthreads();
   const int t0 = blockIdx.x * a.tokens_a_block, t1 = min(a.T, t0 + a.tokens_a_block);
   for (int t = t0 + warp; t < t1; t += RP_WARPS)
-    route_token<VPT>(a, logits, t, sS + (size_t)warp * a.E, sC + (size_t)warp * a.E, sPick + warp * a.top, sCount, lane);
-  __syncthreads();
+    route_token<VPT>(a, logits, t, sC + (size_t)warp * a.E, sPick + warp * a.top, ONE ? nullptr : sCount, lane);
   if (ONE) {
-    plan_experts(a, sCount, sFirst, true);
-    place_slots(a, after_wait(a.sel), 0, a.T * a.top, sFirst, reinterpret_cast<int*>(sC));
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // all choices are written
+    if (blockIdx.x != 0) return;
+    const int* sel = after_wait(a.sel);
+    for (int i = threadIdx.x; i < a.T * a.top; i += RP_THREADS) {
+      const int e = __ldcg(sel + i);
+      if (e >= 0 && e < a.n_real) atomicAdd(&sCount[e], 1);
+    }
+    __syncthreads();
+    plan_experts(a, sCount, sFirst, sTile, true);
+    place_slots(a, sel, 0, a.T * a.top, sFirst, reinterpret_cast<int*>(sC));
   } else {
+    __syncthreads();
     for (int e = threadIdx.x; e < a.n_real; e += RP_THREADS) a.counts[(size_t)blockIdx.x * a.n_real + e] = sCount[e];
   }
 }
 
-__global__ void __launch_bounds__(RP_THREADS) plan_kernel(const __grid_constant__ RouterArgs a, int blocks) {
+__global__ void __launch_bounds__(PL_THREADS) plan_kernel(const __grid_constant__ RouterArgs a, int blocks) {
   extern __shared__ __align__(16) uint8_t rp_smem[];
   int* sTotal = reinterpret_cast<int*>(rp_smem);
-  int* sFirst = sTotal + a.E;
-  int* sWarp = sFirst + a.E;                     // [RP_WARPS][E]
+  int* sBefore = sTotal + a.E;
+  int* sFirst = sBefore + a.E;
+  int* sTile = sFirst + a.E;
+  int* sWarp = sTile + a.E;                      // [PL_WARPS][E]
+  for (int e = threadIdx.x; e < a.n_real; e += PL_THREADS) sTotal[e] = sBefore[e] = 0;
   pdl_wait();
   pdl_trigger();
   const int* counts = after_wait(a.counts);
-  // totals, and what the blocks before this one hold, by warps over the blocks
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* sBefore = sWarp;
-  for (int e = threadIdx.x; e < a.n_real; e += RP_THREADS) sTotal[e] = sBefore[e] = 0;
   __syncthreads();
-  for (int e0 = 0; e0 < a.n_real; e0 += 32) {
-    const int e = e0 + lane;
+  // totals, and what the blocks before this one hold: each expert by several threads, every one a part of the blocks, eight loads out at a time
+  const int width = (a.n_real + 31) & ~31, parts = max(1, PL_THREADS / width);
+  for (int x = threadIdx.x; x < parts * width; x += PL_THREADS) {
+    const int part = x / width, e = x - part * width;
+    if (e >= a.n_real) continue;
     int all = 0, before = 0;
-    if (e < a.n_real)
-      for (int b = warp; b < blocks; b += RP_WARPS) {
-        const int c = counts[(size_t)b * a.n_real + e];
-        all += c;
-        if (b < blockIdx.x) before += c;
+    for (int b0 = part; b0 < blocks; b0 += 8 * parts) {
+      int c[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = b0 + j * parts < blocks ? counts[(size_t)(b0 + j * parts) * a.n_real + e] : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        all += c[j];
+        before += b0 + j * parts < (int)blockIdx.x ? c[j] : 0;
       }
-    if (e < a.n_real && all) { atomicAdd(&sTotal[e], all); atomicAdd(&sBefore[e], before); }
+    }
+    if (all) { atomicAdd(&sTotal[e], all); atomicAdd(&sBefore[e], before); }
   }
   __syncthreads();
-  plan_experts(a, sTotal, sFirst, blockIdx.x == 0);
-  for (int e = threadIdx.x; e < a.n_real; e += RP_THREADS) sFirst[e] += sBefore[e];
+  plan_experts(a, sTotal, sFirst, sTile, blockIdx.x == 0);
+  for (int e = threadIdx.x; e < a.n_real; e += PL_THREADS) sFirst[e] += sBefore[e];
   __syncthreads();
   const int t0 = blockIdx.x * a.tokens_a_block, t1 = min(a.T, t0 + a.tokens_a_block);
   place_slots(a, after_wait(a.sel), t0 * a.top, (t1 - t0) * a.top, sFirst, sWarp);
 }
 
-static int tokens_a_block(int T) { return T <= RP_ONE_BLOCK ? T : max(16, (T + RP_MOST_BLOCKS - 1) / RP_MOST_BLOCKS); }
+// Few tokens: a warp a token in as few CTAs of one cluster as that takes.  Many: one block an SM, at least a token a warp.
+static int tokens_a_block(int T) { return T <= RP_ONE_LAUNCH ? min(T, RP_WARPS) : max(RP_WARPS, (T + RP_MOST_BLOCKS - 1) / RP_MOST_BLOCKS); }
 
 // How many whole numbers of scratch memory a step of T tokens wants.
 MLXB_EXPORT int mlxb_moe_route_scratch(int T, int E) {
-  if (T <= RP_ONE_BLOCK || E <= 0) return 1;
+  if (T <= RP_ONE_LAUNCH || E <= 0) return 1;
   const int tpb = tokens_a_block(T);
   return (T + tpb - 1) / tpb * E;
 }
@@ -386,13 +462,26 @@ template <int VPT>
 static int route_launch(const RouterArgs& a, int blocks, size_t smem, cudaStream_t stream) {
   static SharedLimit one, many;
   constexpr size_t most = 227 * 1024;
-  if (blocks == 1) {
-    if (cudaError_t e = one.raise(route_kernel<VPT, true>, most)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
-    launch_pdl(route_kernel<VPT, true>, dim3(1), dim3(RP_THREADS), smem, stream, a);
-  } else {
+  if (a.T > RP_ONE_LAUNCH) {
     if (cudaError_t e = many.raise(route_kernel<VPT, false>, most)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
     launch_pdl(route_kernel<VPT, false>, dim3(blocks), dim3(RP_THREADS), smem, stream, a);
+    return mlxb_check_launch("moe_route_plan");
   }
+  if (cudaError_t e = one.raise(route_kernel<VPT, true>, most)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(RP_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = mlxb_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, route_kernel<VPT, true>, a);
   return mlxb_check_launch("moe_route_plan");
 }
 
@@ -410,11 +499,15 @@ MLXB_EXPORT int mlxb_moe_route_plan(const float* logits, long long ldl, const in
     const cudaError_t e = cudaMemsetAsync(n_tiles, 0, sizeof(int), stream);
     return e == cudaSuccess ? 0 : mlxb_fail((int)e, "moe_route_plan: %s", cudaGetErrorString(e));
   }
-  RouterArgs a = {logits, ldl, token_req, correction, T, E, top, softmax, two, groups, keep, n_real, renorm, eps, factor, sel, weight, counts,
-                  tokens_a_block(T), tile_rows, max_tiles, sorted, tile_info, n_tiles};
+  int part = 0, shift = -1;
+  for (int i = 0; i < 20; ++i)
+    if (tile_rows == 1 << i) shift = i;
+  if (groups <= 32)
+    for (part = 1; 2 * part * groups <= 32; part *= 2) {}
+  RouterArgs a = {logits, ldl, token_req, correction, T, E, top, softmax, two, groups, keep, n_real, renorm, part, eps, factor, sel, weight, counts,
+                  tokens_a_block(T), tile_rows, shift, max_tiles, sorted, tile_info, n_tiles};
   const int blocks = (T + a.tokens_a_block - 1) / a.tokens_a_block;
-  const size_t head = ((size_t)8 * E + 15) / 16 * 16;
-  const size_t smem = head + (size_t)RP_WARPS * (12 * (size_t)E + 4 * (size_t)top);
+  const size_t smem = ((size_t)12 * E + 15) / 16 * 16 + (size_t)RP_WARPS * (8 * (size_t)E + 4 * (size_t)top);
   int rc;
   if (E <= 32) rc = route_launch<1>(a, blocks, smem, stream);
   else if (E <= 64) rc = route_launch<2>(a, blocks, smem, stream);
@@ -422,9 +515,9 @@ MLXB_EXPORT int mlxb_moe_route_plan(const float* logits, long long ldl, const in
   else if (E <= 256) rc = route_launch<8>(a, blocks, smem, stream);
   else if (E <= 512) rc = route_launch<16>(a, blocks, smem, stream);
   else rc = route_launch<32>(a, blocks, smem, stream);
-  if (rc || blocks == 1) return rc;
+  if (rc || T <= RP_ONE_LAUNCH) return rc;
   static SharedLimit limit;
-  if (cudaError_t e = limit.raise(plan_kernel, 128 * 1024)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
-  launch_pdl(plan_kernel, dim3(blocks), dim3(RP_THREADS), sizeof(int) * (2 + (size_t)RP_WARPS) * E, stream, a, blocks);
+  if (cudaError_t e = limit.raise(plan_kernel, 160 * 1024)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
+  launch_pdl(plan_kernel, dim3(blocks), dim3(PL_THREADS), sizeof(int) * (4 + (size_t)PL_WARPS) * E, stream, a, blocks);
   return mlxb_check_launch("moe_route_plan (plan)");
 }
