@@ -51,11 +51,11 @@ template <int NT, int KIND, bool SPLIT>
 struct FewShape {
   static constexpr int NH = KIND == FEW_GATED ? 2 : 1;
   static constexpr int STAGE = NH * (16384 + FP8_TILE) + NT * 128 + FP8_TILE;
-  static constexpr int SUMS = SPLIT ? NH * NT * 512 : 0;              // bytes of partial sums that arrive
-  // two CTAs an SM where a stage is small (the next kernel's first weights are then on their way while this one ends)
-  static constexpr bool PAIR = NH == 1 && NT <= 64;
+  static constexpr int SUMS = SPLIT ? NH * (NT > 32 ? NT : 32) * 512 : 0;   // bytes of partial sums that arrive
+  // two CTAs an SM where tiles are split and stages small (the next kernel's first weights are then on their way while this one ends)
+  static constexpr bool PAIR = SPLIT && NH == 1 && NT <= 64;
   static constexpr int ROOM = (PAIR ? 112 : 224) * 1024 - SUMS - 2048;
-  static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
+  static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
   static constexpr int SCALES = 4 * NH + 4;                           // columns of a place for scales
   static constexpr int ACC = 2 * NH * NT + 4 * SCALES <= 512 ? 2 : 1;
   static constexpr int USED = ACC * NH * NT + 4 * SCALES;
@@ -69,7 +69,7 @@ struct FewSmem {
   alignas(1024) uint8_t x[S::STAGES][NT * 128];
   alignas(128) uint8_t ws[S::STAGES][S::NH * FP8_TILE];
   alignas(128) uint8_t xs[S::STAGES][FP8_TILE];
-  alignas(16) float sums[SPLIT ? S::NH * NT * 128 : 4];
+  alignas(16) float4 sums[SPLIT ? S::SUMS / 16 : 1];    // [rank][a share's tokens / 4][gate, up][row of W]
   uint32_t top[2][4][32];
   alignas(8) uint64_t full[S::STAGES];
   uint64_t empty[S::STAGES];
@@ -125,7 +125,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   fp8_before_sync();
   __syncthreads();
   fp8_after_sync();
-  if (SPLIT) cluster_sync();            // the others' shared memory is there
+  if (SPLIT) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // its other half stands before the first store to another CTA
   const uint32_t tmem = sm.tmem;
 
   // whether the stage of run k brings scales with it, and its bytes
@@ -291,7 +291,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     return KIND == FEW_LINEAR ? min(NT, a.M - tile * NT) : min(NT, tile_info[3 * tile + 2]);
   };
 
+  // tokens that a CTA of a cluster adds up and writes out
+  const int share = SPLIT ? max(4, NT / ranks) : NT;
   if (warp >= 2) {
+    if (SPLIT) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     int it = 0;
     for (int w = first_item; w < items; w += step, ++it) {
       const int b = S::ACC == 2 ? it & 1 : 0;
@@ -316,15 +319,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         if (c >= live) continue;
         if (SPLIT) {
-          const int share = NT / ranks, shift = 31 - __clz(share);       // powers of two
-          const float* mine = &sm.sums[rank * share * NH * 128 + in_tile];
+          const float4* mine = &sm.sums[rank * (share / 4) * NH * 128 + in_tile];
 #pragma unroll
-          for (int j = 0; j < CH; ++j) {
+          for (int j = 0; j < CH; j += 4) {
             if (c + j >= live) break;
-            const uint32_t at = peer_addr(mine + ((c + j) & (share - 1)) * NH * 128, (uint32_t)((c + j) >> shift));
+            const uint32_t at = peer_addr(mine + ((c + j) % share / 4) * NH * 128, (uint32_t)((c + j) / share));
 #pragma unroll
             for (int h = 0; h < NH; ++h)
-              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + (uint32_t)(h * 512)), "r"(r[h][j]) : "memory");
+              asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};"
+                           ::"r"(at + (uint32_t)(h * 2048)), "r"(r[h][j]), "r"(r[h][j + 1]), "r"(r[h][j + 2]), "r"(r[h][j + 3]) : "memory");
           }
         } else {
           float v[CH], u[CH];
@@ -337,23 +340,29 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   }
   if (SPLIT) {
     __syncwarp();
+    if (warp < 2) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     cluster_sync();                      // all sums have arrived
     if (warp >= 2 && first_item < items) {
-      const int share = NT / ranks, live = live_of(first_item);
+      const int live = live_of(first_item);
 #pragma unroll 1
       for (int c = 0; c < share; c += CH) {
         const int tok0 = rank * share + c, end = min(live, (rank + 1) * share);
         if (tok0 >= end) break;          // the same for all four warps
         float v[CH], u[CH];
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          v[j] = u[j] = 0.f;
-          if (tok0 + j < end)
-            for (int from = 0; from < ranks; ++from) {
-              const float* p = &sm.sums[((from * share + c + j) * NH) * 128 + in_tile];
-              v[j] += p[0];
-              if (NH == 2) u[j] += p[128];
+        for (int j = 0; j < CH; j += 4) {
+          v[j] = v[j + 1] = v[j + 2] = v[j + 3] = u[j] = u[j + 1] = u[j + 2] = u[j + 3] = 0.f;
+          if (tok0 + j < end) {
+            const float4* p = &sm.sums[(c + j) / 4 * NH * 128 + in_tile];
+            for (int from = 0; from < ranks; ++from, p += share / 4 * NH * 128) {
+              const float4 x = p[0];
+              v[j] += x.x; v[j + 1] += x.y; v[j + 2] += x.z; v[j + 3] += x.w;
+              if (NH == 2) {
+                const float4 y = p[128];
+                u[j] += y.x; u[j + 1] += y.y; u[j + 2] += y.z; u[j + 3] += y.w;
+              }
             }
+          }
         }
         finish(first_item, tok0, end, v, u);
       }
@@ -380,6 +389,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
 // CTAs that share a tile's K: as many as keep two an SM busy, no fewer than two runs each, and at least `of` tokens' columns to share out.
 static int few_ranks(long long items, int runs, int per_sm) {
+  if (const char* want = getenv("MLXB_FP8_RANKS")) return atoi(want);      // experiments and tests
   int r = 1;
   while (r < 8 && items * 2 * r <= (long long)per_sm * mlxb_sm_count() && runs >= 4 * r) r *= 2;
   return r;
@@ -422,7 +432,7 @@ static int few_launch(const CUtensorMap& mw, const CUtensorMap& mx, const FewArg
 template <int NT, int KIND, typename TO>
 static int few_choose(const CUtensorMap& mw, const CUtensorMap& mx, const FewArgs& a, cudaStream_t stream) {
   // a split hands every rank whole tokens, and its buffer must leave room for the stages
-  if constexpr (NT <= (KIND == FEW_GATED ? 32 : 64)) {
+  if constexpr (NT <= (KIND == FEW_GATED ? 32 : 128)) {
     const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR ? 2 : 1);
     if (ranks > 1) return few_launch<NT, KIND, true, TO>(mw, mx, a, ranks, stream);
   }
@@ -439,66 +449,60 @@ static int few_width(int nt, const CUtensorMap& mw, const CUtensorMap& mx, const
   }
 }
 
-static int few_check(const char* what, const void* x, const void* xs, const void* w, const void* ws, int N, int K, const void* out) {
-  if (!x || !xs || !w || !ws || !out || N <= 0 || K <= 0 || (K & 15) ||
-      (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws) & 15))
-    return mlxb_fail(MLXB_BAD_ARG, "%s: codes of %d x %d (rows of whole 16 bytes, 16-byte aligned)", what, N, K);
-  return 0;
-}
-
 // x codes [M, K], w codes [N, K] (rows of K bytes, K a multiple of 16), their scales as in fp8.cuh (one group each); bias float32 [N] or null;
 // residual of out's type at out's stride or null (may be out); out bfloat16 or float32 [M, N] at row stride ldo.
-MLXB_EXPORT int mlxb_fp8_linear_few(int out_f32, const void* x, const void* xs, const void* w, const void* ws, const float* bias, const void* residual,
-                                    void* out, int M, int N, int K, long long ldo, int epi, int* status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0) return 0;
-  if (int e = few_check("linear (8 bits)", x, xs, w, ws, N, K, out)) return e;
-  if (ldo < N || !activation_known(epi)) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d outputs at stride %lld, epilogue %d", N, ldo, epi);
+MLXB_EXPORT int mlxb_fp8_linear_few(const Fp8LinearRecord* rec, long long bytes, cudaStream_t stream) {
+  if (!rec || bytes != sizeof(Fp8LinearRecord)) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): a record of %lld bytes", bytes);
+  const Fp8LinearRecord& r = *rec;
+  if (r.M <= 0 || r.N <= 0) return 0;
+  if (int e = fp8_check("linear (8 bits)", r.x, r.xs, r.w, r.ws, r.out, r.M, r.N, r.K, r.ldo)) return e;
+  if (!activation_known((int)r.epi) || !r.status) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): epilogue %lld", r.epi);
+  const int M = (int)r.M, N = (int)r.N, K = (int)r.K;
   FewArgs a = {};
-  a.x_scales = (const uint8_t*)xs; a.w_scales = (const uint8_t*)ws;
+  a.x_scales = (const uint8_t*)r.xs; a.w_scales = (const uint8_t*)r.ws;
   a.M = M; a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.w_tiles = (N + 127) / 128;
-  a.bias = bias; a.residual = residual; a.out = out; a.ldo = ldo; a.status = status; a.act = epi;
+  a.bias = r.bias; a.residual = r.residual; a.out = r.out; a.ldo = r.ldo; a.status = r.status; a.act = (int)r.epi;
   const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const long long items = (long long)a.w_tiles * ((M + nt - 1) / nt);
   if (items > 0x7fffff) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d x %d outputs", M, N);
   a.max_items = (int)items;
   CUtensorMap mw, mx;
-  if (int e = fp8_make_map(&mw, w, N, K, K, 128, "linear (8 bits) w")) return e;
-  if (int e = fp8_make_map(&mx, x, M, K, K, nt, "linear (8 bits) x")) return e;
-  return out_f32 ? few_width<FEW_LINEAR, float>(nt, mw, mx, a, stream) : few_width<FEW_LINEAR, __nv_bfloat16>(nt, mw, mx, a, stream);
+  if (int e = fp8_make_map(&mw, r.w, N, K, K, 128, "linear (8 bits) w")) return e;
+  if (int e = fp8_make_map(&mx, r.x, M, K, K, nt, "linear (8 bits) x")) return e;
+  return r.out_f32 ? few_width<FEW_LINEAR, float>(nt, mw, mx, a, stream) : few_width<FEW_LINEAR, __nv_bfloat16>(nt, mw, mx, a, stream);
 }
 
 // Over a plan with tiles of tile_rows (16, 32 or 64) slots; x codes [max_tiles * tile_rows, K], a tile's rows at tile_rows * t, scales a group a tile.
 // gated: w codes [E][2][N][K] (gate rows, up rows), scales of 2 E groups of N rows; out codes [max_tiles * tile_rows, ldo] with their
 // scales, ldo = N rounded up to 16.  Else w codes [E][N][K]; out bfloat16 or float32 rows [S, ldo], row sorted[i] for place i of the plan.
 // at_most: a bound on the number of tiles.
-MLXB_EXPORT int mlxb_fp8_experts_few(int gated, int out_f32, const void* x, const void* xs, const void* w, const void* ws, int E, int N, int K,
-                                     const int* sorted, const int* tile_info, const int* n_tiles, int max_tiles, int at_most, int tile_rows,
-                                     const float* sel_weight, void* out, long long ldo, void* out_scales, int* status, int act, float limit,
-                                     cudaStream_t stream) {
-  if (max_tiles <= 0 || at_most <= 0) return 0;
-  if (int e = few_check("moe_gemm_fp8", x, xs, w, ws, N, K, out)) return e;
-  if (E <= 0 || ldo < N || (tile_rows != 16 && tile_rows != 32 && tile_rows != 64) || (gated && (!out_scales || ldo != ((N + 15) & ~15))) ||
-      (long long)E * N * 2 > 0x7fffffffLL || (long long)max_tiles * tile_rows > 0x7fffffffLL)
-    return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d experts of %d x %d, tiles of %d rows, results at stride %lld", E, N, K, tile_rows, ldo);
+MLXB_EXPORT int mlxb_fp8_experts_few(const Fp8ExpertsRecord* rec, long long bytes, cudaStream_t stream) {
+  if (!rec || bytes != sizeof(Fp8ExpertsRecord)) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: a record of %lld bytes", bytes);
+  const Fp8ExpertsRecord& r = *rec;
+  if (r.max_tiles <= 0 || r.at_most <= 0) return 0;
+  if (int e = fp8_check_experts(r)) return e;
+  if (r.tile_rows != 16 && r.tile_rows != 32 && r.tile_rows != 64) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: tiles of %lld rows", r.tile_rows);
+  const int N = (int)r.N, K = (int)r.K;
   FewArgs a = {};
-  a.x_scales = (const uint8_t*)xs; a.w_scales = (const uint8_t*)ws;
+  a.x_scales = (const uint8_t*)r.xs; a.w_scales = (const uint8_t*)r.ws;
   a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.w_tiles = (N + 127) / 128;
-  a.sorted = sorted; a.tile_info = tile_info; a.n_tiles = n_tiles; a.sel_weight = sel_weight;
-  a.out = out; a.ldo = ldo; a.out_scales = (uint8_t*)out_scales; a.out_kgs = (N + 511) / 512; a.status = status; a.act = act; a.limit = limit;
-  const long long items = (long long)min(max_tiles, at_most) * a.w_tiles;
-  if (items > 0x7fffff) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d tiles of %d outputs", max_tiles, N);
+  a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
+  a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
+  a.limit = (float)r.limit;
+  const long long items = min(r.max_tiles, r.at_most) * a.w_tiles;
+  if (items > 0x7fffff) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
   a.max_items = (int)items;
   CUtensorMap mw, mx;
-  if (int e = fp8_make_map(&mw, w, (long long)E * (gated ? 2 : 1) * N, K, K, 128, "moe_gemm_fp8 w")) return e;
-  if (int e = fp8_make_map(&mx, x, (long long)max_tiles * tile_rows, K, K, tile_rows, "moe_gemm_fp8 x")) return e;
+  if (int e = fp8_make_map(&mw, r.w, r.E * (r.gated ? 2 : 1) * N, K, K, 128, "moe_gemm_fp8 w")) return e;
+  if (int e = fp8_make_map(&mx, r.x, r.max_tiles * r.tile_rows, K, K, (int)r.tile_rows, "moe_gemm_fp8 x")) return e;
 #define GO(KIND, TO)                                                                  \
-  switch (tile_rows) {                                                                \
+  switch (r.tile_rows) {                                                              \
     case 16: return few_choose<16, KIND, TO>(mw, mx, a, stream);                      \
     case 32: return few_choose<32, KIND, TO>(mw, mx, a, stream);                      \
     default: return few_choose<64, KIND, TO>(mw, mx, a, stream);                      \
   }
-  if (gated) GO(FEW_GATED, float)
-  if (out_f32) GO(FEW_EXPERTS, float)
+  if (r.gated) GO(FEW_GATED, float)
+  if (r.out_f32) GO(FEW_EXPERTS, float)
   GO(FEW_EXPERTS, __nv_bfloat16)
 #undef GO
 }

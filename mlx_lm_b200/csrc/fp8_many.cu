@@ -509,13 +509,6 @@ static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t str
   return mlxb_check_launch("linear (8 bits)");
 }
 
-static int many_check(const char* what, const void* x, const void* xs, const void* w, const void* ws, int N, int K, const void* out) {
-  if (!x || !xs || !w || !ws || !out || N <= 0 || K <= 0 || (K & 15) ||
-      (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws) & 15))
-    return mlxb_fail(MLXB_BAD_ARG, "%s: codes of %d x %d (rows of whole 16 bytes, 16-byte aligned)", what, N, K);
-  return 0;
-}
-
 struct ManyForm { int bn, cg; };
 static ManyForm many_form(int M, int N, int K) {
   const char *want_pair = getenv("MLXB_FP8_PAIR"), *want_bn = getenv("MLXB_FP8_BN");     // experiments and tests
@@ -527,23 +520,25 @@ static ManyForm many_form(int M, int N, int K) {
 }
 
 // As mlxb_fp8_linear_few, for any number of rows.
-MLXB_EXPORT int mlxb_fp8_linear_many(int out_f32, const void* x, const void* xs, const void* w, const void* ws, const float* bias, const void* residual,
-                                     void* out, int M, int N, int K, long long ldo, int epi, int* status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0) return 0;
-  if (int e = many_check("linear (8 bits)", x, xs, w, ws, N, K, out)) return e;
-  if (ldo < N || !activation_known(epi)) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d outputs at stride %lld, epilogue %d", N, ldo, epi);
+MLXB_EXPORT int mlxb_fp8_linear_many(const Fp8LinearRecord* rec, long long bytes, cudaStream_t stream) {
+  if (!rec || bytes != sizeof(Fp8LinearRecord)) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): a record of %lld bytes", bytes);
+  const Fp8LinearRecord& r = *rec;
+  if (r.M <= 0 || r.N <= 0) return 0;
+  if (int e = fp8_check("linear (8 bits)", r.x, r.xs, r.w, r.ws, r.out, r.M, r.N, r.K, r.ldo)) return e;
+  if (!activation_known((int)r.epi) || !r.status) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): epilogue %lld", r.epi);
+  const int M = (int)r.M, N = (int)r.N, K = (int)r.K;
   const ManyForm f = many_form(M, N, K);
   ManyArgs a = {};
   a.M = M; a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = (M + 127) / 128; a.w_tiles = (N + 127) / 128;
   a.tiles_m = (M + 128 * f.cg - 1) / (128 * f.cg); a.tiles_n = (N + f.bn - 1) / f.bn;
-  a.bias = bias; a.residual = residual; a.out = out; a.ldo = ldo; a.status = status; a.act = epi;
+  a.bias = r.bias; a.residual = r.residual; a.out = r.out; a.ldo = r.ldo; a.status = r.status; a.act = (int)r.epi;
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d x %d outputs", M, N);
   ManyMaps maps;
-  if (int e = fp8_make_map(&maps.x, x, M, K, K, 128, "linear (8 bits) x")) return e;
-  if (int e = fp8_make_map(&maps.w, w, N, K, K, f.bn / f.cg, "linear (8 bits) w")) return e;
-  if (int e = scales_map(&maps.xs, xs, (long long)a.x_tiles * a.kgs, "linear (8 bits)")) return e;
-  if (int e = scales_map(&maps.ws, ws, (long long)a.w_tiles * a.kgs, "linear (8 bits)")) return e;
-#define GO(BN, CG) return out_f32 ? many_launch<BN, CG, MANY_LINEAR, float>(maps, a, stream) : many_launch<BN, CG, MANY_LINEAR, __nv_bfloat16>(maps, a, stream);
+  if (int e = fp8_make_map(&maps.x, r.x, M, K, K, 128, "linear (8 bits) x")) return e;
+  if (int e = fp8_make_map(&maps.w, r.w, N, K, K, f.bn / f.cg, "linear (8 bits) w")) return e;
+  if (int e = scales_map(&maps.xs, r.xs, (long long)a.x_tiles * a.kgs, "linear (8 bits)")) return e;
+  if (int e = scales_map(&maps.ws, r.ws, (long long)a.w_tiles * a.kgs, "linear (8 bits)")) return e;
+#define GO(BN, CG) return r.out_f32 ? many_launch<BN, CG, MANY_LINEAR, float>(maps, a, stream) : many_launch<BN, CG, MANY_LINEAR, __nv_bfloat16>(maps, a, stream);
   if (f.cg == 2) {
     if (f.bn == 256) GO(256, 2)
     GO(128, 2)
@@ -554,26 +549,27 @@ MLXB_EXPORT int mlxb_fp8_linear_many(int out_f32, const void* x, const void* xs,
 }
 
 // As mlxb_fp8_experts_few, for plans with tiles of 128 slots.
-MLXB_EXPORT int mlxb_fp8_experts_many(int gated, int out_f32, const void* x, const void* xs, const void* w, const void* ws, int E, int N, int K,
-                                      const int* sorted, const int* tile_info, const int* n_tiles, int max_tiles, int at_most, const float* sel_weight,
-                                      void* out, long long ldo, void* out_scales, int* status, int act, float limit, cudaStream_t stream) {
-  if (max_tiles <= 0 || at_most <= 0) return 0;
-  if (int e = many_check("moe_gemm_fp8", x, xs, w, ws, N, K, out)) return e;
-  if (E <= 0 || ldo < N || (gated && (!out_scales || ldo != ((N + 15) & ~15) || ((uintptr_t)out & 15))) || (long long)E * N * 2 > 0x7fffffffLL ||
-      (long long)max_tiles * 128 > 0x7fffffffLL)
-    return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d experts of %d x %d, results at stride %lld", E, N, K, ldo);
+MLXB_EXPORT int mlxb_fp8_experts_many(const Fp8ExpertsRecord* rec, long long bytes, cudaStream_t stream) {
+  if (!rec || bytes != sizeof(Fp8ExpertsRecord)) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: a record of %lld bytes", bytes);
+  const Fp8ExpertsRecord& r = *rec;
+  if (r.max_tiles <= 0 || r.at_most <= 0) return 0;
+  if (int e = fp8_check_experts(r)) return e;
+  if (r.tile_rows != 128) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: tiles of %lld rows", r.tile_rows);
+  const int N = (int)r.N, K = (int)r.K;
   ManyArgs a = {};
-  a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = max_tiles; a.w_tiles = (N + 127) / 128;
+  a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = (int)r.max_tiles; a.w_tiles = (N + 127) / 128;
   const int bn = 256;
-  a.tiles_m = min(max_tiles, at_most); a.tiles_n = gated ? a.w_tiles : (N + bn - 1) / bn;
-  a.sorted = sorted; a.tile_info = tile_info; a.n_tiles = n_tiles; a.sel_weight = sel_weight;
-  a.out = out; a.ldo = ldo; a.out_scales = (uint8_t*)out_scales; a.out_kgs = (N + 511) / 512; a.status = status; a.act = act; a.limit = limit;
-  if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %d tiles of %d outputs", max_tiles, N);
+  a.tiles_m = (int)min(r.max_tiles, r.at_most); a.tiles_n = r.gated ? a.w_tiles : (N + bn - 1) / bn;
+  a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
+  a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
+  a.limit = (float)r.limit;
+  if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
+  const long long stack = r.E * (r.gated ? 2 : 1);
   ManyMaps maps;
-  if (int e = fp8_make_map(&maps.x, x, (long long)max_tiles * 128, K, K, 128, "moe_gemm_fp8 x")) return e;
-  if (int e = fp8_make_map(&maps.w, w, (long long)E * (gated ? 2 : 1) * N, K, K, gated ? 128 : bn, "moe_gemm_fp8 w")) return e;
-  if (int e = scales_map(&maps.xs, xs, (long long)max_tiles * a.kgs, "moe_gemm_fp8")) return e;
-  if (int e = scales_map(&maps.ws, ws, (long long)E * (gated ? 2 : 1) * a.w_tiles * a.kgs, "moe_gemm_fp8")) return e;
-  if (gated) return many_launch<256, 1, MANY_GATED, float>(maps, a, stream);
-  return out_f32 ? many_launch<256, 1, MANY_EXPERTS, float>(maps, a, stream) : many_launch<256, 1, MANY_EXPERTS, __nv_bfloat16>(maps, a, stream);
+  if (int e = fp8_make_map(&maps.x, r.x, r.max_tiles * 128, K, K, 128, "moe_gemm_fp8 x")) return e;
+  if (int e = fp8_make_map(&maps.w, r.w, stack * N, K, K, r.gated ? 128 : bn, "moe_gemm_fp8 w")) return e;
+  if (int e = scales_map(&maps.xs, r.xs, r.max_tiles * a.kgs, "moe_gemm_fp8")) return e;
+  if (int e = scales_map(&maps.ws, r.ws, stack * a.w_tiles * a.kgs, "moe_gemm_fp8")) return e;
+  if (r.gated) return many_launch<256, 1, MANY_GATED, float>(maps, a, stream);
+  return r.out_f32 ? many_launch<256, 1, MANY_EXPERTS, float>(maps, a, stream) : many_launch<256, 1, MANY_EXPERTS, __nv_bfloat16>(maps, a, stream);
 }

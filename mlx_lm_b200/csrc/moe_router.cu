@@ -375,29 +375,34 @@ __device__ __forceinline__ void plan_experts(const RouterArgs& a, const int* sTo
 
 // ONE: the whole step in this cluster, with its plan.  Shared memory: totals, places and tiles [E], by warp: doubles [E], picks [top]; the
 // plan's [RP_WARPS][E] lie over the latter.
+// A block has 16 warps; in two launches, where a lane has few experts, 32: the work is a chain of votes, and an SM wants more of them.
 template <int VPT, bool ONE>
-__global__ void __launch_bounds__(RP_THREADS) route_kernel(const __grid_constant__ RouterArgs a) {
+constexpr int route_threads() { return !ONE && VPT <= 8 ? 2 * RP_THREADS : RP_THREADS; }
+
+template <int VPT, bool ONE>
+__global__ void __launch_bounds__(route_threads<VPT, ONE>()) route_kernel(const __grid_constant__ RouterArgs a) {
+  constexpr int THREADS = route_threads<VPT, ONE>(), WARPS = THREADS / 32;
   extern __shared__ __align__(16) uint8_t rp_smem[];
   int* sCount = reinterpret_cast<int*>(rp_smem);
   int* sFirst = sCount + a.E;
   int* sTile = sFirst + a.E;
   double* sC = reinterpret_cast<double*>(rp_smem + ((size_t)12 * a.E + 15) / 16 * 16);
-  int* sPick = reinterpret_cast<int*>(sC + (size_t)RP_WARPS * a.E);
+  int* sPick = reinterpret_cast<int*>(sC + (size_t)WARPS * a.E);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < a.E; e += RP_THREADS) sCount[e] = 0;
+  for (int e = threadIdx.x; e < a.E; e += THREADS) sCount[e] = 0;
   pdl_wait();
   pdl_trigger();
   const float* logits = after_wait(a.logits);
   __syncthreads();
   const int t0 = blockIdx.x * a.tokens_a_block, t1 = min(a.T, t0 + a.tokens_a_block);
-  for (int t = t0 + warp; t < t1; t += RP_WARPS)
+  for (int t = t0 + warp; t < t1; t += WARPS)
     route_token<VPT>(a, logits, t, sC + (size_t)warp * a.E, sPick + warp * a.top, ONE ? nullptr : sCount, lane);
   if (ONE) {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // all choices are written
     if (blockIdx.x != 0) return;
     const int* sel = after_wait(a.sel);
-    for (int i = threadIdx.x; i < a.T * a.top; i += RP_THREADS) {
+    for (int i = threadIdx.x; i < a.T * a.top; i += THREADS) {
       const int e = __ldcg(sel + i);
       if (e >= 0 && e < a.n_real) atomicAdd(&sCount[e], 1);
     }
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(RP_THREADS) route_kernel(const __grid_constant
     place_slots(a, sel, 0, a.T * a.top, sFirst, reinterpret_cast<int*>(sC));
   } else {
     __syncthreads();
-    for (int e = threadIdx.x; e < a.n_real; e += RP_THREADS) a.counts[(size_t)blockIdx.x * a.n_real + e] = sCount[e];
+    for (int e = threadIdx.x; e < a.n_real; e += THREADS) a.counts[(size_t)blockIdx.x * a.n_real + e] = sCount[e];
   }
 }
 
@@ -459,12 +464,14 @@ MLXB_EXPORT int mlxb_moe_route_scratch(int T, int E) {
 }
 
 template <int VPT>
-static int route_launch(const RouterArgs& a, int blocks, size_t smem, cudaStream_t stream) {
+static int route_launch(const RouterArgs& a, int blocks, cudaStream_t stream) {
   static SharedLimit one, many;
+  const int warps = (a.T > RP_ONE_LAUNCH ? route_threads<VPT, false>() : RP_THREADS) / 32;
+  const size_t smem = ((size_t)12 * a.E + 15) / 16 * 16 + (size_t)warps * (8 * (size_t)a.E + 4 * (size_t)a.top);
   constexpr size_t most = 227 * 1024;
   if (a.T > RP_ONE_LAUNCH) {
     if (cudaError_t e = many.raise(route_kernel<VPT, false>, most)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
-    launch_pdl(route_kernel<VPT, false>, dim3(blocks), dim3(RP_THREADS), smem, stream, a);
+    launch_pdl(route_kernel<VPT, false>, dim3(blocks), dim3(route_threads<VPT, false>()), smem, stream, a);
     return mlxb_check_launch("moe_route_plan");
   }
   if (cudaError_t e = one.raise(route_kernel<VPT, true>, most)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));
@@ -485,18 +492,32 @@ static int route_launch(const RouterArgs& a, int blocks, size_t smem, cudaStream
   return mlxb_check_launch("moe_route_plan");
 }
 
+// Arguments as a record of 8-byte fields: a caller fills it in a tenth of the time of as many arguments.
+struct RouteRecord {
+  const float* logits;
+  const int* token_req;
+  const float* correction;
+  int* sel;
+  float* weight;
+  int *counts, *sorted, *tile_info, *n_tiles;
+  long long ldl, T, E, top, softmax, two, groups, keep, n_real, renorm, tile_rows, max_tiles;
+  double eps, factor;
+};
+
 // logits float32 [T, E] at row stride ldl.  n_real: experts n_real .. E - 1 have no tensors (identity): chosen, they are marked -2 and the plan passes over them.
 // sel, weight [T * top]; sorted [T * top]; tile_info [max_tiles][3]; n_tiles [1]; counts: mlxb_moe_route_scratch(T, E) whole numbers.
-MLXB_EXPORT int mlxb_moe_route_plan(const float* logits, long long ldl, const int* token_req, const float* correction, int T, int E, int top, int softmax,
-                                    int two, int groups, int keep, int n_real, int renorm, float eps, float factor, int* sel, float* weight, int* counts,
-                                    int tile_rows, int max_tiles, int* sorted, int* tile_info, int* n_tiles, cudaStream_t stream) {
-  if (T < 0 || E <= 0 || E > 1024 || top <= 0 || top > E || top > 64 || ldl < E || groups < 1 || groups > 128 || E % groups || keep < 1 || keep > groups ||
+MLXB_EXPORT int mlxb_moe_route_plan(const RouteRecord* rec, long long bytes, cudaStream_t stream) {
+  if (!rec || bytes != sizeof(RouteRecord)) return mlxb_fail(MLXB_BAD_ARG, "moe_route_plan: a record of %lld bytes", bytes);
+  const RouteRecord& r = *rec;
+  const long long T = r.T, E = r.E, top = r.top, groups = r.groups, keep = r.keep, n_real = r.n_real, tile_rows = r.tile_rows, max_tiles = r.max_tiles;
+  const long long ldl = r.ldl;
+  if (!r.logits || !r.sel || !r.weight || !r.counts || !r.sorted || !r.tile_info || !r.n_tiles || max_tiles > 0x7fffffffLL || tile_rows > 0x7fffffffLL || T < 0 || E <= 0 || E > 1024 || top <= 0 || top > E || top > 64 || ldl < E || groups < 1 || groups > 128 || E % groups || keep < 1 || keep > groups ||
       n_real < 1 || n_real > E || top > keep * (E / groups) || tile_rows < 1 || (long long)T * top > 0x7ffffff0LL ||
       max_tiles < ((long long)T * top + tile_rows - 1) / tile_rows + n_real)
-    return mlxb_fail(MLXB_BAD_ARG, "moe_route_plan: %d tokens, %d of %d experts (%d with tensors; up to 64 of 1024), %d of %d groups (up to 128), tiles of %d rows, room for %d",
+    return mlxb_fail(MLXB_BAD_ARG, "moe_route_plan: %lld tokens, %lld of %lld experts (%lld with tensors; up to 64 of 1024), %lld of %lld groups (up to 128), tiles of %lld rows, room for %lld",
                      T, top, E, n_real, keep, groups, tile_rows, max_tiles);
   if (T == 0) {
-    const cudaError_t e = cudaMemsetAsync(n_tiles, 0, sizeof(int), stream);
+    const cudaError_t e = cudaMemsetAsync(r.n_tiles, 0, sizeof(int), stream);
     return e == cudaSuccess ? 0 : mlxb_fail((int)e, "moe_route_plan: %s", cudaGetErrorString(e));
   }
   int part = 0, shift = -1;
@@ -504,17 +525,17 @@ MLXB_EXPORT int mlxb_moe_route_plan(const float* logits, long long ldl, const in
     if (tile_rows == 1 << i) shift = i;
   if (groups <= 32)
     for (part = 1; 2 * part * groups <= 32; part *= 2) {}
-  RouterArgs a = {logits, ldl, token_req, correction, T, E, top, softmax, two, groups, keep, n_real, renorm, part, eps, factor, sel, weight, counts,
-                  tokens_a_block(T), tile_rows, shift, max_tiles, sorted, tile_info, n_tiles};
-  const int blocks = (T + a.tokens_a_block - 1) / a.tokens_a_block;
-  const size_t smem = ((size_t)12 * E + 15) / 16 * 16 + (size_t)RP_WARPS * (8 * (size_t)E + 4 * (size_t)top);
+  RouterArgs a = {r.logits, ldl, r.token_req, r.correction, (int)T, (int)E, (int)top, (int)r.softmax, (int)r.two, (int)groups, (int)keep, (int)n_real,
+                  (int)r.renorm, part, (float)r.eps, (float)r.factor, r.sel, r.weight, r.counts, tokens_a_block((int)T), (int)tile_rows, shift,
+                  (int)max_tiles, r.sorted, r.tile_info, r.n_tiles};
+  const int blocks = ((int)T + a.tokens_a_block - 1) / a.tokens_a_block;
   int rc;
-  if (E <= 32) rc = route_launch<1>(a, blocks, smem, stream);
-  else if (E <= 64) rc = route_launch<2>(a, blocks, smem, stream);
-  else if (E <= 128) rc = route_launch<4>(a, blocks, smem, stream);
-  else if (E <= 256) rc = route_launch<8>(a, blocks, smem, stream);
-  else if (E <= 512) rc = route_launch<16>(a, blocks, smem, stream);
-  else rc = route_launch<32>(a, blocks, smem, stream);
+  if (E <= 32) rc = route_launch<1>(a, blocks, stream);
+  else if (E <= 64) rc = route_launch<2>(a, blocks, stream);
+  else if (E <= 128) rc = route_launch<4>(a, blocks, stream);
+  else if (E <= 256) rc = route_launch<8>(a, blocks, stream);
+  else if (E <= 512) rc = route_launch<16>(a, blocks, stream);
+  else rc = route_launch<32>(a, blocks, stream);
   if (rc || T <= RP_ONE_LAUNCH) return rc;
   static SharedLimit limit;
   if (cudaError_t e = limit.raise(plan_kernel, 160 * 1024)) return mlxb_fail((int)e, "moe_route_plan: shared memory: %s", cudaGetErrorString(e));

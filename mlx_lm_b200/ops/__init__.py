@@ -2500,30 +2500,46 @@ def fp8_empty(rows: int, columns: int, device, groups: int = 1):
     return codes, scales
 
 
-def _fp8_pair(codes, scales, group_rows: int, what: str):
-    """Checks a matrix (or stack) of codes and its scales; ``(rows, columns of codes, groups)``."""
-    _need(codes, torch.float8_e4m3fn, what + " codes")
-    _need(scales, torch.uint8, what + " scales")
-    if codes.dim() != 2 or not codes.is_contiguous() or codes.shape[1] % 16 or not codes.shape[1]:
-        raise KernelError(f"{what}: codes {tuple(codes.shape)} strides {codes.stride()}: contiguous rows of whole 16 bytes")
-    rows, width = codes.shape
-    if group_rows <= 0 or rows % group_rows:
-        raise KernelError(f"{what}: {rows} rows of codes in matrices of {group_rows}")
-    groups = rows // group_rows
-    if scales.shape != (groups, (group_rows + 127) // 128, (width + 511) // 512, 512) or not scales.is_contiguous():
-        raise KernelError(f"{what}: scales {tuple(scales.shape)} for {groups} matrices of {group_rows} x {width}")
-    if scales.device != codes.device:
-        raise KernelError(f"{what}: codes on {codes.device}, scales on {scales.device}")
-    return rows, width, groups
+_U8T, _F8T = torch.uint8, torch.float8_e4m3fn
+_FP8_ARGS = [c_char_p, ctypes.c_longlong, c_void_p]
 
 
-def _fp8_here(t, what: str) -> None:
-    """The launch goes to the current device."""
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _fp8_codes(codes, scales, group_rows: int, what: str):
+    """``(rows, columns of codes, groups)`` of a stack of matrices of ``group_rows`` rows in 8-bit floating point."""
+    shape = codes.shape
+    if len(shape) == 2 and codes.dtype is _F8T and scales.dtype is _U8T and group_rows > 0 and codes.is_contiguous() and scales.is_contiguous():
+        rows, width = shape
+        groups = rows // group_rows
+        if (groups * group_rows == rows and width and not width & 15
+                and scales.shape == (groups, (group_rows + 127) >> 7, (width + 511) >> 9, 512)):
+            return rows, width, groups
+    raise KernelError(f"{what}: codes {codes.dtype} {tuple(shape)} strides {codes.stride()} and scales {scales.dtype} {tuple(scales.shape)} strides "
+                      f"{scales.stride()} are no matrices of {group_rows} rows as fp8_empty makes them")
 
 
-_FP8Q_ARGS = [c_int, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p]
+def _fp8_rows(t, what: str):
+    """``(rows, columns, row stride)`` of a float32 or bfloat16 matrix whose rows are contiguous."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] != 1) or (t.dtype is not _BF16T and t.dtype is not _F32T):
+        raise KernelError(f"{what}: {t.dtype} {tuple(shape)} strides {strides}: float32 or bfloat16 rows, each contiguous")
+    return shape[0], shape[1], max(strides[0], shape[1])
+
+
+def _fp8_vector(t, dtype, n: int, what: str) -> None:
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous():
+        raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)} strides {t.stride()}: {n} elements of {dtype} in one piece")
+
+
+def _fp8_device(what: str, *tensors) -> None:
+    """All on the current device, which the launch goes to."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: tensors on {sorted({str(x.device) for x in tensors if x is not None})}, "
+                              + (f"the current device is cuda:{here}" if here >= 0 else "not on a CUDA device"))
+
+
+_fp8_quantize_record = _kv8_record("3Q6q")
 
 
 def fp8_quantize(x, codes, scales, stream, group_rows: Optional[int] = None) -> None:
@@ -2531,20 +2547,19 @@ def fp8_quantize(x, codes, scales, stream, group_rows: Optional[int] = None) -> 
     scale ``2**e`` for each run of 128 columns with ``e`` the least whole number for which the run's largest finite magnitude is at most
     ``448 * 2**e`` (within -127 .. 127).  Codes are rounded to nearest, ties to even; what is not finite becomes NaN.  ``group_rows``:
     ``x`` is a stack of matrices of so many rows (default: one matrix)."""
-    _need(x, None, "fp8_quantize x")
-    ldx = _rows(x, "fp8_quantize x")
-    M, K = x.shape
-    group_rows = M if group_rows is None else int(group_rows)
+    M, K, ldx = _fp8_rows(x, "fp8_quantize x")
     if M == 0:
         return
-    rows, width, _ = _fp8_pair(codes, scales, group_rows, "fp8_quantize")
-    if rows != M or width != (K + 15) // 16 * 16 or codes.device != x.device:
-        raise KernelError(f"fp8_quantize: x {tuple(x.shape)} on {x.device} into codes {tuple(codes.shape)} on {codes.device}")
-    _fp8_here(x, "fp8_quantize")
-    _call("fp8_rows", "mlxb_fp8_quantize", _FP8Q_ARGS, dtype_code(x.dtype), _p(x), ldx, M, K, group_rows, _p(codes), width, _p(scales), stream)
+    group_rows = M if group_rows is None else int(group_rows)
+    rows, width, _ = _fp8_codes(codes, scales, group_rows, "fp8_quantize")
+    if rows != M or width != (K + 15) & ~15:
+        raise KernelError(f"fp8_quantize: x {tuple(x.shape)} into codes {tuple(codes.shape)}")
+    _fp8_device("fp8_quantize", x, codes, scales)
+    _call("fp8_rows", "mlxb_fp8_quantize", _FP8_ARGS, *_fp8_quantize_record(
+        x.data_ptr(), codes.data_ptr(), scales.data_ptr(), _DT[x.dtype], ldx, M, K, group_rows, width), stream)
 
 
-_FP8L_ARGS = [c_int] + [c_void_p] * 7 + [c_int] * 3 + [ctypes.c_longlong, c_int, c_void_p, c_void_p]
+_fp8_linear_record = _kv8_record("8Q6q")
 
 
 def linear_fp8(codes, scales, w_codes, w_scales, bias, out, status, stream, epilogue: int = EPI_NONE, residual=None) -> None:
@@ -2552,33 +2567,28 @@ def linear_fp8(codes, scales, w_codes, w_scales, bias, out, status, stream, epil
     with ``x`` and ``w`` the numbers that codes and scales stand for, float32 sums and epilogue; ``out`` (and ``residual``, which may be ``out``)
     bfloat16 or float32.  Up to ``FP8_FEW_ROWS`` rows run in the kernel that streams the weights, more on tiles of rows.  ``status`` receives
     ``ST_WAIT_TIMEOUT`` if a bounded wait gives up."""
-    M, N = out.shape
-    if M == 0:
+    M, N, ldo = _fp8_rows(out, "linear (8 bits) out")
+    if M == 0 or N == 0:
         return
-    rows, K, groups = _fp8_pair(codes, scales, M, "linear (8 bits) x")
-    n, k, w_groups = _fp8_pair(w_codes, w_scales, N, "linear (8 bits) w")
-    if (rows, groups) != (M, 1) or (n, k, w_groups) != (N, K, 1):
+    _, K, groups = _fp8_codes(codes, scales, M, "linear (8 bits) x")
+    _, k, w_groups = _fp8_codes(w_codes, w_scales, N, "linear (8 bits) w")
+    if groups != 1 or w_groups != 1 or k != K:
         raise KernelError(f"linear (8 bits): x {tuple(codes.shape)}, w {tuple(w_codes.shape)}, out {tuple(out.shape)}")
-    _need(out, None, "linear (8 bits) out")
-    _need(status, torch.int32, "linear (8 bits) status")
-    ldo = _rows(out, "linear (8 bits) out")
-    if out.dtype not in (torch.bfloat16, torch.float32):
-        raise KernelError(f"linear (8 bits): output dtype {out.dtype}")
+    _fp8_vector(status, _I32, 1, "linear (8 bits) status")
+    bp = rp = 0
     if bias is not None:
-        _need(bias, torch.float32, "linear (8 bits) bias")
-        if bias.numel() != N or not bias.is_contiguous():
-            raise KernelError(f"linear (8 bits): bias of {bias.numel()} for {N} outputs")
+        _fp8_vector(bias, _F32T, N, "linear (8 bits) bias")
+        bp = bias.data_ptr()
     if residual is not None:
-        _need(residual, out.dtype, "linear (8 bits) residual")
-        if residual.shape != out.shape or _rows(residual, "linear (8 bits) residual") != ldo:
-            raise KernelError("linear (8 bits): residual must have the output's shape and row stride")
-    if len({t.device for t in (codes, w_codes, bias, out, status, residual) if t is not None}) > 1:
-        raise KernelError("linear (8 bits): tensors on different devices")
-    _fp8_here(codes, "linear (8 bits)")
-    few = M <= FP8_FEW_ROWS
-    _call("fp8_few" if few else "fp8_many", "mlxb_fp8_linear_few" if few else "mlxb_fp8_linear_many", _FP8L_ARGS,
-          int(out.dtype == torch.float32), _p(codes), _p(scales), _p(w_codes), _p(w_scales), _p(bias), _p(residual), _p(out), M, N, K, ldo,
-          int(epilogue), _p(status), stream)
+        if residual.dtype is not out.dtype or residual.shape != out.shape or _fp8_rows(residual, "linear (8 bits) residual")[2] != ldo:
+            raise KernelError(f"linear (8 bits): a residual {residual.dtype} {tuple(residual.shape)} strides {residual.stride()} for an output "
+                              f"{out.dtype} {tuple(out.shape)} strides {out.stride()}")
+        rp = residual.data_ptr()
+    _fp8_device("linear (8 bits)", codes, scales, w_codes, w_scales, out, status, bias, residual)
+    lib, fn = ("fp8_few", "mlxb_fp8_linear_few") if M <= FP8_FEW_ROWS else ("fp8_many", "mlxb_fp8_linear_many")
+    _call(lib, fn, _FP8_ARGS, *_fp8_linear_record(
+        codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), bp, rp, out.data_ptr(), status.data_ptr(),
+        out.dtype is _F32T, M, N, K, ldo, epilogue), stream)
 
 
 def moe_fp8_tile_rows(n_slots: int, n_experts: int) -> int:
@@ -2587,37 +2597,35 @@ def moe_fp8_tile_rows(n_slots: int, n_experts: int) -> int:
     return 16 if each <= 8 else 32 if each <= 16 else 64 if each <= 32 else 128
 
 
-def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, what: str) -> None:
-    for t, name in ((sorted_slots, "sorted"), (tile_info, "tile_info"), (n_tiles, "n_tiles")):
-        _need(t, torch.int32, f"{what} {name}")
-        if not t.is_contiguous():
-            raise KernelError(f"{what}: {name} is not contiguous")
-    if tile_rows not in (16, 32, 64, 128) or tile_info.numel() < 3 * max_tiles or n_tiles.numel() < 1:
-        raise KernelError(f"{what}: tiles of {tile_rows} rows (16, 32, 64 or 128), room for {tile_info.numel() // 3} of {max_tiles}")
+def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, what: str) -> int:
+    """Checks a plan; how many slots it is for."""
+    if tile_rows not in (16, 32, 64, 128) or max_tiles < 0:
+        raise KernelError(f"{what}: {max_tiles} tiles of {tile_rows} rows (16, 32, 64 or 128)")
+    _fp8_vector(sorted_slots, _I32, 0, what + " sorted_slots")
+    _fp8_vector(tile_info, _I32, 3 * max_tiles, what + " tile_info")
+    _fp8_vector(n_tiles, _I32, 1, what + " n_tiles")
+    return sorted_slots.numel()
 
 
-_FP8G_ARGS = [c_int, c_void_p, ctypes.c_longlong, c_int, c_int] + [c_void_p] * 3 + [c_int, c_int, c_void_p, c_int, c_void_p, c_void_p]
+_fp8_gather_record = _kv8_record("6Q7q")
 
 
 def moe_gather_fp8(x, a_div: int, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, codes, scales, stream) -> None:
     """The rows ``x[slot // a_div]`` of a plan's slots in 8-bit floating point (``fp8_quantize``): place ``i`` of tile ``t`` is row ``t * tile_rows + i`` of
     ``codes``, and every tile is a matrix of its own in ``scales`` (``fp8_empty(tile_rows, columns, device, groups=max_tiles)``).  Rows of a tile
     behind its last slot, and tiles behind the last, are left as they were."""
-    _need(x, None, "moe_gather_fp8 x")
-    ldx = _rows(x, "moe_gather_fp8 x")
-    _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gather_fp8")
-    rows, width, groups = _fp8_pair(codes, scales, tile_rows, "moe_gather_fp8")
-    if groups < max_tiles or width != (x.shape[1] + 15) // 16 * 16 or codes.device != x.device or a_div <= 0 or sorted_slots.numel() > x.shape[0] * a_div:
-        raise KernelError(f"moe_gather_fp8: x {tuple(x.shape)}, {sorted_slots.numel()} slots, {a_div} a row, codes {tuple(codes.shape)} for {max_tiles} tiles")
-    _fp8_here(x, "moe_gather_fp8")
-    _call("fp8_rows", "mlxb_fp8_gather", _FP8G_ARGS, dtype_code(x.dtype), _p(x), ldx, x.shape[1], int(a_div), _p(sorted_slots), _p(tile_info),
-          _p(n_tiles), int(max_tiles), int(tile_rows), _p(codes), width, _p(scales), stream)
+    T, K, ldx = _fp8_rows(x, "moe_gather_fp8 x")
+    S = _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gather_fp8")
+    _, width, groups = _fp8_codes(codes, scales, tile_rows, "moe_gather_fp8")
+    if groups < max_tiles or width != (K + 15) & ~15 or a_div <= 0 or S > T * a_div:
+        raise KernelError(f"moe_gather_fp8: x {tuple(x.shape)}, {S} slots, {a_div} a row, codes {tuple(codes.shape)} for {max_tiles} tiles")
+    _fp8_device("moe_gather_fp8", x, sorted_slots, tile_info, n_tiles, codes, scales)
+    _call("fp8_rows", "mlxb_fp8_gather", _FP8_ARGS, *_fp8_gather_record(
+        x.data_ptr(), sorted_slots.data_ptr(), tile_info.data_ptr(), n_tiles.data_ptr(), codes.data_ptr(), scales.data_ptr(), _DT[x.dtype], ldx, K,
+        a_div, max_tiles, tile_rows, width), stream)
 
 
-_FP8E_FEW = ([c_int, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 3
-             + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_int, c_float, c_void_p])
-_FP8E_MANY = ([c_int, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 2
-              + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_int, c_float, c_void_p])
+_fp8_experts_record = _kv8_record("11Q10qd")
 
 
 def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, out, status, stream,
@@ -2628,56 +2636,53 @@ def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_ti
     and ``out_scales`` by tiles, as the second product reads them.  Else ``w_codes`` is one matrix an expert and the product of place ``i`` of the plan goes to row
     ``sorted_slots[i]`` of ``out`` (bfloat16 or float32).  Rows of no slot are left as they were.  ``status`` receives ``ST_WAIT_TIMEOUT`` if
     a bounded wait gives up."""
-    _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gemm_fp8")
-    rows, K, groups = _fp8_pair(codes, scales, tile_rows, "moe_gemm_fp8 a")
-    if w_scales.dim() != 4 or w_codes.dim() != 2 or not w_scales.shape[0] or w_scales.shape[0] % (2 if gated else 1):
-        raise KernelError(f"moe_gemm_fp8: weights {tuple(w_codes.shape)} with scales {tuple(w_scales.shape)}")
-    n_out = w_codes.shape[0] // w_scales.shape[0]
-    _, k, w_groups = _fp8_pair(w_codes, w_scales, n_out, "moe_gemm_fp8 w")
-    E = w_groups // (2 if gated else 1)
-    S = sorted_slots.numel()
-    if groups < max_tiles or k != K:
-        raise KernelError(f"moe_gemm_fp8: rows {tuple(codes.shape)} for {max_tiles} tiles of {tile_rows}, weights {tuple(w_codes.shape)}")
-    _need(status, torch.int32, "moe_gemm_fp8 status")
+    S = _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gemm_fp8")
+    _, K, groups = _fp8_codes(codes, scales, tile_rows, "moe_gemm_fp8 rows")
+    w_groups = w_scales.shape[0] if w_scales.dim() == 4 else 0
+    n_out = w_codes.shape[0] // w_groups if w_groups else 0
+    _, k, _ = _fp8_codes(w_codes, w_scales, n_out, "moe_gemm_fp8 weights")
+    if groups < max_tiles or k != K or (gated and w_groups & 1):
+        raise KernelError(f"moe_gemm_fp8: rows {tuple(codes.shape)} for {max_tiles} tiles of {tile_rows}, {w_groups} matrices of {n_out} x {k}")
+    _fp8_vector(status, _I32, 1, "moe_gemm_fp8 status")
+    wp = op = 0
     if gated:
-        o_rows, ldo, o_groups = _fp8_pair(out, out_scales, tile_rows, "moe_gemm_fp8 out")
-        if o_groups < max_tiles or ldo != (n_out + 15) // 16 * 16:
+        if out_scales is None or unit not in GATED_UNITS:
+            raise KernelError(f"moe_gemm_fp8: a gated product needs memory for its scales and a unit out of {sorted(GATED_UNITS)}, not {unit!r}")
+        _, ldo, o_groups = _fp8_codes(out, out_scales, tile_rows, "moe_gemm_fp8 out")
+        if o_groups < max_tiles or ldo != (n_out + 15) & ~15:
             raise KernelError(f"moe_gemm_fp8: {n_out} columns of {max_tiles} tiles into {tuple(out.shape)}")
+        op = out_scales.data_ptr()
         if sel_weight is not None:
-            _need(sel_weight, torch.float32, "moe_gemm_fp8 sel_weight")
-            if sel_weight.numel() < S or not sel_weight.is_contiguous():
-                raise KernelError(f"moe_gemm_fp8: {sel_weight.numel()} weights for {S} slots")
+            _fp8_vector(sel_weight, _F32T, S, "moe_gemm_fp8 sel_weight")
+            wp = sel_weight.data_ptr()
     else:
-        _need(out, None, "moe_gemm_fp8 out")
-        ldo = _rows(out, "moe_gemm_fp8 out")
-        if out.dtype not in (torch.bfloat16, torch.float32) or out.shape[0] < S or out.shape[1] != n_out:
-            raise KernelError(f"moe_gemm_fp8: {S} rows of {n_out} into {out.dtype} {tuple(out.shape)}")
-    if len({t.device for t in (codes, w_codes, sorted_slots, tile_info, n_tiles, out, status)}) > 1:
-        raise KernelError("moe_gemm_fp8: tensors on different devices")
-    _fp8_here(codes, "moe_gemm_fp8")
-    args = [int(bool(gated)), int(out.dtype == torch.float32), _p(codes), _p(scales), _p(w_codes), _p(w_scales), E, n_out, K, _p(sorted_slots),
-            _p(tile_info), _p(n_tiles), groups, min(int(max_tiles), S)]
-    tail = [_p(sel_weight) if gated else None, _p(out), ldo, _p(out_scales) if gated else None, _p(status), GATED_UNITS[unit], float(limit), stream]
-    if tile_rows == 128:
-        _call("fp8_many", "mlxb_fp8_experts_many", _FP8E_MANY, *args, *tail)
-    else:
-        _call("fp8_few", "mlxb_fp8_experts_few", _FP8E_FEW, *args, int(tile_rows), *tail)
+        rows, columns, ldo = _fp8_rows(out, "moe_gemm_fp8 out")
+        if rows < S or columns != n_out:
+            raise KernelError(f"moe_gemm_fp8: {S} rows of {n_out} into {tuple(out.shape)}")
+    _fp8_device("moe_gemm_fp8", codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_tiles, out, status, out_scales if gated else None,
+                sel_weight if gated else None)
+    lib, fn = ("fp8_many", "mlxb_fp8_experts_many") if tile_rows == 128 else ("fp8_few", "mlxb_fp8_experts_few")
+    _call(lib, fn, _FP8_ARGS, *_fp8_experts_record(
+        codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), sorted_slots.data_ptr(), tile_info.data_ptr(),
+        n_tiles.data_ptr(), wp, out.data_ptr(), op, status.data_ptr(), gated, not gated and out.dtype is _F32T, w_groups // 2 if gated else w_groups,
+        n_out, K, groups, min(max_tiles, S), tile_rows, ldo, GATED_UNITS[unit] if gated else 0, limit), stream)
 
 
 # --------------------------------------------------------------------------
 # the router with the plan of the experts' products (csrc/moe_router.cu)
 
 MOE_GROUP_SCORES = {"best": 0, "two": 1}
+MOE_ROUTE_PLAN_EXPERTS, MOE_ROUTE_PLAN_GROUPS, MOE_ROUTE_PLAN_TOP = 1024, 128, 64      # the most of each
 
 
+@functools.lru_cache(maxsize=256)
 def moe_route_scratch(n_tokens: int, n_experts: int) -> int:
     """Elements of int32 scratch memory that ``moe_route_plan`` wants for a step of ``n_tokens``."""
     f, _ = _fn("moe_router", "mlxb_moe_route_scratch", [c_int, c_int])
     return int(f(int(n_tokens), int(n_experts)))
 
 
-_ROUTE_PLAN_ARGS = ([c_void_p, ctypes.c_longlong, c_void_p, c_void_p] + [c_int] * 9 + [c_float, c_float] + [c_void_p] * 3 + [c_int, c_int]
-                    + [c_void_p] * 4)
+_moe_route_plan_record = _kv8_record("9Q12q2d")
 
 
 def moe_route_plan(logits, token_req, top: int, sel_expert, sel_weight, tile_rows: int, sorted_slots, tile_info, n_tiles, scratch, stream,
@@ -2685,34 +2690,37 @@ def moe_route_plan(logits, token_req, top: int, sel_expert, sel_weight, tile_row
                    identity: int = 0, renormalize_eps: float = 0.0, weight_scale: float = 1.0) -> None:
     """``moe_route`` and ``moe_plan`` in one call, with a choice that is exact and a plan in a fixed order.  ``group_score``: a group is judged by its
     ``best`` choice score or by the sum of its ``two`` best.  Of equal scores the lower index is chosen; scores that float32 cannot tell apart
-    are formed again in 64 bits.  A score that is NaN is never chosen, a place nobody can take gets expert -1 and weight 0.  The plan: slots sorted by
+    are formed again in 64 bits; without a correction the order of the logits is the order of the scores.  A score that is NaN, or that a correction makes
+    minus infinity, is never chosen; a place nobody can take gets expert -1 and weight 0.  The plan: slots sorted by
     expert and, within one, by number (``sorted_slots``), tiles of at most ``tile_rows`` of them (``tile_info``, ``n_tiles``); what lies behind the last slot
     and tile is left as it was.  ``scratch``: int32, ``moe_route_scratch`` elements.  Up to 1024 experts, 128 groups, 64 choices."""
-    _need(logits, torch.float32, "moe_route_plan logits")
-    ldl = _rows(logits, "moe_route_plan logits")
-    T, E = logits.shape
-    S, n_real = T * int(top), E - int(identity)
-    if score not in MOE_SCORES or group_score not in MOE_GROUP_SCORES:
-        raise KernelError(f"moe_route_plan: score {score!r}, groups judged by {group_score!r}")
-    max_tiles = moe_max_tiles(S, max(0, n_real), max(1, int(tile_rows)))
-    _need(sel_weight, torch.float32, "moe_route_plan sel_weight")
-    for t, n, what in ((sel_expert, S, "sel_expert"), (sel_weight, S, "sel_weight"), (sorted_slots, S, "sorted"), (tile_info, 3 * max_tiles, "tile_info"),
-                       (n_tiles, 1, "n_tiles"), (scratch, moe_route_scratch(T, E), "scratch")):
-        _need(t, None if t is sel_weight else torch.int32, "moe_route_plan " + what)
-        if t.numel() < n or not t.is_contiguous():
-            raise KernelError(f"moe_route_plan: {what} of {t.numel()} elements for {T} tokens and {top} of {E} experts: {n} in one piece")
+    T, E, ldl = _fp8_rows(logits, "moe_route_plan logits")
+    S, n_real = T * top, E - identity
+    if (logits.dtype is not _F32T or score not in MOE_SCORES or group_score not in MOE_GROUP_SCORES or not 0 < E <= MOE_ROUTE_PLAN_EXPERTS
+            or not 1 <= n_real <= E or not 1 <= groups <= MOE_ROUTE_PLAN_GROUPS or E % groups or not 1 <= keep_groups <= groups
+            or not 1 <= top <= min(MOE_ROUTE_PLAN_TOP, keep_groups * (E // groups)) or not 1 <= tile_rows):
+        raise KernelError(f"moe_route_plan: {logits.dtype} logits {tuple(logits.shape)}, {top} chosen (up to {MOE_ROUTE_PLAN_TOP} of "
+                          f"{MOE_ROUTE_PLAN_EXPERTS}), {keep_groups} of {groups} groups (up to {MOE_ROUTE_PLAN_GROUPS}), {identity} identity experts, tiles of "
+                          f"{tile_rows}, score {score!r}, groups judged by {group_score!r}")
+    max_tiles = (S + tile_rows - 1) // tile_rows + n_real
+    _fp8_vector(sel_expert, _I32, S, "moe_route_plan sel_expert")
+    _fp8_vector(sel_weight, _F32T, S, "moe_route_plan sel_weight")
+    _fp8_vector(sorted_slots, _I32, S, "moe_route_plan sorted_slots")
+    _fp8_vector(tile_info, _I32, 3 * max_tiles, "moe_route_plan tile_info")
+    _fp8_vector(n_tiles, _I32, 1, "moe_route_plan n_tiles")
+    rp = cp = 0
     if token_req is not None:
-        _need(token_req, torch.int32, "moe_route_plan token_req")
-        if token_req.numel() < T or not token_req.is_contiguous():
-            raise KernelError(f"moe_route_plan: requests of {token_req.numel()} tokens for {T}")
+        _fp8_vector(token_req, _I32, T, "moe_route_plan token_req")
+        rp = token_req.data_ptr()
     if correction is not None:
-        _need(correction, torch.float32, "moe_route_plan correction")
-        if correction.numel() != E or not correction.is_contiguous():
-            raise KernelError(f"moe_route_plan: a correction of {correction.numel()} for {E} experts")
-    _fp8_here(logits, "moe_route_plan")
-    _call("moe_router", "mlxb_moe_route_plan", _ROUTE_PLAN_ARGS, _p(logits), ldl, _p(token_req), _p(correction), T, E, int(top), MOE_SCORES[score],
-          MOE_GROUP_SCORES[group_score], int(groups), int(keep_groups), n_real, int(bool(renormalize)), float(renormalize_eps), float(weight_scale),
-          _p(sel_expert), _p(sel_weight), _p(scratch), int(tile_rows), max_tiles, _p(sorted_slots), _p(tile_info), _p(n_tiles), stream)
+        _fp8_vector(correction, _F32T, E, "moe_route_plan correction")
+        cp = correction.data_ptr()
+    _fp8_device("moe_route_plan", logits, token_req, sel_expert, sel_weight, sorted_slots, tile_info, n_tiles, scratch, correction)
+    _fp8_vector(scratch, _I32, moe_route_scratch(T, E), "moe_route_plan scratch")
+    _call("moe_router", "mlxb_moe_route_plan", _FP8_ARGS, *_moe_route_plan_record(
+        logits.data_ptr(), rp, cp, sel_expert.data_ptr(), sel_weight.data_ptr(), scratch.data_ptr(), sorted_slots.data_ptr(), tile_info.data_ptr(),
+        n_tiles.data_ptr(), ldl, T, E, top, MOE_SCORES[score], MOE_GROUP_SCORES[group_score], groups, keep_groups, n_real, renormalize, tile_rows,
+        max_tiles, renormalize_eps, weight_scale), stream)
 
 
 # --------------------------------------------------------------------------
