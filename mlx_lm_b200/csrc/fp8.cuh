@@ -88,6 +88,11 @@ __device__ __forceinline__ void fp8_bulk_load(void* dst, const void* src, uint32
 __device__ __forceinline__ void fp8_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fp8_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fp8_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Numbers that tcgen05.ld was to bring, as they are after the wait: what is formed of them cannot be moved before it.
+__device__ __forceinline__ void fp8_arrived(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 // A bounded wait that looks at no flag: for the way out, where copies and products already issued must come to their end.
 __device__ __forceinline__ void fp8_drain(uint64_t* bar, uint32_t parity) {

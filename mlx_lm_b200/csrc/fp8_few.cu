@@ -78,14 +78,10 @@ struct FewSmem {
   int abort_flag;
 };
 
-template <bool FAST>
-__device__ __forceinline__ float activate_by(int act, float v) {
-  switch (act) {
-    case EPI_GELU_NEW: return activate<EPI_GELU_NEW, FAST>(v);
-    case EPI_RELU: return activate<EPI_RELU, FAST>(v);
-    case EPI_TANH: return activate<EPI_TANH, FAST>(v);
-    default: return v;
-  }
+template <int ACT, bool FAST, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
 }
 
 // 1 if `ok` holds for every thread of the four epilogue warps
@@ -235,17 +231,40 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
   // ---- epilogue: a lane holds a row n of W; tokens are columns
   const int q = warp & 3, in_tile = q * 32 + lane;
-  // Numbers tok0 .. tok0 + count - 1 (below `live`) of item w: v (gated: gate v, up u) of column n.
+  // What the epilogue needs from memory for up to CH tokens from tok0 on, asked for while the products run: a plan's slots and their weights, one
+  // a lane; a linear layer's bias (of column n) and residuals.
+  struct Beside { int slot; float weight, bias, residual[CH]; };
+  auto fetch = [&](int w, int tok0, int live) {
+    Beside x;
+    x.slot = 0;
+    x.weight = 1.f;
+    x.bias = 0.f;
+    const int tile = w / a.w_tiles, n = (w - tile * a.w_tiles) * 128 + in_tile;
+    if (KIND != FEW_LINEAR) {
+      if (tok0 + lane < live) {
+        x.slot = sorted[tile_info[3 * tile + 1] + tok0 + lane];
+        if (KIND == FEW_GATED && sel_weight) x.weight = sel_weight[x.slot];
+      }
+    } else if (n < a.N) {
+      if (a.bias) x.bias = a.bias[n];
+      if (a.residual) {
+        const TO* res = reinterpret_cast<const TO*>(after_wait(a.residual)) + (long long)(tile * NT + tok0) * a.ldo + n;
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+          if (tok0 + j < live) x.residual[j] = to_f(res[j * a.ldo]);
+      }
+    }
+    return x;
+  };
+  // Numbers of tokens tok0 .. (below `live`) of item w: v (gated: gate v, up u) of column n.
   int flip = 0;
-  auto finish = [&](int w, int tok0, int live, float (&v)[CH], float (&u)[CH]) {
+  auto finish = [&](int w, int tok0, int live, float (&v)[CH], float (&u)[CH], const Beside& x) {
     const int tile = w / a.w_tiles, n0 = (w - tile * a.w_tiles) * 128, n = n0 + in_tile;
     if (KIND == FEW_GATED) {
-      const int first = tile_info[3 * tile + 1];
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
-        const bool on = tok0 + j < live;
-        const float wgt = on && sel_weight ? sel_weight[sorted[first + tok0 + j]] : 1.f;
-        v[j] = on && n < a.N ? fp8_gated_unit(a.act, v[j], u[j], wgt, a.limit) : 0.f;
+        const float wgt = __shfl_sync(0xffffffffu, x.weight, j);
+        v[j] = tok0 + j < live && n < a.N ? fp8_gated_unit(a.act, v[j], u[j], wgt, a.limit) : 0.f;
         const uint32_t top = __reduce_max_sync(0xffffffffu, fp8_magnitude(v[j]));
         if (lane == j) sm.top[flip][q][j] = top;
       }
@@ -263,26 +282,27 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
       }
       flip ^= 1;
-    } else if (n < a.N) {
-      TO* out = reinterpret_cast<TO*>(a.out);
+    } else {
+      TO* out = reinterpret_cast<TO*>(a.out) + n;
       if (KIND == FEW_LINEAR) {
-        const TO* res = reinterpret_cast<const TO*>(after_wait(a.residual));
-        const float bias = a.bias ? a.bias[n] : 0.f;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          if (tok0 + j >= live) break;
-          const long long at = (long long)(tile * NT + tok0 + j) * a.ldo + n;
-          float y = activate_by<sizeof(TO) == 2>(a.act, v[j] + bias);
-          if (res) y += to_f(res[at]);
-          out[at] = from_f<TO>(y);
+        for (int j = 0; j < CH; ++j) v[j] += x.bias;
+        switch (a.act) {
+          case EPI_GELU_NEW: activate_all<EPI_GELU_NEW, sizeof(TO) == 2>(v); break;
+          case EPI_RELU: activate_all<EPI_RELU, sizeof(TO) == 2>(v); break;
+          case EPI_TANH: activate_all<EPI_TANH, sizeof(TO) == 2>(v); break;
+          default: break;
         }
-      } else {
-        const int first = tile_info[3 * tile + 1];
+        if (a.residual) {
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          if (tok0 + j >= live) break;
-          out[(long long)sorted[first + tok0 + j] * a.ldo + n] = from_f<TO>(v[j]);
+          for (int j = 0; j < CH; ++j) v[j] += x.residual[j];
         }
+        out += (long long)(tile * NT + tok0) * a.ldo;
+      }
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const long long row = KIND == FEW_LINEAR ? j : __shfl_sync(0xffffffffu, x.slot, j);
+        if (tok0 + j < live && n < a.N) out[row * a.ldo] = from_f<TO>(v[j]);
       }
     }
   };
@@ -299,6 +319,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     for (int w = first_item; w < items; w += step, ++it) {
       const int b = S::ACC == 2 ? it & 1 : 0;
       const int live = live_of(w);
+      Beside x;
+      if (!SPLIT) x = fetch(w, 0, live);
       bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag);
       if (KIND == FEW_GATED) ok = epilogue_agrees(ok);        // the four warps meet at barriers below
       if (!ok) break;
@@ -313,6 +335,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           else tmem_ld16(acc + (uint32_t)(h * NT + c), r[h]);
         }
         fp8_wait_ld();
+        fp8_arrived(r[0]);
+        if (NH == 2) fp8_arrived(r[NH - 1]);
         if (c + CH >= NT) {
           fp8_before_sync();
           mbar_arrive(&sm.acc_empty[b]);
@@ -333,12 +357,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           float v[CH], u[CH];
 #pragma unroll
           for (int j = 0; j < CH; ++j) { v[j] = __uint_as_float(r[0][j]); u[j] = __uint_as_float(r[NH - 1][j]); }
-          finish(w, c, live, v, u);
+          if (c > 0) x = fetch(w, c, live);
+          finish(w, c, live, v, u, x);
         }
       }
     }
   }
   if (SPLIT) {
+    Beside x;
+    if (warp >= 2 && first_item < items) x = fetch(first_item, rank * share, min(live_of(first_item), (rank + 1) * share));
     __syncwarp();
     if (warp < 2) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     cluster_sync();                      // all sums have arrived
@@ -364,7 +391,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
           }
         }
-        finish(first_item, tok0, end, v, u);
+        if (c > 0) x = fetch(first_item, tok0, end);
+        finish(first_item, tok0, end, v, u, x);
       }
     }
   }
@@ -387,12 +415,21 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
 // ---------------------------------------------------------------------------------------------- host side
 
-// CTAs that share a tile's K: as many as keep two an SM busy, no fewer than two runs each, and at least `of` tokens' columns to share out.
-static int few_ranks(long long items, int runs, int per_sm) {
+// CTAs that share a tile's K.  A fit to measured times: a stage takes a CTA that has its SM to itself 0.25 us (62 GB/s, what one SM takes in) and two on one SM
+// 0.42; a split costs 1.4 us and a tenth more for each CTA.  (Microseconds at 1, 2, 4, 8 CTAs: 1 x 4096 x 4096 10.3, 8.2, 6.1, 5.8; 8 x 4096 x
+// 14336 13.2, 14.1, 15.5, 21; 64 x 5120 x 1280 15.7, 13.8, 9.0, 7.4; 1 x 8192 x 8192 19.9, 16.1, 14.0, 16.2.)
+static int few_ranks(long long items, int runs, bool two_an_sm) {
   if (const char* want = getenv("MLXB_FP8_RANKS")) return atoi(want);      // experiments and tests
-  int r = 1;
-  while (r < 8 && items * 2 * r <= (long long)per_sm * mlxb_sm_count() && runs >= 4 * r) r *= 2;
-  return r;
+  const int sms = mlxb_sm_count();
+  int best = 1;
+  double best_cost = 0.;
+  for (int r = 1; r <= 8; r *= 2) {
+    if (r > 1 && (runs < 2 * r || items * r > 4LL * sms)) break;
+    const long long ctas = items * r, room = two_an_sm && r > 1 && ctas > sms ? 2 * sms : sms;
+    const double cost = (double)((ctas + room - 1) / room) * ((runs + r - 1) / r) * (room > sms ? 0.42 : 0.25) + (r > 1 ? 1.4 + 0.1 * r : 0.);
+    if (r == 1 || cost < best_cost) { best = r; best_cost = cost; }
+  }
+  return best;
 }
 
 template <int NT, int KIND, bool SPLIT, typename TO>
@@ -404,9 +441,8 @@ static int few_launch(const CUtensorMap& mw, const CUtensorMap& mx, const FewArg
   auto kern = fp8_few_kernel<NT, KIND, SPLIT, TO>;
   static SharedLimit limit;
   if (cudaError_t e = limit.raise(kern, smem)) return mlxb_fail((int)e, "linear (8 bits): %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-  const int resident = (S::PAIR ? 2 : 1) * mlxb_sm_count();
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SPLIT ? a.max_items * ranks : min(a.max_items, resident));
+  cfg.gridDim = dim3(SPLIT ? a.max_items * ranks : min(a.max_items, mlxb_sm_count()));
   cfg.blockDim = dim3(FEW_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -433,7 +469,7 @@ template <int NT, int KIND, typename TO>
 static int few_choose(const CUtensorMap& mw, const CUtensorMap& mx, const FewArgs& a, cudaStream_t stream) {
   // a split hands every rank whole tokens, and its buffer must leave room for the stages
   if constexpr (NT <= (KIND == FEW_GATED ? 32 : 128)) {
-    const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR ? 2 : 1);
+    const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR);
     if (ranks > 1) return few_launch<NT, KIND, true, TO>(mw, mx, a, ranks, stream);
   }
   return few_launch<NT, KIND, false, TO>(mw, mx, a, 1, stream);

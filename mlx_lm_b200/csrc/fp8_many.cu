@@ -34,6 +34,7 @@ struct ManyArgs {
   long long ldo;
   uint8_t* out_scales;
   int out_kgs;
+  bool whole;                                  // rows of out (and residual) begin on 16 bytes
   int* status;
   int act;
   float limit;
@@ -77,7 +78,7 @@ __device__ __forceinline__ void activate_all(float (&v)[N]) {
 template <typename TO>
 __device__ __forceinline__ void store_whole(uint4 u, int n, int N, TO* row) {
   constexpr int PER = 16 / sizeof(TO);
-  if (n + PER <= N && ((uintptr_t)(row + n) & 15) == 0) {
+  if (n + PER <= N) {
     *reinterpret_cast<uint4*>(row + n) = u;
   } else {
     const TO* e = reinterpret_cast<const TO*>(&u);
@@ -260,6 +261,39 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
     for (int t = first_tile; t < n_tiles; t += step, ++it) {
       const int b = S::ACC == 2 ? it & 1 : 0;
       const Place p = place_of(t);
+      // asked for while the products run: a plan's slots and weights, a linear layer's bias (column 32 c + lane of this warp's) and first residuals
+      constexpr int CHUNKS = HALF / 32;
+      const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = KIND == MANY_GATED ? p.n * 128 + half * 64 : p.n * BN + half * HALF;
+      const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
+      const TO* res = KIND == MANY_LINEAR ? reinterpret_cast<const TO*>(after_wait(a.residual)) : nullptr;
+      int slot = 0;
+      float wgt = 1.f, bias[CHUNKS];
+      if (KIND != MANY_LINEAR && lane < rows) {
+        slot = sorted[tile_info[3 * p.m + 1] + row];
+        if (KIND == MANY_GATED && sel_weight) wgt = sel_weight[slot];
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) bias[c] = KIND == MANY_LINEAR && a.bias != nullptr && n0 + 32 * c + lane < a.N ? a.bias[n0 + 32 * c + lane] : 0.f;
+      uint4 ahead[4];
+      auto fetch = [&](int nc) {             // 32 columns from nc on of this lane's row
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ahead[i] = make_uint4(0u, 0u, 0u, 0u);
+          const int n = nc + 8 * i;
+          if (lane >= rows || n >= a.N) continue;
+          const TO* x = res + (long long)(m0 + lane) * a.ldo + n;
+          if (n + 8 <= a.N) {
+            ahead[i] = *reinterpret_cast<const uint4*>(x);
+          } else {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&ahead[i]);
+            const uint16_t* y = reinterpret_cast<const uint16_t*>(x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (n + j < a.N) w[j >> 1] |= (uint32_t)y[j] << (16 * (j & 1));
+          }
+        }
+      };
+      if (sizeof(TO) == 2 && res != nullptr && a.whole) fetch(n0);
       bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag, peer_abort);
       if (KIND == MANY_GATED) {             // the two warps of a quadrant meet below
         uint32_t all;
@@ -270,7 +304,6 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       if (!ok) break;
       fp8_after_sync();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN);
-      constexpr int CHUNKS = HALF / 32;
       uint32_t r[CHUNKS][32];
       if (KIND == MANY_GATED) {             // 64 columns: gate, then up
 #pragma unroll
@@ -280,15 +313,14 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
         for (int c = 0; c < CHUNKS; ++c) tmem_ld32(acc + (uint32_t)(half * HALF + c * 32), r[c]);
       }
       fp8_wait_ld();
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) fp8_arrived(r[c]);
       fp8_before_sync();
       if (CG == 2) mbar_arrive_cluster(peer_addr(&sm.acc_empty[b], 0));
       else mbar_arrive(&sm.acc_empty[b]);
 
       if constexpr (KIND == MANY_GATED) {
-        const int first = tile_info[3 * p.m + 1], cnt = tile_info[3 * p.m + 2];
-        const bool live = row < cnt;
-        const float wgt = live && sel_weight ? sel_weight[sorted[first + row]] : 1.f;
-        const int n0 = p.n * 128 + half * 64;
+        const bool live = lane < rows;
         uint32_t top = 0;
         auto units = [&](auto kind) {
           constexpr int KIND_OF = decltype(kind)::value;
@@ -341,12 +373,6 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       } else {
         constexpr int PER = 16 / sizeof(TO);
         TO* out = reinterpret_cast<TO*>(a.out);
-        const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = p.n * BN + half * HALF;
-        const int first = KIND == MANY_EXPERTS ? tile_info[3 * p.m + 1] : 0;
-        const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
-        int slot = 0;
-        if (KIND == MANY_EXPERTS && lane < rows) slot = sorted[first + row];
-        const TO* res = reinterpret_cast<const TO*>(after_wait(a.residual));
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           float* v = reinterpret_cast<float*>(r[c]);
@@ -354,16 +380,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
           if (nc >= a.N) break;
           if (KIND == MANY_LINEAR) {
             if (a.bias != nullptr) {
-              const float mine = nc + lane < a.N ? a.bias[nc + lane] : 0.f;
-              reinterpret_cast<float*>(stg)[lane] = mine;
-              __syncwarp();
-              const float4* bp = reinterpret_cast<const float4*>(stg);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 x = bp[i];
-                v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
-              }
-              __syncwarp();
+              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias[c], i);
             }
             float (&vv)[32] = *reinterpret_cast<float (*)[32]>(r[c]);
             switch (a.act) {
@@ -372,22 +390,40 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               case EPI_TANH: activate_all<EPI_TANH, sizeof(TO) == 2>(vv); break;
               default: break;
             }
-            if (sizeof(TO) == 2 && res != nullptr && lane < rows) {       // added before the sum is rounded, by rows
-              const TO* rr = res + (long long)(m0 + lane) * a.ldo;
+          }
+          if (!a.whole) {         // rows that do not begin on 16 bytes: 16 columns at a time through shared memory in float32, two rows an instruction
+            float* f = reinterpret_cast<float*>(stg);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int n = nc + 8 * i;
-                if (n + 8 <= a.N && ((uintptr_t)(rr + n) & 15) == 0) {
-                  float e[8];
-                  unpack8(*reinterpret_cast<const uint4*>(rr + n), e);
+            for (int p0 = 0; p0 < 32; p0 += 16) {
 #pragma unroll
-                  for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
-                } else {
-#pragma unroll
-                  for (int j = 0; j < 8; ++j)
-                    if (n + j < a.N) v[8 * i + j] += to_f(rr[n + j]);
+              for (int i = 0; i < 16; ++i) f[lane * 16 + ((i + 2 * lane) & 15)] = v[p0 + i];
+              __syncwarp();
+              const int col = lane & 15, n = nc + p0 + col;
+#pragma unroll 4
+              for (int rr = lane >> 4; rr < 32; rr += 2) {
+                const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
+                if (rr < rows && n < a.N) {
+                  const long long at = (long long)to * a.ldo + n;
+                  float y = f[rr * 16 + ((col + 2 * rr) & 15)];
+                  if (res != nullptr) y += to_f(res[at]);
+                  out[at] = from_f<TO>(y);
                 }
               }
+              __syncwarp();
+            }
+            continue;
+          }
+          if (sizeof(TO) == 2 && res != nullptr) {       // added before the sum is rounded, by rows; the next chunk's are asked for
+            uint4 now[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i] = ahead[i];
+            if (c + 1 < CHUNKS) fetch(nc + 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float e[8];
+              unpack8(now[i], e);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
             }
           }
 #pragma unroll
@@ -408,27 +444,34 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             }
             __syncwarp();
             const int n = nc + p0 + o_piece * PER;
+            float4 add[4];
+            if (sizeof(TO) == 4 && res != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int rr = 8 * j + o_row;
+                add[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (rr < rows && n < a.N) {
+                  const float* x = reinterpret_cast<const float*>(res) + (long long)(m0 + rr) * a.ldo + n;
+                  if (n + 4 <= a.N) {
+                    add[j] = *reinterpret_cast<const float4*>(x);
+                  } else {
+                    add[j].x = x[0];
+                    if (n + 1 < a.N) add[j].y = x[1];
+                    if (n + 2 < a.N) add[j].z = x[2];
+                  }
+                }
+              }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int rr = 8 * j + o_row;
               uint4 u = stg[many_stage(rr, o_piece)];
               const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
-              if (rr < rows && n < a.N) {
-                TO* o = out + (long long)to * a.ldo;
-                if (KIND == MANY_LINEAR && sizeof(TO) == 4 && res != nullptr) {
-                  float* e = reinterpret_cast<float*>(&u);
-                  const float* x = reinterpret_cast<const float*>(res) + (long long)to * a.ldo + n;
-                  if (n + 4 <= a.N && ((uintptr_t)x & 15) == 0) {
-                    const float4 y = *reinterpret_cast<const float4*>(x);
-                    e[0] += y.x; e[1] += y.y; e[2] += y.z; e[3] += y.w;
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                      if (n + i < a.N) e[i] += x[i];
-                  }
-                }
-                store_whole<TO>(u, n, a.N, o);
+              if (sizeof(TO) == 4 && res != nullptr) {
+                u.x = __float_as_uint(__uint_as_float(u.x) + add[j].x); u.y = __float_as_uint(__uint_as_float(u.y) + add[j].y);
+                u.z = __float_as_uint(__uint_as_float(u.z) + add[j].z); u.w = __float_as_uint(__uint_as_float(u.w) + add[j].w);
               }
+              if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
             }
             __syncwarp();
           }
@@ -532,6 +575,7 @@ MLXB_EXPORT int mlxb_fp8_linear_many(const Fp8LinearRecord* rec, long long bytes
   a.M = M; a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = (M + 127) / 128; a.w_tiles = (N + 127) / 128;
   a.tiles_m = (M + 128 * f.cg - 1) / (128 * f.cg); a.tiles_n = (N + f.bn - 1) / f.bn;
   a.bias = r.bias; a.residual = r.residual; a.out = r.out; a.ldo = r.ldo; a.status = r.status; a.act = (int)r.epi;
+  a.whole = !(((uintptr_t)r.out | (uintptr_t)r.residual | (uintptr_t)(r.ldo * (r.out_f32 ? 4 : 2))) & 15);
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d x %d outputs", M, N);
   ManyMaps maps;
   if (int e = fp8_make_map(&maps.x, r.x, M, K, K, 128, "linear (8 bits) x")) return e;
@@ -563,6 +607,7 @@ MLXB_EXPORT int mlxb_fp8_experts_many(const Fp8ExpertsRecord* rec, long long byt
   a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
   a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
   a.limit = (float)r.limit;
+  a.whole = !(((uintptr_t)r.out | (uintptr_t)(r.ldo * (r.out_f32 ? 4 : 2))) & 15);
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
   const long long stack = r.E * (r.gated ? 2 : 1);
   ManyMaps maps;
