@@ -380,8 +380,15 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
           if (nc >= a.N) break;
           if (KIND == MANY_LINEAR) {
             if (a.bias != nullptr) {
+              reinterpret_cast<float*>(stg)[lane] = bias[c];
+              __syncwarp();
+              const float4* bp = reinterpret_cast<const float4*>(stg);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias[c], i);
+              for (int i = 0; i < 8; ++i) {
+                const float4 x = bp[i];
+                v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
+              }
+              __syncwarp();
             }
             float (&vv)[32] = *reinterpret_cast<float (*)[32]>(r[c]);
             switch (a.act) {
@@ -552,14 +559,26 @@ static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t str
   return mlxb_check_launch("linear (8 bits)");
 }
 
+// Tile width and pairs or not: the form whose time, as a sum of what was measured, is least: a launch (set-up, the first copies, the last tile's
+// results), every run of 128 of K, every further wave of tiles.
 struct ManyForm { int bn, cg; };
+struct ManyCost { int bn, cg; double launch, run, wave; };      // microseconds
+static constexpr ManyCost MANY_FORMS[] = {{256, 2, 8.2, .294, 3.6}, {256, 1, 6.2, .398, 1.4}, {128, 2, 5.4, .235, .9}, {128, 1, 4.5, .273, .65}};
 static ManyForm many_form(int M, int N, int K) {
   const char *want_pair = getenv("MLXB_FP8_PAIR"), *want_bn = getenv("MLXB_FP8_BN");     // experiments and tests
-  ManyForm f = {256, 2};
-  if (M <= 128) f.cg = 1;
-  if (want_pair && M > 128) f.cg = want_pair[0] == '1' ? 2 : 1;
-  if (want_bn) f.bn = atoi(want_bn) == 128 ? 128 : 256;
-  return f;
+  const int sms = mlxb_sm_count(), runs = (K + 127) / 128;
+  ManyForm best = {128, 1};
+  double best_cost = -1.;
+  for (const ManyCost& f : MANY_FORMS) {
+    if (f.cg == 2 && M <= 128) continue;
+    if (want_pair && M > 128 && (want_pair[0] == '1') != (f.cg == 2)) continue;
+    if (want_bn && atoi(want_bn) != f.bn) continue;
+    const long long tiles = (long long)((M + f.cg * 128 - 1) / (f.cg * 128)) * ((N + f.bn - 1) / f.bn);
+    const long long units = sms / f.cg, waves = (tiles + units - 1) / units;
+    const double cost = f.launch + waves * runs * f.run + (waves - 1) * f.wave;
+    if (best_cost < 0. || cost < best_cost) { best = {f.bn, f.cg}; best_cost = cost; }
+  }
+  return best;
 }
 
 // As mlxb_fp8_linear_few, for any number of rows.

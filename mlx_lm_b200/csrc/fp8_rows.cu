@@ -91,58 +91,74 @@ __device__ __forceinline__ void quantize512(const Sixteen<T>& x, int kg, int ld,
   if (lane == 0) *reinterpret_cast<uint32_t*>(scale) = s;
 }
 
-// FQ_AT_ONCE items of a warp have their loads out together.
-constexpr int FQ_AT_ONCE = 2;
-
-template <typename T, bool VEC>
+// AT items of a warp have their loads out together: one where a call is a chain of latencies, four where it is bytes.
+template <typename T, bool VEC, int AT>
 __global__ void __launch_bounds__(32 * FQ_WARPS)
 fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
   pdl_wait();
   pdl_trigger();
   x = after_wait(x);
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, tiles = (group_rows + 127) >> 7;
-  const long long items = (long long)rows * kgs, first = ((long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5)) * FQ_AT_ONCE;
-  Sixteen<T> v[FQ_AT_ONCE];
+  const long long items = (long long)rows * kgs, first = ((long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5)) * AT;
+  if (first >= items) return;
+  Sixteen<T> v[AT];
+  long long r = first / kgs;
+  int kg = (int)(first - r * kgs);
+  const long long r0 = r;
+  const int kg0 = kg;
 #pragma unroll
-  for (int j = 0; j < FQ_AT_ONCE; ++j) {
-    const long long w = min(first + j, items - 1), r = w / kgs;
-    v[j].template load<VEC>(x + r * ldx, 512 * (int)(w - r * kgs) + 16 * lane, K);
+  for (int j = 0; j < AT; ++j) {
+    if (r < rows) v[j].template load<VEC>(x + r * ldx, 512 * kg + 16 * lane, K);
+    if (++kg == kgs) { kg = 0; ++r; }
   }
+  r = r0;
+  kg = kg0;
+  int group = (int)(r / group_rows), in = (int)(r - (long long)group * group_rows);
 #pragma unroll
-  for (int j = 0; j < FQ_AT_ONCE; ++j) {
-    const long long w = first + j, r = w / kgs;
-    if (w >= items) return;
-    const int kg = (int)(w - r * kgs), group = (int)(r / group_rows), in = (int)(r - (long long)group * group_rows);
+  for (int j = 0; j < AT; ++j) {
+    if (r >= rows) return;
     quantize512<T>(v[j], kg, ld, codes + r * ld, scales + (((long long)group * tiles + (in >> 7)) * kgs + kg) * FP8_TILE + fp8_scale_row(in), lane);
+    if (++kg == kgs) {
+      kg = 0;
+      ++r;
+      if (++in == group_rows) { in = 0; ++group; }
+    }
   }
 }
 
+// A warp takes up to four of a tile's rows at a time: their slots are looked up together, and so are the rows' pieces.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * FQ_WARPS)
 fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted, const int* tile_info, const int* n_tiles, int tile_rows,
                   uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
+  constexpr int AT = 4;
   pdl_wait();
   pdl_trigger();
   x = after_wait(x);
   sorted = after_wait(sorted);
   tile_info = after_wait(tile_info);
-  const int t = blockIdx.x;
-  if (t >= after_wait(n_tiles)[0]) return;
-  const int first = tile_info[3 * t + 1], kgs = (K + 511) >> 9, items = tile_info[3 * t + 2] * kgs;
-  const int lane = threadIdx.x & 31;
-  for (int w0 = (blockIdx.y * FQ_WARPS + (threadIdx.x >> 5)) * FQ_AT_ONCE; w0 < items; w0 += gridDim.y * FQ_WARPS * FQ_AT_ONCE) {
-    Sixteen<T> v[FQ_AT_ONCE];
+  const int t = blockIdx.x, have = after_wait(n_tiles)[0], first = tile_info[3 * t + 1], rows = tile_info[3 * t + 2];
+  if (t >= have) return;
+  const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, warps = gridDim.y * FQ_WARPS, warp = blockIdx.y * FQ_WARPS + (threadIdx.x >> 5);
+  // few rows: a warp takes one of them, or a part of its columns; many: four
+  const int parts = max(1, min(kgs, warps / rows)), row_warps = warps / parts;
+  if (warp >= row_warps * parts) return;
+  const int part = warp / row_warps;
+  for (int i = warp - part * row_warps; i < rows; i += AT * row_warps) {
+    long long src[AT];
 #pragma unroll
-    for (int j = 0; j < FQ_AT_ONCE; ++j) {
-      const int w = min(w0 + j, items - 1), r = w / kgs;
-      const long long src = sorted[first + r] / a_div;
-      v[j].template load<VEC>(x + src * ldx, 512 * (w - r * kgs) + 16 * lane, K);
-    }
+    for (int j = 0; j < AT; ++j) src[j] = i + j * row_warps < rows ? sorted[first + i + j * row_warps] / a_div : -1;
+    for (int kg = part; kg < kgs; kg += parts) {
+      Sixteen<T> v[AT];
 #pragma unroll
-    for (int j = 0; j < FQ_AT_ONCE; ++j) {
-      const int w = w0 + j, r = w / kgs, kg = w - r * kgs;
-      if (w < items)
-        quantize512<T>(v[j], kg, ld, codes + ((long long)t * tile_rows + r) * ld, scales + ((long long)t * kgs + kg) * FP8_TILE + fp8_scale_row(r), lane);
+      for (int j = 0; j < AT; ++j)
+        if (src[j] >= 0) v[j].template load<VEC>(x + src[j] * ldx, 512 * kg + 16 * lane, K);
+#pragma unroll
+      for (int j = 0; j < AT; ++j) {
+        const int r = i + j * row_warps;
+        if (src[j] >= 0)
+          quantize512<T>(v[j], kg, ld, codes + ((long long)t * tile_rows + r) * ld, scales + ((long long)t * kgs + kg) * FP8_TILE + fp8_scale_row(r), lane);
+      }
     }
   }
 }
@@ -182,21 +198,29 @@ MLXB_EXPORT int mlxb_fp8_quantize(const QuantizeRecord* rec, long long bytes, cu
   if (rows <= 0) return 0;
   if (int e = check("fp8_quantize", x, K, ldx, codes, ld, scales)) return e;
   if (group_rows <= 0 || rows % group_rows) return mlxb_fail(MLXB_BAD_ARG, "fp8_quantize: %d rows in groups of %d", rows, group_rows);
-  const long long blocks = ((long long)rows * ((K + 511) / 512) + FQ_WARPS * FQ_AT_ONCE - 1) / (FQ_WARPS * FQ_AT_ONCE);
+  const long long items = (long long)rows * ((K + 511) / 512);
+  const bool many = items >= 16LL * FQ_WARPS * mlxb_sm_count();
+  const long long blocks = many ? (items + 4 * FQ_WARPS - 1) / (4 * FQ_WARPS) : (items + FQ_WARPS - 1) / FQ_WARPS;
   if (blocks > 0x7fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "fp8_quantize: %d rows of %d", rows, K);
-#define GO(T, V)                                                                                                                             \
-  launch_pdl(fp8_quantize_kernel<T, V>, dim3((unsigned)blocks), dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, rows, K, group_rows, \
+#define LAUNCH(T, V, AT)                                                                                                                        \
+  launch_pdl(fp8_quantize_kernel<T, V, AT>, dim3((unsigned)blocks), dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, rows, K, group_rows, \
              (uint8_t*)codes, ld, (uint8_t*)scales)
+#define GO(T, V)                          \
+  {                                       \
+    if (many) LAUNCH(T, V, 4);            \
+    else LAUNCH(T, V, 1);                 \
+  }
   if (dtype == MLXB_BF16) {
-    if (whole_pieces<__nv_bfloat16>(x, ldx, K)) GO(__nv_bfloat16, true);
-    else GO(__nv_bfloat16, false);
+    if (whole_pieces<__nv_bfloat16>(x, ldx, K)) GO(__nv_bfloat16, true)
+    else GO(__nv_bfloat16, false)
   } else if (dtype == MLXB_F32) {
-    if (whole_pieces<float>(x, ldx, K)) GO(float, true);
-    else GO(float, false);
+    if (whole_pieces<float>(x, ldx, K)) GO(float, true)
+    else GO(float, false)
   } else {
     return mlxb_fail(MLXB_BAD_DTYPE, "fp8_quantize: dtype code %d", dtype);
   }
 #undef GO
+#undef LAUNCH
   return mlxb_check_launch("fp8_quantize");
 }
 
@@ -213,8 +237,8 @@ MLXB_EXPORT int mlxb_fp8_gather(const GatherRecord* rec, long long bytes, cudaSt
   if (max_tiles <= 0) return 0;
   if (int e = check("moe_gather_fp8", x, K, ldx, codes, ld, scales)) return e;
   if (a_div <= 0 || tile_rows <= 0 || tile_rows > 128) return mlxb_fail(MLXB_BAD_ARG, "moe_gather_fp8: tiles of %d rows", tile_rows);
-  const int most = tile_rows * ((K + 511) / 512);
-  const dim3 grid(max_tiles, max(1, min(16, most / FQ_WARPS / 4)));
+  // a tile's rows over a few blocks: four rows a warp where there are tiles enough for that, else more blocks
+  const dim3 grid(max_tiles, max_tiles >= 2 * mlxb_sm_count() ? max(1, tile_rows / (4 * FQ_WARPS)) : max(1, tile_rows / FQ_WARPS));
 #define GO(T, V)                                                                                                                             \
   launch_pdl(fp8_gather_kernel<T, V>, grid, dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, K, a_div, sorted, tile_info, n_tiles, tile_rows, \
              (uint8_t*)codes, ld, (uint8_t*)scales)
