@@ -39,7 +39,12 @@ __device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t fp8_quad(float a, float b, float c, float d) { return fp8_pair(a, b) | fp8_pair(c, d) << 16; }
+__device__ __forceinline__ uint32_t fp8_quad(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
 
 // Bytes from a row's place to its scales in a tile, without the run.
 __device__ __forceinline__ int fp8_scale_row(int r) { return (r & 31) * 16 + ((r >> 5) & 3) * 4; }

@@ -130,12 +130,13 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
   pdl_trigger();
 
   // Where a tile lies.  A linear layer's tiles go by groups of 8 row tiles, columns after columns, so that those which run together read few
-  // rows of either operand; a plan's by column blocks, neighbours share an expert's rows of W.
+  // rows of either operand; a plan's by its own tiles, so that an expert's are together and its weights and rows come from memory once (by blocks of
+  // columns, 32768 slots of 2048 over 64 experts were read again for every block: 154 us).
   struct Place { int m, n; };
   const int* tile_info = a.tile_info;
   int tiles_m = a.tiles_m;
   auto place_of = [&](int t) {
-    if (KIND != MANY_LINEAR) return Place{t % tiles_m, t / tiles_m};
+    if (KIND != MANY_LINEAR) return Place{t / a.tiles_n, t % a.tiles_n};
     const int per = 8 * a.tiles_n, g = t / per, r = t - g * per, rows = min(8, tiles_m - 8 * g);
     return Place{8 * g + r % rows, r / rows};
   };

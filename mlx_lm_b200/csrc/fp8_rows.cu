@@ -62,10 +62,9 @@ __device__ __forceinline__ uint32_t run_max(uint32_t v) {        // over the eig
   return v;
 }
 
-// 512 columns from 512 * kg on of one row, by a warp: codes to `out` (the row), the four scales to `scale` (the row's word in its tile)
+// 512 columns of one row, by a warp: codes to `out` (this lane's 16; `in`: they exist), the four scales to `scale` (the row's word in its tile)
 template <typename T>
-__device__ __forceinline__ void quantize512(const Sixteen<T>& x, int kg, int ld, uint8_t* out, uint8_t* scale, int lane) {
-  const int c = 512 * kg + 16 * lane;
+__device__ __forceinline__ void quantize512(const Sixteen<T>& x, bool in, uint8_t* out, uint8_t* scale, int lane) {
   uint32_t top = run_max(x.largest());
   const bool odd = __any_sync(0xffffffffu, top >= 0x7f800000u);   // rare: something is not finite
   if (odd) {
@@ -84,7 +83,7 @@ __device__ __forceinline__ void quantize512(const Sixteen<T>& x, int kg, int ld,
     for (int i = 0; i < 4; ++i)
       w[i] = fp8_quad(fp8_or_nan(x.number(4 * i)) * f, fp8_or_nan(x.number(4 * i + 1)) * f, fp8_or_nan(x.number(4 * i + 2)) * f, fp8_or_nan(x.number(4 * i + 3)) * f);
   }
-  if (c < ld) *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (in) *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
   uint32_t s = (uint32_t)(e + 127) << (8 * (lane >> 3));
   s |= __shfl_xor_sync(0xffffffffu, s, 8);
   s |= __shfl_xor_sync(0xffffffffu, s, 16);
@@ -117,7 +116,7 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
 #pragma unroll
   for (int j = 0; j < AT; ++j) {
     if (r >= rows) return;
-    quantize512<T>(v[j], kg, ld, codes + r * ld, scales + (((long long)group * tiles + (in >> 7)) * kgs + kg) * FP8_TILE + fp8_scale_row(in), lane);
+    quantize512<T>(v[j], 512 * kg + 16 * lane < ld, codes + r * ld + 512 * kg + 16 * lane, scales + (((long long)group * tiles + (in >> 7)) * kgs + kg) * FP8_TILE + fp8_scale_row(in), lane);
     if (++kg == kgs) {
       kg = 0;
       ++r;
@@ -126,12 +125,12 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
   }
 }
 
-// A warp takes up to four of a tile's rows at a time: their slots are looked up together, and so are the rows' pieces.
+// A warp takes up to two of a tile's rows at a time: their slots are looked up together, and so are the rows' pieces.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * FQ_WARPS)
 fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted, const int* tile_info, const int* n_tiles, int tile_rows,
                   uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
-  constexpr int AT = 4;
+  constexpr int AT = 2;
   pdl_wait();
   pdl_trigger();
   x = after_wait(x);
@@ -140,24 +139,31 @@ fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted
   const int t = blockIdx.x, have = after_wait(n_tiles)[0], first = tile_info[3 * t + 1], rows = tile_info[3 * t + 2];
   if (t >= have) return;
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, warps = gridDim.y * FQ_WARPS, warp = blockIdx.y * FQ_WARPS + (threadIdx.x >> 5);
-  // few rows: a warp takes one of them, or a part of its columns; many: four
+  // few rows: a warp takes one of them, or a part of its columns
   const int parts = max(1, min(kgs, warps / rows)), row_warps = warps / parts;
   if (warp >= row_warps * parts) return;
   const int part = warp / row_warps;
   for (int i = warp - part * row_warps; i < rows; i += AT * row_warps) {
-    long long src[AT];
+    const T* px[AT];
+    uint8_t *pc[AT], *ps[AT];
 #pragma unroll
-    for (int j = 0; j < AT; ++j) src[j] = i + j * row_warps < rows ? sorted[first + i + j * row_warps] / a_div : -1;
+    for (int j = 0; j < AT; ++j) {
+      const int r = i + j * row_warps;
+      px[j] = r < rows ? x + (long long)(sorted[first + r] / a_div) * ldx : nullptr;
+      pc[j] = codes + ((long long)t * tile_rows + r) * ld + 512 * part + 16 * lane;
+      ps[j] = scales + ((long long)t * kgs + part) * FP8_TILE + fp8_scale_row(r);
+    }
     for (int kg = part; kg < kgs; kg += parts) {
+      const int c = 512 * kg + 16 * lane;
       Sixteen<T> v[AT];
 #pragma unroll
       for (int j = 0; j < AT; ++j)
-        if (src[j] >= 0) v[j].template load<VEC>(x + src[j] * ldx, 512 * kg + 16 * lane, K);
+        if (px[j]) v[j].template load<VEC>(px[j], c, K);
 #pragma unroll
       for (int j = 0; j < AT; ++j) {
-        const int r = i + j * row_warps;
-        if (src[j] >= 0)
-          quantize512<T>(v[j], kg, ld, codes + ((long long)t * tile_rows + r) * ld, scales + ((long long)t * kgs + kg) * FP8_TILE + fp8_scale_row(r), lane);
+        if (px[j]) quantize512<T>(v[j], c < ld, pc[j], ps[j], lane);
+        pc[j] += 512 * parts;
+        ps[j] += FP8_TILE * parts;
       }
     }
   }
