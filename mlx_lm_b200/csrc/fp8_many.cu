@@ -34,7 +34,6 @@ struct ManyArgs {
   long long ldo;
   uint8_t* out_scales;
   int out_kgs;
-  bool whole;                                  // rows of out (and residual) begin on 16 bytes
   int* status;
   int act;
   float limit;
@@ -88,7 +87,8 @@ __device__ __forceinline__ void store_whole(uint4 u, int n, int N, TO* row) {
   }
 }
 
-template <int BN, int CG, int KIND, typename TO>
+// WHOLE: rows of out (and residual) begin on 16 bytes.
+template <int BN, int CG, int KIND, typename TO, bool WHOLE>
 __global__ void __launch_bounds__(MANY_THREADS)
 fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
   using S = ManyShape<BN, CG>;
@@ -262,39 +262,17 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
     for (int t = first_tile; t < n_tiles; t += step, ++it) {
       const int b = S::ACC == 2 ? it & 1 : 0;
       const Place p = place_of(t);
-      // asked for while the products run: a plan's slots and weights, a linear layer's bias (column 32 c + lane of this warp's) and first residuals
+      // asked for while the products run: a plan's slots and their weights
       constexpr int CHUNKS = HALF / 32;
       const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = KIND == MANY_GATED ? p.n * 128 + half * 64 : p.n * BN + half * HALF;
       const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
       const TO* res = KIND == MANY_LINEAR ? reinterpret_cast<const TO*>(after_wait(a.residual)) : nullptr;
       int slot = 0;
-      float wgt = 1.f, bias[CHUNKS];
+      float wgt = 1.f;
       if (KIND != MANY_LINEAR && lane < rows) {
         slot = sorted[tile_info[3 * p.m + 1] + row];
         if (KIND == MANY_GATED && sel_weight) wgt = sel_weight[slot];
       }
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) bias[c] = KIND == MANY_LINEAR && a.bias != nullptr && n0 + 32 * c + lane < a.N ? a.bias[n0 + 32 * c + lane] : 0.f;
-      uint4 ahead[4];
-      auto fetch = [&](int nc) {             // 32 columns from nc on of this lane's row
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ahead[i] = make_uint4(0u, 0u, 0u, 0u);
-          const int n = nc + 8 * i;
-          if (lane >= rows || n >= a.N) continue;
-          const TO* x = res + (long long)(m0 + lane) * a.ldo + n;
-          if (n + 8 <= a.N) {
-            ahead[i] = *reinterpret_cast<const uint4*>(x);
-          } else {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&ahead[i]);
-            const uint16_t* y = reinterpret_cast<const uint16_t*>(x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (n + j < a.N) w[j >> 1] |= (uint32_t)y[j] << (16 * (j & 1));
-          }
-        }
-      };
-      if (sizeof(TO) == 2 && res != nullptr && a.whole) fetch(n0);
       bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag, peer_abort);
       if (KIND == MANY_GATED) {             // the two warps of a quadrant meet below
         uint32_t all;
@@ -374,6 +352,9 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       } else {
         constexpr int PER = 16 / sizeof(TO);
         TO* out = reinterpret_cast<TO*>(a.out);
+        float bias[CHUNKS];                   // column 32 c + lane of this warp's
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) bias[c] = KIND == MANY_LINEAR && a.bias != nullptr && n0 + 32 * c + lane < a.N ? a.bias[n0 + 32 * c + lane] : 0.f;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           float* v = reinterpret_cast<float*>(r[c]);
@@ -399,7 +380,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               default: break;
             }
           }
-          if (!a.whole) {         // rows that do not begin on 16 bytes: 16 columns at a time through shared memory in float32, two rows an instruction
+          if constexpr (!WHOLE) {         // rows that do not begin on 16 bytes: 16 columns at a time through shared memory in float32, two rows an instruction
             float* f = reinterpret_cast<float*>(stg);
 #pragma unroll
             for (int p0 = 0; p0 < 32; p0 += 16) {
@@ -420,18 +401,24 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               __syncwarp();
             }
             continue;
-          }
-          if (sizeof(TO) == 2 && res != nullptr) {       // added before the sum is rounded, by rows; the next chunk's are asked for
-            uint4 now[4];
+          } else {
+          if (sizeof(TO) == 2 && res != nullptr && lane < rows) {       // added before the sum is rounded, by rows
+            const TO* x = res + (long long)(m0 + lane) * a.ldo + nc;
+            if (nc + 32 <= a.N) {
+              uint4 u[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) now[i] = ahead[i];
-            if (c + 1 < CHUNKS) fetch(nc + 32);
+              for (int i = 0; i < 4; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float e[8];
-              unpack8(now[i], e);
+              for (int i = 0; i < 4; ++i) {
+                float e[8];
+                unpack8(u[i], e);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
+                for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (nc + i < a.N) v[i] += to_f(x[i]);
             }
           }
 #pragma unroll
@@ -483,6 +470,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             }
             __syncwarp();
           }
+          }
         }
       }
     }
@@ -527,11 +515,11 @@ static int scales_map(CUtensorMap* map, const void* base, long long tiles, const
   return mlxb_fail(MLXB_BAD_ARG, "%s: cuTensorMapEncodeTiled(%lld tiles of scales): %s", what, tiles, msg ? msg : "?");
 }
 
-template <int BN, int CG, int KIND, typename TO>
-static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
+template <int BN, int CG, int KIND, typename TO, bool WHOLE>
+static int many_launch_as(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
   constexpr size_t smem = sizeof(ManySmem<BN, CG>) + 1024;
   static_assert(smem <= 227 * 1024, "stages and staging buffers fit a CTA's shared memory");
-  auto kern = fp8_many_kernel<BN, CG, KIND, TO>;
+  auto kern = fp8_many_kernel<BN, CG, KIND, TO, WHOLE>;
   static SharedLimit limit;
   if (cudaError_t e = limit.raise(kern, smem)) return mlxb_fail((int)e, "linear (8 bits): %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
   const long long tiles = (long long)a.tiles_m * a.tiles_n;
@@ -558,6 +546,14 @@ static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t str
   cfg.numAttrs = n;
   cudaLaunchKernelEx(&cfg, kern, maps, a);
   return mlxb_check_launch("linear (8 bits)");
+}
+
+template <int BN, int CG, int KIND, typename TO>
+static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
+  if (KIND == MANY_GATED || !(((uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)(a.ldo * (long long)sizeof(TO))) & 15))
+    return many_launch_as<BN, CG, KIND, TO, true>(maps, a, stream);
+  if constexpr (KIND != MANY_GATED) return many_launch_as<BN, CG, KIND, TO, false>(maps, a, stream);
+  return MLXB_BAD_ARG;
 }
 
 // Tile width and pairs or not: the form whose time, as a sum of what was measured, is least: a launch (set-up, the first copies, the last tile's
@@ -595,7 +591,6 @@ MLXB_EXPORT int mlxb_fp8_linear_many(const Fp8LinearRecord* rec, long long bytes
   a.M = M; a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.x_tiles = (M + 127) / 128; a.w_tiles = (N + 127) / 128;
   a.tiles_m = (M + 128 * f.cg - 1) / (128 * f.cg); a.tiles_n = (N + f.bn - 1) / f.bn;
   a.bias = r.bias; a.residual = r.residual; a.out = r.out; a.ldo = r.ldo; a.status = r.status; a.act = (int)r.epi;
-  a.whole = !(((uintptr_t)r.out | (uintptr_t)r.residual | (uintptr_t)(r.ldo * (r.out_f32 ? 4 : 2))) & 15);
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): %d x %d outputs", M, N);
   ManyMaps maps;
   if (int e = fp8_make_map(&maps.x, r.x, M, K, K, 128, "linear (8 bits) x")) return e;
@@ -627,7 +622,6 @@ MLXB_EXPORT int mlxb_fp8_experts_many(const Fp8ExpertsRecord* rec, long long byt
   a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
   a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
   a.limit = (float)r.limit;
-  a.whole = !(((uintptr_t)r.out | (uintptr_t)(r.ldo * (r.out_f32 ? 4 : 2))) & 15);
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
   const long long stack = r.E * (r.gated ? 2 : 1);
   ManyMaps maps;
