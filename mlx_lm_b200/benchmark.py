@@ -24,12 +24,13 @@ def setup_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--delay", type=float, default=0, help="Seconds to wait between trials")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     p.add_argument("--kv-bits", type=int, choices=[8], default=None, help="Keys and values in 8 bits")
+    p.add_argument("--weight-bits", type=int, choices=[8], default=None, help="Weights in 8-bit floating point")
     return p
 
 
 def main(argv=None) -> None:
     args = setup_arg_parser().parse_args(argv)
-    model, tokenizer, config = load(args.model, return_config=True, dtype=args.dtype)
+    model, tokenizer, config = load(args.model, return_config=True, dtype=args.dtype, weight_bits=args.weight_bits)
     tokenizer.eos_token_ids = set()      # no early stop
     g = torch.Generator().manual_seed(0)
     vocab = int(config["vocab_size"])

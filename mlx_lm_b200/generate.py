@@ -50,16 +50,19 @@ DEFAULT_SEED = None
 def load(path: str, tokenizer_config: Optional[dict] = None, model_config: Optional[dict] = None,
          adapter_path: Optional[str] = None, lazy: bool = False, return_config: bool = False,
          revision: Optional[str] = None, trust_remote_code: bool = False, dtype: str = "bfloat16",
-         device: str = "cuda"):
+         device: str = "cuda", weight_bits: Optional[int] = None):
     """Model folder -> ``(model, tokenizer)`` (or ``(model, tokenizer, config)``), the signature of
     mlx-lm's ``load`` (mlx_lm/utils.py:483-541).
 
     Local folders only (``revision`` and ``trust_remote_code`` are accepted and unused; ``adapter_path``
     must be None: adapters are not built).  ``dtype`` is ``"bfloat16"`` (the serving path) or
-    ``"float32"`` (everything in true 32-bit).  ``tokenizer_config`` may carry ``eos_token_ids``."""
+    ``"float32"`` (everything in true 32-bit).  ``weight_bits=8`` (with bfloat16): the weights of linear layers and
+    experts are held in 8-bit floating point with a scale for each row and 128 columns, and the rows that meet them are
+    rounded the same way; half the bytes of a decode step's weights, twice the rate of a prompt's products.
+    ``tokenizer_config`` may carry ``eos_token_ids``."""
     if adapter_path is not None:
         raise ValueError("adapter_path: adapters are not offered by this engine")
-    model, config = load_model(path, dtype=dtype, device=device, model_config=model_config)
+    model, config = load_model(path, dtype=dtype, device=device, model_config=model_config, weight_bits=weight_bits)
     tokenizer = load_tokenizer(path, config, (tokenizer_config or {}).get("eos_token_ids"))
     return (model, tokenizer, config) if return_config else (model, tokenizer)
 
@@ -438,6 +441,8 @@ def setup_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--num-pages", type=int, default=None, help="pages in the pool (default: enough for 64 requests)")
     p.add_argument("--kv-bits", type=int, choices=[8], default=None,
                    help="keep keys and values in 8 bits with a scale for each block of 16 positions and head (default: in --dtype)")
+    p.add_argument("--weight-bits", type=int, choices=[8], default=None,
+                   help="hold the weights of linear layers and experts in 8-bit floating point (default: in --dtype)")
     return p
 
 
@@ -461,7 +466,7 @@ def main(argv: Optional[Sequence[str]] = None) -> None:
         args.model = tmp.name
     if args.model is None:
         parser.error("--model (or --random-weights with --config) is required")
-    model, tokenizer = load(args.model, dtype=args.dtype)
+    model, tokenizer = load(args.model, dtype=args.dtype, weight_bits=args.weight_bits)
     for t in args.extra_eos_token:
         tokenizer.add_eos_token(t)
     prompt = args.prompt.replace("\\n", "\n").replace("\\t", "\t")

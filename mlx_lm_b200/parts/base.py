@@ -132,6 +132,19 @@ class Part:
         for c in self.children():
             c.bind_all(tensors, dtype, device)
 
+    # How the model keeps large weights: None as they are, 8 in 8-bit floating point (ops.fp8_quantize).  Known before the weights are bound.
+    weight_bits: Optional[int] = None
+
+    def set_weight_bits(self, bits: Optional[int]) -> None:
+        self.weight_bits = bits
+        for c in self.children():
+            c.set_weight_bits(bits)
+
+    def hold_eight_bits(self) -> int:
+        """Called on all parts once every weight is bound, if they are kept in 8 bits: this part and its children put theirs into that form; how
+        many weights that were."""
+        return sum(c.hold_eight_bits() for c in self.children())
+
 
 class Norm(Part):
     def forward(self, ctx, x, rows=None):

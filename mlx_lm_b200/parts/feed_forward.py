@@ -94,7 +94,8 @@ class ExpertsMLP(FeedForward):
 
     Options of the router: ``correction`` (a tensor ``<name>.correction``, one number per router output, added to the
     scores for the choice only: the weights are the scores without it); ``groups = (count, keep)``: the router outputs
-    form ``count`` equal groups of neighbours, a group's score is its largest choice score, and only outputs of the
+    form ``count`` equal groups of neighbours, a group's score is its largest choice score (``group_score="best"``) or the
+    sum of its two largest (``"two"``), and only outputs of the
     ``keep`` best groups can be chosen; ``identity``: the router has that many more outputs than there are experts with
     tensors, and a token that chooses one of them gets its own input back (times the weight); ``renormalize_eps`` is
     added to the sum the weights are divided by; ``weight_scale`` multiplies every weight.  ``unit="bounded"`` with
@@ -121,7 +122,7 @@ class ExpertsMLP(FeedForward):
                  init: Init = Init(), router_init: Init = Init(), correction: bool = False, groups=None, identity: int = 0,
                  renormalize_eps: float = 0.0, weight_scale: float = 1.0, unit: str = "silu", limit: float = 0.0,
                  shared: FeedForward = None, correction_name: str = "correction", table_vocab: int = 0,
-                 table_name: str = "table"):
+                 table_name: str = "table", group_score: str = "best"):
         n_outputs = n_experts + int(identity)
         if n_experts < 0 or identity < 0 or not 1 <= top <= n_outputs:
             raise ValueError(f"{name}: {top} of {n_experts} experts and {identity} identity experts")
@@ -137,6 +138,15 @@ class ExpertsMLP(FeedForward):
         count, keep = (int(groups[0]), int(groups[1])) if groups else (1, 1)
         if count < 1 or n_outputs % count or not 1 <= keep <= count or top > keep * (n_outputs // count):
             raise ValueError(f"{name}: {n_outputs} router outputs in {count} groups of which {keep} stay, {top} chosen")
+        if group_score not in ops.MOE_GROUP_SCORES:
+            raise ValueError(f"{name}: groups judged by {group_score!r}, not one of {sorted(ops.MOE_GROUP_SCORES)}")
+        # the router with the plan in one call takes so many; it is what knows group_score="two"
+        self.planned = (n_outputs <= ops.MOE_ROUTE_PLAN_EXPERTS and count <= ops.MOE_ROUTE_PLAN_GROUPS and top <= ops.MOE_ROUTE_PLAN_TOP
+                        and n_experts > 0)
+        if group_score != "best" and not self.planned:
+            raise ValueError(f"{name}: groups judged by {group_score!r}: up to {ops.MOE_ROUTE_PLAN_EXPERTS} router outputs in up to "
+                             f"{ops.MOE_ROUTE_PLAN_GROUPS} groups, {ops.MOE_ROUTE_PLAN_TOP} chosen, some with tensors")
+        self.group_score = group_score
         self.name, self.width, self.inner, self.n_experts, self.top = name, width, inner, n_experts, top
         self.score, self.renormalize, self.scale_input = score, renormalize, scale_input
         self.identity, self.n_outputs, self.groups, self.keep_groups = int(identity), n_outputs, count, keep
@@ -150,13 +160,40 @@ class ExpertsMLP(FeedForward):
             self.kernel_libs = ("moe", "moe_tcgen05")      # the sum over a token's experts is the block's
         else:
             self.router = Linear(f"{name}.{router_name}", width, n_outputs, bias=False, weight_suffix="", init=router_init)
+            self.router.eight_bits = False       # it decides who computes
+            if group_score != "best":
+                self.kernel_libs = type(self).kernel_libs + ("moe_router",)
         self.names = [(f"{name}.{expert_prefix}{e}.{gate_name}", f"{name}.{expert_prefix}{e}.{up_name}",
                        f"{name}.{expert_prefix}{e}.{down_name}") for e in range(n_experts)]
         self.init = init
         self.w_in = self.w_out = None
+        self.held = None          # in 8 bits: ((codes, scales) of the gate and up matrices, of the down matrices)
 
     def children(self):
         return tuple(p for p in (self.router, self.shared) if p is not None)
+
+    def set_weight_bits(self, bits) -> None:
+        super().set_weight_bits(bits)
+        if bits and not self.table_vocab:
+            self.kernel_libs = tuple(dict.fromkeys(self.kernel_libs + ("moe_router",)))
+
+    def hold_eight_bits(self) -> int:
+        """The experts' stacked weights as e4m3 codes with a scale for each row and 128 columns; steps then run ``ops.moe_gather_fp8`` and
+        ``ops.moe_gemm_fp8`` over the plan."""
+        n = super().hold_eight_bits()
+        if self.weight_bits != 8 or self.w_in is None:
+            return n
+        if self.w_in.dtype != torch.bfloat16:
+            raise ValueError(f"{self.name}: weights in 8 bits go with a bfloat16 run, not with {self.w_in.dtype}")
+        stream, held = ops.current_stream(), []
+        for w, rows in ((self.w_in, self.inner), (self.w_out, self.width)):
+            w = w.view(-1, w.shape[-1])
+            codes, scales = ops.fp8_empty(rows, w.shape[1], w.device, groups=w.shape[0] // rows)
+            ops.fp8_quantize(w, codes, scales, stream, group_rows=rows)
+            held.append((codes, scales))
+        self.held = tuple(held)
+        self.w_in = self.w_out = None
+        return n + 1
 
     def param_specs(self):
         specs = []
@@ -205,14 +242,17 @@ class ExpertsMLP(FeedForward):
         T, E, top, F_, D = x.shape[0], self.n_experts, self.top, self.inner, self.width
         S, EO = T * top, self.n_outputs
         sel_e = sel_w = None
+        planned = self.planned and not self.table_vocab and (self.held is not None or self.group_score != "best")
         if not self.table_vocab:
             logits = self.router.forward(ctx, x, ctx.ws.get("moe_logits", T, (EO + 7) // 8 * 8, torch.float32)[:, :EO])
             sel_e = ctx.ws.flat("moe_sel_expert", S, torch.int32)
             sel_w = ctx.ws.flat("moe_sel_weight", S, torch.float32)
             ops.label(self.name + ".route", 8.0 * T * EO, 4.0 * T * EO + 8.0 * S)
-            ops.moe_route(logits, ctx.token_req, top, sel_e, sel_w, ctx.stream, score=self.score, renormalize=self.renormalize,
-                          correction=self.correction, groups=self.groups, keep_groups=self.keep_groups, identity=self.identity,
-                          renormalize_eps=self.renormalize_eps, weight_scale=self.weight_scale)
+            router = dict(score=self.score, renormalize=self.renormalize, correction=self.correction, groups=self.groups,
+                          keep_groups=self.keep_groups, identity=self.identity, renormalize_eps=self.renormalize_eps,
+                          weight_scale=self.weight_scale)
+            if not planned:
+                ops.moe_route(logits, ctx.token_req, top, sel_e, sel_w, ctx.stream, **router)
         y = ctx.ws.get("moe_out", S, D, torch.float32)
         if E == 0:
             return y, sel_e, sel_w
@@ -223,16 +263,23 @@ class ExpertsMLP(FeedForward):
         # of 64 on mma.sync through the sorted list; float32 and odd sizes: the CUDA cores
         many = tc and S >= self.MANY_SLOTS
         few = tc and not many and S <= self.FEW_SLOTS_AN_EXPERT * E and max(D, F_) <= ops.MOE_FEW_MAX_INNER
-        rows = ops.moe_tc05_tile_rows() if many else ops.moe_few_rows() if few else ops.moe_tile_rows(tc)
+        rows = (ops.moe_fp8_tile_rows(S, E) if self.held is not None else ops.moe_tc05_tile_rows() if many
+                else ops.moe_few_rows() if few else ops.moe_tile_rows(tc))
         max_tiles = ops.moe_max_tiles(S, E, rows)
         order = ctx.ws.flat("moe_sorted", S, torch.int32)
         tiles = ctx.ws.flat("moe_tiles", 3 * max_tiles + 1, torch.int32)
         n_tiles = tiles[3 * max_tiles:]
-        if self.table_vocab:
+        if planned:
+            scratch = ctx.ws.flat("moe_route_counts", ops.moe_route_scratch(T, EO), torch.int32)
+            ops.moe_route_plan(logits, ctx.token_req, top, sel_e[:S], sel_w[:S], rows, order[:S], tiles[:3 * max_tiles], n_tiles, scratch, ctx.stream,
+                               group_score=self.group_score, **router)
+        elif self.table_vocab:
             ops.label(self.name + ".plan", 0.0, 8.0 * T + 8.0 * S)
             ops.moe_plan_table(ctx.tokens, ctx.token_req, self.table, T, E, rows, order, tiles, n_tiles, ctx.status, ctx.stream)
         else:
             ops.moe_plan(sel_e, S, E, rows, order, tiles, n_tiles, ctx.stream)
+        if self.held is not None:
+            return self._experts_eight_bits(ctx, x, y, sel_w, (order[:S], tiles[:3 * max_tiles], n_tiles, max_tiles, rows), unit), sel_e, sel_w
         h = ctx.ws.get("moe_hidden", S, F_, x.dtype)
         es = x.element_size()
         if many:
@@ -251,6 +298,26 @@ class ExpertsMLP(FeedForward):
         ops.label(self.name + ".experts.out", 2.0 * S * D * F_, es * (min(E, S) * F_ * D + S * F_) + 4.0 * S * D)
         ops.moe_gemm(h, 1, self.w_out, D, order, tiles, n_tiles, max_tiles, rows, y, ctx.stream)
         return y, sel_e, sel_w
+
+    def _experts_eight_bits(self, ctx, x, y, sel_w, plan, unit):
+        """The experts' products with weights in 8 bits: the slots' rows by tiles of the plan, the gated unit rounded in the first product's epilogue."""
+        T, S, D, F_, (_, _, _, max_tiles, rows) = x.shape[0], plan[0].numel(), self.width, self.inner, plan
+
+        def room(tag, columns):
+            runs = (columns + 511) // 512
+            codes = ctx.ws.get(tag, max_tiles * rows, (columns + 15) // 16 * 16, torch.uint8).view(torch.float8_e4m3fn)
+            return codes, ctx.ws.get(tag + "_scales", max_tiles, runs * 512, torch.uint8).view(max_tiles, 1, runs, 512)
+
+        codes, hidden = room("moe_rows_fp8", D), room("moe_hidden_fp8", F_)
+        ops.label(self.name + ".gather", 0.0, x.element_size() * T * D + S * D)
+        ops.moe_gather_fp8(x, self.top, *plan, *codes, ctx.stream)
+        met = min(self.n_experts, S)
+        ops.label(self.name + ".experts.in", 4.0 * S * D * F_, met * 2 * F_ * D + S * D + S * F_)
+        ops.moe_gemm_fp8(*codes, *self.held[0], *plan, hidden[0], ctx.status, ctx.stream, sel_weight=None if sel_w is None else sel_w[:S], gated=True,
+                         out_scales=hidden[1], **unit)
+        ops.label(self.name + ".experts.out", 2.0 * S * D * F_, met * F_ * D + S * F_ + 4.0 * S * D)
+        ops.moe_gemm_fp8(*hidden, *self.held[1], *plan, y, ctx.status, ctx.stream)
+        return y
 
     def forward(self, ctx, x, residual):
         if self.table_vocab:

@@ -21,6 +21,13 @@ from .base import MATRIX, VECTOR, Init, Normed, ParamSpec, Part
 ACTIVATIONS = {None: ops.EPI_NONE, **ops.ACTIVATION_CODES}
 
 
+def fp8_rows(ctx, rows: int, columns: int):
+    """A step's memory for ``rows`` rows in 8-bit floating point (as ``ops.fp8_empty``)."""
+    codes = ctx.ws.get("fp8_codes", rows, (columns + 15) // 16 * 16, torch.uint8).view(torch.float8_e4m3fn)
+    tiles, runs = (rows + 127) // 128, (columns + 511) // 512
+    return codes, ctx.ws.get("fp8_scales", tiles, runs * 512, torch.uint8).view(1, tiles, runs, 512)
+
+
 class Linear(Part):
     replayable = True
     # (the few-rows kernel with a folded norm is a library of its own, named by the block that folds norms)
@@ -38,6 +45,7 @@ class Linear(Part):
         self.weight: Optional[torch.Tensor] = None
         self.bias: Optional[torch.Tensor] = None
         self.folded = None        # see fold_norm
+        self.held = None          # see hold_eight_bits: (codes, scales) in the place of ``weight``
 
     def param_specs(self) -> List[ParamSpec]:
         shape = (self.n_out, self.n_in) if self.stored == "out_in" else (self.n_in, self.n_out)
@@ -65,6 +73,8 @@ class Linear(Part):
         1/std, which the few-rows kernel finds from the fragments it loads anyway (csrc/gemm_smallm.cuh) and
         which for more rows come from a statistics kernel (``ops.row_stats``).  ``W'`` replaces ``W``: every
         step, of few rows or many, goes through the same weights and the same arithmetic."""
+        if self.in_eight_bits():
+            return False          # the rows are rounded to 8 bits behind the norm
         args = norm.fold_args()
         w = self.weight
         if args is None or w is None or w.dtype != torch.bfloat16 or self.n_in % 8 or self.folded is not None:
@@ -78,6 +88,36 @@ class Linear(Part):
         self.folded = SimpleNamespace(norm=norm, colsum=folded.float().sum(dim=1).contiguous(), eps=float(eps))
         self.weight, self.bias = folded, bias.contiguous()
         return True
+
+    # Whether the weight may be held in 8 bits: an option of the layer (a router's or a gate's small weight decides whole numbers or is read
+    # by other kernels), and from this many inputs and outputs on.
+    eight_bits = True
+    EIGHT_BITS_FROM = 128
+
+    def in_eight_bits(self) -> bool:
+        return bool(self.weight_bits == 8 and self.eight_bits and min(self.n_in, self.n_out) >= self.EIGHT_BITS_FROM)
+
+    def hold_eight_bits(self) -> int:
+        """The weight as e4m3 codes with a scale for each row and 128 columns (``ops.fp8_quantize``), which takes its place; steps then round their rows
+        the same way on the way in (``ops.linear_fp8``)."""
+        if not self.in_eight_bits() or self.weight is None:
+            return 0
+        w = self.weight
+        if w.dtype != torch.bfloat16:
+            raise ValueError(f"{self.name}: weights in 8 bits go with a bfloat16 run, not with {w.dtype}")
+        self.held = ops.fp8_empty(w.shape[0], w.shape[1], w.device)
+        ops.fp8_quantize(w, *self.held, ops.current_stream())
+        self.weight = None
+        return 1
+
+    def _forward_eight_bits(self, ctx, x, out, epi, residual) -> torch.Tensor:
+        M, K = x.shape
+        codes, scales = fp8_rows(ctx, M, K)
+        ops.label(self.name + ".rows", 0.0, (x.element_size() + 1.0) * M * K)
+        ops.fp8_quantize(x, codes, scales, ctx.stream)
+        ops.label(self.name, 2.0 * M * self.n_in * self.n_out, self.n_in * self.n_out + M * K + out.element_size() * M * self.n_out)
+        ops.linear_fp8(codes, scales, *self.held, self.bias, out, ctx.status, ctx.stream, epilogue=epi, residual=residual)
+        return out
 
     # From this many output features on, steps of 33 to 64 rows run on the tcgen05 kernel rather than on the
     # few-rows kernel (measured with a vocabulary-sized output: each of the few-rows kernel's many CTAs reads
@@ -113,6 +153,8 @@ class Linear(Part):
         rounding, so depends on its own request alone and never on how many others share the step.  ``step_rows=False``: the rows
         of ``x`` are not the step's (the wanted ones): the generic kernel."""
         epi = ACTIVATIONS[activation]
+        if self.held is not None:
+            return self._forward_eight_bits(ctx, x.tensor() if isinstance(x, Normed) else x, out, epi, residual)
         M = x.shape[0]
         few = self.few_rows(x.shape[0])      # decided once, before the fold's argument is made for that kernel
         fold = None

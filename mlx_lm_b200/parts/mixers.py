@@ -59,7 +59,7 @@ class Attention(Mixer):
         qkv = ctx.ws.get("qkv", T, self.q_width + 2 * self.kv_width, x.dtype)
         q = qkv[:, :self.q_width]
         src = x.source if isinstance(x, Normed) else x      # a Normed: the norm is folded into the projection
-        if (cache.write and cache.k_scale is None and self.position is None and x.dtype == torch.bfloat16 and self.width % 8 == 0
+        if (cache.write and cache.k_scale is None and self.position is None and self.qkv.held is None and x.dtype == torch.bfloat16 and self.width % 8 == 0
                 and src.stride(0) % 8 == 0 and src.data_ptr() % 16 == 0):
             # nothing to do to q and k before the cache: the projection's epilogue puts keys and values
             # into the pages itself

@@ -223,6 +223,8 @@ class ModelDescription:
         libs: List[str] = []
         for p in self.parts():
             libs.extend(p.all_kernel_libs())
+            if p.weight_bits:
+                libs.extend(("fp8_rows", "fp8_few", "fp8_many"))
         return list(dict.fromkeys(libs))
 
     def cache_specs(self) -> Dict[object, object]:
@@ -249,13 +251,24 @@ class Model:
     """A description bound to tensors on a device in one dtype."""
 
     def __init__(self, description: ModelDescription, tensors: Dict[str, torch.Tensor], dtype: torch.dtype,
-                 device):
+                 device, weight_bits: Optional[int] = None):
+        """``weight_bits=8``: the weights of linear layers and experts are held in 8-bit floating point, with a scale for each row and 128 columns
+        (embeddings, routers, norms and a tied output head stay as they are); bfloat16 runs only."""
+        if weight_bits not in (None, 8):
+            raise ValueError(f"weight_bits {weight_bits!r}: weights in the run's type (None) or in 8 bits")
+        if weight_bits and dtype != torch.bfloat16:
+            raise ValueError(f"weight_bits=8 goes with a bfloat16 run, not with {dtype}")
+        self.weight_bits = weight_bits
         self.description = description
         self.args = description.args
         self.model_type = description.model_type
         self.dtype, self.device = dtype, torch.device(device)
         for p in description.parts():
+            p.set_weight_bits(weight_bits)
+        for p in description.parts():
             p.bind_all(tensors, dtype, self.device)
+        if weight_bits and not sum(p.hold_eight_bits() for p in description.parts()):
+            raise ValueError("weight_bits=8: this model has no weight that is held in 8 bits (linear layers from 128 x 128 on, experts)")
 
     @property
     def layers(self):

@@ -374,6 +374,7 @@ class MLSTMMixer(Mixer):
                                                         (f"{name}.v", self.v_width), (f"{name}.g", self.v_width)], init=init)
         self.gates = FusedLinear(f"{name}.if", width, [(f"{name}.i", n_heads), (f"{name}.f", n_heads)], init=init,
                                  biases={f"{name}.{g}": f"{name}.{g}.b" for g in "if"}, bias_init=Init(0.0, 1.0))
+        self.gates.eight_bits = False        # read by ops.mlstm_gates_single as it is
         self.out = Linear(f"{name}.o", self.v_width, width, bias=False, weight_suffix="", init=Init(0.0, self.v_width ** -0.5))
         self.norm_w = None
 

@@ -95,8 +95,8 @@ def place(spec: ParamSpec, t: torch.Tensor, dtype: torch.dtype, device) -> torch
 
 
 def build_model(config: dict, tensors: Dict[str, torch.Tensor], dtype: torch.dtype = torch.bfloat16,
-                device="cuda", get_model_classes=None) -> Model:
-    """``get_model_classes(config) -> (builder, args class)`` replaces the registry lookup, as the parameter of
+                device="cuda", get_model_classes=None, weight_bits: Optional[int] = None) -> Model:
+    """``weight_bits=8``: large weights are held in 8-bit floating point (``parts.model.Model``).  ``get_model_classes(config) -> (builder, args class)`` replaces the registry lookup, as the parameter of
     the same name does in mlx-lm's ``load_model`` (mlx_lm/utils.py:296-301)."""
     if get_model_classes is not None:
         build, args_class = get_model_classes(config)
@@ -110,7 +110,7 @@ def build_model(config: dict, tensors: Dict[str, torch.Tensor], dtype: torch.dty
     got = check_tensors(description, tensors)
     specs = {s.name: s for s in description.param_specs()}
     placed = {n: place(specs[n], t, dtype, device) for n, t in got.items()}
-    return Model(description, placed, dtype, device)
+    return Model(description, placed, dtype, device, weight_bits=weight_bits)
 
 
 def parse_dtype(dtype) -> torch.dtype:
@@ -127,12 +127,12 @@ def parse_dtype(dtype) -> torch.dtype:
 
 
 def load_model(model_path: str, dtype="bfloat16", device="cuda", model_config: Optional[dict] = None,
-               get_model_classes=None) -> Tuple[Model, dict]:
+               get_model_classes=None, weight_bits: Optional[int] = None) -> Tuple[Model, dict]:
     """Model folder -> (model on the device, config dict)."""
     config = load_config(model_path)
     if model_config:
         config.update(model_config)
-    model = build_model(config, read_safetensors(model_path), parse_dtype(dtype), device, get_model_classes)
+    model = build_model(config, read_safetensors(model_path), parse_dtype(dtype), device, get_model_classes, weight_bits=weight_bits)
     config.setdefault("vocab_size", model.vocab_size)     # callers size their tokens by it, whatever the config calls it
     return model, config
 
