@@ -38,7 +38,7 @@ struct ManyArgs {
   int act;
   float limit;
 };
-struct ManyMaps { CUtensorMap x, w, xs, ws; };
+struct ManyMaps { CUtensorMap x, w, xs, ws, out; };      // out: of a linear layer whose rows begin on 16 bytes
 
 constexpr int MANY_EPI = 8, MANY_THREADS = 64 + 32 * MANY_EPI;
 
@@ -46,7 +46,7 @@ template <int BN, int CG>
 struct ManyShape {
   static constexpr int W_ROWS = BN / CG, W_TILES = BN / 128;
   static constexpr int STAGE = 16384 + W_ROWS * 128 + (1 + W_TILES) * FP8_TILE;
-  static constexpr int STAGES = (227 * 1024 - 2048 - MANY_EPI * 2048) / STAGE < 8 ? (227 * 1024 - 2048 - MANY_EPI * 2048) / STAGE : 8;
+  static constexpr int STAGES = (227 * 1024 - 3072 - MANY_EPI * 4096) / STAGE < 8 ? (227 * 1024 - 3072 - MANY_EPI * 4096) / STAGE : 8;
   static constexpr int SCALES = 4 + 4 * W_TILES;
   static constexpr int ACC = BN == 256 ? 1 : 2;
 };
@@ -58,7 +58,9 @@ struct ManySmem {
   alignas(1024) uint8_t w[S::STAGES][S::W_ROWS * 128];
   alignas(128) uint8_t xs[S::STAGES][FP8_TILE];
   alignas(128) uint8_t ws[S::STAGES][S::W_TILES * FP8_TILE];
-  alignas(16) uint4 stage[MANY_EPI][32 * 4];        // 64 bytes of results of each of a warp's rows on their way out
+  // 64 bytes of results of each of a warp's rows on their way out, two times; the 16-byte pieces lie as a copy with 64-byte swizzle wants them
+  alignas(1024) uint4 stage[MANY_EPI][2][32 * 4];
+  alignas(16) float bias[MANY_EPI][32];
   alignas(8) uint64_t full[S::STAGES];
   uint64_t empty[S::STAGES];
   uint64_t acc_full[2], acc_empty[2], drained;
@@ -72,6 +74,12 @@ template <int ACT, bool FAST, int N>
 __device__ __forceinline__ void activate_all(float (&v)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
+}
+
+// 32 rows of 64 bytes from shared memory to columns x .., rows y .. of a matrix; what lies outside it is left out
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 template <typename TO>
@@ -256,7 +264,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane;
-    uint4* stg = sm.stage[warp - 2];
+    uint4* stg = sm.stage[warp - 2][0];
+    int turn = 0;
     const int o_row = lane >> 2, o_piece = lane & 3;
     int it = 0;
     for (int t = first_tile; t < n_tiles; t += step, ++it) {
@@ -326,7 +335,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
         }
         // the other warp has the other half of the run's columns
         uint32_t* mine = reinterpret_cast<uint32_t*>(stg);
-        const uint32_t* other = reinterpret_cast<const uint32_t*>(sm.stage[(warp - 2) ^ 4]);
+        const uint32_t* other = reinterpret_cast<const uint32_t*>(sm.stage[(warp - 2) ^ 4][0]);
         const int at = (it & 1) * 32 + lane;
         mine[at] = top;
         asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
@@ -362,9 +371,9 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
           if (nc >= a.N) break;
           if (KIND == MANY_LINEAR) {
             if (a.bias != nullptr) {
-              reinterpret_cast<float*>(stg)[lane] = bias[c];
+              sm.bias[warp - 2][lane] = bias[c];
               __syncwarp();
-              const float4* bp = reinterpret_cast<const float4*>(stg);
+              const float4* bp = reinterpret_cast<const float4*>(sm.bias[warp - 2]);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const float4 x = bp[i];
@@ -402,18 +411,23 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             }
             continue;
           } else {
-          if (sizeof(TO) == 2 && res != nullptr && lane < rows) {       // added before the sum is rounded, by rows
+          if (KIND == MANY_LINEAR && res != nullptr && lane < rows) {       // added before the sum is rounded, by rows
             const TO* x = res + (long long)(m0 + lane) * a.ldo + nc;
             if (nc + 32 <= a.N) {
-              uint4 u[4];
+              uint4 u[32 / PER];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
+              for (int i = 0; i < 32 / PER; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float e[8];
-                unpack8(u[i], e);
+              for (int i = 0; i < 32 / PER; ++i) {
+                if constexpr (sizeof(TO) == 2) {
+                  float e[8];
+                  unpack8(u[i], e);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
+                  for (int j = 0; j < 8; ++j) v[8 * i + j] += e[j];
+                } else {
+                  v[4 * i] += __uint_as_float(u[i].x); v[4 * i + 1] += __uint_as_float(u[i].y);
+                  v[4 * i + 2] += __uint_as_float(u[i].z); v[4 * i + 3] += __uint_as_float(u[i].w);
+                }
               }
             } else {
 #pragma unroll
@@ -421,8 +435,18 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
                 if (nc + i < a.N) v[i] += to_f(x[i]);
             }
           }
+          if (KIND == MANY_LINEAR && (a.N & (PER - 1)) != 0 && nc + 32 > a.N && lane < rows) {      // the last columns, less than 16 bytes of them
 #pragma unroll
-          for (int p0 = 0; p0 < 32; p0 += 4 * PER) {          // 64 bytes of each row at a time, written four lanes a row
+            for (int i = 0; i < 32; ++i)
+              if (nc + i >= (a.N & ~(PER - 1)) && nc + i < a.N) out[(long long)(m0 + lane) * a.ldo + nc + i] = from_f<TO>(v[i]);
+          }
+#pragma unroll
+          for (int p0 = 0; p0 < 32; p0 += 4 * PER) {          // 64 bytes of each row at a time
+            uint4* box = stg + (turn & 1) * 128;
+            if (KIND == MANY_LINEAR) {
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // what was sent from this half two turns ago has been read
+              __syncwarp();
+            }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               uint4 u;
@@ -435,45 +459,31 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
                 const int i = (p0 + x * 4) & 31;
                 u = make_uint4(r[c][i], r[c][i + 1], r[c][i + 2], r[c][i + 3]);
               }
-              stg[many_stage(lane, x)] = u;
+              box[many_stage(lane, x)] = u;
             }
-            __syncwarp();
-            const int n = nc + p0 + o_piece * PER;
-            float4 add[4];
-            if (sizeof(TO) == 4 && res != nullptr) {
+            if (KIND == MANY_LINEAR) {            // one copy a box
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0 && rows > 0 && nc + p0 < (a.N & ~(PER - 1))) store_box(&maps.out, box, nc + p0, m0);
+              ++turn;
+            } else {                              // rows of slots, four lanes a row
+              __syncwarp();
+              const int n = nc + p0 + o_piece * PER;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int rr = 8 * j + o_row;
-                add[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (rr < rows && n < a.N) {
-                  const float* x = reinterpret_cast<const float*>(res) + (long long)(m0 + rr) * a.ldo + n;
-                  if (n + 4 <= a.N) {
-                    add[j] = *reinterpret_cast<const float4*>(x);
-                  } else {
-                    add[j].x = x[0];
-                    if (n + 1 < a.N) add[j].y = x[1];
-                    if (n + 2 < a.N) add[j].z = x[2];
-                  }
-                }
+                const uint4 u = box[many_stage(rr, o_piece)];
+                const int to = __shfl_sync(0xffffffffu, slot, rr);
+                if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
               }
+              __syncwarp();
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int rr = 8 * j + o_row;
-              uint4 u = stg[many_stage(rr, o_piece)];
-              const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
-              if (sizeof(TO) == 4 && res != nullptr) {
-                u.x = __float_as_uint(__uint_as_float(u.x) + add[j].x); u.y = __float_as_uint(__uint_as_float(u.y) + add[j].y);
-                u.z = __float_as_uint(__uint_as_float(u.z) + add[j].z); u.w = __float_as_uint(__uint_as_float(u.w) + add[j].w);
-              }
-              if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
-            }
-            __syncwarp();
           }
           }
         }
       }
     }
+    if (KIND == MANY_LINEAR && WHOLE && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   __syncwarp();
@@ -515,8 +525,26 @@ static int scales_map(CUtensorMap* map, const void* base, long long tiles, const
   return mlxb_fail(MLXB_BAD_ARG, "%s: cuTensorMapEncodeTiled(%lld tiles of scales): %s", what, tiles, msg ? msg : "?");
 }
 
+template <typename TO>
+static int out_map(CUtensorMap* map, const ManyArgs& a) {
+  const cuuint64_t dims[2] = {(cuuint64_t)(a.N & ~(16 / (int)sizeof(TO) - 1)), (cuuint64_t)a.M};     // a copy writes whole 16 bytes
+  const cuuint64_t strides[1] = {(cuuint64_t)a.ldo * sizeof(TO)};
+  const cuuint32_t box[2] = {64 / sizeof(TO), 32};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(map, sizeof(TO) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.out, dims, strides,
+                                            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return 0;
+  const char* msg = nullptr;
+  cuGetErrorString(r, &msg);
+  return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): cuTensorMapEncodeTiled(%d x %d results at stride %lld): %s", a.M, a.N, a.ldo, msg ? msg : "?");
+}
+
 template <int BN, int CG, int KIND, typename TO, bool WHOLE>
-static int many_launch_as(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
+static int many_launch_as(const ManyMaps& maps_in, const ManyArgs& a, cudaStream_t stream) {
+  ManyMaps maps = maps_in;
+  if (KIND == MANY_LINEAR && WHOLE)
+    if (int e = out_map<TO>(&maps.out, a)) return e;
   constexpr size_t smem = sizeof(ManySmem<BN, CG>) + 1024;
   static_assert(smem <= 227 * 1024, "stages and staging buffers fit a CTA's shared memory");
   auto kern = fp8_many_kernel<BN, CG, KIND, TO, WHOLE>;
@@ -550,7 +578,7 @@ static int many_launch_as(const ManyMaps& maps, const ManyArgs& a, cudaStream_t 
 
 template <int BN, int CG, int KIND, typename TO>
 static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t stream) {
-  if (KIND == MANY_GATED || !(((uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)(a.ldo * (long long)sizeof(TO))) & 15))
+  if (KIND == MANY_GATED || (a.N >= 8 && !(((uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)(a.ldo * (long long)sizeof(TO))) & 15)))
     return many_launch_as<BN, CG, KIND, TO, true>(maps, a, stream);
   if constexpr (KIND != MANY_GATED) return many_launch_as<BN, CG, KIND, TO, false>(maps, a, stream);
   return MLXB_BAD_ARG;
