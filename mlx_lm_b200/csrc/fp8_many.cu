@@ -6,10 +6,10 @@
 //
 // Operands are rows of codes with scales (fp8.cuh).  Persistent CTAs: warp 0 copies (TMA, 128-byte swizzle, a ring of stages of 128 of K;
 // the scales of 512 of K come with every fourth), warp 1 issues tcgen05.mma kind::mxf8f6f4 (scales by tcgen05.cp into one of four places
-// in turn), warps 2-9 are the epilogue: two a quadrant of the lanes, a lane a row, half of the columns each.
+// in turn), warps 2-17 are the epilogue: four a quadrant of the lanes, a lane a row, a quarter of the columns each.
 //
 // Tiles of 256 columns fill half of the tensor memory and scales want some of the rest, so there is one accumulator: the epilogue takes all of
-// its numbers into registers at once (128 a thread) and hands it back before it does anything with them.  That costs some 500 clocks a
+// its numbers into registers at once (64 a thread) and hands it back before it does anything with them.  That costs some 500 clocks a
 // tile; two accumulators of 128 columns would cost the main loop, whose products read shared memory 128 bytes a clock then.
 //
 // Pairs (CG = 2): two CTAs on a tile of 256 rows x BN columns; each brings its own rows of x, half of the rows of W and its own scales (of all BN
@@ -40,13 +40,13 @@ struct ManyArgs {
 };
 struct ManyMaps { CUtensorMap x, w, xs, ws, out; };      // out: of a linear layer whose rows begin on 16 bytes
 
-constexpr int MANY_EPI = 8, MANY_THREADS = 64 + 32 * MANY_EPI;
+constexpr int MANY_EPI = 16, MANY_THREADS = 64 + 32 * MANY_EPI;     // four warps a quadrant of the lanes, a quarter of the columns each
 
 template <int BN, int CG>
 struct ManyShape {
   static constexpr int W_ROWS = BN / CG, W_TILES = BN / 128;
   static constexpr int STAGE = 16384 + W_ROWS * 128 + (1 + W_TILES) * FP8_TILE;
-  static constexpr int STAGES = (227 * 1024 - 3072 - MANY_EPI * 4096) / STAGE < 8 ? (227 * 1024 - 3072 - MANY_EPI * 4096) / STAGE : 8;
+  static constexpr int STAGES = (227 * 1024 - 9216 - MANY_EPI * 2048) / STAGE < 8 ? (227 * 1024 - 9216 - MANY_EPI * 2048) / STAGE : 8;
   static constexpr int SCALES = 4 + 4 * W_TILES;
   static constexpr int ACC = BN == 256 ? 1 : 2;
 };
@@ -58,8 +58,10 @@ struct ManySmem {
   alignas(1024) uint8_t w[S::STAGES][S::W_ROWS * 128];
   alignas(128) uint8_t xs[S::STAGES][FP8_TILE];
   alignas(128) uint8_t ws[S::STAGES][S::W_TILES * FP8_TILE];
-  // 64 bytes of results of each of a warp's rows on their way out, two times; the 16-byte pieces lie as a copy with 64-byte swizzle wants them
-  alignas(1024) uint4 stage[MANY_EPI][2][32 * 4];
+  // results of a warp's 32 rows on their way out: two boxes of 32 bytes a row, whose 16-byte pieces lie as a copy with 32-byte swizzle wants them
+  // (linear layers), or 64 bytes a row
+  alignas(1024) uint4 stage[MANY_EPI][32 * 4];
+  uint32_t top[2][4][4][32];                       // gated: the largest magnitudes of a row's 32 columns, by quadrant and slice
   alignas(16) float bias[MANY_EPI][32];
   alignas(8) uint64_t full[S::STAGES];
   uint64_t empty[S::STAGES];
@@ -76,10 +78,9 @@ __device__ __forceinline__ void activate_all(float (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
 }
 
-// 32 rows of 64 bytes from shared memory to columns x .., rows y .. of a matrix; what lies outside it is left out
+// 32 rows of 32 bytes from shared memory to columns x .., rows y .. of a matrix; what lies outside it is left out
 __device__ __forceinline__ void store_box(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 template <typename TO>
@@ -100,7 +101,7 @@ template <int BN, int CG, int KIND, typename TO, bool WHOLE>
 __global__ void __launch_bounds__(MANY_THREADS)
 fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
   using S = ManyShape<BN, CG>;
-  constexpr int STAGES = S::STAGES, HALF = BN / 2;
+  constexpr int STAGES = S::STAGES, SLICE = BN / 4;
   extern __shared__ uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<ManySmem<BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -263,8 +264,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       }
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane;
-    uint4* stg = sm.stage[warp - 2][0];
+    const int q = warp & 3, slice = (warp - 2) >> 2, row = q * 32 + lane;
+    uint4* stg = sm.stage[warp - 2];
     int turn = 0;
     const int o_row = lane >> 2, o_piece = lane & 3;
     int it = 0;
@@ -272,8 +273,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       const int b = S::ACC == 2 ? it & 1 : 0;
       const Place p = place_of(t);
       // asked for while the products run: a plan's slots and their weights
-      constexpr int CHUNKS = HALF / 32;
-      const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = KIND == MANY_GATED ? p.n * 128 + half * 64 : p.n * BN + half * HALF;
+      constexpr int CHUNKS = SLICE / 32;
+      const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = KIND == MANY_GATED ? p.n * 128 + slice * 32 : p.n * BN + slice * SLICE;
       const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
       const TO* res = KIND == MANY_LINEAR ? reinterpret_cast<const TO*>(after_wait(a.residual)) : nullptr;
       int slot = 0;
@@ -283,9 +284,9 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
         if (KIND == MANY_GATED && sel_weight) wgt = sel_weight[slot];
       }
       bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag, peer_abort);
-      if (KIND == MANY_GATED) {             // the two warps of a quadrant meet below
+      if (KIND == MANY_GATED) {             // the four warps of a quadrant meet below
         uint32_t all;
-        asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred r, %2, 64, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
+        asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred r, %2, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
                      : "=r"(all) : "r"((uint32_t)ok), "r"(q + 1) : "memory");
         ok = all != 0;
       }
@@ -293,13 +294,9 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       fp8_after_sync();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN);
       uint32_t r[CHUNKS][32];
-      if (KIND == MANY_GATED) {             // 64 columns: gate, then up
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) tmem_ld32(acc + (uint32_t)((c >> 1) * 128 + half * 64 + (c & 1) * 32), r[c]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) tmem_ld32(acc + (uint32_t)(half * HALF + c * 32), r[c]);
-      }
+      for (int c = 0; c < CHUNKS; ++c)      // gated: 32 columns of gate, the same of up
+        tmem_ld32(acc + (uint32_t)(KIND == MANY_GATED ? c * 128 + slice * 32 : slice * SLICE + c * 32), r[c]);
       fp8_wait_ld();
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) fp8_arrived(r[c]);
@@ -313,50 +310,43 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
         auto units = [&](auto kind) {
           constexpr int KIND_OF = decltype(kind)::value;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              r[c][i] = __float_as_uint(fp8_gated_unit(KIND_OF, __uint_as_float(r[c][i]), __uint_as_float(r[2 + c][i]), wgt, a.limit));
-              if (n0 + 64 > a.N && n0 + 32 * c + i >= a.N) r[c][i] = 0u;
-              top = max(top, r[c][i] & 0x7fffffffu);
-            }
+          for (int i = 0; i < 32; ++i) {
+            r[0][i] = __float_as_uint(fp8_gated_unit(KIND_OF, __uint_as_float(r[0][i]), __uint_as_float(r[1][i]), wgt, a.limit));
+            if (n0 + 32 > a.N && n0 + i >= a.N) r[0][i] = 0u;
+            top = max(top, r[0][i] & 0x7fffffffu);
+          }
         };
         if (a.act == MLXB_GU_BOUNDED) units(std::integral_constant<int, MLXB_GU_BOUNDED>{});
         else units(std::integral_constant<int, MLXB_GU_SILU>{});
         if (top >= 0x7f800000u) {             // rare: something is not finite
           top = 0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              top = max(top, fp8_magnitude(__uint_as_float(r[c][i])));
-              r[c][i] = __float_as_uint(fp8_or_nan(__uint_as_float(r[c][i])));
-            }
+          for (int i = 0; i < 32; ++i) {
+            top = max(top, fp8_magnitude(__uint_as_float(r[0][i])));
+            r[0][i] = __float_as_uint(fp8_or_nan(__uint_as_float(r[0][i])));
+          }
         }
-        // the other warp has the other half of the run's columns
-        uint32_t* mine = reinterpret_cast<uint32_t*>(stg);
-        const uint32_t* other = reinterpret_cast<const uint32_t*>(sm.stage[(warp - 2) ^ 4][0]);
-        const int at = (it & 1) * 32 + lane;
-        mine[at] = top;
-        asm volatile("bar.sync %0, 64;" ::"r"(q + 1) : "memory");
-        const int e = fp8_exponent(max(top, other[at]));
+        // the other warps of the quadrant have the rest of the run's columns
+        sm.top[it & 1][q][slice][lane] = top;
+        asm volatile("bar.sync %0, 128;" ::"r"(q + 1) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, sm.top[it & 1][q][i][lane]);
+        const int e = fp8_exponent(top);
         const float f = fp8_power(-e);
         if (live) {
           uint8_t* o = reinterpret_cast<uint8_t*>(a.out) + ((long long)p.m * 128 + row) * a.ldo;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int g = 0; g < 2; ++g) {
+            uint32_t w[4];
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int j = 16 * g + 4 * i;
-                w[i] = fp8_quad(__uint_as_float(r[c][j]) * f, __uint_as_float(r[c][j + 1]) * f, __uint_as_float(r[c][j + 2]) * f, __uint_as_float(r[c][j + 3]) * f);
-              }
-              const int n = n0 + 32 * c + 16 * g;
-              if (n < a.ldo) *reinterpret_cast<uint4*>(o + n) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i) {
+              const int j = 16 * g + 4 * i;
+              w[i] = fp8_quad(__uint_as_float(r[0][j]) * f, __uint_as_float(r[0][j + 1]) * f, __uint_as_float(r[0][j + 2]) * f, __uint_as_float(r[0][j + 3]) * f);
             }
-          if (half == 0) a.out_scales[((long long)p.m * a.out_kgs + (p.n >> 2)) * FP8_TILE + fp8_scale_row(row) + (p.n & 3)] = (uint8_t)(e + 127);
+            const int n = n0 + 16 * g;
+            if (n < a.ldo) *reinterpret_cast<uint4*>(o + n) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (slice == 0) a.out_scales[((long long)p.m * a.out_kgs + (p.n >> 2)) * FP8_TILE + fp8_scale_row(row) + (p.n & 3)] = (uint8_t)(e + 127);
         }
       } else {
         constexpr int PER = 16 / sizeof(TO);
@@ -440,39 +430,42 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             for (int i = 0; i < 32; ++i)
               if (nc + i >= (a.N & ~(PER - 1)) && nc + i < a.N) out[(long long)(m0 + lane) * a.ldo + nc + i] = from_f<TO>(v[i]);
           }
+          auto piece = [&](int i) {                  // 16 bytes of results from this chunk's column i on
+            if (sizeof(TO) == 2) {
+              float w[8];
 #pragma unroll
-          for (int p0 = 0; p0 < 32; p0 += 4 * PER) {          // 64 bytes of each row at a time
-            uint4* box = stg + (turn & 1) * 128;
-            if (KIND == MANY_LINEAR) {
+              for (int j = 0; j < 8; ++j) w[j] = v[(i + j) & 31];
+              return pack8(w);
+            }
+            return make_uint4(r[c][i & 31], r[c][(i + 1) & 31], r[c][(i + 2) & 31], r[c][(i + 3) & 31]);
+          };
+          if constexpr (KIND == MANY_LINEAR) {
+#pragma unroll
+            for (int p0 = 0; p0 < 32; p0 += 2 * PER) {        // 32 bytes of each row a box, one copy a box
+              uint4* box = stg + (turn & 1) * 64;
               if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // what was sent from this half two turns ago has been read
               __syncwarp();
-            }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint4 u;
-              if (sizeof(TO) == 2) {
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = v[(x * 8 + i) & 31];
-                u = pack8(w);
-              } else {
-                const int i = (p0 + x * 4) & 31;
-                u = make_uint4(r[c][i], r[c][i + 1], r[c][i + 2], r[c][i + 3]);
-              }
-              box[many_stage(lane, x)] = u;
-            }
-            if (KIND == MANY_LINEAR) {            // one copy a box
+              for (int x = 0; x < 2; ++x) box[lane * 2 + (x ^ ((lane >> 2) & 1))] = piece(p0 + x * PER);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
-              if (lane == 0 && rows > 0 && nc + p0 < (a.N & ~(PER - 1))) store_box(&maps.out, box, nc + p0, m0);
+              if (lane == 0) {
+                if (rows > 0 && nc + p0 < (a.N & ~(PER - 1))) store_box(&maps.out, box, nc + p0, m0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");          // a box that is not sent counts too: the wait above goes by turns
+              }
               ++turn;
-            } else {                              // rows of slots, four lanes a row
+            }
+          } else {
+#pragma unroll
+            for (int p0 = 0; p0 < 32; p0 += 4 * PER) {        // rows of slots: 64 bytes of each at a time, four lanes a row
+#pragma unroll
+              for (int x = 0; x < 4; ++x) stg[many_stage(lane, x)] = piece(p0 + x * PER);
               __syncwarp();
               const int n = nc + p0 + o_piece * PER;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int rr = 8 * j + o_row;
-                const uint4 u = box[many_stage(rr, o_piece)];
+                const uint4 u = stg[many_stage(rr, o_piece)];
                 const int to = __shfl_sync(0xffffffffu, slot, rr);
                 if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
               }
@@ -529,10 +522,10 @@ template <typename TO>
 static int out_map(CUtensorMap* map, const ManyArgs& a) {
   const cuuint64_t dims[2] = {(cuuint64_t)(a.N & ~(16 / (int)sizeof(TO) - 1)), (cuuint64_t)a.M};     // a copy writes whole 16 bytes
   const cuuint64_t strides[1] = {(cuuint64_t)a.ldo * sizeof(TO)};
-  const cuuint32_t box[2] = {64 / sizeof(TO), 32};
+  const cuuint32_t box[2] = {32 / sizeof(TO), 32};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = cuTensorMapEncodeTiled(map, sizeof(TO) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.out, dims, strides,
-                                            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return 0;
   const char* msg = nullptr;
@@ -588,7 +581,7 @@ static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t str
 // results), every run of 128 of K, every further wave of tiles.
 struct ManyForm { int bn, cg; };
 struct ManyCost { int bn, cg; double launch, run, wave; };      // microseconds
-static constexpr ManyCost MANY_FORMS[] = {{256, 2, 8.2, .294, 3.6}, {256, 1, 6.2, .398, 1.4}, {128, 2, 5.4, .235, .9}, {128, 1, 4.5, .273, .65}};
+static constexpr ManyCost MANY_FORMS[] = {{256, 2, 6.4, .297, 2.2}, {256, 1, 5.2, .442, .9}, {128, 2, 5., .245, .5}, {128, 1, 4.2, .272, .6}};
 static ManyForm many_form(int M, int N, int K) {
   const char *want_pair = getenv("MLXB_FP8_PAIR"), *want_bn = getenv("MLXB_FP8_BN");     // experiments and tests
   const int sms = mlxb_sm_count(), runs = (K + 127) / 128;
