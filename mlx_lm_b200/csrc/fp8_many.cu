@@ -42,27 +42,29 @@ struct ManyMaps { CUtensorMap x, w, xs, ws, out; };      // out: of a linear lay
 
 constexpr int MANY_EPI = 16, MANY_THREADS = 64 + 32 * MANY_EPI;     // four warps a quadrant of the lanes, a quarter of the columns each
 
-template <int BN, int CG>
+template <int BN, int CG, int KIND>
 struct ManyShape {
   static constexpr int W_ROWS = BN / CG, W_TILES = BN / 128;
   static constexpr int STAGE = 16384 + W_ROWS * 128 + (1 + W_TILES) * FP8_TILE;
-  static constexpr int STAGES = (227 * 1024 - 9216 - MANY_EPI * 2048) / STAGE < 8 ? (227 * 1024 - 9216 - MANY_EPI * 2048) / STAGE : 8;
+  // for results on their way out: two boxes a warp, one, or none (the gated unit's leave as they are)
+  static constexpr int OUT = KIND == MANY_LINEAR ? 2048 : KIND == MANY_EXPERTS ? 1024 : 16;
+  static constexpr int ROOM = 227 * 1024 - 4096 - (KIND == MANY_GATED ? 4096 : 2048) - MANY_EPI * OUT;
+  static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
   static constexpr int SCALES = 4 + 4 * W_TILES;
   static constexpr int ACC = BN == 256 ? 1 : 2;
 };
 
-template <int BN, int CG>
+template <int BN, int CG, int KIND>
 struct ManySmem {
-  using S = ManyShape<BN, CG>;
+  using S = ManyShape<BN, CG, KIND>;
   alignas(1024) uint8_t x[S::STAGES][16384];
   alignas(1024) uint8_t w[S::STAGES][S::W_ROWS * 128];
   alignas(128) uint8_t xs[S::STAGES][FP8_TILE];
   alignas(128) uint8_t ws[S::STAGES][S::W_TILES * FP8_TILE];
-  // results of a warp's 32 rows on their way out: two boxes of 32 bytes a row, whose 16-byte pieces lie as a copy with 32-byte swizzle wants them
-  // (linear layers), or 64 bytes a row
-  alignas(1024) uint4 stage[MANY_EPI][32 * 4];
-  uint32_t top[2][4][4][32];                       // gated: the largest magnitudes of a row's 32 columns, by quadrant and slice
-  alignas(16) float bias[MANY_EPI][32];
+  // results of a warp's 32 rows on their way out: boxes of 32 bytes a row, whose 16-byte pieces lie as a copy with 32-byte swizzle wants them
+  alignas(1024) uint4 stage[MANY_EPI][S::OUT / 16];
+  uint32_t top[KIND == MANY_GATED ? 2 : 1][4][4][32];        // gated: the largest magnitudes of a row's 32 columns, by quadrant and slice
+  alignas(16) float bias[KIND == MANY_LINEAR ? MANY_EPI : 1][32];
   alignas(8) uint64_t full[S::STAGES];
   uint64_t empty[S::STAGES];
   uint64_t acc_full[2], acc_empty[2], drained;
@@ -70,7 +72,7 @@ struct ManySmem {
   int abort_flag;
 };
 
-__device__ __forceinline__ int many_stage(int row, int piece) { return row * 4 + (piece ^ ((row >> 1) & 3)); }
+__device__ __forceinline__ int many_stage(int row, int piece) { return row * 2 + (piece ^ ((row >> 2) & 1)); }
 
 template <int ACT, bool FAST, int N>
 __device__ __forceinline__ void activate_all(float (&v)[N]) {
@@ -100,10 +102,10 @@ __device__ __forceinline__ void store_whole(uint4 u, int n, int N, TO* row) {
 template <int BN, int CG, int KIND, typename TO, bool WHOLE>
 __global__ void __launch_bounds__(MANY_THREADS)
 fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
-  using S = ManyShape<BN, CG>;
+  using S = ManyShape<BN, CG, KIND>;
   constexpr int STAGES = S::STAGES, SLICE = BN / 4;
   extern __shared__ uint8_t smem_raw[];
-  auto& sm = *reinterpret_cast<ManySmem<BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  auto& sm = *reinterpret_cast<ManySmem<BN, CG, KIND>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)cluster_rank() : 0;
   const bool leader = rank == 0;
@@ -267,7 +269,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
     const int q = warp & 3, slice = (warp - 2) >> 2, row = q * 32 + lane;
     uint4* stg = sm.stage[warp - 2];
     int turn = 0;
-    const int o_row = lane >> 2, o_piece = lane & 3;
+    const int o_row = lane >> 1, o_piece = lane & 1;
     int it = 0;
     for (int t = first_tile; t < n_tiles; t += step, ++it) {
       const int b = S::ACC == 2 ? it & 1 : 0;
@@ -379,20 +381,21 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               default: break;
             }
           }
-          if constexpr (!WHOLE) {         // rows that do not begin on 16 bytes: 16 columns at a time through shared memory in float32, two rows an instruction
+          if constexpr (!WHOLE) {         // rows that do not begin on 16 bytes: a few columns at a time through shared memory in float32
+            constexpr int COLS = S::OUT / 128, STEP = 32 / COLS;         // 16 or 8 columns, 2 or 4 rows an instruction
             float* f = reinterpret_cast<float*>(stg);
 #pragma unroll
-            for (int p0 = 0; p0 < 32; p0 += 16) {
+            for (int p0 = 0; p0 < 32; p0 += COLS) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) f[lane * 16 + ((i + 2 * lane) & 15)] = v[p0 + i];
+              for (int i = 0; i < COLS; ++i) f[lane * COLS + ((i + 2 * lane) & (COLS - 1))] = v[p0 + i];
               __syncwarp();
-              const int col = lane & 15, n = nc + p0 + col;
+              const int col = lane & (COLS - 1), n = nc + p0 + col;
 #pragma unroll 4
-              for (int rr = lane >> 4; rr < 32; rr += 2) {
+              for (int rr = lane / COLS; rr < 32; rr += STEP) {
                 const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
                 if (rr < rows && n < a.N) {
                   const long long at = (long long)to * a.ldo + n;
-                  float y = f[rr * 16 + ((col + 2 * rr) & 15)];
+                  float y = f[rr * COLS + ((col + 2 * rr) & (COLS - 1))];
                   if (res != nullptr) y += to_f(res[at]);
                   out[at] = from_f<TO>(y);
                 }
@@ -446,7 +449,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // what was sent from this half two turns ago has been read
               __syncwarp();
 #pragma unroll
-              for (int x = 0; x < 2; ++x) box[lane * 2 + (x ^ ((lane >> 2) & 1))] = piece(p0 + x * PER);
+              for (int x = 0; x < 2; ++x) box[many_stage(lane, x)] = piece(p0 + x * PER);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
               if (lane == 0) {
@@ -457,14 +460,14 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             }
           } else {
 #pragma unroll
-            for (int p0 = 0; p0 < 32; p0 += 4 * PER) {        // rows of slots: 64 bytes of each at a time, four lanes a row
+            for (int p0 = 0; p0 < 32; p0 += 2 * PER) {        // rows of slots: 32 bytes of each at a time, two lanes a row
 #pragma unroll
-              for (int x = 0; x < 4; ++x) stg[many_stage(lane, x)] = piece(p0 + x * PER);
+              for (int x = 0; x < 2; ++x) stg[many_stage(lane, x)] = piece(p0 + x * PER);
               __syncwarp();
               const int n = nc + p0 + o_piece * PER;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int rr = 8 * j + o_row;
+              for (int j = 0; j < 2; ++j) {
+                const int rr = 16 * j + o_row;
                 const uint4 u = stg[many_stage(rr, o_piece)];
                 const int to = __shfl_sync(0xffffffffu, slot, rr);
                 if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
@@ -538,7 +541,7 @@ static int many_launch_as(const ManyMaps& maps_in, const ManyArgs& a, cudaStream
   ManyMaps maps = maps_in;
   if (KIND == MANY_LINEAR && WHOLE)
     if (int e = out_map<TO>(&maps.out, a)) return e;
-  constexpr size_t smem = sizeof(ManySmem<BN, CG>) + 1024;
+  constexpr size_t smem = sizeof(ManySmem<BN, CG, KIND>) + 1024;
   static_assert(smem <= 227 * 1024, "stages and staging buffers fit a CTA's shared memory");
   auto kern = fp8_many_kernel<BN, CG, KIND, TO, WHOLE>;
   static SharedLimit limit;
