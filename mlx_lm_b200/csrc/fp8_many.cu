@@ -46,8 +46,8 @@ template <int BN, int CG, int KIND>
 struct ManyShape {
   static constexpr int W_ROWS = BN / CG, W_TILES = BN / 128;
   static constexpr int STAGE = 16384 + W_ROWS * 128 + (1 + W_TILES) * FP8_TILE;
-  // for results on their way out: two boxes a warp, one, or none (the gated unit's leave as they are)
-  static constexpr int OUT = KIND == MANY_LINEAR ? 2048 : KIND == MANY_EXPERTS ? 1024 : 16;
+  // for results on their way out: a box a warp, or none (the gated unit's leave as they are)
+  static constexpr int OUT = KIND == MANY_GATED ? 16 : 1024;
   static constexpr int ROOM = 227 * 1024 - 4096 - (KIND == MANY_GATED ? 4096 : 2048) - MANY_EPI * OUT;
   static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
   static constexpr int SCALES = 4 + 4 * W_TILES;
@@ -445,8 +445,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
           if constexpr (KIND == MANY_LINEAR) {
 #pragma unroll
             for (int p0 = 0; p0 < 32; p0 += 2 * PER) {        // 32 bytes of each row a box, one copy a box
-              uint4* box = stg + (turn & 1) * 64;
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // what was sent from this half two turns ago has been read
+              uint4* box = stg;
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // what was sent from here has been read
               __syncwarp();
 #pragma unroll
               for (int x = 0; x < 2; ++x) box[many_stage(lane, x)] = piece(p0 + x * PER);

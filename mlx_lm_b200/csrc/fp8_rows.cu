@@ -92,7 +92,7 @@ __device__ __forceinline__ void quantize512(const Sixteen<T>& x, bool in, uint8_
 
 // AT items of a warp have their loads out together: one where a call is a chain of latencies, four where it is bytes.
 template <typename T, bool VEC, int AT>
-__global__ void __launch_bounds__(32 * FQ_WARPS)
+__global__ void __launch_bounds__(32 * FQ_WARPS, AT == 1 ? 8 : VEC ? (sizeof(T) == 2 ? 4 : 2) : 2)
 fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
   pdl_wait();
   pdl_trigger();
@@ -127,10 +127,10 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
 
 // A warp takes up to two of a tile's rows at a time: their slots are looked up together, and so are the rows' pieces.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * FQ_WARPS)
+__global__ void __launch_bounds__(32 * FQ_WARPS, VEC && sizeof(T) == 2 ? 7 : 4)
 fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted, const int* tile_info, const int* n_tiles, int tile_rows,
                   uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
-  constexpr int AT = 2;
+  constexpr int AT = 1;
   pdl_wait();
   pdl_trigger();
   x = after_wait(x);
