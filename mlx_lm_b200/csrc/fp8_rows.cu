@@ -45,14 +45,15 @@ struct Sixteen {
   // the bits (of a float32) of the largest magnitude, not finite ones too
   __device__ __forceinline__ uint32_t largest() const {
     uint32_t top = 0;
-    if (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i] & 0x7fff7fffu));
       return max(top << 16, top & 0xffff0000u);
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, w[i] & 0x7fffffffu);
-    return top;
+      for (int i = 0; i < 16; ++i) top = max(top, w[i] & 0x7fffffffu);
+      return top;
+    }
   }
 };
 
@@ -95,7 +96,7 @@ template <typename T, bool VEC, int AT>
 __global__ void __launch_bounds__(32 * FQ_WARPS, AT == 1 ? 8 : VEC ? (sizeof(T) == 2 ? 4 : 2) : 2)
 fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
   pdl_wait();
-  pdl_trigger();
+  if (AT == 1) pdl_trigger();       // many rows: the next kernel's CTAs would take the registers this one runs in
   x = after_wait(x);
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, tiles = (group_rows + 127) >> 7;
   const long long items = (long long)rows * kgs, first = ((long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5)) * AT;
@@ -125,46 +126,31 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
   }
 }
 
-// A warp takes up to two of a tile's rows at a time: their slots are looked up together, and so are the rows' pieces.
+// A warp takes a row of a tile (where there are few, a part of its columns).  Blocks are short so that the last ones to run are few: with four
+// rows a warp 32768 rows of 2048 took 37 us, 1.1 rounds of blocks over the SMs being two.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * FQ_WARPS, VEC && sizeof(T) == 2 ? 7 : 4)
+__global__ void __launch_bounds__(32 * FQ_WARPS, VEC && sizeof(T) == 2 ? 6 : 4)
 fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted, const int* tile_info, const int* n_tiles, int tile_rows,
-                  uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
-  constexpr int AT = 1;
+                  uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales, bool few) {
   pdl_wait();
-  pdl_trigger();
+  if (few) pdl_trigger();           // many rows: the next kernel's CTAs would take the registers this one runs in
   x = after_wait(x);
   sorted = after_wait(sorted);
   tile_info = after_wait(tile_info);
   const int t = blockIdx.x, have = after_wait(n_tiles)[0], first = tile_info[3 * t + 1], rows = tile_info[3 * t + 2];
   if (t >= have) return;
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, warps = gridDim.y * FQ_WARPS, warp = blockIdx.y * FQ_WARPS + (threadIdx.x >> 5);
-  // few rows: a warp takes one of them, or a part of its columns
-  const int parts = max(1, min(kgs, warps / rows)), row_warps = warps / parts;
-  if (warp >= row_warps * parts) return;
-  const int part = warp / row_warps;
-  for (int i = warp - part * row_warps; i < rows; i += AT * row_warps) {
-    const T* px[AT];
-    uint8_t *pc[AT], *ps[AT];
-#pragma unroll
-    for (int j = 0; j < AT; ++j) {
-      const int r = i + j * row_warps;
-      px[j] = r < rows ? x + (long long)(sorted[first + r] / a_div) * ldx : nullptr;
-      pc[j] = codes + ((long long)t * tile_rows + r) * ld + 512 * part + 16 * lane;
-      ps[j] = scales + ((long long)t * kgs + part) * FP8_TILE + fp8_scale_row(r);
-    }
+  const int parts = max(1, min(kgs, warps / rows)), row_warps = warps / parts, part = warp / row_warps;
+  if (part >= parts) return;
+  for (int r = warp - part * row_warps; r < rows; r += row_warps) {
+    const T* px = x + (long long)(sorted[first + r] / a_div) * ldx;
+    uint8_t* pc = codes + ((long long)t * tile_rows + r) * ld;
+    uint8_t* ps = scales + (long long)t * kgs * FP8_TILE + fp8_scale_row(r);
     for (int kg = part; kg < kgs; kg += parts) {
       const int c = 512 * kg + 16 * lane;
-      Sixteen<T> v[AT];
-#pragma unroll
-      for (int j = 0; j < AT; ++j)
-        if (px[j]) v[j].template load<VEC>(px[j], c, K);
-#pragma unroll
-      for (int j = 0; j < AT; ++j) {
-        if (px[j]) quantize512<T>(v[j], c < ld, pc[j], ps[j], lane);
-        pc[j] += 512 * parts;
-        ps[j] += FP8_TILE * parts;
-      }
+      Sixteen<T> v;
+      v.template load<VEC>(px, c, K);
+      quantize512<T>(v, c < ld, pc + c, ps + kg * FP8_TILE, lane);
     }
   }
 }
@@ -243,11 +229,11 @@ MLXB_EXPORT int mlxb_fp8_gather(const GatherRecord* rec, long long bytes, cudaSt
   if (max_tiles <= 0) return 0;
   if (int e = check("moe_gather_fp8", x, K, ldx, codes, ld, scales)) return e;
   if (a_div <= 0 || tile_rows <= 0 || tile_rows > 128) return mlxb_fail(MLXB_BAD_ARG, "moe_gather_fp8: tiles of %d rows", tile_rows);
-  // a tile's rows over a few blocks: four rows a warp where there are tiles enough for that, else more blocks
-  const dim3 grid(max_tiles, max_tiles >= 2 * mlxb_sm_count() ? max(1, tile_rows / (4 * FQ_WARPS)) : max(1, tile_rows / FQ_WARPS));
+  const dim3 grid(max_tiles, max(1, tile_rows / FQ_WARPS));
+  const bool few = (long long)grid.x * grid.y <= 4LL * mlxb_sm_count();
 #define GO(T, V)                                                                                                                             \
   launch_pdl(fp8_gather_kernel<T, V>, grid, dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, K, a_div, sorted, tile_info, n_tiles, tile_rows, \
-             (uint8_t*)codes, ld, (uint8_t*)scales)
+             (uint8_t*)codes, ld, (uint8_t*)scales, few)
   if (dtype == MLXB_BF16) {
     if (whole_pieces<__nv_bfloat16>(x, ldx, K)) GO(__nv_bfloat16, true);
     else GO(__nv_bfloat16, false);
