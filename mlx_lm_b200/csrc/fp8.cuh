@@ -136,7 +136,7 @@ struct Fp8ExpertsRecord {
   const float* sel_weight;
   void *out, *out_scales;
   int* status;
-  long long gated, out_f32, E, N, K, max_tiles, at_most, tile_rows, ldo, act;
+  long long gated, out_f32, E, N, K, S, max_tiles, at_most, tile_rows, ldo, act;
   double limit;
 };
 
@@ -150,7 +150,7 @@ static inline int fp8_check(const char* what, const void* x, const void* xs, con
 }
 static inline int fp8_check_experts(const Fp8ExpertsRecord& r) {
   if (int e = fp8_check("moe_gemm_fp8", r.x, r.xs, r.w, r.ws, r.out, r.max_tiles * r.tile_rows, r.N, r.K, r.ldo)) return e;
-  if (r.E <= 0 || r.E * r.N * 2 > 0x7fffffffLL || !r.sorted || !r.tile_info || !r.n_tiles || !r.status ||
+  if (r.E <= 0 || r.S <= 0 || r.S > 0x7fffffffLL || r.E * r.N * 2 > 0x7fffffffLL || !r.sorted || !r.tile_info || !r.n_tiles || !r.status ||
       (r.gated && (!r.out_scales || r.ldo != ((r.N + 15) & ~15LL) || ((uintptr_t)r.out & 15))))
     return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld experts of %lld x %lld, results at stride %lld", r.E, r.N, r.K, r.ldo);
   return 0;

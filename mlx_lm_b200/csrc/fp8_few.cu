@@ -39,7 +39,7 @@ struct FewArgs {
   void* out;
   long long ldo;
   uint8_t* out_scales;
-  int out_kgs, max_items;
+  int out_kgs, max_items, E, S;        // E, S: experts and slots, a plan's numbers are held to them
   int* status;
   int act;                             // activation, or kind of gated unit
   float limit;
@@ -142,9 +142,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   };
 
   pdl_trigger();
-  // A linear layer's weights come from no kernel of the stream: the first stages' are asked for before the wait.
+  // A linear layer's first weights are asked for before the wait.  What could write them right before this kernel is fp8_quantize, which lets
+  // the next kernel start early only where it has up to 128 rows: more rows of W than that are complete by now.
   int early = 0;
-  if (KIND == FEW_LINEAR && first_item < a.max_items) early = min(STAGES, k1 - k0);
+  if (KIND == FEW_LINEAR && a.N > 128 && first_item < a.max_items) early = min(STAGES, k1 - k0);
   if (threadIdx.x == 0)
     for (int s = 0; s < early; ++s) {
       mbar_expect_tx(&sm.full[s], stage_bytes(k0 + s));
@@ -162,7 +163,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     bool ok = true;
     for (int w = first_item; w < items && ok; w += step) {
       const int tile = w / a.w_tiles, nb = w - tile * a.w_tiles;
-      const int group = KIND == FEW_LINEAR ? 0 : tile_info[3 * tile] * NH;
+      const int group = KIND == FEW_LINEAR ? 0 : max(0, min(a.E - 1, tile_info[3 * tile])) * NH;
       for (int k = k0; k < k1; ++k) {
         if (issued < early) {
           if (elect_one()) load_x(s, k, tile);
@@ -236,14 +237,18 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   struct Beside { int slot; float weight, bias, residual[CH]; };
   auto fetch = [&](int w, int tok0, int live) {
     Beside x;
-    x.slot = 0;
+    x.slot = -1;
     x.weight = 1.f;
     x.bias = 0.f;
     const int tile = w / a.w_tiles, n = (w - tile * a.w_tiles) * 128 + in_tile;
     if (KIND != FEW_LINEAR) {
-      if (tok0 + lane < live) {
-        x.slot = sorted[tile_info[3 * tile + 1] + tok0 + lane];
-        if (KIND == FEW_GATED && sel_weight) x.weight = sel_weight[x.slot];
+      const int place = tile_info[3 * tile + 1] + tok0 + lane;
+      if (tok0 + lane < live && place >= 0 && place < a.S) {
+        const int slot = sorted[place];
+        if (slot >= 0 && slot < a.S) {
+          x.slot = slot;
+          if (KIND == FEW_GATED && sel_weight) x.weight = sel_weight[slot];
+        }
       }
     } else if (n < a.N) {
       if (a.bias) x.bias = a.bias[n];
@@ -302,7 +307,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
         const long long row = KIND == FEW_LINEAR ? j : __shfl_sync(0xffffffffu, x.slot, j);
-        if (tok0 + j < live && n < a.N) out[row * a.ldo] = from_f<TO>(v[j]);
+        if (tok0 + j < live && n < a.N && row >= 0) out[row * a.ldo] = from_f<TO>(v[j]);
       }
     }
   };
@@ -368,8 +373,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp >= 2 && first_item < items) x = fetch(first_item, rank * share, min(live_of(first_item), (rank + 1) * share));
     __syncwarp();
     if (warp < 2) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0 && sm.abort_flag)           // who gave up has sent nothing: nobody adds anything up
+      for (int r = 0; r < ranks; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(&sm.abort_flag, (uint32_t)r)), "r"(1) : "memory");
+    __syncwarp();
     cluster_sync();                      // all sums have arrived
-    if (warp >= 2 && first_item < items) {
+    if (warp >= 2 && first_item < items && !*abort_flag) {
       const int live = live_of(first_item);
 #pragma unroll 1
       for (int c = 0; c < share; c += CH) {
@@ -524,7 +533,7 @@ MLXB_EXPORT int mlxb_fp8_experts_few(const Fp8ExpertsRecord* rec, long long byte
   a.N = N; a.runs = (K + 127) / 128; a.kgs = (K + 511) / 512; a.w_tiles = (N + 127) / 128;
   a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
   a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
-  a.limit = (float)r.limit;
+  a.limit = (float)r.limit; a.E = (int)r.E; a.S = (int)r.S;
   const long long items = min(r.max_tiles, r.at_most) * a.w_tiles;
   if (items > 0x7fffff) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
   a.max_items = (int)items;

@@ -33,7 +33,7 @@ struct ManyArgs {
   void* out;
   long long ldo;
   uint8_t* out_scales;
-  int out_kgs;
+  int out_kgs, E, S;                           // E, S: experts and slots, a plan's numbers are held to them
   int* status;
   int act;
   float limit;
@@ -200,7 +200,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
     bool ok = true;
     for (int t = first_tile; t < n_tiles && ok; t += step) {
       const Place p = place_of(t);
-      const int m0 = p.m * (CG * 128) + rank * 128, expert = KIND == MANY_LINEAR ? 0 : tile_info[3 * p.m];
+      const int m0 = p.m * (CG * 128) + rank * 128, expert = KIND == MANY_LINEAR ? 0 : max(0, min(a.E - 1, tile_info[3 * p.m]));
       for (int k = 0; k < a.runs; ++k) {
         if (issued >= STAGES) {
           ok = mbar_wait_warp(&sm.empty[s], ph ^ 1, abort_flag, peer_abort);
@@ -279,11 +279,13 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
       const int m0 = KIND == MANY_LINEAR ? p.m * (CG * 128) + rank * 128 + q * 32 : 0, n0 = KIND == MANY_GATED ? p.n * 128 + slice * 32 : p.n * BN + slice * SLICE;
       const int rows = KIND == MANY_LINEAR ? a.M - m0 : tile_info[3 * p.m + 2] - q * 32;      // of this warp's 32, those that exist
       const TO* res = KIND == MANY_LINEAR ? reinterpret_cast<const TO*>(after_wait(a.residual)) : nullptr;
-      int slot = 0;
+      int slot = -1;
       float wgt = 1.f;
       if (KIND != MANY_LINEAR && lane < rows) {
-        slot = sorted[tile_info[3 * p.m + 1] + row];
-        if (KIND == MANY_GATED && sel_weight) wgt = sel_weight[slot];
+        const int place = tile_info[3 * p.m + 1] + row;
+        if (place >= 0 && place < a.S) slot = sorted[place];
+        if (slot < 0 || slot >= a.S) slot = -1;
+        else if (KIND == MANY_GATED && sel_weight) wgt = sel_weight[slot];
       }
       bool ok = mbar_wait(&sm.acc_full[b], (uint32_t)((S::ACC == 2 ? it >> 1 : it) & 1), abort_flag, peer_abort);
       if (KIND == MANY_GATED) {             // the four warps of a quadrant meet below
@@ -393,7 +395,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
 #pragma unroll 4
               for (int rr = lane / COLS; rr < 32; rr += STEP) {
                 const int to = KIND == MANY_EXPERTS ? __shfl_sync(0xffffffffu, slot, rr) : m0 + rr;
-                if (rr < rows && n < a.N) {
+                if (rr < rows && n < a.N && to >= 0) {
                   const long long at = (long long)to * a.ldo + n;
                   float y = f[rr * COLS + ((col + 2 * rr) & (COLS - 1))];
                   if (res != nullptr) y += to_f(res[at]);
@@ -470,7 +472,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
                 const int rr = 16 * j + o_row;
                 const uint4 u = stg[many_stage(rr, o_piece)];
                 const int to = __shfl_sync(0xffffffffu, slot, rr);
-                if (rr < rows && n < a.N) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
+                if (rr < rows && n < a.N && to >= 0) store_whole<TO>(u, n, a.N, out + (long long)to * a.ldo);
               }
               __syncwarp();
             }
@@ -645,7 +647,7 @@ MLXB_EXPORT int mlxb_fp8_experts_many(const Fp8ExpertsRecord* rec, long long byt
   a.tiles_m = (int)min(r.max_tiles, r.at_most); a.tiles_n = r.gated ? a.w_tiles : (N + bn - 1) / bn;
   a.sorted = r.sorted; a.tile_info = r.tile_info; a.n_tiles = r.n_tiles; a.sel_weight = r.sel_weight;
   a.out = r.out; a.ldo = r.ldo; a.out_scales = (uint8_t*)r.out_scales; a.out_kgs = (N + 511) / 512; a.status = r.status; a.act = (int)r.act;
-  a.limit = (float)r.limit;
+  a.limit = (float)r.limit; a.E = (int)r.E; a.S = (int)r.S;
   if ((long long)a.tiles_m * a.tiles_n > 0x3fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: %lld tiles of %d outputs", r.max_tiles, N);
   const long long stack = r.E * (r.gated ? 2 : 1);
   ManyMaps maps;

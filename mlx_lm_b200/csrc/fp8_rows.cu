@@ -96,7 +96,9 @@ template <typename T, bool VEC, int AT>
 __global__ void __launch_bounds__(32 * FQ_WARPS, AT == 1 ? 8 : VEC ? (sizeof(T) == 2 ? 4 : 2) : 2)
 fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
   pdl_wait();
-  if (AT == 1) pdl_trigger();       // many rows: the next kernel's CTAs would take the registers this one runs in
+  // The next kernel starts early behind few rows only.  Behind many its CTAs would take the registers this one runs in (8192 x 8192: 75 us instead of 40), and a
+  // kernel that reads weights before its own wait may count on it that a weight's more than 128 rows are complete by then.
+  if (AT == 1 && rows <= 128) pdl_trigger();
   x = after_wait(x);
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, tiles = (group_rows + 127) >> 7;
   const long long items = (long long)rows * kgs, first = ((long long)blockIdx.x * FQ_WARPS + (threadIdx.x >> 5)) * AT;
@@ -131,19 +133,21 @@ fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * FQ_WARPS, VEC && sizeof(T) == 2 ? 6 : 4)
 fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted, const int* tile_info, const int* n_tiles, int tile_rows,
-                  uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales, bool few) {
+                  uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales, int S, bool few) {
   pdl_wait();
   if (few) pdl_trigger();           // many rows: the next kernel's CTAs would take the registers this one runs in
   x = after_wait(x);
   sorted = after_wait(sorted);
   tile_info = after_wait(tile_info);
-  const int t = blockIdx.x, have = after_wait(n_tiles)[0], first = tile_info[3 * t + 1], rows = tile_info[3 * t + 2];
-  if (t >= have) return;
+  const int t = blockIdx.x, have = after_wait(n_tiles)[0], first = tile_info[3 * t + 1], rows = min(tile_rows, tile_info[3 * t + 2]);
+  if (t >= have || rows <= 0) return;
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, warps = gridDim.y * FQ_WARPS, warp = blockIdx.y * FQ_WARPS + (threadIdx.x >> 5);
   const int parts = max(1, min(kgs, warps / rows)), row_warps = warps / parts, part = warp / row_warps;
   if (part >= parts) return;
   for (int r = warp - part * row_warps; r < rows; r += row_warps) {
-    const T* px = x + (long long)(sorted[first + r] / a_div) * ldx;
+    const int place = first + r, slot = place >= 0 && place < S ? sorted[place] : -1;
+    if (slot < 0 || slot >= S) continue;             // no plan says so
+    const T* px = x + (long long)(slot / a_div) * ldx;
     uint8_t* pc = codes + ((long long)t * tile_rows + r) * ld;
     uint8_t* ps = scales + (long long)t * kgs * FP8_TILE + fp8_scale_row(r);
     for (int kg = part; kg < kgs; kg += parts) {
@@ -176,7 +180,7 @@ struct GatherRecord {
   const void* x;
   const int *sorted, *tile_info, *n_tiles;
   void *codes, *scales;
-  long long dtype, ldx, K, a_div, max_tiles, tile_rows, ld;
+  long long dtype, ldx, K, a_div, S, max_tiles, tile_rows, ld;
 };
 
 // x: `dtype` [rows, K] at row stride ldx; codes [rows, ld] with ld = K rounded up to 16; scales as in fp8.cuh for groups of group_rows rows.
@@ -220,11 +224,11 @@ MLXB_EXPORT int mlxb_fp8_quantize(const QuantizeRecord* rec, long long bytes, cu
 // codes; scales are a group a tile.  Rows of a tile behind its last slot are left as they were.
 MLXB_EXPORT int mlxb_fp8_gather(const GatherRecord* rec, long long bytes, cudaStream_t stream) {
   if (!rec || bytes != sizeof(GatherRecord)) return mlxb_fail(MLXB_BAD_ARG, "moe_gather_fp8: a record of %lld bytes", bytes);
-  if (rec->K > 0x7fffff00LL || rec->max_tiles > 0x7fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gather_fp8: rows of %lld, %lld tiles", rec->K, rec->max_tiles);
+  if (rec->K > 0x7fffff00LL || rec->max_tiles > 0x7fffffffLL || rec->S > 0x7fffffffLL) return mlxb_fail(MLXB_BAD_ARG, "moe_gather_fp8: rows of %lld, %lld tiles", rec->K, rec->max_tiles);
   const void* x = rec->x;
   const int *sorted = rec->sorted, *tile_info = rec->tile_info, *n_tiles = rec->n_tiles;
   void *codes = rec->codes, *scales = rec->scales;
-  const int dtype = (int)rec->dtype, K = (int)rec->K, a_div = (int)rec->a_div, max_tiles = (int)rec->max_tiles, tile_rows = (int)rec->tile_rows, ld = (int)rec->ld;
+  const int dtype = (int)rec->dtype, K = (int)rec->K, a_div = (int)rec->a_div, S = (int)rec->S, max_tiles = (int)rec->max_tiles, tile_rows = (int)rec->tile_rows, ld = (int)rec->ld;
   const long long ldx = rec->ldx;
   if (max_tiles <= 0) return 0;
   if (int e = check("moe_gather_fp8", x, K, ldx, codes, ld, scales)) return e;
@@ -233,7 +237,7 @@ MLXB_EXPORT int mlxb_fp8_gather(const GatherRecord* rec, long long bytes, cudaSt
   const bool few = (long long)grid.x * grid.y <= 4LL * mlxb_sm_count();
 #define GO(T, V)                                                                                                                             \
   launch_pdl(fp8_gather_kernel<T, V>, grid, dim3(32 * FQ_WARPS), 0, stream, (const T*)x, ldx, K, a_div, sorted, tile_info, n_tiles, tile_rows, \
-             (uint8_t*)codes, ld, (uint8_t*)scales, few)
+             (uint8_t*)codes, ld, (uint8_t*)scales, S, few)
   if (dtype == MLXB_BF16) {
     if (whole_pieces<__nv_bfloat16>(x, ldx, K)) GO(__nv_bfloat16, true);
     else GO(__nv_bfloat16, false);

@@ -511,15 +511,15 @@ MLXB_EXPORT int mlxb_moe_route_plan(const RouteRecord* rec, long long bytes, cud
   const RouteRecord& r = *rec;
   const long long T = r.T, E = r.E, top = r.top, groups = r.groups, keep = r.keep, n_real = r.n_real, tile_rows = r.tile_rows, max_tiles = r.max_tiles;
   const long long ldl = r.ldl;
+  if (T == 0 && r.n_tiles) {
+    const cudaError_t e = cudaMemsetAsync(r.n_tiles, 0, sizeof(int), stream);
+    return e == cudaSuccess ? 0 : mlxb_fail((int)e, "moe_route_plan: %s", cudaGetErrorString(e));
+  }
   if (!r.logits || !r.sel || !r.weight || !r.counts || !r.sorted || !r.tile_info || !r.n_tiles || max_tiles > 0x7fffffffLL || tile_rows > 0x7fffffffLL || T < 0 || E <= 0 || E > 1024 || top <= 0 || top > E || top > 64 || ldl < E || groups < 1 || groups > 128 || E % groups || keep < 1 || keep > groups ||
       n_real < 1 || n_real > E || top > keep * (E / groups) || tile_rows < 1 || (long long)T * top > 0x7ffffff0LL ||
       max_tiles < ((long long)T * top + tile_rows - 1) / tile_rows + n_real)
     return mlxb_fail(MLXB_BAD_ARG, "moe_route_plan: %lld tokens, %lld of %lld experts (%lld with tensors; up to 64 of 1024), %lld of %lld groups (up to 128), tiles of %lld rows, room for %lld",
                      T, top, E, n_real, keep, groups, tile_rows, max_tiles);
-  if (T == 0) {
-    const cudaError_t e = cudaMemsetAsync(r.n_tiles, 0, sizeof(int), stream);
-    return e == cudaSuccess ? 0 : mlxb_fail((int)e, "moe_route_plan: %s", cudaGetErrorString(e));
-  }
   int part = 0, shift = -1;
   for (int i = 0; i < 20; ++i)
     if (tile_rows == 1 << i) shift = i;

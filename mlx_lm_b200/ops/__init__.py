@@ -2522,7 +2522,12 @@ def _fp8_rows(t, what: str):
     shape, strides = t.shape, t.stride()
     if len(shape) != 2 or (strides[1] != 1 and shape[1] != 1) or (t.dtype is not _BF16T and t.dtype is not _F32T):
         raise KernelError(f"{what}: {t.dtype} {tuple(shape)} strides {strides}: float32 or bfloat16 rows, each contiguous")
-    return shape[0], shape[1], max(strides[0], shape[1])
+    rows, columns = shape
+    if strides[0] < columns:
+        if rows > 1:
+            raise KernelError(f"{what}: {t.dtype} {tuple(shape)} strides {strides}: rows that overlap")
+        return rows, columns, columns
+    return rows, columns, strides[0]
 
 
 def _fp8_vector(t, dtype, n: int, what: str) -> None:
@@ -2607,7 +2612,7 @@ def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, 
     return sorted_slots.numel()
 
 
-_fp8_gather_record = _kv8_record("6Q7q")
+_fp8_gather_record = _kv8_record("6Q8q")
 
 
 def moe_gather_fp8(x, a_div: int, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, codes, scales, stream) -> None:
@@ -2619,13 +2624,15 @@ def moe_gather_fp8(x, a_div: int, sorted_slots, tile_info, n_tiles, max_tiles: i
     _, width, groups = _fp8_codes(codes, scales, tile_rows, "moe_gather_fp8")
     if groups < max_tiles or width != (K + 15) & ~15 or a_div <= 0 or S > T * a_div:
         raise KernelError(f"moe_gather_fp8: x {tuple(x.shape)}, {S} slots, {a_div} a row, codes {tuple(codes.shape)} for {max_tiles} tiles")
+    if S == 0:
+        return
     _fp8_device("moe_gather_fp8", x, sorted_slots, tile_info, n_tiles, codes, scales)
     _call("fp8_rows", "mlxb_fp8_gather", _FP8_ARGS, *_fp8_gather_record(
         x.data_ptr(), sorted_slots.data_ptr(), tile_info.data_ptr(), n_tiles.data_ptr(), codes.data_ptr(), scales.data_ptr(), _DT[x.dtype], ldx, K,
-        a_div, max_tiles, tile_rows, width), stream)
+        a_div, S, max_tiles, tile_rows, width), stream)
 
 
-_fp8_experts_record = _kv8_record("11Q10qd")
+_fp8_experts_record = _kv8_record("11Q11qd")
 
 
 def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, out, status, stream,
@@ -2659,13 +2666,15 @@ def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_ti
         rows, columns, ldo = _fp8_rows(out, "moe_gemm_fp8 out")
         if rows < S or columns != n_out:
             raise KernelError(f"moe_gemm_fp8: {S} rows of {n_out} into {tuple(out.shape)}")
+    if S == 0:
+        return
     _fp8_device("moe_gemm_fp8", codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_tiles, out, status, out_scales if gated else None,
                 sel_weight if gated else None)
     lib, fn = ("fp8_many", "mlxb_fp8_experts_many") if tile_rows == 128 else ("fp8_few", "mlxb_fp8_experts_few")
     _call(lib, fn, _FP8_ARGS, *_fp8_experts_record(
         codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), sorted_slots.data_ptr(), tile_info.data_ptr(),
         n_tiles.data_ptr(), wp, out.data_ptr(), op, status.data_ptr(), gated, not gated and out.dtype is _F32T, w_groups // 2 if gated else w_groups,
-        n_out, K, groups, min(max_tiles, S), tile_rows, ldo, GATED_UNITS[unit] if gated else 0, limit), stream)
+        n_out, K, S, groups, min(max_tiles, S), tile_rows, ldo, GATED_UNITS[unit] if gated else 0, limit), stream)
 
 
 # --------------------------------------------------------------------------

@@ -255,3 +255,227 @@ def test_experts_of_one_and_of_nobody(tile_rows):
     check_experts(60, 2, 5, 256, 128, tile_rows, sel=[3] * 120)
     check_experts(60, 2, 5, 256, 128, tile_rows, sel=[-1] * 119 + [4])
     check_experts(60, 2, 5, 256, 128, tile_rows, sel=[-1] * 120)
+
+
+# ------------------------------------------------------------------------------------------------ how they are used
+
+def test_a_row_that_is_not_finite_keeps_to_itself():
+    o = ops()
+    for M in (20, 300):
+        x = normal((M, 400), 1, torch.bfloat16)
+        x[3, 17], x[5, 399], x[9, 0] = math.nan, math.inf, -math.inf
+        w = normal((260, 400), 2, torch.bfloat16) * 0.05
+        out, st = torch.zeros((M, 260), dtype=torch.bfloat16, device="cuda"), status()
+        o.linear_fp8(*kept(x), *kept(w), None, out, st, o.current_stream())
+        bad = torch.isnan(out).all(1)
+        assert bad.nonzero().view(-1).tolist() == [3, 5, 9] and torch.isfinite(out[~bad]).all()
+
+
+@pytest.mark.parametrize("tile_rows", [16, 128])
+def test_a_slot_that_is_not_finite_keeps_to_itself(tile_rows):
+    o = ops()
+    T, E, D, F = 30, 2, 256, 200
+    x = normal((T, D), 1, torch.bfloat16)
+    x[4, 100], x[7] = math.inf, math.nan
+    wi, wo = kept(normal((E * 2 * F, D), 2, torch.bfloat16) * 0.06, F), kept(normal((E * D, F), 3, torch.bfloat16) * 0.06, D)
+    plan = planned([i % 2 for i in range(T)], E, tile_rows)
+    codes, scales = o.fp8_empty(tile_rows, D, "cuda", groups=plan[3])
+    hc, hs = o.fp8_empty(tile_rows, F, "cuda", groups=plan[3])
+    out, st, stream = torch.zeros((T, D), device="cuda"), status(), o.current_stream()
+    o.moe_gather_fp8(x, 1, *plan, codes, scales, stream)
+    o.moe_gemm_fp8(codes, scales, *wi, *plan, hc, st, stream, gated=True, out_scales=hs)
+    o.moe_gemm_fp8(hc, hs, *wo, *plan, out, st, stream)
+    bad = torch.isnan(out).any(1)
+    assert bad.nonzero().view(-1).tolist() == [4, 7]
+
+
+def test_weights_quantised_right_before_they_are_read():
+    """The product right behind fp8_quantize of its own weights, again and again on other ones: never the ones before."""
+    o = ops()
+    for N in (100, 128, 129, 1000):
+        x = normal((4, 2048), 1, torch.bfloat16)
+        w = [normal((N, 2048), 2 + i, torch.bfloat16) for i in range(4)]
+        want = [ref.values(x) @ ref.values(m).T for m in w]
+        xc, (wc, ws) = kept(x), o.fp8_empty(N, 2048, "cuda")
+        outs, st = [torch.zeros((4, N), device="cuda") for _ in w], status()
+        torch.cuda.synchronize()
+        for m, out in zip(w * 5, outs * 5):
+            o.fp8_quantize(m, wc, ws, o.current_stream())
+            o.linear_fp8(*xc, wc, ws, None, out, st, o.current_stream())
+        for out, y in zip(outs, want):
+            assert float((out.double() - y).abs().max()) <= 1e-3 * float(y.abs().max())
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_captured_and_replayed(M):
+    """A graph of both calls, replayed on other rows; beside it another graph with rows of its own."""
+    o = ops()
+    w, st = kept(normal((500, 640), 9, torch.bfloat16) * 0.04), status()
+    wv = ref.values(normal((500, 640), 9, torch.bfloat16) * 0.04)
+    sets = []
+    for i in range(2):
+        x, out = normal((M, 640), i, torch.bfloat16), torch.zeros((M, 500), device="cuda")
+        codes, scales = o.fp8_empty(M, 640, "cuda")
+        def step(x=x, out=out, codes=codes, scales=scales):
+            o.fp8_quantize(x, codes, scales, o.current_stream())
+            o.linear_fp8(codes, scales, *w, None, out, st, o.current_stream())
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        sets.append((x, out, graph))
+    for turn in range(3):
+        for i, (x, out, graph) in enumerate(sets):
+            x.copy_(normal((M, 640), 50 + 2 * turn + i, torch.bfloat16))
+        streams = [torch.cuda.Stream() for _ in sets]
+        torch.cuda.synchronize()
+        for s, (_, _, graph) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, out, _ in sets:
+            y = ref.values(x) @ wv.T
+            assert float((out.double() - y).abs().max()) <= 1e-4 * float(y.abs().max())
+    assert int(st) == 0
+
+
+def test_the_whole_feed_forward_captured():
+    """Router, gather and both products in one graph, replayed on other tokens: the choices, and rows of a plain computation."""
+    o = ops()
+    T, E, top, D, F = 40, 16, 3, 256, 200
+    S = T * top
+    w_in, w_out = normal((E * 2 * F, D), 1, torch.bfloat16) * D ** -0.5, normal((E * D, F), 2, torch.bfloat16) * F ** -0.5
+    wi, wo = kept(w_in, F), kept(w_out, D)
+    rows = o.moe_fp8_tile_rows(S, E)
+    most = o.moe_max_tiles(S, E, rows)
+    i = dict(dtype=torch.int32, device="cuda")
+    x, logits = torch.zeros((T, D), dtype=torch.bfloat16, device="cuda"), torch.zeros((T, E), device="cuda")
+    sel, weight, order, tiles, n = torch.zeros(S, **i), torch.zeros(S, device="cuda"), torch.zeros(S, **i), torch.zeros((most, 3), **i), torch.zeros(1, **i)
+    scratch, st, out = torch.zeros(o.moe_route_scratch(T, E), **i), status(), torch.zeros((S, D), device="cuda")
+    (c, s), (hc, hs) = o.fp8_empty(rows, D, "cuda", groups=most), o.fp8_empty(rows, F, "cuda", groups=most)
+
+    def step():
+        stream, plan = o.current_stream(), (order, tiles, n, most, rows)
+        o.moe_route_plan(logits, None, top, sel, weight, rows, order, tiles, n, scratch, stream, score="softmax", renormalize=True)
+        o.moe_gather_fp8(x, top, *plan, c, s, stream)
+        o.moe_gemm_fp8(c, s, *wi, *plan, hc, st, stream, sel_weight=weight, gated=True, out_scales=hs)
+        o.moe_gemm_fp8(hc, hs, *wo, *plan, out, st, stream)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    wiv, wov = ref.values(w_in).view(E, 2, F, D), ref.values(w_out).view(E, D, F)
+    for turn in range(3):
+        x.copy_(normal((T, D), 10 + turn, torch.bfloat16))
+        logits.copy_(normal((T, E), 20 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, w = ref.route(logits.cpu(), [True] * T, top, score="softmax", renormalize=True)
+        assert sel.tolist() == [e for row in want for e in row]
+        xv = ref.values(x)
+        for t in range(T):
+            for k, e in enumerate(want[t]):
+                h = ref.values(ref.unit("silu", xv[t:t + 1] @ wiv[e, 0].T, xv[t:t + 1] @ wiv[e, 1].T, w[t][k], 0.0).float())
+                y = (h @ wov[e].T)[0]
+                # a hidden number that falls on the other side of a border of codes is 2^-3 of itself off, one of 200
+                assert float((out[t * top + k].double() - y).norm() / y.norm()) <= 1e-2
+    assert int(st) == 0
+
+
+def test_nothing_to_do():
+    o = ops()
+    st, stream = status(), o.current_stream()
+    i = dict(dtype=torch.int32, device="cuda")
+    w = kept(normal((64, 128), 1, torch.bfloat16))
+    empty = torch.zeros((0, 128), dtype=torch.bfloat16, device="cuda")
+    some = o.fp8_empty(16, 128, "cuda", groups=4)
+    o.fp8_quantize(empty, *some, stream)
+    o.linear_fp8(*some, *w, None, torch.zeros((0, 64), device="cuda"), st, stream)
+    none, tiles, n = torch.zeros(0, **i), torch.full((4, 3), -1, **i), torch.full((1,), 9, **i)
+    o.moe_route_plan(torch.zeros((0, 4), device="cuda"), None, 2, none, torch.zeros(0, device="cuda"), 16, none, tiles, n, torch.zeros(1, **i), stream)
+    assert int(n) == 0 and (tiles == -1).all()
+    o.moe_gather_fp8(empty, 2, none, tiles, n, 4, 16, *some, stream)
+    o.moe_gemm_fp8(*some, *kept(normal((4 * 32, 128), 1, torch.bfloat16), 32), none, tiles, n, 4, 16, torch.zeros((0, 32), device="cuda"), st, stream)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+
+
+def test_a_plan_with_numbers_out_of_range_reaches_nothing():
+    """Places, slots and experts that do not exist, and a tile longer than tiles are: left out or held to what there is, on the host's word for sizes."""
+    o = ops()
+    E, D, F, S = 3, 128, 96, 20
+    i = dict(dtype=torch.int32, device="cuda")
+    x = normal((S, D), 1, torch.bfloat16)
+    wi, wo = kept(normal((E * 2 * F, D), 2, torch.bfloat16), F), kept(normal((E * D, F), 3, torch.bfloat16), D)
+    for rows in (16, 128):
+        most = 5
+        order = torch.tensor([0, 1, -5, 10 ** 9] + list(range(4, S)), **i)
+        tiles = torch.tensor([[0, 0, 4], [99, 4, 3], [-7, 7, 3], [1, 15, 2000], [2, 10 ** 9, 4]], **i)
+        n = torch.tensor([5], **i)
+        (c, s), (hc, hs) = o.fp8_empty(rows, D, "cuda", groups=most), o.fp8_empty(rows, F, "cuda", groups=most)
+        out, st, stream = torch.full((S, D), 5.0, device="cuda"), status(), o.current_stream()
+        plan = (order, tiles, n, most, rows)
+        o.moe_gather_fp8(x, 1, *plan, c, s, stream)
+        o.moe_gemm_fp8(c, s, *wi, *plan, hc, st, stream, sel_weight=torch.ones(S, device="cuda"), gated=True, out_scales=hs)
+        o.moe_gemm_fp8(hc, hs, *wo, *plan, out, st, stream)
+        torch.cuda.synchronize()
+        assert (out[2:4] == 5.0).all() and not (out[:2] == 5.0).all(1).any()
+        assert torch.isfinite(out).all() and int(st) == 0
+
+
+def test_codes_beyond_2_31_bytes():
+    """More codes than 32 bits count, the last rows among those that are looked at."""
+    o = ops()
+    N, K = 70000, 32768
+    codes, scales = o.fp8_empty(N, K, "cuda")
+    w = torch.empty((N, K), dtype=torch.bfloat16, device="cuda")
+    for a in range(0, N, 10000):
+        w[a:a + 10000].normal_(generator=torch.Generator(device="cuda").manual_seed(a))
+    o.fp8_quantize(w, codes, scales, o.current_stream())
+    at = torch.tensor([0, 1, 65535, 65536, 65537, N - 129, N - 1], device="cuda")
+    few = ref.values(w[at])
+    del w
+    for M in (3, 200):
+        x = normal((M, K), 1, torch.bfloat16)
+        out, st = torch.zeros((M, N), device="cuda"), status()
+        o.linear_fp8(*kept(x), codes, scales, None, out, st, o.current_stream())
+        y = ref.values(x) @ few.T
+        assert float((out[:, at].double() - y).abs().max()) <= 1e-4 * float(y.abs().max())
+        assert int(st) == 0
+
+
+@pytest.mark.parametrize("name,M,N,K", [("fp8_few", 5, 40000, 512), ("fp8_few", 5, 512, 2048), ("fp8_many", 300, 300, 512), ("fp8_many", 100, 300, 512)])
+def test_a_wait_that_runs_out(name, M, N, K):
+    """An arrival that never comes (left out by the test's build): the kernel comes back by itself, says so and has written nothing; the next launch is right."""
+    from ctypes import c_int
+
+    from mlx_lm_b200.ops import build
+
+    o = ops()
+    lib_name = name + ":MLXB_TEST_WAIT_TIMEOUT=1"
+    lib = build.load(lib_name)
+    lib.mlxb_test_withhold_arrival.argtypes, lib.mlxb_test_withhold_arrival.restype = [c_int], c_int
+    x, w = normal((M, K), 1, torch.bfloat16), normal((N, K), 2, torch.bfloat16) * 0.05
+    (xc, xs), (wc, ws) = kept(x), kept(w)
+    out, st = torch.zeros((M, N), device="cuda"), status()
+
+    def launch():
+        o._call(lib_name, "mlxb_fp8_linear_few" if name == "fp8_few" else "mlxb_fp8_linear_many", o._FP8_ARGS, *o._fp8_linear_record(
+            xc.data_ptr(), xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), 0, 0, out.data_ptr(), st.data_ptr(), True, M, N, K, N, 0), o.current_stream())
+        torch.cuda.synchronize()
+
+    assert lib.mlxb_test_withhold_arrival(1) == 0
+    try:
+        launch()
+        assert int(st) == o.ST_WAIT_TIMEOUT
+        if N < 40000:                      # more tiles than CTAs: only each one's first is lost
+            assert not out.any()
+    finally:
+        assert lib.mlxb_test_withhold_arrival(0) == 0
+    st.zero_()
+    launch()
+    y = ref.values(x) @ ref.values(w).T
+    assert int(st) == 0 and float((out.double() - y).abs().max()) <= 1e-4 * float(y.abs().max())

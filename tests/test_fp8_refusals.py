@@ -23,6 +23,7 @@ def test_memory_of_a_matrix():
     (torch.zeros(20, 200, dtype=torch.float16), pair(), {}),
     (torch.zeros(20), pair(), {}),
     (torch.zeros(200, 20).t(), pair(), {}),
+    (torch.zeros(1, 200).expand(20, 200), pair(), {}),
     (torch.zeros(21, 200), pair(), {}),
     (torch.zeros(20, 210), pair(), {}),
     (torch.zeros(20, 200), pair(20, 700), {}),

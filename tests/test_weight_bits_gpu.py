@@ -212,8 +212,7 @@ def test_a_model_without_such_weights_is_refused(tmp_path):
 
 # ------------------------------------------------------------------------------------------------ groups judged by two
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("bits", [None, 8])
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, None), (torch.float32, None), (torch.bfloat16, 8)])
 @pytest.mark.parametrize("T", [3, 200])
 def test_experts_in_groups_judged_by_two(dtype, bits, T):
     """A feed-forward of experts with such a router in bfloat16, float32 and 8 bits, its parts by hand."""
@@ -223,8 +222,6 @@ def test_experts_in_groups_judged_by_two(dtype, bits, T):
     from mlx_lm_b200.engine.step import Workspace
     from mlx_lm_b200.parts.feed_forward import ExpertsMLP
 
-    if bits and dtype == torch.float32:
-        pytest.skip("8 bits go with bfloat16")
     D, F, E, top = 160, 136, 16, 3
     part = ExpertsMLP("ff", D, F, E, top, score="sigmoid", renormalize=True, correction=True, groups=(4, 2), group_score="two", weight_scale=1.5)
     part.set_weight_bits(bits)
