@@ -34,7 +34,7 @@ struct RouterArgs {
   float eps, factor;
   int* sel;
   float* weight;
-  int* counts;                 // [blocks][n_real] slots by expert of each block of tokens
+  int* counts;                 // [blocks][n_real rounded up to 4] slots by expert of each block of tokens
   int tokens_a_block, tile_rows, tile_shift, max_tiles;       // tile_shift: -1 where tile_rows is no power of two
   int *sorted, *tile_info, *n_tiles;
 };
@@ -137,6 +137,27 @@ __device__ __noinline__ void choose_exactly(const RouterArgs& a, const float* z,
     }
   }
   __syncwarp();
+}
+
+// What the choice of expert e goes by, in 64 bits.
+__device__ __forceinline__ double exact_sigmoid(const RouterArgs& a, const float* z, int e) {
+  return 1. / (1. + exp(-(double)z[e])) + (a.correction ? (double)a.correction[e] : 0.);
+}
+// The two largest of a group's, added up, in 64 bits by the whole warp; numbers out of the race are minus infinity.
+__device__ __noinline__ double exact_two(const RouterArgs& a, const float* z, int first, int per, int lane) {
+  double b1 = -INFINITY, b2 = -INFINITY;
+  for (int i = lane; i < per; i += 32) {
+    double v = exact_sigmoid(a, z, first + i);
+    v = v == v ? v : -INFINITY;
+    if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) { b2 = v; }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double o1 = __shfl_xor_sync(0xffffffffu, b1, o), o2 = __shfl_xor_sync(0xffffffffu, b2, o);
+    b2 = fmax(fmax(b2, o2), fmin(b1, o1));
+    b1 = fmax(b1, o1);
+  }
+  return a.two && b2 > -INFINITY ? b1 + b2 : b1;
 }
 
 // Descending, by a network of comparisons (odd-even merging).
@@ -249,7 +270,20 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
       // the worst that stays against the best that goes
       const uint32_t worst = __reduce_min_sync(0xffffffffu, stays ? order_of(score) : ~0u);
       const uint32_t best = __reduce_max_sync(0xffffffffu, mine && !stays ? order_of(score) : 0u);
-      if (best && worst != ~0u && near(number_of(worst), number_of(best), !a.correction && !a.two)) close = true;
+      const bool by_score = a.correction || a.two;
+      if (best && worst != ~0u && near(number_of(worst), number_of(best), !by_score)) {
+        // one on either side: formed again in 64 bits; more than that, the whole token
+        const uint32_t here = __ballot_sync(0xffffffffu, j == 0 && stays && order_of(score) == worst), there = __ballot_sync(0xffffffffu, j == 0 && mine && !stays && order_of(score) == best);
+        const bool other = j == 0 && mine && !(here >> lane & 1) && !(there >> lane & 1) &&
+                           (stays ? near(score, number_of(best), !by_score) : near(number_of(worst), score, !by_score));
+        if (a.softmax || !by_score || __popc(here) != 1 || __popc(there) != 1 || __any_sync(0xffffffffu, other)) {
+          close = true;
+        } else {
+          const int la = __ffs(here) - 1, lb = __ffs(there) - 1, ga = la / a.part, gb = lb / a.part;
+          const double x = exact_two(a, z, ga * per, per, lane), y = exact_two(a, z, gb * per, per, lane);
+          if (y > x || (y == x && gb < ga)) kept = (kept & ~(1u << la)) | 1u << lb;
+        }
+      }
       __syncwarp();
     }
   }
@@ -265,25 +299,41 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
   }
   sort_down(key);
   uint32_t last = 0;
+  int last_e = -1;
+  bool again = false;
   for (int c = 0; c <= a.top; ++c) {                        // one more than are chosen: was the last choice close?
     const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
-    if (c > 0 && best && near(number_of(last), number_of(best), !a.correction)) { close = true; break; }
-    if (c == a.top) break;
-    last = best;
     if (!best) {
       for (int x = c + lane; x < a.top; x += 32) sPick[x] = -1;
       break;
     }
     const int l = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-    if (lane == l) {
-      int at = 0;
+    int at = 0;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) at = was[i] == best ? i : at;     // two equal ones are close
-      sPick[c] = e0 + at;
+    for (int i = 0; i < VPT; ++i) at = was[i] == best ? i : at;       // two equal ones are close
+    int e = __shfl_sync(0xffffffffu, e0 + at, l);
+    if (c > 0 && near(number_of(last), number_of(best), !a.correction)) {
+      // two that are close, and none beside them: lane 0 has the one before, the others this one
+      if (a.softmax || again || e == last_e || !a.correction) { close = true; break; }
+      again = true;
+      const double x = exact_sigmoid(a, z, lane == 0 ? last_e : e), before = __shfl_sync(0xffffffffu, x, 0), now = __shfl_sync(0xffffffffu, x, 1);
+      if (now > before || (now == before && e < last_e)) {
+        if (lane == 0) sPick[c - 1] = e;
+        e = last_e;
+      }
+    } else {
+      again = false;
+    }
+    if (c == a.top) break;
+    last = best;
+    last_e = e;
+    if (lane == l) {
+      sPick[c] = e;
 #pragma unroll
       for (int i = 0; i + 1 < VPT; ++i) key[i] = key[i + 1];
       key[VPT - 1] = 0;
     }
+    __syncwarp();
   }
   __syncwarp();
   if (close) choose_exactly<VPT>(a, z, zmax, sC, sPick, lane);    // the same answer in every lane: all it goes by came from votes
@@ -411,7 +461,8 @@ __global__ void __launch_bounds__(route_threads<VPT, ONE>()) route_kernel(const 
     place_slots(a, sel, 0, a.T * a.top, sFirst, reinterpret_cast<int*>(sC));
   } else {
     __syncthreads();
-    for (int e = threadIdx.x; e < a.n_real; e += THREADS) a.counts[(size_t)blockIdx.x * a.n_real + e] = sCount[e];
+    const int width = (a.n_real + 3) & ~3;
+    for (int e = threadIdx.x; e < width; e += THREADS) a.counts[(size_t)blockIdx.x * width + e] = e < a.n_real ? sCount[e] : 0;
   }
 }
 
@@ -427,23 +478,26 @@ __global__ void __launch_bounds__(PL_THREADS) plan_kernel(const __grid_constant_
   pdl_trigger();
   const int* counts = after_wait(a.counts);
   __syncthreads();
-  // totals, and what the blocks before this one hold: each expert by several threads, every one a part of the blocks, eight loads out at a time
-  const int width = (a.n_real + 31) & ~31, parts = max(1, PL_THREADS / width);
-  for (int x = threadIdx.x; x < parts * width; x += PL_THREADS) {
-    const int part = x / width, e = x - part * width;
-    if (e >= a.n_real) continue;
-    int all = 0, before = 0;
+  // totals, and what the blocks before this one hold: four experts a thread, every thread a part of the blocks, eight loads out at a time
+  const int quads = (a.n_real + 3) >> 2, parts = max(1, PL_THREADS / quads);
+  for (int x = threadIdx.x; x < parts * quads; x += PL_THREADS) {
+    const int part = x / quads, e = 4 * (x - part * quads);
+    const int4* p = reinterpret_cast<const int4*>(counts) + (e >> 2);
+    int all[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0};
     for (int b0 = part; b0 < blocks; b0 += 8 * parts) {
-      int c[8];
+      int4 c[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = b0 + j * parts < blocks ? counts[(size_t)(b0 + j * parts) * a.n_real + e] : 0;
+      for (int j = 0; j < 8; ++j) c[j] = b0 + j * parts < blocks ? p[(size_t)(b0 + j * parts) * quads] : make_int4(0, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        all += c[j];
-        before += b0 + j * parts < (int)blockIdx.x ? c[j] : 0;
+        const bool old = b0 + j * parts < (int)blockIdx.x;
+        all[0] += c[j].x; all[1] += c[j].y; all[2] += c[j].z; all[3] += c[j].w;
+        before[0] += old ? c[j].x : 0; before[1] += old ? c[j].y : 0; before[2] += old ? c[j].z : 0; before[3] += old ? c[j].w : 0;
       }
     }
-    if (all) { atomicAdd(&sTotal[e], all); atomicAdd(&sBefore[e], before); }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e + i < a.n_real && all[i]) { atomicAdd(&sTotal[e + i], all[i]); atomicAdd(&sBefore[e + i], before[i]); }
   }
   __syncthreads();
   plan_experts(a, sTotal, sFirst, sTile, blockIdx.x == 0);
@@ -460,7 +514,7 @@ static int tokens_a_block(int T) { return T <= RP_ONE_LAUNCH ? min(T, RP_WARPS) 
 MLXB_EXPORT int mlxb_moe_route_scratch(int T, int E) {
   if (T <= RP_ONE_LAUNCH || E <= 0) return 1;
   const int tpb = tokens_a_block(T);
-  return (T + tpb - 1) / tpb * E;
+  return (T + tpb - 1) / tpb * ((E + 3) & ~3);
 }
 
 template <int VPT>
@@ -515,7 +569,7 @@ MLXB_EXPORT int mlxb_moe_route_plan(const RouteRecord* rec, long long bytes, cud
     const cudaError_t e = cudaMemsetAsync(r.n_tiles, 0, sizeof(int), stream);
     return e == cudaSuccess ? 0 : mlxb_fail((int)e, "moe_route_plan: %s", cudaGetErrorString(e));
   }
-  if (!r.logits || !r.sel || !r.weight || !r.counts || !r.sorted || !r.tile_info || !r.n_tiles || max_tiles > 0x7fffffffLL || tile_rows > 0x7fffffffLL || T < 0 || E <= 0 || E > 1024 || top <= 0 || top > E || top > 64 || ldl < E || groups < 1 || groups > 128 || E % groups || keep < 1 || keep > groups ||
+  if (!r.logits || !r.sel || !r.weight || !r.counts || ((uintptr_t)r.counts & 15) || !r.sorted || !r.tile_info || !r.n_tiles || max_tiles > 0x7fffffffLL || tile_rows > 0x7fffffffLL || T < 0 || E <= 0 || E > 1024 || top <= 0 || top > E || top > 64 || ldl < E || groups < 1 || groups > 128 || E % groups || keep < 1 || keep > groups ||
       n_real < 1 || n_real > E || top > keep * (E / groups) || tile_rows < 1 || (long long)T * top > 0x7ffffff0LL ||
       max_tiles < ((long long)T * top + tile_rows - 1) / tile_rows + n_real)
     return mlxb_fail(MLXB_BAD_ARG, "moe_route_plan: %lld tokens, %lld of %lld experts (%lld with tensors; up to 64 of 1024), %lld of %lld groups (up to 128), tiles of %lld rows, room for %lld",

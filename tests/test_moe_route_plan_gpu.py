@@ -92,6 +92,51 @@ def test_ties_and_near_ties(T):
     check(z.cuda(), 7, correction=near.cuda(), groups=8, keep_groups=3, group_score="best", score="softmax")
 
 
+def logit(p):
+    return math.log(p / (1.0 - p))
+
+
+@pytest.mark.parametrize("steps", [0, 1, 3])
+def test_two_that_are_close(steps):
+    """Next to one of the best, at every rank and at the border of those chosen, an expert whose score is a few steps of float32 above or below."""
+    T, E, top = 300, 64, 6
+    z, c = logits_of(T, E, 7).cpu(), correction_of(E).cpu()
+    for t in range(T):
+        by = (torch.sigmoid(z[t].double()) + c.double()).sort(descending=True)
+        r = t % (top + 1)
+        a, b = int(by.indices[r]), int(by.indices[r + 1])
+        p = float(by.values[r]) - float(c[b])
+        if 0.01 < p < 0.99:
+            x = torch.tensor(logit(p), dtype=torch.float32)
+            for _ in range(steps):
+                x = torch.nextafter(x, torch.tensor(math.inf if t % 2 else -math.inf))
+            z[t, b] = x
+    check(z.cuda(), top, correction=c.cuda(), renormalize=True)
+    check(z.cuda(), top, correction=c.cuda(), score="softmax")
+
+
+@pytest.mark.parametrize("steps", [0, 1, 4])
+@pytest.mark.parametrize("corrected", [False, True])
+@pytest.mark.parametrize("E,groups,keep", [(64, 8, 3), (60, 4, 2), (96, 3, 1), (320, 5, 2)])
+def test_two_groups_that_are_close(E, groups, keep, corrected, steps):
+    """The last group that stays and the first that does not: sums of two a few steps of float32 apart."""
+    T, per = 200, E // groups
+    z, c = logits_of(T, E, 8).cpu(), correction_of(E).cpu() if corrected else torch.zeros(E)
+    for t in range(T):
+        by = (torch.sigmoid(z[t].double()) + c.double()).view(groups, per)
+        two = by.topk(2, 1)
+        order = two.values.sum(1).sort(descending=True).indices
+        a, b = int(order[keep - 1]), int(order[keep])
+        e = b * per + int(two.indices[b, 0])
+        p = float(two.values[a].sum()) - float(two.values[b, 1]) - float(c[e])
+        if 0.01 < p < 0.99:
+            x = torch.tensor(logit(p), dtype=torch.float32)
+            for _ in range(steps):
+                x = torch.nextafter(x, torch.tensor(math.inf if t % 2 else -math.inf))
+            z[t, e] = x
+    check(z.cuda(), 3, correction=c.cuda() if corrected else None, groups=groups, keep_groups=keep, group_score="two")
+
+
 def test_numbers_that_are_none():
     E = 40
     z = logits_of(70, E, 5)
