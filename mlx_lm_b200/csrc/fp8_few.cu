@@ -1,12 +1,12 @@
 // Products with weights in 8-bit floating point for few rows (decode steps): the weights are what is read.
 //
 //   linear      out[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) (+ residual[m, n])
-//   gated       per tile of a plan (up to NT slots of one expert): h = unit of (gate, up), rounded to 8 bits in the epilogue, ready to be the
+//   gated       per tile of a plan (up to 16 slots of one expert): h = unit of (gate, up), rounded to 8 bits in the epilogue, ready to be the
 //               next product's operand
 //   experts     per tile of a plan: out[slot, n] = sum_k h[row, k] w[expert][n, k]
 //
 // Both operands are rows of codes with scales (fp8.cuh); tcgen05.mma kind::mxf8f6f4 multiplies codes and scales and adds in float32.  The sides
-// are exchanged: 128 rows of W are the product's M side and the NT (16 to 128) rows of x its N side, so that a step of one token
+// are exchanged: 128 rows of W are the product's M side and the NT (16 to 128; of a plan 16) rows of x its N side, so that a step of one token
 // wastes 15 columns of a small product instead of 127 rows of a large one, and a CTA's tile is 16 KB of weights a stage whatever the
 // number of tokens.  Gated: a stage holds 128 gate rows and the 128 up rows of the same columns, two accumulators, and one thread
 // has both numbers of a unit.  The 128 columns of a tile are one run of the result: its scale is found in the epilogue.
@@ -476,21 +476,18 @@ static int few_launch(const CUtensorMap& mw, const CUtensorMap& mx, const FewArg
 
 template <int NT, int KIND, typename TO>
 static int few_choose(const CUtensorMap& mw, const CUtensorMap& mx, const FewArgs& a, cudaStream_t stream) {
-  // a split hands every rank whole tokens, and its buffer must leave room for the stages
-  if constexpr (NT <= (KIND == FEW_GATED ? 32 : 128)) {
-    const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR);
-    if (ranks > 1) return few_launch<NT, KIND, true, TO>(mw, mx, a, ranks, stream);
-  }
+  const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR);
+  if (ranks > 1) return few_launch<NT, KIND, true, TO>(mw, mx, a, ranks, stream);
   return few_launch<NT, KIND, false, TO>(mw, mx, a, 1, stream);
 }
 
-template <int KIND, typename TO>
+template <typename TO>
 static int few_width(int nt, const CUtensorMap& mw, const CUtensorMap& mx, const FewArgs& a, cudaStream_t stream) {
   switch (nt) {
-    case 16: return few_choose<16, KIND, TO>(mw, mx, a, stream);
-    case 32: return few_choose<32, KIND, TO>(mw, mx, a, stream);
-    case 64: return few_choose<64, KIND, TO>(mw, mx, a, stream);
-    default: return few_choose<128, KIND, TO>(mw, mx, a, stream);
+    case 16: return few_choose<16, FEW_LINEAR, TO>(mw, mx, a, stream);
+    case 32: return few_choose<32, FEW_LINEAR, TO>(mw, mx, a, stream);
+    case 64: return few_choose<64, FEW_LINEAR, TO>(mw, mx, a, stream);
+    default: return few_choose<128, FEW_LINEAR, TO>(mw, mx, a, stream);
   }
 }
 
@@ -514,10 +511,10 @@ MLXB_EXPORT int mlxb_fp8_linear_few(const Fp8LinearRecord* rec, long long bytes,
   CUtensorMap mw, mx;
   if (int e = fp8_make_map(&mw, r.w, N, K, K, 128, "linear (8 bits) w")) return e;
   if (int e = fp8_make_map(&mx, r.x, M, K, K, nt, "linear (8 bits) x")) return e;
-  return r.out_f32 ? few_width<FEW_LINEAR, float>(nt, mw, mx, a, stream) : few_width<FEW_LINEAR, __nv_bfloat16>(nt, mw, mx, a, stream);
+  return r.out_f32 ? few_width<float>(nt, mw, mx, a, stream) : few_width<__nv_bfloat16>(nt, mw, mx, a, stream);
 }
 
-// Over a plan with tiles of tile_rows (16, 32 or 64) slots; x codes [max_tiles * tile_rows, K], a tile's rows at tile_rows * t, scales a group a tile.
+// Over a plan with tiles of 16 slots; x codes [max_tiles * 16, K], a tile's rows at 16 t, scales a group a tile.
 // gated: w codes [E][2][N][K] (gate rows, up rows), scales of 2 E groups of N rows; out codes [max_tiles * tile_rows, ldo] with their
 // scales, ldo = N rounded up to 16.  Else w codes [E][N][K]; out bfloat16 or float32 rows [S, ldo], row sorted[i] for place i of the plan.
 // at_most: a bound on the number of tiles.
@@ -526,7 +523,7 @@ MLXB_EXPORT int mlxb_fp8_experts_few(const Fp8ExpertsRecord* rec, long long byte
   const Fp8ExpertsRecord& r = *rec;
   if (r.max_tiles <= 0 || r.at_most <= 0) return 0;
   if (int e = fp8_check_experts(r)) return e;
-  if (r.tile_rows != 16 && r.tile_rows != 32 && r.tile_rows != 64) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: tiles of %lld rows", r.tile_rows);
+  if (r.tile_rows != 16) return mlxb_fail(MLXB_BAD_ARG, "moe_gemm_fp8: tiles of %lld rows", r.tile_rows);
   const int N = (int)r.N, K = (int)r.K;
   FewArgs a = {};
   a.x_scales = (const uint8_t*)r.xs; a.w_scales = (const uint8_t*)r.ws;
@@ -540,14 +537,6 @@ MLXB_EXPORT int mlxb_fp8_experts_few(const Fp8ExpertsRecord* rec, long long byte
   CUtensorMap mw, mx;
   if (int e = fp8_make_map(&mw, r.w, r.E * (r.gated ? 2 : 1) * N, K, K, 128, "moe_gemm_fp8 w")) return e;
   if (int e = fp8_make_map(&mx, r.x, r.max_tiles * r.tile_rows, K, K, (int)r.tile_rows, "moe_gemm_fp8 x")) return e;
-#define GO(KIND, TO)                                                                  \
-  switch (r.tile_rows) {                                                              \
-    case 16: return few_choose<16, KIND, TO>(mw, mx, a, stream);                      \
-    case 32: return few_choose<32, KIND, TO>(mw, mx, a, stream);                      \
-    default: return few_choose<64, KIND, TO>(mw, mx, a, stream);                      \
-  }
-  if (r.gated) GO(FEW_GATED, float)
-  if (r.out_f32) GO(FEW_EXPERTS, float)
-  GO(FEW_EXPERTS, __nv_bfloat16)
-#undef GO
+  if (r.gated) return few_choose<16, FEW_GATED, float>(mw, mx, a, stream);
+  return r.out_f32 ? few_choose<16, FEW_EXPERTS, float>(mw, mx, a, stream) : few_choose<16, FEW_EXPERTS, __nv_bfloat16>(mw, mx, a, stream);
 }

@@ -583,10 +583,12 @@ static int many_launch(const ManyMaps& maps, const ManyArgs& a, cudaStream_t str
 }
 
 // Tile width and pairs or not: the form whose time, as a sum of what was measured, is least: a launch (set-up, the first copies, the last tile's
-// results), every run of 128 of K, every further wave of tiles.
+// results), every run of 128 of K, every further wave of tiles.  A fit to 48 sizes (129 to 4096 rows, K and N of 512 to 14336) where the choice is within 5 % of
+// the best form (us at 256 columns in pairs | alone | 128 in pairs | alone): 129 x 4096 x 4096 15.0 | 16.6 | 12.4 | 12.9; 1024 x 1024 x 4096
+// 8.9 | 7.7 | 9.5 | 9.0; 1024 x 1024 x 1024 7.5 | 6.8 | 6.3 | 5.7; 4096 x 4096 x 4096 53 | 60 | 71 | 75.
 struct ManyForm { int bn, cg; };
 struct ManyCost { int bn, cg; double launch, run, wave; };      // microseconds
-static constexpr ManyCost MANY_FORMS[] = {{256, 2, 6.4, .297, 2.2}, {256, 1, 5.2, .442, .9}, {128, 2, 5., .245, .5}, {128, 1, 4.2, .272, .6}};
+static constexpr ManyCost MANY_FORMS[] = {{256, 2, 5., .323, 1.9}, {256, 1, 3.8, .395, 1.5}, {128, 2, 4.5, .245, .6}, {128, 1, 3.5, .294, .5}};
 static ManyForm many_form(int M, int N, int K) {
   const char *want_pair = getenv("MLXB_FP8_PAIR"), *want_bn = getenv("MLXB_FP8_BN");     // experiments and tests
   const int sms = mlxb_sm_count(), runs = (K + 127) / 128;

@@ -2486,7 +2486,15 @@ def moe_gemm_tc05(a, w, n_out: int, sorted_slots, tile_info, n_tiles, max_tiles:
 # weights in 8-bit floating point (csrc/fp8.cuh, fp8_rows.cu, fp8_few.cu, fp8_many.cu)
 
 FP8_RUN = 128            # columns of a row that share a scale
-FP8_FEW_ROWS = 128       # up to so many rows, a linear layer streams its weights (csrc/fp8_few.cu)
+
+
+def _fp8_few(M: int, N: int, K: int) -> bool:
+    """Whether a linear layer runs in the kernel that streams the weights (csrc/fp8_few.cu): up to 32 rows always (32 x 4096 x 4096: 8.3 us beside
+    12.7 on tiles of rows, 32 x 1024 x 4096: 5.1 beside 6.0).  More rows are tiles of 64 or 128 there, and what it still has over the other is that it
+    splits a long K: up to 64 rows from K = 2048 on (64 x 4096 x 4096: 9.8 beside 12.7; 64 x 1024 x 4096: 6.8 beside 6.1), up to 128 from
+    4096 on (128 x 8192 x 4096: 15.0 beside 21.6; 128 x 2048 x 4096: 10.3 beside 8.5), while N leaves SMs over to split it on (64 x 4096
+    x 16384: 16.5 beside 15.2; 128 x 4096 x 8192: 17.6 beside 13.4)."""
+    return M <= 32 or (M <= 64 and K > 1024 and N < 16384) or (M <= 128 and K > 2048 and N < 8192)
 
 
 def fp8_empty(rows: int, columns: int, device, groups: int = 1):
@@ -2570,7 +2578,7 @@ _fp8_linear_record = _kv8_record("8Q6q")
 def linear_fp8(codes, scales, w_codes, w_scales, bias, out, status, stream, epilogue: int = EPI_NONE, residual=None) -> None:
     """``linear_generic``'s contract for rows and weights in 8-bit floating point (``fp8_quantize``): ``out = act(x w^T + bias) (+ residual)``
     with ``x`` and ``w`` the numbers that codes and scales stand for, float32 sums and epilogue; ``out`` (and ``residual``, which may be ``out``)
-    bfloat16 or float32.  Up to ``FP8_FEW_ROWS`` rows run in the kernel that streams the weights, more on tiles of rows.  ``status`` receives
+    bfloat16 or float32.  Few rows run in the kernel that streams the weights, more on tiles of rows.  ``status`` receives
     ``ST_WAIT_TIMEOUT`` if a bounded wait gives up."""
     M, N, ldo = _fp8_rows(out, "linear (8 bits) out")
     if M == 0 or N == 0:
@@ -2590,22 +2598,23 @@ def linear_fp8(codes, scales, w_codes, w_scales, bias, out, status, stream, epil
                               f"{out.dtype} {tuple(out.shape)} strides {out.stride()}")
         rp = residual.data_ptr()
     _fp8_device("linear (8 bits)", codes, scales, w_codes, w_scales, out, status, bias, residual)
-    lib, fn = ("fp8_few", "mlxb_fp8_linear_few") if M <= FP8_FEW_ROWS else ("fp8_many", "mlxb_fp8_linear_many")
+    lib, fn = ("fp8_few", "mlxb_fp8_linear_few") if _fp8_few(M, N, K) else ("fp8_many", "mlxb_fp8_linear_many")
     _call(lib, fn, _FP8_ARGS, *_fp8_linear_record(
         codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), bp, rp, out.data_ptr(), status.data_ptr(),
         out.dtype is _F32T, M, N, K, ldo, epilogue), stream)
 
 
 def moe_fp8_tile_rows(n_slots: int, n_experts: int) -> int:
-    """Slots a tile of a plan for ``moe_gemm_fp8`` had best take, by how many an expert gets on average."""
-    each = n_slots / max(1, n_experts)
-    return 16 if each <= 8 else 32 if each <= 16 else 64 if each <= 32 else 128
+    """Slots a tile of a plan for ``moe_gemm_fp8`` had best take, 16 or 128, by how many an expert gets on average.  (64 experts, 2048 to twice 1024 columns,
+    us with tiles of 16 | 128: 4 slots an expert 48.6 | 49.9, 8 48.6 | 51.7, 16 51.7 | 52.3, 32 65.4 | 52.6; 16 experts, 1024 to twice
+    2048: 11.8 | 12.8, 12.4 | 12.9, 18.2 | 12.8, 27.2 | 12.9.  Tiles of 32 and 64 were within 4 % of the better one at best.)"""
+    return 16 if n_slots <= 8 * n_experts else 128
 
 
 def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, what: str) -> int:
     """Checks a plan; how many slots it is for."""
-    if tile_rows not in (16, 32, 64, 128) or max_tiles < 0:
-        raise KernelError(f"{what}: {max_tiles} tiles of {tile_rows} rows (16, 32, 64 or 128)")
+    if tile_rows not in (16, 128) or max_tiles < 0:
+        raise KernelError(f"{what}: {max_tiles} tiles of {tile_rows} rows (16 or 128)")
     _fp8_vector(sorted_slots, _I32, 0, what + " sorted_slots")
     _fp8_vector(tile_info, _I32, 3 * max_tiles, what + " tile_info")
     _fp8_vector(n_tiles, _I32, 1, what + " n_tiles")

@@ -119,8 +119,7 @@ def test_route(change):
 
 
 def test_tile_rows_follow_the_slots_of_an_expert():
-    rows = [ops.moe_fp8_tile_rows(n, 16) for n in (1, 128, 129, 256, 257, 512, 513, 100000)]
-    assert rows == sorted(rows) and set(rows) == {16, 32, 64, 128}
+    assert [ops.moe_fp8_tile_rows(n, 16) for n in (1, 128, 129, 256, 100000)] == [16, 16, 128, 128, 128]
 
 
 def test_parts():
@@ -143,8 +142,9 @@ def test_parts():
 
 
 def test_command_lines():
-    from mlx_lm_b200 import benchmark, generate
+    import importlib
 
+    benchmark, generate = (importlib.import_module("mlx_lm_b200." + name) for name in ("benchmark", "generate"))
     assert generate.setup_arg_parser().parse_args([]).weight_bits is None
     assert generate.setup_arg_parser().parse_args(["--weight-bits", "8"]).weight_bits == 8
     assert benchmark.setup_arg_parser().parse_args(["--model", "m", "--weight-bits", "8"]).weight_bits == 8
