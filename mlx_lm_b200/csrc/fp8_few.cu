@@ -18,7 +18,9 @@
 // Bound by the bytes of W where there are enough tiles; N / 128 tiles of a square layer are too few for 148 SMs, so K is split over
 // a cluster of up to eight CTAs: each sends its sums for a share of the tokens to that share's CTA (distributed shared memory), which
 // adds them in the order of the ranks.  How many CTAs share a tile depends on N and K (experts: on the largest number of tiles too), not
-// on the rows.
+// on the rows.  What an SM takes in, 64 bytes a clock, bounds a CTA; 148 of them together the memory.  Behind another kernel, in us: 1 x 4096 x 4096
+// 5.8 (2.9 TB/s; of this 3 are a kernel's start, its first bytes and its end), 8 x 4096 x 14336 12.9 (4.6 TB/s, 112 tiles for 148 SMs), gated
+// products of 32 tokens, 8 of 128 experts each, 2048 to twice 768 columns: 57 (6.1 TB/s).
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
 #include "activations.cuh"

@@ -5,8 +5,9 @@
 //                own, so that the products' tiles begin where their scales do, wherever an expert's slots begin.
 //
 // A warp takes 512 columns of a row, a lane 16 neighbours: the eight lanes of a run of 128 find its largest magnitude in three
-// exchanges, a lane's codes are one store of 16 bytes and the four scales one word.  Every number is read once; the kernel is bound by
-// its bytes.
+// exchanges, a lane's codes are one store of 16 bytes and the four scales one word.  Every number is read once.  Large matrices are bound by their bytes (8192 x
+// 8192 bfloat16: 34 us, 5.9 TB/s), small ones are a chain of latencies (1.5 us behind another kernel).  Gathering rounds a row once for each of its slots:
+// 32768 slots of 2048 columns, 8 a row, take 33 us, bound by instructions (71 % of the issue slots; 201 MB through the L2, 29 MB of them from memory).
 #include "fp8.cuh"
 
 MLXB_DEFINE_LAST_ERROR()

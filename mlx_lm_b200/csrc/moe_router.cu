@@ -5,8 +5,10 @@
 //            scores (ties: the lower index); weights: the scores s, divided by their sum plus eps if wanted, times a factor.
 // plan       the (token, choice) slots sorted by expert and, within one, by number; tiles of at most tile_rows slots of one expert.
 //
-// The choice is exact: without a correction scores are in the order of the logits, and these are compared; with one, a warp compares float32 scores, which it forms with the hardware's exponential and quotient, and where any choice was by less than they can be off it forms the token's scores again in 64 bits and chooses
-// by those.  A score that is NaN, or that a correction makes minus infinity, is never chosen; places that nobody can take hold expert -1 and weight 0.
+// The choice is exact: without a correction scores are in the order of the logits, and these are compared; with one, a warp compares float32 scores,
+// which it forms with the hardware's exponential and quotient.  Where a choice was by less than they can be off, the two scores it was
+// between, if they were two, are formed again in 64 bits, else all of the token's are and it chooses by those.  A score that is NaN, or that a correction
+// makes minus infinity, is never chosen; places that nobody can take hold expert -1 and weight 0.
 //
 // A warp takes a token, a lane neighbouring experts.  Each lane sorts its scores once (a network of minima and maxima); a choice is then a redux.sync
 // over the lanes' best, a vote, and a shift in the lane that had it.  Groups: 2^p lanes search one
@@ -15,6 +17,9 @@
 // Steps of up to 128 tokens are one launch: a cluster of up to eight CTAs, a warp a token, of which the first makes the plan.  More are two launches:
 // blocks of tokens that also count their slots by expert, then the same blocks, which add up the counts before theirs and put their slots in place.
 // No atomics decide an order.
+//
+// In us: 64 tokens of 256 experts, 8 groups of which 4 stay, top 8: 10.5, a chain of latencies; 8192 of the same 30: 22 of choosing (8 MB of logits;
+// bound by instructions), 8 of the plan, which adds up 148 blocks' counts.
 #include <float.h>
 
 #include "common.cuh"
@@ -301,7 +306,8 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
   uint32_t last = 0;
   int last_e = -1;
   bool again = false;
-  for (int c = 0; c <= a.top; ++c) {                        // one more than are chosen: was the last choice close?
+  // one more than are chosen: was the last choice close?  One more again if it was: a third one may be as close
+  for (int c = 0; c <= a.top + 1; ++c) {
     const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
     if (!best) {
       for (int x = c + lane; x < a.top; x += 32) sPick[x] = -1;
@@ -324,11 +330,11 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
     } else {
       again = false;
     }
-    if (c == a.top) break;
+    if (c >= a.top && !again) break;
     last = best;
     last_e = e;
     if (lane == l) {
-      sPick[c] = e;
+      if (c < a.top) sPick[c] = e;
 #pragma unroll
       for (int i = 0; i + 1 < VPT; ++i) key[i] = key[i + 1];
       key[VPT - 1] = 0;

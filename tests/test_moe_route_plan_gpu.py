@@ -115,6 +115,25 @@ def test_two_that_are_close(steps):
     check(z.cuda(), top, correction=c.cuda(), score="softmax")
 
 
+@pytest.mark.parametrize("spread", [0.0, 2e-8, 1e-7])
+@pytest.mark.parametrize("n", [3, 4])
+@pytest.mark.parametrize("E,top", [(64, 6), (64, 1), (256, 8), (7, 2)])
+def test_several_that_are_close(E, top, n, spread):
+    """Three or four scores within the rounding of float32, at every rank and on both sides of the border of those chosen."""
+    T = 300
+    z, c = logits_of(T, E, 9).cpu(), correction_of(E).cpu()
+    g = torch.Generator().manual_seed(n)
+    for t in range(T):
+        by = (torch.sigmoid(z[t].double()) + c.double()).sort(descending=True)
+        r = max(0, min(E - n, t % (top + 2) - 1))
+        for j in range(1, n):
+            b = int(by.indices[r + j])
+            p = float(by.values[r]) - float(c[b]) + float(torch.randn((), generator=g)) * spread
+            if 0.01 < p < 0.99:
+                z[t, b] = logit(p)
+    check(z.cuda(), top, correction=c.cuda(), renormalize=True)
+
+
 @pytest.mark.parametrize("steps", [0, 1, 4])
 @pytest.mark.parametrize("corrected", [False, True])
 @pytest.mark.parametrize("E,groups,keep", [(64, 8, 3), (60, 4, 2), (96, 3, 1), (320, 5, 2)])
