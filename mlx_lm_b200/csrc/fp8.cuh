@@ -12,6 +12,7 @@
 // column r / 32, byte b % 4.  Groups: the matrices of a stack (experts), or the tiles of a plan.
 #pragma once
 
+#include "activations.cuh"
 #include "gated_unit.cuh"
 #include "tcgen05.cuh"
 
@@ -110,11 +111,25 @@ __device__ __forceinline__ void fp8_drain(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// The gated unit of gated_unit.cuh with the hardware's exponential and quotient (some 2^-21 of the value off; the result is rounded to 8 bits).
+// An activation of the list on all of a thread's numbers.  NaN stays NaN: a row that was not finite must show.
+template <bool FAST, int N>
+__device__ __forceinline__ void fp8_activate(int act, float (&v)[N]) {
+  switch (act) {
+#define MLXB_FP8_ACT(ID, CODE, NAME)                                                                            \
+  case CODE:                                                                                                    \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = v[i] == v[i] ? activate<CODE, FAST>(v[i]) : v[i];      \
+    break;
+    MLXB_ACTIVATION_LIST(MLXB_FP8_ACT)
+#undef MLXB_FP8_ACT
+  }
+}
+
+// The gated unit of gated_unit.cuh with the hardware's exponential and quotient (some 2^-21 of the value off; the result is rounded to 8 bits), in
+// which NaN stays NaN.
 __device__ __forceinline__ float fp8_gated_unit(int kind, float g, float u, float w, float limit) {
   if (kind == MLXB_GU_BOUNDED) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
     return w * __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
   }
   const float a = w * g;

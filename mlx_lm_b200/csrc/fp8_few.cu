@@ -23,7 +23,6 @@
 // products of 32 tokens, 8 of 128 experts each, 2048 to twice 768 columns: 57 (6.1 TB/s).
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
-#include "activations.cuh"
 #include "fp8.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -79,12 +78,6 @@ struct FewSmem {
   uint32_t tmem;
   int abort_flag;
 };
-
-template <int ACT, bool FAST, int N>
-__device__ __forceinline__ void activate_all(float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
-}
 
 // 1 if `ok` holds for every thread of the four epilogue warps
 __device__ __forceinline__ bool epilogue_agrees(bool ok) {
@@ -294,12 +287,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       if (KIND == FEW_LINEAR) {
 #pragma unroll
         for (int j = 0; j < CH; ++j) v[j] += x.bias;
-        switch (a.act) {
-          case EPI_GELU_NEW: activate_all<EPI_GELU_NEW, sizeof(TO) == 2>(v); break;
-          case EPI_RELU: activate_all<EPI_RELU, sizeof(TO) == 2>(v); break;
-          case EPI_TANH: activate_all<EPI_TANH, sizeof(TO) == 2>(v); break;
-          default: break;
-        }
+        fp8_activate<sizeof(TO) == 2>(a.act, v);
         if (a.residual) {
 #pragma unroll
           for (int j = 0; j < CH; ++j) v[j] += x.residual[j];

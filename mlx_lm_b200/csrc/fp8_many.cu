@@ -21,7 +21,6 @@
 // both CTAs wait for the slower one's epilogue, and an expert's odd tile leaves half a pair idle.
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
-#include "activations.cuh"
 #include "fp8.cuh"
 
 MLXB_DEFINE_LAST_ERROR()
@@ -78,12 +77,6 @@ struct ManySmem {
 };
 
 __device__ __forceinline__ int many_stage(int row, int piece) { return row * 2 + (piece ^ ((row >> 2) & 1)); }
-
-template <int ACT, bool FAST, int N>
-__device__ __forceinline__ void activate_all(float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = activate<ACT, FAST>(v[i]);
-}
 
 // 32 rows of 32 bytes from shared memory to columns x .., rows y .. of a matrix; what lies outside it is left out
 __device__ __forceinline__ void store_box(const CUtensorMap* map, const void* src, int x, int y) {
@@ -381,12 +374,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               __syncwarp();
             }
             float (&vv)[32] = *reinterpret_cast<float (*)[32]>(r[c]);
-            switch (a.act) {
-              case EPI_GELU_NEW: activate_all<EPI_GELU_NEW, sizeof(TO) == 2>(vv); break;
-              case EPI_RELU: activate_all<EPI_RELU, sizeof(TO) == 2>(vv); break;
-              case EPI_TANH: activate_all<EPI_TANH, sizeof(TO) == 2>(vv); break;
-              default: break;
-            }
+            fp8_activate<sizeof(TO) == 2>(a.act, vv);
           }
           if constexpr (!WHOLE) {         // rows that do not begin on 16 bytes: a few columns at a time through shared memory in float32
             constexpr int COLS = S::OUT / 128, STEP = 32 / COLS;         // 16 or 8 columns, 2 or 4 rows an instruction

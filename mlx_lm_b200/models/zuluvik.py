@@ -24,7 +24,8 @@ config.json keys: ``architecture``, ``vocab``, ``width``, ``embedding.scale``, `
 ``mixer``, ``mlp``, ``weights_of``).  Mixer keys: ``heads, kv_heads, dim, vdim, scale`` and ``diff, conv`` (attention),
 ``rot`` (attention_2), ``heads, dim, rot_dim, vdim, kv_rank, scale, rot`` (latent_attention); ``rot``: ``base, dims`` and
 optionally ``scaling`` (``factor, original, fast, slow``).  ``mlp``: ``kind: moe``, ``expert`` (``ff, limit``), ``router``
-(``experts, top, identity, scale, groups.count, groups.keep``), ``shared`` (``ff, limit``).  Tensor names: ``embed``,
+(``experts, top, identity, scale, groups.count, groups.keep``; optionally ``groups.score``: a group is judged by its
+``best`` choice score or by the sum of its ``two`` best), ``shared`` (``ff, limit``).  Tensor names: ``embed``,
 ``l<i>.norm1``, ``l<i>.mix.*``, ``l<i>.mlp.router|correction``, ``l<i>.mlp.e<n>.gate|up|down``,
 ``l<i>.mlp.shared.gate|up|down``, ``final.norm``, ``head``.
 """
@@ -37,6 +38,7 @@ import torch
 
 from ..config.base import BaseModelArgs, ConfigError, _positive_int
 from ..config.registry import register_architecture
+from ..ops import MOE_GROUP_SCORES
 from ..parts import (DifferentialAttention, ExpertsMLP, GatedMLP, Init, LatentAttention, ModelDescription, OutputHead,
                      ParallelBlock, RMSNorm, RunEntry, TalkingHeadsAttention, TokenEmbedding)
 
@@ -128,6 +130,8 @@ class ModelArgs(BaseModelArgs):
                             or r["top"] > g["keep"] * (outputs // g["count"]):
                         raise ConfigError(f"{where}.router.groups: {outputs} router outputs in {g['count']} groups, "
                                           f"{g['keep']} kept, {r['top']} chosen")
+                    if g.get("score", "best") not in MOE_GROUP_SCORES:
+                        raise ConfigError(f"{where}.router.groups.score {g['score']!r}: one of {sorted(MOE_GROUP_SCORES)}")
                 if mlp.get("shared"):
                     _need(mlp["shared"], ["ff", "limit"], where + ".shared")
 
@@ -164,7 +168,7 @@ def _feed_forward(name: str, D: int, mlp: dict):
     return ExpertsMLP(name, D, int(e["ff"]), int(r["experts"]), int(r["top"]), score="softmax", renormalize=True,
                       scale_input=False, init=lin, router_init=lin, correction=True,
                       groups=(int(g["count"]), int(g["keep"])) if g else None, identity=int(r.get("identity") or 0),
-                      renormalize_eps=RENORMALIZE_EPS, weight_scale=float(r.get("scale", 1.0)), unit="bounded",
+                      group_score=g.get("score", "best") if g else "best", renormalize_eps=RENORMALIZE_EPS, weight_scale=float(r.get("scale", 1.0)), unit="bounded",
                       limit=float(e["limit"]), shared=shared)
 
 

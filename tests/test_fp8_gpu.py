@@ -284,20 +284,22 @@ def test_experts_of_one_and_of_nobody(tile_rows):
 
 # ------------------------------------------------------------------------------------------------ how they are used
 
-def test_a_row_that_is_not_finite_keeps_to_itself():
+@pytest.mark.parametrize("act", ["none", "relu", "gelu_new", "tanh"])
+def test_a_row_that_is_not_finite_keeps_to_itself(act):
     o = ops()
     for M in (20, 300):
         x = normal((M, 400), 1, torch.bfloat16)
         x[3, 17], x[5, 399], x[9, 0] = math.nan, math.inf, -math.inf
         w = normal((260, 400), 2, torch.bfloat16) * 0.05
         out, st = torch.zeros((M, 260), dtype=torch.bfloat16, device="cuda"), status()
-        o.linear_fp8(*kept(x), *kept(w), None, out, st, o.current_stream())
+        o.linear_fp8(*kept(x), *kept(w), None, out, st, o.current_stream(), epilogue=o.ACTIVATION_CODES[act])
         bad = torch.isnan(out).all(1)
         assert bad.nonzero().view(-1).tolist() == [3, 5, 9] and torch.isfinite(out[~bad]).all()
 
 
 @pytest.mark.parametrize("tile_rows", [16, 128])
-def test_a_slot_that_is_not_finite_keeps_to_itself(tile_rows):
+@pytest.mark.parametrize("unit", ["silu", "bounded"])
+def test_a_slot_that_is_not_finite_keeps_to_itself(tile_rows, unit):
     o = ops()
     T, E, D, F = 30, 2, 256, 200
     x = normal((T, D), 1, torch.bfloat16)
@@ -308,7 +310,7 @@ def test_a_slot_that_is_not_finite_keeps_to_itself(tile_rows):
     hc, hs = o.fp8_empty(tile_rows, F, "cuda", groups=plan[3])
     out, st, stream = torch.zeros((T, D), device="cuda"), status(), o.current_stream()
     o.moe_gather_fp8(x, 1, *plan, codes, scales, stream)
-    o.moe_gemm_fp8(codes, scales, *wi, *plan, hc, st, stream, gated=True, out_scales=hs)
+    o.moe_gemm_fp8(codes, scales, *wi, *plan, hc, st, stream, gated=True, out_scales=hs, unit=unit, limit=2.0)
     o.moe_gemm_fp8(hc, hs, *wo, *plan, out, st, stream)
     bad = torch.isnan(out).any(1)
     assert bad.nonzero().view(-1).tolist() == [4, 7]
