@@ -2543,13 +2543,21 @@ def _fp8_vector(t, dtype, n: int, what: str) -> None:
         raise KernelError(f"{what}: {t.dtype} {tuple(t.shape)} strides {t.stride()}: {n} elements of {dtype} in one piece")
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _fp8_device(what: str, *tensors) -> None:
     """All on the current device, which the launch goes to."""
-    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise KernelError(f"{what}: tensors on {sorted({str(x.device) for x in tensors if x is not None})}, "
-                              + (f"the current device is cuda:{here}" if here >= 0 else "not on a CUDA device"))
+    here = tensors[0].get_device()
+    if here >= 0 and here == _current_device():
+        for t in tensors:
+            if t is not None and t.get_device() != here:
+                break
+        else:
+            return
+    here = _current_device() if torch.cuda.is_initialized() else -2
+    raise KernelError(f"{what}: tensors on {sorted({str(x.device) for x in tensors if x is not None})}, "
+                      + (f"the current device is cuda:{here}" if here >= 0 else "not on a CUDA device"))
 
 
 _fp8_quantize_record = _kv8_record("3Q6q")
@@ -2615,10 +2623,13 @@ def _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles: int, tile_rows: int, 
     """Checks a plan; how many slots it is for."""
     if tile_rows not in (16, 128) or max_tiles < 0:
         raise KernelError(f"{what}: {max_tiles} tiles of {tile_rows} rows (16 or 128)")
+    if (sorted_slots.dtype is _I32 and tile_info.dtype is _I32 and n_tiles.dtype is _I32 and tile_info.numel() >= 3 * max_tiles and n_tiles.numel()
+            and sorted_slots.is_contiguous() and tile_info.is_contiguous() and n_tiles.is_contiguous()):
+        return sorted_slots.numel()
     _fp8_vector(sorted_slots, _I32, 0, what + " sorted_slots")
     _fp8_vector(tile_info, _I32, 3 * max_tiles, what + " tile_info")
     _fp8_vector(n_tiles, _I32, 1, what + " n_tiles")
-    return sorted_slots.numel()
+    raise AssertionError(what)
 
 
 _fp8_gather_record = _kv8_record("6Q8q")
