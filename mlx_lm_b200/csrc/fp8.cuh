@@ -111,13 +111,14 @@ __device__ __forceinline__ void fp8_drain(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// An activation of the list on all of a thread's numbers.  NaN stays NaN: a row that was not finite must show.
+// An activation of the list on all of a thread's numbers.  NaN stays NaN: a row that was not finite must show.  (The others than relu see to it themselves; a
+// comparison more for each number costs 2048 x 1600 x 6400 with gelu_new 4 us of 32.)
 template <bool FAST, int N>
 __device__ __forceinline__ void fp8_activate(int act, float (&v)[N]) {
   switch (act) {
-#define MLXB_FP8_ACT(ID, CODE, NAME)                                                                            \
-  case CODE:                                                                                                    \
-    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = v[i] == v[i] ? activate<CODE, FAST>(v[i]) : v[i];      \
+#define MLXB_FP8_ACT(ID, CODE, NAME)                                                                                              \
+  case CODE:                                                                                                                      \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = CODE == EPI_RELU && !(v[i] == v[i]) ? v[i] : activate<CODE, FAST>(v[i]); \
     break;
     MLXB_ACTIVATION_LIST(MLXB_FP8_ACT)
 #undef MLXB_FP8_ACT

@@ -14,8 +14,8 @@ MLXB_DEFINE_LAST_ERROR()
 
 constexpr int FQ_WARPS = 8;
 
-// 16 neighbours of a row of T, as they lie in memory; zeros behind column K.  VEC: K, the row's stride and its address are such that 16 of them
-// are whole 16-byte pieces.
+// 16 neighbours of a row of T, as they lie in memory; zeros behind column K.  VEC: K, the row's stride and its address are such that they
+// lie in whole 16-byte pieces.
 template <typename T>
 struct Sixteen {
   uint32_t w[4 * sizeof(T)];
@@ -24,7 +24,7 @@ struct Sixteen {
     if (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T); ++i) {
-        const uint4 u = c < K ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 u = c + i * (16 / (int)sizeof(T)) < K ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0u, 0u, 0u, 0u);
         w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
       }
     } else if (sizeof(T) == 2) {
@@ -163,7 +163,7 @@ fp8_gather_kernel(const T* x, long long ldx, int K, int a_div, const int* sorted
 
 template <typename T>
 static bool whole_pieces(const void* x, long long ldx, int K) {
-  return !(K & 15) && !(((uintptr_t)x | (uintptr_t)(ldx * (long long)sizeof(T))) & 15);
+  return !(K & (16 / (int)sizeof(T) - 1)) && !(((uintptr_t)x | (uintptr_t)(ldx * (long long)sizeof(T))) & 15);
 }
 
 static int check(const char* what, const void* x, int K, long long ldx, const void* codes, int ld, const void* scales) {
