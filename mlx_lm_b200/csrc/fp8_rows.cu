@@ -43,14 +43,16 @@ struct Sixteen {
     if (sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
     return __uint_as_float(w[i]);
   }
-  // the bits (of a float32) of the largest magnitude, not finite ones too
+  // the bits (of a float32) of the largest magnitude, not finite ones too: NaN beats all others
   __device__ __forceinline__ uint32_t largest() const {
-    uint32_t top = 0;
     if constexpr (sizeof(T) == 2) {
+      uint32_t top = w[0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i] & 0x7fff7fffu));
+      for (int i = 1; i < 8; ++i) asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i]));
+      top &= 0x7fff7fffu;
       return max(top << 16, top & 0xffff0000u);
     } else {
+      uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = max(top, w[i] & 0x7fffffffu);
       return top;
@@ -68,19 +70,19 @@ __device__ __forceinline__ uint32_t run_max(uint32_t v) {        // over the eig
 template <typename T>
 __device__ __forceinline__ void quantize512(const Sixteen<T>& x, bool in, uint8_t* out, uint8_t* scale, int lane) {
   uint32_t top = run_max(x.largest());
-  const bool odd = __any_sync(0xffffffffu, top >= 0x7f800000u);   // rare: something is not finite
-  if (odd) {
+  int e;
+  uint32_t w[4];
+  if (__all_sync(0xffffffffu, top < 0x7f800000u)) {
+    e = fp8_exponent(top);
+    const float f = fp8_power(-e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = fp8_quad(x.number(4 * i) * f, x.number(4 * i + 1) * f, x.number(4 * i + 2) * f, x.number(4 * i + 3) * f);
+  } else {                                                        // rare: something is not finite
     top = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = max(top, fp8_magnitude(x.number(i)));
-    top = run_max(top);
-  }
-  const int e = fp8_exponent(top);
-  const float f = fp8_power(-e);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = fp8_quad(x.number(4 * i) * f, x.number(4 * i + 1) * f, x.number(4 * i + 2) * f, x.number(4 * i + 3) * f);
-  if (odd) {
+    e = fp8_exponent(run_max(top));
+    const float f = fp8_power(-e);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = fp8_quad(fp8_or_nan(x.number(4 * i)) * f, fp8_or_nan(x.number(4 * i + 1)) * f, fp8_or_nan(x.number(4 * i + 2)) * f, fp8_or_nan(x.number(4 * i + 3)) * f);
