@@ -295,16 +295,32 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
 
   uint32_t key[VPT], was[VPT];
   const float inv_per = 1.f / (float)per;
+  uint32_t open = ~0u;                                      // by this lane's experts: their group stays
+  if (kept != ~0u) {
+    if (!(per & (VPT - 1))) {                               // all of one group
+      open = kept >> (((int)(((float)e0 + 0.5f) * inv_per) * a.part) & 31) & 1 ? ~0u : 0u;
+    } else {
+      open = 0u;
+#pragma unroll 1
+      for (int i = 0; i < VPT; ++i) open |= (kept >> (((int)(((float)(e0 + i) + 0.5f) * inv_per) * a.part) & 31) & 1) << i;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     if (a.correction) v[i] = s[i];
-    const int g = kept == ~0u ? 0 : (int)(((float)(e0 + i) + 0.5f) * inv_per);
-    const bool in = v[i] > -INFINITY && (kept == ~0u || kept >> ((g * a.part) & 31) & 1);
-    was[i] = key[i] = in ? order_of(v[i]) : 0u;
+    was[i] = key[i] = v[i] > -INFINITY && (open >> i & 1) ? order_of(v[i]) : 0u;
   }
   sort_down(key);
+  // A choice is the lane and the key; which of the lane's experts it was is looked up for all choices at once, and before that only for two that are close.
+  uint32_t* sKey = reinterpret_cast<uint32_t*>(sC);         // [top], no more than experts
+  auto expert_of = [&](uint32_t k, int l) {
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) at = was[i] == k ? i : at;         // two equal ones of a lane are close
+    return __shfl_sync(0xffffffffu, e0 + at, l);
+  };
   uint32_t last = 0;
-  int last_e = -1;
+  int last_l = 0;
   bool again = false;
   // one more than are chosen: was the last choice close?  One more again if it was: a third one may be as close
   for (int c = 0; c <= a.top + 1; ++c) {
@@ -314,34 +330,44 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
       break;
     }
     const int l = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) at = was[i] == best ? i : at;       // two equal ones are close
-    int e = __shfl_sync(0xffffffffu, e0 + at, l);
+    uint32_t put = best;
+    int put_l = l;
     if (c > 0 && near(number_of(last), number_of(best), !a.correction)) {
       // two that are close, and none beside them: lane 0 has the one before, the others this one
+      const int e = expert_of(best, l), last_e = expert_of(last, last_l);
       if (a.softmax || again || e == last_e || !a.correction) { close = true; break; }
       again = true;
       const double x = exact_sigmoid(a, z, lane == 0 ? last_e : e), before = __shfl_sync(0xffffffffu, x, 0), now = __shfl_sync(0xffffffffu, x, 1);
       if (now > before || (now == before && e < last_e)) {
-        if (lane == 0) sPick[c - 1] = e;
-        e = last_e;
+        if (lane == 0) { sPick[c - 1] = l; sKey[c - 1] = best; }
+        put = last;
+        put_l = last_l;
       }
     } else {
       again = false;
     }
     if (c >= a.top && !again) break;
+    if (lane == 0 && c < a.top) { sPick[c] = put_l; sKey[c] = put; }
     last = best;
-    last_e = e;
+    last_l = l;
     if (lane == l) {
-      if (c < a.top) sPick[c] = e;
 #pragma unroll
       for (int i = 0; i + 1 < VPT; ++i) key[i] = key[i + 1];
       key[VPT - 1] = 0;
     }
-    __syncwarp();
   }
   __syncwarp();
+  if (!close) {
+    for (int c0 = 0; c0 < a.top; c0 += 32) {
+      const int c = c0 + lane, l = c < a.top ? sPick[c] : -1;
+      const uint32_t k = l >= 0 ? sKey[c] : 0u;
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) at = __shfl_sync(0xffffffffu, was[i], l & 31) == k ? i : at;
+      if (l >= 0) sPick[c] = l * VPT + at;
+    }
+    __syncwarp();
+  }
   if (close) choose_exactly<VPT>(a, z, zmax, sC, sPick, lane);    // the same answer in every lane: all it goes by came from votes
   __syncwarp();
   // the weights of those that were chosen, with the library's exponential
