@@ -18,7 +18,7 @@
 // blocks of tokens that also count their slots by expert, then the same blocks, which add up the counts before theirs and put their slots in place.
 // No atomics decide an order.
 //
-// In us: 64 tokens of 256 experts, 8 groups of which 4 stay, top 8: 10.5, a chain of latencies; 8192 of the same 30: 22 of choosing (8 MB of logits;
+// In us: 64 tokens of 256 experts, 8 groups of which 4 stay, top 8: 10.1, a chain of latencies; 8192 of the same 29.5: 21 of choosing (8 MB of logits;
 // bound by instructions), 8 of the plan, which adds up 148 blocks' counts.
 #include <float.h>
 
