@@ -12,7 +12,7 @@
 // has both numbers of a unit.  The 128 columns of a tile are one run of the result: its scale is found in the epilogue.
 //
 // One CTA: warp 0 copies (TMA; a ring of stages of 128 of K), warp 1 issues the products, warps 2-5 are the epilogue (a lane a row of W).  A linear
-// layer's first stages of W are on their way before the wait for the kernel before.  Tensor memory: two accumulators where they fit, and four
+// layer's first stages of W are on their way to the L2 before the wait for the kernel before.  Tensor memory: two accumulators where they fit, and four
 // places for scales, one for each 512 of K in turn.
 //
 // Bound by the bytes of W where there are enough tiles; N / 128 tiles of a square layer are too few for 148 SMs, so K is split over
@@ -137,14 +137,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   };
 
   pdl_trigger();
-  // A linear layer's first weights are asked for before the wait.  What could write them right before this kernel is fp8_quantize, which lets
-  // the next kernel start early only where it has up to 128 rows: more rows of W than that are complete by now.
-  int early = 0;
-  if (KIND == FEW_LINEAR && a.N > 128 && first_item < a.max_items) early = min(STAGES, k1 - k0);
-  if (threadIdx.x == 0)
-    for (int s = 0; s < early; ++s) {
-      mbar_expect_tx(&sm.full[s], stage_bytes(k0 + s));
-      load_w(s, k0 + s, 0, first_item % a.w_tiles);
+  // A linear layer's first weights are on their way to the L2 before the wait, and read behind it: the kernel before may be the one that writes them.
+  if (KIND == FEW_LINEAR && threadIdx.x == 0 && first_item < a.max_items)
+    for (int k = k0; k < min(k1, k0 + STAGES); ++k) {
+      asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&map_w), "r"(k * FP8_RUN), "r"(first_item % a.w_tiles * 128) : "memory");
+      if (brings(k))
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w_scales + ((long long)(first_item % a.w_tiles) * a.kgs + (k >> 2)) * FP8_TILE), "r"(FP8_TILE) : "memory");
     }
   pdl_wait();
   const int* tile_info = after_wait(a.tile_info);
@@ -160,16 +158,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const int tile = w / a.w_tiles, nb = w - tile * a.w_tiles;
       const int group = KIND == FEW_LINEAR ? 0 : max(0, min(a.E - 1, tile_info[3 * tile])) * NH;
       for (int k = k0; k < k1; ++k) {
-        if (issued < early) {
-          if (elect_one()) load_x(s, k, tile);
-        } else {
-          ok = mbar_wait_warp(&sm.empty[s], ph ^ 1, abort_flag);
-          if (!ok) break;
-          if (elect_one()) {
-            mbar_expect_tx(&sm.full[s], stage_bytes(k));
-            load_w(s, k, group, nb);
-            load_x(s, k, tile);
-          }
+        ok = mbar_wait_warp(&sm.empty[s], ph ^ 1, abort_flag);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&sm.full[s], stage_bytes(k));
+          load_w(s, k, group, nb);
+          load_x(s, k, tile);
         }
         ++issued;
         if (++s == STAGES) { s = 0; ph ^= 1; }

@@ -100,8 +100,7 @@ template <typename T, bool VEC, int AT>
 __global__ void __launch_bounds__(32 * FQ_WARPS, AT == 1 ? 8 : 4)
 fp8_quantize_kernel(const T* x, long long ldx, int rows, int K, int group_rows, uint8_t* __restrict__ codes, int ld, uint8_t* __restrict__ scales) {
   pdl_wait();
-  // The next kernel starts early behind few rows only.  Behind many its CTAs would take the registers this one runs in (8192 x 8192: 75 us instead of 40), and a
-  // kernel that reads weights before its own wait may count on it that a weight's more than 128 rows are complete by then.
+  // The next kernel starts early behind few rows only: behind many its CTAs would take the registers this one runs in (8192 x 8192: 75 us instead of 40).
   if (AT == 1 && rows <= 128) pdl_trigger();
   x = after_wait(x);
   const int lane = threadIdx.x & 31, kgs = (K + 511) >> 9, tiles = (group_rows + 127) >> 7;

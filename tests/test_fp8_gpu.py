@@ -333,6 +333,39 @@ def test_weights_quantised_right_before_they_are_read():
             assert float((out.double() - y).abs().max()) <= 1e-3 * float(y.abs().max())
 
 
+@pytest.mark.parametrize("M", [4, 200])
+def test_weights_quantised_in_blocks_right_before_they_are_read(M):
+    """A weight that is rounded 128 rows a call, first to last and last to first, and read by the launch behind the last of them."""
+    o = ops()
+    N, K = 1024, 2048
+    x = normal((M, K), 1, torch.bfloat16)
+    xc, (wc, ws) = kept(x), o.fp8_empty(N, K, "cuda")
+    w = [normal((N, K), 2 + i, torch.bfloat16) for i in range(6)]
+    outs, st = [torch.zeros((M, N), device="cuda") for _ in w], status()
+
+    def step():
+        for turn, (m, out) in enumerate(zip(w, outs)):
+            for b in range(0, N, 128) if turn & 1 else range(N - 128, -1, -128):
+                o.fp8_quantize(m[b:b + 128], wc[b:b + 128], ws[:, b // 128:b // 128 + 1], o.current_stream())
+            o.linear_fp8(*xc, wc, ws, None, out, st, o.current_stream())
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    for out in outs:
+        out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    for m, out in zip(w, outs):
+        y = ref.values(x) @ ref.values(m).T
+        assert float((out.double() - y).abs().max()) <= 1e-4 * float(y.abs().max())
+    assert int(st) == 0
+
+
 @pytest.mark.parametrize("M", [5, 300])
 def test_captured_and_replayed(M):
     """A graph of both calls, replayed on other rows; beside it another graph with rows of its own."""
