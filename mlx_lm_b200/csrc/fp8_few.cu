@@ -19,7 +19,7 @@
 // a cluster of up to eight CTAs: each sends its sums for a share of the tokens to that share's CTA (distributed shared memory), which
 // adds them in the order of the ranks.  How many CTAs share a tile depends on N and K (experts: on the largest number of tiles too), not
 // on the rows.  What an SM takes in, 64 bytes a clock, bounds a CTA; 148 of them together the memory.  Behind another kernel, in us: 1 x 4096 x 4096
-// 5.8 (2.9 TB/s; of this 3 are a kernel's start, its first bytes and its end), 8 x 4096 x 14336 12.9 (4.6 TB/s, 112 tiles for 148 SMs), gated
+// 6.5 (2.6 TB/s; of this 3 are a kernel's start, its first bytes and its end), 8 x 4096 x 14336 13.0 (4.5 TB/s, 112 tiles for 148 SMs), gated
 // products of 32 tokens, 8 of 128 experts each, 2048 to twice 768 columns: 57 (6.1 TB/s).
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.
@@ -409,8 +409,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // ---------------------------------------------------------------------------------------------- host side
 
 // CTAs that share a tile's K.  A fit to measured times: a stage takes a CTA that has its SM to itself 0.25 us (62 GB/s, what one SM takes in) and two on one SM
-// 0.42; a split costs 1.4 us and a tenth more for each CTA.  (Microseconds at 1, 2, 4, 8 CTAs: 1 x 4096 x 4096 10.3, 8.2, 6.1, 5.8; 8 x 4096 x
-// 14336 13.2, 14.1, 15.5, 21; 64 x 5120 x 1280 15.7, 13.8, 9.0, 7.4; 1 x 8192 x 8192 19.9, 16.1, 14.0, 16.2.)
+// 0.42; a split costs 1.4 us and CTAs that do not find room at once 3.  Within 6 % of the best at 17 sizes.  (Microseconds at 1, 2, 4, 8 CTAs, the rounding of x before
+// it included: 1 x 4096 x 4096 13.3, 11.2, 9.4, 9.1; 1 x 1600 x 6400 8.8, 8.6, 8.1, 11.8; 1 x 4096 x 14336 14.8, 15.9, 18.1, 23.9; 64 x 5120 x 1280
+// 17.5, 16.3, 12.0, 10.2; 128 x 4096 x 6144 18.5, 19.6, 25.1, 40.5.)
 static int few_ranks(long long items, int runs, bool two_an_sm) {
   if (const char* want = getenv("MLXB_FP8_RANKS")) return atoi(want);      // experiments and tests
   const int sms = mlxb_sm_count();
@@ -419,7 +420,8 @@ static int few_ranks(long long items, int runs, bool two_an_sm) {
   for (int r = 1; r <= 8; r *= 2) {
     if (r > 1 && (runs < 2 * r || items * r > 4LL * sms)) break;
     const long long ctas = items * r, room = two_an_sm && r > 1 && ctas > sms ? 2 * sms : sms;
-    const double cost = (double)((ctas + room - 1) / room) * ((runs + r - 1) / r) * (room > sms ? 0.42 : 0.25) + (r > 1 ? 1.4 + 0.1 * r : 0.);
+    const long long waves = (ctas + room - 1) / room;
+    const double cost = (double)waves * ((runs + r - 1) / r) * (room > sms ? 0.42 : 0.25) + (r > 1 ? 1.4 : 0.) + 3. * (double)(waves - 1);
     if (r == 1 || cost < best_cost) { best = r; best_cost = cost; }
   }
   return best;

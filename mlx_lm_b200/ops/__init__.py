@@ -2493,8 +2493,8 @@ def _fp8_few(M: int, N: int, K: int) -> bool:
     12.7 on tiles of rows, 32 x 1024 x 4096: 5.1 beside 6.0).  More rows are tiles of 64 or 128 there, and what it still has over the other is that it
     splits a long K: up to 64 rows from K = 2048 on (64 x 4096 x 4096: 9.8 beside 12.7; 64 x 1024 x 4096: 6.8 beside 6.1), up to 128 from
     4096 on (128 x 8192 x 4096: 15.0 beside 21.6; 128 x 2048 x 4096: 10.3 beside 8.5), while N leaves SMs over to split it on (64 x 4096
-    x 16384: 16.5 beside 15.2; 128 x 4096 x 8192: 17.6 beside 13.4)."""
-    return M <= 32 or (M <= 64 and K > 1024 and N < 16384) or (M <= 128 and K > 2048 and N < 8192)
+    x 16384: 16.5 beside 15.2; 128 x 4096 x 6144: 16.7 beside 13.1)."""
+    return M <= 32 or (M <= 64 and K > 1024 and N < 16384) or (M <= 128 and K > 2048 and N <= 4096)
 
 
 def fp8_empty(rows: int, columns: int, device, groups: int = 1):
