@@ -2492,9 +2492,9 @@ def _fp8_few(M: int, N: int, K: int) -> bool:
     """Whether a linear layer runs in the kernel that streams the weights (csrc/fp8_few.cu): up to 32 rows always (32 x 4096 x 4096: 8.3 us beside
     12.7 on tiles of rows, 32 x 1024 x 4096: 5.1 beside 6.0).  More rows are tiles of 64 or 128 there, and what it still has over the other is that it
     splits a long K: up to 64 rows from K = 2048 on (64 x 4096 x 4096: 9.8 beside 12.7; 64 x 1024 x 4096: 6.8 beside 6.1), up to 128 from
-    4096 on (128 x 8192 x 4096: 15.0 beside 21.6; 128 x 2048 x 4096: 10.3 beside 8.5), while N leaves SMs over to split it on (64 x 4096
-    x 16384: 16.5 beside 15.2; 128 x 4096 x 6144: 16.7 beside 13.1)."""
-    return M <= 32 or (M <= 64 and K > 1024 and N < 16384) or (M <= 128 and K > 2048 and N <= 4096)
+    3584 on (128 x 8192 x 4096: 15.3 beside 21.7; 128 x 2304 x 4096: 10.8 beside 9.0), while N leaves SMs over to split it on (64 x 4096 x 8192: 11.2
+    beside 13.2, x 12288: 15.5 beside 14.1; 128 x 4096 x 4096: 12.0 beside 12.8, x 5120: 17.0 beside 12.9)."""
+    return M <= 32 or (M <= 64 and K > 1024 and N <= 8192) or (M <= 128 and K >= 3584 and N <= 4096)
 
 
 def fp8_empty(rows: int, columns: int, device, groups: int = 1):

@@ -136,8 +136,8 @@ def test_linear_many_sizes(M, N, K, out_dtype):
     check_linear(M, N, K, out_dtype=out_dtype)
 
 
-@pytest.mark.parametrize("M,N,K", [(33, 200, 1200), (64, 300, 2048), (65, 200, 2100), (100, 1000, 4096), (128, 129, 2064), (64, 16400, 1100), (48, 300, 1024),
-                                   (128, 4200, 2200), (100, 700, 2048)])
+@pytest.mark.parametrize("M,N,K", [(33, 200, 1200), (64, 300, 2048), (65, 200, 3584), (100, 1000, 4096), (128, 129, 3600), (64, 8200, 1100), (64, 8192, 1100),
+                                   (48, 300, 1024), (128, 4200, 3600), (128, 4096, 3600), (100, 700, 3568)])
 def test_linear_between_few_and_many(M, N, K):
     """Rows that either kernel may have, at both sides of every limit of the rule."""
     check_linear(M, N, K, bias=True)
