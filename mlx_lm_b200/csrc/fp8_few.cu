@@ -17,8 +17,8 @@
 //
 // Bound by the bytes of W where there are enough tiles; N / 128 tiles of a square layer are too few for 148 SMs, so K is split over
 // a cluster of up to eight CTAs: each sends its sums for a share of the tokens to that share's CTA (distributed shared memory), which
-// adds them in the order of the ranks.  How many CTAs share a tile depends on N and K (experts: on the largest number of tiles too), not
-// on the rows.  What an SM takes in, 64 bytes a clock, bounds a CTA; 148 of them together the memory.  Behind another kernel, in us: 1 x 4096 x 4096
+// adds them in the order of the ranks.  How many CTAs share a tile depends on N, K and whether there are more than 64 rows (experts: on
+// the largest number of tiles).  What an SM takes in, 64 bytes a clock, bounds a CTA; 148 of them together the memory.  Behind another kernel, in us: 1 x 4096 x 4096
 // 6.5 (2.6 TB/s; of this 3 are a kernel's start, its first bytes and its end), 8 x 4096 x 14336 13.0 (4.5 TB/s, 112 tiles for 148 SMs), gated
 // products of 32 tokens, 8 of 128 experts each, 2048 to twice 768 columns: 57 (6.1 TB/s).
 //
