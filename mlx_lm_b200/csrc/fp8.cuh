@@ -125,16 +125,18 @@ __device__ __forceinline__ void fp8_activate(int act, float (&v)[N]) {
   }
 }
 
-// The gated unit of gated_unit.cuh with the hardware's exponential and quotient (some 2^-21 of the value off; the result is rounded to 8 bits), in
-// which NaN stays NaN.
+// The gated unit of gated_unit.cuh with the library's exponential and the hardware's quotient, in which NaN stays NaN.  The silu unit is off by 10 * 2^-24 of
+// its value at most (exponential 2 units in the last place, quotient 2, a sum and a product), whatever a is; where the quotient's divisor passes 2^126, below a = -87, it
+// is 0.  (The hardware's exponential is off by more the larger |a| is, and each of these steps that crosses a border of 8 bits moves a number by up to 1/8.  4096
+// tokens of 64 experts take 267.9 us in all with this one, 267.0 with the hardware's, 284 with an exact quotient too, whose code is long: 300 tokens 30.7, 30.1 and 37.8.)
 __device__ __forceinline__ float fp8_gated_unit(int kind, float g, float u, float w, float limit) {
   if (kind == MLXB_GU_BOUNDED) {
     g = g > limit ? limit : g;
     u = u > limit ? limit : u < -limit ? -limit : u;
-    return w * __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
+    return w * __fdividef(g, 1.f + expf(-1.702f * g)) * (u + 1.f);
   }
   const float a = w * g;
-  return __fdividef(a, 1.f + __expf(-a)) * (w * u);
+  return __fdividef(a, 1.f + expf(-a)) * (w * u);
 }
 
 // Arguments as records of 8-byte fields (a caller fills one in a tenth of the time of as many arguments), the same for few and for many rows.
