@@ -212,11 +212,15 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
     for (int i = 0; i < VPT; ++i) zmax = fmaxf(zmax, s[i]);
     zmax = warp_max(zmax);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      s[i] = __expf(s[i] - zmax);
-      sum += s[i] == s[i] ? s[i] : 0.f;
-    }
-    sum = warp_sum(sum);
+    for (int i = 0; i < VPT; ++i) s[i] = __expf(s[i] - zmax);
+    float part[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) part[i] = s[i] == s[i] ? s[i] : 0.f;
+#pragma unroll
+    for (int n = VPT / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int i = 0; i < n; ++i) part[i] += part[i + n];
+    sum = warp_sum(part[0]);
     range = __fdividef(1.f, sum);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) s[i] *= range;
@@ -235,10 +239,17 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
       for (int i = 0; i < VPT; ++i) s[i] = v[i];
     }
   }
-  // A score is off by less than 2^-22 of the range (sigmoid: a quarter of the exponential's relative error; softmax: that error grows with its
-  // argument, 2^-24 of it, but the value falls faster), its sum with a correction or of two by 2^-24 of itself.
+  // How far a choice score is off, in steps of 2^-24.  Sigmoid: by less than 4 (a quarter of the exponential's relative error, a sum, a quotient), so that
+  // the difference of two scores is by 8, of two sums of two by 16.  Softmax, steps of the range (the largest score): a term exp(-y) is off by 2 (2 + 1.173 y) + y of
+  // itself, with its product by no more than 5 of the range; the sum, added in a tree, by 10 for its additions and by what its terms are off, 19 at most (1024
+  // terms, one at y = 0, the others near y = 5); its inverse by 4.  So the range is off by 33 of its own steps, and with it every difference by 33 of itself: 43 for
+  // two scores, 86 for two sums of two.  Each sum with a correction or of two adds one step of itself.  Without a correction the logits decide, as they are.
   bool close = false;
-  auto near = [&](float hi, float lo, bool logits) { return !(hi - lo > (logits ? 0.f : 9.6e-7f * range + 1.2e-7f * (fabsf(hi) + fabsf(lo)))); };
+  const bool by_score = a.correction || a.two;              // what groups are judged by
+  const float steps_one = !a.correction ? 0.f : a.softmax ? 43.f : 16.f, steps_group = !by_score ? 0.f : !a.softmax ? 16.f : a.two ? 86.f : 43.f;
+  auto near = [&](float hi, float lo, float steps) {
+    return !(hi - lo > (steps == 0.f ? 0.f : steps * 0x1p-24f * range + 1.2e-7f * (fabsf(hi) + fabsf(lo))));
+  };
 
   uint32_t kept = ~0u;                                      // by the first lane of a group
   const int per = a.E / a.groups;
@@ -275,12 +286,11 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
       // the worst that stays against the best that goes
       const uint32_t worst = __reduce_min_sync(0xffffffffu, stays ? order_of(score) : ~0u);
       const uint32_t best = __reduce_max_sync(0xffffffffu, mine && !stays ? order_of(score) : 0u);
-      const bool by_score = a.correction || a.two;
-      if (best && worst != ~0u && near(number_of(worst), number_of(best), !by_score)) {
+      if (best && worst != ~0u && near(number_of(worst), number_of(best), steps_group)) {
         // one on either side: formed again in 64 bits; more than that, the whole token
         const uint32_t here = __ballot_sync(0xffffffffu, j == 0 && stays && order_of(score) == worst), there = __ballot_sync(0xffffffffu, j == 0 && mine && !stays && order_of(score) == best);
         const bool other = j == 0 && mine && !(here >> lane & 1) && !(there >> lane & 1) &&
-                           (stays ? near(score, number_of(best), !by_score) : near(number_of(worst), score, !by_score));
+                           (stays ? near(score, number_of(best), steps_group) : near(number_of(worst), score, steps_group));
         if (a.softmax || !by_score || __popc(here) != 1 || __popc(there) != 1 || __any_sync(0xffffffffu, other)) {
           close = true;
         } else {
@@ -332,7 +342,7 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
     const int l = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
     uint32_t put = best;
     int put_l = l;
-    if (c > 0 && near(number_of(last), number_of(best), !a.correction)) {
+    if (c > 0 && near(number_of(last), number_of(best), steps_one)) {
       // two that are close, and none beside them: lane 0 has the one before, the others this one
       const int e = expert_of(best, l), last_e = expert_of(last, last_l);
       if (a.softmax || again || e == last_e || !a.correction) { close = true; break; }
