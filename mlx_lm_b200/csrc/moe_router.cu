@@ -275,7 +275,10 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
         b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
         b1 = fmaxf(b1, o1);
       }
-      const float score = a.two && b2 > -INFINITY ? b1 + b2 : b1;
+      const bool pair = a.two && b2 > -INFINITY;
+      const float score = pair ? fmaxf(b1 + b2, -FLT_MAX) : b1;                       // two of the lowest numbers are still in the race
+      // its two may be far larger than their sum: half of what a difference is off, and the roundings of each and of the sum
+      const float err = by_score ? 0.5f * steps_group * 0x1p-24f * range + 2.4e-7f * fminf(fabsf(b1) + (pair ? fabsf(b2) : 0.f), FLT_MAX) : 0.f;
       int better = 0;
       for (int x = 0; x < a.groups; ++x) {
         const float other = __shfl_sync(0xffffffffu, score, x * a.part);
@@ -283,15 +286,15 @@ __device__ __forceinline__ void route_token(const RouterArgs& a, const float* lo
       }
       const bool mine = g < a.groups && score > -INFINITY, stays = mine && better < a.keep;
       kept = __ballot_sync(0xffffffffu, stays && j == 0);
-      // the worst that stays against the best that goes
-      const uint32_t worst = __reduce_min_sync(0xffffffffu, stays ? order_of(score) : ~0u);
-      const uint32_t best = __reduce_max_sync(0xffffffffu, mine && !stays ? order_of(score) : 0u);
-      if (best && worst != ~0u && near(number_of(worst), number_of(best), steps_group)) {
+      // the worst that may stay against the best that may go
+      const float least = score - err, most = score + err;
+      const uint32_t worst = __reduce_min_sync(0xffffffffu, stays ? order_of(least) : ~0u);
+      const uint32_t best = __reduce_max_sync(0xffffffffu, mine && !stays ? order_of(most) : 0u);
+      if (best && worst != ~0u && !(number_of(worst) > number_of(best))) {
         // one on either side: formed again in 64 bits; more than that, the whole token
-        const uint32_t here = __ballot_sync(0xffffffffu, j == 0 && stays && order_of(score) == worst), there = __ballot_sync(0xffffffffu, j == 0 && mine && !stays && order_of(score) == best);
-        const bool other = j == 0 && mine && !(here >> lane & 1) && !(there >> lane & 1) &&
-                           (stays ? near(score, number_of(best), steps_group) : near(number_of(worst), score, steps_group));
-        if (a.softmax || !by_score || __popc(here) != 1 || __popc(there) != 1 || __any_sync(0xffffffffu, other)) {
+        const uint32_t here = __ballot_sync(0xffffffffu, j == 0 && stays && !(least > number_of(best)));
+        const uint32_t there = __ballot_sync(0xffffffffu, j == 0 && mine && !stays && !(number_of(worst) > most));
+        if (a.softmax || !by_score || __popc(here) != 1 || __popc(there) != 1) {
           close = true;
         } else {
           const int la = __ffs(here) - 1, lb = __ffs(there) - 1, ga = la / a.part, gb = lb / a.part;

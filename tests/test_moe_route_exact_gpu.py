@@ -1,10 +1,10 @@
-"""The router's choice where float32 says otherwise than 64 bits: scores under a softmax whose sum is off."""
+"""The router's choice where float32 says otherwise than 64 bits: scores under a softmax whose sum is off, groups whose two best cancel."""
 import math
 
 import pytest
 import torch
 
-from test_moe_route_plan_gpu import run
+from test_moe_route_plan_gpu import check, correction_of, logits_of, run
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,37 @@ def test_softmax_groups_of_two_one_far_ahead(E, by):
         c[E // 2] = float(s[0] - s[1] + by)
         got, want = choices(z.cuda(), c.cuda(), 2, groups=4, keep_groups=1, group_score="two")
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("size", [30.0, 1000.0, 1e5])
+@pytest.mark.parametrize("groups,per", [(8, 2), (4, 3), (16, 4)])
+def test_two_best_that_cancel(size, groups, per):
+    """Corrections far above and far below zero in every group: sums of two are small, their float32 roundings are not."""
+    T, E, keep = 200, groups * per, groups // 2
+    g = torch.Generator().manual_seed(groups)
+    c = torch.full((groups, per), -10.0 * size)
+    c[:, 0], c[:, 1] = size, -size
+    z = torch.randn((T, groups, per), generator=g)
+    for t in range(T):                # the last that stays and the first that goes, nearer to one another than the size's rounding
+        two = torch.sigmoid(z[t, :, :2].double()).sum(1)
+        order = two.sort(descending=True).indices
+        a, b = int(order[keep - 1]), int(order[keep])
+        p = float(two[a]) - float(torch.sigmoid(z[t, b, 1].double())) + float(torch.randn((), generator=g)) * size * 2.0 ** -26
+        if 0.01 < p < 0.99:
+            z[t, b, 0] = math.log(p / (1.0 - p))
+    check(z.view(T, E).cuda(), 2, correction=c.view(E).cuda(), groups=groups, keep_groups=keep, group_score="two", renormalize=True)
+
+
+@pytest.mark.parametrize("corrected", ["lowest", "halves"])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_out_of_the_lowest_numbers(corrected, score):
+    """Groups whose corrections are the type's lowest number, or half of it: they come last, and are chosen from where nothing else is left."""
+    T, groups, per = 90, 8, 4
+    lowest = torch.finfo(torch.float32).min
+    c = correction_of(groups * per).view(groups, per)
+    c[3:] = lowest if corrected == "lowest" else 0.5 * lowest
+    c[1, 2:] = lowest
+    c[5, 1] = -math.inf
+    for keep, top in ((2, 3), (3, 8), (5, 14)):
+        for two in ("best", "two"):
+            check(logits_of(T, groups * per, keep), top, correction=c.view(-1).contiguous(), groups=groups, keep_groups=keep, group_score=two, score=score)
