@@ -408,12 +408,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
 // ---------------------------------------------------------------------------------------------- host side
 
-// CTAs that share a tile's K.  A fit to measured times: a stage takes a CTA that has its SM to itself 0.25 us (62 GB/s, what one SM takes in) and two on one SM
+// CTAs that share a tile's K (0: the environment asks for a number that cannot be).  A fit to measured times: a stage takes a CTA that has its SM to itself 0.25 us (62 GB/s, what one SM takes in) and two on one SM
 // 0.42; a split costs 1.4 us and CTAs that do not find room at once 3.  Within 6 % of the best at 17 sizes.  (Microseconds at 1, 2, 4, 8 CTAs, the rounding of x before
 // it included: 1 x 4096 x 4096 13.3, 11.2, 9.4, 9.1; 1 x 1600 x 6400 8.8, 8.6, 8.1, 11.8; 1 x 4096 x 14336 14.8, 15.9, 18.1, 23.9; 64 x 5120 x 1280
 // 17.5, 16.3, 12.0, 10.2; 128 x 4096 x 6144 18.5, 19.6, 25.1, 40.5.)
 static int few_ranks(long long items, int runs, bool two_an_sm) {
-  if (const char* want = getenv("MLXB_FP8_RANKS")) return atoi(want);      // experiments and tests
+  if (const char* want = getenv("MLXB_FP8_RANKS")) {      // experiments and tests
+    const int r = atoi(want);                             // shares of tokens are whole quadruples and every CTA has a run
+    return r == 1 || ((r == 2 || r == 4 || r == 8) && runs >= r) ? r : 0;
+  }
   const int sms = mlxb_sm_count();
   int best = 1;
   double best_cost = 0.;
@@ -463,6 +466,7 @@ static int few_launch(const CUtensorMap& mw, const CUtensorMap& mx, const FewArg
 template <int NT, int KIND, typename TO>
 static int few_choose(const CUtensorMap& mw, const CUtensorMap& mx, const FewArgs& a, cudaStream_t stream) {
   const int ranks = few_ranks(a.max_items, a.runs, FewShape<NT, KIND, true>::PAIR);
+  if (!ranks) return mlxb_fail(MLXB_BAD_ARG, "linear (8 bits): MLXB_FP8_RANKS is 1, 2, 4 or 8 and no more than the %d runs of 128 columns", a.runs);
   if (ranks > 1) return few_launch<NT, KIND, true, TO>(mw, mx, a, ranks, stream);
   return few_launch<NT, KIND, false, TO>(mw, mx, a, 1, stream);
 }

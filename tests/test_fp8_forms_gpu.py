@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_fp8_gpu import check_experts
+from test_fp8_gpu import check_experts, kept, normal, planned, status
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,22 @@ def test_experts_of_more_tiles_than_ctas(D, F, unit, out_dtype):
 
 def test_few_slots_of_more_tiles_than_ctas():
     check_experts(200, 8, 64, 1152, 1160, 16)
+
+
+@pytest.mark.parametrize("ranks,K", [("3", 2048), ("0", 2048), ("16", 4096), ("-2", 2048), ("many", 2048), ("", 2048), ("8", 896), ("2", 128)])
+def test_ranks_that_cannot_be(monkeypatch, ranks, K):
+    """A number of CTAs that the sums' exchange has no form for, or more of them than there are runs of K: refused before anything is launched."""
+    from mlx_lm_b200 import ops as o
+
+    x, w = kept(normal((4, K), 1)), kept(normal((300, K), 2))
+    out, st = torch.full((4, 300), 3.0, device="cuda"), status()
+    codes = o.fp8_empty(16, K, "cuda", groups=2)
+    stack, plan = kept(normal((2 * 128, K), 3), 128), planned([0, 1], 2, 16, most=2)
+    torch.cuda.synchronize()
+    monkeypatch.setenv("MLXB_FP8_RANKS", ranks)
+    with pytest.raises(o.KernelError, match="MLXB_FP8_RANKS"):
+        o.linear_fp8(*x, *w, None, out, st, o.current_stream())
+    with pytest.raises(o.KernelError, match="MLXB_FP8_RANKS"):
+        o.moe_gemm_fp8(*codes, *stack, *plan, torch.zeros((2, 128), device="cuda"), st, o.current_stream())
+    torch.cuda.synchronize()
+    assert int(st) == 0 and (out == 3.0).all()
