@@ -141,8 +141,8 @@ class Part:
             c.set_weight_bits(bits)
 
     def hold_eight_bits(self) -> int:
-        """Called on all parts once every weight is bound, if they are kept in 8 bits: this part and its children put theirs into that form; how
-        many weights that were."""
+        """Called on each part of a description once its weights and its children's are bound, if they are kept in 8 bits: they put theirs into that
+        form; how many weights that were."""
         return sum(c.hold_eight_bits() for c in self.children())
 
 

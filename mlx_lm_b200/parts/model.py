@@ -265,9 +265,12 @@ class Model:
         self.dtype, self.device = dtype, torch.device(device)
         for p in description.parts():
             p.set_weight_bits(weight_bits)
+        held = 0
         for p in description.parts():
             p.bind_all(tensors, dtype, self.device)
-        if weight_bits and not sum(p.hold_eight_bits() for p in description.parts()):
+            if weight_bits:               # before the next part's weights come, see weights.loader.Placed
+                held += p.hold_eight_bits()
+        if weight_bits and not held:
             raise ValueError("weight_bits=8: this model has no weight that is held in 8 bits (linear layers from 128 x 128 on, experts)")
 
     @property

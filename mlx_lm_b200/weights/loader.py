@@ -19,7 +19,7 @@ import glob
 import json
 import os
 import re
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Mapping, Optional, Tuple
 
 import torch
 
@@ -94,6 +94,23 @@ def place(spec: ParamSpec, t: torch.Tensor, dtype: torch.dtype, device) -> torch
     return t.to(device=device, dtype=target).contiguous()
 
 
+class Placed(Mapping):
+    """A model's tensors on their way to the device: each is placed when a part asks for it and lives as long as what was asked for, so that a part
+    whose weights take another form (``weight_bits``) gives the memory back before the next one's arrive."""
+
+    def __init__(self, specs: Dict[str, ParamSpec], tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device):
+        self.specs, self.tensors, self.dtype, self.device = specs, tensors, dtype, device
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        return place(self.specs[name], self.tensors[name], self.dtype, self.device)
+
+    def __iter__(self):
+        return iter(self.tensors)
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+
 def build_model(config: dict, tensors: Dict[str, torch.Tensor], dtype: torch.dtype = torch.bfloat16,
                 device="cuda", get_model_classes=None, weight_bits: Optional[int] = None) -> Model:
     """``weight_bits=8``: large weights are held in 8-bit floating point (``parts.model.Model``).  ``get_model_classes(config) -> (builder, args class)`` replaces the registry lookup, as the parameter of
@@ -109,7 +126,9 @@ def build_model(config: dict, tensors: Dict[str, torch.Tensor], dtype: torch.dty
     description = build(args)
     got = check_tensors(description, tensors)
     specs = {s.name: s for s in description.param_specs()}
-    placed = {n: place(specs[n], t, dtype, device) for n, t in got.items()}
+    placed = Placed(specs, got, dtype, device)
+    if weight_bits is None:
+        placed = dict(placed)
     return Model(description, placed, dtype, device, weight_bits=weight_bits)
 
 
