@@ -134,9 +134,11 @@ class Part:
 
     # How the model keeps large weights: None as they are, 8 in 8-bit floating point (ops.fp8_quantize).  Known before the weights are bound.
     weight_bits: Optional[int] = None
+    held = None              # what a part has in the place of its weights then, see hold_eight_bits
 
     def set_weight_bits(self, bits: Optional[int]) -> None:
-        self.weight_bits = bits
+        """Before the weights are bound: what was held of others goes."""
+        self.weight_bits, self.held = bits, None
         for c in self.children():
             c.set_weight_bits(bits)
 

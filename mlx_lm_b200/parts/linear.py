@@ -45,7 +45,7 @@ class Linear(Part):
         self.weight: Optional[torch.Tensor] = None
         self.bias: Optional[torch.Tensor] = None
         self.folded = None        # see fold_norm
-        self.held = None          # see hold_eight_bits: (codes, scales) in the place of ``weight``
+        self.held = None          # (codes, scales) in the place of ``weight``
 
     def param_specs(self) -> List[ParamSpec]:
         shape = (self.n_out, self.n_in) if self.stored == "out_in" else (self.n_in, self.n_out)
