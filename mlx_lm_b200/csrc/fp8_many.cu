@@ -266,7 +266,6 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
   } else {
     const int q = warp & 3, slice = (warp - 2) >> 2, row = q * 32 + lane;
     uint4* stg = sm.stage[warp - 2];
-    int turn = 0;
     const int o_row = lane >> 1, o_piece = lane & 1;
     int it = 0;
     for (int t = first_tile; t < n_tiles; t += step, ++it) {
@@ -377,7 +376,7 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
             fp8_activate<sizeof(TO) == 2>(a.act, vv);
           }
           if constexpr (!WHOLE) {         // rows that do not begin on 16 bytes: a few columns at a time through shared memory in float32
-            constexpr int COLS = S::OUT / 128, STEP = 32 / COLS;         // 16 or 8 columns, 2 or 4 rows an instruction
+            constexpr int COLS = S::OUT / 128, STEP = 32 / COLS;         // 8 columns, 4 rows an instruction
             float* f = reinterpret_cast<float*>(stg);
 #pragma unroll
             for (int p0 = 0; p0 < 32; p0 += COLS) {
@@ -449,9 +448,8 @@ fp8_many_kernel(const __grid_constant__ ManyMaps maps, ManyArgs a) {
               __syncwarp();
               if (lane == 0) {
                 if (rows > 0 && nc + p0 < (a.N & ~(PER - 1))) store_box(&maps.out, box, nc + p0, m0);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");          // a box that is not sent counts too: the wait above goes by turns
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
               }
-              ++turn;
             }
           } else {
 #pragma unroll
