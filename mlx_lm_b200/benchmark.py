@@ -24,7 +24,7 @@ def setup_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--delay", type=float, default=0, help="Seconds to wait between trials")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     p.add_argument("--kv-bits", type=int, choices=[8], default=None, help="Keys and values in 8 bits")
-    p.add_argument("--weight-bits", type=int, choices=[8], default=None, help="Weights in 8-bit floating point")
+    p.add_argument("--weight-bits", type=int, choices=[8], default=None, help="Weights, and the rows that meet them, in 8-bit floating point")
     return p
 
 

@@ -17,7 +17,7 @@
 //
 // In us: 8192 x 8192 x 8192 375 (2.9 PFLOP/s; under the power limit's clocks 390 to 450), 4096 x 4096 x 4096 53 (2.6), 1024 x 4096 x 4096 16.1 (2.1),
 // 32768 slots over 64 experts 2048 -> 2 x 1024 134 (2.05; tensor pipe 58 % of the time, the rest is the unit's arithmetic where one accumulator is
-// waited for) and 1024 -> 2048 84 (1.6; 134 MB of results, tensor pipe 45 %).  Experts in pairs of CTAs were slower (145 and 103; 300 tokens: 17 beside 11):
+// waited for) and 1024 -> 2048 84 (1.6; 134 MB of results, tensor pipe 45 %), with float32 results 126 to 140 (268 MB, 30 %).  Experts in pairs of CTAs were slower (145 and 103; 300 tokens: 17 beside 11):
 // both CTAs wait for the slower one's epilogue, and an expert's odd tile leaves half a pair idle.
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out raises a status bit and all roles leave through the common exit.

@@ -6,7 +6,7 @@
 // plan       the (token, choice) slots sorted by expert and, within one, by number; tiles of at most tile_rows slots of one expert.
 //
 // The choice is exact: without a correction scores are in the order of the logits, and these are compared; with one, a warp compares float32 scores,
-// which it forms with the hardware's exponential and quotient.  Where a choice was by less than they can be off, the two scores it was
+// which it forms with the hardware's exponential and quotient.  Where a choice was by less than these can be off, the two scores it was
 // between, if they were two, are formed again in 64 bits, else all of the token's are and it chooses by those.  A score that is NaN, or that a correction
 // makes minus infinity, is never chosen; places that nobody can take hold expert -1 and weight 0.
 //

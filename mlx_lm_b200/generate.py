@@ -58,7 +58,9 @@ def load(path: str, tokenizer_config: Optional[dict] = None, model_config: Optio
     must be None: adapters are not built).  ``dtype`` is ``"bfloat16"`` (the serving path) or
     ``"float32"`` (everything in true 32-bit).  ``weight_bits=8`` (with bfloat16): the weights of linear layers and
     experts are held in 8-bit floating point with a scale for each row and 128 columns, and the rows that meet them are
-    rounded the same way; half the bytes of a decode step's weights, twice the rate of a prompt's products.
+    rounded the same way (4 significant bits: logits of random weights move by some 11 %).  Half the memory of these weights; faster
+    than bfloat16 from some 2560 columns on, slower below (924 tokens/s instead of 2023 for one request at width 1024).  A request's
+    logits then depend by such roundings on how its steps are cut and what shares them.
     ``tokenizer_config`` may carry ``eos_token_ids``."""
     if adapter_path is not None:
         raise ValueError("adapter_path: adapters are not offered by this engine")
@@ -442,7 +444,8 @@ def setup_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--kv-bits", type=int, choices=[8], default=None,
                    help="keep keys and values in 8 bits with a scale for each block of 16 positions and head (default: in --dtype)")
     p.add_argument("--weight-bits", type=int, choices=[8], default=None,
-                   help="hold the weights of linear layers and experts in 8-bit floating point (default: in --dtype)")
+                   help="hold the weights of linear layers and experts in 8-bit floating point and round the rows that meet them the "
+                        "same way: half the memory, faster from some 2560 columns on (default: in --dtype)")
     return p
 
 

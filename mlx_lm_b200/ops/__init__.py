@@ -2662,7 +2662,8 @@ def moe_gemm_fp8(codes, scales, w_codes, w_scales, sorted_slots, tile_info, n_ti
     unit of the two products (``unit``, ``limit`` and the slot's routing weight as in ``moe_gemm``), in float32 and then in 8-bit floating point: ``out``
     and ``out_scales`` by tiles, as the second product reads them.  Else ``w_codes`` is one matrix an expert and the product of place ``i`` of the plan goes to row
     ``sorted_slots[i]`` of ``out`` (bfloat16 or float32).  Rows of no slot are left as they were.  ``status`` receives ``ST_WAIT_TIMEOUT`` if
-    a bounded wait gives up."""
+    a bounded wait gives up.  A hidden number next to a border of codes may fall on either side of it: float32 sums of another order, as another split of K for another
+    number of slots makes them, move such a number by up to 1/8 of itself."""
     S = _fp8_plan(sorted_slots, tile_info, n_tiles, max_tiles, tile_rows, "moe_gemm_fp8")
     _, K, groups = _fp8_codes(codes, scales, tile_rows, "moe_gemm_fp8 rows")
     w_groups = w_scales.shape[0] if w_scales.dim() == 4 else 0

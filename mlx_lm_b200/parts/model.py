@@ -253,7 +253,8 @@ class Model:
     def __init__(self, description: ModelDescription, tensors: Dict[str, torch.Tensor], dtype: torch.dtype,
                  device, weight_bits: Optional[int] = None):
         """``weight_bits=8``: the weights of linear layers and experts are held in 8-bit floating point, with a scale for each row and 128 columns
-        (embeddings, routers, norms and a tied output head stay as they are); bfloat16 runs only."""
+        (embeddings, routers, norms and a tied output head stay as they are), and the rows that meet them are rounded the same way; bfloat16 runs
+        only.  Parts give their bfloat16 weights back one by one as they are bound, if ``tensors`` does not keep them (``weights.loader.Placed``)."""
         if weight_bits not in (None, 8):
             raise ValueError(f"weight_bits {weight_bits!r}: weights in the run's type (None) or in 8 bits")
         if weight_bits and dtype != torch.bfloat16:
