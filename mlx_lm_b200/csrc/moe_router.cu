@@ -44,15 +44,15 @@ struct RouterArgs {
   int *sorted, *tile_info, *n_tiles;
 };
 
-// Whole numbers in the order of floats; 0 (below every number's): not a number, or out of the race.
+// Whole numbers in the order of floats, the two zeros one (the sum makes them +0); 0 (below every number's): not a number, or out of the race.
 __device__ __forceinline__ uint32_t order_of(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.f);
   return v == v ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
 }
 __device__ __forceinline__ float number_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 __device__ __forceinline__ unsigned long long order_of(double v) {
-  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.);
   return v == v ? (b >> 63 ? ~b : b | 1ull << 63) : 0ull;
 }
 

@@ -85,3 +85,14 @@ def test_groups_out_of_the_lowest_numbers(corrected, score):
     for keep, top in ((2, 3), (3, 8), (5, 14)):
         for two in ("best", "two"):
             check(logits_of(T, groups * per, keep), top, correction=c.view(-1).contiguous(), groups=groups, keep_groups=keep, group_score=two, score=score)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,groups,keep", [(40, 1, 1), (64, 8, 3), (96, 48, 7), (600, 6, 2)])
+def test_the_two_zeros_are_equal(E, groups, keep, score):
+    """Logits of plus and minus zero among others: the lower index is chosen."""
+    z = (torch.randn((130, E), generator=torch.Generator().manual_seed(E)) * 0.3).round()
+    assert (torch.signbit(z) & (z == 0)).any(1).all() and (~torch.signbit(z) & (z == 0)).any(1).all()
+    for two in ("best", "two"):
+        check(z.cuda(), 6, score=score, groups=groups, keep_groups=keep, group_score=two)
+        check(z.cuda(), 6, score=score, groups=groups, keep_groups=keep, group_score=two, correction=torch.zeros(E, device="cuda"))
