@@ -93,7 +93,8 @@ class ExpertsMLP(FeedForward):
     products, which are linear in the input.)
 
     Options of the router: ``correction`` (a tensor ``<name>.correction``, one number per router output, added to the
-    scores for the choice only: the weights are the scores without it); ``groups = (count, keep)``: the router outputs
+    scores for the choice only: the weights are the scores without it; minus infinity leaves an expert out, as long as ``top`` are
+    left); ``groups = (count, keep)``: the router outputs
     form ``count`` equal groups of neighbours, a group's score is its largest choice score (``group_score="best"``) or the
     sum of its two largest (``"two"``), and only outputs of the
     ``keep`` best groups can be chosen; ``identity``: the router has that many more outputs than there are experts with
@@ -209,6 +210,12 @@ class ExpertsMLP(FeedForward):
 
     def bind(self, tensors, dtype, device) -> None:
         self.correction = tensors[self.correction_name].contiguous() if self.correction_name else None
+        if self.correction is not None and not self.identity:
+            # a place nobody can take has no row, and the sum over a token's choices would read what an earlier step left there
+            left = (self.correction > -float("inf")).view(self.groups, -1).sum(dim=1).tolist()
+            if sum(sorted(n for n in left if n)[:self.keep_groups]) < self.top:
+                raise ValueError(f"{self.correction_name}: leaves {left} experts to choose from in {self.groups} groups of which {self.keep_groups} stay, "
+                                 f"fewer than the {self.top} that are chosen")
         if self.table_vocab:
             self.table = tensors[self.table_name]
             if self.table.numel() and not 0 <= int(self.table.min()) <= int(self.table.max()) < self.n_experts:
